@@ -433,6 +433,52 @@ int lk_pf_gemm_q4_0(const void * qs, const void * d, int N, int bpr, const int8_
                     const float * asc, int ntok, const float * scale, float * out, int out_ld,
                     int add, void * stream);
 
+/* ---- behind the attention projection: the 8-bit feed-forward half -------------
+ * The residual addition with its RMS norm and 8-bit output, the int8 product that
+ * takes its rows, and the mixture-of-experts layer for a few tokens.  Rows of
+ * floats are fp32, fp16 or bf16 (`type`); arithmetic is fp32 or wider, rounded to
+ * the type once.  Row strides (ld*) count elements. */
+#define LK_F32  0
+#define LK_F16  1
+#define LK_BF16 2
+
+/* Per row of n values (1 <= n <= LK_NORM_MAX_N), fp32 unless stated:
+ *   h = x + delta (delta NULL: h = x);  r = 1/sqrt(mean of h^2 + eps), the mean in
+ *   fp64 and r rounded once;  y = (h * r) * w
+ * res (may be x or delta itself, or NULL) takes h and y (or NULL) takes y, rounded
+ * to the type; the 8-bit output is of the unrounded y:
+ *   LK_Q8_ROW     q int8 [rows][ldq], sc fp32 [rows]: a = max |y|, sc = a / 127,
+ *                 q = rint(y * (127 / a)); a < 2^-120: sc and q are 0; a row with a
+ *                 value that is not finite: sc is NaN, q 0, y NaN
+ *   LK_Q81_PLANAR q int8 [rows][n], sc fp32 [rows][n/32][2]: the bytes
+ *                 lk_pf_quant_rows makes of y (the operand of lk_pf_gemm_q4_0)
+ *   LK_Q81_BLOCK  q lk_block_q8_1 [rows][n/32], sc not used: the same quants and
+ *                 scales as blocks (the operand of lk_gemv_q4_0)
+ * The Q8_1 forms need n a multiple of 32 and ldq == n.  Rows need the alignment of
+ * their elements only (sc of the planar form 8 bytes, blocks 4).  x, delta, res
+ * and y may share a buffer where row and stride are the same. */
+#define LK_NORM_MAX_N 32768
+#define LK_Q8_ROW     0
+#define LK_Q81_PLANAR 1
+#define LK_Q81_BLOCK  2
+int lk_norm_q8(int type, const void * x, int ldx, const void * delta, int ldd, const float * w,
+               float eps, int rows, int n, void * res, int ldr, void * y, int ldy, int form,
+               int8_t * q, int ldq, float * sc, void * stream);
+
+/* out[t][r] = (res ? res[t][r] : 0) + ((float) sum_k x[t][k] * w[r][k]) * sx[t] * sw[r]
+ *   x   : int8 [M][ldx] tokens, sx fp32 [M];  w: int8 [N][ldw] channels, sw fp32 [N]
+ *   out : `type` [M][ldo], res `type` [M][ldr] or NULL (it may be out itself)
+ * The sums are exact (int32, all of -128..127); the conversion, the two products
+ * and the addition round in fp32, the result once to the type.  1 <= K <=
+ * LK_GEMM_I8_MAX_K.  x and w are 16-byte aligned with ldx, ldw multiples of 16 of
+ * at least K and at most LK_GEMM_I8_MAX_LD; each row's bytes between K and the next
+ * multiple of 16 must be readable and do not count. */
+#define LK_GEMM_I8_MAX_K  131071
+#define LK_GEMM_I8_MAX_LD 8388608
+int lk_gemm_i8(const int8_t * x, int ldx, const float * sx, const int8_t * w, int ldw,
+               const float * sw, int M, int N, int K, int type, const void * res, int ldr,
+               void * out, int ldo, void * stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -35,7 +35,7 @@ EXPORTS = (
     "lk_pf_attn8_q81", "lk_pf_attn_q81", "lk_pf_quant_rows", "lk_gemv_q4_0", "lk_pf_gemm_q4_0",
     "lk_attn_decode_noalloc", "lk_rope_freq_table",
     "lk_pf_part_bytes", "lk_pf_attn8_ws", "lk_pf_attn_ws", "lk_pf_gsync_limit", "lk_pf_gsync_faults",
-    "lk_synth_f32",
+    "lk_synth_f32", "lk_norm_q8", "lk_gemm_i8",
 )
 
 
@@ -109,6 +109,8 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
         "lk_pf_gsync_limit": ([I], I),
         "lk_pf_gsync_faults": ([P, I], I),
         "lk_synth_f32": ([I, ctypes.c_uint64, S, ctypes.c_float, ctypes.c_float, P, P], I),
+        "lk_norm_q8": ([I, P, I, P, I, P, ctypes.c_float, I, I, P, I, P, I, I, P, I, P, P], I),
+        "lk_gemm_i8": ([P, I, P, P, I, P, I, I, I, I, P, I, P, I, P], I),
     }
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)
@@ -448,6 +450,136 @@ def qk_norm_rope(qf, kf, vf, qn, kn, d_pos, kc, vc, stream=None) -> None:
 def pf_qknr(Y, qn, kn, m, P, qh, kc, vc, k8=None, ksc=None, kstride=0, cm=None, stream=None) -> None:
     _check(load().lk_pf_qknr(_ptr(Y), _ptr(qn), _ptr(kn), int(m), int(P), _ptr(qh), _ptr(kc), _ptr(vc),
                              _ptr(k8), _ptr(ksc), int(kstride), _ptr(cm), _stream(stream)), "lk_pf_qknr")
+
+
+# ---- the 8-bit feed-forward half -------------------------------------------------
+# These check types, shapes and devices themselves (rows may be strided views),
+# and enqueue on the tensors' device, whichever is current: on its current stream,
+# or on `stream`, which must be one of that device.
+F32, F16, BF16 = 0, 1, 2
+Q8_ROW, Q81_PLANAR, Q81_BLOCK = 0, 1, 2
+_types = None                               # torch dtype -> LK_F32 / LK_F16 / LK_BF16
+
+
+def _type_of(t, what: str) -> int:
+    global _types
+    if _types is None:
+        import torch
+        _types = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+    if t.dtype not in _types:
+        raise ValueError(f"{what}: fp32, fp16 or bf16 rows, not {t.dtype}")
+    return _types[t.dtype]
+
+
+def _rows2(t, rows: int, n: int, dtype, dev: int, what: str) -> tuple:
+    """(pointer, row stride) of a [rows][n] tensor of a dtype on device `dev` whose
+    rows are contiguous; (None, 0) for None."""
+    if t is None:
+        return None, 0
+    if t.dtype is not dtype or t.dim() != 2 or t.shape[0] != rows or t.shape[1] != n:
+        raise ValueError(f"{what}: {dtype} [{rows}, {n}] wanted, not {t.dtype} {list(t.shape)}")
+    if t.get_device() != dev:
+        raise ValueError(f"{what}: on another device, or not in device memory")
+    s0, s1 = t.stride()
+    if (s1 != 1 and n > 1) or (rows > 1 and s0 < n):
+        raise ValueError(f"{what}: rows must be contiguous and must not overlap (strides {s0}, {s1})")
+    return t.data_ptr(), s0 if rows > 1 and s0 >= n else max(n, s0)
+
+
+def _flat(t, shape: tuple, dtype, dev: int, what: str):
+    """Pointer of a contiguous tensor of a shape and dtype on device `dev`."""
+    if t.dtype is not dtype or tuple(t.shape) != shape or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError(f"{what}: contiguous {dtype} {list(shape)} on the rows' device wanted, not {t.dtype} "
+                         f"{list(t.shape)}")
+    return t.data_ptr()
+
+
+def _on(dev: int, stream, call, *args) -> int:
+    """call(*args, stream) with `dev` as the current device: the given stream, or
+    the device's current one."""
+    if dev < 0:
+        raise ValueError("lk_attn: tensors must live in device memory")
+    if _raw_stream is not None and _device is not None and _device() == dev:
+        return call(*args, (_raw_stream(dev) if stream is None else stream.cuda_stream) or None)
+    import torch
+    with torch.cuda.device(dev):
+        return call(*args, (torch.cuda.current_stream() if stream is None else stream).cuda_stream or None)
+
+
+def norm_q8(x, w, q, sc=None, delta=None, res=None, y=None, eps: float = 1e-5, stream=None) -> None:
+    """h = x + delta, y = rmsnorm(h) * w, and y in 8 bits, in one pass over the
+    rows [rows][n] of fp32, fp16 or bf16 (lk_norm_q8).  `res` takes h (it may be x or
+    delta), `y` the normed rows, both of x's type.  The 8-bit form follows from the outputs:
+      sc fp32 [rows], q int8 [rows][n]                    a scale a row (gemm_i8)
+      sc fp32 [rows][n/32][2], q int8 [rows][n]           planar Q8_1 (pf_gemm_q4_0)
+      sc None, q uint8 [rows][n/32 * 36]                  Q8_1 blocks (gemv_q4_0)"""
+    import torch
+    lib = load()
+    ty = _type_of(x, "norm_q8")
+    if x.dim() != 2:
+        raise ValueError("norm_q8: x must be [rows, n]")
+    rows, n = x.shape
+    dev = x.get_device()
+    px, ldx = _rows2(x, rows, n, x.dtype, dev, "norm_q8: x")
+    pd, ldd = _rows2(delta, rows, n, x.dtype, dev, "norm_q8: delta")
+    pr, ldr = _rows2(res, rows, n, x.dtype, dev, "norm_q8: res")
+    py, ldy = _rows2(y, rows, n, x.dtype, dev, "norm_q8: y")
+    pw = _flat(w, (n,), torch.float32, dev, "norm_q8: w")
+    if sc is None:
+        form, ldq, ps = Q81_BLOCK, n, None
+        pq = _flat(q, (rows, n // 32 * Q8_1_BYTES), torch.uint8, dev, "norm_q8: q")
+    elif sc.dim() == 1:
+        form, ps = Q8_ROW, _flat(sc, (rows,), torch.float32, dev, "norm_q8: sc")
+        pq, ldq = _rows2(q, rows, n, torch.int8, dev, "norm_q8: q")
+    else:
+        form, ldq, ps = Q81_PLANAR, n, _flat(sc, (rows, n // 32, 2), torch.float32, dev, "norm_q8: sc")
+        pq = _flat(q, (rows, n), torch.int8, dev, "norm_q8: q")
+    rc = _on(dev, stream, lib.lk_norm_q8, ty, px, ldx, pd, ldd, pw, eps, rows, n, pr, ldr, py, ldy, form, pq, ldq, ps)
+    if rc:
+        _check(rc, "lk_norm_q8")
+
+
+def i8_rows(rows: int, n: int, device="cuda"):
+    """An int8 [rows][n] tensor whose rows lie a multiple of 16 bytes apart, as
+    gemm_i8 takes them (zeroed)."""
+    import torch
+    return torch.zeros(rows, (n + 15) // 16 * 16, dtype=torch.int8, device=device)[:, :n]
+
+
+def _padded(t, ld: int, what: str) -> int:
+    """Row stride of int8 rows of which the last, too, has readable bytes up to
+    the next multiple of 16 (a single row has no stride of its own)."""
+    rows, n = t.shape
+    if rows == 1:
+        ld = n + 15 & ~15
+    end = t.storage_offset() + (rows - 1) * ld + (n + 15 & ~15)
+    if rows and end > t.untyped_storage().nbytes():
+        raise ValueError(f"{what}: the last row's bytes up to a multiple of 16 lie past its storage (see i8_rows)")
+    return ld
+
+
+def gemm_i8(x, sx, w, sw, out, res=None, stream=None) -> None:
+    """out[t][r] = (res[t][r] +) (x[t] . w[r]) * sx[t] * sw[r] (lk_gemm_i8): x int8
+    [M][K] and w int8 [N][K] with rows a multiple of 16 bytes apart (i8_rows), sx fp32
+    [M], sw fp32 [N], out (and res, which may be out) fp32, fp16 or bf16 [M][N]."""
+    import torch
+    lib = load()
+    ty = _type_of(out, "gemm_i8")
+    if x.dim() != 2 or w.dim() != 2:
+        raise ValueError("gemm_i8: x must be [M, K] and w [N, K]")
+    M, K = x.shape
+    N = w.shape[0]
+    dev = x.get_device()
+    px, ldx = _rows2(x, M, K, torch.int8, dev, "gemm_i8: x")
+    pw, ldw = _rows2(w, N, K, torch.int8, dev, "gemm_i8: w")
+    po, ldo = _rows2(out, M, N, out.dtype, dev, "gemm_i8: out")
+    pr, ldr = _rows2(res, M, N, out.dtype, dev, "gemm_i8: res")
+    if K % 16:
+        ldx, ldw = _padded(x, ldx, "gemm_i8: x"), _padded(w, ldw, "gemm_i8: w")
+    rc = _on(dev, stream, lib.lk_gemm_i8, px, ldx, _flat(sx, (M,), torch.float32, dev, "gemm_i8: sx"), pw, ldw,
+             _flat(sw, (N,), torch.float32, dev, "gemm_i8: sw"), M, N, K, ty, pr, ldr, po, ldo)
+    if rc:
+        _check(rc, "lk_gemm_i8")
 
 
 class PrefillCtx:
