@@ -479,6 +479,53 @@ int lk_gemm_i8(const int8_t * x, int ldx, const float * sx, const int8_t * w, in
                const float * sw, int M, int N, int K, int type, const void * res, int ldr,
                void * out, int ldo, void * stream);
 
+/* A mixture-of-experts layer of Q4_0 experts for up to LK_MOE_MAX_TOKENS tokens
+ * (decode steps, small batches, drafts), per token t in fp32:
+ *   l_e = router_e . x;  s_e = sigmoid(l_e) or softmax over the experts
+ *   the top_k experts of the largest s_e + bias_e (bias NULL: of the largest l_e);
+ *   of equals the lowest index, NaN counts below every number
+ *   w_j = s_j, divided by their sum (+ 1e-20) when renorm; times scale
+ *   out = (res ? res : 0) + sum_j w_j * down_j . (silu(gate_j . x) * (up_j . x))
+ * Expert planes are [n_experts][rows][cols / 32] blocks as in lk_gemv_q4_0 (16 quant
+ * bytes, 16-byte aligned; fp16 scales apart): gate and up [ffn][hidden], down
+ * [hidden][ffn]; hidden and ffn multiples of 32 up to LK_MOE_MAX_DIM.  router fp32
+ * [n_experts][hidden], bias fp32 [n_experts] or NULL. */
+#define LK_MOE_MAX_TOKENS  64
+#define LK_MOE_MAX_EXPERTS 256
+#define LK_MOE_MAX_TOP_K   8
+#define LK_MOE_MAX_DIM     32768
+#define LK_MOE_SIGMOID     0
+#define LK_MOE_SOFTMAX     1
+typedef struct lk_moe {
+    int n_experts, top_k, hidden, ffn;
+    int score;                      /* LK_MOE_SIGMOID or LK_MOE_SOFTMAX */
+    int renorm;
+    float scale;
+    const float * router;
+    const float * bias;
+    const void * gate_qs;
+    const void * gate_d;
+    const void * up_qs;
+    const void * up_d;
+    const void * down_qs;
+    const void * down_d;
+} lk_moe;
+
+/* Bytes of workspace that T tokens need (0 on bad arguments). */
+size_t lk_moe_work_bytes(const lk_moe * moe, int T);
+
+/* x `type` [T][ldx], out and res `type` [T][ldo], [T][ldr] (res may be NULL, or out;
+ * out may be x).  x and the activation between the products enter the products exactly
+ * (fp32 rows) or to 16 bits of mantissa (fp16 and bf16 rows, which are exact in them); sums
+ * are fp32.  ids int32 [T][top_k] and weights fp32 [T][top_k], in the order of choice,
+ * where not NULL.  work: 16-byte aligned device memory of lk_moe_work_bytes();
+ * launches that share it must be ordered (one stream, or the caller's events).
+ * The description is read during the call; a token whose x is not finite gives NaN
+ * in its own row only. */
+int lk_moe_q4_0(const lk_moe * moe, int type, const void * x, int ldx, int T, const void * res,
+                int ldr, void * out, int ldo, int32_t * ids, float * weights, void * work,
+                size_t work_bytes, void * stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -36,6 +36,7 @@ EXPORTS = (
     "lk_attn_decode_noalloc", "lk_rope_freq_table",
     "lk_pf_part_bytes", "lk_pf_attn8_ws", "lk_pf_attn_ws", "lk_pf_gsync_limit", "lk_pf_gsync_faults",
     "lk_synth_f32", "lk_norm_q8", "lk_gemm_i8",
+    "lk_moe_work_bytes", "lk_moe_q4_0",
 )
 
 
@@ -110,6 +111,8 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
         "lk_pf_gsync_faults": ([P, I], I),
         "lk_synth_f32": ([I, ctypes.c_uint64, S, ctypes.c_float, ctypes.c_float, P, P], I),
         "lk_norm_q8": ([I, P, I, P, I, P, ctypes.c_float, I, I, P, I, P, I, I, P, I, P, P], I),
+        "lk_moe_work_bytes": ([P, I], S),
+        "lk_moe_q4_0": ([P, I, P, I, I, P, I, P, I, P, P, P, S, P], I),
         "lk_gemm_i8": ([P, I, P, P, I, P, I, I, I, I, P, I, P, I, P], I),
     }
     for name, (args, res) in sig.items():
@@ -580,6 +583,83 @@ def gemm_i8(x, sx, w, sw, out, res=None, stream=None) -> None:
              _flat(sw, (N,), torch.float32, dev, "gemm_i8: sw"), M, N, K, ty, pr, ldr, po, ldo)
     if rc:
         _check(rc, "lk_gemm_i8")
+
+
+class MoeDesc(ctypes.Structure):
+    """lk_moe (include/lk_attn.h)."""
+    _fields_ = [(n, ctypes.c_int) for n in ("n_experts", "top_k", "hidden", "ffn", "score", "renorm")] + \
+        [("scale", ctypes.c_float)] + \
+        [(n, ctypes.c_void_p) for n in ("router", "bias", "gate_qs", "gate_d", "up_qs", "up_d", "down_qs", "down_d")]
+
+
+class MoeQ4_0:
+    """A mixture-of-experts layer of Q4_0 experts for up to `max_tokens` tokens a
+    call (lk_moe_q4_0): router fp32 [E][hidden]; gate and up pairs (qs uint8
+    [E][ffn][hidden/32][16], d fp16 [E][ffn][hidden/32]), down the same as
+    [E][hidden][ffn/32]; score "sigmoid" or "softmax", bias fp32 [E] for the choice
+    only.  Keeps the weights and one workspace: calls on it must be ordered (one
+    stream, or events); calls that may overlap, captured graphs among them, are given
+    workspaces of their own (`work`, uint8 of work_bytes())."""
+
+    def __init__(self, router, gate, up, down, top_k: int, score: str = "sigmoid", bias=None, renorm: bool = True,
+                 scale: float = 1.0, max_tokens: int = 64):
+        import torch
+        if score not in ("sigmoid", "softmax"):
+            raise ValueError(f"MoeQ4_0: score {score!r}")
+        if router.dim() != 2 or gate[0].dim() != 4:
+            raise ValueError("MoeQ4_0: router must be [E, hidden], quants [E, rows, blocks, 16]")
+        dev, (E, hidden), ffn = router.get_device(), router.shape, gate[0].shape[1]
+        if hidden % 32 or ffn % 32 or hidden < 32 or ffn < 32:
+            raise ValueError(f"MoeQ4_0: hidden {hidden}, ffn {ffn} must be multiples of 32")
+        ptr = [_flat(router, (E, hidden), torch.float32, dev, "MoeQ4_0: router"),
+               None if bias is None else _flat(bias, (E,), torch.float32, dev, "MoeQ4_0: bias")]
+        for what, (qs, d), rows, cols in (("gate", gate, ffn, hidden), ("up", up, ffn, hidden),
+                                          ("down", down, hidden, ffn)):
+            ptr += [_flat(qs, (E, rows, cols // 32, 16), torch.uint8, dev, f"MoeQ4_0: {what} quants"),
+                    _flat(d, (E, rows, cols // 32), torch.float16, dev, f"MoeQ4_0: {what} scales")]
+        self._keep = (router, bias, gate, up, down)
+        self._dev, self._hidden, self._k = dev, hidden, int(top_k)
+        self._desc = MoeDesc(E, int(top_k), hidden, ffn, ("sigmoid", "softmax").index(score), int(bool(renorm)),
+                             float(scale), *ptr)
+        self._ref = ctypes.addressof(self._desc)
+        self.max_tokens = int(max_tokens)
+        n = self.work_bytes()
+        if dev < 0:
+            raise ValueError("MoeQ4_0: tensors must live in device memory")
+        self._work = torch.empty(n, dtype=torch.uint8, device=router.device)
+
+    def work_bytes(self) -> int:
+        """Bytes of workspace for max_tokens tokens."""
+        n = int(load().lk_moe_work_bytes(self._ref, self.max_tokens))
+        if n == 0 and self.max_tokens != 0:
+            raise LkError(f"lk_moe_work_bytes: {load().lk_last_error().decode(errors='replace')} "
+                          f"({self.max_tokens} tokens)")
+        return n
+
+    def __call__(self, x, out, res=None, ids=None, weights=None, work=None, stream=None) -> None:
+        """out[t] = (res[t] +) the layer of x[t], rows [T][hidden] of fp32, fp16 or bf16
+        (out may be x, res may be out); ids int32 and weights fp32 [T][top_k] where
+        given."""
+        import torch
+        ty = _type_of(x, "MoeQ4_0")
+        if x.dim() != 2:
+            raise ValueError("MoeQ4_0: x must be [tokens, hidden]")
+        T, dev = x.shape[0], self._dev
+        if T > self.max_tokens:
+            raise ValueError(f"MoeQ4_0: {T} tokens, made for {self.max_tokens}")
+        px, ldx = _rows2(x, T, self._hidden, x.dtype, dev, "MoeQ4_0: x")
+        po, ldo = _rows2(out, T, self._hidden, x.dtype, dev, "MoeQ4_0: out")
+        pr, ldr = _rows2(res, T, self._hidden, x.dtype, dev, "MoeQ4_0: res")
+        pi = None if ids is None else _flat(ids, (T, self._k), torch.int32, dev, "MoeQ4_0: ids")
+        pw = None if weights is None else _flat(weights, (T, self._k), torch.float32, dev, "MoeQ4_0: weights")
+        if work is None:
+            work = self._work
+        elif work.dtype is not torch.uint8 or work.get_device() != dev or not work.is_contiguous():
+            raise ValueError("MoeQ4_0: work must be contiguous uint8 on the layer's device")
+        rc = _on(dev, stream, load().lk_moe_q4_0, self._ref, ty, px, ldx, T, pr, ldr, po, ldo, pi, pw,
+                 work.data_ptr(), work.numel())
+        if rc:
+            _check(rc, "lk_moe_q4_0")
 
 
 class PrefillCtx:

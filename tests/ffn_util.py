@@ -60,3 +60,46 @@ def gemm_ref(x, sx, w, sw, dtype, res=None):
     if res is not None:
         v = res.float() + v
     return v.to(dtype)
+
+
+# ---- mixture of experts -----------------------------------------------------------
+def q4_planes(g, E, rows, cols, lo=0.002, hi=0.02):
+    """Random Q4_0 planes (qs uint8 [E][rows][cols/32][16], d fp16 [E][rows][cols/32])."""
+    qs = torch.randint(0, 256, (E, rows, cols // 32, 16), generator=g, dtype=torch.uint8)
+    return qs, (lo + (hi - lo) * torch.rand(E, rows, cols // 32, generator=g)).half()
+
+
+def q4_pack(w):
+    """Quant bytes of integer weights -8..7, [..., cols]: element i of a block in the
+    low bits of byte i, element 16 + i in its high bits."""
+    n = (w + 8).reshape(*w.shape[:-1], -1, 32).to(torch.uint8)
+    return n[..., :16] | (n[..., 16:] << 4)
+
+
+def q4_dense(p, e):
+    """One expert's weights in fp64, [rows][cols]."""
+    qs, d = p[0][e], p[1][e].double()
+    n = torch.cat([qs & 15, qs >> 4], -1).double() - 8
+    return (n * d[..., None]).flatten(-2)
+
+
+def moe_ref(x, router, bias, gate, up, down, k, score, renorm=True, scale=1.0, res=None):
+    """(out, ids, weights) in fp64: choice by the score plus bias, of equals the
+    lowest index, NaN last."""
+    x, E = x.double(), router.shape[0]
+    logit = x @ router.double().t()
+    s = torch.sigmoid(logit) if score == "sigmoid" else torch.softmax(logit, -1)
+    rank = logit if bias is None else s + bias.double()
+    order = [sorted(range(E), key=lambda e: (not (r[e] == r[e]), -r[e] if r[e] == r[e] else 0.0, e)) for r in rank.tolist()]
+    ids = torch.tensor([o[:k] for o in order])
+    w = torch.gather(s, 1, ids)
+    if renorm:
+        w = w / (w.sum(-1, keepdim=True) + 1e-20)
+    w = w * scale
+    out = torch.zeros_like(x) if res is None else res.double().clone()
+    for e in sorted(set(ids.flatten().tolist())):
+        G, U, D = (q4_dense(p, e) for p in (gate, up, down))
+        for t, j in (ids == e).nonzero().tolist():
+            g, u = G @ x[t], U @ x[t]
+            out[t] += w[t, j] * (D @ (g * torch.sigmoid(g) * u))
+    return out, ids, w

@@ -1,4 +1,4 @@
-"""What lk_norm_q8 and lk_gemm_i8 refuse, through the C ABI and through the Python
+"""What lk_norm_q8, lk_gemm_i8 and lk_moe_q4_0 refuse, through the C ABI and through the Python
 mirror.  CPU only: every call here fails its checks, or has nothing to do, before
 anything is launched."""
 import ctypes
@@ -67,3 +67,52 @@ def test_mirror_refusals(lk_host):
                      (dict(x=torch.zeros(3, 50, dtype=torch.int8)), "storage"), (dict(w=b.t().contiguous().t()), "contiguous")):
         with pytest.raises(ValueError, match=word):
             lk.gemm_i8(**{**dict(x=a, sx=sa, w=b, sw=sb, out=o), **kw})
+
+
+def _desc(lk, **kw):
+    d = dict(n_experts=8, top_k=2, hidden=64, ffn=32, score=0, renorm=1, scale=1.0, router=0x1000, bias=None, gate_qs=0x1000,
+             gate_d=0x1000, up_qs=0x1000, up_d=0x1000, down_qs=0x1000, down_d=0x1000)
+    return lk.MoeDesc(**{**d, **kw})
+
+
+def test_moe_c_refusals(lk_host):
+    lib = lk_host.load()
+    need = lib.lk_moe_work_bytes(ctypes.byref(_desc(lk_host)), 4)
+    assert need > 0 and need % 16 == 0
+    assert need < lib.lk_moe_work_bytes(ctypes.byref(_desc(lk_host)), 5)
+    ok = dict(type=0, x=P, ldx=64, T=4, res=None, ldr=0, out=P, ldo=64, ids=None, weights=None, work=P, work_bytes=need, stream=None)
+
+    def rc(desc={}, **kw):
+        return lib.lk_moe_q4_0(ctypes.byref(_desc(lk_host, **desc)), *{**ok, **kw}.values())
+    for bad in (dict(n_experts=0), dict(n_experts=257), dict(top_k=0), dict(top_k=9), dict(n_experts=1), dict(hidden=0), dict(hidden=48),
+                dict(hidden=32800), dict(ffn=0), dict(ffn=40), dict(ffn=32800), dict(score=2), dict(score=-1)):
+        assert rc(bad) == 1 and b"lk_moe" in lib.lk_last_error(), bad
+        assert lib.lk_moe_work_bytes(ctypes.byref(_desc(lk_host, **bad)), 4) == 0, bad
+    for bad in (dict(router=None), dict(gate_qs=None), dict(gate_d=None), dict(up_qs=None), dict(up_d=None), dict(down_qs=None),
+                dict(down_d=None), dict(gate_qs=0x1008), dict(up_qs=0x1008), dict(down_qs=0x1008), dict(gate_d=0x1001),
+                dict(router=0x1002), dict(bias=0x1002)):
+        assert rc(bad) == 1 and b"lk_moe_q4_0" in lib.lk_last_error(), bad
+    for bad in (dict(type=3), dict(T=-1), dict(T=65), dict(x=None), dict(out=None), dict(work=None), dict(work_bytes=need - 1),
+                dict(work=ctypes.c_void_p(0x1008)), dict(ldx=63), dict(ldo=63), dict(res=P, ldr=63), dict(x=O), dict(out=O),
+                dict(res=O, ldr=64), dict(ids=O), dict(weights=O)):
+        assert rc(**bad) == 1 and b"lk_moe_q4_0" in lib.lk_last_error(), bad
+    assert lib.lk_moe_q4_0(None, *ok.values()) == 1
+    assert rc(T=0, x=None, out=None, work=None, work_bytes=0) == 0
+    assert lib.lk_moe_work_bytes(None, 4) == 0 and lib.lk_moe_work_bytes(ctypes.byref(_desc(lk_host)), 65) == 0
+
+
+def test_moe_mirror_refusals(lk_host):
+    lk = lk_host
+    q = lambda r, c: (torch.zeros(4, r, c // 32, 16, dtype=torch.uint8), torch.zeros(4, r, c // 32).half())  # noqa: E731
+    ok = dict(router=torch.zeros(4, 64), gate=q(32, 64), up=q(32, 64), down=q(64, 32), top_k=2)
+    with pytest.raises(ValueError, match="device memory"):
+        lk.MoeQ4_0(**ok)
+    for kw, word in ((dict(score="tanh"), "score"), (dict(router=torch.zeros(4)), "router"), (dict(router=torch.zeros(5, 64)), "gate"),
+                     (dict(router=torch.zeros(4, 48)), "multiples"), (dict(gate=q(64, 32)), "gate"), (dict(up=q(32, 96)), "up"),
+                     (dict(down=q(32, 64)), "down"), (dict(bias=torch.zeros(3)), "bias"), (dict(bias=torch.zeros(4).half()), "bias"),
+                     (dict(gate=(ok["gate"][0], ok["gate"][1].float())), "gate scales")):
+        with pytest.raises(ValueError, match=word):
+            lk.MoeQ4_0(**{**ok, **kw})
+    for kw, word in ((dict(top_k=0), "top_k"), (dict(top_k=5), "top_k"), (dict(max_tokens=65), "65 tokens")):
+        with pytest.raises(lk.LkError, match=word):
+            lk.MoeQ4_0(**{**ok, **kw})
