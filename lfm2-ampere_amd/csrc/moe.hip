@@ -12,20 +12,35 @@
 // A Q4_0 block of 32 weights is (n - 8) * d, n = 0..15 (byte i of its 16: element i
 // low, element 16 + i high), d fp16.
 //
-// Exactness: the products run on v_mfma_f32_16x16x32_bf16 with operands that are
-// exact.  The weight enters as the bf16 number 16 + n (one AND-OR on two nibbles:
-// n at the top of the mantissa of 16.0); the -24 it is too large by is
-// -24 * (sum of the block's x), put into the accumulator first.  x and h enter as
-// bf16 terms that add up to the value: three (24 bits, all of fp32) for fp32 rows, two
-// (16 bits; fp16 and bf16 rows exact, h to 2^-17) for 16-bit rows.  A block's sum is scaled
-// by d in fp32 and added in fp32.
+// The products are integer dot products (v_dot4_i32_i8): a block of 32 values of x or h
+// becomes whole numbers i = rint(v * 2^p), the largest just inside the range, in NP
+// int8 digits of base 256: three for fp32 rows (24 bits of the block's largest value), two
+// for fp16 and bf16 rows (16 bits).  sum (n - 8) i is exact in int32 digit by digit
+// (-8 * the digits' sum is where the sum starts), the digits are put together and scaled by
+// d * 2^-p in fp32, and blocks are added in fp32.  A block that holds a value
+// that is not finite gets the scale NaN; one whose largest value is under 2^-100 counts as
+// zero.
 #include "lk_types.h"
 
-typedef __bf16 lk_b8 __attribute__((ext_vector_type(8)));
 typedef uint32_t lk_u4 __attribute__((ext_vector_type(4)));
 
-#define LK_MOE_THREADS 256
-static_assert(LK_MOE_THREADS == LK_MOE_MAX_EXPERTS, "lk_moe_slot: a thread per expert");
+// Up to this many tokens every workgroup chooses the experts itself, a wave per
+// token, and the down product adds the experts up itself (three launches); above it a
+// launch of one workgroup chooses once and sorts the tokens by expert, and another
+// adds up (five).
+#define LK_MOE_FEW 8
+#define LK_MOE_THREADS 256                // router and sum
+#define LK_MOE_NW 8                       // waves of a gate/up or down workgroup
+#define LK_MOE_NWF 16                     // of a down workgroup for few tokens
+
+// The assignments (token * k + j) sorted by expert: expert e[s] of slot s has those of
+// list[from[s]] .. list[from[s + 1] - 1].
+struct LkMoeTab {
+    int32_t slots;
+    int32_t e[LK_MOE_MAX_EXPERTS];
+    int32_t from[LK_MOE_MAX_EXPERTS + 1];
+    int32_t list[LK_MOE_MAX_TOKENS * LK_MOE_MAX_TOP_K];
+};
 
 struct LkMoeArgs {
     const void * x;
@@ -39,59 +54,53 @@ struct LkMoeArgs {
     float * wts_out;
     // workspace
     float * logits;                      // [T][E]
-    __bf16 * xp;                         // [T][NP][hidden] terms of x, permuted within blocks
-    float * xs;                          // [T][hidden / 16] -24 * sums of half blocks
-    __bf16 * hp;                         // [T * k][NP][ffn]
-    float * hs;                          // [T * k][ffn / 16]
+    uint8_t * xr;                        // [T][hidden / 32] records (LkMoeRec) of x
+    uint8_t * hr;                        // [T * k][ffn / 32] records of h
     float * y;                           // [T * k][hidden]
     int32_t * ids;                       // [T * k]
     float * wts;                         // [T * k]
+    int32_t * tab;                       // LkMoeTab, for more than LK_MOE_FEW tokens
     int ldx, ldr, ldo, T, E, k, hidden, ffn, score, renorm;
     float scale;
 };
 
-// Position of element m of a block in its plane: lane group g of an MFMA holds the
-// eight weights of dword g of the block, in the order in which lk_moe_dequant takes
-// them out of it (bytes 0, 2 low, 0, 2 high, 1, 3 low, 1, 3 high).
-__device__ __forceinline__ constexpr int lk_moe_pos(int m) {
-    return 8 * ((m & 15) >> 2) + 4 * (m & 1) + 2 * (m >> 4) + ((m & 3) >> 1);
-}
-// The 8 weights of a dword as bf16 16 + n.
-__device__ __forceinline__ lk_b8 lk_moe_dequant(uint32_t w) {
-    constexpr uint32_t M = 0x00780078u, S = 0x41804180u;
-    const lk_u4 v = { ((w << 3) & M) | S, ((w >> 1) & M) | S, ((w >> 5) & M) | S, ((w >> 9) & M) | S };
-    return __builtin_bit_cast(lk_b8, v);
-}
-// v as NP bf16 terms by truncation: every remainder is exact, and no term
-// overflows.
+// ---- whole numbers of a block -------------------------------------------------------
+// A block's record: NP planes of 32 int8 digits, highest first, then int32 -8 * sum of
+// each plane (0 for a third of two) and the fp32 scale 2^-p.
 template <int NP>
-__device__ __forceinline__ void lk_moe_split(float v, uint16_t (&t)[NP]) {
-#pragma unroll
-    for (int p = 0; p < NP; ++p) {
-        const uint32_t u = __builtin_bit_cast(uint32_t, v);
-        if (p + 1 == NP && NP == 2) {                    // the last of two: rounded
-            t[p] = __builtin_bit_cast(uint16_t, (__bf16) v);
-        } else {
-            t[p] = (uint16_t) (u >> 16);
-            v -= __builtin_bit_cast(float, u & 0xFFFF0000u);
-        }
-    }
+struct LkMoeRec {
+    static constexpr int PIECES = 2 * NP + 1, BYTES = 16 * PIECES;
+};
+// 2^p for a block whose largest |v| has the bits am; 0 for a block of zeros and for one
+// that is not finite.  The digits reach 127 * (1 + 256 (+ 65536)): the largest value
+// goes to the top binade where its leading bits allow, else one below.
+template <int NP>
+__device__ __forceinline__ float lk_moe_up2(uint32_t am) {
+    constexpr float TOP = NP == 3 ? 8355711.0f : 32639.0f;
+    constexpr int B = NP == 3 ? 22 : 14;
+    if (am >= 0x7F800000u || am < (27u << 23)) return 0.0f;                       // not finite; under 2^-100
+    // 2^(B - E), E the exponent of am, by way of two factors: the exponent of one may leave the range
+    const int E = (int) (am >> 23) - 127;
+    const float f = ldexpf(1.0f, B - E);
+    return __builtin_bit_cast(float, am) * f > TOP ? 0.5f * f : f;
 }
-// Dwords j of lane groups g (16 lanes each) transposed: afterwards register j of
-// group g is what register g of group j was.
-__device__ __forceinline__ void lk_moe_transpose(lk_u4 & w) {
-#ifdef __HIP_DEVICE_COMPILE__
-    uint32_t a = w[0], b = w[1], c = w[2], d = w[3];
-    asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %2\n\tv_permlane32_swap_b32 %1, %3\n\ts_nop 1\n\t"
-        "v_permlane16_swap_b32 %0, %1\n\tv_permlane16_swap_b32 %2, %3\n\ts_nop 1"
-        : "+v"(a), "+v"(b), "+v"(c), "+v"(d));
-    w = lk_u4{ a, b, c, d };
-#endif
+__device__ __forceinline__ float lk_moe_scale(uint32_t am, float up) {            // 2^-p; NaN for what is not finite
+    return am >= 0x7F800000u ? __builtin_nanf("") : up == 0.0f ? 0.0f : 1.0f / up; // a power of two: exact
+}
+template <int NP>
+__device__ __forceinline__ void lk_moe_digits(float v, float up, int (&q)[NP]) {
+    int i = up == 0.0f ? 0 : (int) __builtin_rintf(v * up);
+#pragma unroll
+    for (int p = NP - 1; p > 0; --p) {
+        q[p] = (int) (int8_t) i;
+        i = (i - q[p]) >> 8;
+    }
+    q[0] = i;
 }
 
-// ---- router scores, and the terms of x -------------------------------------------
+// ---- router scores, and the records of x -------------------------------------------
 // Workgroups 0 .. nE-1 (of blockIdx.x): one expert per wave, four tokens; the rest:
-// the terms and half-block sums of four tokens, four threads per block of 32.
+// the records of four tokens, four threads per block of 32.
 template <int TYPE, int NP>
 __global__ void __launch_bounds__(LK_MOE_THREADS)
 lk_k_moe_router(const LkMoeArgs a, int nE) {
@@ -124,310 +133,520 @@ lk_k_moe_router(const LkMoeArgs a, int nE) {
         return;
     }
     const int u = (blockIdx.x - nE) * LK_MOE_THREADS + threadIdx.x, b = u >> 2, g = u & 3, bpr = H / 32;
+    constexpr int REC = LkMoeRec<NP>::BYTES;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         const int t = t0 + k;
         const bool ok = t < a.T && b < bpr;              // the same for the four threads of a block
-        float lo[4] = { 0 }, hi[4] = { 0 };
-        if (ok) {
-            lk_load<4>(x + (size_t) t * a.ldx + 32 * b + 4 * g, lo);
-            lk_load<4>(x + (size_t) t * a.ldx + 32 * b + 16 + 4 * g, hi);
-        }
-        float s0 = (lo[0] + lo[1]) + (lo[2] + lo[3]), s1 = (hi[0] + hi[1]) + (hi[2] + hi[3]);
-        s0 += lk_dpp<LK_DPP_QP_XOR1>(s0);
-        s0 += lk_dpp<LK_DPP_QP_XOR2>(s0);
-        s1 += lk_dpp<LK_DPP_QP_XOR1>(s1);
-        s1 += lk_dpp<LK_DPP_QP_XOR2>(s1);
-        if (!ok) continue;
-        uint16_t q[8][NP];
+        float v[8] = { 0 };
+        if (ok) lk_load<8>(x + (size_t) t * a.ldx + 32 * b + 8 * g, v);
+        uint32_t am = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            lk_moe_split<NP>(lo[j], q[lk_moe_pos(j)]);
-            lk_moe_split<NP>(hi[j], q[lk_moe_pos(16 + j)]);
+        for (int j = 0; j < 8; ++j) am = lk_umax(am, __builtin_bit_cast(uint32_t, v[j]) & 0x7FFFFFFFu);
+        am = lk_umax(am, lk_dpp_u<LK_DPP_QP_XOR1>(am));
+        am = lk_umax(am, lk_dpp_u<LK_DPP_QP_XOR2>(am));
+        const float up = lk_moe_up2<NP>(am);
+        uint32_t w[NP][2] = {};
+        int s[3] = { 0, 0, 0 };
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            int q[NP];
+            lk_moe_digits<NP>(v[j], up, q);
+#pragma unroll
+            for (int p = 0; p < NP; ++p) {
+                w[p][j / 4] |= (uint32_t) (uint8_t) q[p] << (8 * (j % 4));
+                s[p] += q[p];
+            }
         }
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
-            lk_u16x8 v;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = q[j][p];
-            *(lk_u16x8 *) (a.xp + ((size_t) (t * NP + p) * bpr + b) * 32 + 8 * g) = v;
+            s[p] += (int) lk_dpp_u<LK_DPP_QP_XOR1>((uint32_t) s[p]);
+            s[p] += (int) lk_dpp_u<LK_DPP_QP_XOR2>((uint32_t) s[p]);
         }
-        if (g == 0) *(float2 *) (a.xs + ((size_t) t * bpr + b) * 2) = make_float2(-24.0f * s0, -24.0f * s1);
+        if (!ok) continue;
+        uint8_t * r = a.xr + ((size_t) t * bpr + b) * REC;
+#pragma unroll
+        for (int p = 0; p < NP; ++p) *(uint2 *) (r + 32 * p + 8 * g) = make_uint2(w[p][0], w[p][1]);
+        if (g == 0)
+            *(lk_i4 *) (r + 32 * NP) = lk_i4{ -8 * s[0], -8 * s[1], -8 * s[2], __builtin_bit_cast(int, lk_moe_scale(am, up)) };
     }
 }
 
 // ---- choice of experts --------------------------------------------------------------
-// 16 lanes per token: lane i holds experts i, i + 16, ...; a round finds the best that
-// is left over the 16 lanes.
-__device__ __forceinline__ uint32_t lk_moe_key(float r) {    // orderable bits; NaN lowest, -0 as 0
+// A wave per token: lane i holds experts i, i + 64, ...  A round takes the largest key
+// that is left; the first register and then the first lane that holds it are the
+// lowest index.
+__device__ __forceinline__ uint32_t lk_moe_key(float r) {    // orderable bits; 0: taken, 1: NaN; -0 as 0
     const uint32_t u = __builtin_bit_cast(uint32_t, r + 0.0f);
-    return r != r ? 0u : (u >> 31) ? ~u : u | 0x80000000u;
+    return r != r ? 1u : (u >> 31) ? ~u : u | 0x80000000u;
 }
-template <int CTRL>
-__device__ __forceinline__ void lk_moe_better(uint32_t & key, uint32_t & e) {
-    const uint32_t k2 = lk_dpp_u<CTRL>(key), e2 = lk_dpp_u<CTRL>(e);
-    const bool take = k2 > key || (k2 == key && e2 < e);
-    key = take ? k2 : key;
-    e = take ? e2 : e;
-}
-// The experts of every token and their weights into LDS (ids, wts: [T * k]); all
-// threads of the workgroup, a barrier at the end.
-__device__ __forceinline__ void lk_moe_choose(const LkMoeArgs & a, int * ids, float * wts) {
-    constexpr int NL = LK_MOE_MAX_EXPERTS / 16;
-    const int i16 = threadIdx.x & 15;
-    for (int t = threadIdx.x >> 4; t < a.T; t += LK_MOE_THREADS / 16) {
-        float l[NL];
-        uint32_t key[NL];
+// Token t's experts and weights into ids[0 .. k-1] and wts[0 .. k-1] (LDS).
+__device__ __forceinline__ void lk_moe_choose(const LkMoeArgs & a, int t, int * ids, float * wts) {
+    constexpr int NL = LK_MOE_MAX_EXPERTS / 64;
+    const int lane = threadIdx.x & 63;
+    float l[NL];
+    uint32_t key[NL];
 #pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            const int e = 16 * i + i16;
-            l[i] = 16 * i < a.E && e < a.E ? a.logits[(size_t) t * a.E + e] : -__builtin_inff();
-        }
-        float m = -__builtin_inff(), z = 0.0f;
-        if (a.score == LK_MOE_SOFTMAX) {
-#pragma unroll
-            for (int i = 0; i < NL; ++i) if (16 * i < a.E) m = fmaxf(m, l[i]);
-            m = lk_row_max16(m);
-#pragma unroll
-            for (int i = 0; i < NL; ++i) if (16 * i < a.E) z += 16 * i + i16 < a.E ? expf(l[i] - m) : 0.0f;
-            z = lk_row_sum16(z);
-        }
-        auto score = [&](float v) {
-            return a.score == LK_MOE_SOFTMAX ? expf(v - m) / z : 1.0f / (1.0f + expf(-v));
-        };
-#pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            const int e = 16 * i + i16;
-            key[i] = 0;
-            if (16 * i < a.E && e < a.E) key[i] = lk_moe_key(a.bias ? score(l[i]) + a.bias[e] : l[i]);
-        }
-        uint32_t used = 0;
-        float sum = 0.0f, mine = 0.0f;
-        for (int j = 0; j < a.k; ++j) {
-            uint32_t bk = 0, be = 0xFFFFu;
-            float bl = 0.0f;
-#pragma unroll
-            for (int i = 0; i < NL; ++i) if (16 * i < a.E) {
-                const uint32_t e = 16 * i + i16;
-                const bool take = (int) e < a.E && !(used >> i & 1) && (be == 0xFFFFu || key[i] > bk);
-                bk = take ? key[i] : bk;
-                bl = take ? l[i] : bl;
-                be = take ? e : be;
-            }
-            const uint32_t own = be;
-            lk_moe_better<LK_DPP_QP_XOR1>(bk, be);
-            lk_moe_better<LK_DPP_QP_XOR2>(bk, be);
-            lk_moe_better<LK_DPP_HMIRROR>(bk, be);
-            lk_moe_better<LK_DPP_MIRROR>(bk, be);
-            if (own == be) used |= 1u << (be / 16);
-            // the chosen expert's logit, from the lane that holds it (j < k <= E: there is one)
-            const float s = score(__shfl(bl, (threadIdx.x & 48) + (int) (be & 15), 64));
-            sum += s;
-            if (i16 == j) mine = s;
-            if (i16 == 0) ids[t * a.k + j] = (int) be;
-        }
-        if (a.renorm) mine = mine / (sum + 1e-20f);
-        if (i16 < a.k) wts[t * a.k + i16] = mine * a.scale;
+    for (int i = 0; i < NL; ++i) {
+        const int e = 64 * i + lane;
+        l[i] = e < a.E ? a.logits[(size_t) t * a.E + e] : -__builtin_inff();
     }
-    __syncthreads();
+    float m = -__builtin_inff(), z = 1.0f;
+    if (a.score == LK_MOE_SOFTMAX) {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) m = fmaxf(m, l[i]);
+        m = lk_xrow_max(lk_row_max16(m));
+        z = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NL; ++i) if (64 * i < a.E) z += 64 * i + lane < a.E ? expf(l[i] - m) : 0.0f;
+        z = lk_wave_sum(z);
+    }
+    auto score = [&](float v) {
+        return a.score == LK_MOE_SOFTMAX ? expf(v - m) / z : 1.0f / (1.0f + expf(-v));
+    };
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+        const int e = 64 * i + lane;
+        key[i] = 0;
+        if (64 * i < a.E) {
+            const float r = a.bias ? score(l[i]) + a.bias[e < a.E ? e : 0] : l[i];
+            key[i] = e < a.E ? lk_moe_key(r) : 0;
+        }
+    }
+    float mine = 0.0f;                                   // lane j: the logit of choice j
+    int id = 0;
+    for (int j = 0; j < a.k; ++j) {
+        uint32_t best = key[0];
+#pragma unroll
+        for (int i = 1; i < NL; ++i) best = lk_umax(best, key[i]);
+        best = (uint32_t) __builtin_amdgcn_readfirstlane((int) lk_wave_umax(best));
+        int e = -1;
+        float v = 0.0f;
+#pragma unroll
+        for (int i = NL - 1; i >= 0; --i) {
+            const uint64_t b = __ballot(key[i] == best);
+            if (b) {                                     // at least one: k <= E
+                e = 64 * i + __builtin_ctzll(b);
+                v = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, l[i]), e & 63));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NL; ++i) key[i] = 64 * i + lane == e ? 0 : key[i];
+        mine = lane == j ? v : mine;
+        id = lane == j ? e : id;
+    }
+    const float s = lane < a.k ? score(mine) : 0.0f;
+    float w = s;
+    if (a.renorm) w = s / (lk_row_sum16(s) + 1e-20f);    // k <= 8: the first row of 16 lanes
+    if (lane < a.k) {
+        ids[lane] = id;
+        wts[lane] = w * a.scale;
+    }
+}
+// The choices of all tokens for the caller and the launches that follow.
+__device__ __forceinline__ void lk_moe_publish(const LkMoeArgs & a, const int * ids, const float * wts) {
+    for (int i = threadIdx.x; i < a.T * a.k; i += blockDim.x) {
+        a.ids[i] = ids[i];
+        a.wts[i] = wts[i];
+        if (a.ids_out) a.ids_out[i] = ids[i];
+        if (a.wts_out) a.wts_out[i] = wts[i];
+    }
 }
 
-// The expert of a slot (the slot-th of those that any token chose, by index) and the
-// assignments t * k + j that chose it, in order, into list; returns the expert or
-// -1, their number in count.  All threads, barriers inside.
-__device__ __forceinline__ int lk_moe_slot(const LkMoeArgs & a, const int * ids, int slot, int * list, int & count) {
-    __shared__ uint8_t met[LK_MOE_MAX_EXPERTS];
+// More than LK_MOE_FEW tokens: one workgroup of 16 waves chooses for all of them and
+// sorts the assignments by expert (counting sort; a wave per expert keeps their order).
+__global__ void __launch_bounds__(1024)
+lk_k_moe_route(const LkMoeArgs a) {
+    __shared__ int ids[LK_MOE_MAX_TOKENS * LK_MOE_MAX_TOP_K];
+    __shared__ float wts[LK_MOE_MAX_TOKENS * LK_MOE_MAX_TOP_K];
+    __shared__ int cnt[LK_MOE_MAX_EXPERTS], from[LK_MOE_MAX_EXPERTS];
     __shared__ uint64_t words[LK_MOE_MAX_EXPERTS / 64];
-    __shared__ int s_e, s_n;
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, na = a.T * a.k;
-    if (tid < LK_MOE_MAX_EXPERTS) met[tid] = 0;
-    if (tid == 0) s_e = -1;
+    __shared__ int sums[LK_MOE_MAX_EXPERTS / 64];
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), na = a.T * a.k;
+    LkMoeTab & tab = *(LkMoeTab *) a.tab;
+    if (tid < LK_MOE_MAX_EXPERTS) cnt[tid] = 0;
+    for (int t = wv; t < a.T; t += 16) lk_moe_choose(a, t, ids + t * a.k, wts + t * a.k);
     __syncthreads();
-    for (int i = tid; i < na; i += LK_MOE_THREADS) met[ids[i]] = 1;
+    lk_moe_publish(a, ids, wts);
+    if (tid < na) atomicAdd(&cnt[ids[tid]], 1);          // na <= 512; counts have no order
     __syncthreads();
-    const bool m = met[tid] != 0;                        // LK_MOE_THREADS == LK_MOE_MAX_EXPERTS
-    const uint64_t word = __ballot(m);
-    if (lane == 0) words[wv] = word;
+    int c = 0, before = 0, slot = 0;
+    if (tid < LK_MOE_MAX_EXPERTS) {                      // waves 0 .. 3: exclusive sums over the experts
+        c = cnt[tid];
+        int s = c;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int u = __shfl_up(s, o, 64);
+            if (lane >= o) s += u;
+        }
+        before = s - c;
+        const uint64_t b = __ballot(c > 0);
+        slot = __popcll(b & ((1ull << lane) - 1));
+        if (lane == 63) { words[wv] = b; sums[wv] = s; }
+    }
     __syncthreads();
-    int before = __popcll(word & ((1ull << lane) - 1));
-    for (int i = 0; i < wv; ++i) before += __popcll(words[i]);
-    if (m && before == slot) s_e = tid;
+    if (tid < LK_MOE_MAX_EXPERTS) {
+        for (int i = 0; i < wv; ++i) { before += sums[i]; slot += __popcll(words[i]); }
+        from[tid] = before;
+        if (c > 0) {
+            tab.e[slot] = tid;
+            tab.from[slot] = before;
+        }
+        if (tid == LK_MOE_MAX_EXPERTS - 1) {
+            slot += c > 0;
+            tab.slots = slot;
+            tab.from[slot] = na;
+        }
+    }
     __syncthreads();
-    const int e = s_e;
-    if (e >= 0 && wv == 0) {
-        int n = 0;
+    for (int e = wv; e < a.E; e += 16) {
+        if (cnt[e] == 0) continue;
+        int n = from[e];
         for (int i0 = 0; i0 < na; i0 += 64) {
             const bool hit = i0 + lane < na && ids[i0 + lane] == e;
             const uint64_t b = __ballot(hit);
-            if (hit) list[n + __popcll(b & ((1ull << lane) - 1))] = i0 + lane;
+            if (hit) tab.list[n + __popcll(b & ((1ull << lane) - 1))] = i0 + lane;
             n += __popcll(b);
         }
-        if (lane == 0) s_n = n;
     }
-    __syncthreads();
-    count = e >= 0 ? s_n : 0;
-    return e;
 }
 
 // ---- the products -------------------------------------------------------------------
-// 16 weight rows of NM matrices times 4 rows of terms, over the block groups
-// (4 blocks) g0, g0 + gs, ... below (bpr + 3) / 4.  Lane (c = l % 16, g = l / 16)
-// loads block g of a group of its weight row c, whole (16 bytes); the transpose gives it
-// dword g of each of the four.  The A operand has row 4b + t = block b of term row
-// t, so that one register serves all four blocks: in the product with block j's
-// weights only rows 4j + t mean something, and those arrive in lane group j.  Lane
-// group g takes its four results of block g there, times its own row's d.
-// acc[m][t]: the part of this lane's block column; the sum over the four lane groups
-// is the caller's.
-template <int NP, int NM, int U>
+// R weight rows of NM matrices (qs, d: the first of the rows) times TK rows of records
+// (rec + trow[t] * bpr records), over the groups of 64 / R blocks of a row,
+// U consecutive ones at a time, of which this is part g0 of gs.  Lane (c = l % R, g = l /
+// R) takes block g of a group of weight row c, whole: 16 bytes, its scale, and of every
+// record row the block's digits.  Those are the same for the R lanes of a block: the
+// wave copies them, one run of memory, into its own part of LDS (xs) and every lane reads
+// them there.
+// acc[t][m]: this lane's blocks; the sum over the lanes of a row is the caller's.
+// Every address is a wave-uniform base and a 32-bit offset: an expert's planes are below
+// 4 GiB (LK_MOE_MAX_DIM).
+template <typename V>
+__device__ __forceinline__ V lk_moe_ld(const void * base, uint32_t off) { return *(const V *) ((const char *) base + off); }
+template <int NP, int R, int U>
+struct LkMoeX {                                          // one row's digits of a step: Z pieces of 16 bytes
+    static constexpr int NB = 64 / R, Z = U * NB * LkMoeRec<NP>::PIECES, NZ = (Z + 63) / 64;
+    lk_u4 x[64 * NZ];
+};
+template <int NP, int NM, int R, int U, int TK>
 __device__ __forceinline__ void lk_moe_rows(const uint8_t * const (&qs)[NM], const _Float16 * const (&d)[NM],
-                                            const __bf16 * planes, const float * seeds, int bpr, int arow,
-                                            const int (&trow)[4], int g0, int gs, float (&acc)[NM][4]) {
-    const int lane = threadIdx.x & 63, g = lane >> 4, ab = (lane & 15) >> 2;
-    const int ng = (bpr + 3) / 4;
-    const __bf16 * ap = planes + (size_t) arow * NP * bpr * 32 + 8 * g;
-    const float * sp[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) sp[r] = seeds + (size_t) trow[r] * bpr * 2;
-    for (int gi = g0; gi < ng; gi += gs * U) {
-        lk_u4 w[U][NM];
+                                            const uint8_t * rec, int bpr, const int (&trow)[TK], int g0, int gs,
+                                            LkMoeX<NP, R, U> * xs, float (&acc)[TK][NM]) {
+    typedef LkMoeX<NP, R, U> X;
+    constexpr int NB = X::NB, PC = LkMoeRec<NP>::PIECES, NZ = X::NZ;
+    const int lane = threadIdx.x & 63, c = lane % R, g = lane / R;
+    const int ng = (bpr + NB - 1) / NB;
+#pragma unroll 1
+    for (int gi = g0 * U; gi < ng; gi += gs * U) {
+        lk_u4 xv[TK][NZ], w[U][NM];
         _Float16 dw[U][NM];
-        lk_b8 av[U][NP];
-        float2 sd[U][4];
+        const int end = bpr * PC - gi * NB * PC;         // pieces from here to the row's end
+#pragma unroll
+        for (int t = 0; t < TK; ++t)
+#pragma unroll
+            for (int z = 0; z < NZ; ++z)
+                xv[t][z] = lk_moe_ld<lk_u4>(rec + ((size_t) trow[t] * bpr + gi * NB) * (PC * 16),
+                                            64 * z + lane < end ? 16u * (64 * z + lane) : 0u);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int i = gi + u * gs < ng ? gi + u * gs : ng - 1;
-            const int bw = 4 * i + g < bpr ? 4 * i + g : bpr - 1, ba = 4 * i + ab < bpr ? 4 * i + ab : bpr - 1;   // in bounds
+            const int b = (gi + u) * NB + g;
+            const uint32_t wb = (uint32_t) (c * bpr + (b < bpr ? b : bpr - 1));                  // in bounds
 #pragma unroll
             for (int m = 0; m < NM; ++m) {
-                w[u][m] = *(const lk_u4 *) (qs[m] + (size_t) bw * 16);
-                dw[u][m] = d[m][bw];
+                w[u][m] = lk_moe_ld<lk_u4>(qs[m], wb * 16u);
+                dw[u][m] = lk_moe_ld<_Float16>(d[m], wb * 2u);
             }
-#pragma unroll
-            for (int p = 0; p < NP; ++p) av[u][p] = *(const lk_b8 *) (ap + ((size_t) p * bpr + ba) * 32);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) sd[u][r] = *(const float2 *) (sp[r] + 2 * bw);
         }
+#pragma unroll
+        for (int t = 0; t < TK; ++t)
+#pragma unroll
+            for (int z = 0; z < NZ; ++z) xs[t].x[64 * z + lane] = xv[t][z];        // past the row's end: its first piece here
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (gi + u * gs >= ng) break;                // wave-uniform
-            const bool in = 4 * (gi + u * gs) + g < bpr; // a block of the last, ragged group that is not there: d 0
-            lk_f4 seed;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) seed[r] = sd[u][r].x + sd[u][r].y;
+            if (gi + u >= ng) break;                     // wave-uniform
+            const bool in = (gi + u) * NB + g < bpr;
+            uint32_t lo[NM][4], hi[NM][4];
+            float dv[NM];
 #pragma unroll
             for (int m = 0; m < NM; ++m) {
-                lk_moe_transpose(w[u][m]);
-                lk_f4 D[4];
+                dv[m] = (float) dw[u][m];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const lk_b8 b = lk_moe_dequant(w[u][m][j]);
-                    D[j] = seed;
-#pragma unroll
-                    for (int p = NP - 1; p >= 0; --p) D[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av[u][p], b, D[j], 0, 0, 0);
-                }
-                const float dv = in ? (float) dw[u][m] : 0.0f;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float s = g == 0 ? D[0][r] : g == 1 ? D[1][r] : g == 2 ? D[2][r] : D[3][r];
-                    acc[m][r] = __builtin_fmaf(dv, s, acc[m][r]);
+                for (int k = 0; k < 4; ++k) {
+                    lo[m][k] = w[u][m][k] & 0x0F0F0F0Fu;
+                    hi[m][k] = (w[u][m][k] >> 4) & 0x0F0F0F0Fu;
                 }
             }
-        }
-    }
-}
-
-template <int NP>
-__global__ void __launch_bounds__(LK_MOE_THREADS)
-lk_k_moe_up(const LkMoeArgs a) {
-    __shared__ int ids[LK_MOE_MAX_TOKENS * LK_MOE_MAX_TOP_K];
-    __shared__ float wts[LK_MOE_MAX_TOKENS * LK_MOE_MAX_TOP_K];
-    __shared__ int list[LK_MOE_MAX_TOKENS];
-    __shared__ float part[4][2][4][16];
-    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
-    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-    lk_moe_choose(a, ids, wts);
-    if (blockIdx.x == 0 && blockIdx.y == 0)
-        for (int i = tid; i < a.T * a.k; i += LK_MOE_THREADS) {
-            a.ids[i] = ids[i];
-            a.wts[i] = wts[i];
-            if (a.ids_out) a.ids_out[i] = ids[i];
-            if (a.wts_out) a.wts_out[i] = wts[i];
-        }
-    int n;
-    const int e = __builtin_amdgcn_readfirstlane(lk_moe_slot(a, ids, blockIdx.y, list, n));
-    if (e < 0) return;
-    const int bpr = a.hidden / 32, F = a.ffn, r0 = blockIdx.x * 16;
-    const size_t row = (size_t) e * F + r0 + c;          // F is a multiple of 32: whole tiles
-    const uint8_t * const qs[2] = { a.qs[0] + row * bpr * 16, a.qs[1] + row * bpr * 16 };
-    const _Float16 * const d[2] = { a.d[0] + row * bpr, a.d[1] + row * bpr };
-    for (int n0 = 0; n0 < n; n0 += 4) {
-        int trow[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) trow[r] = list[n0 + r < n ? n0 + r : n0] / a.k;
-        const int arow = list[n0 + (lane & 3) < n ? n0 + (lane & 3) : n0] / a.k;
-        float acc[2][4] = {};
-        lk_moe_rows<NP, 2, 4>(qs, d, a.xp, a.xs, bpr, arow, trow, wv, 4, acc);
+            for (int t = 0; t < TK; ++t) {
+                asm volatile("" ::: "memory");           // one token's digits at a time: all at once spill
+                const lk_u4 * x = xs[t].x + (u * NB + g) * PC;
+                lk_u4 q[2 * NP];
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+                for (int p = 0; p < 2 * NP; ++p) q[p] = x[p];
+                const lk_i4 meta = __builtin_bit_cast(lk_i4, x[2 * NP]);
+                const int m3 = meta[3];                  // a copy: bit_cast of a vector's element takes element 0
+                const float sc = in ? __builtin_bit_cast(float, m3) : 0.0f;        // a block past the row's end counts nothing
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float v = lk_xrow_sum(acc[m][r]);
-                if (g == r) part[wv][m][r][c] = v;
-            }
-        __syncthreads();
-        if (tid < 64) {                                  // token g of the four, row c
-            const float gt = (part[0][0][g][c] + part[1][0][g][c]) + (part[2][0][g][c] + part[3][0][g][c]);
-            const float up = (part[0][1][g][c] + part[1][1][g][c]) + (part[2][1][g][c] + part[3][1][g][c]);
-            const float h = gt / (1.0f + expf(-gt)) * up;
-            const float s = -24.0f * lk_row_sum16(h);
-            if (n0 + g < n) {
-                const int as = list[n0 + g], f = r0 + c;
-                uint16_t q[NP];
-                lk_moe_split<NP>(h, q);
+                for (int m = 0; m < NM; ++m) {
+                    float f = 0.0f;
 #pragma unroll
-                for (int p = 0; p < NP; ++p)
-                    ((uint16_t *) a.hp)[(size_t) (as * NP + p) * F + (f & ~31) + lk_moe_pos(f & 31)] = q[p];
-                if (c == 0) a.hs[(size_t) as * (F / 16) + r0 / 16] = s;
+                    for (int p = 0; p < NP; ++p) {
+                        int s = meta[p];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            s = __builtin_amdgcn_sdot4((int) lo[m][k], (int) q[2 * p][k], s, false);
+                            s = __builtin_amdgcn_sdot4((int) hi[m][k], (int) q[2 * p + 1][k], s, false);
+                        }
+                        f = p ? __builtin_fmaf(f, 256.0f, (float) s) : (float) s;
+                    }
+                    acc[t][m] = __builtin_fmaf(dv[m] * sc, f, acc[t][m]);
+                }
             }
         }
-        __syncthreads();
+        __builtin_amdgcn_wave_barrier();
     }
 }
+// The sum over the lanes that hold blocks of one row (64 / R of them), in every lane.
+template <int R>
+__device__ __forceinline__ float lk_moe_lanes(float v) {
+    if constexpr (R == 8) v += lk_dpp<LK_DPP_ROR8>(v);
+    return lk_xrow_sum(v);
+}
 
+// 32 rows of one expert's gate and up products for N assignments (as[0 .. N-1]), and
+// what follows of them: the records of h.  N is known at compile time: with branches on
+// it the compiler keeps the digits of all tokens at once and spills.
 template <int NP>
-__global__ void __launch_bounds__(LK_MOE_THREADS)
-lk_k_moe_down(const LkMoeArgs a) {
-    __shared__ int ids[LK_MOE_MAX_TOKENS * LK_MOE_MAX_TOP_K];
-    __shared__ int list[LK_MOE_MAX_TOKENS];
-    __shared__ float part[4][4][16];
+struct LkMoeUp {
+    static constexpr int U = 2, TK = 4;
+    LkMoeX<NP, 16, U> xs[LK_MOE_NW][TK];
+    float part[LK_MOE_NW][4][TK][16];
+};
+template <int NP, int N>
+__device__ __forceinline__ void lk_moe_up_tile(const LkMoeArgs & a, int e, const int * as, LkMoeUp<NP> & sh) {
+    constexpr int U = LkMoeUp<NP>::U, REC = LkMoeRec<NP>::BYTES;
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-    for (int i = tid; i < a.T * a.k; i += LK_MOE_THREADS) ids[i] = a.ids[i];
+    const int bpr = a.hidden / 32, F = a.ffn, r0 = blockIdx.x * 32;
+    const size_t row = (size_t) e * F + r0;              // F is a multiple of 32: whole tiles
+    const uint8_t * qs[4];
+    const _Float16 * d[4];
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+        qs[m] = a.qs[m >> 1] + (row + 16 * (m & 1)) * bpr * 16;
+        d[m] = a.d[m >> 1] + (row + 16 * (m & 1)) * bpr;
+    }
+    int trow[N];
+#pragma unroll
+    for (int r = 0; r < N; ++r) trow[r] = __builtin_amdgcn_readfirstlane(as[r] / a.k);
+    float acc[N][4] = {};
+    lk_moe_rows<NP, 4, 16, U, N>(qs, d, a.xr, bpr, trow, wv, LK_MOE_NW, sh.xs[wv], acc);
+#pragma unroll
+    for (int t = 0; t < N; ++t)
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            const float v = lk_moe_lanes<16>(acc[t][m]);
+            if (g == m) sh.part[wv][m][t][c] = v;
+        }
     __syncthreads();
-    int n;
-    const int e = __builtin_amdgcn_readfirstlane(lk_moe_slot(a, ids, blockIdx.y, list, n));
-    if (e < 0) return;
-    const int bpr = a.ffn / 32, H = a.hidden, r0 = blockIdx.x * 16;
-    const size_t row = (size_t) e * H + r0 + c;
-    const uint8_t * const qs[1] = { a.qs[2] + row * bpr * 16 };
-    const _Float16 * const d[1] = { a.d[2] + row * bpr };
-    for (int n0 = 0; n0 < n; n0 += 4) {
-        int trow[4];
+    if (tid < 32 * N) {                                  // token t, row r of the 32
+        const int t = tid >> 5, r = tid & 31;
+        float gt = 0.0f, up = 0.0f;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) trow[r] = list[n0 + r < n ? n0 + r : n0];
-        const int arow = list[n0 + (lane & 3) < n ? n0 + (lane & 3) : n0];
-        float acc[1][4] = {};
-        lk_moe_rows<NP, 1, 4>(qs, d, a.hp, a.hs, bpr, arow, trow, wv, 4, acc);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const float v = lk_xrow_sum(acc[0][r]);
-            if (g == r) part[wv][r][c] = v;
+        for (int k = 0; k < LK_MOE_NW; ++k) {
+            gt += sh.part[k][r >> 4][t][r & 15];
+            up += sh.part[k][2 + (r >> 4)][t][r & 15];
         }
-        __syncthreads();
-        if (tid < 64 && n0 + g < n)
-            a.y[(size_t) list[n0 + g] * H + r0 + c] = (part[0][g][c] + part[1][g][c]) + (part[2][g][c] + part[3][g][c]);
-        __syncthreads();
+        const float h = gt / (1.0f + expf(-gt)) * up;
+        uint32_t am = __builtin_bit_cast(uint32_t, h) & 0x7FFFFFFFu;
+        for (int o = 16; o > 0; o >>= 1) am = lk_umax(am, (uint32_t) __shfl_xor((int) am, o, 32));
+        const float p2 = lk_moe_up2<NP>(am);
+        int q[NP], s[3] = { 0, 0, 0 };
+        lk_moe_digits<NP>(h, p2, q);
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            s[p] = q[p];
+            for (int o = 16; o > 0; o >>= 1) s[p] += __shfl_xor(s[p], o, 32);
+        }
+        uint8_t * rc = a.hr + ((size_t) as[t] * (F / 32) + blockIdx.x) * REC;
+#pragma unroll
+        for (int p = 0; p < NP; ++p) rc[32 * p + r] = (uint8_t) q[p];
+        if (r == 0)
+            *(lk_i4 *) (rc + 32 * NP) = lk_i4{ -8 * s[0], -8 * s[1], -8 * s[2], __builtin_bit_cast(int, lk_moe_scale(am, p2)) };
+    }
+}
+
+// n assignments, four at a time.
+template <int NP>
+__device__ __forceinline__ void lk_moe_up_tiles(const LkMoeArgs & a, int e, const int * as, int n, LkMoeUp<NP> & sh) {
+    for (; n > 0; n -= 4, as += 4) {
+        if (n >= 4)      lk_moe_up_tile<NP, 4>(a, e, as, sh);
+        else if (n == 3) lk_moe_up_tile<NP, 3>(a, e, as, sh);
+        else if (n == 2) lk_moe_up_tile<NP, 2>(a, e, as, sh);
+        else             lk_moe_up_tile<NP, 1>(a, e, as, sh);
+        if (n > 4) __syncthreads();                      // part has been read
+    }
+}
+
+// Up to LK_MOE_FEW tokens; grid (ffn / 32, T * k): the workgroups of an assignment
+// whose expert an earlier one has end at once.
+template <int NP>
+__global__ void __launch_bounds__(64 * LK_MOE_NW, 4)
+lk_k_moe_up_few(const LkMoeArgs a) {
+    __shared__ int ids[LK_MOE_FEW * LK_MOE_MAX_TOP_K], as[LK_MOE_FEW];
+    __shared__ float wts[LK_MOE_FEW * LK_MOE_MAX_TOP_K];
+    __shared__ LkMoeUp<NP> sh;
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), na = a.T * a.k;
+    if (wv < a.T) lk_moe_choose(a, wv, ids + wv * a.k, wts + wv * a.k);
+    __syncthreads();
+    if (blockIdx.x == 0 && blockIdx.y == 0) lk_moe_publish(a, ids, wts);
+    const int mine = lane < na ? ids[lane] : -1;
+    const int e = __builtin_amdgcn_readlane(mine, blockIdx.y);
+    const uint64_t hits = __ballot(mine == e);
+    if (__builtin_ctzll(hits) != (int) blockIdx.y) return;
+    if (wv == 0 && mine == e) as[__popcll(hits & ((1ull << lane) - 1))] = lane;
+    __syncthreads();
+    lk_moe_up_tiles<NP>(a, e, as, __popcll(hits), sh);
+}
+
+template <int NP>
+__global__ void __launch_bounds__(64 * LK_MOE_NW, 4)
+lk_k_moe_up(const LkMoeArgs a) {
+    __shared__ int as[LK_MOE_MAX_TOKENS];
+    __shared__ LkMoeUp<NP> sh;
+    const LkMoeTab & tab = *(const LkMoeTab *) a.tab;
+    if ((int) blockIdx.y >= tab.slots) return;
+    const int e = tab.e[blockIdx.y], from = tab.from[blockIdx.y], n = tab.from[blockIdx.y + 1] - from;
+    if ((int) threadIdx.x < n) as[threadIdx.x] = tab.list[from + threadIdx.x];
+    __syncthreads();
+    lk_moe_up_tiles<NP>(a, e, as, n, sh);
+}
+
+// Up to LK_MOE_FEW tokens: a workgroup of 16 waves has 8 rows of every expert that was
+// chosen (at most 64), and adds them up itself.  The waves share the experts, Q = 16 /
+// experts of them (at least one) to each, taking its block groups in turn.
+template <int TYPE, int NP>
+__global__ void __launch_bounds__(64 * LK_MOE_NWF, 4)
+lk_k_moe_down_few(const LkMoeArgs a) {
+    typedef typename LkElem<TYPE>::type T;
+    constexpr int R = 8, U = 2, TK = 2, MAXA = LK_MOE_FEW * LK_MOE_MAX_TOP_K;
+    __shared__ LkMoeX<NP, R, U> xs[LK_MOE_NWF][TK];
+    // [q][assignment][row]: q * assignments is at most 16 / experts * (experts * LK_MOE_FEW), or MAXA
+    __shared__ float part[LK_MOE_NWF * LK_MOE_FEW][R];
+    static_assert(LK_MOE_NWF * LK_MOE_FEW >= MAXA, "part");
+    const int tid = threadIdx.x, lane = tid & 63, c = lane % R, g = lane / R;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), na = a.T * a.k, r0 = blockIdx.x * R, bpr = a.ffn / 32;
+    const int mine = lane < na ? a.ids[lane] : -1;
+    // what the sum at the end needs, asked for now (T * R <= 64: the first wave)
+    const int ot = tid / R, orow = r0 + tid % R;
+    const bool sums = tid < a.T * R;
+    float wt[LK_MOE_MAX_TOP_K], rs = 0.0f;
+#pragma unroll
+    for (int j = 0; j < LK_MOE_MAX_TOP_K; ++j) wt[j] = sums && j < a.k ? a.wts[ot * a.k + j] : 0.0f;
+    if (sums && a.res) rs = (float) ((const T *) a.res)[(size_t) ot * a.ldr + orow];
+    uint64_t first = 0;                                  // the assignments that are their expert's first
+    for (int i = 0; i < na; ++i) {
+        const uint64_t b = __ballot(mine == __builtin_amdgcn_readlane(mine, i));
+        first |= (uint64_t) (__builtin_ctzll(b) == i) << i;
+    }
+    const int nd = __popcll(first), Q = nd >= LK_MOE_NWF ? 1 : LK_MOE_NWF / nd;
+    for (int item = wv; item < nd * Q; item += LK_MOE_NWF) {       // expert item / Q, part item % Q
+        uint64_t left = first;
+        for (int i = item / Q; i > 0; --i) left &= left - 1;
+        const int e = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left)), q = item % Q;
+        const size_t row = (size_t) e * a.hidden + r0;   // hidden is a multiple of 32: whole tiles
+        const uint8_t * const qs[1] = { a.qs[2] + row * bpr * 16 };
+        const _Float16 * const d[1] = { a.d[2] + row * bpr };
+        uint64_t hits = __ballot(mine == e);
+        while (hits) {                                   // two assignments at a time
+            const int t0 = __builtin_ctzll(hits);
+            hits &= hits - 1;
+            if (hits) {
+                const int trow[2] = { t0, __builtin_ctzll(hits) };
+                hits &= hits - 1;
+                float acc[2][1] = {};
+                lk_moe_rows<NP, 1, R, U, 2>(qs, d, a.hr, bpr, trow, q, Q, xs[wv], acc);
+                const float v0 = lk_moe_lanes<R>(acc[0][0]), v1 = lk_moe_lanes<R>(acc[1][0]);
+                if (g < 2) part[q * na + trow[g]][c] = g ? v1 : v0;
+            } else {
+                const int trow[1] = { t0 };
+                float acc[1][1] = {};
+                lk_moe_rows<NP, 1, R, U, 1>(qs, d, a.hr, bpr, trow, q, Q, xs[wv], acc);
+                const float v0 = lk_moe_lanes<R>(acc[0][0]);
+                if (g == 0) part[q * na + t0][c] = v0;
+            }
+        }
+    }
+    __syncthreads();
+    if (sums) {
+        float o = 0.0f;
+#pragma unroll
+        for (int j = 0; j < LK_MOE_MAX_TOP_K; ++j) {
+            if (j >= a.k) break;
+            float y = 0.0f;
+            for (int q = 0; q < Q; ++q) y += part[q * na + ot * a.k + j][tid % R];
+            o = __builtin_fmaf(wt[j], y, o);
+        }
+        if (a.res) o = rs + o;
+        ((T *) a.out)[(size_t) ot * a.ldo + orow] = (T) o;
+    }
+}
+
+// 32 rows of one expert's down product for N assignments.
+template <int NP>
+struct LkMoeDown {
+    static constexpr int U = 2, TK = 4;
+    LkMoeX<NP, 16, U> xs[LK_MOE_NW][TK];
+    float part[LK_MOE_NW][2][TK][16];
+};
+template <int NP, int N>
+__device__ __forceinline__ void lk_moe_down_tile(const LkMoeArgs & a, int e, const int * as, LkMoeDown<NP> & sh) {
+    constexpr int U = LkMoeDown<NP>::U;
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), r0 = blockIdx.x * 32, bpr = a.ffn / 32;
+    const size_t row = (size_t) e * a.hidden + r0;
+    const uint8_t * const qs[2] = { a.qs[2] + row * bpr * 16, a.qs[2] + (row + 16) * bpr * 16 };
+    const _Float16 * const d[2] = { a.d[2] + row * bpr, a.d[2] + (row + 16) * bpr };
+    int trow[N];
+#pragma unroll
+    for (int r = 0; r < N; ++r) trow[r] = __builtin_amdgcn_readfirstlane(as[r]);
+    float acc[N][2] = {};
+    lk_moe_rows<NP, 2, 16, U, N>(qs, d, a.hr, bpr, trow, wv, LK_MOE_NW, sh.xs[wv], acc);
+#pragma unroll
+    for (int t = 0; t < N; ++t)
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            const float v = lk_moe_lanes<16>(acc[t][m]);
+            if (g == m) sh.part[wv][m][t][c] = v;
+        }
+    __syncthreads();
+    if (tid < 32 * N) {
+        const int t = tid >> 5, r = tid & 31;
+        float y = 0.0f;
+#pragma unroll
+        for (int k = 0; k < LK_MOE_NW; ++k) y += sh.part[k][r >> 4][t][r & 15];
+        a.y[(size_t) as[t] * a.hidden + r0 + r] = y;
+    }
+}
+
+template <int NP>
+__global__ void __launch_bounds__(64 * LK_MOE_NW, 4)
+lk_k_moe_down(const LkMoeArgs a) {
+    __shared__ int as[LK_MOE_MAX_TOKENS];
+    __shared__ LkMoeDown<NP> sh;
+    const LkMoeTab & tab = *(const LkMoeTab *) a.tab;
+    if ((int) blockIdx.y >= tab.slots) return;
+    const int e = tab.e[blockIdx.y], from = tab.from[blockIdx.y], n = tab.from[blockIdx.y + 1] - from;
+    if ((int) threadIdx.x < n) as[threadIdx.x] = tab.list[from + threadIdx.x];
+    __syncthreads();
+    const int * p = as;
+    for (int left = n; left > 0; left -= 4, p += 4) {
+        if (left >= 4)      lk_moe_down_tile<NP, 4>(a, e, p, sh);
+        else if (left == 3) lk_moe_down_tile<NP, 3>(a, e, p, sh);
+        else if (left == 2) lk_moe_down_tile<NP, 2>(a, e, p, sh);
+        else                lk_moe_down_tile<NP, 1>(a, e, p, sh);
+        if (left > 4) __syncthreads();                   // part has been read
     }
 }
 
@@ -471,7 +690,7 @@ static int lk_moe_check(const lk_moe * m) {
 // The workspace's parts, every one at a multiple of 16 bytes.
 static size_t lk_moe_layout(const lk_moe * m, int T, void * work, LkMoeArgs * a) {
     size_t at = 0;
-    const size_t k = m->top_k, H = m->hidden, F = m->ffn, NP = 3;
+    const size_t k = m->top_k, H = m->hidden, F = m->ffn, REC = LkMoeRec<3>::BYTES;        // of two digits: less
     auto take = [&](size_t bytes) {
         char * p = work ? (char *) work + at : nullptr;
         at += (bytes + 15) & ~(size_t) 15;
@@ -480,13 +699,12 @@ static size_t lk_moe_layout(const lk_moe * m, int T, void * work, LkMoeArgs * a)
     LkMoeArgs b = {};
     LkMoeArgs * o = a ? a : &b;
     o->logits = (float *) take(4 * (size_t) T * m->n_experts);
-    o->xp = (__bf16 *) take(2 * T * NP * H);
-    o->xs = (float *) take(4 * T * (H / 16));
-    o->hp = (__bf16 *) take(2 * T * k * NP * F);
-    o->hs = (float *) take(4 * T * k * (F / 16));
+    o->xr = (uint8_t *) take(T * (H / 32) * REC);
+    o->hr = (uint8_t *) take(T * k * (F / 32) * REC);
     o->y = (float *) take(4 * T * k * H);
     o->ids = (int32_t *) take(4 * T * k);
     o->wts = (float *) take(4 * T * k);
+    o->tab = (int32_t *) take(sizeof(LkMoeTab));
     return at;
 }
 extern "C" size_t lk_moe_work_bytes(const lk_moe * moe, int T) {
@@ -497,11 +715,17 @@ extern "C" size_t lk_moe_work_bytes(const lk_moe * moe, int T) {
 template <int TYPE>
 static void lk_moe_go(const LkMoeArgs & a, hipStream_t st) {
     constexpr int NP = TYPE == LK_F32 ? 3 : 2;
-    const int nE = (a.E + 3) / 4, slots = a.T * a.k < a.E ? a.T * a.k : a.E;
+    const int nE = (a.E + 3) / 4, na = a.T * a.k, slots = na < a.E ? na : a.E;
     hipLaunchKernelGGL((lk_k_moe_router<TYPE, NP>), dim3(nE + (a.hidden / 8 + LK_MOE_THREADS - 1) / LK_MOE_THREADS, (a.T + 3) / 4),
                        dim3(LK_MOE_THREADS), 0, st, a, nE);
-    hipLaunchKernelGGL((lk_k_moe_up<NP>), dim3(a.ffn / 16, slots), dim3(LK_MOE_THREADS), 0, st, a);
-    hipLaunchKernelGGL((lk_k_moe_down<NP>), dim3(a.hidden / 16, slots), dim3(LK_MOE_THREADS), 0, st, a);
+    if (a.T <= LK_MOE_FEW) {
+        hipLaunchKernelGGL((lk_k_moe_up_few<NP>), dim3(a.ffn / 32, na), dim3(64 * LK_MOE_NW), 0, st, a);
+        hipLaunchKernelGGL((lk_k_moe_down_few<TYPE, NP>), dim3(a.hidden / 8), dim3(64 * LK_MOE_NWF), 0, st, a);
+        return;
+    }
+    hipLaunchKernelGGL(lk_k_moe_route, dim3(1), dim3(1024), 0, st, a);
+    hipLaunchKernelGGL((lk_k_moe_up<NP>), dim3(a.ffn / 32, slots), dim3(64 * LK_MOE_NW), 0, st, a);
+    hipLaunchKernelGGL((lk_k_moe_down<NP>), dim3(a.hidden / 32, slots), dim3(64 * LK_MOE_NW), 0, st, a);
     hipLaunchKernelGGL((lk_k_moe_sum<TYPE>), dim3((a.hidden / 4 + LK_MOE_THREADS - 1) / LK_MOE_THREADS, a.T), dim3(LK_MOE_THREADS), 0, st, a);
 }
 
