@@ -29,17 +29,16 @@ typedef uint32_t lk_u4 __attribute__((ext_vector_type(4)));
 // launch of one workgroup chooses once and sorts the tokens by expert, and another
 // adds up (five).
 #define LK_MOE_FEW 8
-#define LK_MOE_THREADS 256                // router and sum
-#define LK_MOE_NW 8                       // waves of a gate/up or down workgroup
-#define LK_MOE_NWF 16                     // of a down workgroup for few tokens
+#define LK_MOE_THREADS 256
+#define LK_MOE_NW 8                       // waves of a gate/up workgroup for few tokens
+#define LK_MOE_NWF 16                     // of a down workgroup
+template <int N> struct LkInt { static constexpr int value = N; };
 
-// The assignments (token * k + j) sorted by expert: expert e[s] of slot s has those of
-// list[from[s]] .. list[from[s + 1] - 1].
+// The experts by the number of their assignments (token * k + j), most first, equals by
+// index: slot s has expert e with n assignments, list[s][0 .. n-1] in order.
 struct LkMoeTab {
-    int32_t slots;
-    int32_t e[LK_MOE_MAX_EXPERTS];
-    int32_t from[LK_MOE_MAX_EXPERTS + 1];
-    int32_t list[LK_MOE_MAX_TOKENS * LK_MOE_MAX_TOP_K];
+    struct { int32_t e, n, pad[2]; } slot[LK_MOE_MAX_EXPERTS];
+    int32_t list[LK_MOE_MAX_EXPERTS][LK_MOE_MAX_TOKENS];
 };
 
 struct LkMoeArgs {
@@ -60,7 +59,7 @@ struct LkMoeArgs {
     int32_t * ids;                       // [T * k]
     float * wts;                         // [T * k]
     int32_t * tab;                       // LkMoeTab, for more than LK_MOE_FEW tokens
-    int ldx, ldr, ldo, T, E, k, hidden, ffn, score, renorm;
+    int ldx, ldr, ldo, T, E, k, hidden, ffn, score, renorm, kinv;
     float scale;
 };
 
@@ -79,13 +78,12 @@ __device__ __forceinline__ float lk_moe_up2(uint32_t am) {
     constexpr float TOP = NP == 3 ? 8355711.0f : 32639.0f;
     constexpr int B = NP == 3 ? 22 : 14;
     if (am >= 0x7F800000u || am < (27u << 23)) return 0.0f;                       // not finite; under 2^-100
-    // 2^(B - E), E the exponent of am, by way of two factors: the exponent of one may leave the range
-    const int E = (int) (am >> 23) - 127;
-    const float f = ldexpf(1.0f, B - E);
+    // 2^(B - E), E the exponent of am: between 2^(B - 127) and 2^(B + 100)
+    const float f = __builtin_bit_cast(float, (uint32_t) (B + 254 - (int) (am >> 23)) << 23);
     return __builtin_bit_cast(float, am) * f > TOP ? 0.5f * f : f;
 }
 __device__ __forceinline__ float lk_moe_scale(uint32_t am, float up) {            // 2^-p; NaN for what is not finite
-    return am >= 0x7F800000u ? __builtin_nanf("") : up == 0.0f ? 0.0f : 1.0f / up; // a power of two: exact
+    return am >= 0x7F800000u ? __builtin_nanf("") : up == 0.0f ? 0.0f : __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, up));
 }
 template <int NP>
 __device__ __forceinline__ void lk_moe_digits(float v, float up, int (&q)[NP]) {
@@ -96,6 +94,64 @@ __device__ __forceinline__ void lk_moe_digits(float v, float up, int (&q)[NP]) {
         i = (i - q[p]) >> 8;
     }
     q[0] = i;
+}
+
+// The token of an assignment: as / k, as < 512, k <= 8, by a multiplication (kinv = 65536 / k + 1).
+__device__ __forceinline__ int lk_moe_token(const LkMoeArgs & a, int as) { return (int) ((uint32_t) (as * a.kinv) >> 16); }
+
+// ---- small helpers --------------------------------------------------------------------
+// exp(-|x|) on v_exp_f32 with the product's rounding error put back (about one unit of
+// 2^-23): expf's branches cost more than they are worth in kernels of a microsecond.
+__device__ __forceinline__ float lk_moe_expn(float x) {
+    const float y = fmaxf(-fabsf(x), -104.0f);           // 0 from there on; NaN too (the callers see to it)
+    const float t = y * LK_LOG2E_F, r = __builtin_fmaf(y, LK_LOG2E_F, -t) + y * 1.925963033500e-8f;
+    const float z = lk_exp2(t);
+    return __builtin_fmaf(z, r * 0.6931471805599453f, z);
+}
+__device__ __forceinline__ float lk_moe_sigmoid(float x) {   // of a NaN: 0 or NaN
+    const float z = lk_moe_expn(x), q = __builtin_amdgcn_rcpf(1.0f + z);
+    return x >= 0.0f ? q : z * q;
+}
+__device__ __forceinline__ float lk_moe_h(float g, float u) { return g * lk_moe_sigmoid(g) * u; }   // NaN * 0 is NaN
+// Largest of a wave's unsigned values, wave-uniform.
+__device__ __forceinline__ uint32_t lk_moe_top(uint32_t v) {
+    v = lk_umax(v, lk_dpp_u<LK_DPP_QP_XOR1>(v));
+    v = lk_umax(v, lk_dpp_u<LK_DPP_QP_XOR2>(v));
+    v = lk_umax(v, lk_dpp_u<LK_DPP_HMIRROR>(v));
+    v = lk_umax(v, lk_dpp_u<LK_DPP_MIRROR>(v));
+    const uint32_t a = (uint32_t) __builtin_amdgcn_readlane((int) v, 0), b = (uint32_t) __builtin_amdgcn_readlane((int) v, 16);
+    const uint32_t c = (uint32_t) __builtin_amdgcn_readlane((int) v, 32), d = (uint32_t) __builtin_amdgcn_readlane((int) v, 48);
+    return lk_umax(lk_umax(a, b), lk_umax(c, d));
+}
+// Sum over each half of a wave.
+__device__ __forceinline__ int lk_moe_sum32(int v) {
+    float x = __builtin_bit_cast(float, v), y = x;
+    lk_swap16(x, y);
+    v = __builtin_bit_cast(int, x) + __builtin_bit_cast(int, y);
+    v += (int) lk_dpp_u<LK_DPP_ROR8>((uint32_t) v);
+    v += (int) lk_dpp_u<LK_DPP_ROR4>((uint32_t) v);
+    v += (int) lk_dpp_u<LK_DPP_QP_XOR2>((uint32_t) v);
+    v += (int) lk_dpp_u<LK_DPP_QP_XOR1>((uint32_t) v);
+    return v;
+}
+// The record of a block whose 32 values h lie on the 32 lanes of a half-wave (r: the
+// lane's place); nothing is stored where !ok.
+template <int NP>
+__device__ __forceinline__ void lk_moe_record(float h, int r, bool ok, uint8_t * rec) {
+    const float m = lk_bfly32_max(h == h ? fabsf(h) : __builtin_inff());
+    const uint32_t am = __builtin_bit_cast(uint32_t, m);
+    const float up = lk_moe_up2<NP>(am);
+    int q[NP];
+    lk_moe_digits<NP>(h, up, q);
+    // two sums at once: each is at most 32 * 128
+    const int s01 = lk_moe_sum32(q[0] * 65536 + q[1]), s1 = (int) (short) s01, s0 = (s01 - s1) >> 16;
+    int s2 = 0;
+    if constexpr (NP == 3) s2 = lk_moe_sum32(q[2]);
+    if (!ok) return;
+#pragma unroll
+    for (int p = 0; p < NP; ++p) rec[32 * p + r] = (uint8_t) q[p];
+    if (r == 0)
+        *(lk_i4 *) (rec + 32 * NP) = lk_i4{ -8 * s0, -8 * s1, -8 * s2, __builtin_bit_cast(int, lk_moe_scale(am, up)) };
 }
 
 // ---- router scores, and the records of x -------------------------------------------
@@ -173,60 +229,58 @@ lk_k_moe_router(const LkMoeArgs a, int nE) {
 }
 
 // ---- choice of experts --------------------------------------------------------------
-// A wave per token: lane i holds experts i, i + 64, ...  A round takes the largest key
-// that is left; the first register and then the first lane that holds it are the
-// lowest index.
+// A wave per token: lane i holds experts i, i + 64, ... (NL registers, for up to 64 *
+// NL experts).  A round takes the largest key that is left; the first register and then the
+// first lane that holds it are the lowest index.
 __device__ __forceinline__ uint32_t lk_moe_key(float r) {    // orderable bits; 0: taken, 1: NaN; -0 as 0
     const uint32_t u = __builtin_bit_cast(uint32_t, r + 0.0f);
     return r != r ? 1u : (u >> 31) ? ~u : u | 0x80000000u;
 }
-// Token t's experts and weights into ids[0 .. k-1] and wts[0 .. k-1] (LDS).
-__device__ __forceinline__ void lk_moe_choose(const LkMoeArgs & a, int t, int * ids, float * wts) {
-    constexpr int NL = LK_MOE_MAX_EXPERTS / 64;
+// Token t's choice j and its weight in lane j < k; the other lanes hold -1.
+template <int NL>
+__device__ __forceinline__ void lk_moe_choose(const LkMoeArgs & a, int t, int & id, float & w) {
     const int lane = threadIdx.x & 63;
-    float l[NL];
+    float l[NL], b[NL];
     uint32_t key[NL];
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-        const int e = 64 * i + lane;
-        l[i] = e < a.E ? a.logits[(size_t) t * a.E + e] : -__builtin_inff();
+        const int e = 64 * i + lane < a.E ? 64 * i + lane : 0;
+        l[i] = a.logits[(size_t) t * a.E + e];
+        b[i] = a.bias ? a.bias[e] : 0.0f;
     }
-    float m = -__builtin_inff(), z = 1.0f;
+    float m = 0.0f, zi = 1.0f;
     if (a.score == LK_MOE_SOFTMAX) {
+        m = l[0];
 #pragma unroll
-        for (int i = 0; i < NL; ++i) m = fmaxf(m, l[i]);
-        m = lk_xrow_max(lk_row_max16(m));
-        z = 0.0f;
+        for (int i = 1; i < NL; ++i) m = fmaxf(m, l[i]);
+        m = lk_xrow_max(lk_row_max16(m));                // lanes past the experts repeat expert 0
+        float z = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NL; ++i) if (64 * i < a.E) z += 64 * i + lane < a.E ? expf(l[i] - m) : 0.0f;
-        z = lk_wave_sum(z);
+        for (int i = 0; i < NL; ++i) z += 64 * i + lane < a.E ? lk_moe_expn(l[i] - m) + (l[i] - l[i]) : 0.0f;
+        zi = 1.0f / lk_wave_sum(z);
     }
-    auto score = [&](float v) {
-        return a.score == LK_MOE_SOFTMAX ? expf(v - m) / z : 1.0f / (1.0f + expf(-v));
+    auto score = [&](float v) {                          // v - v: 0, or NaN for what is not finite
+        return a.score == LK_MOE_SOFTMAX ? (lk_moe_expn(v - m) + (v - v)) * zi : v == v ? lk_moe_sigmoid(v) : v;
     };
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-        const int e = 64 * i + lane;
-        key[i] = 0;
-        if (64 * i < a.E) {
-            const float r = a.bias ? score(l[i]) + a.bias[e < a.E ? e : 0] : l[i];
-            key[i] = e < a.E ? lk_moe_key(r) : 0;
-        }
+        const float r = a.bias ? score(l[i]) + b[i] : l[i];
+        key[i] = 64 * i + lane < a.E ? lk_moe_key(r) : 0;
     }
     float mine = 0.0f;                                   // lane j: the logit of choice j
-    int id = 0;
+    id = -1;
     for (int j = 0; j < a.k; ++j) {
         uint32_t best = key[0];
 #pragma unroll
         for (int i = 1; i < NL; ++i) best = lk_umax(best, key[i]);
-        best = (uint32_t) __builtin_amdgcn_readfirstlane((int) lk_wave_umax(best));
-        int e = -1;
+        best = lk_moe_top(best);
+        int e = 0;
         float v = 0.0f;
 #pragma unroll
         for (int i = NL - 1; i >= 0; --i) {
-            const uint64_t b = __ballot(key[i] == best);
-            if (b) {                                     // at least one: k <= E
-                e = 64 * i + __builtin_ctzll(b);
+            const uint64_t at = __ballot(key[i] == best);
+            if (NL == 1 || at) {                         // in one register at least: k <= E
+                e = 64 * i + __builtin_ctzll(at);
                 v = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, l[i]), e & 63));
             }
         }
@@ -235,106 +289,109 @@ __device__ __forceinline__ void lk_moe_choose(const LkMoeArgs & a, int t, int * 
         mine = lane == j ? v : mine;
         id = lane == j ? e : id;
     }
-    const float s = lane < a.k ? score(mine) : 0.0f;
-    float w = s;
-    if (a.renorm) w = s / (lk_row_sum16(s) + 1e-20f);    // k <= 8: the first row of 16 lanes
-    if (lane < a.k) {
-        ids[lane] = id;
-        wts[lane] = w * a.scale;
-    }
+    w = lane < a.k ? score(mine) : 0.0f;
+    if (a.renorm) w = w / (lk_row_sum16(w) + 1e-20f);    // k <= 8: the first row of 16 lanes
+    w *= a.scale;
 }
-// The choices of all tokens for the caller and the launches that follow.
-__device__ __forceinline__ void lk_moe_publish(const LkMoeArgs & a, const int * ids, const float * wts) {
-    for (int i = threadIdx.x; i < a.T * a.k; i += blockDim.x) {
-        a.ids[i] = ids[i];
-        a.wts[i] = wts[i];
-        if (a.ids_out) a.ids_out[i] = ids[i];
-        if (a.wts_out) a.wts_out[i] = wts[i];
-    }
-}
-
 // More than LK_MOE_FEW tokens: one workgroup of 16 waves chooses for all of them and
-// sorts the assignments by expert (counting sort; a wave per expert keeps their order).
+// sorts the assignments by expert.
+template <int NL>
 __global__ void __launch_bounds__(1024)
 lk_k_moe_route(const LkMoeArgs a) {
-    __shared__ int ids[LK_MOE_MAX_TOKENS * LK_MOE_MAX_TOP_K];
-    __shared__ float wts[LK_MOE_MAX_TOKENS * LK_MOE_MAX_TOP_K];
-    __shared__ int cnt[LK_MOE_MAX_EXPERTS], from[LK_MOE_MAX_EXPERTS];
-    __shared__ uint64_t words[LK_MOE_MAX_EXPERTS / 64];
-    __shared__ int sums[LK_MOE_MAX_EXPERTS / 64];
+    __shared__ int ids[LK_MOE_MAX_TOKENS * LK_MOE_MAX_TOP_K], cnt[LK_MOE_MAX_EXPERTS], slot[LK_MOE_MAX_EXPERTS];
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), na = a.T * a.k;
     LkMoeTab & tab = *(LkMoeTab *) a.tab;
     if (tid < LK_MOE_MAX_EXPERTS) cnt[tid] = 0;
-    for (int t = wv; t < a.T; t += 16) lk_moe_choose(a, t, ids + t * a.k, wts + t * a.k);
     __syncthreads();
-    lk_moe_publish(a, ids, wts);
-    if (tid < na) atomicAdd(&cnt[ids[tid]], 1);          // na <= 512; counts have no order
-    __syncthreads();
-    int c = 0, before = 0, slot = 0;
-    if (tid < LK_MOE_MAX_EXPERTS) {                      // waves 0 .. 3: exclusive sums over the experts
-        c = cnt[tid];
-        int s = c;
-        for (int o = 1; o < 64; o <<= 1) {
-            const int u = __shfl_up(s, o, 64);
-            if (lane >= o) s += u;
-        }
-        before = s - c;
-        const uint64_t b = __ballot(c > 0);
-        slot = __popcll(b & ((1ull << lane) - 1));
-        if (lane == 63) { words[wv] = b; sums[wv] = s; }
-    }
-    __syncthreads();
-    if (tid < LK_MOE_MAX_EXPERTS) {
-        for (int i = 0; i < wv; ++i) { before += sums[i]; slot += __popcll(words[i]); }
-        from[tid] = before;
-        if (c > 0) {
-            tab.e[slot] = tid;
-            tab.from[slot] = before;
-        }
-        if (tid == LK_MOE_MAX_EXPERTS - 1) {
-            slot += c > 0;
-            tab.slots = slot;
-            tab.from[slot] = na;
+    for (int t = wv; t < a.T; t += 16) {
+        int id;
+        float w;
+        lk_moe_choose<NL>(a, t, id, w);
+        if (id >= 0) {
+            const int i = t * a.k + lane;
+            ids[i] = id;
+            a.wts[i] = w;
+            if (a.ids_out) a.ids_out[i] = id;
+            if (a.wts_out) a.wts_out[i] = w;
+            atomicAdd(&cnt[id], 1);                      // counts have no order
         }
     }
     __syncthreads();
-    for (int e = wv; e < a.E; e += 16) {
+    if (tid < a.E) {
+        const int c = cnt[tid];
+        int s = 0;
+        for (int e = 0; e < a.E; ++e) s += cnt[e] > c || (cnt[e] == c && e < tid);
+        slot[tid] = s;
+        tab.slot[s].e = tid;
+        tab.slot[s].n = c;
+    }
+    __syncthreads();
+    for (int e = wv; e < a.E; e += 16) {                 // a wave per expert keeps the order
         if (cnt[e] == 0) continue;
-        int n = from[e];
+        int32_t * list = tab.list[slot[e]];
+        int n = 0;
         for (int i0 = 0; i0 < na; i0 += 64) {
             const bool hit = i0 + lane < na && ids[i0 + lane] == e;
             const uint64_t b = __ballot(hit);
-            if (hit) tab.list[n + __popcll(b & ((1ull << lane) - 1))] = i0 + lane;
+            if (hit) list[n + __popcll(b & ((1ull << lane) - 1))] = i0 + lane;
             n += __popcll(b);
         }
     }
 }
 
 // ---- the products -------------------------------------------------------------------
-// R weight rows of NM matrices (qs, d: the first of the rows) times TK rows of records
-// (rec + trow[t] * bpr records), over the groups of 64 / R blocks of a row,
-// U consecutive ones at a time, of which this is part g0 of gs.  Lane (c = l % R, g = l /
-// R) takes block g of a group of weight row c, whole: 16 bytes, its scale, and of every
-// record row the block's digits.  Those are the same for the R lanes of a block: the
-// wave copies them, one run of memory, into its own part of LDS (xs) and every lane reads
-// them there.
+// 8 weight rows of NM matrices (qs, d: the first of the rows) times TK rows of records
+// (rec + trow[t] * bpr records), over the steps of 8 blocks of a row, U consecutive ones at
+// a time, of which this is part g0 of gs.  Lane (c = l % 8, g = l / 8) takes block g of a
+// step of weight row c, whole: 16 bytes, its scale, and of every record row the block's
+// digits.  So a load covers a whole 128-byte line of each of 8 rows: with 16 rows and 64
+// bytes of each, 141 MB of weights came at 3.0 TB/s, and no other part of the kernel was
+// the limit.  The digits are the same for the 8 lanes of a block: the wave copies them, one
+// run of memory, into its own part of LDS (xs) and every lane reads them there.
 // acc[t][m]: this lane's blocks; the sum over the lanes of a row is the caller's.
 // Every address is a wave-uniform base and a 32-bit offset: an expert's planes are below
 // 4 GiB (LK_MOE_MAX_DIM).
 template <typename V>
 __device__ __forceinline__ V lk_moe_ld(const void * base, uint32_t off) { return *(const V *) ((const char *) base + off); }
-template <int NP, int R, int U>
-struct LkMoeX {                                          // one row's digits of a step: Z pieces of 16 bytes
-    static constexpr int NB = 64 / R, Z = U * NB * LkMoeRec<NP>::PIECES, NZ = (Z + 63) / 64;
+// A block's record x times the lane's block of NM weight rows (its 32 nibbles: lo, hi).
+template <int NP, int NM>
+__device__ __forceinline__ void lk_moe_token_dots(const lk_u4 * x, bool in, const uint32_t (&lo)[NM][4], const uint32_t (&hi)[NM][4],
+                                                  const float (&dv)[NM], float (&acc)[NM]) {
+    lk_u4 q[2 * NP];
+#pragma unroll
+    for (int p = 0; p < 2 * NP; ++p) q[p] = x[p];
+    const lk_i4 meta = __builtin_bit_cast(lk_i4, x[2 * NP]);
+    const int m3 = meta[3];                              // a copy: bit_cast of a vector's element takes element 0
+    const float sc = in ? __builtin_bit_cast(float, m3) : 0.0f;                    // a block past the row's end counts nothing
+#pragma unroll
+    for (int m = 0; m < NM; ++m) {
+        float f = 0.0f;
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            int s = meta[p];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                s = __builtin_amdgcn_sdot4((int) lo[m][k], (int) q[2 * p][k], s, false);
+                s = __builtin_amdgcn_sdot4((int) hi[m][k], (int) q[2 * p + 1][k], s, false);
+            }
+            f = p ? __builtin_fmaf(f, 256.0f, (float) s) : (float) s;
+        }
+        acc[m] = __builtin_fmaf(dv[m] * sc, f, acc[m]);
+        // done here: left to itself the compiler reads the digits of all tokens first and spills
+        asm volatile("" : "+v"(acc[m]) :: "memory");
+    }
+}
+template <int NP, int U>
+struct LkMoeX {                                          // one row's digits of U steps: Z pieces of 16 bytes
+    static constexpr int Z = U * 8 * LkMoeRec<NP>::PIECES, NZ = (Z + 63) / 64;
     lk_u4 x[64 * NZ];
 };
-template <int NP, int NM, int R, int U, int TK>
+template <int NP, int NM, int U, int TK>
 __device__ __forceinline__ void lk_moe_rows(const uint8_t * const (&qs)[NM], const _Float16 * const (&d)[NM],
                                             const uint8_t * rec, int bpr, const int (&trow)[TK], int g0, int gs,
-                                            LkMoeX<NP, R, U> * xs, float (&acc)[TK][NM]) {
-    typedef LkMoeX<NP, R, U> X;
-    constexpr int NB = X::NB, PC = LkMoeRec<NP>::PIECES, NZ = X::NZ;
-    const int lane = threadIdx.x & 63, c = lane % R, g = lane / R;
+                                            LkMoeX<NP, U> * xs, float (&acc)[TK][NM]) {
+    constexpr int PC = LkMoeRec<NP>::PIECES, NZ = LkMoeX<NP, U>::NZ, NB = 8;
+    const int lane = threadIdx.x & 63, c = lane & 7, g = lane >> 3;
     const int ng = (bpr + NB - 1) / NB;
 #pragma unroll 1
     for (int gi = g0 * U; gi < ng; gi += gs * U) {
@@ -379,101 +436,67 @@ __device__ __forceinline__ void lk_moe_rows(const uint8_t * const (&qs)[NM], con
             }
 #pragma unroll
             for (int t = 0; t < TK; ++t) {
-                asm volatile("" ::: "memory");           // one token's digits at a time: all at once spill
-                const lk_u4 * x = xs[t].x + (u * NB + g) * PC;
-                lk_u4 q[2 * NP];
-#pragma unroll
-                for (int p = 0; p < 2 * NP; ++p) q[p] = x[p];
-                const lk_i4 meta = __builtin_bit_cast(lk_i4, x[2 * NP]);
-                const int m3 = meta[3];                  // a copy: bit_cast of a vector's element takes element 0
-                const float sc = in ? __builtin_bit_cast(float, m3) : 0.0f;        // a block past the row's end counts nothing
-#pragma unroll
-                for (int m = 0; m < NM; ++m) {
-                    float f = 0.0f;
-#pragma unroll
-                    for (int p = 0; p < NP; ++p) {
-                        int s = meta[p];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            s = __builtin_amdgcn_sdot4((int) lo[m][k], (int) q[2 * p][k], s, false);
-                            s = __builtin_amdgcn_sdot4((int) hi[m][k], (int) q[2 * p + 1][k], s, false);
-                        }
-                        f = p ? __builtin_fmaf(f, 256.0f, (float) s) : (float) s;
-                    }
-                    acc[t][m] = __builtin_fmaf(dv[m] * sc, f, acc[t][m]);
-                }
+                lk_moe_token_dots<NP, NM>(xs[t].x + (u * NB + g) * PC, in, lo, hi, dv, acc[t]);
             }
         }
         __builtin_amdgcn_wave_barrier();
     }
 }
-// The sum over the lanes that hold blocks of one row (64 / R of them), in every lane.
-template <int R>
-__device__ __forceinline__ float lk_moe_lanes(float v) {
-    if constexpr (R == 8) v += lk_dpp<LK_DPP_ROR8>(v);
-    return lk_xrow_sum(v);
+// The sum over the eight lanes that hold blocks of one row, in every lane.
+__device__ __forceinline__ float lk_moe_lanes(float v) { return lk_xrow_sum(v + lk_dpp<LK_DPP_ROR8>(v)); }
+
+// Where a wave of a gate/up workgroup finds its 16 + 16 of the tile's 32 rows (half:
+// 0 or 1): matrices 0, 1 the gate's rows 16 half .. +15, eight each, 2, 3 the up's.
+__device__ __forceinline__ void lk_moe_up_rows(const LkMoeArgs & a, int e, int half, const uint8_t * (&qs)[4], const _Float16 * (&d)[4]) {
+    const int bpr = a.hidden / 32;
+    const size_t row = (size_t) e * a.ffn + blockIdx.x * 32 + 16 * half;        // ffn is a multiple of 32: whole tiles
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+        qs[m] = a.qs[m >> 1] + (row + 8 * (m & 1)) * bpr * 16;
+        d[m] = a.d[m >> 1] + (row + 8 * (m & 1)) * bpr;
+    }
 }
 
-// 32 rows of one expert's gate and up products for N assignments (as[0 .. N-1]), and
-// what follows of them: the records of h.  N is known at compile time: with branches on
-// it the compiler keeps the digits of all tokens at once and spills.
+// 32 rows of one expert's gate and up products for N assignments (as[0 .. N-1] in LDS; the
+// only one: as0), and what follows of them: the records of h.  Wave w has half w & 1 of the rows and part w >>
+// 1 of K.  N is known at compile time: with branches on it the compiler keeps the digits
+// of all tokens at once and spills.
 template <int NP>
 struct LkMoeUp {
     static constexpr int U = 2, TK = 4;
-    LkMoeX<NP, 16, U> xs[LK_MOE_NW][TK];
-    float part[LK_MOE_NW][4][TK][16];
+    LkMoeX<NP, U> xs[LK_MOE_NW][TK];
+    float part[LK_MOE_NW / 2][2][TK][32];                // [part of K][gate, up][token][row]
 };
 template <int NP, int N>
-__device__ __forceinline__ void lk_moe_up_tile(const LkMoeArgs & a, int e, const int * as, LkMoeUp<NP> & sh) {
+__device__ __forceinline__ void lk_moe_up_tile(const LkMoeArgs & a, int e, const int * as, int as0, LkMoeUp<NP> & sh) {
     constexpr int U = LkMoeUp<NP>::U, REC = LkMoeRec<NP>::BYTES;
-    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
-    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int bpr = a.hidden / 32, F = a.ffn, r0 = blockIdx.x * 32;
-    const size_t row = (size_t) e * F + r0;              // F is a multiple of 32: whole tiles
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 7, g = lane >> 3;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), half = wv & 1, kp = wv >> 1, F = a.ffn;
     const uint8_t * qs[4];
     const _Float16 * d[4];
-#pragma unroll
-    for (int m = 0; m < 4; ++m) {
-        qs[m] = a.qs[m >> 1] + (row + 16 * (m & 1)) * bpr * 16;
-        d[m] = a.d[m >> 1] + (row + 16 * (m & 1)) * bpr;
-    }
+    lk_moe_up_rows(a, e, half, qs, d);
     int trow[N];
 #pragma unroll
-    for (int r = 0; r < N; ++r) trow[r] = __builtin_amdgcn_readfirstlane(as[r] / a.k);
+    for (int r = 0; r < N; ++r) trow[r] = lk_moe_token(a, N == 1 ? as0 : __builtin_amdgcn_readfirstlane(as[r]));
     float acc[N][4] = {};
-    lk_moe_rows<NP, 4, 16, U, N>(qs, d, a.xr, bpr, trow, wv, LK_MOE_NW, sh.xs[wv], acc);
+    lk_moe_rows<NP, 4, U, N>(qs, d, a.xr, a.hidden / 32, trow, kp, LK_MOE_NW / 2, sh.xs[wv], acc);
 #pragma unroll
     for (int t = 0; t < N; ++t)
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-            const float v = lk_moe_lanes<16>(acc[t][m]);
-            if (g == m) sh.part[wv][m][t][c] = v;
+            const float v = lk_moe_lanes(acc[t][m]);
+            if (g == m) sh.part[kp][m >> 1][t][16 * half + 8 * (m & 1) + c] = v;
         }
     __syncthreads();
     if (tid < 32 * N) {                                  // token t, row r of the 32
         const int t = tid >> 5, r = tid & 31;
         float gt = 0.0f, up = 0.0f;
 #pragma unroll
-        for (int k = 0; k < LK_MOE_NW; ++k) {
-            gt += sh.part[k][r >> 4][t][r & 15];
-            up += sh.part[k][2 + (r >> 4)][t][r & 15];
+        for (int k = 0; k < LK_MOE_NW / 2; ++k) {
+            gt += sh.part[k][0][t][r];
+            up += sh.part[k][1][t][r];
         }
-        const float h = gt / (1.0f + expf(-gt)) * up;
-        uint32_t am = __builtin_bit_cast(uint32_t, h) & 0x7FFFFFFFu;
-        for (int o = 16; o > 0; o >>= 1) am = lk_umax(am, (uint32_t) __shfl_xor((int) am, o, 32));
-        const float p2 = lk_moe_up2<NP>(am);
-        int q[NP], s[3] = { 0, 0, 0 };
-        lk_moe_digits<NP>(h, p2, q);
-#pragma unroll
-        for (int p = 0; p < NP; ++p) {
-            s[p] = q[p];
-            for (int o = 16; o > 0; o >>= 1) s[p] += __shfl_xor(s[p], o, 32);
-        }
-        uint8_t * rc = a.hr + ((size_t) as[t] * (F / 32) + blockIdx.x) * REC;
-#pragma unroll
-        for (int p = 0; p < NP; ++p) rc[32 * p + r] = (uint8_t) q[p];
-        if (r == 0)
-            *(lk_i4 *) (rc + 32 * NP) = lk_i4{ -8 * s[0], -8 * s[1], -8 * s[2], __builtin_bit_cast(int, lk_moe_scale(am, p2)) };
+        lk_moe_record<NP>(lk_moe_h(gt, up), r, true, a.hr + ((size_t) (N == 1 ? as0 : as[t]) * (F / 32) + blockIdx.x) * REC);
     }
 }
 
@@ -481,46 +504,208 @@ __device__ __forceinline__ void lk_moe_up_tile(const LkMoeArgs & a, int e, const
 template <int NP>
 __device__ __forceinline__ void lk_moe_up_tiles(const LkMoeArgs & a, int e, const int * as, int n, LkMoeUp<NP> & sh) {
     for (; n > 0; n -= 4, as += 4) {
-        if (n >= 4)      lk_moe_up_tile<NP, 4>(a, e, as, sh);
-        else if (n == 3) lk_moe_up_tile<NP, 3>(a, e, as, sh);
-        else if (n == 2) lk_moe_up_tile<NP, 2>(a, e, as, sh);
-        else             lk_moe_up_tile<NP, 1>(a, e, as, sh);
+        if (n >= 4)      lk_moe_up_tile<NP, 4>(a, e, as, 0, sh);
+        else if (n == 3) lk_moe_up_tile<NP, 3>(a, e, as, 0, sh);
+        else if (n == 2) lk_moe_up_tile<NP, 2>(a, e, as, 0, sh);
+        else             lk_moe_up_tile<NP, 1>(a, e, as, __builtin_amdgcn_readfirstlane(as[0]), sh);
         if (n > 4) __syncthreads();                      // part has been read
     }
 }
 
 // Up to LK_MOE_FEW tokens; grid (ffn / 32, T * k): the workgroups of an assignment
 // whose expert an earlier one has end at once.
-template <int NP>
+template <int NP, int NL>
 __global__ void __launch_bounds__(64 * LK_MOE_NW, 4)
 lk_k_moe_up_few(const LkMoeArgs a) {
     __shared__ int ids[LK_MOE_FEW * LK_MOE_MAX_TOP_K], as[LK_MOE_FEW];
-    __shared__ float wts[LK_MOE_FEW * LK_MOE_MAX_TOP_K];
     __shared__ LkMoeUp<NP> sh;
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), na = a.T * a.k;
-    if (wv < a.T) lk_moe_choose(a, wv, ids + wv * a.k, wts + wv * a.k);
-    __syncthreads();
-    if (blockIdx.x == 0 && blockIdx.y == 0) lk_moe_publish(a, ids, wts);
-    const int mine = lane < na ? ids[lane] : -1;
+    const bool tells = blockIdx.x == 0 && blockIdx.y == 0;          // the one that writes the choices down
+    int mine = -1;
+    if (a.T == 1 || wv < a.T) {                          // one token: every wave for itself
+        const int t = a.T == 1 ? 0 : wv;
+        float w;
+        lk_moe_choose<NL>(a, t, mine, w);
+        if (mine >= 0) {
+            if (a.T > 1) ids[t * a.k + lane] = mine;
+            if (tells && (a.T > 1 || wv == 0)) {
+                const int i = t * a.k + lane;
+                a.ids[i] = mine;
+                a.wts[i] = w;
+                if (a.ids_out) a.ids_out[i] = mine;
+                if (a.wts_out) a.wts_out[i] = w;
+            }
+        }
+    }
+    if (a.T > 1) {
+        __syncthreads();
+        mine = lane < na ? ids[lane] : -1;
+    }
     const int e = __builtin_amdgcn_readlane(mine, blockIdx.y);
     const uint64_t hits = __ballot(mine == e);
     if (__builtin_ctzll(hits) != (int) blockIdx.y) return;
+    if (a.T == 1) {
+        lk_moe_up_tile<NP, 1>(a, e, as, blockIdx.y, sh);
+        return;
+    }
     if (wv == 0 && mine == e) as[__popcll(hits & ((1ull << lane) - 1))] = lane;
     __syncthreads();
     lk_moe_up_tiles<NP>(a, e, as, __popcll(hits), sh);
 }
 
+// More tokens: a workgroup of 4 waves has 32 rows (up: of gate and up) or 64 (down) of
+// one expert and up to eight of its assignments at a time.  Wave w has half w & 1 of the rows
+// (four matrices of 8 rows) and every second step of 8 blocks of K; it copies a step's
+// digits into its own part of LDS while the step's weights are on their way, which are
+// asked for before the dots of the step before.  The loop is kept short (one step, four
+// counts of tokens): with two steps and six counts the kernel had 57 KB of code, and
+// fetching it under a saturated memory took up to 5 us a workgroup.
 template <int NP>
-__global__ void __launch_bounds__(64 * LK_MOE_NW, 4)
-lk_k_moe_up(const LkMoeArgs a) {
-    __shared__ int as[LK_MOE_MAX_TOKENS];
-    __shared__ LkMoeUp<NP> sh;
-    const LkMoeTab & tab = *(const LkMoeTab *) a.tab;
-    if ((int) blockIdx.y >= tab.slots) return;
-    const int e = tab.e[blockIdx.y], from = tab.from[blockIdx.y], n = tab.from[blockIdx.y + 1] - from;
-    if ((int) threadIdx.x < n) as[threadIdx.x] = tab.list[from + threadIdx.x];
+struct LkMoeShare {
+    static constexpr int Z = 8 * LkMoeRec<NP>::PIECES;   // pieces of a step's digits
+    lk_u4 x[4][8][Z];
+    float part[2][8][64];                                // [part of K][token][row of 32 gate and 32 up, or of 64]
+};
+template <int NP, int N>
+__device__ __forceinline__ void lk_moe_many_rows(const uint8_t * const (&qs)[4], const _Float16 * const (&d)[4], const uint8_t * rec,
+                                                 int bpr, const int (&trow)[N], LkMoeShare<NP> & sh, float (&acc)[N][4]) {
+    constexpr int PC = LkMoeRec<NP>::PIECES, Z = LkMoeShare<NP>::Z;
+    static_assert(Z <= 64, "a step's digits are one copy");
+    const int lane = threadIdx.x & 63, c = lane & 7, g = lane >> 3, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int ns = (bpr + 7) / 8;                        // steps; this wave's are s0, s0 + 2, ...
+    const uint32_t lds = lk_lds_addr(&sh.x[wv][0][0]);
+    lk_u4 w[4];
+    _Float16 dw[4];
+    auto load = [&](int s) {
+        const int b = 8 * s + g;
+        const uint32_t wb = (uint32_t) (c * bpr + (b < bpr ? b : bpr - 1));                      // in bounds
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            w[m] = lk_moe_ld<lk_u4>(qs[m], wb * 16u);
+            dw[m] = lk_moe_ld<_Float16>(d[m], wb * 2u);
+        }
+    };
+    auto copy = [&](int s) {
+        const int left = (bpr - 8 * s) * PC;             // pieces to the row's end; none: the row's first
+#pragma unroll
+        for (int t = 0; t < N; ++t) {
+            const uint8_t * src = rec + ((size_t) trow[t] * bpr + (left > 0 ? 8 * s : 0)) * (PC * 16);
+            if (lane < Z) lk_dma16c_so(src, 16u * (lane < left ? lane : 0), lds + 16u * (t * Z));
+        }
+    };
+    load(wv >> 1);
+    copy(wv >> 1);
+#pragma unroll 1
+    for (int s = wv >> 1; s < ns; s += 2) {
+        const bool in = 8 * s + g < bpr;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // the copies; the weights, asked for before, come with them
+        uint32_t lo[4][4], hi[4][4];
+        float dv[4];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            dv[m] = (float) dw[m];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                lo[m][k] = w[m][k] & 0x0F0F0F0Fu;
+                hi[m][k] = (w[m][k] >> 4) & 0x0F0F0F0Fu;
+            }
+        }
+        load(s + 2);                                     // past the last: in bounds, not used
+#pragma unroll
+        for (int t = 0; t < N; ++t) {
+            lk_moe_token_dots<NP, 4>(&sh.x[wv][t][g * PC], in, lo, hi, dv, acc[t]);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");          // the digits have been read
+        copy(s + 2);
+    }
+    // the last copies, not used, end before LDS is given to another workgroup
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
+// N assignments (as, of which n count) of an expert.
+template <int NP, int N>
+__device__ __forceinline__ void lk_moe_up_many(const LkMoeArgs & a, int e, const int (&as)[N], int n, LkMoeShare<NP> & sh) {
+    const int F = a.ffn, tid = threadIdx.x, lane = tid & 63, c = lane & 7, g = lane >> 3;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), half = wv & 1;
+    const uint8_t * qs[4];
+    const _Float16 * d[4];
+    lk_moe_up_rows(a, e, half, qs, d);
+    int trow[N];
+#pragma unroll
+    for (int t = 0; t < N; ++t) trow[t] = lk_moe_token(a, as[t]);
+    float acc[N][4] = {};
+    lk_moe_many_rows<NP, N>(qs, d, a.xr, a.hidden / 32, trow, sh, acc);
+#pragma unroll
+    for (int t = 0; t < N; ++t)
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            const float v = lk_moe_lanes(acc[t][m]);
+            if (g == m) sh.part[wv >> 1][t][32 * (m >> 1) + 16 * half + 8 * (m & 1) + c] = v;
+        }
     __syncthreads();
-    lk_moe_up_tiles<NP>(a, e, as, n, sh);
+    const int t = tid >> 5, r = tid & 31;
+    if (t < N) {                                         // whole halves of waves
+        const float gt = sh.part[0][t][r] + sh.part[1][t][r], up = sh.part[0][t][32 + r] + sh.part[1][t][32 + r];
+        int at = as[0];
+#pragma unroll
+        for (int k = 1; k < N; ++k) at = t == k ? as[k] : at;
+        lk_moe_record<NP>(lk_moe_h(gt, up), r, t < n, a.hr + ((size_t) at * (F / 32) + blockIdx.x) * LkMoeRec<NP>::BYTES);
+    }
+}
+template <int NP, int N>
+__device__ __forceinline__ void lk_moe_down_many(const LkMoeArgs & a, int e, const int (&as)[N], int n, LkMoeShare<NP> & sh) {
+    const int bpr = a.ffn / 32, H = a.hidden, r0 = blockIdx.x * 64, tid = threadIdx.x, lane = tid & 63, c = lane & 7, g = lane >> 3;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), half = wv & 1;
+    const uint8_t * qs[4];
+    const _Float16 * d[4];
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {                        // a last tile of 32 rows: those twice
+        const size_t row = (size_t) e * H + (r0 + 32 * half < H ? r0 + 32 * half : r0) + 8 * m;
+        qs[m] = a.qs[2] + row * bpr * 16;
+        d[m] = a.d[2] + row * bpr;
+    }
+    float acc[N][4] = {};
+    lk_moe_many_rows<NP, N>(qs, d, a.hr, bpr, as, sh, acc);
+#pragma unroll
+    for (int t = 0; t < N; ++t)
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            const float v = lk_moe_lanes(acc[t][m]);
+            if (g == m) sh.part[wv >> 1][t][32 * half + 8 * m + c] = v;
+        }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < N; ++t)                          // a wave per assignment
+        if ((t & 3) == wv && t < n && r0 + lane < H)
+            a.y[(size_t) as[t] * H + r0 + lane] = sh.part[0][t][lane] + sh.part[1][t][lane];
+}
+
+// grid (row tiles, slots)
+template <int NP, bool UP>
+__global__ void __launch_bounds__(LK_MOE_THREADS, NP == 3 ? 3 : 4)
+lk_k_moe_many(const LkMoeArgs a) {
+    __shared__ LkMoeShare<NP> sh;
+    // written by the launch before: read as constants, by scalar loads
+    typedef const __attribute__((address_space(4))) LkMoeTab Tab;
+    Tab & tab = *(Tab *) (uintptr_t) a.tab;
+    const int slot = blockIdx.y, e = tab.slot[slot].e, n = tab.slot[slot].n;
+    auto go = [&](auto count, int at) {
+        constexpr int N = decltype(count)::value;
+        const int left = n - at < N ? n - at : N;
+        int as[N];
+#pragma unroll
+        for (int t = 0; t < N; ++t) as[t] = tab.list[slot][at + (t < left ? t : 0)];
+        if constexpr (UP) lk_moe_up_many<NP, N>(a, e, as, left, sh);
+        else              lk_moe_down_many<NP, N>(a, e, as, left, sh);
+    };
+    for (int at = 0; at < n; at += 8) {
+        if (at) __syncthreads();                         // part has been read
+        const int left = n - at;
+        if (left > 4)       go(LkInt<8>{}, at);
+        else if (left > 2)  go(LkInt<4>{}, at);
+        else if (left == 2) go(LkInt<2>{}, at);
+        else                go(LkInt<1>{}, at);
+    }
 }
 
 // Up to LK_MOE_FEW tokens: a workgroup of 16 waves has 8 rows of every expert that was
@@ -531,7 +716,7 @@ __global__ void __launch_bounds__(64 * LK_MOE_NWF, 4)
 lk_k_moe_down_few(const LkMoeArgs a) {
     typedef typename LkElem<TYPE>::type T;
     constexpr int R = 8, U = 2, TK = 2, MAXA = LK_MOE_FEW * LK_MOE_MAX_TOP_K;
-    __shared__ LkMoeX<NP, R, U> xs[LK_MOE_NWF][TK];
+    __shared__ LkMoeX<NP, U> xs[LK_MOE_NWF][TK];
     // [q][assignment][row]: q * assignments is at most 16 / experts * (experts * LK_MOE_FEW), or MAXA
     __shared__ float part[LK_MOE_NWF * LK_MOE_FEW][R];
     static_assert(LK_MOE_NWF * LK_MOE_FEW >= MAXA, "part");
@@ -566,14 +751,14 @@ lk_k_moe_down_few(const LkMoeArgs a) {
                 const int trow[2] = { t0, __builtin_ctzll(hits) };
                 hits &= hits - 1;
                 float acc[2][1] = {};
-                lk_moe_rows<NP, 1, R, U, 2>(qs, d, a.hr, bpr, trow, q, Q, xs[wv], acc);
-                const float v0 = lk_moe_lanes<R>(acc[0][0]), v1 = lk_moe_lanes<R>(acc[1][0]);
+                lk_moe_rows<NP, 1, U, 2>(qs, d, a.hr, bpr, trow, q, Q, xs[wv], acc);
+                const float v0 = lk_moe_lanes(acc[0][0]), v1 = lk_moe_lanes(acc[1][0]);
                 if (g < 2) part[q * na + trow[g]][c] = g ? v1 : v0;
             } else {
                 const int trow[1] = { t0 };
                 float acc[1][1] = {};
-                lk_moe_rows<NP, 1, R, U, 1>(qs, d, a.hr, bpr, trow, q, Q, xs[wv], acc);
-                const float v0 = lk_moe_lanes<R>(acc[0][0]);
+                lk_moe_rows<NP, 1, U, 1>(qs, d, a.hr, bpr, trow, q, Q, xs[wv], acc);
+                const float v0 = lk_moe_lanes(acc[0][0]);
                 if (g == 0) part[q * na + t0][c] = v0;
             }
         }
@@ -590,63 +775,6 @@ lk_k_moe_down_few(const LkMoeArgs a) {
         }
         if (a.res) o = rs + o;
         ((T *) a.out)[(size_t) ot * a.ldo + orow] = (T) o;
-    }
-}
-
-// 32 rows of one expert's down product for N assignments.
-template <int NP>
-struct LkMoeDown {
-    static constexpr int U = 2, TK = 4;
-    LkMoeX<NP, 16, U> xs[LK_MOE_NW][TK];
-    float part[LK_MOE_NW][2][TK][16];
-};
-template <int NP, int N>
-__device__ __forceinline__ void lk_moe_down_tile(const LkMoeArgs & a, int e, const int * as, LkMoeDown<NP> & sh) {
-    constexpr int U = LkMoeDown<NP>::U;
-    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
-    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), r0 = blockIdx.x * 32, bpr = a.ffn / 32;
-    const size_t row = (size_t) e * a.hidden + r0;
-    const uint8_t * const qs[2] = { a.qs[2] + row * bpr * 16, a.qs[2] + (row + 16) * bpr * 16 };
-    const _Float16 * const d[2] = { a.d[2] + row * bpr, a.d[2] + (row + 16) * bpr };
-    int trow[N];
-#pragma unroll
-    for (int r = 0; r < N; ++r) trow[r] = __builtin_amdgcn_readfirstlane(as[r]);
-    float acc[N][2] = {};
-    lk_moe_rows<NP, 2, 16, U, N>(qs, d, a.hr, bpr, trow, wv, LK_MOE_NW, sh.xs[wv], acc);
-#pragma unroll
-    for (int t = 0; t < N; ++t)
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            const float v = lk_moe_lanes<16>(acc[t][m]);
-            if (g == m) sh.part[wv][m][t][c] = v;
-        }
-    __syncthreads();
-    if (tid < 32 * N) {
-        const int t = tid >> 5, r = tid & 31;
-        float y = 0.0f;
-#pragma unroll
-        for (int k = 0; k < LK_MOE_NW; ++k) y += sh.part[k][r >> 4][t][r & 15];
-        a.y[(size_t) as[t] * a.hidden + r0 + r] = y;
-    }
-}
-
-template <int NP>
-__global__ void __launch_bounds__(64 * LK_MOE_NW, 4)
-lk_k_moe_down(const LkMoeArgs a) {
-    __shared__ int as[LK_MOE_MAX_TOKENS];
-    __shared__ LkMoeDown<NP> sh;
-    const LkMoeTab & tab = *(const LkMoeTab *) a.tab;
-    if ((int) blockIdx.y >= tab.slots) return;
-    const int e = tab.e[blockIdx.y], from = tab.from[blockIdx.y], n = tab.from[blockIdx.y + 1] - from;
-    if ((int) threadIdx.x < n) as[threadIdx.x] = tab.list[from + threadIdx.x];
-    __syncthreads();
-    const int * p = as;
-    for (int left = n; left > 0; left -= 4, p += 4) {
-        if (left >= 4)      lk_moe_down_tile<NP, 4>(a, e, p, sh);
-        else if (left == 3) lk_moe_down_tile<NP, 3>(a, e, p, sh);
-        else if (left == 2) lk_moe_down_tile<NP, 2>(a, e, p, sh);
-        else                lk_moe_down_tile<NP, 1>(a, e, p, sh);
-        if (left > 4) __syncthreads();                   // part has been read
     }
 }
 
@@ -718,14 +846,21 @@ static void lk_moe_go(const LkMoeArgs & a, hipStream_t st) {
     const int nE = (a.E + 3) / 4, na = a.T * a.k, slots = na < a.E ? na : a.E;
     hipLaunchKernelGGL((lk_k_moe_router<TYPE, NP>), dim3(nE + (a.hidden / 8 + LK_MOE_THREADS - 1) / LK_MOE_THREADS, (a.T + 3) / 4),
                        dim3(LK_MOE_THREADS), 0, st, a, nE);
+    auto go = [&](auto regs) {                           // registers of 64 experts a choosing wave holds
+        constexpr int NL = decltype(regs)::value;
+        if (a.T <= LK_MOE_FEW)
+            hipLaunchKernelGGL((lk_k_moe_up_few<NP, NL>), dim3(a.ffn / 32, na), dim3(64 * LK_MOE_NW), 0, st, a);
+        else
+            hipLaunchKernelGGL((lk_k_moe_route<NL>), dim3(1), dim3(1024), 0, st, a);
+    };
+    if (a.E <= 64) go(LkInt<1>{});
+    else           go(LkInt<LK_MOE_MAX_EXPERTS / 64>{});
     if (a.T <= LK_MOE_FEW) {
-        hipLaunchKernelGGL((lk_k_moe_up_few<NP>), dim3(a.ffn / 32, na), dim3(64 * LK_MOE_NW), 0, st, a);
         hipLaunchKernelGGL((lk_k_moe_down_few<TYPE, NP>), dim3(a.hidden / 8), dim3(64 * LK_MOE_NWF), 0, st, a);
         return;
     }
-    hipLaunchKernelGGL(lk_k_moe_route, dim3(1), dim3(1024), 0, st, a);
-    hipLaunchKernelGGL((lk_k_moe_up<NP>), dim3(a.ffn / 32, slots), dim3(64 * LK_MOE_NW), 0, st, a);
-    hipLaunchKernelGGL((lk_k_moe_down<NP>), dim3(a.hidden / 32, slots), dim3(64 * LK_MOE_NW), 0, st, a);
+    hipLaunchKernelGGL((lk_k_moe_many<NP, true>), dim3(a.ffn / 32, slots), dim3(LK_MOE_THREADS), 0, st, a);
+    hipLaunchKernelGGL((lk_k_moe_many<NP, false>), dim3((a.hidden + 63) / 64, slots), dim3(LK_MOE_THREADS), 0, st, a);
     hipLaunchKernelGGL((lk_k_moe_sum<TYPE>), dim3((a.hidden / 4 + LK_MOE_THREADS - 1) / LK_MOE_THREADS, a.T), dim3(LK_MOE_THREADS), 0, st, a);
 }
 
@@ -757,7 +892,7 @@ extern "C" int lk_moe_q4_0(const lk_moe * moe, int type, const void * x, int ldx
     a.d[0] = (const _Float16 *) moe->gate_d; a.d[1] = (const _Float16 *) moe->up_d; a.d[2] = (const _Float16 *) moe->down_d;
     a.ids_out = ids; a.wts_out = weights;
     a.ldx = ldx; a.ldr = ldr; a.ldo = ldo; a.T = T; a.E = moe->n_experts; a.k = moe->top_k;
-    a.hidden = moe->hidden; a.ffn = moe->ffn; a.score = moe->score; a.renorm = moe->renorm; a.scale = moe->scale;
+    a.hidden = moe->hidden; a.ffn = moe->ffn; a.score = moe->score; a.renorm = moe->renorm; a.kinv = 65536 / moe->top_k + 1; a.scale = moe->scale;
     const hipStream_t st = lk_stream(stream);
     if (type == LK_F32)      lk_moe_go<LK_F32>(a, st);
     else if (type == LK_F16) lk_moe_go<LK_F16>(a, st);
