@@ -236,18 +236,24 @@ __device__ __forceinline__ uint32_t lk_moe_key(float r) {    // orderable bits; 
     const uint32_t u = __builtin_bit_cast(uint32_t, r + 0.0f);
     return r != r ? 1u : (u >> 31) ? ~u : u | 0x80000000u;
 }
-// Token t's choice j and its weight in lane j < k; the other lanes hold -1.
+// A token's logits and the biases, as a lane holds them (past the experts: expert 0's).
 template <int NL>
-__device__ __forceinline__ void lk_moe_choose(const LkMoeArgs & a, int t, int & id, float & w) {
+__device__ __forceinline__ void lk_moe_logits(const LkMoeArgs & a, int t, float (&l)[NL]) {
     const int lane = threadIdx.x & 63;
-    float l[NL], b[NL];
-    uint32_t key[NL];
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-        const int e = 64 * i + lane < a.E ? 64 * i + lane : 0;
-        l[i] = a.logits[(size_t) t * a.E + e];
-        b[i] = a.bias ? a.bias[e] : 0.0f;
-    }
+    for (int i = 0; i < NL; ++i) l[i] = a.logits[(size_t) t * a.E + (64 * i + lane < a.E ? 64 * i + lane : 0)];
+}
+template <int NL>
+__device__ __forceinline__ void lk_moe_bias(const LkMoeArgs & a, float (&b)[NL]) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) b[i] = a.bias ? a.bias[64 * i + lane < a.E ? 64 * i + lane : 0] : 0.0f;
+}
+// The token's choice j and its weight in lane j < k; the other lanes hold -1.
+template <int NL>
+__device__ __forceinline__ void lk_moe_choose(const LkMoeArgs & a, const float (&l)[NL], const float (&b)[NL], int & id, float & w) {
+    const int lane = threadIdx.x & 63;
+    uint32_t key[NL];
     float m = 0.0f, zi = 1.0f;
     if (a.score == LK_MOE_SOFTMAX) {
         m = l[0];
@@ -303,10 +309,18 @@ lk_k_moe_route(const LkMoeArgs a) {
     LkMoeTab & tab = *(LkMoeTab *) a.tab;
     if (tid < LK_MOE_MAX_EXPERTS) cnt[tid] = 0;
     __syncthreads();
-    for (int t = wv; t < a.T; t += 16) {
+    constexpr int TW = LK_MOE_MAX_TOKENS / 16;           // tokens of a wave, their logits asked for together
+    float l[TW][NL], b[NL];
+#pragma unroll
+    for (int i = 0; i < TW; ++i) lk_moe_logits<NL>(a, wv + 16 * i < a.T ? wv + 16 * i : a.T - 1, l[i]);
+    lk_moe_bias<NL>(a, b);
+#pragma unroll
+    for (int i = 0; i < TW; ++i) {
+        const int t = wv + 16 * i;
+        if (t >= a.T) break;
         int id;
         float w;
-        lk_moe_choose<NL>(a, t, id, w);
+        lk_moe_choose<NL>(a, l[i], b, id, w);
         if (id >= 0) {
             const int i = t * a.k + lane;
             ids[i] = id;
@@ -320,6 +334,7 @@ lk_k_moe_route(const LkMoeArgs a) {
     if (tid < a.E) {
         const int c = cnt[tid];
         int s = 0;
+#pragma unroll 8
         for (int e = 0; e < a.E; ++e) s += cnt[e] > c || (cnt[e] == c && e < tid);
         slot[tid] = s;
         tab.slot[s].e = tid;
@@ -365,17 +380,18 @@ __device__ __forceinline__ void lk_moe_token_dots(const lk_u4 * x, bool in, cons
     const float sc = in ? __builtin_bit_cast(float, m3) : 0.0f;                    // a block past the row's end counts nothing
 #pragma unroll
     for (int m = 0; m < NM; ++m) {
-        float f = 0.0f;
+        int s[NP];
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
-            int s = meta[p];
+            s[p] = meta[p];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                s = __builtin_amdgcn_sdot4((int) lo[m][k], (int) q[2 * p][k], s, false);
-                s = __builtin_amdgcn_sdot4((int) hi[m][k], (int) q[2 * p + 1][k], s, false);
+                s[p] = __builtin_amdgcn_sdot4((int) lo[m][k], (int) q[2 * p][k], s[p], false);
+                s[p] = __builtin_amdgcn_sdot4((int) hi[m][k], (int) q[2 * p + 1][k], s[p], false);
             }
-            f = p ? __builtin_fmaf(f, 256.0f, (float) s) : (float) s;
         }
+        float f = (float) (s[0] * 256 + s[1]);           // a digit's sum is at most 32 * 8 * 128 = 2^15
+        if constexpr (NP == 3) f = __builtin_fmaf(f, 256.0f, (float) s[2]);
         acc[m] = __builtin_fmaf(dv[m] * sc, f, acc[m]);
         // done here: left to itself the compiler reads the digits of all tokens first and spills
         asm volatile("" : "+v"(acc[m]) :: "memory");
@@ -524,8 +540,10 @@ lk_k_moe_up_few(const LkMoeArgs a) {
     int mine = -1;
     if (a.T == 1 || wv < a.T) {                          // one token: every wave for itself
         const int t = a.T == 1 ? 0 : wv;
-        float w;
-        lk_moe_choose<NL>(a, t, mine, w);
+        float l[NL], b[NL], w;
+        lk_moe_logits<NL>(a, t, l);
+        lk_moe_bias<NL>(a, b);
+        lk_moe_choose<NL>(a, l, b, mine, w);
         if (mine >= 0) {
             if (a.T > 1) ids[t * a.k + lane] = mine;
             if (tells && (a.T > 1 || wv == 0)) {
@@ -557,9 +575,9 @@ lk_k_moe_up_few(const LkMoeArgs a) {
 // one expert and up to eight of its assignments at a time.  Wave w has half w & 1 of the rows
 // (four matrices of 8 rows) and every second step of 8 blocks of K; it copies a step's
 // digits into its own part of LDS while the step's weights are on their way, which are
-// asked for before the dots of the step before.  The loop is kept short (one step, four
-// counts of tokens): with two steps and six counts the kernel had 57 KB of code, and
-// fetching it under a saturated memory took up to 5 us a workgroup.
+// asked for before the dots of the step before.  The loop is kept short (one step): with two
+// steps the kernel had 57 KB of code, and fetching it under a saturated memory took up to 5
+// us a workgroup.
 template <int NP>
 struct LkMoeShare {
     static constexpr int Z = 8 * LkMoeRec<NP>::PIECES;   // pieces of a step's digits
@@ -701,10 +719,16 @@ lk_k_moe_many(const LkMoeArgs a) {
     for (int at = 0; at < n; at += 8) {
         if (at) __syncthreads();                         // part has been read
         const int left = n - at;
-        if (left > 4)       go(LkInt<8>{}, at);
-        else if (left > 2)  go(LkInt<4>{}, at);
-        else if (left == 2) go(LkInt<2>{}, at);
-        else                go(LkInt<1>{}, at);
+        switch (left < 8 ? left : 8) {
+        case 1:  go(LkInt<1>{}, at); break;
+        case 2:  go(LkInt<2>{}, at); break;
+        case 3:  go(LkInt<3>{}, at); break;
+        case 4:  go(LkInt<4>{}, at); break;
+        case 5:  go(LkInt<5>{}, at); break;
+        case 6:  go(LkInt<6>{}, at); break;
+        case 7:  go(LkInt<7>{}, at); break;
+        default: go(LkInt<8>{}, at);
+        }
     }
 }
 
