@@ -41,84 +41,76 @@ struct LkI8Args {
 };
 
 // ---- few tokens -------------------------------------------------------------------
-// 16 weight rows per workgroup against TT tiles of 16 tokens
-// (v_mfma_i32_16x16x64_i8); the NW waves take 128-byte pieces of K in turn and
-// load them straight into the operand layout (lane: row or token l % 16, 16
-// bytes at 16 * (l / 16) of a 64-byte step), so that nothing waits for anything
-// but its own loads.  The int32 parts meet in LDS; integer sums have no order.
-template <int TYPE, int TT, int NW>
+// 16 weight rows per workgroup against up to 16 tokens (v_mfma_i32_16x16x64_i8); the
+// NW waves take 128-byte pieces of K in turn, two at a time, and load them straight into
+// the operand layout (lane: row or token l % 16, 16 bytes at 16 * (l / 16) of a 64-byte
+// step), so that nothing waits for anything but its own loads.  The int32 parts meet in
+// LDS; integer sums have no order.  Bound by the latency of one round of loads and the
+// launch for short rows (1 x 4096 x 1024: 2.5 us with 4 waves, 3.1 with 8, of which half
+// find no piece), by the weights' way from the cache for long ones (1 x 4096 x 8192, 34 MB:
+// 6.5 us with 8 waves, 5.2 TB/s; 7.6 with 4).
+template <int TYPE, int NW>
 __global__ void __launch_bounds__(64 * NW)
 lk_k_gemm_i8_few(const LkI8Args a) {
     typedef typename LkElem<TYPE>::type T;
-    constexpr int U = TT > 2 ? 2 : 4;                    // 64-byte steps in flight per wave
-    __shared__ __attribute__((aligned(16))) lk_i4 part[NW][TT][64];
+    constexpr int U = 4;                                 // 64-byte steps in flight per wave
+    __shared__ __attribute__((aligned(16))) lk_i4 part[NW][64];
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int c = lane & 15, g = lane >> 4;
-    const int r0 = blockIdx.x * 16, t0 = blockIdx.y * (16 * TT);
+    const int c = lane & 15, g = lane >> 4, r0 = blockIdx.x * 16;
     const int8_t * wp = a.w + (size_t) (r0 + c < a.N ? r0 + c : a.N - 1) * a.ldw;
-    const int8_t * xp[TT];
-#pragma unroll
-    for (int j = 0; j < TT; ++j) {
-        const int t = t0 + 16 * j + c;
-        xp[j] = a.x + (size_t) (t < a.M ? t : a.M - 1) * a.ldx;
-    }
-    lk_i4 acc[TT];
-#pragma unroll
-    for (int j = 0; j < TT; ++j) acc[j] = lk_i4{ 0, 0, 0, 0 };
+    const int8_t * xp = a.x + (size_t) (c < a.M ? c : a.M - 1) * a.ldx;
+    lk_i4 acc = { 0, 0, 0, 0 };
     const int K = a.K, nst = (K + 63) / 64;
     for (int s0 = 2 * wv; s0 < nst; s0 += U * NW) {
-        lk_i4 wv4[U], xv[U][TT];
+        lk_i4 wv4[U], xv[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int k0 = (s0 + (u / 2) * 2 * NW + u % 2) * 64 + 16 * g;
             const int kc = k0 < K ? k0 : 0;              // in bounds; masked below
             wv4[u] = *(const lk_i4 *) (wp + kc);
-#pragma unroll
-            for (int j = 0; j < TT; ++j) xv[u][j] = *(const lk_i4 *) (xp[j] + kc);
+            xv[u] = *(const lk_i4 *) (xp + kc);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int st = s0 + (u / 2) * 2 * NW + u % 2;
-            if (st * 64 + 64 > K) {                      // wave-uniform: the last step, or past it
-#pragma unroll
-                for (int j = 0; j < TT; ++j) xv[u][j] = lk_i8_mask(xv[u][j], st * 64 + 16 * g, K);
-            }
-#pragma unroll
-            for (int j = 0; j < TT; ++j) acc[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv4[u], xv[u][j], acc[j], 0, 0, 0);
+            if (st * 64 + 64 > K) xv[u] = lk_i8_mask(xv[u], st * 64 + 16 * g, K);      // wave-uniform: the last step, or past it
+            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv4[u], xv[u], acc, 0, 0, 0);
         }
     }
-#pragma unroll
-    for (int j = 0; j < TT; ++j) part[wv][j][lane] = acc[j];
+    part[wv][lane] = acc;
     __syncthreads();
-    // output (token tc of tile j, row r): lane r / 4 * 16 + tc holds it in r % 4
+    // output (token t, row r): lane r / 4 * 16 + t holds it in r % 4
     const T * res = (const T *) a.res;
     T * out = (T *) a.out;
-    for (int i = threadIdx.x; i < TT * 256; i += 64 * NW) {
-        const int r = i & 15, tt = i >> 4, j = tt >> 4, tc = tt & 15;
-        int s = 0;
+    if (threadIdx.x >= 256) return;
+    const int r = threadIdx.x & 15, t = threadIdx.x >> 4, rr = r0 + r;
+    int s = 0;
 #pragma unroll
-        for (int k = 0; k < NW; ++k) s += part[k][j][(r >> 2) * 16 + tc][r & 3];
-        const int t = t0 + tt, rr = r0 + r;
-        if (t < a.M && rr < a.N) {
-            float v = lk_i8_out(s, a.sx[t], a.sw[rr]);
-            if (res) v = (float) res[(size_t) t * a.ldr + rr] + v;
-            out[(size_t) t * a.ldo + rr] = (T) v;
-        }
+    for (int k = 0; k < NW; ++k) s += part[k][(r >> 2) * 16 + t][r & 3];
+    if (t < a.M && rr < a.N) {
+        float v = lk_i8_out(s, a.sx[t], a.sw[rr]);
+        if (res) v = (float) res[(size_t) t * a.ldr + rr] + v;
+        out[(size_t) t * a.ldo + rr] = (T) v;
     }
 }
 
 // ---- tiles ------------------------------------------------------------------------
 // A wave covers TM x TN tiles of v_mfma_i32_32x32x32_i8 (TM along the weight rows, TN
-// along the tokens), WM x WN waves a workgroup; K in stages of KC bytes, a ring of
-// NB of them in LDS, filled by LDS DMA.
-template <int TM_, int TN_, int WM_, int WN_, int KC_, int NB_, int OCC_>
+// along the tokens), WM x WN of them a workgroup, or WK times as many
+// that share K: each takes its part of every stage.  K in stages of KC bytes, a ring of NB of
+// them in LDS, filled by LDS DMA.
+template <int TM_, int TN_, int WM_, int WN_, int WK_, int KC_, int NB_, int OCC_>
 struct LkI8Shape {
-    static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, KC = KC_, NB = NB_, OCC = OCC_;   // OCC: waves per SIMD
-    static constexpr int NW = WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN, PC = KC / 16;
+    static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, WK = WK_, KC = KC_, NB = NB_, OCC = OCC_;   // OCC: waves per SIMD
+    static constexpr int NW = WM * WN * WK, BM = 32 * TM * WM, BN = 32 * TN * WN, PC = KC / 16;
     static constexpr int BYTES = (BM + BN) * KC;         // a stage: BM weight rows, then BN token rows
     static constexpr int NA = BM * PC / 64, NI = (BM + BN) * PC / 64, PW = NI / NW;
     static_assert(NI % NW == 0 && BM * PC % 64 == 0 && BN * PC % 64 == 0, "whole DMA instructions, the same for every wave");
     static_assert((NB - 2) * PW < 64, "vmcnt range");
+    // the ring, or the parts of K and the outputs on their way (below) where those are more
+    static constexpr int PARTS = WM * WN * (WK - 1) * TM * TN * 4096, OUTS = PARTS + WM * WN * 32 * (32 * TM + 4) * 4;
+    static constexpr int LDS = NB * BYTES > OUTS ? NB * BYTES : OUTS;
+    static_assert(KC % (32 * WK) == 0 && 16 % PC == 0, "whole steps; a row's pieces divide the 16 slots of all banks");
 };
 // 16-byte slot of piece p of a row of n pieces: XOR-permuted so that the same piece
 // of 16 consecutive rows lies in 16 different slots modulo 256 bytes (all banks).
@@ -128,8 +120,9 @@ template <class SH, int TYPE>
 __global__ void __launch_bounds__(64 * SH::NW, SH::OCC)
 lk_k_gemm_i8(const LkI8Args a) {
     typedef typename LkElem<TYPE>::type T;
-    constexpr int TM = SH::TM, TN = SH::TN, KC = SH::KC, NB = SH::NB, NW = SH::NW, PC = SH::PC, PW = SH::PW, NQ = KC / 32;
-    __shared__ __attribute__((aligned(16))) uint8_t stg[NB * SH::BYTES];
+    constexpr int TM = SH::TM, TN = SH::TN, KC = SH::KC, NB = SH::NB, NW = SH::NW, PC = SH::PC, PW = SH::PW;
+    constexpr int WMN = SH::WM * SH::WN, NQ = KC / 32 / SH::WK;        // a wave's steps of a stage
+    __shared__ __attribute__((aligned(16))) uint8_t stg[SH::LDS];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     // XCD-aware tile order: workgroups go round-robin over the 8 XCDs (id % 8), so
     // consecutive tiles L are given to one XCD; L runs through groups of 8 row tiles,
@@ -140,7 +133,8 @@ lk_k_gemm_i8(const LkI8Args a) {
     const int L = x8 * (ntile >> 3) + (x8 < rem ? x8 : rem) + (id >> 3);
     const int gr = L / (8 * ntt), gw = nrt - 8 * gr < 8 ? nrt - 8 * gr : 8, li = L - gr * 8 * ntt;
     const int row0 = (8 * gr + li % gw) * SH::BM, tok0 = (li / gw) * SH::BN;
-    const int wr = (w % SH::WM) * 32 * TM, wt = (w / SH::WM) * 32 * TN;
+    const int kw = w / WMN;                              // the wave's part of every stage
+    const int wr = (w % SH::WM) * 32 * TM, wt = (w % WMN / SH::WM) * 32 * TN;
     const int lm = lane & 31, h = lane >> 5;
     const int K = a.K, nst = (K + KC - 1) / KC;
 
@@ -157,23 +151,10 @@ lk_k_gemm_i8(const LkI8Args a) {
     }
     const int8_t * wb = a.w + (size_t) row0 * a.ldw, * xb = a.x + (size_t) tok0 * a.ldx;
     const uint32_t lds0 = lk_lds_addr(stg);
-    auto fetch = [&](int s) {
-        const uint32_t sb = lds0 + (uint32_t) (s % NB * SH::BYTES);
-        const int k0 = s * KC;
-        if (k0 + KC <= K) {
-#pragma unroll
-            for (int i = 0; i < PW; ++i) {
-                const int j = i * NW + w;
-                lk_dma16c_so((j < SH::NA ? wb : xb) + k0, roff[i] + pc[i], sb + (uint32_t) (1024 * j));
-            }
-        } else {                                         // pieces past the row: its first piece instead
-#pragma unroll
-            for (int i = 0; i < PW; ++i) {
-                const int j = i * NW + w;
-                const uint32_t k = (uint32_t) k0 + pc[i];
-                lk_dma16c_so(j < SH::NA ? wb : xb, roff[i] + (k < (uint32_t) K ? k : 0u), sb + (uint32_t) (1024 * j));
-            }
-        }
+    auto fetch = [&](int s, int i) {                     // pieces past the row: its first piece instead
+        const int j = i * NW + w;
+        const uint32_t k = (uint32_t) (s * KC) + pc[i];
+        lk_dma16c_so(j < SH::NA ? wb : xb, roff[i] + (k < (uint32_t) K ? k : 0u), lds0 + (uint32_t) (s % NB * SH::BYTES + 1024 * j));
     };
     lk_i16v acc[TM][TN];
 #pragma unroll
@@ -183,84 +164,150 @@ lk_k_gemm_i8(const LkI8Args a) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
     lk_i4 av[2][TM], bv[2][TN];
-    auto load = [&](int s, int q, int u) {               // operands of step q of stage s
+    auto read = [&](int s, int q, int u, int k) {        // operand k of step q of stage s
         const uint8_t * S = stg + s % NB * SH::BYTES;
-#pragma unroll
-        for (int i = 0; i < TM; ++i) av[u][i] = *(const lk_i4 *) (S + lk_i8_slot(PC, wr + 32 * i + lm, 2 * q + h) * 16);
-#pragma unroll
-        for (int j = 0; j < TN; ++j) bv[u][j] = *(const lk_i4 *) (S + SH::BM * KC + lk_i8_slot(PC, wt + 32 * j + lm, 2 * q + h) * 16);
+        if (k < TM) av[u][k] = *(const lk_i4 *) (S + lk_i8_slot(PC, wr + 32 * k + lm, 2 * (kw * NQ + q) + h) * 16);
+        else bv[u][k - TM] = *(const lk_i4 *) (S + SH::BM * KC + lk_i8_slot(PC, wt + 32 * (k - TM) + lm, 2 * (kw * NQ + q) + h) * 16);
     };
-    // all of this wave's LDS reads are in registers, stage s + 1 of every wave has
-    // landed; afterwards the buffer of stage s may be overwritten
-    auto turn = [&](int s) {
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        if (s + NB - 1 < nst) lk_wait_vm<(NB - 2) * PW>();
-        else lk_wait_vm<0>();
+    auto meet = [&] {                                    // the next stage of every wave has landed
+        lk_wait_vm<(NB - 2) * PW>();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    for (int s = 0; s < NB - 1 && s < nst; ++s) fetch(s);
-    if (nst > NB - 2) lk_wait_vm<(NB - 2) * PW>();
-    else lk_wait_vm<0>();
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    load(0, 0, 0);
-    for (int s = 0; s < nst; ++s) {
-        if (s + NB - 1 < nst) fetch(s + NB - 1);
-        const bool whole = (s + 1) * KC <= K;
+    // A stage: NQ steps of TM x TN MFMAs, in TM groups of TN.  Before each group come its share
+    // of the next step's operand reads and of the DMA of stage s + NB - 1 (the ring's free
+    // buffer), pinned there: issued all at once at the start of a stage, the DMAs of 8 waves
+    // kept the address unit, and with it every wave's MFMAs, waiting.  Before the last step's
+    // reads, which are of the next stage, the waves meet: each has its reads of this stage in
+    // registers, and its part of the next has landed.
+    auto stage = [&](int s, bool last) {
 #pragma unroll
         for (int q = 0; q < NQ; ++q) {
             const int u = q & 1;
-            if (q + 1 < NQ) load(s, q + 1, u ^ 1);
-            else if (s + 1 < nst) { turn(s); load(s + 1, 0, u ^ 1); }
-            if (!whole) {
-#pragma unroll
-                for (int j = 0; j < TN; ++j) bv[u][j] = lk_i8_mask(bv[u][j], s * KC + 32 * q + 16 * h, K);
+            if (q + 1 == NQ && !last) {
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                meet();
             }
+            if (last) {
+#pragma unroll
+                for (int j = 0; j < TN; ++j) bv[u][j] = lk_i8_mask(bv[u][j], s * KC + 32 * (kw * NQ + q) + 16 * h, K);
+            }
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                constexpr int ND = TM * (NQ > 1 ? NQ / 2 : 1);       // groups that the DMAs are spread over
+#pragma unroll
+                for (int k = (TM + TN) * i / TM; k < (TM + TN) * (i + 1) / TM; ++k) {
+                    if (q + 1 < NQ) read(s, q + 1, u ^ 1, k);
+                    else if (!last) read(s + 1, 0, u ^ 1, k);
+                }
+                const int g = q * TM + i;
+                if (g < ND)
+#pragma unroll
+                    for (int k = PW * g / ND; k < PW * (g + 1) / ND; ++k) fetch(s + NB - 1, k);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(av[u][i], bv[u][j], acc[i][j], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    };
+#pragma unroll
+    for (int s = 0; s < NB - 1; ++s)
+#pragma unroll
+        for (int i = 0; i < PW; ++i) fetch(s, i);        // those past the end: the rows' first pieces, not used
+    meet();
+#pragma unroll
+    for (int k = 0; k < TM + TN; ++k) read(0, 0, 0, k);
+#pragma unroll 1
+    for (int s = 0; s + 1 < nst; ++s) stage(s, false);
+    stage(nst - 1, true);
+    lk_wait_vm<0>();                                     // the DMAs past the end, before LDS is used otherwise
+    // Outputs by way of LDS (the ring is free now), 32 tokens of the wave at a time: a
+    // lane has token lm and rows 8 * e4 + 4 * h .. +3 of every MFMA tile, 8 bytes of 32
+    // output rows per store; from LDS it takes 8 consecutive rows of one token, whole
+    // runs of 64 * TM bytes (bf16).  The rows are 16 bytes longer in LDS, so that the 16-byte
+    // writes of 16 tokens lie in different banks.
+    constexpr int RW = 32 * TM, LS = RW + 4;             // rows of the wave's tile; floats from token to token
+    __syncthreads();                                     // every wave has read its last operands
+    if constexpr (SH::WK > 1) {                          // the parts of K meet: integer sums have no order
+        lk_i16v * pt = (lk_i16v *) stg;
+        if (kw > 0) {
 #pragma unroll
             for (int i = 0; i < TM; ++i)
 #pragma unroll
-                for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(av[u][i], bv[u][j], acc[i][j], 0, 0, 0);
+                for (int j = 0; j < TN; ++j) pt[((w - WMN) * TM * TN + i * TN + j) * 64 + lane] = acc[i][j];
         }
+        __syncthreads();
+        if (kw > 0) return;
+#pragma unroll
+        for (int k = 1; k < SH::WK; ++k)
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] += pt[((k * WMN + w - WMN) * TM * TN + i * TN + j) * 64 + lane];
     }
-    // lane: token lm of a tile, rows 8 * e4 + 4 * h .. +3
+    // (behind the parts of K, which other waves may still be reading)
+    float * st = (float *) (stg + SH::PARTS) + (w % WMN) * 32 * LS;
     const T * res = (const T *) a.res;
     T * out = (T *) a.out;
+    float sw[TM][4][4];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int e4 = 0; e4 < 4; ++e4) {
+            const int r = row0 + wr + 32 * i + 8 * e4 + 4 * h;
+            if (r + 4 <= a.N) lk_load<4>(a.sw + r, sw[i][e4]);
+            else
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sw[i][e4][e] = r + e < a.N ? a.sw[r + e] : 0.0f;
+        }
+    constexpr int LT = RW / 8, TP = 64 / LT;             // lanes a token, tokens a step
+    const int r8 = (lane % LT) * 8, r = row0 + wr + r8;
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
-        const int t = tok0 + wt + 32 * j + lm;
-        if (t >= a.M) continue;
-        const float sx = a.sx[t];
+        const int t0 = tok0 + wt + 32 * j;               // wave-uniform
+        const float sx = a.sx[t0 + lm < a.M ? t0 + lm : a.M - 1];
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
             for (int e4 = 0; e4 < 4; ++e4) {
-                const int r = row0 + wr + 32 * i + 8 * e4 + 4 * h;
-                float v[4], s4[4], r4[4];
-                if (r + 4 <= a.N) {
-                    lk_load<4>(a.sw + r, s4);
-                    if (res) lk_load<4>(res + (size_t) t * a.ldr + r, r4);
+                lk_f4 v;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        v[e] = lk_i8_out(acc[i][j][4 * e4 + e], sx, s4[e]);
-                        if (res) v[e] = r4[e] + v[e];
-                    }
-                    lk_store<4>(out + (size_t) t * a.ldo + r, v);
-                } else {
+                for (int e = 0; e < 4; ++e) v[e] = lk_i8_out(acc[i][j][4 * e4 + e], sx, sw[i][e4][e]);
+                *(lk_f4 *) (st + lm * LS + 32 * i + 8 * e4 + 4 * h) = v;
+            }
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) if (r + e < a.N) {
-                        float u = lk_i8_out(acc[i][j][4 * e4 + e], sx, a.sw[r + e]);
-                        if (res) u = (float) res[(size_t) t * a.ldr + r + e] + u;
-                        out[(size_t) t * a.ldo + r + e] = (T) u;
-                    }
+        for (int k = 0; k < 32 / TP; ++k) {
+            const int tl = k * TP + lane / LT, t = t0 + tl;
+            float v[8];
+            *(lk_f4 *) v = *(const lk_f4 *) (st + tl * LS + r8);
+            *(lk_f4 *) (v + 4) = *(const lk_f4 *) (st + tl * LS + r8 + 4);
+            if (t >= a.M || r >= a.N) continue;
+            if (r + 8 <= a.N) {
+                if (res) {
+                    float o[8];
+                    lk_load<8>(res + (size_t) t * a.ldr + r, o);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = o[e] + v[e];
+                }
+                lk_store<8>(out + (size_t) t * a.ldo + r, v);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) if (r + e < a.N) {
+                    float u = v[e];
+                    if (res) u = (float) res[(size_t) t * a.ldr + r + e] + u;
+                    out[(size_t) t * a.ldo + r + e] = (T) u;
                 }
             }
+        }
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
-template <int TYPE, int TT, int NW>
+template <int TYPE, int NW>
 static void lk_i8_few(const LkI8Args & a, hipStream_t st) {
-    hipLaunchKernelGGL((lk_k_gemm_i8_few<TYPE, TT, NW>), dim3((a.N + 15) / 16, (a.M + 16 * TT - 1) / (16 * TT)), dim3(64 * NW), 0, st, a);
+    hipLaunchKernelGGL((lk_k_gemm_i8_few<TYPE, NW>), dim3((a.N + 15) / 16), dim3(64 * NW), 0, st, a);
 }
 template <class SH, int TYPE>
 static int lk_i8_tiles(const LkI8Args & a, hipStream_t st) {
@@ -269,15 +316,44 @@ static int lk_i8_tiles(const LkI8Args & a, hipStream_t st) {
     hipLaunchKernelGGL((lk_k_gemm_i8<SH, TYPE>), dim3((unsigned) n), dim3(64 * SH::NW), 0, st, a);
     return 0;
 }
+// Which kernel.  A compute unit holds one or two workgroups of a shape, so what counts is
+// how many rounds of 256 units the tiles take; the largest tile whose tiles still fill one
+// round loses to the next smaller one, which shares less but splits K over the waves (WK).
+// Measured (bf16 out, operands in the cache, us; * is what the rule takes):
+//   M x N x K          few   32x32  64x32  64x64  128x64  128x128  2/unit  256x256
+//   1 x 4096 x 4096    4.3*   5.7    6.8    7.8
+//   16 x 4096 x 4096   5.7*   5.7
+//   1 x 8192 x 2048    4.0*   4.6    5.0    5.5
+//   16 x 8192 x 2048   5.4    4.7*   5.2    5.6
+//   1 x 8192 x 8192   13.4   11.8*  12.3   14.8    22.5
+//   128 x 2048 x 2048         4.9*   5.5    6.1     8.6
+//   192 x 2048 x 2048         6.3    5.7*   6.2     8.7
+//   333 x 2048 x 2048         9.3    9.9    6.6*    8.9     11.0
+//   640 x 2048 x 2048                      10.0     9.3*    11.2    12.8
+//   1000 x 4096 x 2048                     18.0    15.5     14.1*   16.5    28.6
+//   2048 x 4096 x 2048                             28.7     26.5    25.4*   31.2
+//   2600 x 4096 x 2048                             39.7     36.2    38.1    33.9*
+//   2600 x 8192 x 2048                             71.3     71.3    60.6*   65.7
+//   4096 x 8192 x 2048                            104.8    100.8    86.0    76.3*
+// A round of 256 256x256 tiles takes about 5 / 3 of one of 512 128x128 tiles.
+template <int BM, int BN>
+static long lk_i8_ntile(const LkI8Args & a) { return (long) ((a.N + BM - 1) / BM) * ((a.M + BN - 1) / BN); }
+
 template <int TYPE>
 static int lk_i8_shape(const LkI8Args & a, hipStream_t st) {
-    if (a.M <= 16) { lk_i8_few<TYPE, 1, 8>(a, st); return 0; }
-    if (a.M <= 32) { lk_i8_few<TYPE, 2, 8>(a, st); return 0; }
-    const long t256 = (long) ((a.N + 255) / 256) * ((a.M + 255) / 256);
-    if (t256 >= 256) return lk_i8_tiles<LkI8Shape<4, 4, 2, 2, 64, 4, 1>, TYPE>(a, st);
-    const long t128 = (long) ((a.N + 127) / 128) * ((a.M + 127) / 128);
-    if (t128 >= 256) return lk_i8_tiles<LkI8Shape<2, 2, 2, 2, 64, 4, 2>, TYPE>(a, st);
-    return lk_i8_tiles<LkI8Shape<1, 1, 2, 2, 128, 4, 2>, TYPE>(a, st);
+    if (a.M <= 16 && (a.N <= 4096 || (a.N <= 8192 && a.K <= 2048 && a.M <= 8))) {
+        if (a.K <= 2048) lk_i8_few<TYPE, 4>(a, st);
+        else lk_i8_few<TYPE, 8>(a, st);
+        return 0;
+    }
+    if (lk_i8_ntile<32, 32>(a) <= 256) return lk_i8_tiles<LkI8Shape<1, 1, 1, 1, 4, 256, 4, 2>, TYPE>(a, st);
+    if (lk_i8_ntile<64, 32>(a) <= 256) return lk_i8_tiles<LkI8Shape<1, 1, 2, 1, 4, 256, 4, 2>, TYPE>(a, st);
+    if (lk_i8_ntile<64, 64>(a) <= 256) return lk_i8_tiles<LkI8Shape<1, 1, 2, 2, 2, 128, 4, 2>, TYPE>(a, st);
+    if (lk_i8_ntile<128, 64>(a) <= 256) return lk_i8_tiles<LkI8Shape<2, 1, 2, 2, 2, 128, 3, 2>, TYPE>(a, st);
+    const long t128 = lk_i8_ntile<128, 128>(a), t256 = lk_i8_ntile<256, 256>(a);
+    if (t128 <= 256) return lk_i8_tiles<LkI8Shape<2, 1, 2, 4, 1, 128, 3, 2>, TYPE>(a, st);
+    if (5 * ((t256 + 255) / 256) > 3 * ((t128 + 511) / 512)) return lk_i8_tiles<LkI8Shape<2, 2, 2, 2, 1, 128, 2, 2>, TYPE>(a, st);
+    return lk_i8_tiles<LkI8Shape<4, 2, 2, 4, 1, 128, 2, 2>, TYPE>(a, st);
 }
 
 extern "C" int lk_gemm_i8(const int8_t * x, int ldx, const float * sx, const int8_t * w, int ldw, const float * sw,

@@ -461,37 +461,39 @@ def pf_qknr(Y, qn, kn, m, P, qh, kc, vc, k8=None, ksc=None, kstride=0, cm=None, 
 # or on `stream`, which must be one of that device.
 F32, F16, BF16 = 0, 1, 2
 Q8_ROW, Q81_PLANAR, Q81_BLOCK = 0, 1, 2
-_types = None                               # torch dtype -> LK_F32 / LK_F16 / LK_BF16
+_torch = _types = None                      # torch; its dtype -> LK_F32 / LK_F16 / LK_BF16
 
 
 def _type_of(t, what: str) -> int:
-    global _types
+    global _torch, _types
     if _types is None:
         import torch
-        _types = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
-    if t.dtype not in _types:
+        _torch, _types = torch, {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+    ty = _types.get(t.dtype)
+    if ty is None:
         raise ValueError(f"{what}: fp32, fp16 or bf16 rows, not {t.dtype}")
-    return _types[t.dtype]
+    return ty
 
 
-def _rows2(t, rows: int, n: int, dtype, dev: int, what: str) -> tuple:
+def _rows2(t, shape: tuple, dtype, dev: int, what: str) -> tuple:
     """(pointer, row stride) of a [rows][n] tensor of a dtype on device `dev` whose
     rows are contiguous; (None, 0) for None."""
     if t is None:
         return None, 0
-    if t.dtype is not dtype or t.dim() != 2 or t.shape[0] != rows or t.shape[1] != n:
-        raise ValueError(f"{what}: {dtype} [{rows}, {n}] wanted, not {t.dtype} {list(t.shape)}")
+    if t.dtype is not dtype or t.shape != shape:
+        raise ValueError(f"{what}: {dtype} {list(shape)} wanted, not {t.dtype} {list(t.shape)}")
     if t.get_device() != dev:
         raise ValueError(f"{what}: on another device, or not in device memory")
+    rows, n = shape
     s0, s1 = t.stride()
     if (s1 != 1 and n > 1) or (rows > 1 and s0 < n):
         raise ValueError(f"{what}: rows must be contiguous and must not overlap (strides {s0}, {s1})")
-    return t.data_ptr(), s0 if rows > 1 and s0 >= n else max(n, s0)
+    return t.data_ptr(), s0 if rows > 1 else n
 
 
 def _flat(t, shape: tuple, dtype, dev: int, what: str):
     """Pointer of a contiguous tensor of a shape and dtype on device `dev`."""
-    if t.dtype is not dtype or tuple(t.shape) != shape or t.get_device() != dev or not t.is_contiguous():
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
         raise ValueError(f"{what}: contiguous {dtype} {list(shape)} on the rows' device wanted, not {t.dtype} "
                          f"{list(t.shape)}")
     return t.data_ptr()
@@ -516,27 +518,26 @@ def norm_q8(x, w, q, sc=None, delta=None, res=None, y=None, eps: float = 1e-5, s
       sc fp32 [rows], q int8 [rows][n]                    a scale a row (gemm_i8)
       sc fp32 [rows][n/32][2], q int8 [rows][n]           planar Q8_1 (pf_gemm_q4_0)
       sc None, q uint8 [rows][n/32 * 36]                  Q8_1 blocks (gemv_q4_0)"""
-    import torch
-    lib = load()
+    lib = _lib or load()
     ty = _type_of(x, "norm_q8")
     if x.dim() != 2:
         raise ValueError("norm_q8: x must be [rows, n]")
-    rows, n = x.shape
+    shape = rows, n = x.shape
     dev = x.get_device()
-    px, ldx = _rows2(x, rows, n, x.dtype, dev, "norm_q8: x")
-    pd, ldd = _rows2(delta, rows, n, x.dtype, dev, "norm_q8: delta")
-    pr, ldr = _rows2(res, rows, n, x.dtype, dev, "norm_q8: res")
-    py, ldy = _rows2(y, rows, n, x.dtype, dev, "norm_q8: y")
-    pw = _flat(w, (n,), torch.float32, dev, "norm_q8: w")
+    px, ldx = _rows2(x, shape, x.dtype, dev, "norm_q8: x")
+    pd, ldd = _rows2(delta, shape, x.dtype, dev, "norm_q8: delta")
+    pr, ldr = _rows2(res, shape, x.dtype, dev, "norm_q8: res")
+    py, ldy = _rows2(y, shape, x.dtype, dev, "norm_q8: y")
+    pw = _flat(w, (n,), _torch.float32, dev, "norm_q8: w")
     if sc is None:
         form, ldq, ps = Q81_BLOCK, n, None
-        pq = _flat(q, (rows, n // 32 * Q8_1_BYTES), torch.uint8, dev, "norm_q8: q")
+        pq = _flat(q, (rows, n // 32 * Q8_1_BYTES), _torch.uint8, dev, "norm_q8: q")
     elif sc.dim() == 1:
-        form, ps = Q8_ROW, _flat(sc, (rows,), torch.float32, dev, "norm_q8: sc")
-        pq, ldq = _rows2(q, rows, n, torch.int8, dev, "norm_q8: q")
+        form, ps = Q8_ROW, _flat(sc, (rows,), _torch.float32, dev, "norm_q8: sc")
+        pq, ldq = _rows2(q, shape, _torch.int8, dev, "norm_q8: q")
     else:
-        form, ldq, ps = Q81_PLANAR, n, _flat(sc, (rows, n // 32, 2), torch.float32, dev, "norm_q8: sc")
-        pq = _flat(q, (rows, n), torch.int8, dev, "norm_q8: q")
+        form, ldq, ps = Q81_PLANAR, n, _flat(sc, (rows, n // 32, 2), _torch.float32, dev, "norm_q8: sc")
+        pq = _flat(q, shape, _torch.int8, dev, "norm_q8: q")
     rc = _on(dev, stream, lib.lk_norm_q8, ty, px, ldx, pd, ldd, pw, eps, rows, n, pr, ldr, py, ldy, form, pq, ldq, ps)
     if rc:
         _check(rc, "lk_norm_q8")
@@ -565,22 +566,21 @@ def gemm_i8(x, sx, w, sw, out, res=None, stream=None) -> None:
     """out[t][r] = (res[t][r] +) (x[t] . w[r]) * sx[t] * sw[r] (lk_gemm_i8): x int8
     [M][K] and w int8 [N][K] with rows a multiple of 16 bytes apart (i8_rows), sx fp32
     [M], sw fp32 [N], out (and res, which may be out) fp32, fp16 or bf16 [M][N]."""
-    import torch
-    lib = load()
+    lib = _lib or load()
     ty = _type_of(out, "gemm_i8")
     if x.dim() != 2 or w.dim() != 2:
         raise ValueError("gemm_i8: x must be [M, K] and w [N, K]")
     M, K = x.shape
     N = w.shape[0]
     dev = x.get_device()
-    px, ldx = _rows2(x, M, K, torch.int8, dev, "gemm_i8: x")
-    pw, ldw = _rows2(w, N, K, torch.int8, dev, "gemm_i8: w")
-    po, ldo = _rows2(out, M, N, out.dtype, dev, "gemm_i8: out")
-    pr, ldr = _rows2(res, M, N, out.dtype, dev, "gemm_i8: res")
+    px, ldx = _rows2(x, x.shape, _torch.int8, dev, "gemm_i8: x")
+    pw, ldw = _rows2(w, (N, K), _torch.int8, dev, "gemm_i8: w")
+    po, ldo = _rows2(out, (M, N), out.dtype, dev, "gemm_i8: out")
+    pr, ldr = _rows2(res, (M, N), out.dtype, dev, "gemm_i8: res")
     if K % 16:
         ldx, ldw = _padded(x, ldx, "gemm_i8: x"), _padded(w, ldw, "gemm_i8: w")
-    rc = _on(dev, stream, lib.lk_gemm_i8, px, ldx, _flat(sx, (M,), torch.float32, dev, "gemm_i8: sx"), pw, ldw,
-             _flat(sw, (N,), torch.float32, dev, "gemm_i8: sw"), M, N, K, ty, pr, ldr, po, ldo)
+    rc = _on(dev, stream, lib.lk_gemm_i8, px, ldx, _flat(sx, (M,), _torch.float32, dev, "gemm_i8: sx"), pw, ldw,
+             _flat(sw, (N,), _torch.float32, dev, "gemm_i8: sw"), M, N, K, ty, pr, ldr, po, ldo)
     if rc:
         _check(rc, "lk_gemm_i8")
 
@@ -640,21 +640,21 @@ class MoeQ4_0:
         """out[t] = (res[t] +) the layer of x[t], rows [T][hidden] of fp32, fp16 or bf16
         (out may be x, res may be out); ids int32 and weights fp32 [T][top_k] where
         given."""
-        import torch
         ty = _type_of(x, "MoeQ4_0")
         if x.dim() != 2:
             raise ValueError("MoeQ4_0: x must be [tokens, hidden]")
         T, dev = x.shape[0], self._dev
+        shape = (T, self._hidden)
         if T > self.max_tokens:
             raise ValueError(f"MoeQ4_0: {T} tokens, made for {self.max_tokens}")
-        px, ldx = _rows2(x, T, self._hidden, x.dtype, dev, "MoeQ4_0: x")
-        po, ldo = _rows2(out, T, self._hidden, x.dtype, dev, "MoeQ4_0: out")
-        pr, ldr = _rows2(res, T, self._hidden, x.dtype, dev, "MoeQ4_0: res")
-        pi = None if ids is None else _flat(ids, (T, self._k), torch.int32, dev, "MoeQ4_0: ids")
-        pw = None if weights is None else _flat(weights, (T, self._k), torch.float32, dev, "MoeQ4_0: weights")
+        px, ldx = _rows2(x, shape, x.dtype, dev, "MoeQ4_0: x")
+        po, ldo = _rows2(out, shape, x.dtype, dev, "MoeQ4_0: out")
+        pr, ldr = _rows2(res, shape, x.dtype, dev, "MoeQ4_0: res")
+        pi = None if ids is None else _flat(ids, (T, self._k), _torch.int32, dev, "MoeQ4_0: ids")
+        pw = None if weights is None else _flat(weights, (T, self._k), _torch.float32, dev, "MoeQ4_0: weights")
         if work is None:
             work = self._work
-        elif work.dtype is not torch.uint8 or work.get_device() != dev or not work.is_contiguous():
+        elif work.dtype is not _torch.uint8 or work.get_device() != dev or not work.is_contiguous():
             raise ValueError("MoeQ4_0: work must be contiguous uint8 on the layer's device")
         rc = _on(dev, stream, load().lk_moe_q4_0, self._ref, ty, px, ldx, T, pr, ldr, po, ldo, pi, pw,
                  work.data_ptr(), work.numel())

@@ -60,6 +60,17 @@ def test_large_shapes_bit_exact(lk, M, N, K, res):
     _case(lk, M, N, K, dt, res, 0, M + N + K)
 
 
+# tile counts on both sides of every line between the tiles: 32x32 / 64x32 / 64x64 /
+# 128x64 / 128x128 (one and two workgroups a unit) / 256x256; ragged in every direction
+@pytest.mark.parametrize("M,N,K", [(16, 4096, 300), (16, 4097, 300), (130, 1650, 515), (250, 2040, 260), (257, 2050, 1025),
+                                   (500, 2040, 130), (513, 2049, 129), (1000, 1030, 385), (1020, 2047, 641), (1030, 2050, 300),
+                                   (2000, 2020, 257), (2060, 2049, 129), (4090, 2040, 200), (3000, 4090, 400)])
+def test_lines_between_tiles_bit_exact(lk, M, N, K):
+    dt = list(TYPES.values())[(M + N) % 3]
+    note(f"gemm_i8 M={M} N={N} K={K} {dt}")
+    _case(lk, M, N, K, dt, (M + N + K) % 2 == 1, 16, M + N + K)
+
+
 @pytest.mark.parametrize("M", [1, 40])
 def test_largest_sums(lk, M):
     """-128 * -128 over the longest K: 2^31 - 2^14, the int32 range's end; and its
