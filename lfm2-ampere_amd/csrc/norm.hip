@@ -37,8 +37,12 @@ struct LkNormArgs {
     float eps;
 };
 
-// NW waves hold a row, 8 consecutive values per lane and chunk, C chunks; a
-// workgroup of 4 waves (16 for NW 16) holds 4 / NW rows.
+// NW waves hold a row, 8 consecutive values per lane and chunk, C chunks; a workgroup
+// has 4 waves or one row's, whichever is more.  One pass: the row stays in registers
+// between the sum of squares, the largest value and the quants, and w is asked for along
+// with x and delta.  What bounds it: one row, the launch and one load's latency (2.5 us a
+// call in a graph, 1 x 2048); many rows, memory: 4096 x 2048 with delta and res, bf16, 59 MB
+// in 12.6 us (4.6 TB/s), fp32, 109 MB in 18.2 us (6.0), next to 5.15 TB/s of a 1 GiB copy.
 template <int TYPE, int FORM, int NW, int C>
 __global__ void __launch_bounds__(NW > 4 ? 64 * NW : 256)
 lk_k_norm_q8(const LkNormArgs a) {
@@ -217,11 +221,24 @@ static void lk_norm_launch(const LkNormArgs & a, hipStream_t st) {
     hipLaunchKernelGGL((lk_k_norm_q8<TYPE, FORM, NW, C>), dim3((unsigned) ((a.rows - 1) / RW + 1)),
                        dim3(NW > 4 ? 64 * NW : 256), 0, st, a);
 }
+// As many waves as a row has runs of 512 values, so that all lanes have work and a lane one
+// chunk.  Measured, row form, us (<NW, C>):
+//   4096 x 1024 bf16   <2,1>  7.1   <1,2>  6.6   <4,1> 10.8 (half of the lanes idle)
+//   1 x 2048 fp32      <4,1>  2.6   <2,2>  3.3   <1,4>  4.1
+//   333 x 2048 bf16    <4,1>  3.5   <2,2>  3.9   <1,4>  5.0
+//   4096 x 2048 bf16   <4,1> 12.7   <2,2> 12.6   <1,4> 12.2
+//   1 x 4096 bf16      <8,1>  3.0   <4,2>  3.3   <4,4>  5.8
+//   4096 x 4096 bf16   <8,1> 21.4   <4,2> 21.8   <4,4> 31.3
+//   64 x 8192 bf16     <16,1> 4.2   <8,2>  4.3   <4,4>  5.1
+//   1024 x 16384 bf16  <16,2> 23.0  <8,4> 23.8   <16,4> 40.6
 template <int TYPE, int FORM>
 static void lk_norm_shape(const LkNormArgs & a, hipStream_t st) {
     if (a.n <= 512)        lk_norm_launch<TYPE, FORM, 1, 1>(a, st);
+    else if (a.n <= 1024)  lk_norm_launch<TYPE, FORM, 2, 1>(a, st);
     else if (a.n <= 2048)  lk_norm_launch<TYPE, FORM, 4, 1>(a, st);
-    else if (a.n <= 8192)  lk_norm_launch<TYPE, FORM, 4, 4>(a, st);
+    else if (a.n <= 4096)  lk_norm_launch<TYPE, FORM, 8, 1>(a, st);
+    else if (a.n <= 8192)  lk_norm_launch<TYPE, FORM, 16, 1>(a, st);
+    else if (a.n <= 16384) lk_norm_launch<TYPE, FORM, 16, 2>(a, st);
     else                   lk_norm_launch<TYPE, FORM, 16, 4>(a, st);
 }
 template <int TYPE>

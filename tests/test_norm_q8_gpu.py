@@ -65,6 +65,13 @@ def test_row_form(lk, rows, n, t):
     assert bool((off <= step / 2 + 8 * 2.0 ** -24 * ref.abs().amax(-1, keepdim=True)).all())
 
 
+@pytest.mark.parametrize("rows,n", [(9, 512), (3, 513), (5, 1024), (3, 1025), (2, 4096), (3, 4097), (2, 8192), (2, 8193), (1, 16384),
+                                    (2, 16385)])
+def test_row_form_at_the_lines_between_launch_shapes(lk, rows, n):
+    """One value more or less than the lanes of a launch shape hold."""
+    test_row_form(lk, rows, n, list(TYPES)[(rows + n) % 3])
+
+
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("rows,n", [(1, 32), (5, 64), (3, 2048), (2, 2080), (3, 4128), (1, 8224), (67, 256)])
 def test_q81_forms_are_the_quantisers_bytes(lk, rows, n, t):
