@@ -357,12 +357,13 @@ lk_k_moe_route(const LkMoeArgs a) {
 // ---- the products -------------------------------------------------------------------
 // 8 weight rows of NM matrices (qs, d: the first of the rows) times TK rows of records
 // (rec + trow[t] * bpr records), over the steps of 8 blocks of a row, U consecutive ones at
-// a time, of which this is part g0 of gs.  Lane (c = l % 8, g = l / 8) takes block g of a
+// a time, of which this is part g0 of gs.  Lane (c = l / 8, g = l % 8) takes block g of a
 // step of weight row c, whole: 16 bytes, its scale, and of every record row the block's
-// digits.  So a load covers a whole 128-byte line of each of 8 rows: with 16 rows and 64
-// bytes of each, 141 MB of weights came at 3.0 TB/s, and no other part of the kernel was
-// the limit.  The digits are the same for the 8 lanes of a block: the wave copies them, one
-// run of memory, into its own part of LDS (xs) and every lane reads them there.
+// digits.  So eight lanes in a row load a whole 128-byte line of a weight row, and 16 bytes
+// of its scales: with c = l % 8, another row in every lane, the scales' loads took as long
+// again as the weights' (64 tokens, gate and up, 226 MB: 70 us, so 63).  The digits are the
+// same for the 8 lanes of a block: the wave copies them, one run of memory, into its own
+// part of LDS (xs) and every lane reads them there.
 // acc[t][m]: this lane's blocks; the sum over the lanes of a row is the caller's.
 // Every address is a wave-uniform base and a 32-bit offset: an expert's planes are below
 // 4 GiB (LK_MOE_MAX_DIM).
@@ -407,7 +408,7 @@ __device__ __forceinline__ void lk_moe_rows(const uint8_t * const (&qs)[NM], con
                                             const uint8_t * rec, int bpr, const int (&trow)[TK], int g0, int gs,
                                             LkMoeX<NP, U> * xs, float (&acc)[TK][NM]) {
     constexpr int PC = LkMoeRec<NP>::PIECES, NZ = LkMoeX<NP, U>::NZ, NB = 8;
-    const int lane = threadIdx.x & 63, c = lane & 7, g = lane >> 3;
+    const int lane = threadIdx.x & 63, c = lane >> 3, g = lane & 7;
     const int ng = (bpr + NB - 1) / NB;
 #pragma unroll 1
     for (int gi = g0 * U; gi < ng; gi += gs * U) {
@@ -459,7 +460,11 @@ __device__ __forceinline__ void lk_moe_rows(const uint8_t * const (&qs)[NM], con
     }
 }
 // The sum over the eight lanes that hold blocks of one row, in every lane.
-__device__ __forceinline__ float lk_moe_lanes(float v) { return lk_xrow_sum(v + lk_dpp<LK_DPP_ROR8>(v)); }
+__device__ __forceinline__ float lk_moe_lanes(float v) {
+    v += lk_dpp<LK_DPP_QP_XOR1>(v);
+    v += lk_dpp<LK_DPP_QP_XOR2>(v);
+    return v + lk_dpp<LK_DPP_HMIRROR>(v);
+}
 
 // Where a wave of a gate/up workgroup finds its 16 + 16 of the tile's 32 rows (half:
 // 0 or 1): matrices 0, 1 the gate's rows 16 half .. +15, eight each, 2, 3 the up's.
@@ -486,7 +491,7 @@ struct LkMoeUp {
 template <int NP, int N>
 __device__ __forceinline__ void lk_moe_up_tile(const LkMoeArgs & a, int e, const int * as, int as0, LkMoeUp<NP> & sh) {
     constexpr int U = LkMoeUp<NP>::U, REC = LkMoeRec<NP>::BYTES;
-    const int tid = threadIdx.x, lane = tid & 63, c = lane & 7, g = lane >> 3;
+    const int tid = threadIdx.x, lane = tid & 63, c = lane >> 3, g = lane & 7;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), half = wv & 1, kp = wv >> 1, F = a.ffn;
     const uint8_t * qs[4];
     const _Float16 * d[4];
@@ -589,7 +594,7 @@ __device__ __forceinline__ void lk_moe_many_rows(const uint8_t * const (&qs)[4],
                                                  int bpr, const int (&trow)[N], LkMoeShare<NP> & sh, float (&acc)[N][4]) {
     constexpr int PC = LkMoeRec<NP>::PIECES, Z = LkMoeShare<NP>::Z;
     static_assert(Z <= 64, "a step's digits are one copy");
-    const int lane = threadIdx.x & 63, c = lane & 7, g = lane >> 3, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, c = lane >> 3, g = lane & 7, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ns = (bpr + 7) / 8;                        // steps; this wave's are s0, s0 + 2, ...
     const uint32_t lds = lk_lds_addr(&sh.x[wv][0][0]);
     lk_u4 w[4];
@@ -643,7 +648,7 @@ __device__ __forceinline__ void lk_moe_many_rows(const uint8_t * const (&qs)[4],
 // N assignments (as, of which n count) of an expert.
 template <int NP, int N>
 __device__ __forceinline__ void lk_moe_up_many(const LkMoeArgs & a, int e, const int (&as)[N], int n, LkMoeShare<NP> & sh) {
-    const int F = a.ffn, tid = threadIdx.x, lane = tid & 63, c = lane & 7, g = lane >> 3;
+    const int F = a.ffn, tid = threadIdx.x, lane = tid & 63, c = lane >> 3, g = lane & 7;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), half = wv & 1;
     const uint8_t * qs[4];
     const _Float16 * d[4];
@@ -672,7 +677,7 @@ __device__ __forceinline__ void lk_moe_up_many(const LkMoeArgs & a, int e, const
 }
 template <int NP, int N>
 __device__ __forceinline__ void lk_moe_down_many(const LkMoeArgs & a, int e, const int (&as)[N], int n, LkMoeShare<NP> & sh) {
-    const int bpr = a.ffn / 32, H = a.hidden, r0 = blockIdx.x * 64, tid = threadIdx.x, lane = tid & 63, c = lane & 7, g = lane >> 3;
+    const int bpr = a.ffn / 32, H = a.hidden, r0 = blockIdx.x * 64, tid = threadIdx.x, lane = tid & 63, c = lane >> 3, g = lane & 7;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), half = wv & 1;
     const uint8_t * qs[4];
     const _Float16 * d[4];
@@ -744,7 +749,7 @@ lk_k_moe_down_few(const LkMoeArgs a) {
     // [q][assignment][row]: q * assignments is at most 16 / experts * (experts * LK_MOE_FEW), or MAXA
     __shared__ float part[LK_MOE_NWF * LK_MOE_FEW][R];
     static_assert(LK_MOE_NWF * LK_MOE_FEW >= MAXA, "part");
-    const int tid = threadIdx.x, lane = tid & 63, c = lane % R, g = lane / R;
+    const int tid = threadIdx.x, lane = tid & 63, c = lane >> 3, g = lane & 7;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), na = a.T * a.k, r0 = blockIdx.x * R, bpr = a.ffn / 32;
     const int mine = lane < na ? a.ids[lane] : -1;
     // what the sum at the end needs, asked for now (T * R <= 64: the first wave)
