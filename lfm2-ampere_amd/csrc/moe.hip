@@ -577,17 +577,32 @@ lk_k_moe_up_few(const LkMoeArgs a) {
 }
 
 // More tokens: a workgroup of 4 waves has 32 rows (up: of gate and up) or 64 (down) of
-// one expert and up to eight of its assignments at a time.  Wave w has half w & 1 of the rows
+// one expert and up to TG of its assignments at a time.  Wave w has half w & 1 of the rows
 // (four matrices of 8 rows) and every second step of 8 blocks of K; it copies a step's
 // digits into its own part of LDS while the step's weights are on their way, which are
-// asked for before the dots of the step before.  The loop is kept short (one step): with two
-// steps the kernel had 57 KB of code, and fetching it under a saturated memory took up to 5
-// us a workgroup.
+// asked for before the products of the step before.
+// One or two assignments: the dots above.  More: v_mfma_i32_16x16x32_i8, a block of 16 weight
+// rows (the second operand) against the digits of TG assignments (the first: NP = 2, row 2 t +
+// p is digit p of t; NP = 3, row 4 t + p, and p = 3 the last digit again), for which the
+// weights go by way of LDS: they come as whole blocks a lane, and lane (row l % 16, g =
+// l / 16) multiplies dword g of a block, nibbles as 16 (n - 8).  The products of 8
+// assignments cost a wave about 13 vector operations for 16 rows of a block and of one
+// assignment 20 as dots, so that they start to pay at three.
 template <int NP>
 struct LkMoeShare {
     static constexpr int Z = 8 * LkMoeRec<NP>::PIECES;   // pieces of a step's digits
-    lk_u4 x[4][8][Z];
-    float part[2][8][64];                                // [part of K][token][row of 32 gate and 32 up, or of 64]
+    static constexpr int TG = NP == 2 ? 8 : 4;
+    // the digits of assignment t, so far apart that the 16 rows' reads use all banks alike
+    static __device__ __forceinline__ constexpr int at(int t) { return t * Z + 4 * (t / 2); }
+    struct Wave {
+        lk_u4 x[TG * Z + 4 * ((TG - 1) / 2)];
+        lk_u4 w[32][8];                                  // rows' blocks, block b of row r in slot b ^ r / 2 % 8
+        lk_u4 d[32];                                     // their scales
+    };
+    union {
+        Wave wave[4];
+        float part[2][TG][64];                           // [part of K][assignment][row of 32 gate and 32 up, or of 64]
+    };
 };
 template <int NP, int N>
 __device__ __forceinline__ void lk_moe_many_rows(const uint8_t * const (&qs)[4], const _Float16 * const (&d)[4], const uint8_t * rec,
@@ -596,7 +611,8 @@ __device__ __forceinline__ void lk_moe_many_rows(const uint8_t * const (&qs)[4],
     static_assert(Z <= 64, "a step's digits are one copy");
     const int lane = threadIdx.x & 63, c = lane >> 3, g = lane & 7, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ns = (bpr + 7) / 8;                        // steps; this wave's are s0, s0 + 2, ...
-    const uint32_t lds = lk_lds_addr(&sh.x[wv][0][0]);
+    typename LkMoeShare<NP>::Wave & me = sh.wave[wv];
+    const uint32_t lds = lk_lds_addr(me.x);
     lk_u4 w[4];
     _Float16 dw[4];
     auto load = [&](int s) {
@@ -613,7 +629,7 @@ __device__ __forceinline__ void lk_moe_many_rows(const uint8_t * const (&qs)[4],
 #pragma unroll
         for (int t = 0; t < N; ++t) {
             const uint8_t * src = rec + ((size_t) trow[t] * bpr + (left > 0 ? 8 * s : 0)) * (PC * 16);
-            if (lane < Z) lk_dma16c_so(src, 16u * (lane < left ? lane : 0), lds + 16u * (t * Z));
+            if (lane < Z) lk_dma16c_so(src, 16u * (lane < left ? lane : 0), lds + 16u * LkMoeShare<NP>::at(t));
         }
     };
     load(wv >> 1);
@@ -636,7 +652,7 @@ __device__ __forceinline__ void lk_moe_many_rows(const uint8_t * const (&qs)[4],
         load(s + 2);                                     // past the last: in bounds, not used
 #pragma unroll
         for (int t = 0; t < N; ++t) {
-            lk_moe_token_dots<NP, 4>(&sh.x[wv][t][g * PC], in, lo, hi, dv, acc[t]);
+            lk_moe_token_dots<NP, 4>(me.x + LkMoeShare<NP>::at(t) + g * PC, in, lo, hi, dv, acc[t]);
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");          // the digits have been read
         copy(s + 2);
@@ -645,39 +661,170 @@ __device__ __forceinline__ void lk_moe_many_rows(const uint8_t * const (&qs)[4],
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-// N assignments (as, of which n count) of an expert.
-template <int NP, int N>
-__device__ __forceinline__ void lk_moe_up_many(const LkMoeArgs & a, int e, const int (&as)[N], int n, LkMoeShare<NP> & sh) {
-    const int F = a.ffn, tid = threadIdx.x, lane = tid & 63, c = lane >> 3, g = lane & 7;
-    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), half = wv & 1;
-    const uint8_t * qs[4];
-    const _Float16 * d[4];
-    lk_moe_up_rows(a, e, half, qs, d);
-    int trow[N];
+// The same for n of up to TG assignments.  sum[j][q]: 16 rows of matrices 2 j and 2 j + 1, row l %
+// 16; assignment 2 (l / 16) + q of two digits, l / 16 of three.  The blocks of a step are summed
+// apart over the steps and joined as the dots' lanes are, so that a token's result does not
+// depend, by a bit, on how many others chose its expert.
+template <int NP>
+__device__ __forceinline__ void lk_moe_many_mfma(const uint8_t * const (&qs)[4], const _Float16 * const (&d)[4], const uint8_t * rec,
+                                                 int bpr, const int (&trow)[LkMoeShare<NP>::TG], int n, LkMoeShare<NP> & sh,
+                                                 float (&sum)[2][4 - NP]) {
+    constexpr int PC = LkMoeRec<NP>::PIECES, Z = LkMoeShare<NP>::Z, TG = LkMoeShare<NP>::TG, NQ = 4 - NP;
+    const int lane = threadIdx.x & 63, c = lane >> 3, g = lane & 7, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, h = lane >> 4, ns = (bpr + 7) / 8;
+    typename LkMoeShare<NP>::Wave & me = sh.wave[wv];
+    const uint32_t lds = lk_lds_addr(me.x);
+    const int t = NP == 2 ? r >> 1 : r >> 2, p = NP == 2 ? r & 1 : (r & 3) < 3 ? r & 3 : 2;
+    const uint32_t * xa = (const uint32_t *) (me.x + LkMoeShare<NP>::at(t) + 2 * p) + h;   // + 4 PC b: the row's digits 4 h ..; 16 + 4 h .. behind 4
+    const float * xs[NQ];                                // + 4 PC b: the scales
 #pragma unroll
-    for (int t = 0; t < N; ++t) trow[t] = lk_moe_token(a, as[t]);
-    float acc[N][4] = {};
-    lk_moe_many_rows<NP, N>(qs, d, a.xr, a.hidden / 32, trow, sh, acc);
-#pragma unroll
-    for (int t = 0; t < N; ++t)
+    for (int q = 0; q < NQ; ++q) xs[q] = (const float *) (me.x + LkMoeShare<NP>::at(NQ * h + q) + 2 * NP) + 3;
+    lk_u4 w[4];
+    _Float16 dw[4];
+    auto load = [&](int s) {
+        const int b = 8 * s + g;
+        const uint32_t wb = (uint32_t) (c * bpr + (b < bpr ? b : bpr - 1));                      // in bounds
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-            const float v = lk_moe_lanes(acc[t][m]);
-            if (g == m) sh.part[wv >> 1][t][32 * (m >> 1) + 16 * half + 8 * (m & 1) + c] = v;
+            w[m] = lk_moe_ld<lk_u4>(qs[m], wb * 16u);
+            dw[m] = lk_moe_ld<_Float16>(d[m], wb * 2u);
         }
+    };
+    auto copy = [&](int s) {
+        if (s >= ns) return;                             // wave-uniform, as the next two
+        const int left = (bpr - 8 * s) * PC;             // pieces to the row's end
+#pragma unroll
+        for (int t = 0; t < TG; ++t) {
+            if (t >= n) break;
+            const uint8_t * src = rec + ((size_t) trow[t] * bpr + 8 * s) * (PC * 16);
+            if (lane < Z && lane < left) lk_dma16c_so(src, 16u * lane, lds + 16u * LkMoeShare<NP>::at(t));
+            if (left < Z && lane >= left && lane < Z) me.x[LkMoeShare<NP>::at(t) + lane] = lk_u4{ 0, 0, 0, 0 };
+        }
+    };
+    float acc[8][2][NQ] = {};
+    load(wv >> 1);
+    copy(wv >> 1);
+#pragma unroll 1
+    for (int s = wv >> 1; s < ns; s += 2) {
+        const bool in = 8 * s + g < bpr;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // the copies; the weights, asked for before, come with them
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            me.w[8 * m + c][g ^ (4 * (m & 1) + (c >> 1))] = w[m];
+            ((_Float16 *) &me.d[8 * m + c])[g] = in ? dw[m] : (_Float16) 0.0f;
+        }
+        __builtin_amdgcn_wave_barrier();
+        load(s + 2);                                     // past the last: in bounds, not used
+        union { lk_u4 q; _Float16 h[8]; } dv[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) dv[j].q = me.d[16 * j + r];
+        uint64_t xd[2];
+        float sc[2][NQ];
+        uint32_t v[2][2];
+        auto read = [&](int b) {
+            xd[b & 1] = xa[4 * PC * b] | (uint64_t) xa[4 * PC * b + 4] << 32;
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) sc[b & 1][q] = xs[q][4 * PC * b];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) v[b & 1][j] = ((const uint32_t *) &me.w[16 * j + r][b ^ (r >> 1)])[h];
+        };
+        read(0);
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {                    // a block's operands are read before the products of the one before
+            if (b < 7) read(b + 1);
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const uint32_t u = v[b & 1][j], lo = (u << 4 & 0xF0F0F0F0u) ^ 0x80808080u, hi = (u & 0xF0F0F0F0u) ^ 0x80808080u;
+                const lk_i4 s4 = __builtin_amdgcn_mfma_i32_16x16x32_i8((long) xd[b & 1], (long) (lo | (uint64_t) hi << 32),
+                                                                       lk_i4{ 0, 0, 0, 0 }, 0, 0, 0);
+                const float dd = (float) dv[j].h[b] * 0.0625f;       // the nibbles are 16 times theirs
+                if constexpr (NP == 2) {                 // a digit's sum is at most 32 * 128 * 128 = 2^19
+                    acc[b][j][0] = __builtin_fmaf(dd * sc[b & 1][0], (float) (s4[0] * 256 + s4[1]), acc[b][j][0]);
+                    acc[b][j][1] = __builtin_fmaf(dd * sc[b & 1][1], (float) (s4[2] * 256 + s4[3]), acc[b][j][1]);
+                } else {
+                    const float f = __builtin_fmaf((float) (s4[0] * 256 + s4[1]), 256.0f, (float) s4[2]);
+                    acc[b][j][0] = __builtin_fmaf(dd * sc[b & 1][0], f, acc[b][j][0]);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) asm volatile("" : "+v"(acc[b][j][q]) :: "memory");
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");          // the digits have been read
+        copy(s + 2);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+            sum[j][q] = ((acc[0][j][q] + acc[1][j][q]) + (acc[2][j][q] + acc[3][j][q])) +
+                        ((acc[4][j][q] + acc[5][j][q]) + (acc[6][j][q] + acc[7][j][q]));
+}
+
+// n of up to TG assignments (as, the rows of records trow) of an expert: the sums of the
+// workgroup's 64 rows over each part of K, into sh.part.
+template <int NP, bool UP>
+__device__ __forceinline__ void lk_moe_many_part(const uint8_t * const (&qs)[4], const _Float16 * const (&d)[4], const uint8_t * rec,
+                                                 int bpr, const int (&trow)[LkMoeShare<NP>::TG], int n, LkMoeShare<NP> & sh) {
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = wv & 1, kp = wv >> 1;
+    if (n <= 2) {
+        const int c = lane >> 3, g = lane & 7;
+        auto go = [&](auto count) {
+            constexpr int N = decltype(count)::value;
+            int tr[N];
+#pragma unroll
+            for (int t = 0; t < N; ++t) tr[t] = trow[t];
+            float acc[N][4] = {};
+            lk_moe_many_rows<NP, N>(qs, d, rec, bpr, tr, sh, acc);
+            __syncthreads();                             // part lies where the digits were
+#pragma unroll
+            for (int t = 0; t < N; ++t)
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+                    const float v = lk_moe_lanes(acc[t][m]);
+                    if (g == m) sh.part[kp][t][UP ? 32 * (m >> 1) + 16 * half + 8 * (m & 1) + c : 32 * half + 8 * m + c] = v;
+                }
+        };
+        if (n == 1) go(LkInt<1>{});
+        else        go(LkInt<2>{});
+    } else {
+        constexpr int NQ = 4 - NP;
+        float acc[2][NQ];
+        lk_moe_many_mfma<NP>(qs, d, rec, bpr, trow, n, sh, acc);
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int q = 0; q < NQ; ++q)
+                sh.part[kp][NQ * (lane >> 4) + q][(UP ? 32 * j + 16 * half : 32 * half + 16 * j) + (lane & 15)] = acc[j][q];
+    }
     __syncthreads();
+}
+template <int NP>
+__device__ __forceinline__ void lk_moe_up_many(const LkMoeArgs & a, int e, const int (&as)[LkMoeShare<NP>::TG], int n, LkMoeShare<NP> & sh) {
+    constexpr int TG = LkMoeShare<NP>::TG;
+    const int F = a.ffn, tid = threadIdx.x;
+    const uint8_t * qs[4];
+    const _Float16 * d[4];
+    lk_moe_up_rows(a, e, __builtin_amdgcn_readfirstlane(tid >> 6) & 1, qs, d);
+    int trow[TG];
+#pragma unroll
+    for (int t = 0; t < TG; ++t) trow[t] = lk_moe_token(a, as[t]);
+    lk_moe_many_part<NP, true>(qs, d, a.xr, a.hidden / 32, trow, n, sh);
     const int t = tid >> 5, r = tid & 31;
-    if (t < N) {                                         // whole halves of waves
+    if (t < n) {                                         // whole halves of waves
         const float gt = sh.part[0][t][r] + sh.part[1][t][r], up = sh.part[0][t][32 + r] + sh.part[1][t][32 + r];
         int at = as[0];
 #pragma unroll
-        for (int k = 1; k < N; ++k) at = t == k ? as[k] : at;
-        lk_moe_record<NP>(lk_moe_h(gt, up), r, t < n, a.hr + ((size_t) at * (F / 32) + blockIdx.x) * LkMoeRec<NP>::BYTES);
+        for (int k = 1; k < TG; ++k) at = t == k ? as[k] : at;
+        lk_moe_record<NP>(lk_moe_h(gt, up), r, true, a.hr + ((size_t) at * (F / 32) + blockIdx.x) * LkMoeRec<NP>::BYTES);
     }
 }
-template <int NP, int N>
-__device__ __forceinline__ void lk_moe_down_many(const LkMoeArgs & a, int e, const int (&as)[N], int n, LkMoeShare<NP> & sh) {
-    const int bpr = a.ffn / 32, H = a.hidden, r0 = blockIdx.x * 64, tid = threadIdx.x, lane = tid & 63, c = lane >> 3, g = lane & 7;
+template <int NP>
+__device__ __forceinline__ void lk_moe_down_many(const LkMoeArgs & a, int e, const int (&as)[LkMoeShare<NP>::TG], int n, LkMoeShare<NP> & sh) {
+    const int bpr = a.ffn / 32, H = a.hidden, r0 = blockIdx.x * 64, tid = threadIdx.x, lane = tid & 63;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), half = wv & 1;
     const uint8_t * qs[4];
     const _Float16 * d[4];
@@ -687,53 +834,32 @@ __device__ __forceinline__ void lk_moe_down_many(const LkMoeArgs & a, int e, con
         qs[m] = a.qs[2] + row * bpr * 16;
         d[m] = a.d[2] + row * bpr;
     }
-    float acc[N][4] = {};
-    lk_moe_many_rows<NP, N>(qs, d, a.hr, bpr, as, sh, acc);
+    lk_moe_many_part<NP, false>(qs, d, a.hr, bpr, as, n, sh);
 #pragma unroll
-    for (int t = 0; t < N; ++t)
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            const float v = lk_moe_lanes(acc[t][m]);
-            if (g == m) sh.part[wv >> 1][t][32 * half + 8 * m + c] = v;
-        }
-    __syncthreads();
-#pragma unroll
-    for (int t = 0; t < N; ++t)                          // a wave per assignment
+    for (int t = 0; t < LkMoeShare<NP>::TG; ++t)         // a wave per assignment
         if ((t & 3) == wv && t < n && r0 + lane < H)
             a.y[(size_t) as[t] * H + r0 + lane] = sh.part[0][t][lane] + sh.part[1][t][lane];
 }
 
 // grid (row tiles, slots)
 template <int NP, bool UP>
-__global__ void __launch_bounds__(LK_MOE_THREADS, NP == 3 ? 3 : 4)
+__global__ void __launch_bounds__(LK_MOE_THREADS, 4)
 lk_k_moe_many(const LkMoeArgs a) {
+    constexpr int TG = LkMoeShare<NP>::TG;
     __shared__ LkMoeShare<NP> sh;
     // written by the launch before: read as constants, by scalar loads
     typedef const __attribute__((address_space(4))) LkMoeTab Tab;
     Tab & tab = *(Tab *) (uintptr_t) a.tab;
     const int slot = blockIdx.y, e = tab.slot[slot].e, n = tab.slot[slot].n;
-    auto go = [&](auto count, int at) {
-        constexpr int N = decltype(count)::value;
-        const int left = n - at < N ? n - at : N;
-        int as[N];
-#pragma unroll
-        for (int t = 0; t < N; ++t) as[t] = tab.list[slot][at + (t < left ? t : 0)];
-        if constexpr (UP) lk_moe_up_many<NP, N>(a, e, as, left, sh);
-        else              lk_moe_down_many<NP, N>(a, e, as, left, sh);
-    };
-    for (int at = 0; at < n; at += 8) {
+#pragma unroll 1
+    for (int at = 0; at < n; at += TG) {
         if (at) __syncthreads();                         // part has been read
-        const int left = n - at;
-        switch (left < 8 ? left : 8) {
-        case 1:  go(LkInt<1>{}, at); break;
-        case 2:  go(LkInt<2>{}, at); break;
-        case 3:  go(LkInt<3>{}, at); break;
-        case 4:  go(LkInt<4>{}, at); break;
-        case 5:  go(LkInt<5>{}, at); break;
-        case 6:  go(LkInt<6>{}, at); break;
-        case 7:  go(LkInt<7>{}, at); break;
-        default: go(LkInt<8>{}, at);
-        }
+        const int left = n - at < TG ? n - at : TG;
+        int as[TG];
+#pragma unroll
+        for (int t = 0; t < TG; ++t) as[t] = tab.list[slot][at + (t < left ? t : 0)];
+        if constexpr (UP) lk_moe_up_many<NP>(a, e, as, left, sh);
+        else              lk_moe_down_many<NP>(a, e, as, left, sh);
     }
 }
 
