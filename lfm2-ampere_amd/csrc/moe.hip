@@ -581,13 +581,14 @@ lk_k_moe_up_few(const LkMoeArgs a) {
 // (four matrices of 8 rows) and every second step of 8 blocks of K; it copies a step's
 // digits into its own part of LDS while the step's weights are on their way, which are
 // asked for before the products of the step before.
-// One or two assignments: the dots above.  More: v_mfma_i32_16x16x32_i8, a block of 16 weight
+// One assignment: the dots above.  More: v_mfma_i32_16x16x32_i8, a block of 16 weight
 // rows (the second operand) against the digits of TG assignments (the first: NP = 2, row 2 t +
 // p is digit p of t; NP = 3, row 4 t + p, and p = 3 the last digit again), for which the
 // weights go by way of LDS: they come as whole blocks a lane, and lane (row l % 16, g =
 // l / 16) multiplies dword g of a block, nibbles as 16 (n - 8).  The products of 8
 // assignments cost a wave about 13 vector operations for 16 rows of a block and of one
-// assignment 20 as dots, so that they start to pay at three.
+// assignment 20 as dots, so that they pay from two on: 19 tokens 61 us with dots up to two,
+// 58 up to one, 62 without; 64 tokens (four an expert) 97, 92, 92; dots alone 65 and 112.
 template <int NP>
 struct LkMoeShare {
     static constexpr int Z = 8 * LkMoeRec<NP>::PIECES;   // pieces of a step's digits
@@ -604,9 +605,9 @@ struct LkMoeShare {
         float part[2][TG][64];                           // [part of K][assignment][row of 32 gate and 32 up, or of 64]
     };
 };
-template <int NP, int N>
-__device__ __forceinline__ void lk_moe_many_rows(const uint8_t * const (&qs)[4], const _Float16 * const (&d)[4], const uint8_t * rec,
-                                                 int bpr, const int (&trow)[N], LkMoeShare<NP> & sh, float (&acc)[N][4]) {
+template <int NP>
+__device__ __forceinline__ void lk_moe_many_dots(const uint8_t * const (&qs)[4], const _Float16 * const (&d)[4], const uint8_t * rec,
+                                                 int bpr, int trow, LkMoeShare<NP> & sh, float (&acc)[4]) {
     constexpr int PC = LkMoeRec<NP>::PIECES, Z = LkMoeShare<NP>::Z;
     static_assert(Z <= 64, "a step's digits are one copy");
     const int lane = threadIdx.x & 63, c = lane >> 3, g = lane & 7, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -626,11 +627,8 @@ __device__ __forceinline__ void lk_moe_many_rows(const uint8_t * const (&qs)[4],
     };
     auto copy = [&](int s) {
         const int left = (bpr - 8 * s) * PC;             // pieces to the row's end; none: the row's first
-#pragma unroll
-        for (int t = 0; t < N; ++t) {
-            const uint8_t * src = rec + ((size_t) trow[t] * bpr + (left > 0 ? 8 * s : 0)) * (PC * 16);
-            if (lane < Z) lk_dma16c_so(src, 16u * (lane < left ? lane : 0), lds + 16u * LkMoeShare<NP>::at(t));
-        }
+        const uint8_t * src = rec + ((size_t) trow * bpr + (left > 0 ? 8 * s : 0)) * (PC * 16);
+        if (lane < Z) lk_dma16c_so(src, 16u * (lane < left ? lane : 0), lds);
     };
     load(wv >> 1);
     copy(wv >> 1);
@@ -650,10 +648,7 @@ __device__ __forceinline__ void lk_moe_many_rows(const uint8_t * const (&qs)[4],
             }
         }
         load(s + 2);                                     // past the last: in bounds, not used
-#pragma unroll
-        for (int t = 0; t < N; ++t) {
-            lk_moe_token_dots<NP, 4>(me.x + LkMoeShare<NP>::at(t) + g * PC, in, lo, hi, dv, acc[t]);
-        }
+        lk_moe_token_dots<NP, 4>(me.x + g * PC, in, lo, hi, dv, acc);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");          // the digits have been read
         copy(s + 2);
     }
@@ -769,26 +764,16 @@ template <int NP, bool UP>
 __device__ __forceinline__ void lk_moe_many_part(const uint8_t * const (&qs)[4], const _Float16 * const (&d)[4], const uint8_t * rec,
                                                  int bpr, const int (&trow)[LkMoeShare<NP>::TG], int n, LkMoeShare<NP> & sh) {
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = wv & 1, kp = wv >> 1;
-    if (n <= 2) {
+    if (n == 1) {
         const int c = lane >> 3, g = lane & 7;
-        auto go = [&](auto count) {
-            constexpr int N = decltype(count)::value;
-            int tr[N];
+        float acc[4] = {};
+        lk_moe_many_dots<NP>(qs, d, rec, bpr, trow[0], sh, acc);
+        __syncthreads();                                 // part lies where the digits were
 #pragma unroll
-            for (int t = 0; t < N; ++t) tr[t] = trow[t];
-            float acc[N][4] = {};
-            lk_moe_many_rows<NP, N>(qs, d, rec, bpr, tr, sh, acc);
-            __syncthreads();                             // part lies where the digits were
-#pragma unroll
-            for (int t = 0; t < N; ++t)
-#pragma unroll
-                for (int m = 0; m < 4; ++m) {
-                    const float v = lk_moe_lanes(acc[t][m]);
-                    if (g == m) sh.part[kp][t][UP ? 32 * (m >> 1) + 16 * half + 8 * (m & 1) + c : 32 * half + 8 * m + c] = v;
-                }
-        };
-        if (n == 1) go(LkInt<1>{});
-        else        go(LkInt<2>{});
+        for (int m = 0; m < 4; ++m) {
+            const float v = lk_moe_lanes(acc[m]);
+            if (g == m) sh.part[kp][0][UP ? 32 * (m >> 1) + 16 * half + 8 * (m & 1) + c : 32 * half + 8 * m + c] = v;
+        }
     } else {
         constexpr int NQ = 4 - NP;
         float acc[2][NQ];
