@@ -27,7 +27,11 @@ typedef uint32_t lk_u4 __attribute__((ext_vector_type(4)));
 // Up to this many tokens every workgroup chooses the experts itself, a wave per
 // token, and the down product adds the experts up itself (three launches); above it a
 // launch of one workgroup chooses once and sorts the tokens by expert, and another
-// adds up (five).
+// adds up (five).  us with three / five launches, bf16:
+//   tokens                          2          4          5          8
+//   64 experts, 4 of 2048 x 1536    20 / 26    30 / 33    33 / 34    47 / 47
+//   32 experts, 2 of 2048 x 1792    16 / 21    20 / 25    23 / 29    32 / 35
+//   128 experts, 8 of 2048 x 768     23 / 30    36 / 38    39 / 43    55 / 55
 #define LK_MOE_FEW 8
 #define LK_MOE_THREADS 256
 #define LK_MOE_NW 8                       // waves of a gate/up workgroup for few tokens
@@ -621,7 +625,8 @@ __device__ __forceinline__ void lk_moe_many_dots(const uint8_t * const (&qs)[4],
         const uint32_t wb = (uint32_t) (c * bpr + (b < bpr ? b : bpr - 1));                      // in bounds
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-            w[m] = lk_moe_ld<lk_u4>(qs[m], wb * 16u);
+            // read once: past the caches' order, so that the lines of scales stay (10 tokens 53 us, so 50)
+            w[m] = __builtin_nontemporal_load((const lk_u4 *) ((const char *) qs[m] + wb * 16u));
             dw[m] = lk_moe_ld<_Float16>(d[m], wb * 2u);
         }
     };
