@@ -276,3 +276,18 @@ def test_fewer_tokens_than_made_for(lk):
             continue
         out, _, _ = _run(lk, layer, x, hidden, torch.float32, 2)
         _close(out, moe_ref(x, k=2, score="sigmoid", **L)[0], torch.float32, T)
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_a_token_does_not_depend_on_the_others(lk, t):
+    """Above eight tokens a row's bytes are the same alone with few at its experts and among
+    many: experts met once take one kind of product, the others another."""
+    hidden, ffn, E, k = 544, 352, 12, 3                  # 17 and 11 blocks: last steps of one and three
+    dt = TYPES[t]
+    layer = _make(lk, _layer(41, E, hidden, ffn), k)
+    x = _x(42, 64, hidden, dt)
+    note(f"moe rows in batches of 64, 32, 16 and 9 {t}")
+    whole, _, _ = _run(lk, layer, x, hidden, dt, k)
+    for T in (32, 16, 9):
+        for at in range(0, 64 - T + 1, T):
+            assert torch.equal(_run(lk, layer, x[at:at + T], hidden, dt, k)[0], whole[at:at + T]), (T, at)
