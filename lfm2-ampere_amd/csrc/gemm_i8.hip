@@ -128,7 +128,7 @@ lk_k_gemm_i8(const LkI8Args a) {
     // consecutive tiles L are given to one XCD; L runs through groups of 8 row tiles,
     // row tiles first, so that the tiles an XCD works on at a time form a patch
     // whose operands its L2 holds once.
-    const int nrt = (a.N + SH::BM - 1) / SH::BM, ntt = (a.M + SH::BN - 1) / SH::BN, ntile = nrt * ntt;
+    const int nrt = (a.N - 1) / SH::BM + 1, ntt = (a.M - 1) / SH::BN + 1, ntile = nrt * ntt;
     const int id = blockIdx.x, x8 = id & 7, rem = ntile & 7;
     const int L = x8 * (ntile >> 3) + (x8 < rem ? x8 : rem) + (id >> 3);
     const int gr = L / (8 * ntt), gw = nrt - 8 * gr < 8 ? nrt - 8 * gr : 8, li = L - gr * 8 * ntt;
@@ -309,10 +309,12 @@ template <int TYPE, int NW>
 static void lk_i8_few(const LkI8Args & a, hipStream_t st) {
     hipLaunchKernelGGL((lk_k_gemm_i8_few<TYPE, NW>), dim3((a.N + 15) / 16), dim3(64 * NW), 0, st, a);
 }
+template <int BM, int BN>
+static long lk_i8_ntile(const LkI8Args & a) { return (long) ((a.N - 1) / BM + 1) * ((a.M - 1) / BN + 1); }        // M, N >= 1
 template <class SH, int TYPE>
 static int lk_i8_tiles(const LkI8Args & a, hipStream_t st) {
-    const long n = (long) ((a.N + SH::BM - 1) / SH::BM) * ((a.M + SH::BN - 1) / SH::BN);
-    if (n > 0x7FFFFFFF) return lk_fail(hipErrorInvalidValue, "lk_gemm_i8: %d x %d outputs", a.M, a.N);
+    const long n = lk_i8_ntile<SH::BM, SH::BN>(a);       // a grid has fewer than 2^32 threads
+    if (n * 64 * SH::NW >= 1l << 32) return lk_fail(hipErrorInvalidValue, "lk_gemm_i8: %d x %d outputs", a.M, a.N);
     hipLaunchKernelGGL((lk_k_gemm_i8<SH, TYPE>), dim3((unsigned) n), dim3(64 * SH::NW), 0, st, a);
     return 0;
 }
@@ -336,9 +338,6 @@ static int lk_i8_tiles(const LkI8Args & a, hipStream_t st) {
 //   2600 x 8192 x 2048                             71.3     71.3    60.6*   65.7
 //   4096 x 8192 x 2048                            104.8    100.8    86.0    76.3*
 // A round of 256 256x256 tiles takes about 5 / 3 of one of 512 128x128 tiles.
-template <int BM, int BN>
-static long lk_i8_ntile(const LkI8Args & a) { return (long) ((a.N + BM - 1) / BM) * ((a.M + BN - 1) / BN); }
-
 template <int TYPE>
 static int lk_i8_shape(const LkI8Args & a, hipStream_t st) {
     if (a.M <= 16 && (a.N <= 4096 || (a.N <= 8192 && a.K <= 2048 && a.M <= 8))) {

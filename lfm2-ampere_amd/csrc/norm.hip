@@ -259,6 +259,9 @@ extern "C" int lk_norm_q8(int type, const void * x, int ldx, const void * delta,
     if (form != LK_Q8_ROW && n % 32 != 0)
         return lk_fail(hipErrorInvalidValue, "lk_norm_q8: n %d must be a multiple of 32 for Q8_1 blocks", n);
     if (rows == 0) return 0;
+    // a grid has fewer than 2^32 threads, a workgroup 256 or more (1024 above 4096 values)
+    if ((n > 4096 ? 1024l : n > 2048 ? 512l : n > 1024 ? 256l : n > 512 ? 128l : 64l) * rows > 0xFFFFFE00l)
+        return lk_fail(hipErrorInvalidValue, "lk_norm_q8: %d rows of %d", rows, n);
     if (!x || !w || !q || (form != LK_Q81_BLOCK && !sc))
         return lk_fail(hipErrorInvalidValue, "lk_norm_q8: null pointer argument");
     if (ldx < n || (delta && ldd < n) || (res && ldr < n) || (y && ldy < n) || (form == LK_Q8_ROW && ldq < n) ||

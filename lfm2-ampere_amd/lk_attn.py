@@ -488,6 +488,8 @@ def _rows2(t, shape: tuple, dtype, dev: int, what: str) -> tuple:
     s0, s1 = t.stride()
     if (s1 != 1 and n > 1) or (rows > 1 and s0 < n):
         raise ValueError(f"{what}: rows must be contiguous and must not overlap (strides {s0}, {s1})")
+    if s0 > 0x7FFFFFFF and rows > 1 or rows > 0x7FFFFFFF or n > 0x7FFFFFFF:
+        raise ValueError(f"{what}: {rows} rows of {n}, {s0} apart: beyond what the entry points count")
     return t.data_ptr(), s0 if rows > 1 else n
 
 

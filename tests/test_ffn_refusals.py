@@ -23,7 +23,8 @@ def test_norm_c_refusals(lk_host):
                 dict(sc=None), dict(ldx=63), dict(delta=P, ldd=63), dict(res=P, ldr=63), dict(y=P, ldy=63), dict(ldq=63),
                 dict(form=1, ldq=80), dict(form=2, ldq=80), dict(form=1, n=48, ldq=48), dict(form=2, n=48, ldq=48),
                 dict(x=O), dict(delta=O, ldd=64), dict(res=O, ldr=64), dict(y=O, ldy=64), dict(w=O), dict(sc=O),
-                dict(form=1, sc=ctypes.c_void_p(0x1004)), dict(form=2, q=O, sc=None), dict(type=1, x=O)):
+                dict(form=1, sc=ctypes.c_void_p(0x1004)), dict(form=2, q=O, sc=None), dict(type=1, x=O),
+                dict(rows=2 ** 26), dict(rows=2 ** 22, n=5000, ldx=5000, ldq=5000)):
         assert rc(**bad) == 1, bad
         assert b"lk_norm_q8" in lk_host.load().lk_last_error(), bad
     assert rc(rows=0, x=None, w=None, q=None, sc=None) == 0
@@ -38,7 +39,8 @@ def test_gemm_c_refusals(lk_host):
     for bad in (dict(type=3), dict(M=-1), dict(N=-1), dict(K=0), dict(K=131072, ldx=131072, ldw=131072), dict(x=None), dict(sx=None),
                 dict(w=None), dict(sw=None), dict(out=None), dict(ldx=48), dict(ldx=72), dict(ldw=48), dict(ldw=65), dict(ldo=3),
                 dict(res=P, ldr=3), dict(ldx=8388624), dict(ldw=8388624), dict(x=ctypes.c_void_p(0x1008)),
-                dict(w=ctypes.c_void_p(0x1008)), dict(sx=O), dict(sw=O), dict(out=O), dict(res=O, ldr=4)):
+                dict(w=ctypes.c_void_p(0x1008)), dict(sx=O), dict(sw=O), dict(out=O), dict(res=O, ldr=4),
+                dict(M=2 ** 31 - 1), dict(N=2 ** 31 - 1, ldo=2 ** 31 - 1), dict(M=2 ** 31 - 1, N=2 ** 31 - 1, ldo=2 ** 31 - 1)):
         assert rc(**bad) == 1, bad
         assert b"lk_gemm_i8" in lk_host.load().lk_last_error(), bad
     assert rc(M=0, x=None) == 0 and rc(N=0, w=None) == 0
@@ -67,6 +69,19 @@ def test_mirror_refusals(lk_host):
                      (dict(x=torch.zeros(3, 50, dtype=torch.int8)), "storage"), (dict(w=b.t().contiguous().t()), "contiguous")):
         with pytest.raises(ValueError, match=word):
             lk.gemm_i8(**{**dict(x=a, sx=sa, w=b, sw=sb, out=o), **kw})
+
+
+def test_mirror_refuses_what_an_int_cannot_count(lk_host):
+    """Strides and counts past 2^31 - 1, which the C entry points take as int (meta tensors:
+    shapes without memory)."""
+    lk, big = lk_host, 2 ** 31
+    m = lambda shape, dt=torch.float32, stride=None: torch.empty_strided(  # noqa: E731
+        shape, stride or (shape[-1], 1)[-len(shape):], dtype=dt, device="meta")
+    for x, q, sc in ((m((2, 8), stride=(big, 1)), m((2, 8), torch.int8), m((2,))), (m((big, 8)), m((big, 8), torch.int8), m((big,)))):
+        with pytest.raises(ValueError, match="beyond"):
+            lk.norm_q8(x, m((8,)), q, sc)
+    with pytest.raises(ValueError, match="beyond"):
+        lk.gemm_i8(m((2, 16), torch.int8, (2 * big, 1)), m((2,)), m((3, 16), torch.int8), m((3,)), m((2, 3)))
 
 
 def _desc(lk, **kw):
