@@ -253,59 +253,70 @@ __device__ __forceinline__ void lk_moe_bias(const LkMoeArgs & a, float (&b)[NL])
 #pragma unroll
     for (int i = 0; i < NL; ++i) b[i] = a.bias ? a.bias[64 * i + lane < a.E ? 64 * i + lane : 0] : 0.0f;
 }
-// The token's choice j and its weight in lane j < k; the other lanes hold -1.
-template <int NL>
-__device__ __forceinline__ void lk_moe_choose(const LkMoeArgs & a, const float (&l)[NL], const float (&b)[NL], int & id, float & w) {
+// Of TW tokens, one after the other in every step, the choice j and its weight in lane j < k; the
+// other lanes hold -1.
+template <int NL, int TW>
+__device__ __forceinline__ void lk_moe_choose(const LkMoeArgs & a, const float (&l)[TW][NL], const float (&b)[NL], int (&id)[TW], float (&w)[TW]) {
     const int lane = threadIdx.x & 63;
-    uint32_t key[NL];
-    float m = 0.0f, zi = 1.0f;
-    if (a.score == LK_MOE_SOFTMAX) {
-        m = l[0];
-#pragma unroll
-        for (int i = 1; i < NL; ++i) m = fmaxf(m, l[i]);
-        m = lk_xrow_max(lk_row_max16(m));                // lanes past the experts repeat expert 0
-        float z = 0.0f;
-#pragma unroll
-        for (int i = 0; i < NL; ++i) z += 64 * i + lane < a.E ? lk_moe_expn(l[i] - m) + (l[i] - l[i]) : 0.0f;
-        zi = 1.0f / lk_wave_sum(z);
-    }
-    auto score = [&](float v) {                          // v - v: 0, or NaN for what is not finite
-        return a.score == LK_MOE_SOFTMAX ? (lk_moe_expn(v - m) + (v - v)) * zi : v == v ? lk_moe_sigmoid(v) : v;
+    uint32_t key[TW][NL];
+    float m[TW], zi[TW], mine[TW];                       // mine: lane j: the logit of choice j
+    auto score = [&](int t, float v) {                   // v - v: 0, or NaN for what is not finite
+        return a.score == LK_MOE_SOFTMAX ? (lk_moe_expn(v - m[t]) + (v - v)) * zi[t] : v == v ? lk_moe_sigmoid(v) : v;
     };
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-        const float r = a.bias ? score(l[i]) + b[i] : l[i];
-        key[i] = 64 * i + lane < a.E ? lk_moe_key(r) : 0;
-    }
-    float mine = 0.0f;                                   // lane j: the logit of choice j
-    id = -1;
-    for (int j = 0; j < a.k; ++j) {
-        uint32_t best = key[0];
+    for (int t = 0; t < TW; ++t) {
+        m[t] = 0.0f, zi[t] = 1.0f, mine[t] = 0.0f, id[t] = -1;
+        if (a.score == LK_MOE_SOFTMAX) {
+            m[t] = l[t][0];
 #pragma unroll
-        for (int i = 1; i < NL; ++i) best = lk_umax(best, key[i]);
-        best = lk_moe_top(best);
-        int e = 0;
-        float v = 0.0f;
+            for (int i = 1; i < NL; ++i) m[t] = fmaxf(m[t], l[t][i]);
+            m[t] = lk_xrow_max(lk_row_max16(m[t]));      // lanes past the experts repeat expert 0
+            float z = 0.0f;
 #pragma unroll
-        for (int i = NL - 1; i >= 0; --i) {
-            const uint64_t at = __ballot(key[i] == best);
-            if (NL == 1 || at) {                         // in one register at least: k <= E
-                e = 64 * i + __builtin_ctzll(at);
-                v = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, l[i]), e & 63));
-            }
+            for (int i = 0; i < NL; ++i) z += 64 * i + lane < a.E ? lk_moe_expn(l[t][i] - m[t]) + (l[t][i] - l[t][i]) : 0.0f;
+            zi[t] = 1.0f / lk_wave_sum(z);
         }
 #pragma unroll
-        for (int i = 0; i < NL; ++i) key[i] = 64 * i + lane == e ? 0 : key[i];
-        mine = lane == j ? v : mine;
-        id = lane == j ? e : id;
+        for (int i = 0; i < NL; ++i) {
+            const float r = a.bias ? score(t, l[t][i]) + b[i] : l[t][i];
+            key[t][i] = 64 * i + lane < a.E ? lk_moe_key(r) : 0;
+        }
     }
-    w = lane < a.k ? score(mine) : 0.0f;
-    if (a.renorm) w = w / (lk_row_sum16(w) + 1e-20f);    // k <= 8: the first row of 16 lanes
-    w *= a.scale;
+    for (int j = 0; j < a.k; ++j)
+#pragma unroll
+        for (int t = 0; t < TW; ++t) {
+            uint32_t best = key[t][0];
+#pragma unroll
+            for (int i = 1; i < NL; ++i) best = lk_umax(best, key[t][i]);
+            best = lk_moe_top(best);
+            int e = 0;
+            float v = 0.0f;
+#pragma unroll
+            for (int i = NL - 1; i >= 0; --i) {
+                const uint64_t at = __ballot(key[t][i] == best);
+                if (NL == 1 || at) {                     // in one register at least: k <= E
+                    e = 64 * i + __builtin_ctzll(at);
+                    v = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, l[t][i]), e & 63));
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < NL; ++i) key[t][i] = 64 * i + lane == e ? 0 : key[t][i];
+            mine[t] = lane == j ? v : mine[t];
+            id[t] = lane == j ? e : id[t];
+        }
+#pragma unroll
+    for (int t = 0; t < TW; ++t) {
+        w[t] = lane < a.k ? score(t, mine[t]) : 0.0f;
+        if (a.renorm) w[t] = w[t] / (lk_row_sum16(w[t]) + 1e-20f);         // k <= 8: the first row of 16 lanes
+        w[t] *= a.scale;
+    }
 }
 // More than LK_MOE_FEW tokens: one workgroup of 16 waves chooses for all of them and
-// sorts the assignments by expert.
-template <int NL>
+// sorts the assignments by expert: TW tokens a wave, whose steps fill each other's waits, and
+// several lanes to an expert's rank among the counts (64 tokens 9.0 us, 19 tokens 5.6; a token, an
+// expert and a count at a time 11.1 and 6.1; 64 tokens: 1 us of it the logits' way, 4 the choice, the
+// instructions of 16 tokens on each SIMD).
+template <int NL, int TW>
 __global__ void __launch_bounds__(1024)
 lk_k_moe_route(const LkMoeArgs a) {
     __shared__ int ids[LK_MOE_MAX_TOKENS * LK_MOE_MAX_TOP_K], cnt[LK_MOE_MAX_EXPERTS], slot[LK_MOE_MAX_EXPERTS];
@@ -313,46 +324,54 @@ lk_k_moe_route(const LkMoeArgs a) {
     LkMoeTab & tab = *(LkMoeTab *) a.tab;
     if (tid < LK_MOE_MAX_EXPERTS) cnt[tid] = 0;
     __syncthreads();
-    constexpr int TW = LK_MOE_MAX_TOKENS / 16;           // tokens of a wave, their logits asked for together
     float l[TW][NL], b[NL];
 #pragma unroll
     for (int i = 0; i < TW; ++i) lk_moe_logits<NL>(a, wv + 16 * i < a.T ? wv + 16 * i : a.T - 1, l[i]);
     lk_moe_bias<NL>(a, b);
+    int id[TW];
+    float w[TW];
+    lk_moe_choose<NL, TW>(a, l, b, id, w);               // past the last token: the last again, not used
 #pragma unroll
     for (int i = 0; i < TW; ++i) {
         const int t = wv + 16 * i;
-        if (t >= a.T) break;
-        int id;
-        float w;
-        lk_moe_choose<NL>(a, l[i], b, id, w);
-        if (id >= 0) {
-            const int i = t * a.k + lane;
-            ids[i] = id;
-            a.wts[i] = w;
-            if (a.ids_out) a.ids_out[i] = id;
-            if (a.wts_out) a.wts_out[i] = w;
-            atomicAdd(&cnt[id], 1);                      // counts have no order
+        if (t < a.T && id[i] >= 0) {
+            const int at = t * a.k + lane;
+            ids[at] = id[i];
+            a.wts[at] = w[i];
+            if (a.ids_out) a.ids_out[at] = id[i];
+            if (a.wts_out) a.wts_out[at] = w[i];
+            atomicAdd(&cnt[id[i]], 1);                   // counts have no order
         }
     }
     __syncthreads();
-    if (tid < a.E) {
-        const int c = cnt[tid];
+    constexpr int NS = NL == 1 ? 16 : 4;                 // lanes that share an expert's comparisons
+    {
+        const int e = tid / NS, c = e < a.E ? cnt[e] : 0;
         int s = 0;
-#pragma unroll 8
-        for (int e = 0; e < a.E; ++e) s += cnt[e] > c || (cnt[e] == c && e < tid);
-        slot[tid] = s;
-        tab.slot[s].e = tid;
-        tab.slot[s].n = c;
+#pragma unroll 4
+        for (int o = tid % NS; o < a.E; o += NS) s += cnt[o] > c || (cnt[o] == c && o < e);
+#pragma unroll
+        for (int x = 1; x < NS; x *= 2) s += __shfl_xor(s, x);
+        if (e < a.E && tid % NS == 0) {
+            slot[e] = s;
+            tab.slot[s].e = e;
+            tab.slot[s].n = c;
+        }
     }
     __syncthreads();
+    constexpr int NC = LK_MOE_MAX_TOKENS * LK_MOE_MAX_TOP_K / 64;
+    int mine[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) mine[i] = 64 * i + lane < na ? ids[64 * i + lane] : -1;
     for (int e = wv; e < a.E; e += 16) {                 // a wave per expert keeps the order
         if (cnt[e] == 0) continue;
         int32_t * list = tab.list[slot[e]];
         int n = 0;
-        for (int i0 = 0; i0 < na; i0 += 64) {
-            const bool hit = i0 + lane < na && ids[i0 + lane] == e;
-            const uint64_t b = __ballot(hit);
-            if (hit) list[n + __popcll(b & ((1ull << lane) - 1))] = i0 + lane;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            if (64 * i >= na) break;
+            const uint64_t b = __ballot(mine[i] == e);
+            if (mine[i] == e) list[n + __popcll(b & ((1ull << lane) - 1))] = 64 * i + lane;
             n += __popcll(b);
         }
     }
@@ -549,18 +568,20 @@ lk_k_moe_up_few(const LkMoeArgs a) {
     int mine = -1;
     if (a.T == 1 || wv < a.T) {                          // one token: every wave for itself
         const int t = a.T == 1 ? 0 : wv;
-        float l[NL], b[NL], w;
-        lk_moe_logits<NL>(a, t, l);
+        int id[1];
+        float l[1][NL], b[NL], w[1];
+        lk_moe_logits<NL>(a, t, l[0]);
         lk_moe_bias<NL>(a, b);
-        lk_moe_choose<NL>(a, l, b, mine, w);
+        lk_moe_choose<NL, 1>(a, l, b, id, w);
+        mine = id[0];
         if (mine >= 0) {
             if (a.T > 1) ids[t * a.k + lane] = mine;
             if (tells && (a.T > 1 || wv == 0)) {
                 const int i = t * a.k + lane;
                 a.ids[i] = mine;
-                a.wts[i] = w;
+                a.wts[i] = w[0];
                 if (a.ids_out) a.ids_out[i] = mine;
-                if (a.wts_out) a.wts_out[i] = w;
+                if (a.wts_out) a.wts_out[i] = w[0];
             }
         }
     }
@@ -991,12 +1012,18 @@ static void lk_moe_go(const LkMoeArgs & a, hipStream_t st) {
     const int nE = (a.E + 3) / 4, na = a.T * a.k, slots = na < a.E ? na : a.E;
     hipLaunchKernelGGL((lk_k_moe_router<TYPE, NP>), dim3(nE + (a.hidden / 8 + LK_MOE_THREADS - 1) / LK_MOE_THREADS, (a.T + 3) / 4),
                        dim3(LK_MOE_THREADS), 0, st, a, nE);
+    auto route = [&](auto regs) {
+        constexpr int NL = decltype(regs)::value;
+        if (a.T <= 16)      hipLaunchKernelGGL((lk_k_moe_route<NL, 1>), dim3(1), dim3(1024), 0, st, a);
+        else if (a.T <= 32) hipLaunchKernelGGL((lk_k_moe_route<NL, 2>), dim3(1), dim3(1024), 0, st, a);
+        else                hipLaunchKernelGGL((lk_k_moe_route<NL, 4>), dim3(1), dim3(1024), 0, st, a);
+    };
     auto go = [&](auto regs) {                           // registers of 64 experts a choosing wave holds
         constexpr int NL = decltype(regs)::value;
         if (a.T <= LK_MOE_FEW)
             hipLaunchKernelGGL((lk_k_moe_up_few<NP, NL>), dim3(a.ffn / 32, na), dim3(64 * LK_MOE_NW), 0, st, a);
         else
-            hipLaunchKernelGGL((lk_k_moe_route<NL>), dim3(1), dim3(1024), 0, st, a);
+            route(LkInt<NL>{});
     };
     if (a.E <= 64) go(LkInt<1>{});
     else           go(LkInt<LK_MOE_MAX_EXPERTS / 64>{});
