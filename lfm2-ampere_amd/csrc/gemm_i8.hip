@@ -96,9 +96,15 @@ lk_k_gemm_i8_few(const LkI8Args a) {
 
 // ---- tiles ------------------------------------------------------------------------
 // A wave covers TM x TN tiles of v_mfma_i32_32x32x32_i8 (TM along the weight rows, TN
-// along the tokens), WM x WN of them a workgroup, or WK times as many
-// that share K: each takes its part of every stage.  K in stages of KC bytes, a ring of NB of
-// them in LDS, filled by LDS DMA.
+// along the tokens), WM x WN of them a workgroup, or WK times as many that share K: each takes
+// its part of every stage, and integer sums have no order.  K in stages of KC bytes, a ring of
+// NB of them in LDS, filled by LDS DMA.
+// What bounds it.  Large: the matrix instructions at the clock that the power leaves: 8192^3 in
+// 446 to 500 us, 2200 to 2470 TOPS, where MFMAs alone, without a load, reach 2630 and the
+// library's int8 product 2090; 4 waves of 4 x 4 tiles, which read less from LDS, 470, a ring of
+// 4 stages of 64 bytes 467 to 498.  4096 x 8192 x 2048, two rounds of tiles: 74 us (1860), of
+// which a tile's first loads and its outputs, 16 MB a round, take about 6.  Small: the latency of
+// the ring's start, of a stage and of the launch (333 x 2048 x 2048: 6.5 us).
 template <int TM_, int TN_, int WM_, int WN_, int WK_, int KC_, int NB_, int OCC_>
 struct LkI8Shape {
     static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, WK = WK_, KC = KC_, NB = NB_, OCC = OCC_;   // OCC: waves per SIMD

@@ -614,6 +614,9 @@ lk_k_moe_up_few(const LkMoeArgs a) {
 // assignments cost a wave about 13 vector operations for 16 rows of a block and of one
 // assignment 20 as dots, so that they pay from two on: 19 tokens 61 us with dots up to two,
 // 58 up to one, 62 without; 64 tokens (four an expert) 97, 92, 92; dots alone 65 and 112.
+// Bound by memory: 64 tokens at 64 experts read 226 MB (gate, up) in 49 us and 113 MB in 26, 4.9
+// TB/s less the launch (a 1 GiB copy 5.15), and not a byte twice (counters: 209 and 108 MB; the rest
+// is in the cache).
 template <int NP>
 struct LkMoeShare {
     static constexpr int Z = 8 * LkMoeRec<NP>::PIECES;   // pieces of a step's digits
