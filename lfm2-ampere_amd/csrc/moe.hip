@@ -172,24 +172,37 @@ lk_k_moe_router(const LkMoeArgs a, int nE) {
         const int e = blockIdx.x * 4 + wv;
         if (e >= a.E) return;
         const float * r = a.router + (size_t) e * H;
-        float s[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
-        for (int i = lane * 8; i < H; i += 512) {        // H is a multiple of 32: whole pieces
-            float w[8];
-            lk_load<8>(r + i, w);
+        // H is a multiple of 32: whole pieces of 8.  U pieces of the row and of NT tokens are asked
+        // for before the first is used: a piece at a time each took a round trip
+        auto go = [&](auto tokens, auto pieces) {
+            constexpr int NT = decltype(tokens)::value, U = decltype(pieces)::value;
+            float s[NT] = {};
+            for (int i0 = lane * 8; i0 < H; i0 += 512 * U) {
+                float w[U][8], v[U][NT][8];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int t = t0 + k < a.T ? t0 + k : a.T - 1;
-                float v[8];
-                lk_load<8>(x + (size_t) t * a.ldx + i, v);
+                for (int u = 0; u < U; ++u) {
+                    const int i = i0 + 512 * u < H ? i0 + 512 * u : i0;                          // past the end: not used
+                    lk_load<8>(r + i, w[u]);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) s[k] = __builtin_fmaf(w[j], v[j], s[k]);
+                    for (int k = 0; k < NT; ++k) lk_load<8>(x + (size_t) (t0 + k < a.T ? t0 + k : a.T - 1) * a.ldx + i, v[u][k]);
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (i0 + 512 * u >= H) break;
+#pragma unroll
+                    for (int k = 0; k < NT; ++k)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) s[k] = __builtin_fmaf(w[u][j], v[u][k][j], s[k]);
+                }
             }
-        }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            s[k] = lk_wave_sum(s[k]);
-            if (lane == 0 && t0 + k < a.T) a.logits[(size_t) (t0 + k) * a.E + e] = s[k];
-        }
+            for (int k = 0; k < NT; ++k) {
+                s[k] = lk_wave_sum(s[k]);
+                if (lane == 0 && t0 + k < a.T) a.logits[(size_t) (t0 + k) * a.E + e] = s[k];
+            }
+        };
+        if (a.T == 1) go(LkInt<1>{}, LkInt<4>{});
+        else          go(LkInt<4>{}, LkInt<2>{});
         return;
     }
     const int u = (blockIdx.x - nE) * LK_MOE_THREADS + threadIdx.x, b = u >> 2, g = u & 3, bpr = H / 32;
