@@ -291,3 +291,17 @@ def test_a_token_does_not_depend_on_the_others(lk, t):
     for T in (32, 16, 9):
         for at in range(0, 64 - T + 1, T):
             assert torch.equal(_run(lk, layer, x[at:at + T], hidden, dt, k)[0], whole[at:at + T]), (T, at)
+
+
+@pytest.mark.parametrize("T", [1, 7, 9, 64])
+@pytest.mark.parametrize("hidden,ffn", [(32768, 32), (32, 32768)])
+def test_longest_rows(lk, hidden, ffn, T):
+    """The largest dimensions, in both kinds of launch."""
+    dt = TYPES["f32"] if T % 2 else TYPES["bf16"]
+    L = _layer(T, 3, hidden, ffn, bias=True)
+    x = _x(50 + T, T, hidden, dt)
+    note(f"moe hidden={hidden} ffn={ffn} T={T}")
+    out, ids, _ = _run(lk, _make(lk, L, 2), x, hidden, dt, 2)
+    want, ids1, _ = moe_ref(x, k=2, score="sigmoid", **L)
+    assert torch.equal(ids.long(), ids1)
+    _close(out, want, dt, (hidden, ffn, T))
