@@ -868,7 +868,11 @@ __device__ __forceinline__ void lk_moe_down_many(const LkMoeArgs & a, int e, con
             a.y[(size_t) as[t] * H + r0 + lane] = sh.part[0][t][lane] + sh.part[1][t][lane];
 }
 
-// grid (row tiles, slots)
+// grid (row tiles, slots, groups of TG assignments that an expert may have).  An expert of many
+// assignments has a workgroup for each group, which finds the weights in the cache: 64 tokens, all 8
+// experts of 2048 x 768 chosen, 58 us, fp32 rows 74, where the same workgroup took group after group
+// in 112 and 162; 64 experts, 4 of 2048 x 1536 chosen, 98.5 and 112 for 99.2 and 141: the workgroups of
+// groups that an expert has not got cost less than they save.
 template <int NP, bool UP>
 __global__ void __launch_bounds__(LK_MOE_THREADS, 4)
 lk_k_moe_many(const LkMoeArgs a) {
@@ -877,17 +881,13 @@ lk_k_moe_many(const LkMoeArgs a) {
     // written by the launch before: read as constants, by scalar loads
     typedef const __attribute__((address_space(4))) LkMoeTab Tab;
     Tab & tab = *(Tab *) (uintptr_t) a.tab;
-    const int slot = blockIdx.y, e = tab.slot[slot].e, n = tab.slot[slot].n;
-#pragma unroll 1
-    for (int at = 0; at < n; at += TG) {
-        if (at) __syncthreads();                         // part has been read
-        const int left = n - at < TG ? n - at : TG;
-        int as[TG];
+    const int slot = blockIdx.y, at = TG * blockIdx.z, e = tab.slot[slot].e, left = tab.slot[slot].n - at, n = left < TG ? left : TG;
+    if (n <= 0) return;
+    int as[TG];
 #pragma unroll
-        for (int t = 0; t < TG; ++t) as[t] = tab.list[slot][at + (t < left ? t : 0)];
-        if constexpr (UP) lk_moe_up_many<NP>(a, e, as, left, sh);
-        else              lk_moe_down_many<NP>(a, e, as, left, sh);
-    }
+    for (int t = 0; t < TG; ++t) as[t] = tab.list[slot][at + (t < n ? t : 0)];
+    if constexpr (UP) lk_moe_up_many<NP>(a, e, as, n, sh);
+    else              lk_moe_down_many<NP>(a, e, as, n, sh);
 }
 
 // Up to LK_MOE_FEW tokens: a workgroup of 16 waves has 8 rows of every expert that was
@@ -1047,8 +1047,9 @@ static void lk_moe_go(const LkMoeArgs & a, hipStream_t st) {
         hipLaunchKernelGGL((lk_k_moe_down_few<TYPE, NP>), dim3(a.hidden / 8), dim3(64 * LK_MOE_NWF), 0, st, a);
         return;
     }
-    hipLaunchKernelGGL((lk_k_moe_many<NP, true>), dim3(a.ffn / 32, slots), dim3(LK_MOE_THREADS), 0, st, a);
-    hipLaunchKernelGGL((lk_k_moe_many<NP, false>), dim3((a.hidden + 63) / 64, slots), dim3(LK_MOE_THREADS), 0, st, a);
+    const int groups = (a.T - 1) / LkMoeShare<NP>::TG + 1;
+    hipLaunchKernelGGL((lk_k_moe_many<NP, true>), dim3(a.ffn / 32, slots, groups), dim3(LK_MOE_THREADS), 0, st, a);
+    hipLaunchKernelGGL((lk_k_moe_many<NP, false>), dim3((a.hidden + 63) / 64, slots, groups), dim3(LK_MOE_THREADS), 0, st, a);
     hipLaunchKernelGGL((lk_k_moe_sum<TYPE>), dim3((a.hidden / 4 + LK_MOE_THREADS - 1) / LK_MOE_THREADS, a.T), dim3(LK_MOE_THREADS), 0, st, a);
 }
 
