@@ -100,11 +100,11 @@ lk_k_gemm_i8_few(const LkI8Args a) {
 // its part of every stage, and integer sums have no order.  K in stages of KC bytes, a ring of
 // NB of them in LDS, filled by LDS DMA.
 // What bounds it.  Large: the matrix instructions at the clock that the power leaves: 8192^3 in
-// 446 to 500 us, 2200 to 2470 TOPS, where MFMAs alone, without a load, reach 2630 and the
+// 440 to 490 us, 2240 to 2500 TOPS, where MFMAs alone, without a load, reach 2630 and the
 // library's int8 product 2090; 4 waves of 4 x 4 tiles, which read less from LDS, 470, a ring of
-// 4 stages of 64 bytes 467 to 498.  4096 x 8192 x 2048, two rounds of tiles: 74 us (1860), of
-// which a tile's first loads and its outputs, 16 MB a round, take about 6.  Small: the latency of
-// the ring's start, of a stage and of the launch (333 x 2048 x 2048: 6.5 us).
+// 4 stages of 64 bytes 467 to 498.  4096 x 8192 x 2048, two rounds of tiles: 73 us (1880), of
+// which the outputs, 34 MB of every unit's at once, take 5.7 a round (6 TB/s).  Small: the latency
+// of the ring's start, of a stage and of the launch (333 x 2048 x 2048: 6.4 us).
 template <int TM_, int TN_, int WM_, int WN_, int WK_, int KC_, int NB_, int OCC_>
 struct LkI8Shape {
     static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, WK = WK_, KC = KC_, NB = NB_, OCC = OCC_;   // OCC: waves per SIMD
@@ -113,9 +113,15 @@ struct LkI8Shape {
     static constexpr int NA = BM * PC / 64, NI = (BM + BN) * PC / 64, PW = NI / NW;
     static_assert(NI % NW == 0 && BM * PC % 64 == 0 && BN * PC % 64 == 0, "whole DMA instructions, the same for every wave");
     static_assert((NB - 2) * PW < 64, "vmcnt range");
-    // the ring, or the parts of K and the outputs on their way (below) where those are more
-    static constexpr int PARTS = WM * WN * (WK - 1) * TM * TN * 4096, OUTS = PARTS + WM * WN * 32 * (32 * TM + 4) * 4;
+    // Rings of two stages go on from tile to tile (MORE): the outputs leave by way of the last
+    // stage's buffer while the next tile's first stage is in the other (a workgroup a tile, us:
+    // 8192 x 8192 x 2048 146, so 136; 4096 x 8192 x 2048 77 and 73; 8192^3 462 and 448).
+    static constexpr bool MORE = NB == 2;
+    static constexpr int RS = TM < 2 ? TM : 2, STG = 32 * 32 * RS * 4;       // MFMA tiles of outputs on their way at a time; bytes of a wave
+    // the ring, or the parts of K and the outputs where those are more
+    static constexpr int PARTS = WM * WN * (WK - 1) * TM * TN * 4096, OUTS = PARTS + WM * WN * STG;
     static constexpr int LDS = NB * BYTES > OUTS ? NB * BYTES : OUTS;
+    static_assert(!MORE || (WK == 1 && NW * STG <= BYTES), "the outputs' room");
     static_assert(KC % (32 * WK) == 0 && 16 % PC == 0, "whole steps; a row's pieces divide the 16 slots of all banks");
 };
 // 16-byte slot of piece p of a row of n pieces: XOR-permuted so that the same piece
@@ -127,6 +133,7 @@ __global__ void __launch_bounds__(64 * SH::NW, SH::OCC)
 lk_k_gemm_i8(const LkI8Args a) {
     typedef typename LkElem<TYPE>::type T;
     constexpr int TM = SH::TM, TN = SH::TN, KC = SH::KC, NB = SH::NB, NW = SH::NW, PC = SH::PC, PW = SH::PW;
+    constexpr bool MORE = SH::MORE;
     constexpr int WMN = SH::WM * SH::WN, NQ = KC / 32 / SH::WK;        // a wave's steps of a stage
     __shared__ __attribute__((aligned(16))) uint8_t stg[SH::LDS];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -135,43 +142,48 @@ lk_k_gemm_i8(const LkI8Args a) {
     // row tiles first, so that the tiles an XCD works on at a time form a patch
     // whose operands its L2 holds once.
     const int nrt = (a.N - 1) / SH::BM + 1, ntt = (a.M - 1) / SH::BN + 1, ntile = nrt * ntt;
-    const int id = blockIdx.x, x8 = id & 7, rem = ntile & 7;
-    const int L = x8 * (ntile >> 3) + (x8 < rem ? x8 : rem) + (id >> 3);
-    const int gr = L / (8 * ntt), gw = nrt - 8 * gr < 8 ? nrt - 8 * gr : 8, li = L - gr * 8 * ntt;
-    const int row0 = (8 * gr + li % gw) * SH::BM, tok0 = (li / gw) * SH::BN;
+    auto place = [&](int id, int & row0, int & tok0) {
+        const int x8 = id & 7, rem = ntile & 7;
+        const int L = x8 * (ntile >> 3) + (x8 < rem ? x8 : rem) + (id >> 3);
+        const int gr = L / (8 * ntt), gw = nrt - 8 * gr < 8 ? nrt - 8 * gr : 8, li = L - gr * 8 * ntt;
+        row0 = (8 * gr + li % gw) * SH::BM;
+        tok0 = (li / gw) * SH::BN;
+    };
+    int row0, tok0;
+    place(blockIdx.x, row0, tok0);
     const int kw = w / WMN;                              // the wave's part of every stage
     const int wr = (w % SH::WM) * 32 * TM, wt = (w % WMN / SH::WM) * 32 * TN;
     const int lm = lane & 31, h = lane >> 5;
     const int K = a.K, nst = (K + KC - 1) / KC;
 
     // DMA instruction i of this wave: slots 64 * (i * NW + w) + lane of a stage
-    uint32_t roff[PW], pc[PW];
+    uint32_t roff[PW];
+    const uint32_t pc = (uint32_t) (lk_i8_slot(PC, (64 * w + lane) / PC, lane % PC) % PC * 16);   // the same for all i
+    static_assert(4 * NW % PC == 0 && SH::BM % 16 == 0, "a permutation that the wave's instructions share");
+    const int8_t * wb, * xb;
+    auto aim = [&](int row0, int tok0) {                 // at a tile
 #pragma unroll
-    for (int i = 0; i < PW; ++i) {
-        const int j = i * NW + w;
-        const bool isa = j < SH::NA;
-        const int slot = 64 * (isa ? j : j - SH::NA) + lane, r = slot / PC;
-        pc[i] = (uint32_t) (lk_i8_slot(PC, r, slot % PC) % PC * 16);
-        const int lim = isa ? a.N - 1 - row0 : a.M - 1 - tok0;
-        roff[i] = (uint32_t) (r < lim ? r : lim) * (uint32_t) (isa ? a.ldw : a.ldx);       // clamped: in bounds
-    }
-    const int8_t * wb = a.w + (size_t) row0 * a.ldw, * xb = a.x + (size_t) tok0 * a.ldx;
+        for (int i = 0; i < PW; ++i) {
+            const int j = i * NW + w;
+            const bool isa = j < SH::NA;
+            const int r = (64 * (isa ? j : j - SH::NA) + lane) / PC;
+            const int lim = isa ? a.N - 1 - row0 : a.M - 1 - tok0;
+            roff[i] = (uint32_t) (r < lim ? r : lim) * (uint32_t) (isa ? a.ldw : a.ldx);   // clamped: in bounds
+        }
+        wb = a.w + (size_t) row0 * a.ldw;
+        xb = a.x + (size_t) tok0 * a.ldx;
+    };
     const uint32_t lds0 = lk_lds_addr(stg);
-    auto fetch = [&](int s, int i) {                     // pieces past the row: its first piece instead
+    int sb = 0;                                          // the ring's place of the tile's stage 0
+    auto fetch = [&](int s, int at, int i) {             // stage s into place at; pieces past the row: its first piece instead
         const int j = i * NW + w;
-        const uint32_t k = (uint32_t) (s * KC) + pc[i];
-        lk_dma16c_so(j < SH::NA ? wb : xb, roff[i] + (k < (uint32_t) K ? k : 0u), lds0 + (uint32_t) (s % NB * SH::BYTES + 1024 * j));
+        const uint32_t k = (uint32_t) (s * KC) + pc;
+        lk_dma16c_so(j < SH::NA ? wb : xb, roff[i] + (k < (uint32_t) K ? k : 0u), lds0 + (uint32_t) (at % NB * SH::BYTES + 1024 * j));
     };
     lk_i16v acc[TM][TN];
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int j = 0; j < TN; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
     lk_i4 av[2][TM], bv[2][TN];
     auto read = [&](int s, int q, int u, int k) {        // operand k of step q of stage s
-        const uint8_t * S = stg + s % NB * SH::BYTES;
+        const uint8_t * S = stg + (s + sb) % NB * SH::BYTES;
         if (k < TM) av[u][k] = *(const lk_i4 *) (S + lk_i8_slot(PC, wr + 32 * k + lm, 2 * (kw * NQ + q) + h) * 16);
         else bv[u][k - TM] = *(const lk_i4 *) (S + SH::BM * KC + lk_i8_slot(PC, wt + 32 * (k - TM) + lm, 2 * (kw * NQ + q) + h) * 16);
     };
@@ -209,7 +221,7 @@ lk_k_gemm_i8(const LkI8Args a) {
                 const int g = q * TM + i;
                 if (g < ND)
 #pragma unroll
-                    for (int k = PW * g / ND; k < PW * (g + 1) / ND; ++k) fetch(s + NB - 1, k);
+                    for (int k = PW * g / ND; k < PW * (g + 1) / ND; ++k) fetch(MORE && last ? 0 : s + NB - 1, s + sb + NB - 1, k);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(av[u][i], bv[u][j], acc[i][j], 0, 0, 0);
@@ -217,97 +229,123 @@ lk_k_gemm_i8(const LkI8Args a) {
             }
         }
     };
+    aim(row0, tok0);
 #pragma unroll
     for (int s = 0; s < NB - 1; ++s)
 #pragma unroll
-        for (int i = 0; i < PW; ++i) fetch(s, i);        // those past the end: the rows' first pieces, not used
+        for (int i = 0; i < PW; ++i) fetch(s, s, i);     // those past the end: the rows' first pieces, not used
     meet();
-#pragma unroll
-    for (int k = 0; k < TM + TN; ++k) read(0, 0, 0, k);
-#pragma unroll 1
-    for (int s = 0; s + 1 < nst; ++s) stage(s, false);
-    stage(nst - 1, true);
-    lk_wait_vm<0>();                                     // the DMAs past the end, before LDS is used otherwise
-    // Outputs by way of LDS (the ring is free now), 32 tokens of the wave at a time: a
-    // lane has token lm and rows 8 * e4 + 4 * h .. +3 of every MFMA tile, 8 bytes of 32
-    // output rows per store; from LDS it takes 8 consecutive rows of one token, whole
-    // runs of 64 * TM bytes (bf16).  The rows are 16 bytes longer in LDS, so that the 16-byte
-    // writes of 16 tokens lie in different banks.
-    constexpr int RW = 32 * TM, LS = RW + 4;             // rows of the wave's tile; floats from token to token
-    __syncthreads();                                     // every wave has read its last operands
-    if constexpr (SH::WK > 1) {                          // the parts of K meet: integer sums have no order
-        lk_i16v * pt = (lk_i16v *) stg;
-        if (kw > 0) {
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int j = 0; j < TN; ++j) pt[((w - WMN) * TM * TN + i * TN + j) * 64 + lane] = acc[i][j];
-        }
-        __syncthreads();
-        if (kw > 0) return;
-#pragma unroll
-        for (int k = 1; k < SH::WK; ++k)
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int j = 0; j < TN; ++j) acc[i][j] += pt[((k * WMN + w - WMN) * TM * TN + i * TN + j) * 64 + lane];
-    }
-    // (behind the parts of K, which other waves may still be reading)
-    float * st = (float *) (stg + SH::PARTS) + (w % WMN) * 32 * LS;
-    const T * res = (const T *) a.res;
-    T * out = (T *) a.out;
-    float sw[TM][4][4];
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int e4 = 0; e4 < 4; ++e4) {
-            const int r = row0 + wr + 32 * i + 8 * e4 + 4 * h;
-            if (r + 4 <= a.N) lk_load<4>(a.sw + r, sw[i][e4]);
-            else
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sw[i][e4][e] = r + e < a.N ? a.sw[r + e] : 0.0f;
-        }
-    constexpr int LT = RW / 8, TP = 64 / LT;             // lanes a token, tokens a step
-    const int r8 = (lane % LT) * 8, r = row0 + wr + r8;
-#pragma unroll
-    for (int j = 0; j < TN; ++j) {
-        const int t0 = tok0 + wt + 32 * j;               // wave-uniform
-        const float sx = a.sx[t0 + lm < a.M ? t0 + lm : a.M - 1];
+    for (int id = blockIdx.x;;) {
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
-            for (int e4 = 0; e4 < 4; ++e4) {
-                lk_f4 v;
+            for (int j = 0; j < TN; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = lk_i8_out(acc[i][j][4 * e4 + e], sx, sw[i][e4][e]);
-                *(lk_f4 *) (st + lm * LS + 32 * i + 8 * e4 + 4 * h) = v;
+                for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
+#pragma unroll
+        for (int k = 0; k < TM + TN; ++k) read(0, 0, 0, k);
+#pragma unroll 1
+        for (int s = 0; s + 1 < nst; ++s) stage(s, false);
+        // the last stage brings the next tile's first; after the last tile, its own again
+        int row1 = row0, tok1 = tok0;
+        if (MORE) {
+            id += gridDim.x;
+            if (id < ntile) place(id, row1, tok1);
+            aim(row1, tok1);
+        }
+        stage(nst - 1, true);
+        // What is on its way lands before LDS is used otherwise (MORE: so that the next tile's first stage
+        // needs no wait that the stores below would be part of), and every wave has read its last operands.
+        lk_wait_vm<0>();
+        // Outputs by way of LDS, 32 tokens and 32 RS rows of the wave at a time: a lane has token
+        // lm and rows 8 * e4 + 4 * h .. +3 of every MFMA tile, 8 bytes of 32 output rows per store;
+        // from LDS it takes 8 consecutive rows of one token, whole runs of 64 * RS bytes (bf16).
+        // A token's 16-byte pieces are XOR-permuted so that writes and reads use all banks alike.
+        constexpr int RS = SH::RS, RW = 32 * RS;
+        __syncthreads();
+        if constexpr (SH::WK > 1) {                          // the parts of K meet: integer sums have no order
+            lk_i16v * pt = (lk_i16v *) stg;
+            if (kw > 0) {
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) pt[((w - WMN) * TM * TN + i * TN + j) * 64 + lane] = acc[i][j];
             }
-        __builtin_amdgcn_wave_barrier();
+            __syncthreads();
+            if (kw > 0) return;
 #pragma unroll
-        for (int k = 0; k < 32 / TP; ++k) {
-            const int tl = k * TP + lane / LT, t = t0 + tl;
-            float v[8];
-            *(lk_f4 *) v = *(const lk_f4 *) (st + tl * LS + r8);
-            *(lk_f4 *) (v + 4) = *(const lk_f4 *) (st + tl * LS + r8 + 4);
-            if (t >= a.M || r >= a.N) continue;
-            if (r + 8 <= a.N) {
-                if (res) {
-                    float o[8];
-                    lk_load<8>(res + (size_t) t * a.ldr + r, o);
+            for (int k = 1; k < SH::WK; ++k)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = o[e] + v[e];
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) acc[i][j] += pt[((k * WMN + w - WMN) * TM * TN + i * TN + j) * 64 + lane];
+        }
+        // (behind the parts of K, which other waves may still be reading)
+        uint8_t * st = stg + (MORE ? (nst - 1 + sb) % NB * SH::BYTES : SH::PARTS) + (w % WMN) * SH::STG;
+        auto piece = [&](int t, int p) { return st + t * (RW * 4) + (p ^ (RS == 2 ? t & 15 : t >> 1 & 7)) * 16; };
+        const T * res = (const T *) a.res;
+        T * out = (T *) a.out;
+        constexpr int LT = RW / 8, TP = 64 / LT;             // lanes a token, tokens a step
+#pragma unroll
+        for (int i0 = 0; i0 < TM; i0 += RS) {
+            float sw[RS][4][4];
+#pragma unroll
+            for (int i = 0; i < RS; ++i)
+#pragma unroll
+                for (int e4 = 0; e4 < 4; ++e4) {
+                    const int r = row0 + wr + 32 * (i0 + i) + 8 * e4 + 4 * h;
+                    if (r + 4 <= a.N) lk_load<4>(a.sw + r, sw[i][e4]);
+                    else
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) sw[i][e4][e] = r + e < a.N ? a.sw[r + e] : 0.0f;
                 }
-                lk_store<8>(out + (size_t) t * a.ldo + r, v);
-            } else {
+            const int r8 = lane % LT, r = row0 + wr + 32 * i0 + 8 * r8;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) if (r + e < a.N) {
-                    float u = v[e];
-                    if (res) u = (float) res[(size_t) t * a.ldr + r + e] + u;
-                    out[(size_t) t * a.ldo + r + e] = (T) u;
+            for (int j = 0; j < TN; ++j) {
+                const int t0 = tok0 + wt + 32 * j;           // wave-uniform
+                const float sx = a.sx[t0 + lm < a.M ? t0 + lm : a.M - 1];
+#pragma unroll
+                for (int i = 0; i < RS; ++i)
+#pragma unroll
+                    for (int e4 = 0; e4 < 4; ++e4) {
+                        lk_f4 v;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] = lk_i8_out(acc[i0 + i][j][4 * e4 + e], sx, sw[i][e4][e]);
+                        *(lk_f4 *) piece(lm, 8 * i + 2 * e4 + h) = v;
+                    }
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int k = 0; k < 32 / TP; ++k) {
+                    const int tl = k * TP + lane / LT, t = t0 + tl;
+                    float v[8];
+                    *(lk_f4 *) v = *(const lk_f4 *) piece(tl, 2 * r8);
+                    *(lk_f4 *) (v + 4) = *(const lk_f4 *) piece(tl, 2 * r8 + 1);
+                    if (t >= a.M || r >= a.N) continue;
+                    if (r + 8 <= a.N) {
+                        if (res) {
+                            float o[8];
+                            lk_load<8>(res + (size_t) t * a.ldr + r, o);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) v[e] = o[e] + v[e];
+                        }
+                        lk_store<8>(out + (size_t) t * a.ldo + r, v);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) if (r + e < a.N) {
+                            float u = v[e];
+                            if (res) u = (float) res[(size_t) t * a.ldr + r + e] + u;
+                            out[(size_t) t * a.ldo + r + e] = (T) u;
+                        }
+                    }
                 }
+                __builtin_amdgcn_wave_barrier();
             }
         }
-        __builtin_amdgcn_wave_barrier();
+        if (!MORE || id >= ntile) return;
+        row0 = row1;
+        tok0 = tok1;
+        sb = (sb + nst) % NB;
+        __syncthreads();                                     // every wave has left the outputs' room
     }
 }
 
@@ -321,7 +359,9 @@ template <class SH, int TYPE>
 static int lk_i8_tiles(const LkI8Args & a, hipStream_t st) {
     const long n = lk_i8_ntile<SH::BM, SH::BN>(a);       // a grid has fewer than 2^32 threads
     if (n * 64 * SH::NW >= 1l << 32) return lk_fail(hipErrorInvalidValue, "lk_gemm_i8: %d x %d outputs", a.M, a.N);
-    hipLaunchKernelGGL((lk_k_gemm_i8<SH, TYPE>), dim3((unsigned) n), dim3(64 * SH::NW), 0, st, a);
+    // rings that go on: as many workgroups as the units hold (a multiple of the XCDs)
+    const long most = SH::MORE ? 256 * ((160 << 10) / SH::LDS) : n;
+    hipLaunchKernelGGL((lk_k_gemm_i8<SH, TYPE>), dim3((unsigned) (n < most ? n : most)), dim3(64 * SH::NW), 0, st, a);
     return 0;
 }
 // Which kernel.  A compute unit holds one or two workgroups of a shape, so what counts is

@@ -54,8 +54,9 @@ def q8_row_ref(y):
 
 
 def gemm_ref(x, sx, w, sw, dtype, res=None):
-    """The exact sum (below 2^53 in fp64), then the roundings of the definition."""
-    s = (x.double() @ w.double().t()).float()
+    """The exact sum (below 2^53 in fp64), then the roundings of the definition.  An integer
+    zero is +0; the product of one column in fp64 may make it -0."""
+    s = (x.double() @ w.double().t()).float() + 0.0
     v = (s * sx[:, None]) * sw[None, :]
     if res is not None:
         v = res.float() + v
