@@ -71,6 +71,15 @@ def test_lines_between_tiles_bit_exact(lk, M, N, K):
     _case(lk, M, N, K, dt, (M + N + K) % 2 == 1, 16, M + N + K)
 
 
+# more tiles than the units hold at once, so that a workgroup goes on to a second and third, with one,
+# two and three stages of K (the ring's place changes from tile to tile, or not)
+@pytest.mark.parametrize("M,N,K", [(4100, 8200, 100), (4100, 8200, 130), (4100, 8200, 300), (2600, 8190, 300), (2600, 8190, 128)])
+def test_workgroups_of_several_tiles_bit_exact(lk, M, N, K):
+    dt = TYPES["bf16"] if K != 130 else TYPES["f32"]
+    note(f"gemm_i8 M={M} N={N} K={K} {dt}")
+    _case(lk, M, N, K, dt, K == 130, 0, M + N + K)
+
+
 @pytest.mark.parametrize("M", [1, 40])
 def test_largest_sums(lk, M):
     """-128 * -128 over the longest K: 2^31 - 2^14, the int32 range's end; and its
