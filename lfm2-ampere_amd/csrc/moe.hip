@@ -24,14 +24,20 @@
 
 typedef uint32_t lk_u4 __attribute__((ext_vector_type(4)));
 
-// Up to this many tokens every workgroup chooses the experts itself, a wave per
-// token, and the down product adds the experts up itself (three launches); above it a
+// For a few tokens (at most this many) every workgroup chooses the experts itself, a wave
+// per token, and the down product adds the experts up itself (three launches); for more a
 // launch of one workgroup chooses once and sorts the tokens by expert, and another
-// adds up (five).  us with three / five launches, bf16:
-//   tokens                          2          4          5          8
-//   64 experts, 4 of 2048 x 1536    20 / 26    30 / 33    33 / 34    47 / 47
-//   32 experts, 2 of 2048 x 1792    16 / 21    20 / 25    23 / 29    32 / 35
-//   128 experts, 8 of 2048 x 768     23 / 30    36 / 38    39 / 43    55 / 55
+// adds up (five).  us with three / five launches, bf16 and fp32 rows; the rule (lk_moe_few)
+// takes three for up to 5 tokens and for up to 16 choices in all:
+//   tokens                           2        4        5        6        7        8
+//   64 experts, 4 of 2048 x 1536   20/26    30/33    33/33    39/38    46/42    48/44
+//                            fp32  20/26    29/31    34/33    38/34    44/38    46/39
+//   128 experts, 8 of 2048 x 768   22/30    36/37    40/42    45/43    52/49    56/52
+//                            fp32  23/30    35/35    39/38    44/38    49/44    54/45
+//   16 experts, 4 of 1280 x 1184   16/22    21/25    22/25    25/27    27/28    28/28
+//                            fp32  17/22    24/25    24/26    29/27    31/27    35/28
+//   32 experts, 2 of 2048 x 1792   15/22    20/26    23/30    27/32    29/33    33/35
+//                            fp32  16/22    21/27    23/27    25/27    27/28    32/29
 #define LK_MOE_FEW 8
 #define LK_MOE_THREADS 256
 #define LK_MOE_NW 8                       // waves of a gate/up workgroup for few tokens
@@ -62,7 +68,7 @@ struct LkMoeArgs {
     float * y;                           // [T * k][hidden]
     int32_t * ids;                       // [T * k]
     float * wts;                         // [T * k]
-    int32_t * tab;                       // LkMoeTab, for more than LK_MOE_FEW tokens
+    int32_t * tab;                       // LkMoeTab, for more than a few tokens
     int ldx, ldr, ldo, T, E, k, hidden, ffn, score, renorm, kinv;
     float scale;
 };
@@ -324,7 +330,7 @@ __device__ __forceinline__ void lk_moe_choose(const LkMoeArgs & a, const float (
         w[t] *= a.scale;
     }
 }
-// More than LK_MOE_FEW tokens: one workgroup of 16 waves chooses for all of them and
+// More than a few tokens: one workgroup of 16 waves chooses for all of them and
 // sorts the assignments by expert: TW tokens a wave, whose steps fill each other's waits, and
 // several lanes to an expert's rank among the counts (64 tokens 9.0 us, 19 tokens 5.6; a token, an
 // expert and a count at a time 11.1 and 6.1; 64 tokens: 1 us of it the logits' way, 4 the choice, the
@@ -569,7 +575,7 @@ __device__ __forceinline__ void lk_moe_up_tiles(const LkMoeArgs & a, int e, cons
     }
 }
 
-// Up to LK_MOE_FEW tokens; grid (ffn / 32, T * k): the workgroups of an assignment
+// A few tokens; grid (ffn / 32, T * k): the workgroups of an assignment
 // whose expert an earlier one has end at once.
 template <int NP, int NL>
 __global__ void __launch_bounds__(64 * LK_MOE_NW, 4)
@@ -890,7 +896,7 @@ lk_k_moe_many(const LkMoeArgs a) {
     else              lk_moe_down_many<NP>(a, e, as, n, sh);
 }
 
-// Up to LK_MOE_FEW tokens: a workgroup of 16 waves has 8 rows of every expert that was
+// A few tokens: a workgroup of 16 waves has 8 rows of every expert that was
 // chosen (at most 64), and adds them up itself.  The waves share the experts, Q = 16 /
 // experts of them (at least one) to each, taking its block groups in turn.
 template <int TYPE, int NP>
@@ -1022,9 +1028,12 @@ extern "C" size_t lk_moe_work_bytes(const lk_moe * moe, int T) {
     return lk_moe_layout(moe, T, nullptr, nullptr);
 }
 
+static bool lk_moe_few(const LkMoeArgs & a) { return a.T <= 5 || (a.T <= LK_MOE_FEW && a.T * a.k <= 16); }
+
 template <int TYPE>
 static void lk_moe_go(const LkMoeArgs & a, hipStream_t st) {
     constexpr int NP = TYPE == LK_F32 ? 3 : 2;
+    const bool few = lk_moe_few(a);
     const int nE = (a.E + 3) / 4, na = a.T * a.k, slots = na < a.E ? na : a.E;
     hipLaunchKernelGGL((lk_k_moe_router<TYPE, NP>), dim3(nE + (a.hidden / 8 + LK_MOE_THREADS - 1) / LK_MOE_THREADS, (a.T + 3) / 4),
                        dim3(LK_MOE_THREADS), 0, st, a, nE);
@@ -1036,14 +1045,14 @@ static void lk_moe_go(const LkMoeArgs & a, hipStream_t st) {
     };
     auto go = [&](auto regs) {                           // registers of 64 experts a choosing wave holds
         constexpr int NL = decltype(regs)::value;
-        if (a.T <= LK_MOE_FEW)
+        if (few)
             hipLaunchKernelGGL((lk_k_moe_up_few<NP, NL>), dim3(a.ffn / 32, na), dim3(64 * LK_MOE_NW), 0, st, a);
         else
             route(LkInt<NL>{});
     };
     if (a.E <= 64) go(LkInt<1>{});
     else           go(LkInt<LK_MOE_MAX_EXPERTS / 64>{});
-    if (a.T <= LK_MOE_FEW) {
+    if (few) {
         hipLaunchKernelGGL((lk_k_moe_down_few<TYPE, NP>), dim3(a.hidden / 8), dim3(64 * LK_MOE_NWF), 0, st, a);
         return;
     }

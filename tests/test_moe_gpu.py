@@ -305,3 +305,17 @@ def test_longest_rows(lk, hidden, ffn, T):
     want, ids1, _ = moe_ref(x, k=2, score="sigmoid", **L)
     assert torch.equal(ids.long(), ids1)
     _close(out, want, dt, (hidden, ffn, T))
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("T,k", [(5, 8), (6, 2), (6, 3), (8, 2), (8, 1), (7, 3), (8, 8)])
+def test_both_sides_of_the_line_between_launches(lk, T, k, t):
+    """Up to 5 tokens or 16 choices in three launches, more in five."""
+    hidden, ffn, E, dt = 288, 160, 9, TYPES[t]
+    L = _layer(60 + T, E, hidden, ffn, bias=k > 2)
+    x, res = _x(T, T, hidden, dt), _x(T + 1, T, hidden, dt)
+    note(f"moe T={T} k={k} {t}")
+    out, ids, _ = _run(lk, _make(lk, L, k), x, hidden, dt, k, res)
+    want, ids1, _ = moe_ref(x, k=k, score="sigmoid", res=res, **L)
+    assert torch.equal(ids.long(), ids1)
+    _close(out, want, dt, (T, k))
