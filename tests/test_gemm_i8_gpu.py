@@ -71,6 +71,13 @@ def test_lines_between_tiles_bit_exact(lk, M, N, K):
     _case(lk, M, N, K, dt, (M + N + K) % 2 == 1, 16, M + N + K)
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 16385, 70), (17, 16500, 260), (32, 20001, 515), (33, 16390, 130)])
+def test_few_tokens_and_many_rows_bit_exact(lk, M, N, K):
+    dt = list(TYPES.values())[M % 3]
+    note(f"gemm_i8 M={M} N={N} K={K} {dt}")
+    _case(lk, M, N, K, dt, M % 2 == 1, 16, M + N + K)
+
+
 # more tiles than the units hold at once, so that a workgroup goes on to a second and third, with one,
 # two and three stages of K (the ring's place changes from tile to tile, or not)
 @pytest.mark.parametrize("M,N,K", [(4100, 8200, 100), (4100, 8200, 130), (4100, 8200, 300), (2600, 8190, 300), (2600, 8190, 128)])
