@@ -384,8 +384,10 @@ static int lk_i8_tiles(const LkI8Args & a, hipStream_t st) {
 //   2600 x 8192 x 2048                             71.3     71.3    60.6*   65.7
 //   4096 x 8192 x 2048                            104.8    100.8    86.0    76.3*
 // A round of 256 256x256 tiles takes about 5 / 3 of one of 512 128x128 tiles.
-// Up to 32 tokens, wider tiles have nothing to share: many weight rows take 64x32 with K over two
-// waves and short stages (three workgroups a unit): 1 x 32000 x 2048 11.9 (64x64 12.3, 128x64 12.8,
+// 64x32 has two forms: K over four waves in stages of 256 bytes (4096 x 128 x 8192 12.2 us, 13.9 with two
+// waves and 128), and over two in stages of 128 where K is short (8192 x 64 x 512 4.0, 4.6).
+// Up to 32 tokens, wider tiles have nothing to share: many weight rows take the second
+// form too, three workgroups a unit: 1 x 32000 x 2048 11.9 (64x64 12.3, 128x64 12.8,
 // few 11.3), 32 x 65536 x 2048 22.3 (24.4, 22.9), 16 x 128256 x 4096 92 (96, 98; 5.7 TB/s of weights).
 template <int TYPE>
 static int lk_i8_shape(const LkI8Args & a, hipStream_t st) {
@@ -395,8 +397,9 @@ static int lk_i8_shape(const LkI8Args & a, hipStream_t st) {
         return 0;
     }
     if (lk_i8_ntile<32, 32>(a) <= 256) return lk_i8_tiles<LkI8Shape<1, 1, 1, 1, 4, 256, 4, 2>, TYPE>(a, st);
-    if (lk_i8_ntile<64, 32>(a) <= 256) return lk_i8_tiles<LkI8Shape<1, 1, 2, 1, 4, 256, 4, 2>, TYPE>(a, st);
-    if (a.M <= 32) return lk_i8_tiles<LkI8Shape<1, 1, 2, 1, 2, 128, 4, 2>, TYPE>(a, st);
+    const bool one = lk_i8_ntile<64, 32>(a) <= 256;      // round
+    if (one && a.K >= 2048) return lk_i8_tiles<LkI8Shape<1, 1, 2, 1, 4, 256, 4, 2>, TYPE>(a, st);
+    if (one || a.M <= 32) return lk_i8_tiles<LkI8Shape<1, 1, 2, 1, 2, 128, 4, 2>, TYPE>(a, st);
     if (lk_i8_ntile<64, 64>(a) <= 256) return lk_i8_tiles<LkI8Shape<1, 1, 2, 2, 2, 128, 4, 2>, TYPE>(a, st);
     if (lk_i8_ntile<128, 64>(a) <= 256) return lk_i8_tiles<LkI8Shape<2, 1, 2, 2, 2, 128, 3, 2>, TYPE>(a, st);
     const long t128 = lk_i8_ntile<128, 128>(a), t256 = lk_i8_ntile<256, 256>(a);
