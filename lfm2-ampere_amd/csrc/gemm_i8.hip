@@ -364,9 +364,9 @@ static int lk_i8_tiles(const LkI8Args & a, hipStream_t st) {
     hipLaunchKernelGGL((lk_k_gemm_i8<SH, TYPE>), dim3((unsigned) (n < most ? n : most)), dim3(64 * SH::NW), 0, st, a);
     return 0;
 }
-// Which kernel.  A compute unit holds one or two workgroups of a shape, so what counts is
-// how many rounds of 256 units the tiles take; the largest tile whose tiles still fill one
-// round loses to the next smaller one, which shares less but splits K over the waves (WK).
+// Which kernel.  What counts is how many rounds of 256 units the tiles take: the smallest
+// tile that fits one round is the best, for a larger one leaves units idle and has fewer waves
+// to share K, and a smaller one takes a second round.
 // Measured (bf16 out, operands in the cache, us; * is what the rule takes):
 //   M x N x K          few   32x32  64x32  64x64  128x64  128x128  2/unit  256x256
 //   1 x 4096 x 4096    4.3*   5.7    6.8    7.8
