@@ -28,16 +28,16 @@ typedef uint32_t lk_u4 __attribute__((ext_vector_type(4)));
 // per token, and the down product adds the experts up itself (three launches); for more a
 // launch of one workgroup chooses once and sorts the tokens by expert, and another
 // adds up (five).  us with three / five launches, bf16 and fp32 rows; the rule (lk_moe_few)
-// takes three for up to 5 tokens and for up to 16 choices in all:
+// takes three for up to 5 tokens, and 8 of up to 28 choices in all (fp32 rows: 16):
 //   tokens                           2        4        5        6        7        8
-//   64 experts, 4 of 2048 x 1536   20/26    30/33    33/33    39/38    46/42    48/44
-//                            fp32  20/26    29/31    34/33    38/34    44/38    46/39
-//   128 experts, 8 of 2048 x 768   22/30    36/37    40/42    45/43    52/49    56/52
-//                            fp32  23/30    35/35    39/38    44/38    49/44    54/45
-//   16 experts, 4 of 1280 x 1184   16/22    21/25    22/25    25/27    27/28    28/28
-//                            fp32  17/22    24/25    24/26    29/27    31/27    35/28
-//   32 experts, 2 of 2048 x 1792   15/22    20/26    23/30    27/32    29/33    33/35
-//                            fp32  16/22    21/27    23/27    25/27    27/28    32/29
+//   64 experts, 4 of 2048 x 1536   19/26    27/33    32/33    36/38    41/43    45/43
+//                            fp32  20/26    29/31    33/33    35/34    39/39    40/39
+//   128 experts, 8 of 2048 x 768   21/30    33/37    38/42    43/43    50/49    55/52
+//                            fp32  22/30    34/35    38/38    41/38    44/44    49/45
+//   16 experts, 4 of 1280 x 1184   16/22    20/25    22/25    25/27    27/28    29/28
+//                            fp32  16/22    21/25    23/26    26/26    28/27    31/28
+//   32 experts, 2 of 2048 x 1792   15/22    19/26    23/30    25/32    27/33    31/35
+//                            fp32  15/22    20/27    22/27    23/27    24/28    28/29
 #define LK_MOE_FEW 8
 #define LK_MOE_THREADS 256
 #define LK_MOE_NW 8                       // waves of a gate/up workgroup for few tokens
@@ -520,106 +520,6 @@ __device__ __forceinline__ void lk_moe_up_rows(const LkMoeArgs & a, int e, int h
     }
 }
 
-// 32 rows of one expert's gate and up products for N assignments (as[0 .. N-1] in LDS; the
-// only one: as0), and what follows of them: the records of h.  Wave w has half w & 1 of the rows and part w >>
-// 1 of K.  N is known at compile time: with branches on it the compiler keeps the digits
-// of all tokens at once and spills.
-template <int NP>
-struct LkMoeUp {
-    static constexpr int U = 2, TK = 4;
-    LkMoeX<NP, U> xs[LK_MOE_NW][TK];
-    float part[LK_MOE_NW / 2][2][TK][32];                // [part of K][gate, up][token][row]
-};
-template <int NP, int N>
-__device__ __forceinline__ void lk_moe_up_tile(const LkMoeArgs & a, int e, const int * as, int as0, LkMoeUp<NP> & sh) {
-    constexpr int U = LkMoeUp<NP>::U, REC = LkMoeRec<NP>::BYTES;
-    const int tid = threadIdx.x, lane = tid & 63, c = lane >> 3, g = lane & 7;
-    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), half = wv & 1, kp = wv >> 1, F = a.ffn;
-    const uint8_t * qs[4];
-    const _Float16 * d[4];
-    lk_moe_up_rows(a, e, half, qs, d);
-    int trow[N];
-#pragma unroll
-    for (int r = 0; r < N; ++r) trow[r] = lk_moe_token(a, N == 1 ? as0 : __builtin_amdgcn_readfirstlane(as[r]));
-    float acc[N][4] = {};
-    lk_moe_rows<NP, 4, U, N>(qs, d, a.xr, a.hidden / 32, trow, kp, LK_MOE_NW / 2, sh.xs[wv], acc);
-#pragma unroll
-    for (int t = 0; t < N; ++t)
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            const float v = lk_moe_lanes(acc[t][m]);
-            if (g == m) sh.part[kp][m >> 1][t][16 * half + 8 * (m & 1) + c] = v;
-        }
-    __syncthreads();
-    if (tid < 32 * N) {                                  // token t, row r of the 32
-        const int t = tid >> 5, r = tid & 31;
-        float gt = 0.0f, up = 0.0f;
-#pragma unroll
-        for (int k = 0; k < LK_MOE_NW / 2; ++k) {
-            gt += sh.part[k][0][t][r];
-            up += sh.part[k][1][t][r];
-        }
-        lk_moe_record<NP>(lk_moe_h(gt, up), r, true, a.hr + ((size_t) (N == 1 ? as0 : as[t]) * (F / 32) + blockIdx.x) * REC);
-    }
-}
-
-// n assignments, four at a time.
-template <int NP>
-__device__ __forceinline__ void lk_moe_up_tiles(const LkMoeArgs & a, int e, const int * as, int n, LkMoeUp<NP> & sh) {
-    for (; n > 0; n -= 4, as += 4) {
-        if (n >= 4)      lk_moe_up_tile<NP, 4>(a, e, as, 0, sh);
-        else if (n == 3) lk_moe_up_tile<NP, 3>(a, e, as, 0, sh);
-        else if (n == 2) lk_moe_up_tile<NP, 2>(a, e, as, 0, sh);
-        else             lk_moe_up_tile<NP, 1>(a, e, as, __builtin_amdgcn_readfirstlane(as[0]), sh);
-        if (n > 4) __syncthreads();                      // part has been read
-    }
-}
-
-// A few tokens; grid (ffn / 32, T * k): the workgroups of an assignment
-// whose expert an earlier one has end at once.
-template <int NP, int NL>
-__global__ void __launch_bounds__(64 * LK_MOE_NW, 4)
-lk_k_moe_up_few(const LkMoeArgs a) {
-    __shared__ int ids[LK_MOE_FEW * LK_MOE_MAX_TOP_K], as[LK_MOE_FEW];
-    __shared__ LkMoeUp<NP> sh;
-    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), na = a.T * a.k;
-    const bool tells = blockIdx.x == 0 && blockIdx.y == 0;          // the one that writes the choices down
-    int mine = -1;
-    if (a.T == 1 || wv < a.T) {                          // one token: every wave for itself
-        const int t = a.T == 1 ? 0 : wv;
-        int id[1];
-        float l[1][NL], b[NL], w[1];
-        lk_moe_logits<NL>(a, t, l[0]);
-        lk_moe_bias<NL>(a, b);
-        lk_moe_choose<NL, 1>(a, l, b, id, w);
-        mine = id[0];
-        if (mine >= 0) {
-            if (a.T > 1) ids[t * a.k + lane] = mine;
-            if (tells && (a.T > 1 || wv == 0)) {
-                const int i = t * a.k + lane;
-                a.ids[i] = mine;
-                a.wts[i] = w[0];
-                if (a.ids_out) a.ids_out[i] = mine;
-                if (a.wts_out) a.wts_out[i] = w[0];
-            }
-        }
-    }
-    if (a.T > 1) {
-        __syncthreads();
-        mine = lane < na ? ids[lane] : -1;
-    }
-    const int e = __builtin_amdgcn_readlane(mine, blockIdx.y);
-    const uint64_t hits = __ballot(mine == e);
-    if (__builtin_ctzll(hits) != (int) blockIdx.y) return;
-    if (a.T == 1) {
-        lk_moe_up_tile<NP, 1>(a, e, as, blockIdx.y, sh);
-        return;
-    }
-    if (wv == 0 && mine == e) as[__popcll(hits & ((1ull << lane) - 1))] = lane;
-    __syncthreads();
-    lk_moe_up_tiles<NP>(a, e, as, __popcll(hits), sh);
-}
-
 // More tokens: a workgroup of 4 waves has 32 rows (up: of gate and up) or 64 (down) of
 // one expert and up to TG of its assignments at a time.  Wave w has half w & 1 of the rows
 // (four matrices of 8 rows) and every second step of 8 blocks of K; it copies a step's
@@ -704,18 +604,18 @@ __device__ __forceinline__ void lk_moe_many_dots(const uint8_t * const (&qs)[4],
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-// The same for n of up to TG assignments.  sum[j][q]: 16 rows of matrices 2 j and 2 j + 1, row l %
+// The same for n of up to TG assignments, over the steps s0, s0 + 2, ..., or of PAIRS, s0, s0 + 1, s0 + 8,
+// s0 + 9, ....  sum[j][q]: 16 rows of matrices 2 j and 2 j + 1, row l %
 // 16; assignment 2 (l / 16) + q of two digits, l / 16 of three.  The blocks of a step are summed
 // apart over the steps and joined as the dots' lanes are, so that a token's result does not
 // depend, by a bit, on how many others chose its expert.
-template <int NP>
-__device__ __forceinline__ void lk_moe_many_mfma(const uint8_t * const (&qs)[4], const _Float16 * const (&d)[4], const uint8_t * rec,
-                                                 int bpr, const int (&trow)[LkMoeShare<NP>::TG], int n, LkMoeShare<NP> & sh,
-                                                 float (&sum)[2][4 - NP]) {
+template <int NP, bool PAIRS>
+__device__ __forceinline__ void lk_moe_mfma(const uint8_t * const (&qs)[4], const _Float16 * const (&d)[4], const uint8_t * rec,
+                                                 int bpr, const int (&trow)[LkMoeShare<NP>::TG], int n, int s0, typename LkMoeShare<NP>::Wave & me,
+                                            float (&sum)[2][4 - NP]) {
     constexpr int PC = LkMoeRec<NP>::PIECES, Z = LkMoeShare<NP>::Z, TG = LkMoeShare<NP>::TG, NQ = 4 - NP;
-    const int lane = threadIdx.x & 63, c = lane >> 3, g = lane & 7, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, c = lane >> 3, g = lane & 7;
     const int r = lane & 15, h = lane >> 4, ns = (bpr + 7) / 8;
-    typename LkMoeShare<NP>::Wave & me = sh.wave[wv];
     const uint32_t lds = lk_lds_addr(me.x);
     const int t = NP == 2 ? r >> 1 : r >> 2, p = NP == 2 ? r & 1 : (r & 3) < 3 ? r & 3 : 2;
     const uint32_t * xa = (const uint32_t *) (me.x + LkMoeShare<NP>::at(t) + 2 * p) + h;   // + 4 PC b: the row's digits 4 h ..; 16 + 4 h .. behind 4
@@ -745,10 +645,11 @@ __device__ __forceinline__ void lk_moe_many_mfma(const uint8_t * const (&qs)[4],
         }
     };
     float acc[8][2][NQ] = {};
-    load(wv >> 1);
-    copy(wv >> 1);
+    auto next = [](int s) { return !PAIRS ? s + 2 : s & 1 ? s + 7 : s + 1; };
+    load(s0);
+    copy(s0);
 #pragma unroll 1
-    for (int s = wv >> 1; s < ns; s += 2) {
+    for (int s = s0; s < ns; s = next(s)) {
         const bool in = 8 * s + g < bpr;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // the copies; the weights, asked for before, come with them
 #pragma unroll
@@ -757,7 +658,7 @@ __device__ __forceinline__ void lk_moe_many_mfma(const uint8_t * const (&qs)[4],
             ((_Float16 *) &me.d[8 * m + c])[g] = in ? dw[m] : (_Float16) 0.0f;
         }
         __builtin_amdgcn_wave_barrier();
-        load(s + 2);                                     // past the last: in bounds, not used
+        load(next(s));                                   // past the last: in bounds, not used
         union { lk_u4 q; _Float16 h[8]; } dv[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) dv[j].q = me.d[16 * j + r];
@@ -796,7 +697,7 @@ __device__ __forceinline__ void lk_moe_many_mfma(const uint8_t * const (&qs)[4],
                 for (int q = 0; q < NQ; ++q) asm volatile("" : "+v"(acc[b][j][q]) :: "memory");
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");          // the digits have been read
-        copy(s + 2);
+        copy(next(s));
     }
 #pragma unroll
     for (int j = 0; j < 2; ++j)
@@ -804,6 +705,116 @@ __device__ __forceinline__ void lk_moe_many_mfma(const uint8_t * const (&qs)[4],
         for (int q = 0; q < NQ; ++q)
             sum[j][q] = ((acc[0][j][q] + acc[1][j][q]) + (acc[2][j][q] + acc[3][j][q])) +
                         ((acc[4][j][q] + acc[5][j][q]) + (acc[6][j][q] + acc[7][j][q]));
+}
+
+// 32 rows of one expert's gate and up products for n of its assignments (as, in LDS; the only one:
+// as0), all in all `of` them, and what follows: the records of h.  Wave w has half w & 1 of the rows
+// and of K the pairs of steps w >> 1, + 4, ...  One assignment by dots, more by matrix instructions;
+// both add the blocks in the same order.  (Dots for up to four at a time: 4 tokens, 4 of 64 experts, 30
+// us, so 27; 5 tokens, all of 8 experts of two each, 24 and 22.)
+template <int NP>
+struct LkMoeUp {
+    static constexpr int U = 2, TG = LkMoeShare<NP>::TG;
+    struct One {
+        LkMoeX<NP, U> xs[LK_MOE_NW][1];
+        float part[LK_MOE_NW / 2][64];                   // [part of K][row of 32 gate and 32 up]
+    };
+    union {
+        One one;
+        typename LkMoeShare<NP>::Wave wave[LK_MOE_NW];
+        float part[LK_MOE_NW / 2][TG][64];               // of more: [part of K][assignment][row], where the digits were
+    };
+};
+template <int NP>
+__device__ __forceinline__ void lk_moe_up_few(const LkMoeArgs & a, int e, const int * as, int as0, int n, int of, LkMoeUp<NP> & sh) {
+    constexpr int TG = LkMoeUp<NP>::TG;
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), half = wv & 1, kp = wv >> 1, F = a.ffn;
+    const uint8_t * qs[4];
+    const _Float16 * d[4];
+    lk_moe_up_rows(a, e, half, qs, d);
+    if (n == 1) {
+        const int c = lane >> 3, g = lane & 7, trow[1] = { lk_moe_token(a, of == 1 ? as0 : __builtin_amdgcn_readfirstlane(as[0])) };
+        float acc[1][4] = {};
+        lk_moe_rows<NP, 4, LkMoeUp<NP>::U, 1>(qs, d, a.xr, a.hidden / 32, trow, kp, LK_MOE_NW / 2, sh.one.xs[wv], acc);
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            const float v = lk_moe_lanes(acc[0][m]);
+            if (g == m) sh.one.part[kp][32 * (m >> 1) + 16 * half + 8 * (m & 1) + c] = v;
+        }
+    } else {
+        constexpr int NQ = 4 - NP;
+        int trow[TG];
+#pragma unroll
+        for (int t = 0; t < TG; ++t) trow[t] = lk_moe_token(a, __builtin_amdgcn_readfirstlane(as[t < n ? t : 0]));
+        float acc[2][NQ];
+        lk_moe_mfma<NP, true>(qs, d, a.xr, a.hidden / 32, trow, n, 2 * kp, sh.wave[wv], acc);
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) sh.part[kp][NQ * (lane >> 4) + q][32 * j + 16 * half + (lane & 15)] = acc[j][q];
+    }
+    __syncthreads();
+    const int t = tid >> 5, r = tid & 31;
+    if (t < n) {                                         // whole halves of waves
+        float gt = 0.0f, up = 0.0f;
+#pragma unroll
+        for (int k = 0; k < LK_MOE_NW / 2; ++k) {
+            const float * p = n == 1 ? sh.one.part[k] : sh.part[k][t];
+            gt += p[r];
+            up += p[32 + r];
+        }
+        lk_moe_record<NP>(lk_moe_h(gt, up), r, true,
+                          a.hr + ((size_t) (of == 1 ? as0 : as[t]) * (F / 32) + blockIdx.x) * LkMoeRec<NP>::BYTES);
+    }
+}
+
+// A few tokens; grid (ffn / 32, T * k): the workgroups of an assignment
+// whose expert an earlier one has end at once.
+template <int NP, int NL>
+__global__ void __launch_bounds__(64 * LK_MOE_NW, 4)
+lk_k_moe_up_few(const LkMoeArgs a) {
+    __shared__ int ids[LK_MOE_FEW * LK_MOE_MAX_TOP_K], as[LK_MOE_FEW];
+    __shared__ LkMoeUp<NP> sh;
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), na = a.T * a.k;
+    const bool tells = blockIdx.x == 0 && blockIdx.y == 0;          // the one that writes the choices down
+    int mine = -1;
+    if (a.T == 1 || wv < a.T) {                          // one token: every wave for itself
+        const int t = a.T == 1 ? 0 : wv;
+        int id[1];
+        float l[1][NL], b[NL], w[1];
+        lk_moe_logits<NL>(a, t, l[0]);
+        lk_moe_bias<NL>(a, b);
+        lk_moe_choose<NL, 1>(a, l, b, id, w);
+        mine = id[0];
+        if (mine >= 0) {
+            if (a.T > 1) ids[t * a.k + lane] = mine;
+            if (tells && (a.T > 1 || wv == 0)) {
+                const int i = t * a.k + lane;
+                a.ids[i] = mine;
+                a.wts[i] = w[0];
+                if (a.ids_out) a.ids_out[i] = mine;
+                if (a.wts_out) a.wts_out[i] = w[0];
+            }
+        }
+    }
+    if (a.T > 1) {
+        __syncthreads();
+        mine = lane < na ? ids[lane] : -1;
+    }
+    const int e = __builtin_amdgcn_readlane(mine, blockIdx.y);
+    const uint64_t hits = __ballot(mine == e);
+    if (__builtin_ctzll(hits) != (int) blockIdx.y) return;
+    const int n = __popcll(hits);
+    if (n > 1) {
+        if (wv == 0 && mine == e) as[__popcll(hits & ((1ull << lane) - 1))] = lane;
+        __syncthreads();
+    }
+    constexpr int TG = LkMoeUp<NP>::TG;
+    for (int at = 0; at < n; at += TG) {
+        if (at) __syncthreads();                         // part has been read
+        lk_moe_up_few<NP>(a, e, as + at, blockIdx.y, n - at < TG ? n - at : TG, n, sh);
+    }
 }
 
 // n of up to TG assignments (as, the rows of records trow) of an expert: the sums of the
@@ -825,7 +836,7 @@ __device__ __forceinline__ void lk_moe_many_part(const uint8_t * const (&qs)[4],
     } else {
         constexpr int NQ = 4 - NP;
         float acc[2][NQ];
-        lk_moe_many_mfma<NP>(qs, d, rec, bpr, trow, n, sh, acc);
+        lk_moe_mfma<NP, false>(qs, d, rec, bpr, trow, n, kp, sh.wave[wv], acc);
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < 2; ++j)
@@ -1028,12 +1039,12 @@ extern "C" size_t lk_moe_work_bytes(const lk_moe * moe, int T) {
     return lk_moe_layout(moe, T, nullptr, nullptr);
 }
 
-static bool lk_moe_few(const LkMoeArgs & a) { return a.T <= 5 || (a.T <= LK_MOE_FEW && a.T * a.k <= 16); }
+static bool lk_moe_few(const LkMoeArgs & a, int type) { return a.T <= 5 || (a.T <= LK_MOE_FEW && a.T * a.k <= (type == LK_F32 ? 16 : 28)); }
 
 template <int TYPE>
 static void lk_moe_go(const LkMoeArgs & a, hipStream_t st) {
     constexpr int NP = TYPE == LK_F32 ? 3 : 2;
-    const bool few = lk_moe_few(a);
+    const bool few = lk_moe_few(a, TYPE);
     const int nE = (a.E + 3) / 4, na = a.T * a.k, slots = na < a.E ? na : a.E;
     hipLaunchKernelGGL((lk_k_moe_router<TYPE, NP>), dim3(nE + (a.hidden / 8 + LK_MOE_THREADS - 1) / LK_MOE_THREADS, (a.T + 3) / 4),
                        dim3(LK_MOE_THREADS), 0, st, a, nE);

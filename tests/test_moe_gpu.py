@@ -308,9 +308,9 @@ def test_longest_rows(lk, hidden, ffn, T):
 
 
 @pytest.mark.parametrize("t", TYPES)
-@pytest.mark.parametrize("T,k", [(5, 8), (6, 2), (6, 3), (8, 2), (8, 1), (7, 3), (8, 8)])
+@pytest.mark.parametrize("T,k", [(5, 8), (6, 2), (6, 3), (8, 2), (8, 1), (7, 3), (7, 4), (8, 4), (8, 8)])
 def test_both_sides_of_the_line_between_launches(lk, T, k, t):
-    """Up to 5 tokens or 16 choices in three launches, more in five."""
+    """Up to 5 tokens, or 8 of 28 choices in all (fp32 rows: 16), in three launches, more in five."""
     hidden, ffn, E, dt = 288, 160, 9, TYPES[t]
     L = _layer(60 + T, E, hidden, ffn, bias=k > 2)
     x, res = _x(T, T, hidden, dt), _x(T + 1, T, hidden, dt)
