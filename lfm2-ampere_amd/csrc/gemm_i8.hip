@@ -328,7 +328,7 @@ lk_k_gemm_i8(const LkI8Args a) {
 #pragma unroll
                             for (int e = 0; e < 8; ++e) v[e] = o[e] + v[e];
                         }
-                        lk_store<8>(out + (size_t) t * a.ldo + r, v);
+                        lk_store_nt<8>(out + (size_t) t * a.ldo + r, v);
                     } else {
 #pragma unroll
                         for (int e = 0; e < 8; ++e) if (r + e < a.N) {

@@ -31,6 +31,19 @@ __device__ __forceinline__ void lk_store(T * p, const float (&v)[N]) {
     __builtin_memcpy(p, &b, sizeof b);
 }
 
+// The same, past the caches' order (non-temporal): for outputs that the kernel does not read again,
+// which otherwise wait in the L2s to be written back when it ends.
+template <int N, typename T>
+__device__ __forceinline__ void lk_store_nt(T * p, const float (&v)[N]) {
+    typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(2)));       // the elements' alignment
+    static_assert(N * sizeof(T) % 16 == 0, "whole 16-byte stores");
+    union { T e[N]; u4 q[N * sizeof(T) / 16]; } b;
+#pragma unroll
+    for (int i = 0; i < N; ++i) b.e[i] = (T) v[i];
+#pragma unroll
+    for (int i = 0; i < (int) (N * sizeof(T) / 16); ++i) __builtin_nontemporal_store(b.q[i], (u4 *) p + i);
+}
+
 // ---- reductions over the 64 lanes of a wave, every lane left with the same bits --
 __device__ __forceinline__ float lk_wave_sum(float v) { return lk_xrow_sum(lk_row_sum16(v)); }
 template <int CTRL>
