@@ -100,11 +100,12 @@ lk_k_gemm_i8_few(const LkI8Args a) {
 // its part of every stage, and integer sums have no order.  K in stages of KC bytes, a ring of
 // NB of them in LDS, filled by LDS DMA.
 // What bounds it.  Large: the matrix instructions at the clock that the power leaves: 8192^3 in
-// 440 to 490 us, 2240 to 2500 TOPS, where MFMAs alone, without a load, reach 2630 and the
-// library's int8 product 2090; 4 waves of 4 x 4 tiles, which read less from LDS, 470, a ring of
-// 4 stages of 64 bytes 467 to 498.  4096 x 8192 x 2048, two rounds of tiles: 73 us (1880), of
-// which the outputs, 34 MB of every unit's at once, take 5.7 a round (6 TB/s).  Small: the latency
-// of the ring's start, of a stage and of the launch (333 x 2048 x 2048: 6.4 us).
+// 419 to 484 us, 2270 to 2620 TOPS from card to card, where MFMAs alone, without a load, reach 2630 and the
+// library's int8 product 2090 (earlier: 4 waves of 4 x 4 tiles, which read less from LDS, 470 for
+// 446, a ring of 4 stages of 64 bytes 467 to 498).  4096 x 8192 x 2048, two rounds of tiles: 64
+// to 73 us (1880 to 2150), of which the outputs, 34 MB of every unit's at once, are a part that
+// nothing hides.  Small: the latency of the ring's start, of a stage and of the launch (333 x 2048 x
+// 2048: 5.7 us).
 template <int TM_, int TN_, int WM_, int WN_, int WK_, int KC_, int NB_, int OCC_>
 struct LkI8Shape {
     static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, WK = WK_, KC = KC_, NB = NB_, OCC = OCC_;   // OCC: waves per SIMD
@@ -259,7 +260,10 @@ lk_k_gemm_i8(const LkI8Args a) {
         lk_wait_vm<0>();
         // Outputs by way of LDS, 32 tokens and 32 RS rows of the wave at a time: a lane has token
         // lm and rows 8 * e4 + 4 * h .. +3 of every MFMA tile, 8 bytes of 32 output rows per store;
-        // from LDS it takes 8 consecutive rows of one token, whole runs of 64 * RS bytes (bf16).
+        // from LDS it takes 16 bytes of one token, whole runs of 64 * RS bytes (fp32 128).  They go
+        // past the caches' order, which the L2s need for the operands (4096 x 8192 x 2048 bf16 73 us, so
+        // 67; 2000 x 4096 x 2048 23.5 and 19.5), and 16 bytes of neighbouring lanes side by side (fp32, 32
+        // bytes a lane in two stores: 103 us for 80, and in the caches' order 86).
         // A token's 16-byte pieces are XOR-permuted so that writes and reads use all banks alike.
         constexpr int RS = SH::RS, RW = 32 * RS;
         __syncthreads();
@@ -285,7 +289,7 @@ lk_k_gemm_i8(const LkI8Args a) {
         auto piece = [&](int t, int p) { return st + t * (RW * 4) + (p ^ (RS == 2 ? t & 15 : t >> 1 & 7)) * 16; };
         const T * res = (const T *) a.res;
         T * out = (T *) a.out;
-        constexpr int LT = RW / 8, TP = 64 / LT;             // lanes a token, tokens a step
+        constexpr int VL = 16 / sizeof(T), LT = RW / VL, TP = 64 / LT;       // rows a lane, lanes a token, tokens a step
 #pragma unroll
         for (int i0 = 0; i0 < TM; i0 += RS) {
             float sw[RS][4][4];
@@ -299,7 +303,7 @@ lk_k_gemm_i8(const LkI8Args a) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) sw[i][e4][e] = r + e < a.N ? a.sw[r + e] : 0.0f;
                 }
-            const int r8 = lane % LT, r = row0 + wr + 32 * i0 + 8 * r8;
+            const int rl = lane % LT, r = row0 + wr + 32 * i0 + VL * rl;
 #pragma unroll
             for (int j = 0; j < TN; ++j) {
                 const int t0 = tok0 + wt + 32 * j;           // wave-uniform
@@ -314,24 +318,27 @@ lk_k_gemm_i8(const LkI8Args a) {
                         *(lk_f4 *) piece(lm, 8 * i + 2 * e4 + h) = v;
                     }
                 __builtin_amdgcn_wave_barrier();
+                float vv[32 / TP][VL];                       // all of them asked for before the first is stored
+#pragma unroll
+                for (int k = 0; k < 32 / TP; ++k)
+#pragma unroll
+                    for (int p = 0; p < VL / 4; ++p) *(lk_f4 *) (vv[k] + 4 * p) = *(const lk_f4 *) piece(k * TP + lane / LT, VL / 4 * rl + p);
 #pragma unroll
                 for (int k = 0; k < 32 / TP; ++k) {
-                    const int tl = k * TP + lane / LT, t = t0 + tl;
-                    float v[8];
-                    *(lk_f4 *) v = *(const lk_f4 *) piece(tl, 2 * r8);
-                    *(lk_f4 *) (v + 4) = *(const lk_f4 *) piece(tl, 2 * r8 + 1);
+                    float (&v)[VL] = vv[k];
+                    const int t = t0 + k * TP + lane / LT;
                     if (t >= a.M || r >= a.N) continue;
-                    if (r + 8 <= a.N) {
+                    if (r + VL <= a.N) {
                         if (res) {
-                            float o[8];
-                            lk_load<8>(res + (size_t) t * a.ldr + r, o);
+                            float o[VL];
+                            lk_load<VL>(res + (size_t) t * a.ldr + r, o);
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) v[e] = o[e] + v[e];
+                            for (int e = 0; e < VL; ++e) v[e] = o[e] + v[e];
                         }
-                        lk_store_nt<8>(out + (size_t) t * a.ldo + r, v);
+                        lk_store_nt<VL>(out + (size_t) t * a.ldo + r, v);
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) if (r + e < a.N) {
+                        for (int e = 0; e < VL; ++e) if (r + e < a.N) {
                             float u = v[e];
                             if (res) u = (float) res[(size_t) t * a.ldr + r + e] + u;
                             out[(size_t) t * a.ldo + r + e] = (T) u;

@@ -37,12 +37,23 @@ struct LkNormArgs {
     float eps;
 };
 
+// Rows of h and y, which the next kernel does not need (q it does: with q past the caches' order
+// too, the int8 product that follows lost what was gained and more, 4096 x 2048 x 2048 35.1 us
+// together for 32.5): 16-bit rows go past the caches' order, 4096 x 2048 bf16 11.7 us for 13.0, 1024 x
+// 16384 21.3 for 22.9; fp32 rows gain and lose (4096 x 1024 9.6 for 11.1, 2048 x 8192 38.1 for 35.1)
+// and stay.
+template <typename T>
+__device__ __forceinline__ void lk_norm_store(T * o, const float (&v)[8]) {
+    if constexpr (sizeof(T) == 2) lk_store_nt<8>(o, v);
+    else                          lk_store<8>(o, v);
+}
+
 // NW waves hold a row, 8 consecutive values per lane and chunk, C chunks; a workgroup
 // has 4 waves or one row's, whichever is more.  One pass: the row stays in registers
 // between the sum of squares, the largest value and the quants, and w is asked for along
 // with x and delta.  What bounds it: one row, the launch and one load's latency (2.5 us a
 // call in a graph, 1 x 2048); many rows, memory: 4096 x 2048 with delta and res, bf16, 59 MB
-// in 12.6 us (4.6 TB/s), fp32, 109 MB in 18.2 us (6.0), next to 5.15 TB/s of a 1 GiB copy.
+// in 11.7 us (5.0 TB/s), fp32, 109 MB in 18.2 us (6.0), next to 5.15 TB/s of a 1 GiB copy.
 template <int TYPE, int FORM, int NW, int C>
 __global__ void __launch_bounds__(NW > 4 ? 64 * NW : 256)
 lk_k_norm_q8(const LkNormArgs a) {
@@ -107,7 +118,7 @@ lk_k_norm_q8(const LkNormArgs a) {
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int i = ((c * NW + wr) * 64 + lane) * 8;
-            if (i + 8 <= n) lk_store<8>(o + i, h[c]);
+            if (i + 8 <= n) lk_norm_store(o + i, h[c]);
             else
 #pragma unroll
                 for (int e = 0; e < 8; ++e) if (i + e < n) o[i + e] = (T) h[c][e];
@@ -138,7 +149,7 @@ lk_k_norm_q8(const LkNormArgs a) {
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int i = ((c * NW + wr) * 64 + lane) * 8;
-            if (i + 8 <= n) lk_store<8>(o + i, h[c]);
+            if (i + 8 <= n) lk_norm_store(o + i, h[c]);
             else
 #pragma unroll
                 for (int e = 0; e < 8; ++e) if (i + e < n) o[i + e] = (T) h[c][e];
