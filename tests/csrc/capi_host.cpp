@@ -110,6 +110,8 @@ extern "C" int capi_host_run(const float * q_h, const uint16_t * kc_h, const uin
     const size_t work_bytes = lk_pf_part_bytes();
     void * work = R.alloc<void>(work_bytes);
     REQ(qh && pkc && pvc && k8 && ksc && o[0] && o[1] && work, "hipMalloc (prefill)");
+    // columns P+m .. kstride-1 are padding that nothing writes, and the caller compares them with zeros
+    REQ(hipMemset(ksc, 0, (size_t) (8 * kstride + 4) * sizeof(float)) == hipSuccess, "clear ksc");
     REQ(hipMemcpy(qh, pq_h, (size_t) m * 2048 * 2, hipMemcpyHostToDevice) == hipSuccess, "copy qh");
     REQ(hipMemcpy(pkc, pk_h, (size_t) S * row * 2, hipMemcpyHostToDevice) == hipSuccess, "copy prefill kc");
     REQ(hipMemcpy(pvc, pv_h, (size_t) S * row * 2, hipMemcpyHostToDevice) == hipSuccess, "copy prefill vc");
