@@ -49,7 +49,8 @@ def q8_row_ref(y):
     fin = torch.isfinite(a)
     some = fin & (a >= 2.0 ** -120)
     sc = torch.where(some, a / 127.0, torch.where(fin, 0.0, float("nan")))
-    q = torch.where(some, torch.round(y * (127.0 / a)), torch.zeros_like(y))
+    # a tensor over a tensor: a number over one is its reciprocal, rounded, times the number
+    q = torch.where(some, torch.round(y * (torch.full_like(a, 127.0) / a)), torch.zeros_like(y))
     return q.to(torch.int8), sc[:, 0]
 
 

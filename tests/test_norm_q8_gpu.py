@@ -73,6 +73,12 @@ def test_row_form_at_the_lines_between_launch_shapes(lk, rows, n):
 
 
 @pytest.mark.parametrize("t", TYPES)
+def test_many_rows(lk, t):
+    """Eight million values: those next to a rounding border among them."""
+    test_row_form(lk, 4096, 2048, t)
+
+
+@pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("rows,n", [(1, 32), (5, 64), (3, 2048), (2, 2080), (3, 4128), (1, 8224), (67, 256)])
 def test_q81_forms_are_the_quantisers_bytes(lk, rows, n, t):
     """Planar Q8_1 byte for byte what lk_pf_quant_rows makes of the normed fp32 row,
