@@ -11,8 +11,6 @@
 // of each x row is masked, and 0 times anything is 0.
 #include "lk_types.h"
 
-typedef int lk_i16v __attribute__((ext_vector_type(16)));
-
 // The result of one output: every step rounded as written.
 __device__ __forceinline__ float lk_i8_out(int s, float sx, float sw) {
 #pragma clang fp contract(off)

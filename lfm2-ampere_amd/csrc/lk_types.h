@@ -4,6 +4,8 @@
 #pragma once
 #include "lk_common.h"
 
+typedef int lk_i16v __attribute__((ext_vector_type(16)));                // a tile of v_mfma_i32_32x32x32_i8, a lane's part
+
 // ---- 16- and 32-bit float elements (LK_F32, LK_F16, LK_BF16) --------------------
 template <int TYPE> struct LkElem;
 template <> struct LkElem<LK_F32>  { typedef float type; };

@@ -14,12 +14,15 @@
 //
 // The products are integer dot products (v_dot4_i32_i8): a block of 32 values of x or h
 // becomes whole numbers i = rint(v * 2^p), the largest just inside the range, in NP
-// int8 digits of base 256: three for fp32 rows (24 bits of the block's largest value), two
-// for fp16 and bf16 rows (16 bits).  sum (n - 8) i is exact in int32 digit by digit
+// int8 digits of base 256: four for fp32 rows (32 bits of the block's largest value), three
+// for fp16 and bf16 rows (24 bits).  sum (n - 8) i is exact in int32 digit by digit
 // (-8 * the digits' sum is where the sum starts), the digits are put together and scaled by
 // d * 2^-p in fp32, and blocks are added in fp32.  A block that holds a value
-// that is not finite gets the scale NaN; one whose largest value is under 2^-100 counts as
+// that is not finite gets the scale NaN; one whose largest value is under 2^-96 counts as
 // zero.
+// Why that many: a channel, of x or of h, that is 1000 times the others leaves its 31 neighbours
+// 10 bits fewer.  With a digit less a row whose large channels meet weights of zero
+// was off by 2e-2 to 4e-2 (16-bit rows) and 1.7e-4 (fp32), so 2e-4 and 6e-7.
 #include "lk_types.h"
 
 typedef uint32_t lk_u4 __attribute__((ext_vector_type(4)));
@@ -30,14 +33,14 @@ typedef uint32_t lk_u4 __attribute__((ext_vector_type(4)));
 // adds up (five).  us with three / five launches, bf16 and fp32 rows; the rule (lk_moe_few)
 // takes three for up to 5 tokens, and 8 of up to 28 choices in all (fp32 rows: 16):
 //   tokens                           2        4        5        6        7        8
-//   64 experts, 4 of 2048 x 1536   19/26    27/33    32/33    36/38    41/43    45/43
-//                            fp32  20/26    29/31    33/33    35/34    39/39    40/39
-//   128 experts, 8 of 2048 x 768   21/30    33/37    38/42    43/43    50/49    55/52
-//                            fp32  22/30    34/35    38/38    41/38    44/44    49/45
-//   16 experts, 4 of 1280 x 1184   16/22    20/25    22/25    25/27    27/28    29/28
-//                            fp32  16/22    21/25    23/26    26/26    28/27    31/28
-//   32 experts, 2 of 2048 x 1792   15/22    19/26    23/30    25/32    27/33    31/35
-//                            fp32  15/22    20/27    22/27    23/27    24/28    28/29
+//   64 experts, 4 of 2048 x 1536   20/26    29/32    33/36    37/38    42/41    47/45
+//                            fp32  21/27    29/33    35/37    39/39    44/42    50/47
+//   128 experts, 8 of 2048 x 768   21/30    33/37    37/41    45/44    50/48    55/51
+//                            fp32  22/31    34/38    39/42    46/46    52/50    58/53
+//   16 experts, 4 of 1280 x 1184   17/22    21/26    24/27    25/27    27/28    29/29
+//                            fp32  17/23    22/27    25/28    27/28    30/29    31/30
+//   32 experts, 2 of 2048 x 1792   15/22    20/27    21/28    25/31    27/32    29/34
+//                            fp32  16/23    21/28    22/29    27/32    30/33    32/35
 #define LK_MOE_FEW 8
 #define LK_MOE_THREADS 256
 #define LK_MOE_NW 8                       // waves of a gate/up workgroup for few tokens
@@ -74,21 +77,23 @@ struct LkMoeArgs {
 };
 
 // ---- whole numbers of a block -------------------------------------------------------
-// A block's record: NP planes of 32 int8 digits, highest first, then int32 -8 * sum of
-// each plane (0 for a third of two) and the fp32 scale 2^-p.
+// A block's record: NP planes of 32 int8 digits, highest first, then a piece of int32 -8 * the
+// sums of the planes, two planes put together (the first * 256 + the second; the third of
+// three alone), 0, and the fp32 scale 2^-p.  A plane holds elements 0 .. 7, 16 .. 23, then 8 .. 15, 24
+// .. 31: dwords 2 h, 2 h + 1 of a weight block are the elements of piece h.
 template <int NP>
 struct LkMoeRec {
     static constexpr int PIECES = 2 * NP + 1, BYTES = 16 * PIECES;
 };
 // 2^p for a block whose largest |v| has the bits am; 0 for a block of zeros and for one
-// that is not finite.  The digits reach 127 * (1 + 256 (+ 65536)): the largest value
+// that is not finite.  The digits reach 127 * (1 + 256 + 65536 (+ 2^24)): the largest value
 // goes to the top binade where its leading bits allow, else one below.
 template <int NP>
 __device__ __forceinline__ float lk_moe_up2(uint32_t am) {
-    constexpr float TOP = NP == 3 ? 8355711.0f : 32639.0f;
-    constexpr int B = NP == 3 ? 22 : 14;
-    if (am >= 0x7F800000u || am < (27u << 23)) return 0.0f;                       // not finite; under 2^-100
-    // 2^(B - E), E the exponent of am: between 2^(B - 127) and 2^(B + 100)
+    constexpr float TOP = NP == 4 ? 2139062016.0f : 8355711.0f;                   // 24 bits of the four digits' end
+    constexpr int B = NP == 4 ? 30 : 22;
+    if (am >= 0x7F800000u || am < (31u << 23)) return 0.0f;                       // not finite; under 2^-96
+    // 2^(B - E), E the exponent of am: between 2^(B - 127) and 2^(B + 96), and its inverse is normal too
     const float f = __builtin_bit_cast(float, (uint32_t) (B + 254 - (int) (am >> 23)) << 23);
     return __builtin_bit_cast(float, am) * f > TOP ? 0.5f * f : f;
 }
@@ -144,6 +149,7 @@ __device__ __forceinline__ int lk_moe_sum32(int v) {
     v += (int) lk_dpp_u<LK_DPP_QP_XOR1>((uint32_t) v);
     return v;
 }
+__device__ __forceinline__ constexpr int lk_moe_place(int i) { return 16 * (i / 8 % 2) + 8 * (i / 16) + i % 8; }    // of element i
 // The record of a block whose 32 values h lie on the 32 lanes of a half-wave (r: the
 // lane's place); nothing is stored where !ok.
 template <int NP>
@@ -153,15 +159,12 @@ __device__ __forceinline__ void lk_moe_record(float h, int r, bool ok, uint8_t *
     const float up = lk_moe_up2<NP>(am);
     int q[NP];
     lk_moe_digits<NP>(h, up, q);
-    // two sums at once: each is at most 32 * 128
-    const int s01 = lk_moe_sum32(q[0] * 65536 + q[1]), s1 = (int) (short) s01, s0 = (s01 - s1) >> 16;
-    int s2 = 0;
-    if constexpr (NP == 3) s2 = lk_moe_sum32(q[2]);
+    const int s01 = lk_moe_sum32(q[0] * 256 + q[1]), s23 = lk_moe_sum32(NP == 4 ? q[2] * 256 + q[NP - 1] : q[2]);
     if (!ok) return;
 #pragma unroll
-    for (int p = 0; p < NP; ++p) rec[32 * p + r] = (uint8_t) q[p];
+    for (int p = 0; p < NP; ++p) rec[32 * p + lk_moe_place(r)] = (uint8_t) q[p];
     if (r == 0)
-        *(lk_i4 *) (rec + 32 * NP) = lk_i4{ -8 * s0, -8 * s1, -8 * s2, __builtin_bit_cast(int, lk_moe_scale(am, up)) };
+        *(lk_i4 *) (rec + 32 * NP) = lk_i4{ -8 * s01, -8 * s23, 0, __builtin_bit_cast(int, lk_moe_scale(am, up)) };
 }
 
 // ---- router scores, and the records of x -------------------------------------------
@@ -226,7 +229,7 @@ lk_k_moe_router(const LkMoeArgs a, int nE) {
         am = lk_umax(am, lk_dpp_u<LK_DPP_QP_XOR2>(am));
         const float up = lk_moe_up2<NP>(am);
         uint32_t w[NP][2] = {};
-        int s[3] = { 0, 0, 0 };
+        int s[2] = { 0, 0 };
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             int q[NP];
@@ -234,20 +237,20 @@ lk_k_moe_router(const LkMoeArgs a, int nE) {
 #pragma unroll
             for (int p = 0; p < NP; ++p) {
                 w[p][j / 4] |= (uint32_t) (uint8_t) q[p] << (8 * (j % 4));
-                s[p] += q[p];
+                s[p / 2] += p == 0 || (NP == 4 && p == 2) ? q[p] * 256 : q[p];
             }
         }
 #pragma unroll
-        for (int p = 0; p < NP; ++p) {
+        for (int p = 0; p < 2; ++p) {
             s[p] += (int) lk_dpp_u<LK_DPP_QP_XOR1>((uint32_t) s[p]);
             s[p] += (int) lk_dpp_u<LK_DPP_QP_XOR2>((uint32_t) s[p]);
         }
         if (!ok) continue;
         uint8_t * r = a.xr + ((size_t) t * bpr + b) * REC;
 #pragma unroll
-        for (int p = 0; p < NP; ++p) *(uint2 *) (r + 32 * p + 8 * g) = make_uint2(w[p][0], w[p][1]);
+        for (int p = 0; p < NP; ++p) *(uint2 *) (r + 32 * p + lk_moe_place(8 * g)) = make_uint2(w[p][0], w[p][1]);
         if (g == 0)
-            *(lk_i4 *) (r + 32 * NP) = lk_i4{ -8 * s[0], -8 * s[1], -8 * s[2], __builtin_bit_cast(int, lk_moe_scale(am, up)) };
+            *(lk_i4 *) (r + 32 * NP) = lk_i4{ -8 * s[0], -8 * s[1], 0, __builtin_bit_cast(int, lk_moe_scale(am, up)) };
     }
 }
 
@@ -411,32 +414,51 @@ lk_k_moe_route(const LkMoeArgs a) {
 // 4 GiB (LK_MOE_MAX_DIM).
 template <typename V>
 __device__ __forceinline__ V lk_moe_ld(const void * base, uint32_t off) { return *(const V *) ((const char *) base + off); }
+// The digits' sums of a block put together: two at a time exactly (below 2^24, or 16 times
+// that where all are multiples of 16), and one rounding.
+template <int NP, typename V>
+__device__ __forceinline__ float lk_moe_digits_sum(const V & s) {
+    const float f = (float) (s[0] * 256 + s[1]);
+    return NP == 4 ? __builtin_fmaf(f, 65536.0f, (float) (s[2] * 256 + s[3])) : __builtin_fmaf(f, 256.0f, (float) s[2]);
+}
 // A block's record x times the lane's block of NM weight rows (its 32 nibbles: lo, hi).
 template <int NP, int NM>
 __device__ __forceinline__ void lk_moe_token_dots(const lk_u4 * x, bool in, const uint32_t (&lo)[NM][4], const uint32_t (&hi)[NM][4],
                                                   const float (&dv)[NM], float (&acc)[NM]) {
-    lk_u4 q[2 * NP];
-#pragma unroll
-    for (int p = 0; p < 2 * NP; ++p) q[p] = x[p];
     const lk_i4 meta = __builtin_bit_cast(lk_i4, x[2 * NP]);
     const int m3 = meta[3];                              // a copy: bit_cast of a vector's element takes element 0
     const float sc = in ? __builtin_bit_cast(float, m3) : 0.0f;                    // a block past the row's end counts nothing
+    // of four planes two at a time: all their digits take 32 registers (1 token fp32 15.9 us, so 15.3; three
+    // planes in two steps 15.2, at once 14.8)
+    constexpr int P = NP == 4 ? 2 : NP;
+    int s[NP][NM];
+#pragma unroll
+    for (int a = 0; a < NP; a += P) {
+        lk_u4 q[2 * P];
+#pragma unroll
+        for (int i = 0; i < 2 * P; ++i) q[i] = x[2 * a + i];
+#pragma unroll
+        for (int m = 0; m < NM; ++m)
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                int v = a + p == 1 ? meta[0] : a + p == NP - 1 ? meta[1] : 0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    v = __builtin_amdgcn_sdot4((int) lo[m][k], (int) q[2 * p + k / 2][k % 2], v, false);
+                    v = __builtin_amdgcn_sdot4((int) hi[m][k], (int) q[2 * p + k / 2][2 + k % 2], v, false);
+                }
+                s[a + p][m] = v;                         // at most 32 * 8 * 128 = 2^15 without meta
+            }
+        // done here: left to itself the compiler reads the digits of all tokens first and spills
+#pragma unroll
+        for (int m = 0; m < NM; ++m)
+#pragma unroll
+            for (int p = 0; p < P; ++p) asm volatile("" : "+v"(s[a + p][m]) :: "memory");
+    }
 #pragma unroll
     for (int m = 0; m < NM; ++m) {
-        int s[NP];
-#pragma unroll
-        for (int p = 0; p < NP; ++p) {
-            s[p] = meta[p];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                s[p] = __builtin_amdgcn_sdot4((int) lo[m][k], (int) q[2 * p][k], s[p], false);
-                s[p] = __builtin_amdgcn_sdot4((int) hi[m][k], (int) q[2 * p + 1][k], s[p], false);
-            }
-        }
-        float f = (float) (s[0] * 256 + s[1]);           // a digit's sum is at most 32 * 8 * 128 = 2^15
-        if constexpr (NP == 3) f = __builtin_fmaf(f, 256.0f, (float) s[2]);
-        acc[m] = __builtin_fmaf(dv[m] * sc, f, acc[m]);
-        // done here: left to itself the compiler reads the digits of all tokens first and spills
+        const int s4[4] = { s[0][m], s[1][m], s[2][m], s[NP - 1][m] };
+        acc[m] = __builtin_fmaf(dv[m] * sc, lk_moe_digits_sum<NP>(s4), acc[m]);
         asm volatile("" : "+v"(acc[m]) :: "memory");
     }
 }
@@ -525,26 +547,28 @@ __device__ __forceinline__ void lk_moe_up_rows(const LkMoeArgs & a, int e, int h
 // (four matrices of 8 rows) and every second step of 8 blocks of K; it copies a step's
 // digits into its own part of LDS while the step's weights are on their way, which are
 // asked for before the products of the step before.
-// One assignment: the dots above.  More: v_mfma_i32_16x16x32_i8, a block of 16 weight
-// rows (the second operand) against the digits of TG assignments (the first: NP = 2, row 2 t +
-// p is digit p of t; NP = 3, row 4 t + p, and p = 3 the last digit again), for which the
-// weights go by way of LDS: they come as whole blocks a lane, and lane (row l % 16, g =
-// l / 16) multiplies dword g of a block, nibbles as 16 (n - 8).  The products of 8
-// assignments cost a wave about 13 vector operations for 16 rows of a block and of one
-// assignment 20 as dots, so that they pay from two on: 19 tokens 61 us with dots up to two,
-// 58 up to one, 62 without; 64 tokens (four an expert) 97, 92, 92; dots alone 65 and 112.
-// Bound by memory: 64 tokens at 64 experts read 226 MB (gate, up) in 49 us and 113 MB in 26, 4.9
-// TB/s less the launch (a 1 GiB copy 5.15), and not a byte twice (counters: 209 and 108 MB; the rest
-// is in the cache).
-template <int NP>
+// One assignment: the dots above.  More: v_mfma_i32_32x32x32_i8, a block of 32 weight rows (the
+// second operand) against the digits of TG assignments (the first: row 4 t + p is digit p of
+// t; of three, p = 3 is the last digit again), for which the weights go by way of LDS: they
+// come as whole blocks a lane, and lane (row l % 32, h = l / 32) multiplies dwords 2 h and 2 h + 1 of a
+// block, nibbles as 16 (n - 8).  It pays from two assignments on: with matrix instructions for one as
+// well 12 tokens 59.3 us for 53.3, 19 tokens 74.0 for 71.0, 64 tokens (four an expert) 105.9 for 106.2.
+// TG: what LDS holds of four workgroups a unit.  16-bit rows (three digits) with TG 4, 6, 8 (8: three
+// workgroups): 12 tokens 52.6, 52.8, 55.4, 19 tokens 70.7, 70.8, 72.4, 48 tokens 105, 96, 99, 64 tokens 122,
+// 106, 105; fp32 rows (four digits) with 4 and 8 (two workgroups): 19 tokens 72.7, 83.5, 64 tokens 129, 130.
+// Bound by memory: 64 tokens at 64 experts, bf16, read 226 MB (gate, up) in 54.7 us and 113 MB in 28.2, 4.1
+// TB/s (a 1 GiB copy 5.15); about a tenth is the third digit's, its copies and products (with two
+// digits, which do not hold enough, 50.0 and 26.4).
+template <int NP, int TG_>
 struct LkMoeShare {
-    static constexpr int Z = 8 * LkMoeRec<NP>::PIECES;   // pieces of a step's digits
-    static constexpr int TG = NP == 2 ? 8 : 4;
+    static constexpr int Z = 8 * LkMoeRec<NP>::PIECES, NZ = (Z + 63) / 64;      // pieces of a step's digits
+    static constexpr int TG = TG_;                       // assignments at a time
     // the digits of assignment t, so far apart that the 16 rows' reads use all banks alike
-    static __device__ __forceinline__ constexpr int at(int t) { return t * Z + 4 * (t / 2); }
+    static __device__ __forceinline__ constexpr int at(int t) { return t * Z + t / 2; }
     struct Wave {
-        lk_u4 x[TG * Z + 4 * ((TG - 1) / 2)];
-        lk_u4 w[32][8];                                  // rows' blocks, block b of row r in slot b ^ r / 2 % 8
+        lk_u4 x[TG * Z + (TG - 1) / 2];
+        lk_u4 w[32][8];                                  // rows' blocks, block b of row r in slot b ^ r / 2 % 8; of rows 16 .. 31
+                                                         // the halves changed over, so that 32 lanes' reads use all banks
         lk_u4 d[32];                                     // their scales
     };
     union {
@@ -552,14 +576,13 @@ struct LkMoeShare {
         float part[2][TG][64];                           // [part of K][assignment][row of 32 gate and 32 up, or of 64]
     };
 };
-template <int NP>
+template <int NP, int TG>
 __device__ __forceinline__ void lk_moe_many_dots(const uint8_t * const (&qs)[4], const _Float16 * const (&d)[4], const uint8_t * rec,
-                                                 int bpr, int trow, LkMoeShare<NP> & sh, float (&acc)[4]) {
-    constexpr int PC = LkMoeRec<NP>::PIECES, Z = LkMoeShare<NP>::Z;
-    static_assert(Z <= 64, "a step's digits are one copy");
+                                                 int bpr, int trow, LkMoeShare<NP, TG> & sh, float (&acc)[4]) {
+    constexpr int PC = LkMoeRec<NP>::PIECES, Z = LkMoeShare<NP, TG>::Z, NZ = LkMoeShare<NP, TG>::NZ;
     const int lane = threadIdx.x & 63, c = lane >> 3, g = lane & 7, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ns = (bpr + 7) / 8;                        // steps; this wave's are s0, s0 + 2, ...
-    typename LkMoeShare<NP>::Wave & me = sh.wave[wv];
+    typename LkMoeShare<NP, TG>::Wave & me = sh.wave[wv];
     const uint32_t lds = lk_lds_addr(me.x);
     lk_u4 w[4];
     _Float16 dw[4];
@@ -576,7 +599,11 @@ __device__ __forceinline__ void lk_moe_many_dots(const uint8_t * const (&qs)[4],
     auto copy = [&](int s) {
         const int left = (bpr - 8 * s) * PC;             // pieces to the row's end; none: the row's first
         const uint8_t * src = rec + ((size_t) trow * bpr + (left > 0 ? 8 * s : 0)) * (PC * 16);
-        if (lane < Z) lk_dma16c_so(src, 16u * (lane < left ? lane : 0), lds);
+#pragma unroll
+        for (int z = 0; z < NZ; ++z) {
+            const int i = 64 * z + lane;
+            if (i < Z) lk_dma16c_so(src, 16u * (i < left ? i : 0), lds + 1024u * z);
+        }
     };
     load(wv >> 1);
     copy(wv >> 1);
@@ -605,23 +632,22 @@ __device__ __forceinline__ void lk_moe_many_dots(const uint8_t * const (&qs)[4],
 }
 
 // The same for n of up to TG assignments, over the steps s0, s0 + 2, ..., or of PAIRS, s0, s0 + 1, s0 + 8,
-// s0 + 9, ....  sum[j][q]: 16 rows of matrices 2 j and 2 j + 1, row l %
-// 16; assignment 2 (l / 16) + q of two digits, l / 16 of three.  The blocks of a step are summed
-// apart over the steps and joined as the dots' lanes are, so that a token's result does not
-// depend, by a bit, on how many others chose its expert.
-template <int NP, bool PAIRS>
-__device__ __forceinline__ void lk_moe_mfma(const uint8_t * const (&qs)[4], const _Float16 * const (&d)[4], const uint8_t * rec,
-                                                 int bpr, const int (&trow)[LkMoeShare<NP>::TG], int n, int s0, typename LkMoeShare<NP>::Wave & me,
-                                            float (&sum)[2][4 - NP]) {
-    constexpr int PC = LkMoeRec<NP>::PIECES, Z = LkMoeShare<NP>::Z, TG = LkMoeShare<NP>::TG, NQ = 4 - NP;
+// s0 + 9, ....  sum[i]: the 32 rows of the four matrices, row l % 32; assignment 2 i + l / 32.  The
+// blocks of a step are summed apart over the steps and joined as the dots' lanes are, so that a
+// token's result does not depend, by a bit, on how many others chose its expert.
+template <bool PAIRS, int NP, int TG>
+__device__ __forceinline__ void lk_moe_mfma(const uint8_t * const (&qs)[4], const _Float16 * const (&d)[4], const uint8_t * rec, int bpr,
+                                            const int (&trow)[TG], int n, int s0, typename LkMoeShare<NP, TG>::Wave & me, float (&sum)[TG / 2]) {
+    typedef LkMoeShare<NP, TG> Share;
+    constexpr int PC = LkMoeRec<NP>::PIECES, Z = Share::Z, NZ = Share::NZ, NE = TG / 2;
     const int lane = threadIdx.x & 63, c = lane >> 3, g = lane & 7;
-    const int r = lane & 15, h = lane >> 4, ns = (bpr + 7) / 8;
+    const int r = lane & 31, h = lane >> 5, ns = (bpr + 7) / 8;
     const uint32_t lds = lk_lds_addr(me.x);
-    const int t = NP == 2 ? r >> 1 : r >> 2, p = NP == 2 ? r & 1 : (r & 3) < 3 ? r & 3 : 2;
-    const uint32_t * xa = (const uint32_t *) (me.x + LkMoeShare<NP>::at(t) + 2 * p) + h;   // + 4 PC b: the row's digits 4 h ..; 16 + 4 h .. behind 4
-    const float * xs[NQ];                                // + 4 PC b: the scales
+    const int p = (r & 3) < NP ? r & 3 : NP - 1;
+    const lk_i4 * xa = (const lk_i4 *) (me.x + Share::at(r / 4 % TG) + 2 * p + h);       // + PC b: the row's digits
+    const float * xs[NE];                                // + 4 PC b: the scales
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) xs[q] = (const float *) (me.x + LkMoeShare<NP>::at(NQ * h + q) + 2 * NP) + 3;
+    for (int e = 0; e < NE; ++e) xs[e] = (const float *) (me.x + Share::at(2 * e + h) + 2 * NP) + 3;
     lk_u4 w[4];
     _Float16 dw[4];
     auto load = [&](int s) {
@@ -640,11 +666,15 @@ __device__ __forceinline__ void lk_moe_mfma(const uint8_t * const (&qs)[4], cons
         for (int t = 0; t < TG; ++t) {
             if (t >= n) break;
             const uint8_t * src = rec + ((size_t) trow[t] * bpr + 8 * s) * (PC * 16);
-            if (lane < Z && lane < left) lk_dma16c_so(src, 16u * lane, lds + 16u * LkMoeShare<NP>::at(t));
-            if (left < Z && lane >= left && lane < Z) me.x[LkMoeShare<NP>::at(t) + lane] = lk_u4{ 0, 0, 0, 0 };
+#pragma unroll
+            for (int z = 0; z < NZ; ++z) {
+                const int i = 64 * z + lane;
+                if (i < Z && i < left) lk_dma16c_so(src, 16u * i, lds + 16u * Share::at(t) + 1024u * z);
+                if (left < Z && i >= left && i < Z) me.x[Share::at(t) + i] = lk_u4{ 0, 0, 0, 0 };
+            }
         }
     };
-    float acc[8][2][NQ] = {};
+    float acc[8][NE] = {};
     auto next = [](int s) { return !PAIRS ? s + 2 : s & 1 ? s + 7 : s + 1; };
     load(s0);
     copy(s0);
@@ -654,74 +684,65 @@ __device__ __forceinline__ void lk_moe_mfma(const uint8_t * const (&qs)[4], cons
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // the copies; the weights, asked for before, come with them
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-            me.w[8 * m + c][g ^ (4 * (m & 1) + (c >> 1))] = w[m];
+            me.w[8 * m + c][g ^ (4 * (m & 1) + (c >> 1))] = m < 2 ? w[m] : lk_u4{ w[m][2], w[m][3], w[m][0], w[m][1] };
             ((_Float16 *) &me.d[8 * m + c])[g] = in ? dw[m] : (_Float16) 0.0f;
         }
         __builtin_amdgcn_wave_barrier();
         load(next(s));                                   // past the last: in bounds, not used
-        union { lk_u4 q; _Float16 h[8]; } dv[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) dv[j].q = me.d[16 * j + r];
-        uint64_t xd[2];
-        float sc[2][NQ];
-        uint32_t v[2][2];
+        union { lk_u4 q; _Float16 h[8]; } dv;
+        dv.q = me.d[r];
+        lk_i4 x[2];
+        float sc[2][NE];
+        uint64_t v[2];
         auto read = [&](int b) {
-            xd[b & 1] = xa[4 * PC * b] | (uint64_t) xa[4 * PC * b + 4] << 32;
+            x[b & 1] = xa[PC * b];
 #pragma unroll
-            for (int q = 0; q < NQ; ++q) sc[b & 1][q] = xs[q][4 * PC * b];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) v[b & 1][j] = ((const uint32_t *) &me.w[16 * j + r][b ^ (r >> 1)])[h];
+            for (int e = 0; e < NE; ++e) sc[b & 1][e] = xs[e][4 * PC * b];
+            v[b & 1] = ((const uint64_t *) &me.w[r][b ^ (r >> 1 & 7)])[h ^ r >> 4];
         };
         read(0);
 #pragma unroll
         for (int b = 0; b < 8; ++b) {                    // a block's operands are read before the products of the one before
             if (b < 7) read(b + 1);
             asm volatile("" ::: "memory");
+            const uint32_t u0 = (uint32_t) v[b & 1], u1 = (uint32_t) (v[b & 1] >> 32);
+            const lk_i4 wv = { (int) ((u0 << 4 & 0xF0F0F0F0u) ^ 0x80808080u), (int) ((u1 << 4 & 0xF0F0F0F0u) ^ 0x80808080u),
+                               (int) ((u0 & 0xF0F0F0F0u) ^ 0x80808080u), (int) ((u1 & 0xF0F0F0F0u) ^ 0x80808080u) };
+            lk_i16v zero = {};
+            const lk_i16v sv = __builtin_amdgcn_mfma_i32_32x32x32_i8(x[b & 1], wv, zero, 0, 0, 0);
+            const float dd = (float) dv.h[b] * 0.0625f;  // the nibbles are 16 times theirs
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const uint32_t u = v[b & 1][j], lo = (u << 4 & 0xF0F0F0F0u) ^ 0x80808080u, hi = (u & 0xF0F0F0F0u) ^ 0x80808080u;
-                const lk_i4 s4 = __builtin_amdgcn_mfma_i32_16x16x32_i8((long) xd[b & 1], (long) (lo | (uint64_t) hi << 32),
-                                                                       lk_i4{ 0, 0, 0, 0 }, 0, 0, 0);
-                const float dd = (float) dv[j].h[b] * 0.0625f;       // the nibbles are 16 times theirs
-                if constexpr (NP == 2) {                 // a digit's sum is at most 32 * 128 * 128 = 2^19
-                    acc[b][j][0] = __builtin_fmaf(dd * sc[b & 1][0], (float) (s4[0] * 256 + s4[1]), acc[b][j][0]);
-                    acc[b][j][1] = __builtin_fmaf(dd * sc[b & 1][1], (float) (s4[2] * 256 + s4[3]), acc[b][j][1]);
-                } else {
-                    const float f = __builtin_fmaf((float) (s4[0] * 256 + s4[1]), 256.0f, (float) s4[2]);
-                    acc[b][j][0] = __builtin_fmaf(dd * sc[b & 1][0], f, acc[b][j][0]);
-                }
+            for (int e = 0; e < NE; ++e) {
+                if (2 * e >= n) break;                   // wave-uniform
+                // a plane's products: at most 32 * 128 * 128 = 2^19
+                const int s4[4] = { sv[4 * e], sv[4 * e + 1], sv[4 * e + 2], sv[4 * e + 3] };
+                acc[b][e] = __builtin_fmaf(dd * sc[b & 1][e], lk_moe_digits_sum<NP>(s4), acc[b][e]);
             }
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int q = 0; q < NQ; ++q) asm volatile("" : "+v"(acc[b][j][q]) :: "memory");
+            for (int e = 0; e < NE; ++e) asm volatile("" : "+v"(acc[b][e]) :: "memory");
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");          // the digits have been read
         copy(next(s));
     }
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int q = 0; q < NQ; ++q)
-            sum[j][q] = ((acc[0][j][q] + acc[1][j][q]) + (acc[2][j][q] + acc[3][j][q])) +
-                        ((acc[4][j][q] + acc[5][j][q]) + (acc[6][j][q] + acc[7][j][q]));
+    for (int e = 0; e < NE; ++e)
+        sum[e] = ((acc[0][e] + acc[1][e]) + (acc[2][e] + acc[3][e])) + ((acc[4][e] + acc[5][e]) + (acc[6][e] + acc[7][e]));
 }
 
 // 32 rows of one expert's gate and up products for n of its assignments (as, in LDS; the only one:
 // as0), all in all `of` them, and what follows: the records of h.  Wave w has half w & 1 of the rows
 // and of K the pairs of steps w >> 1, + 4, ...  One assignment by dots, more by matrix instructions;
-// both add the blocks in the same order.  (Dots for up to four at a time: 4 tokens, 4 of 64 experts, 30
-// us, so 27; 5 tokens, all of 8 experts of two each, 24 and 22.)
+// both add the blocks in the same order.
 template <int NP>
 struct LkMoeUp {
-    static constexpr int U = 2, TG = LkMoeShare<NP>::TG;
+    static constexpr int U = 2, TG = 4;
     struct One {
         LkMoeX<NP, U> xs[LK_MOE_NW][1];
         float part[LK_MOE_NW / 2][64];                   // [part of K][row of 32 gate and 32 up]
     };
     union {
         One one;
-        typename LkMoeShare<NP>::Wave wave[LK_MOE_NW];
+        typename LkMoeShare<NP, TG>::Wave wave[LK_MOE_NW];
         float part[LK_MOE_NW / 2][TG][64];               // of more: [part of K][assignment][row], where the digits were
     };
 };
@@ -742,17 +763,14 @@ __device__ __forceinline__ void lk_moe_up_few(const LkMoeArgs & a, int e, const 
             if (g == m) sh.one.part[kp][32 * (m >> 1) + 16 * half + 8 * (m & 1) + c] = v;
         }
     } else {
-        constexpr int NQ = 4 - NP;
         int trow[TG];
 #pragma unroll
         for (int t = 0; t < TG; ++t) trow[t] = lk_moe_token(a, __builtin_amdgcn_readfirstlane(as[t < n ? t : 0]));
-        float acc[2][NQ];
-        lk_moe_mfma<NP, true>(qs, d, a.xr, a.hidden / 32, trow, n, 2 * kp, sh.wave[wv], acc);
+        float acc[TG / 2];
+        lk_moe_mfma<true, NP, TG>(qs, d, a.xr, a.hidden / 32, trow, n, 2 * kp, sh.wave[wv], acc);
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int q = 0; q < NQ; ++q) sh.part[kp][NQ * (lane >> 4) + q][32 * j + 16 * half + (lane & 15)] = acc[j][q];
+        for (int i = 0; i < TG / 2; ++i) sh.part[kp][2 * i + (lane >> 5)][2 * (lane & 16) + 16 * half + (lane & 15)] = acc[i];
     }
     __syncthreads();
     const int t = tid >> 5, r = tid & 31;
@@ -819,14 +837,14 @@ lk_k_moe_up_few(const LkMoeArgs a) {
 
 // n of up to TG assignments (as, the rows of records trow) of an expert: the sums of the
 // workgroup's 64 rows over each part of K, into sh.part.
-template <int NP, bool UP>
+template <bool UP, int NP, int TG>
 __device__ __forceinline__ void lk_moe_many_part(const uint8_t * const (&qs)[4], const _Float16 * const (&d)[4], const uint8_t * rec,
-                                                 int bpr, const int (&trow)[LkMoeShare<NP>::TG], int n, LkMoeShare<NP> & sh) {
+                                                 int bpr, const int (&trow)[TG], int n, LkMoeShare<NP, TG> & sh) {
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = wv & 1, kp = wv >> 1;
     if (n == 1) {
         const int c = lane >> 3, g = lane & 7;
         float acc[4] = {};
-        lk_moe_many_dots<NP>(qs, d, rec, bpr, trow[0], sh, acc);
+        lk_moe_many_dots<NP, TG>(qs, d, rec, bpr, trow[0], sh, acc);
         __syncthreads();                                 // part lies where the digits were
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
@@ -834,21 +852,17 @@ __device__ __forceinline__ void lk_moe_many_part(const uint8_t * const (&qs)[4],
             if (g == m) sh.part[kp][0][UP ? 32 * (m >> 1) + 16 * half + 8 * (m & 1) + c : 32 * half + 8 * m + c] = v;
         }
     } else {
-        constexpr int NQ = 4 - NP;
-        float acc[2][NQ];
-        lk_moe_mfma<NP, false>(qs, d, rec, bpr, trow, n, kp, sh.wave[wv], acc);
+        float acc[TG / 2];
+        lk_moe_mfma<false, NP, TG>(qs, d, rec, bpr, trow, n, kp, sh.wave[wv], acc);
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int q = 0; q < NQ; ++q)
-                sh.part[kp][NQ * (lane >> 4) + q][(UP ? 32 * j + 16 * half : 32 * half + 16 * j) + (lane & 15)] = acc[j][q];
+        for (int i = 0; i < TG / 2; ++i)
+            sh.part[kp][2 * i + (lane >> 5)][UP ? 2 * (lane & 16) + 16 * half + (lane & 15) : 32 * half + (lane & 31)] = acc[i];
     }
     __syncthreads();
 }
-template <int NP>
-__device__ __forceinline__ void lk_moe_up_many(const LkMoeArgs & a, int e, const int (&as)[LkMoeShare<NP>::TG], int n, LkMoeShare<NP> & sh) {
-    constexpr int TG = LkMoeShare<NP>::TG;
+template <int NP, int TG>
+__device__ __forceinline__ void lk_moe_up_many(const LkMoeArgs & a, int e, const int (&as)[TG], int n, LkMoeShare<NP, TG> & sh) {
     const int F = a.ffn, tid = threadIdx.x;
     const uint8_t * qs[4];
     const _Float16 * d[4];
@@ -856,7 +870,7 @@ __device__ __forceinline__ void lk_moe_up_many(const LkMoeArgs & a, int e, const
     int trow[TG];
 #pragma unroll
     for (int t = 0; t < TG; ++t) trow[t] = lk_moe_token(a, as[t]);
-    lk_moe_many_part<NP, true>(qs, d, a.xr, a.hidden / 32, trow, n, sh);
+    lk_moe_many_part<true, NP, TG>(qs, d, a.xr, a.hidden / 32, trow, n, sh);
     const int t = tid >> 5, r = tid & 31;
     if (t < n) {                                         // whole halves of waves
         const float gt = sh.part[0][t][r] + sh.part[1][t][r], up = sh.part[0][t][32 + r] + sh.part[1][t][32 + r];
@@ -866,8 +880,8 @@ __device__ __forceinline__ void lk_moe_up_many(const LkMoeArgs & a, int e, const
         lk_moe_record<NP>(lk_moe_h(gt, up), r, true, a.hr + ((size_t) at * (F / 32) + blockIdx.x) * LkMoeRec<NP>::BYTES);
     }
 }
-template <int NP>
-__device__ __forceinline__ void lk_moe_down_many(const LkMoeArgs & a, int e, const int (&as)[LkMoeShare<NP>::TG], int n, LkMoeShare<NP> & sh) {
+template <int NP, int TG>
+__device__ __forceinline__ void lk_moe_down_many(const LkMoeArgs & a, int e, const int (&as)[TG], int n, LkMoeShare<NP, TG> & sh) {
     const int bpr = a.ffn / 32, H = a.hidden, r0 = blockIdx.x * 64, tid = threadIdx.x, lane = tid & 63;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), half = wv & 1;
     const uint8_t * qs[4];
@@ -878,23 +892,22 @@ __device__ __forceinline__ void lk_moe_down_many(const LkMoeArgs & a, int e, con
         qs[m] = a.qs[2] + row * bpr * 16;
         d[m] = a.d[2] + row * bpr;
     }
-    lk_moe_many_part<NP, false>(qs, d, a.hr, bpr, as, n, sh);
+    lk_moe_many_part<false, NP, TG>(qs, d, a.hr, bpr, as, n, sh);
 #pragma unroll
-    for (int t = 0; t < LkMoeShare<NP>::TG; ++t)         // a wave per assignment
+    for (int t = 0; t < TG; ++t)         // a wave per assignment
         if ((t & 3) == wv && t < n && r0 + lane < H)
             a.y[(size_t) as[t] * H + r0 + lane] = sh.part[0][t][lane] + sh.part[1][t][lane];
 }
 
 // grid (row tiles, slots, groups of TG assignments that an expert may have).  An expert of many
 // assignments has a workgroup for each group, which finds the weights in the cache: 64 tokens, all 8
-// experts of 2048 x 768 chosen, 58 us, fp32 rows 74, where the same workgroup took group after group
-// in 112 and 162; 64 experts, 4 of 2048 x 1536 chosen, 98.5 and 112 for 99.2 and 141: the workgroups of
-// groups that an expert has not got cost less than they save.
-template <int NP, bool UP>
+// experts of 2048 x 768 chosen, 62 us, fp32 rows 76 (one workgroup for all groups of an expert, when
+// rows had a digit less: 112 for 58 and 162 for 74).  The workgroups of groups that an expert has not
+// got cost less than they save.
+template <int NP, int TG, bool UP>
 __global__ void __launch_bounds__(LK_MOE_THREADS, 4)
 lk_k_moe_many(const LkMoeArgs a) {
-    constexpr int TG = LkMoeShare<NP>::TG;
-    __shared__ LkMoeShare<NP> sh;
+    __shared__ LkMoeShare<NP, TG> sh;
     // written by the launch before: read as constants, by scalar loads
     typedef const __attribute__((address_space(4))) LkMoeTab Tab;
     Tab & tab = *(Tab *) (uintptr_t) a.tab;
@@ -903,8 +916,8 @@ lk_k_moe_many(const LkMoeArgs a) {
     int as[TG];
 #pragma unroll
     for (int t = 0; t < TG; ++t) as[t] = tab.list[slot][at + (t < n ? t : 0)];
-    if constexpr (UP) lk_moe_up_many<NP>(a, e, as, n, sh);
-    else              lk_moe_down_many<NP>(a, e, as, n, sh);
+    if constexpr (UP) lk_moe_up_many<NP, TG>(a, e, as, n, sh);
+    else              lk_moe_down_many<NP, TG>(a, e, as, n, sh);
 }
 
 // A few tokens: a workgroup of 16 waves has 8 rows of every expert that was
@@ -1017,7 +1030,7 @@ static int lk_moe_check(const lk_moe * m) {
 // The workspace's parts, every one at a multiple of 16 bytes.
 static size_t lk_moe_layout(const lk_moe * m, int T, void * work, LkMoeArgs * a) {
     size_t at = 0;
-    const size_t k = m->top_k, H = m->hidden, F = m->ffn, REC = LkMoeRec<3>::BYTES;        // of two digits: less
+    const size_t k = m->top_k, H = m->hidden, F = m->ffn, REC = LkMoeRec<4>::BYTES;        // of three digits: less
     auto take = [&](size_t bytes) {
         char * p = work ? (char *) work + at : nullptr;
         at += (bytes + 15) & ~(size_t) 15;
@@ -1043,7 +1056,7 @@ static bool lk_moe_few(const LkMoeArgs & a, int type) { return a.T <= 5 || (a.T 
 
 template <int TYPE>
 static void lk_moe_go(const LkMoeArgs & a, hipStream_t st) {
-    constexpr int NP = TYPE == LK_F32 ? 3 : 2;
+    constexpr int NP = TYPE == LK_F32 ? 4 : 3, TG = NP == 4 ? 4 : 6;
     const bool few = lk_moe_few(a, TYPE);
     const int nE = (a.E + 3) / 4, na = a.T * a.k, slots = na < a.E ? na : a.E;
     hipLaunchKernelGGL((lk_k_moe_router<TYPE, NP>), dim3(nE + (a.hidden / 8 + LK_MOE_THREADS - 1) / LK_MOE_THREADS, (a.T + 3) / 4),
@@ -1067,9 +1080,9 @@ static void lk_moe_go(const LkMoeArgs & a, hipStream_t st) {
         hipLaunchKernelGGL((lk_k_moe_down_few<TYPE, NP>), dim3(a.hidden / 8), dim3(64 * LK_MOE_NWF), 0, st, a);
         return;
     }
-    const int groups = (a.T - 1) / LkMoeShare<NP>::TG + 1;
-    hipLaunchKernelGGL((lk_k_moe_many<NP, true>), dim3(a.ffn / 32, slots, groups), dim3(LK_MOE_THREADS), 0, st, a);
-    hipLaunchKernelGGL((lk_k_moe_many<NP, false>), dim3((a.hidden + 63) / 64, slots, groups), dim3(LK_MOE_THREADS), 0, st, a);
+    const int groups = (a.T - 1) / TG + 1;
+    hipLaunchKernelGGL((lk_k_moe_many<NP, TG, true>), dim3(a.ffn / 32, slots, groups), dim3(LK_MOE_THREADS), 0, st, a);
+    hipLaunchKernelGGL((lk_k_moe_many<NP, TG, false>), dim3((a.hidden + 63) / 64, slots, groups), dim3(LK_MOE_THREADS), 0, st, a);
     hipLaunchKernelGGL((lk_k_moe_sum<TYPE>), dim3((a.hidden / 4 + LK_MOE_THREADS - 1) / LK_MOE_THREADS, a.T), dim3(LK_MOE_THREADS), 0, st, a);
 }
 
