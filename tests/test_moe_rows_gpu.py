@@ -6,7 +6,7 @@ Tolerances are those of test_moe_gpu.py where nothing else is said.
 import pytest
 import torch
 
-from ffn_util import TYPES, moe_ref, q4_planes
+from ffn_util import HALF_STEP, TYPES, moe_ref
 from gpu_util import note
 from test_moe_gpu import _close, _layer, _make, _run, _x
 
@@ -59,3 +59,79 @@ def test_large_channels(lk, T, t):
     want, ids1, _ = moe_ref(x, k=k, score="sigmoid", **L)
     assert torch.equal(ids.long(), ids1)
     _close(out, want, dt, (T, t))
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("T", [3, 5, 10, 64])
+@pytest.mark.parametrize("t", TYPES)
+def test_rows_that_are_not_numbers_stay_alone(lk, t, T, score):
+    """A NaN or an infinity in a token makes its own row NaN; the others, which share all their
+    experts with it (3 of 3 are chosen), keep their bytes, in all kinds of launch."""
+    hidden, ffn, E, dt = 96, 64, 3, TYPES[t]
+    x = _x(80 + T, T, hidden, dt)
+    layer = _make(lk, _layer(81, E, hidden, ffn), 3, score=score, max_tokens=T)
+    clean, ids0, w0 = _run(lk, layer, x, hidden, dt, 3)
+    for at, value in ((0, float("nan")), (T // 2, float("inf")), (T - 1, -float("inf"))):
+        bad = x.clone()
+        bad[at, (at * 31) % hidden] = value
+        note(f"moe row {at} of {T} with {value} {score} {t}")
+        out, ids, w = _run(lk, layer, bad, hidden, dt, 3)
+        rows = [i for i in range(T) if i != at]
+        assert torch.equal(out[rows], clean[rows]) and torch.equal(ids[rows], ids0[rows]) and torch.equal(w[rows], w0[rows])
+        assert torch.isnan(out[at]).all() and sorted(ids[at].tolist()) == [0, 1, 2]
+
+
+@pytest.mark.parametrize("tokens", [1, 5, 40, 64])
+def test_every_gate_and_up_weight(lk, tokens):
+    """Unit vectors for every column of gate and up, as many tokens at a time: one or five and
+    forty tokens that each have an expert of their own (dot products in both kinds of launch), 64
+    of one expert (matrix instructions)."""
+    hidden, ffn = 160, 96
+    E = 1 if tokens == 64 else 40
+    L = _layer(84, E, hidden, ffn)
+    if E > 1:                                            # column c chooses expert c / 4
+        L["router"] = (torch.arange(hidden)[None, :] // 4 == torch.arange(E)[:, None]).float()
+    layer = _make(lk, L, 1, max_tokens=tokens)
+    cols = torch.arange(hidden).view(40, 4).t().flatten()                # neighbours have different experts
+    for c in cols.split(tokens):
+        x = torch.zeros(len(c), hidden)
+        x[torch.arange(len(c)), c] = 100.0
+        note(f"moe unit vectors {len(c)} from {int(c[0])}")
+        out, ids, _ = _run(lk, layer, x, hidden, torch.float32, 1)
+        want, ids1, _ = moe_ref(x, k=1, score="sigmoid", **L)
+        assert torch.equal(ids.long(), ids1)
+        _close(out, want, torch.float32, (tokens, int(c[0])))
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("tokens,each", [(1, 1), (5, 1), (8, 2), (64, 1), (64, 2), (64, 7)])
+def test_every_down_weight(lk, tokens, each, t):
+    """Expert j has one row of up that is not zero, row j, and its tokens are unit vectors: h has a
+    single value, and the layer's output is column j of its down weights times that, compared
+    value by value.
+
+    Tolerance: g and u are single products of 15 bits, exact.  silu takes 3 units of 2^-23 for
+    the exponential and the reciprocal and 3 roundings, h times u one, h's whole number is off by
+    at most 2^-23 of it, the product, its scale and the sum round 4 times: 24 of 2^-24, and the
+    output's half step (outputs are 2e-4 and more, normal in fp16)."""
+    hidden, ffn, dt = 96, 64, TYPES[t]
+    E, e = ffn, torch.arange(ffn)
+    L = _layer(90, E, hidden, ffn)
+    for w in ("gate", "up"):                             # the weight that counts: 7 (of 8 zero would be left)
+        qs, b, i = L[w][0], e // 32, e % 32
+        qs[e, e, b, i % 16] = torch.where(i < 16, qs[e, e, b, i % 16] | 0x0F, qs[e, e, b, i % 16] | 0xF0)
+    d = torch.zeros_like(L["up"][1])
+    d[e, e] = L["up"][1][e, e]
+    L["up"] = (L["up"][0], d)
+    L["router"] = torch.zeros(E, hidden)
+    L["router"][e, e] = 1.0
+    layer = _make(lk, L, 1, max_tokens=tokens)
+    for some in e.repeat_interleave(each).split(tokens):
+        x = torch.zeros(len(some), hidden)
+        x[torch.arange(len(some)), some] = 32.0
+        note(f"moe down columns {int(some[0])}..{int(some[-1])}, {each} tokens each, {tokens} at a time {t}")
+        out, ids, _ = _run(lk, layer, x.to(dt), hidden, dt, 1)
+        want, _, _ = moe_ref(x, k=1, score="sigmoid", **L)
+        assert torch.equal(ids[:, 0].long(), some) and bool((want != 0).any(1).all())
+        off = (out.cpu().double() - want).abs()
+        assert bool((off <= (24 * 2.0 ** -24 + (0 if t == "f32" else HALF_STEP[dt])) * want.abs()).all())
