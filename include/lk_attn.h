@@ -511,7 +511,7 @@ typedef struct lk_moe {
     const void * down_d;
 } lk_moe;
 
-/* Bytes of workspace that T tokens need (0 on bad arguments). */
+/* Bytes of workspace that T tokens need (0 on bad arguments; lk_last_error() says which). */
 size_t lk_moe_work_bytes(const lk_moe * moe, int T);
 
 /* x `type` [T][ldx], out and res `type` [T][ldo], [T][ldr] (res may be NULL, or out;

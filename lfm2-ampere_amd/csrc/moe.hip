@@ -1048,7 +1048,11 @@ static size_t lk_moe_layout(const lk_moe * m, int T, void * work, LkMoeArgs * a)
     return at;
 }
 extern "C" size_t lk_moe_work_bytes(const lk_moe * moe, int T) {
-    if (lk_moe_check(moe) || T < 0 || T > LK_MOE_MAX_TOKENS) return 0;
+    if (lk_moe_check(moe)) return 0;
+    if (T < 0 || T > LK_MOE_MAX_TOKENS) {
+        lk_fail(hipErrorInvalidValue, "lk_moe_work_bytes: %d tokens (0..%d)", T, LK_MOE_MAX_TOKENS);
+        return 0;
+    }
     return lk_moe_layout(moe, T, nullptr, nullptr);
 }
 

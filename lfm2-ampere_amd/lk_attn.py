@@ -633,9 +633,8 @@ class MoeQ4_0:
     def work_bytes(self) -> int:
         """Bytes of workspace for max_tokens tokens."""
         n = int(load().lk_moe_work_bytes(self._ref, self.max_tokens))
-        if n == 0 and self.max_tokens != 0:
-            raise LkError(f"lk_moe_work_bytes: {load().lk_last_error().decode(errors='replace')} "
-                          f"({self.max_tokens} tokens)")
+        if n == 0:
+            raise LkError(load().lk_last_error().decode(errors="replace"))
         return n
 
     def __call__(self, x, out, res=None, ids=None, weights=None, work=None, stream=None) -> None:
