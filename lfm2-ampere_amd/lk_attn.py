@@ -601,7 +601,9 @@ class MoeQ4_0:
     [E][hidden][ffn/32]; score "sigmoid" or "softmax", bias fp32 [E] for the choice
     only.  Keeps the weights and one workspace: calls on it must be ordered (one
     stream, or events); calls that may overlap, captured graphs among them, are given
-    workspaces of their own (`work`, uint8 of work_bytes())."""
+    workspaces of their own (`work`, uint8 of work_bytes()).  A layer may be dropped while
+    streams still work on it, as far as its workspace goes (Tensor.record_stream; the weights are
+    the caller's tensors); a captured graph needs its layer as long as it is replayed."""
 
     def __init__(self, router, gate, up, down, top_k: int, score: str = "sigmoid", bias=None, renorm: bool = True,
                  scale: float = 1.0, max_tokens: int = 64):
@@ -629,6 +631,7 @@ class MoeQ4_0:
         if dev < 0:
             raise ValueError("MoeQ4_0: tensors must live in device memory")
         self._work = torch.empty(n, dtype=torch.uint8, device=router.device)
+        self._streams = {torch.cuda.current_stream(dev).cuda_stream}     # those that the workspace's memory is known to
 
     def work_bytes(self) -> int:
         """Bytes of workspace for max_tokens tokens."""
@@ -636,6 +639,14 @@ class MoeQ4_0:
         if n == 0:
             raise LkError(load().lk_last_error().decode(errors="replace"))
         return n
+
+    def _tell(self, stream) -> None:
+        """Tells the allocator of a stream that uses the layer's workspace, so that a layer dropped
+        while the stream has work left does not give the memory away."""
+        raw = stream.cuda_stream if stream is not None else _raw_stream(self._dev)
+        if raw not in self._streams:
+            self._work.record_stream(_torch.cuda.current_stream(self._dev) if stream is None else stream)
+            self._streams.add(raw)
 
     def __call__(self, x, out, res=None, ids=None, weights=None, work=None, stream=None) -> None:
         """out[t] = (res[t] +) the layer of x[t], rows [T][hidden] of fp32, fp16 or bf16
@@ -661,6 +672,8 @@ class MoeQ4_0:
                  work.data_ptr(), work.numel())
         if rc:
             _check(rc, "lk_moe_q4_0")
+        if work is self._work:
+            self._tell(stream)
 
 
 class PrefillCtx:

@@ -1,0 +1,41 @@
+"""Streams other than the one that owns a layer's memory, on the GPU."""
+import pytest
+import torch
+
+from ffn_util import moe_ref
+from gpu_util import note
+from test_moe_gpu import _close, _layer, _make, _x
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("current", [False, True])
+def test_a_layer_dropped_while_a_stream_works_on_it(lk, current):
+    """The workspace is the layer's own: dropped with the layer while a side stream has still to
+    run, its memory is not handed to the next allocation."""
+    hidden, ffn, E, k, T = 256, 128, 8, 2, 20
+    L = _layer(95, E, hidden, ffn)
+    layer = _make(lk, L, k, max_tokens=T)
+    keep = layer._keep                                   # the weights are the caller's tensors
+    x = _x(96, T, hidden, torch.float32).cuda()
+    out = torch.empty_like(x)
+    a = torch.ones(8192, 8192, device="cuda", dtype=torch.bfloat16)
+    b = torch.empty_like(a)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    note(f"a layer dropped while a side stream works, current {current}")
+    with torch.cuda.stream(side):
+        for _ in range(20):                              # some 20 ms before the layer's turn
+            torch.mm(a, a, out=b)
+        if current:
+            layer(x, out)
+    if not current:
+        layer(x, out, stream=side)
+    at, n = layer._work.data_ptr(), layer._work.numel()
+    del layer
+    new = torch.empty(n, dtype=torch.uint8, device="cuda")
+    early, other = not side.query(), new.data_ptr() != at
+    torch.cuda.synchronize()
+    assert early and other                               # nothing is written to it: the choices lie there
+    _close(out, moe_ref(x.cpu(), k=k, score="sigmoid", **L)[0], torch.float32, "dropped layer")
+    del keep
