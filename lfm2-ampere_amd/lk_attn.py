@@ -506,6 +506,8 @@ def _on(dev: int, stream, call, *args) -> int:
     the device's current one."""
     if dev < 0:
         raise ValueError("lk_attn: tensors must live in device memory")
+    if stream is not None and getattr(stream, "device_index", dev) != dev:
+        raise ValueError("lk_attn: the stream is one of another device than the tensors'")
     if _raw_stream is not None and _device is not None and _device() == dev:
         return call(*args, (_raw_stream(dev) if stream is None else stream.cuda_stream) or None)
     import torch

@@ -39,3 +39,20 @@ def test_a_layer_dropped_while_a_stream_works_on_it(lk, current):
     assert early and other                               # nothing is written to it: the choices lie there
     _close(out, moe_ref(x.cpu(), k=k, score="sigmoid", **L)[0], torch.float32, "dropped layer")
     del keep
+
+
+class _Elsewhere:
+    """A stream of a device that the tensors are not on."""
+    device_index, cuda_stream = 1, 0x1000
+
+
+def test_a_stream_of_another_device_is_refused(lk):
+    x = torch.ones(2, 64, device="cuda")
+    q, sc = lk.i8_rows(2, 64), torch.ones(2, device="cuda")
+    layer = _make(lk, _layer(97, 2, 64, 32), 1, max_tokens=2)
+    note("a stream of another device")
+    for call in (lambda: lk.norm_q8(x, torch.ones(64, device="cuda"), q, sc, stream=_Elsewhere()),
+                 lambda: lk.gemm_i8(q, sc, q, sc, torch.empty(2, 2, device="cuda"), stream=_Elsewhere()),
+                 lambda: layer(x, x, stream=_Elsewhere())):
+        with pytest.raises(ValueError, match="another device"):
+            call()
