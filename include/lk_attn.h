@@ -522,8 +522,8 @@ size_t lk_moe_work_bytes(const lk_moe * moe, int T);
  * fp32, the blocks are added in fp32.  ids int32 [T][top_k] and weights fp32 [T][top_k], in the order of choice,
  * where not NULL.  work: 16-byte aligned device memory of lk_moe_work_bytes();
  * launches that share it must be ordered (one stream, or the caller's events).
- * The description is read during the call; a token whose x is not finite gives NaN
- * in its own row only. */
+ * The description is read during the call; a token whose x, or whose gate . x, up . x or
+ * activation in fp32, is not finite gives NaN in all of its own row and in no other. */
 int lk_moe_q4_0(const lk_moe * moe, int type, const void * x, int ldx, int T, const void * res,
                 int ldr, void * out, int ldo, int32_t * ids, float * weights, void * work,
                 size_t work_bytes, void * stream);

@@ -135,3 +135,23 @@ def test_every_down_weight(lk, tokens, each, t):
         assert torch.equal(ids[:, 0].long(), some) and bool((want != 0).any(1).all())
         off = (out.cpu().double() - want).abs()
         assert bool((off <= (24 * 2.0 ** -24 + (0 if t == "f32" else HALF_STEP[dt])) * want.abs()).all())
+
+
+@pytest.mark.parametrize("T", [1, 5, 10, 64])
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_activations_beyond_fp32(lk, t, T):
+    """silu(gate . x) * (up . x) beyond fp32's range makes the token's row NaN (the formula's would be
+    infinities of both signs and NaN), and no other row."""
+    hidden, ffn, E, dt = 96, 64, 3, TYPES[t]
+    L = _layer(82, E, hidden, ffn)
+    L["router"] *= 1e-20
+    layer = _make(lk, L, 3, max_tokens=T)
+    x = _x(83 + T, T, hidden, dt)
+    clean, ids0, _ = _run(lk, layer, x, hidden, dt, 3)
+    big = x.clone()
+    big[T // 2] = big[T // 2] * 1e25                     # h of 1e48
+    note(f"moe activations beyond fp32 T={T} {t}")
+    out, ids, w = _run(lk, layer, big, hidden, dt, 3)
+    rows = [i for i in range(T) if i != T // 2]
+    assert torch.isnan(out[T // 2]).all() and torch.isfinite(w).all() and sorted(ids[T // 2].tolist()) == [0, 1, 2]
+    assert torch.equal(out[rows], clean[rows]) and torch.equal(ids[rows], ids0[rows])
