@@ -448,12 +448,14 @@ int lk_pf_gemm_q4_0(const void * qs, const void * d, int N, int bpr, const int8_
  * res (may be x or delta itself, or NULL) takes h and y (or NULL) takes y, rounded
  * to the type; the 8-bit output is of the unrounded y:
  *   LK_Q8_ROW     q int8 [rows][ldq], sc fp32 [rows]: a = max |y|, sc = a / 127,
- *                 q = rint(y * (127 / a)); a < 2^-120: sc and q are 0; a row with a
- *                 value that is not finite: sc is NaN, q 0, y NaN
+ *                 q = rint(y * (127 / a)); a < 2^-120: sc and q are 0; a not
+ *                 finite: sc is NaN, q 0
  *   LK_Q81_PLANAR q int8 [rows][n], sc fp32 [rows][n/32][2]: the bytes
  *                 lk_pf_quant_rows makes of y (the operand of lk_pf_gemm_q4_0)
  *   LK_Q81_BLOCK  q lk_block_q8_1 [rows][n/32], sc not used: the same quants and
  *                 scales as blocks (the operand of lk_gemv_q4_0)
+ * A row of h with a value that is not finite has NaN for all of y, and so has a row
+ * of zeros with eps 0; a y that overflows is infinite in its own place.
  * The Q8_1 forms need n a multiple of 32 and ldq == n.  Rows need the alignment of
  * their elements only (sc of the planar form 8 bytes, blocks 4).  x, delta, res
  * and y may share a buffer where row and stride are the same. */

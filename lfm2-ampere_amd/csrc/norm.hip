@@ -12,14 +12,15 @@
 // for the Q4_0 GEMV, the bytes lk_pf_quant_rows and the decode combine make of y.
 // h and y are also stored where the caller asks, rounded once to the rows' type;
 // the norm goes on from the unrounded h.
-// The sum of squares is taken in 64 bits: q is a rounding of y, and with a sum that
-// does not depend on the number of lanes it is the same for every launch shape
-// (fp32 partial sums of 2048 squares differ in their last bits, which moved 1 of
-// about 10^5 quants by one).
-// A row with a value that is not finite gets the scale NaN and zeros (row form),
+// The sum of squares is taken in 64 bits: q is a rounding of y, and fp32 partial sums of
+// 2048 squares differ in their last bits with the number of lanes, which moved 1 of
+// about 10^5 quants by one.  The orders of 64-bit sums differ by about 2^-50, so the launch
+// shapes agree but where 1 / sqrt lies that close to the middle of two fp32 numbers: one row
+// of some 10^8.
+// A row of h with a value that is not finite gets the scale NaN and zeros (row form),
 // and NaN in h * r, so that everything computed from it is NaN and no other row
-// is touched; a row whose largest |y| is below 2^-120 gets scale and quants 0 (127 /
-// a would overflow).
+// is touched (with eps 0, a row of zeros too: 0 / 0); a row whose largest |y| is below
+// 2^-120 gets scale and quants 0 (127 / a would overflow).
 #include "lk_types.h"
 #include "lk_q81.h"
 
