@@ -653,7 +653,7 @@ class MoeQ4_0:
     def __call__(self, x, out, res=None, ids=None, weights=None, work=None, stream=None) -> None:
         """out[t] = (res[t] +) the layer of x[t], rows [T][hidden] of fp32, fp16 or bf16
         (out may be x, res may be out); ids int32 and weights fp32 [T][top_k] where
-        given."""
+        given.  Up to 8 tokens a row's last fp32 bits depend on the batch, from 9 on not."""
         ty = _type_of(x, "MoeQ4_0")
         if x.dim() != 2:
             raise ValueError("MoeQ4_0: x must be [tokens, hidden]")
