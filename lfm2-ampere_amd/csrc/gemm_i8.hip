@@ -44,9 +44,9 @@ struct LkI8Args {
 // the operand layout (lane: row or token l % 16, 16 bytes at 16 * (l / 16) of a 64-byte
 // step), so that nothing waits for anything but its own loads.  The int32 parts meet in
 // LDS; integer sums have no order.  Bound by the latency of one round of loads and the
-// launch for short rows (1 x 4096 x 1024: 2.5 us with 4 waves, 3.1 with 8, of which half
+// launch for short rows (1 x 4096 x 1024: 3.0 us with 4 waves, 3.7 with 8, of which half
 // find no piece), by the weights' way from the cache for long ones (1 x 4096 x 8192, 34 MB:
-// 6.5 us with 8 waves, 5.2 TB/s; 7.6 with 4).
+// 7.1 us with 8 waves, 4.7 TB/s; 8.0 with 4).
 template <int TYPE, int NW>
 __global__ void __launch_bounds__(64 * NW)
 lk_k_gemm_i8_few(const LkI8Args a) {
@@ -98,12 +98,12 @@ lk_k_gemm_i8_few(const LkI8Args a) {
 // its part of every stage, and integer sums have no order.  K in stages of KC bytes, a ring of
 // NB of them in LDS, filled by LDS DMA.
 // What bounds it.  Large: the matrix instructions at the clock that the power leaves: 8192^3 in
-// 419 to 484 us, 2270 to 2620 TOPS from card to card, where MFMAs alone, without a load, reach 2630 and the
-// library's int8 product 2090 (earlier: 4 waves of 4 x 4 tiles, which read less from LDS, 470 for
-// 446, a ring of 4 stages of 64 bytes 467 to 498).  4096 x 8192 x 2048, two rounds of tiles: 64
-// to 73 us (1880 to 2150), of which the outputs, 34 MB of every unit's at once, are a part that
-// nothing hides.  Small: the latency of the ring's start, of a stage and of the launch (333 x 2048 x
-// 2048: 5.7 us).
+// 441 and 459 us in a row of ten or more on two cards (2400 to 2490 TOPS), 517 and 523 for a call alone after a
+// wait; the library's int8 product with int32 out, in turn with it, 448 and 463, and 505 and 528 (earlier: 4
+// waves of 4 x 4 tiles, which read less from LDS, 5 % slower, a ring of 4 stages of 64 bytes 5 to 10 %).
+// 4096 x 8192 x 2048, two rounds of tiles: 70 to 72 us (1930 TOPS; the library 78), of which the outputs, 34
+// MB of every unit's at once, are a part that nothing hides.  Small: the latency of the ring's
+// start, of a stage and of the launch (333 x 2048 x 2048: 6.1 us).
 template <int TM_, int TN_, int WM_, int WN_, int WK_, int KC_, int NB_, int OCC_>
 struct LkI8Shape {
     static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, WK = WK_, KC = KC_, NB = NB_, OCC = OCC_;   // OCC: waves per SIMD
@@ -372,22 +372,28 @@ static int lk_i8_tiles(const LkI8Args & a, hipStream_t st) {
 // Which kernel.  What counts is how many rounds of 256 units the tiles take: the smallest
 // tile that fits one round is the best, for a larger one leaves units idle and has fewer waves
 // to share K, and a smaller one takes a second round.
-// Measured (bf16 out, operands in the cache, us; * is what the rule takes):
+// Measured (bf16 out, operands in the cache, ten calls in a graph, us each; * is what the rule takes):
 //   M x N x K          few   32x32  64x32  64x64  128x64  128x128  2/unit  256x256
-//   1 x 4096 x 4096    4.3*   5.7    6.8    7.8
-//   16 x 4096 x 4096   5.7*   5.7
-//   1 x 8192 x 2048    4.0*   4.6    5.0    5.5
-//   16 x 8192 x 2048   5.4    4.7*   5.2    5.6
-//   1 x 8192 x 8192   13.4   11.8*  12.3   14.8    22.5
-//   128 x 2048 x 2048         4.9*   5.5    6.1     8.6
-//   192 x 2048 x 2048         6.3    5.7*   6.2     8.7
-//   333 x 2048 x 2048         9.3    9.9    6.6*    8.9     11.0
-//   640 x 2048 x 2048                      10.0     9.3*    11.2    12.8
-//   1000 x 4096 x 2048                     18.0    15.5     14.1*   16.5    28.6
-//   2048 x 4096 x 2048                             28.7     26.5    25.4*   31.2
-//   2600 x 4096 x 2048                             39.7     36.2    38.1    33.9*
-//   2600 x 8192 x 2048                             71.3     71.3    60.6*   65.7
-//   4096 x 8192 x 2048                            104.8    100.8    86.0    76.3*
+//   1 x 4096 x 4096    4.8*   5.3    6.6    7.4
+//   16 x 4096 x 4096   6.1    5.3*
+//   1 x 8192 x 2048    4.4*   4.5    5.3    5.6
+//   8 x 8192 x 2048    5.0    4.5*   5.4    5.7
+//   1 x 8192 x 8192   13.5   12.3*  13.0   15.1    23.1
+//   128 x 2048 x 2048         4.7*   5.6    5.8     8.4
+//   192 x 2048 x 2048         6.5    5.7*   5.9     8.5     10.0
+//   333 x 2048 x 2048         9.0    9.6    6.1*    8.6      9.9
+//   640 x 2048 x 2048        13.2   13.7    9.3     8.9*    10.3    12.5
+//   1000 x 4096 x 2048                     17.8    15.6     13.7*   15.8    27.9
+//   1500 x 4096 x 2048                     26.8    22.5     23.3    20.2*   28.4
+//   2048 x 4096 x 2048                     35.8    29.3     27.4    22.5*   29.3
+//   2600 x 4096 x 2048                     46.6    40.9     37.8    34.1    30.4*
+//   2600 x 8192 x 2048                             73.2     75.3    55.8*   60.3
+//   3000 x 8192 x 2048                             80.8     83.6    60.2*   61.3
+//   4096 x 8192 x 2048                            107.5    110.8    79.2    70.3*
+// Few tokens: 16 rows a workgroup read every token's row again, so that their time grows with M K where
+// that of 32x32 does not (few / 32x32; 1, 4, 16 tokens): 4096 x 2048 3.6, 3.7, 4.1 / 4.5; 4096 x 4096 4.8, 5.1,
+// 6.1 / 5.3; 4096 x 8192 7.1, 7.8, 9.7 / 8.6 to 9.2; 2048 x 8192 6.8, 7.5, 9.5 / 7.0; 8192 x 1024 3.5, 3.7, 4.2 /
+// 4.1; 8192 x 2048 4.4, 4.7, 5.8 / 4.5.
 // A round of 256 256x256 tiles takes about 5 / 3 of one of 512 128x128 tiles.
 // 64x32 has two forms: K over four waves in stages of 256 bytes (4096 x 128 x 8192 12.2 us, 13.9 with two
 // waves and 128), and over two in stages of 128 where K is short (8192 x 64 x 512 4.0, 4.6).
@@ -396,7 +402,8 @@ static int lk_i8_tiles(const LkI8Args & a, hipStream_t st) {
 // few 11.3), 32 x 65536 x 2048 22.3 (24.4, 22.9), 16 x 128256 x 4096 92 (96, 98; 5.7 TB/s of weights).
 template <int TYPE>
 static int lk_i8_shape(const LkI8Args & a, hipStream_t st) {
-    if (a.M <= 16 && (a.N <= 4096 || (a.N <= 8192 && a.K <= 2048 && a.M <= 8))) {
+    const long mk = (long) a.M * a.K;
+    if (a.M <= 16 && ((a.N <= 4096 && (a.K <= 2048 || mk <= 16384)) || (a.N <= 8192 && a.K <= 2048 && mk <= 8192))) {
         if (a.K <= 2048) lk_i8_few<TYPE, 4>(a, st);
         else lk_i8_few<TYPE, 8>(a, st);
         return 0;
