@@ -645,10 +645,12 @@ class MoeQ4_0:
     def _tell(self, stream) -> None:
         """Tells the allocator of a stream that uses the layer's workspace, so that a layer dropped
         while the stream has work left does not give the memory away."""
-        raw = stream.cuda_stream if stream is not None else _raw_stream(self._dev)
-        if raw not in self._streams:
-            self._work.record_stream(_torch.cuda.current_stream(self._dev) if stream is None else stream)
-            self._streams.add(raw)
+        if stream is None and _raw_stream is not None and _raw_stream(self._dev) in self._streams:
+            return
+        s = _torch.cuda.current_stream(self._dev) if stream is None else stream
+        if s.cuda_stream not in self._streams:
+            self._work.record_stream(s)
+            self._streams.add(s.cuda_stream)
 
     def __call__(self, x, out, res=None, ids=None, weights=None, work=None, stream=None) -> None:
         """out[t] = (res[t] +) the layer of x[t], rows [T][hidden] of fp32, fp16 or bf16
