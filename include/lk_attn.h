@@ -519,14 +519,15 @@ size_t lk_moe_work_bytes(const lk_moe * moe, int T);
 /* x `type` [T][ldx], out and res `type` [T][ldo], [T][ldr] (res may be NULL, or out;
  * out may be x).  x and the activation between the products enter the products in
  * blocks of 32 as whole numbers of 32 bits (fp32 rows) or 24 bits (fp16 and bf16 rows) of the
- * block's largest value: each value is off by at most 2^-31 or 2^-23 of that.  A block whose
- * largest is under 2^-96 counts as zero.  A block's sum is exact up to its one rounding to
- * fp32, the blocks are added in fp32.  Among 9 tokens and more a token's result is the same, bit
- * for bit, whatever the others are; up to 8 the order of the additions depends on how many
- * tokens there are and how many experts they choose, so that a token checked in a draft and the
- * same token decoded alone may differ by roundings of fp32.  ids int32 [T][top_k] and weights fp32 [T][top_k], in the order of choice,
- * where not NULL.  work: 16-byte aligned device memory of lk_moe_work_bytes();
- * launches that share it must be ordered (one stream, or the caller's events).
+ * block's largest value: each value is off by at most 2^-31 or 2^-23 of that (2^-27 where it is
+ * under 2^-96).  A block whose largest is under 2^-100 counts as zero.  A block's sum is exact up
+ * to its one rounding to fp32, the blocks are added in fp32.  Among 9 tokens and more a token's
+ * result is the same, bit for bit, whatever the others are; up to 8 the order of the
+ * additions depends on how many tokens there are and how many experts they choose, so that a
+ * token checked in a draft and the same token decoded alone may differ by roundings of fp32.
+ * ids int32 [T][top_k] and weights fp32 [T][top_k], in the order of choice, where not NULL.
+ * work: 16-byte aligned device memory of lk_moe_work_bytes(); launches that share it must be
+ * ordered (one stream, or the caller's events).
  * The description is read during the call; a token whose x, or whose gate . x, up . x or
  * activation in fp32, is not finite gives NaN in all of its own row and in no other. */
 int lk_moe_q4_0(const lk_moe * moe, int type, const void * x, int ldx, int T, const void * res,

@@ -18,7 +18,7 @@
 // for fp16 and bf16 rows (24 bits).  sum (n - 8) i is exact in int32 digit by digit
 // (-8 * the digits' sum is where the sum starts), the digits are put together and scaled by
 // d * 2^-p in fp32, and blocks are added in fp32.  A block that holds a value
-// that is not finite gets the scale NaN; one whose largest value is under 2^-96 counts as
+// that is not finite gets the scale NaN; one whose largest value is under 2^-100 counts as
 // zero.
 // Why that many: a channel, of x or of h, that is 1000 times the others leaves its 31 neighbours
 // 10 bits fewer.  With a digit less a row whose large channels meet weights of zero
@@ -92,9 +92,11 @@ template <int NP>
 __device__ __forceinline__ float lk_moe_up2(uint32_t am) {
     constexpr float TOP = NP == 4 ? 2139062016.0f : 8355711.0f;                   // 24 bits of the four digits' end
     constexpr int B = NP == 4 ? 30 : 22;
-    if (am >= 0x7F800000u || am < (31u << 23)) return 0.0f;                       // not finite; under 2^-96
-    // 2^(B - E), E the exponent of am: between 2^(B - 127) and 2^(B + 96), and its inverse is normal too
-    const float f = __builtin_bit_cast(float, (uint32_t) (B + 254 - (int) (am >> 23)) << 23);
+    if (am >= 0x7F800000u || am < (27u << 23)) return 0.0f;                       // not finite; under 2^-100
+    // 2^(B - E), E the exponent of am, up to 2^126, whose inverse is normal (four digits: blocks of 2^-96 to
+    // 2^-100 have 30 to 26 bits)
+    const int e = B + 254 - (int) (am >> 23);
+    const float f = __builtin_bit_cast(float, (uint32_t) (e < 253 ? e : 253) << 23);
     return __builtin_bit_cast(float, am) * f > TOP ? 0.5f * f : f;
 }
 __device__ __forceinline__ float lk_moe_scale(uint32_t am, float up) {            // 2^-p; NaN for what is not finite

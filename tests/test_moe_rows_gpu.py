@@ -6,7 +6,7 @@ Tolerances are those of test_moe_gpu.py where nothing else is said.
 import pytest
 import torch
 
-from ffn_util import HALF_STEP, TYPES, moe_ref
+from ffn_util import HALF_STEP, TYPES, moe_ref, q4_pack
 from gpu_util import note
 from test_moe_gpu import _close, _layer, _make, _run, _x
 
@@ -155,3 +155,20 @@ def test_activations_beyond_fp32(lk, t, T):
     rows = [i for i in range(T) if i != T // 2]
     assert torch.isnan(out[T // 2]).all() and torch.isfinite(w).all() and sorted(ids[T // 2].tolist()) == [0, 1, 2]
     assert torch.equal(out[rows], clean[rows]) and torch.equal(ids[rows], ids0[rows])
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("T", [1, 12])
+def test_small_activations(lk, T, t):
+    """Down to 2^-100 a block of h counts: x of 2^-p, 32 weights of one each, make g and u 2^(5 - p) and
+    h half their product, 2^(9 - 2 p); the output is 32 of it, exact (silu's half is off by 2^-50
+    of itself)."""
+    hidden = ffn = 32
+    one = torch.ones(1, 32, 32, dtype=torch.int64)
+    plane = (q4_pack(one), torch.ones(1, 32, 1).half())
+    layer = _make(lk, {"router": torch.zeros(1, hidden), "bias": None, "gate": plane, "up": plane, "down": plane}, 1, max_tokens=T)
+    for p in (50, 52, 53, 54, 55):
+        note(f"moe activations of 2^{9 - 2 * p} T={T} {t}")
+        out, _, _ = _run(lk, layer, torch.full((T, hidden), 2.0 ** -p).to(TYPES[t]), hidden, TYPES[t], 1)
+        want = 2.0 ** (14 - 2 * p) if 9 - 2 * p >= -100 else 0.0
+        assert bool((out.double().cpu() == want).all()), (p, out[0, 0].item())
