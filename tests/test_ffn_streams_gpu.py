@@ -56,3 +56,32 @@ def test_a_stream_of_another_device_is_refused(lk):
                  lambda: layer(x, x, stream=_Elsewhere())):
         with pytest.raises(ValueError, match="another device"):
             call()
+
+
+def test_captured_on_the_layers_own_workspace(lk):
+    """A graph of calls on the layer's own workspace, replayed between eager calls on another
+    stream in order; the layer goes after the graph."""
+    hidden, ffn, E, k, T = 256, 128, 8, 2, 20
+    layer = _make(lk, _layer(98, E, hidden, ffn), k, max_tokens=T)
+    x, out = torch.empty(T, hidden, device="cuda"), torch.empty(T, hidden, device="cuda")
+    x.copy_(_x(99, T, hidden, torch.float32))
+    note("a layer captured on its own workspace")
+    layer(x, out)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        layer(x, out)
+    for rep in range(4):
+        x.copy_(_x(110 + rep, T, hidden, torch.float32))
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        side, want = torch.cuda.Stream(), torch.empty_like(out)
+        torch.cuda.synchronize()
+        layer(x, want, stream=side)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want), rep
+    del g, layer
+    torch.cuda.synchronize()
+    torch.empty(1 << 20, device="cuda").zero_()
+    torch.cuda.synchronize()
