@@ -534,6 +534,98 @@ int lk_moe_q4_0(const lk_moe * moe, int type, const void * x, int ldx, int T, co
                 int ldr, void * out, int ldo, int32_t * ids, float * weights, void * work,
                 size_t work_bytes, void * stream);
 
+/* ---- many sequences over a paged cache ------------------------------------------
+ * What the producers and the attention above do for one sequence in one contiguous
+ * cache, for a batch of sequences whose positions lie in pages of a shared pool, in any
+ * order: a step's append, the attention of its new tokens, and the commit of a draft.
+ * All tables are device memory, read on the device during the call (the calls may be
+ * captured and replayed with other contents); what the kernels read of them is bounded
+ * by the sizes below, so that a wrong entry gives a wrong result and no access out of
+ * bounds. */
+
+/* The pools of one layer and the heads that read them.  head_dim 64 or 128; n_heads a
+ * multiple of n_kv_heads, up to LK_PAGED_MAX_HEADS, up to LK_PAGED_MAX_GROUP of them a
+ * kv head; page (positions a page) a power of two from 16 to 65536. */
+#define LK_PAGED_MAX_HEADS 256
+#define LK_PAGED_MAX_GROUP 64
+typedef struct lk_pages {
+    int type;                       /* of the pools: LK_F16 or LK_BF16 */
+    int n_heads, n_kv_heads, head_dim;
+    int page, n_pages;
+    void * k;                       /* [n_pages][page][n_kv_heads][head_dim], 16-byte aligned */
+    void * v;
+} lk_pages;
+
+/* One step of n_seqs sequences: sequence b has lens[b] positions in its pages and n_b =
+ * first[b + 1] - first[b] new tokens (0 or more), whose rows are first[b] .. of the step's
+ * `rows` rows and which take the slots lens[b], lens[b] + 1, ...  Slot s of b lies in page
+ * table[b * ldt + s / page], 0 <= s < width * page (at most 2^30).
+ * Rows that no sequence names (behind the last one: padding) are left as they were.
+ * Values out of range: a length counts as the nearest of 0 .. width * page, a row bound
+ * as the nearest of 0 .. rows, and n_b below 0 as 0; slots past the table and pages outside
+ * the pool are not written, and attended to as keys and values of zero (slots past the
+ * table: not at all). */
+typedef struct lk_step {
+    int n_seqs, rows;
+    const int32_t * first;          /* [n_seqs + 1], not decreasing */
+    const int32_t * lens;           /* [n_seqs] */
+    const int32_t * table;          /* [n_seqs][ldt], of which `width` pages count */
+    int ldt, width;
+    const int32_t * pos;            /* [rows] positions of the new tokens, or NULL: lens[b] + i */
+    const uint64_t * mask;          /* [rows] which new tokens a row sees, or NULL: causal */
+    int max_new;                    /* the largest n_b, for the choice of a kernel only (0: unknown) */
+} lk_step;
+
+/* Per row: q and k heads normed and rotated, q to qo, k and v to the row's slot.
+ *   y = x * (1/sqrt(mean of x^2 + eps)) * w     (w = qn / kn fp32 [head_dim]; NULL: y = x),
+ *   a_i = position * freq_i, i < rot / 2, the product and its sine and cosine in fp64;
+ *   LK_ROPE_HALVES: the pair is (y_i, y_{i + rot/2}), LK_ROPE_PAIRS: (y_2i, y_{2i+1});
+ *   (u, v) -> (u cos a - v sin a, u sin a + v cos a); values from rot on are not rotated
+ * in fp32, rounded once.  freq fp32 [rot / 2], rot a multiple of 8 up to head_dim, or freq NULL
+ * with rot 0: no rotation.  |a_i| below 2^31.  Squares are summed in fp32.
+ * q, k, v, qo are rows of `type` (LK_F32 or LK_F16 with fp16 pools, LK_BF16 with bf16 pools) of
+ * n_heads or n_kv_heads heads side by side, ld* elements apart (parts of one wide row as
+ * well); q and qo may be NULL (keys and values only), and qo may be q.  Rows need the
+ * alignment of their elements; qn, kn, freq 16 bytes.  k, v and the pools must not overlap. */
+#define LK_ROPE_HALVES 0
+#define LK_ROPE_PAIRS  1
+int lk_paged_append(const lk_pages * pages, const lk_step * step, int type, const void * q, int ldq,
+                    const void * k, int ldk, const void * v, int ldv, const float * qn, const float * kn,
+                    float eps, const float * freq, int rot, int style, void * qo, int ldqo, void * stream);
+
+/* Attention of the new tokens (which the pools already hold, lk_paged_append): row i of
+ * sequence b (counted from 0) sees its sequence's lens[b] earlier positions and of the new ones
+ *   mask NULL: tokens 0 .. i;
+ *   else: token 64 * (i / 64) + j where bit j of its word is set, and all tokens before
+ *   64 * (i / 64): for up to 64 drafted tokens any tree, each row's bit set for itself and
+ *   its ancestors.
+ *   x = scale * q.k;  cap > 0: x = cap * tanh(x / cap);  slopes: x += slopes[h] * (position of
+ *   the key - position of the row), a cached key's position being its slot;  out = softmax(x) . v
+ * and zeros for a row that sees nothing.  Keys and values a row does not see do not touch
+ * it, infinities and NaN among them.
+ * q, out rows of `type` as in lk_paged_append, n_heads heads side by side; scale > 0;
+ * slopes fp32 [n_heads] or NULL.  Scores, softmax and sums are fp32.  For 16-bit rows the weights
+ * enter the product with v rounded to the type, and so does their sum; for fp32 rows q and the
+ * weights enter as two fp16 parts (22 bits).  Results do not depend on the run; the last bits
+ * depend on how the batch's keys are divided among the workgroups.
+ * work: 16-byte aligned device memory of lk_paged_attn_work_bytes() (0 on bad arguments;
+ * lk_last_error() says which); launches that share it must be ordered (one stream, or the
+ * caller's events), and graphs that may run at once need two. */
+size_t lk_paged_attn_work_bytes(const lk_pages * pages, int type, int max_new);
+int lk_paged_attn(const lk_pages * pages, const lk_step * step, int type, const void * q, int ldq,
+                  float scale, float cap, const float * slopes, void * out, int ldo, void * work,
+                  size_t work_bytes, void * stream);
+
+/* What is accepted of each sequence's new tokens becomes part of its cache: path[b * ldp + j],
+ * j < count[b] <= ldp, are the accepted tokens' places among the n_b, strictly increasing (a
+ * path of a tree from its root); token path[j]'s key and value move to slot lens[b] + j, and
+ * new_lens[b] = lens[b] + count[b].  path NULL: the first count[b] tokens.  Where the list stops
+ * increasing or leaves 0 .. n_b - 1 or the table, or names a page outside the pool, it ends.
+ * ldp up to LK_PAGED_MAX_PATH.  new_lens may be step->lens. */
+#define LK_PAGED_MAX_PATH 64
+int lk_paged_commit(const lk_pages * pages, const lk_step * step, const int32_t * path, int ldp,
+                    const int32_t * count, int32_t * new_lens, void * stream);
+
 #ifdef __cplusplus
 }
 #endif

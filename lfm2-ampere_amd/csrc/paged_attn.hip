@@ -1,0 +1,891 @@
+// paged_attn.hip - attention of a batch's new tokens over its sequences' pages: single
+// tokens, trees of drafted tokens, causal runs (lk_paged_attn).
+//
+//     x_ij = scale * q_i . k_j;  x = cap * tanh(x / cap);  x += slope_h * (position of j - position of i)
+//     out_i = sum_j exp(x_ij) v_j / sum_j exp(x_ij)      over the j that i sees
+//
+// The work is one line of key tiles: per sequence, chunk of its new tokens and group of kv
+// heads ("item") the tiles of the keys that the chunk sees.  Each of LK_PA_WGS workgroups
+// takes an equal run of that line, whatever the lengths are: it finds its place from the
+// lengths on the device, walks on from item to item, and its DMA runs ahead over the
+// borders.  An item inside one run is finished there; one that is cut leaves partials
+// (max, sum, unnormalised rows), which a second kernel joins in order.  A workgroup has at
+// most two cut items, one at each end of its run, so the workspace does not depend on the
+// batch.
+//
+// In a workgroup a tile (16 KB of K rows and 16 KB of V rows of the group's heads, fetched by LDS DMA into a
+// ring) is shared by waves that differ in kv head, in the query columns they hold, and, where
+// there are too few heads and columns, in the keys they take.  A wave computes S^T = K.Q^T and
+// O^T += V^T.P^T on 16x16 tiles of the matrix cores: a score tile leaves the matrix core as the
+// operand the second product takes, so P stays in registers.  Columns are (token, query head)
+// pairs of one kv head.
+// The sum of the weights comes from the same product (a row of ones), so weights and sum are
+// rounded alike.
+#include "lk_paged.h"
+
+#define LK_PA_WGS   256            // workgroups: one a CU (a ring of 128 KB each)
+#define LK_PA_NBUF  4
+#define LK_PA_TILEB 32768          // K rows, then V rows
+#define LK_PA_HEADROOM 8.0f        // the running max is raised when a score passes it by 2^8
+
+typedef short lk_s4 __attribute__((ext_vector_type(4)));
+typedef __bf16 lk_b8 __attribute__((ext_vector_type(8)));
+typedef __bf16 lk_b4 __attribute__((ext_vector_type(4)));
+
+template <int CTYPE> struct LkMm;
+template <> struct LkMm<LK_F16> {
+    typedef _Float16 T;
+    typedef lk_h8 V8;
+    typedef lk_h4 V4;
+#ifdef __HIP_DEVICE_COMPILE__
+    static __device__ __forceinline__ lk_f4 k32(V8 a, V8 b, lk_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ lk_f4 k16(V4 a, V4 b, lk_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0); }
+#else
+    static __device__ __forceinline__ lk_f4 k32(V8, V8, lk_f4 c) { return c; }
+    static __device__ __forceinline__ lk_f4 k16(V4, V4, lk_f4 c) { return c; }
+#endif
+    static constexpr uint16_t INF = 0x7C00;
+};
+template <> struct LkMm<LK_BF16> {
+    typedef __bf16 T;
+    typedef lk_b8 V8;
+    typedef lk_b4 V4;
+#ifdef __HIP_DEVICE_COMPILE__
+    static __device__ __forceinline__ lk_f4 k32(V8 a, V8 b, lk_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ lk_f4 k16(V4 a, V4 b, lk_f4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(lk_s4, a), __builtin_bit_cast(lk_s4, b), c, 0, 0, 0);
+    }
+#else
+    static __device__ __forceinline__ lk_f4 k32(V8, V8, lk_f4 c) { return c; }
+    static __device__ __forceinline__ lk_f4 k16(V4, V4, lk_f4 c) { return c; }
+#endif
+    static constexpr uint16_t INF = 0x7F80;
+};
+
+struct LkPaArgs {
+    const void * q;
+    void * out;
+    const char * kp, * vp;
+    const char * zeros;            // 1 KB of zeros: what keys that no row sees are fetched from
+    const int32_t * first, * lens, * table, * pos;
+    const uint64_t * mask;
+    const float * slopes;
+    float * acc;                   // partials: [2 * workgroup + end][block of columns][D / 16][column][4][4 dims]
+    float2 * ml;                   // and their (max, sum): [..][..][16]
+    int4 * cut;                    // per workgroup the cut item that begins in it: (pieces, first row, rows, kv head group)
+    int ldq, ldo, n_seqs, rows, ldt, width, page_sh, n_pages;
+    int hq, hkv, g;                // g = query heads a kv head
+    int nhg, hg_sh, qw_sh, kw_sh;  // groups of 2^hg_sh kv heads; a workgroup's waves = heads x column groups x key shares
+    int qc;                        // tokens a chunk, a power of two up to 64
+    float sc, scale, cap;          // sc = scale * log2(e)
+};
+
+// Wave-uniform loads of the tables by the scalar unit: they are counted apart from the DMA in flight,
+// which a vector load would be waited for together with.
+__device__ __forceinline__ int lk_sld(const int32_t * p, long i) {
+#ifdef __HIP_DEVICE_COMPILE__
+    return ((const __attribute__((address_space(4))) int32_t *) (uintptr_t) p)[i];
+#else
+    return p[i];
+#endif
+}
+
+// ---- the line of tiles ----------------------------------------------------------------
+// Tiles of chunk c of a sequence: the keys up to the last one that a row of the chunk sees.
+__device__ __forceinline__ int lk_pa_vis(const LkPaArgs & a, const LkSeq & s, int c) {
+    int e = a.mask ? ((c * a.qc) & ~63) + 64 : (c + 1) * a.qc;
+    e = s.len + (e < s.n ? e : s.n);
+    const int cap = a.width << a.page_sh;
+    return e < cap ? e : cap;
+}
+__device__ __forceinline__ int lk_pa_tiles(int vis, int tk_sh) {
+    const int t = (vis + (1 << tk_sh) - 1) >> tk_sh;
+    return t > 0 ? t : 1;                                  // a chunk that sees nothing still has its zeros to write
+}
+__device__ __forceinline__ LkSeq lk_pa_seq(const LkPaArgs & a, int b) {     // by a lane
+    return lk_seq(a.first[b], a.first[b + 1], a.lens[b], a.rows, a.width << a.page_sh);
+}
+__device__ __forceinline__ long lk_pa_seq_tiles(const LkPaArgs & a, const LkSeq & s, int tk_sh) {
+    long n = 0;
+    for (int c = 0; c * a.qc < s.n; ++c) n += lk_pa_tiles(lk_pa_vis(a, s, c), tk_sh);
+    return n * a.nhg;
+}
+
+__device__ __forceinline__ long lk_shfl64(long v, int src) {
+    const int lo = __shfl((int) v, src, 64), hi = __shfl((int) (v >> 32), src, 64);
+    return (long) ((unsigned long) (unsigned) hi << 32 | (unsigned) lo);
+}
+__device__ __forceinline__ long lk_uniform64(long v) {
+    const unsigned lo = __builtin_amdgcn_readfirstlane((int) v), hi = __builtin_amdgcn_readfirstlane((int) (v >> 32));
+    return (long) ((unsigned long) hi << 32 | lo);
+}
+
+// A place on the line: tile t of the nt tiles of (sequence b, chunk c, head group h).
+struct LkPaAt {
+    int b, c, h, t, nt, vis;
+    LkSeq s;
+};
+__device__ __forceinline__ void lk_pa_item(const LkPaArgs & a, LkPaAt & p, int tk_sh) {
+    p.vis = lk_pa_vis(a, p.s, p.c);
+    p.nt = lk_pa_tiles(p.vis, tk_sh);
+}
+// The next tile; behind the last one b is n_seqs.
+__device__ __forceinline__ void lk_pa_next(const LkPaArgs & a, LkPaAt & p, int tk_sh) {
+    if (++p.t < p.nt) return;
+    p.t = 0;
+    if (++p.h < a.nhg) return;
+    p.h = 0;
+    ++p.c;
+    while (p.c * a.qc >= p.s.n) {
+        p.c = 0;
+        if (++p.b >= a.n_seqs) return;
+        p.s = lk_seq(lk_sld(a.first, p.b), lk_sld(a.first, p.b + 1), lk_sld(a.lens, p.b), a.rows, a.width << a.page_sh);
+    }
+    lk_pa_item(a, p, tk_sh);
+}
+
+// tanh of t: below 1/2 by its series (the difference of two numbers near 1 would lose what is
+// left), the first term left out below 2^-26 of the value; above by the exponential.
+__device__ __forceinline__ float lk_tanh(float t) {
+    const float u = fabsf(t), z = t * t;
+    float p = 21844.0f / 6081075.0f;
+    p = __builtin_fmaf(-p, z, 1382.0f / 155925.0f);
+    p = __builtin_fmaf(-p, z, 62.0f / 2835.0f);
+    p = __builtin_fmaf(-p, z, 17.0f / 315.0f);
+    p = __builtin_fmaf(-p, z, 2.0f / 15.0f);
+    p = __builtin_fmaf(-p, z, 1.0f / 3.0f);
+    const float small = __builtin_fmaf(-p * z, u, u);
+    const float e = lk_exp2(u * (-2.0f * LK_LOG2E_F));
+    const float large = (1.0f - e) / (1.0f + e);
+    return copysignf(u < 0.5f ? small : large, t);
+}
+
+// D: head_dim.  RT: rows (LK_F32: q and the weights as two parts).  CT: pools.  CB: blocks of 16
+// columns a wave holds.  STEP: keys a wave takes at once, 32 by K = 32 products of both kinds, 16 by
+// K = 16 for P.V.  NW: waves.  MOD: capped or biased scores.
+template <int D, int RT, int CT, int CB, int STEP, int NW, bool MOD>
+__global__ void __launch_bounds__(64 * NW)
+lk_k_paged_attn(const LkPaArgs a) {
+    typedef LkMm<CT> M;
+    typedef typename M::T T;
+    typedef typename M::V8 V8;
+    typedef typename M::V4 V4;
+    typedef typename LkElem<RT>::type RowT;
+    constexpr bool TWO = RT == LK_F32;
+    constexpr int KS = D / 32, DB = D / 16, DC = D / 8;        // steps of q.k, blocks of output dims, 16-byte pieces of a head's row
+    constexpr int RPW = 32 / NW;                               // DMAs of 1 KB a wave and tile
+    constexpr int AHEAD = LK_PA_NBUF - 1;
+    __shared__ __attribute__((aligned(16))) unsigned char s_tile[LK_PA_NBUF][LK_PA_TILEB];
+    __shared__ lk_f4 s_x[2][NW][64];                           // key shares' rows on their way to one wave
+    __shared__ float2 s_ml[NW][16];
+
+    const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kw = w & ((1 << a.kw_sh) - 1), qw = (w >> a.kw_sh) & ((1 << a.qw_sh) - 1), hh = w >> (a.kw_sh + a.qw_sh);
+    const int rb_sh = a.hg_sh + (D == 64 ? 7 : 8);             // bytes of a position's piece: its group's heads
+    const int rb = 1 << rb_sh;
+    const int tk_sh = 14 - rb_sh;                              // keys a tile: 16 KB of K rows
+    const int kpw = (1 << tk_sh) >> a.kw_sh;                   // of them the wave's
+
+    // ---- this workgroup's run of the line ---------------------------------------------
+    long total = 0, mine = 0, before = 0;
+    LkSeq ls = { 0, 0, 0 };
+    for (int b = lane; b < a.n_seqs; b += 64) {
+        ls = lk_pa_seq(a, b);
+        mine = lk_pa_seq_tiles(a, ls, tk_sh);
+        total += mine;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) total += lk_shfl64(total, lane ^ o);
+    total = lk_uniform64(total);
+    const long share = (total + LK_PA_WGS - 1) / LK_PA_WGS;
+    const long f0 = share * blockIdx.x, f1 = f0 + share < total ? f0 + share : total;
+    if (f0 >= f1) {
+        if (threadIdx.x == 0) a.cut[blockIdx.x] = make_int4(0, 0, 0, 0);
+        return;
+    }
+    LkPaAt at;
+    for (int b0 = 0;; b0 += 64) {                              // ends: f0 is below the total
+        const int b = b0 + lane;
+        if (a.n_seqs > 64) {
+            mine = 0;
+            if (b < a.n_seqs) {
+                ls = lk_pa_seq(a, b);
+                mine = lk_pa_seq_tiles(a, ls, tk_sh);
+            }
+        }
+        long sum = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const long t = lk_shfl64(sum, lane - o & 63);
+            if (lane >= o) sum += t;
+        }
+        const uint64_t here = __ballot(before + sum > f0);
+        if (here) {
+            const int src = __builtin_ctzll(here);
+            long rem = lk_uniform64(lk_shfl64(f0 - before - (sum - mine), src));
+            at.b = b0 + src;
+            at.s.r0 = __builtin_amdgcn_readlane(ls.r0, src);
+            at.s.n = __builtin_amdgcn_readlane(ls.n, src);
+            at.s.len = __builtin_amdgcn_readlane(ls.len, src);
+            for (at.c = 0;; ++at.c) {                          // ends: rem is below the sequence's tiles
+                lk_pa_item(a, at, tk_sh);
+                const long u = (long) at.nt * a.nhg;
+                if (rem < u) break;
+                rem -= u;
+            }
+            at.h = (int) (rem / at.nt);
+            at.t = (int) (rem % at.nt);
+            break;
+        }
+        before += lk_uniform64(lk_shfl64(sum, 63));
+    }
+
+    // ---- fetch: wave w brings the 1 KB pieces w, w + NW, .. of a tile, K before V ----------
+    // Piece i of K holds the keys i * rpp .. of the tile, all in one page (a page is a multiple of 16).
+    // Within a head's row the 16-byte pieces are permuted by the key, so that the lanes' reads below
+    // meet different banks.
+    const int rpp_sh = 10 - rb_sh;
+    const uint32_t lds0 = lk_lds_addr(&s_tile[0][0]);
+    const size_t row_bytes = (size_t) a.hkv * D * 2;
+    auto swk = [](int key) -> int { return key & (DC - 1); };
+    auto swv = [](int key) -> int { return (((key & 3) << 1) | ((key >> 2) & 1) | (key & 8)) & (DC - 1); };
+    const int frow = lane >> (6 - rpp_sh), fpiece = lane & ((1 << (6 - rpp_sh)) - 1);
+    auto fetch = [&](const LkPaAt & p, int slot) {
+        const uint32_t base = lds0 + (uint32_t) slot * LK_PA_TILEB;
+#pragma unroll
+        for (int i = 0; i < RPW / 2; ++i) {
+            const int piece = w + NW * i, k0 = piece << rpp_sh, p0 = (p.t << tk_sh) + k0;
+            const int key = k0 + frow;
+            const int page = p0 < p.vis ? lk_sld(a.table, (long) p.b * a.ldt + (p0 >> a.page_sh)) : -1;
+            const bool ok = page >= 0 && page < a.n_pages;
+            const size_t off = (((size_t) (ok ? page : 0) << a.page_sh) + (p0 & ((1 << a.page_sh) - 1)) + frow) * row_bytes +
+                               (size_t) p.h * rb;
+            const bool live = ok && p0 + frow < p.vis;
+            const int hd = fpiece & ~(DC - 1), jj = fpiece & (DC - 1);
+            const char * ks = a.kp + off + 16 * (hd + (jj ^ swk(key)));
+            const char * vs = a.vp + off + 16 * (hd + (jj ^ swv(key)));
+            const char * zs = a.zeros + 16 * lane;
+            if constexpr (STEP == 16) {                        // few rows: what is read is not read again
+                lk_dma16(live ? ks : zs, base + piece * 1024);
+                lk_dma16(live ? vs : zs, base + LK_PA_TILEB / 2 + piece * 1024);
+            } else {
+                lk_dma16c(live ? ks : zs, base + piece * 1024);
+                lk_dma16c(live ? vs : zs, base + LK_PA_TILEB / 2 + piece * 1024);
+            }
+        }
+    };
+    auto wait_tile = [&](long left) {                          // left: tiles of the run behind this one
+        if (left >= 2)      lk_wait_vm<2 * RPW>();
+        else if (left == 1) lk_wait_vm<RPW>();
+        else                lk_wait_vm<0>();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    static_assert(AHEAD == 3, "wait_tile: two tiles may stay in flight behind the awaited one");
+
+    LkPaAt ft = at;
+    for (int i = 0; i < AHEAD && f0 + i < f1; ++i) {
+        fetch(ft, i);
+        lk_pa_next(a, ft, tk_sh);
+    }
+
+    // ---- a column's state ----------------------------------------------------------------
+    V8 qh[CB][KS], ql[TWO ? CB : 1][KS];
+    lk_f4 acc[CB][DB], accl[CB];
+    float mrun[CB], mneg[CB], csc[CB];                          // running max, -max (0 while it is -inf), score factor
+    uint64_t see[CB];                                           // of the 64 tokens from `base` on
+    float slope[CB];
+    int qpos[CB];
+    int base = 0, orow[CB], ohead[CB];                          // keys below base are seen by all; the column's row (-1: none) and head
+    int crow0 = 0, cm = 0;
+
+    auto begin = [&]() {
+        const int i0 = at.c * a.qc, blk = i0 & ~63;
+        crow0 = at.s.r0 + i0;
+        cm = at.s.n - i0 < a.qc ? at.s.n - i0 : a.qc;
+        const int cap = a.width << a.page_sh;
+        base = at.s.len + blk < cap ? at.s.len + blk : cap;
+        const int limit = at.vis - base;                        // new tokens of the block that have a slot, at most 64
+        const uint64_t lim = limit >= 64 ? ~0ull : limit > 0 ? (1ull << limit) - 1 : 0;
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) {
+            const int c = (qw * CB + cb) * 16 + col, i = c / a.g;
+            const bool live = i < cm;
+            const int row = crow0 + (live ? i : 0), head = (((at.h << a.hg_sh) + hh) * a.g) + (c - i * a.g);
+            orow[cb] = live ? row : -1;
+            ohead[cb] = live ? head : 0;
+            see[cb] = (a.mask ? a.mask[row] : ~0ull >> (63 - ((i0 + (live ? i : 0)) & 63))) & lim;
+            if constexpr (MOD) {
+                slope[cb] = a.slopes ? a.slopes[ohead[cb]] * LK_LOG2E_F : 0.0f;
+                qpos[cb] = a.pos ? a.pos[row] : at.s.len + (row - at.s.r0);
+            }
+            const RowT * src = (const RowT *) a.q + (size_t) row * a.ldq + (size_t) ohead[cb] * D + 8 * g;
+            csc[cb] = MOD ? a.scale : a.sc;
+            if constexpr (TWO) {
+                // both halves must be finite in fp16: a head whose largest value reaches 2^15 is scaled
+                // by a power of two, and its scores back
+                float v[KS][8], am = 0.0f;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    lk_load<8>(src + 32 * ks, v[ks]);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        v[ks][e] = live ? v[ks][e] : 0.0f;
+                        am = fmaxf(am, fabsf(v[ks][e]));
+                    }
+                }
+                am = lk_xrow_max(am);
+                int e2 = 0;
+                if (am >= 32768.0f && am <= 3.4e38f) {
+                    (void) frexpf(am, &e2);
+                    e2 -= 15;
+                    csc[cb] = ldexpf(csc[cb], e2);
+                }
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float x = ldexpf(v[ks][e], -e2);
+                        const T h = (T) x;
+                        qh[cb][ks][e] = h;
+                        ql[cb][ks][e] = (T) (x - (float) h);
+                    }
+            } else {
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    V8 v;
+                    __builtin_memcpy(&v, src + 32 * ks, 16);
+                    qh[cb][ks] = live ? v : V8{};
+                }
+            }
+            mrun[cb] = -INFINITY;
+            mneg[cb] = 0.0f;
+            accl[cb] = (lk_f4){ 0.f, 0.f, 0.f, 0.f };
+#pragma unroll
+            for (int db = 0; db < DB; ++db) acc[cb][db] = (lk_f4){ 0.f, 0.f, 0.f, 0.f };
+        }
+    };
+
+    // ---- one block of 16 keys ---------------------------------------------------------------
+    const int kadr = hh * (D * 2) + col * rb, ksw = g ^ swk(col);
+    const int vadr = hh * (D * 2) + (4 * g + (col >> 2)) * rb + 8 * (col & 1), vsw = swv(4 * g + (col >> 2)) ^ ((col >> 1) & 1);
+    auto kload = [&](const unsigned char * kt, int kb, V8 (&kf)[KS]) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) kf[ks] = *(const V8 *) (kt + kadr + ((kb * 16) << rb_sh) + ((ksw ^ (4 * ks)) << 4));
+    };
+    auto vload = [&](const unsigned char * vt, int kb, int db) -> V4 {
+        return __builtin_bit_cast(V4, lk_ds_tr4(vt + vadr + ((kb * 16) << rb_sh) + ((vsw ^ (2 * db)) << 4)));
+    };
+    auto scores = [&](const V8 (&kf)[KS], int cb) -> lk_f4 {
+        lk_f4 c = { 0.f, 0.f, 0.f, 0.f };
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            c = M::k32(kf[ks], qh[cb][ks], c);
+            if constexpr (TWO) c = M::k32(kf[ks], ql[cb][ks], c);
+        }
+        return c;
+    };
+    // capped and biased scores in units of log2, of keys k0 .. k0 + 3 (k0: the lane's first)
+    auto shaped = [&](lk_f4 & c, int cb, int k0) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            float x = c[r] * csc[cb];
+            if (a.cap > 0.0f) x = a.cap * lk_tanh(x / a.cap);
+            int kp = k0 + r;
+            if (a.pos && kp >= at.s.len && kp < at.vis) kp = a.pos[at.s.r0 + kp - at.s.len];
+            c[r] = __builtin_fmaf(slope[cb], (float) (kp - qpos[cb]), x * LK_LOG2E_F);
+        }
+    };
+    const float one = 1.0f;
+    // raises the running max of column block cb to cover scores v (units of log2)
+    auto raise = [&](int cb, float top) {
+        if (__ballot(top > mrun[cb] + LK_PA_HEADROOM)) {        // wave-uniform
+            const float mx = lk_xrow_max(top);
+            if (mx > mrun[cb] + LK_PA_HEADROOM) {
+                const float f = lk_exp2(mrun[cb] - mx);
+                mrun[cb] = mx;
+                mneg[cb] = -mx;
+#pragma unroll
+                for (int db = 0; db < DB; ++db) acc[cb][db] *= f;
+                accl[cb] *= f;
+            }
+        }
+    };
+    // weights of four scores, and (fp32 rows) what their rounding leaves
+    auto weights = [&](const lk_f4 & c, int cb, V4 & ph, V4 & pl) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float p = lk_exp2(MOD ? c[r] + mneg[cb] : __builtin_fmaf(c[r], csc[cb], mneg[cb]));
+            ph[r] = (T) p;
+            if constexpr (TWO) pl[r] = (T) (p - (float) ph[r]);
+        }
+    };
+    auto top4 = [&](const lk_f4 & c, int cb) -> float {
+        const float t = fmaxf(fmaxf(c[0], c[1]), fmaxf(c[2], c[3]));
+        return MOD ? t : t * csc[cb];
+    };
+    V4 ones4;
+    V8 ones8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ones4[i] = (T) one;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ones8[i] = (T) one;
+
+    // Keys that every row sees.
+    auto step_open = [&](const unsigned char * kt, const unsigned char * vt, int kb, int key0) {
+        constexpr int NB = STEP / 16;
+        V8 kf[NB][KS];
+        V4 ph[CB][NB], pl[TWO ? CB : 1][NB];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) kload(kt, kb + n, kf[n]);
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) {
+            lk_f4 c[NB];
+            float top = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                c[n] = scores(kf[n], cb);
+                if constexpr (MOD) shaped(c[n], cb, key0 + 16 * n + 4 * g);
+                top = fmaxf(top, top4(c[n], cb));
+            }
+            raise(cb, top);
+#pragma unroll
+            for (int n = 0; n < NB; ++n) weights(c[n], cb, ph[cb][n], pl[TWO ? cb : 0][n]);
+        }
+        auto join = [](const V4 & x, const V4 & y) -> V8 { return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7); };
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+            V4 vf[NB];
+#pragma unroll
+            for (int n = 0; n < NB; ++n) vf[n] = vload(vt, kb + n, db);
+#pragma unroll
+            for (int cb = 0; cb < CB; ++cb) {
+                if constexpr (NB == 2) {
+                    const V8 v8 = join(vf[0], vf[1]);
+                    acc[cb][db] = M::k32(v8, join(ph[cb][0], ph[cb][1]), acc[cb][db]);
+                    if constexpr (TWO) acc[cb][db] = M::k32(v8, join(pl[cb][0], pl[cb][1]), acc[cb][db]);
+                } else {
+                    acc[cb][db] = M::k16(vf[0], ph[cb][0], acc[cb][db]);
+                    if constexpr (TWO) acc[cb][db] = M::k16(vf[0], pl[cb][0], acc[cb][db]);
+                }
+            }
+        }
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) {
+            if constexpr (NB == 2) {
+                accl[cb] = M::k32(ones8, join(ph[cb][0], ph[cb][1]), accl[cb]);
+                if constexpr (TWO) accl[cb] = M::k32(ones8, join(pl[cb][0], pl[cb][1]), accl[cb]);
+            } else {
+                accl[cb] = M::k16(ones4, ph[cb][0], accl[cb]);
+                if constexpr (TWO) accl[cb] = M::k16(ones4, pl[cb][0], accl[cb]);
+            }
+        }
+    };
+    // 16 keys of which some rows see only some: the new tokens, and the keys around them.
+    auto step_masked = [&](const unsigned char * kt, const unsigned char * vt, int kb, int key0) {
+        V8 kf[KS];
+        kload(kt, kb, kf);
+        V4 vf[DB];
+        bool odd = false;                                       // an infinity or NaN among the values
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+            vf[db] = vload(vt, kb, db);
+            const lk_u16x4 u = __builtin_bit_cast(lk_u16x4, vf[db]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) odd |= (u[r] & M::INF) == M::INF;
+        }
+        const bool any_odd = __ballot(odd) != 0;                // wave-uniform
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) {
+            lk_f4 c = scores(kf, cb);
+            if constexpr (MOD) shaped(c, cb, key0 + 4 * g);
+            uint32_t sees = 0;                                  // bit r: the column sees the lane's key r
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int d = key0 + 4 * g + r - base;
+                const bool s = d < 0 || (d < 64 && ((see[cb] >> d) & 1));
+                sees |= (uint32_t) s << r;
+                c[r] = s ? c[r] : -INFINITY;
+            }
+            raise(cb, top4(c, cb));
+            V4 ph, pl;
+            weights(c, cb, ph, pl);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)                         // also where the max is still -inf, or a score is NaN
+                if (!((sees >> r) & 1)) {
+                    ph[r] = (T) 0.0f;
+                    if constexpr (TWO) pl[r] = (T) 0.0f;
+                }
+            accl[cb] = M::k16(ones4, ph, accl[cb]);
+            if constexpr (TWO) accl[cb] = M::k16(ones4, pl, accl[cb]);
+            if (!any_odd) {
+#pragma unroll
+                for (int db = 0; db < DB; ++db) {
+                    acc[cb][db] = M::k16(vf[db], ph, acc[cb][db]);
+                    if constexpr (TWO) acc[cb][db] = M::k16(vf[db], pl, acc[cb][db]);
+                }
+                continue;
+            }
+            // 0 times an infinity is NaN: one key after the other, and only the columns that see it
+            for (int k = 0; k < 16; ++k) {
+                const int kg = k >> 2, kr = k & 3;
+                const uint32_t s = __shfl((int) sees, 16 * kg + col, 64);
+                const bool take = (s >> kr) & 1;
+#pragma unroll
+                for (int db = 0; db < DB; ++db) {
+                    V4 v = {};
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) v[r] = g == kg && r == kr ? vf[db][r] : (T) 0.0f;
+                    lk_f4 o = { 0.f, 0.f, 0.f, 0.f };
+                    o = M::k16(v, ph, o);
+                    if constexpr (TWO) {
+                        // (a low part of 0 against an infinity would be NaN: it is left out there)
+                        V4 vl = v;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if ((__builtin_bit_cast(lk_u16x4, v)[r] & M::INF) == M::INF) vl[r] = (T) 0.0f;
+                        o = M::k16(vl, pl, o);
+                    }
+                    if (take) acc[cb][db] += o;
+                }
+            }
+        }
+    };
+    auto consume = [&](int slot) {
+        const unsigned char * kt = s_tile[slot], * vt = kt + LK_PA_TILEB / 2;
+        const int key_t = at.t << tk_sh;
+        for (int k = 0; k < kpw; k += STEP) {
+            const int kk = kw * kpw + k, key0 = key_t + kk;
+            if (key0 + STEP <= base) {
+                step_open(kt, vt, kk >> 4, key0);
+            } else {
+                for (int n = 0; n < STEP / 16; ++n)
+                    if (key0 + 16 * n < at.vis) step_masked(kt, vt, (kk >> 4) + n, key0 + 16 * n);
+            }
+        }
+    };
+
+    // ---- an item's end, or the run's ----------------------------------------------------------
+    // The key shares of a head and its columns meet in the wave with the first of them.
+    auto join_shares = [&]() {
+        const int kws = 1 << a.kw_sh;
+        for (int cb = 0; cb < CB; ++cb) {
+            // (a loop over registers must unroll: the block is picked by selects of the whole state)
+        }
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) {
+            if (g == 0) s_ml[w][col] = make_float2(mrun[cb], accl[cb][0]);
+            __syncthreads();
+            float mx = mrun[cb];
+            for (int k = 0; k < kws; ++k) mx = fmaxf(mx, s_ml[w - kw + k][col].x);
+            const float f = mx == -INFINITY ? 0.0f : lk_exp2(mrun[cb] - mx);
+            float l = 0.0f;
+            for (int k = 0; k < kws; ++k) {
+                const float2 o = s_ml[w - kw + k][col];
+                l += mx == -INFINITY ? 0.0f : o.y * lk_exp2(o.x - mx);
+            }
+            mrun[cb] = mx;
+            accl[cb][0] = l;
+#pragma unroll
+            for (int db = 0; db < DB; db += 2) {
+                s_x[0][w][lane] = acc[cb][db] * f;
+                s_x[1][w][lane] = acc[cb][db + 1] * f;
+                __syncthreads();
+                if (kw == 0) {
+                    lk_f4 o0 = s_x[0][w][lane], o1 = s_x[1][w][lane];
+                    for (int k = 1; k < kws; ++k) {
+                        o0 += s_x[0][w + k][lane];
+                        o1 += s_x[1][w + k][lane];
+                    }
+                    acc[cb][db] = o0;
+                    acc[cb][db + 1] = o1;
+                }
+                __syncthreads();
+            }
+        }
+    };
+    int t_begin = at.t;                                         // the item's first tile in this run
+    const int nblk = CB << (a.qw_sh + a.hg_sh);
+    auto finish = [&](bool whole) {
+        if (a.kw_sh) join_shares();
+        if (kw != 0) return;
+        const int slot = 2 * blockIdx.x + (t_begin == 0);
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) {
+            if (orow[cb] < 0) continue;
+            if (whole) {
+                const float il = accl[cb][0] > 0.0f ? 1.0f / accl[cb][0] : accl[cb][0] == 0.0f ? 0.0f : __builtin_nanf("");
+                RowT * o = (RowT *) a.out + (size_t) orow[cb] * a.ldo + (size_t) ohead[cb] * D + 4 * g;
+#pragma unroll
+                for (int db = 0; db < DB; ++db) {
+                    const float v[4] = { acc[cb][db][0] * il, acc[cb][db][1] * il, acc[cb][db][2] * il, acc[cb][db][3] * il };
+                    lk_store<4>(o + 16 * db, v);
+                }
+            } else {
+                const size_t blk = (size_t) slot * nblk + ((hh << a.qw_sh) + qw) * CB + cb;
+#pragma unroll
+                for (int db = 0; db < DB; ++db) *(lk_f4 *) (a.acc + ((blk * DB + db) * 64 + col * 4 + g) * 4) = acc[cb][db];
+                if (g == 0) a.ml[blk * 16 + col] = make_float2(mrun[cb], accl[cb][0]);
+            }
+        }
+    };
+
+    // ---- the run ---------------------------------------------------------------------------------
+    int4 cut = make_int4(0, 0, 0, 0);
+    bool fresh = true;
+    for (long f = f0; f < f1; ++f) {
+        const int slot = (int) ((f - f0) % LK_PA_NBUF);
+        wait_tile(f1 - 1 - f);
+        // the buffer of tile f - 1: every wave has read it before the barrier above
+        if (f + AHEAD < f1) {
+            fetch(ft, (slot + AHEAD) % LK_PA_NBUF);
+            lk_pa_next(a, ft, tk_sh);
+        }
+        if (fresh) {
+            begin();
+            t_begin = at.t;
+            fresh = false;
+        }
+        consume(slot);
+        const bool last = at.t == at.nt - 1;
+        if (last || f + 1 == f1) {
+            finish(last && t_begin == 0);
+            if (!last && t_begin == 0) {
+                // the workgroups that the rest of the item falls to, this one counted
+                const long end = f + (at.nt - at.t);            // behind the item's last tile
+                cut = make_int4((int) ((end - 1) / share - blockIdx.x + 1), crow0, cm, at.h);
+            }
+            fresh = true;
+        }
+        lk_pa_next(a, at, tk_sh);
+    }
+    if (threadIdx.x == 0) a.cut[blockIdx.x] = cut;
+}
+
+// ---- joining cut items ------------------------------------------------------------------------
+// grid (k, blocks of 16 columns); workgroup (x, blk) joins column block blk of the cut items number x,
+// x + gridDim.x, .. .  Wave v takes the pieces v, v + NV, ..; the waves' sums are joined in order.
+#define LK_PA_JOIN_WAVES 16
+template <int D, int RT>
+__global__ void __launch_bounds__(64 * LK_PA_JOIN_WAVES)
+lk_k_paged_join(const LkPaArgs a, int cb_n) {
+    typedef typename LkElem<RT>::type RowT;
+    constexpr int DB = D / 16, NV = LK_PA_JOIN_WAVES;
+    __shared__ int s_list[LK_PA_WGS];
+    __shared__ int s_count[LK_PA_WGS / 64 + 1];
+    __shared__ float2 s_ml[NV][16];
+    __shared__ lk_f4 s_o[NV][64];
+    const int lane = threadIdx.x & 63, col = lane >> 2, g = lane & 3;      // the partials' order
+    const int v = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+    int4 mine = make_int4(0, 0, 0, 0);
+    uint64_t b = 0;
+    if (v < LK_PA_WGS / 64) {
+        mine = a.cut[threadIdx.x];
+        b = __ballot(mine.x > 0);
+        if (lane == 0) s_count[v] = __builtin_popcountll(b);
+    }
+    __syncthreads();
+    int n = 0, off = 0;
+#pragma unroll
+    for (int k = 0; k < LK_PA_WGS / 64; ++k) {
+        if (k < v) off += s_count[k];
+        n += s_count[k];
+    }
+    if (mine.x > 0) s_list[off + __builtin_popcountll(b & ((1ull << lane) - 1))] = threadIdx.x;
+    __syncthreads();
+
+    const int blk = blockIdx.y, nblk = gridDim.y;
+    for (int x = blockIdx.x; x < n; x += gridDim.x) {
+        const int w0 = s_list[x];
+        const int4 it = a.cut[w0];
+        // the block's columns: kv head hh of the group, column group qw, block cb
+        const int cb = blk % cb_n, qw = (blk / cb_n) & ((1 << a.qw_sh) - 1), hh = blk / cb_n >> a.qw_sh;
+        const int c = (qw * cb_n + cb) * 16 + col, i = c / a.g;
+        const bool live = i < it.z;
+        if (__ballot(live) == 0) continue;                     // the same for every wave
+        float m = -INFINITY, l = 0.0f;
+        lk_f4 o[DB];
+#pragma unroll
+        for (int db = 0; db < DB; ++db) o[db] = (lk_f4){ 0.f, 0.f, 0.f, 0.f };
+        if (live) {
+#pragma unroll 4
+            for (int k = v; k < it.x; k += NV) {
+                const size_t p = (size_t) (2 * (w0 + k) + (k == 0)) * nblk + blk;
+                const float2 ml = a.ml[p * 16 + col];
+                lk_f4 x4[DB];
+#pragma unroll
+                for (int db = 0; db < DB; ++db) x4[db] = *(const lk_f4 *) (a.acc + ((p * DB + db) * 64 + lane) * 4);
+                const float mx = fmaxf(m, ml.x);
+                const float f0 = mx == -INFINITY ? 0.0f : lk_exp2(m - mx), f1 = mx == -INFINITY ? 0.0f : lk_exp2(ml.x - mx);
+                m = mx;
+                l = l * f0 + ml.y * f1;
+#pragma unroll
+                for (int db = 0; db < DB; ++db) o[db] = o[db] * f0 + x4[db] * f1;
+            }
+        }
+        if (g == 0) s_ml[v][col] = make_float2(m, l);
+        __syncthreads();
+        float mx = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) mx = fmaxf(mx, s_ml[k][col].x);
+#pragma unroll
+        for (int k = 0; k < NV; ++k) sum += mx == -INFINITY ? 0.0f : s_ml[k][col].y * lk_exp2(s_ml[k][col].x - mx);
+        const float f = mx == -INFINITY ? 0.0f : lk_exp2(m - mx);
+        const float il = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : __builtin_nanf("");
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+            __syncthreads();
+            s_o[v][lane] = o[db] * f;
+            __syncthreads();
+            if (v == db % NV && live) {
+                lk_f4 r = s_o[0][lane];
+#pragma unroll
+                for (int k = 1; k < NV; ++k) r += s_o[k][lane];
+                const int head = ((it.w << a.hg_sh) + hh) * a.g + (c - i * a.g);
+                RowT * dst = (RowT *) a.out + (size_t) (it.y + i) * a.ldo + (size_t) head * D + 16 * db + 4 * g;
+                const float t[4] = { r[0] * il, r[1] * il, r[2] * il, r[3] * il };
+                lk_store<4>(dst, t);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// ---- host ---------------------------------------------------------------------------------------
+// How a workgroup's waves divide a tile, for chunks of `want` tokens of g query heads a kv head.
+struct LkPaShape { int cb, step, nw, hg_sh, qw_sh, kw_sh, qc; };
+static LkPaShape lk_pa_shape(const lk_pages * p, int type, int max_new) {
+    const int g = p->n_heads / p->n_kv_heads, d = p->head_dim;
+    const int cb_max = type == LK_F32 ? 2 : 4, qw_max = type == LK_F32 ? 8 : 4;       // 256 columns
+    int want = max_new < 1 ? 1 : max_new > 64 ? 64 : max_new;
+    LkPaShape s;
+    const int nb = (want * g + 15) / 16;                       // blocks of columns
+    s.cb = nb >= 3 ? cb_max : nb >= 2 ? 2 : 1;
+    s.qw_sh = 0;
+    while ((s.cb << s.qw_sh) < nb && (1 << s.qw_sh) < qw_max) ++s.qw_sh;
+    s.nw = d == 128 && s.qw_sh == 0 ? 4 : 8;
+    const int qw = 1 << s.qw_sh;
+    s.hg_sh = 0;
+    while ((2 << s.hg_sh) * qw <= s.nw && p->n_kv_heads % (2 << s.hg_sh) == 0) ++s.hg_sh;
+    s.kw_sh = lk_log2(s.nw / qw) - s.hg_sh;
+    // keys a wave and tile: 16 KB of K rows over the group's heads and the key shares
+    const int kpw = 8192 / d * qw / s.nw;
+    s.step = kpw >= 32 ? 32 : 16;
+    int qc = s.cb * 16 * qw / g;                               // at least 1: nb covers g columns
+    if (qc > 64) qc = 64;
+    s.qc = 1 << lk_log2(qc);
+    return s;
+}
+static int lk_pa_blocks(const LkPaShape & s) { return s.cb << (s.qw_sh + s.hg_sh); }
+
+template <int D, int RT, int CT, int CB, int STEP, int NW>
+static void lk_pa_run(const LkPaArgs & a, bool mod, hipStream_t st) {
+    if (mod) hipLaunchKernelGGL((lk_k_paged_attn<D, RT, CT, CB, STEP, NW, true>), dim3(LK_PA_WGS), dim3(64 * NW), 0, st, a);
+    else     hipLaunchKernelGGL((lk_k_paged_attn<D, RT, CT, CB, STEP, NW, false>), dim3(LK_PA_WGS), dim3(64 * NW), 0, st, a);
+}
+template <int RT, int CT>
+static void lk_pa_launch(const LkPaShape & s, int d, const LkPaArgs & a, bool mod, hipStream_t st) {
+    constexpr int CBM = RT == LK_F32 ? 2 : 4;
+    if (d == 64) {
+        if (s.step == 32)    lk_pa_run<64, RT, CT, CBM, 32, 8>(a, mod, st);
+        else if (s.cb == 1)  lk_pa_run<64, RT, CT, 1, 16, 8>(a, mod, st);
+        else if (s.cb == 2)  lk_pa_run<64, RT, CT, 2, 16, 8>(a, mod, st);
+        else if constexpr (CBM == 4) lk_pa_run<64, RT, CT, 4, 16, 8>(a, mod, st);
+    } else {
+        if (s.step == 32)    lk_pa_run<128, RT, CT, CBM, 32, 8>(a, mod, st);
+        else if (s.nw == 8)  lk_pa_run<128, RT, CT, CBM, 16, 8>(a, mod, st);
+        else if (s.cb == 1)  lk_pa_run<128, RT, CT, 1, 16, 4>(a, mod, st);
+        else if (s.cb == 2)  lk_pa_run<128, RT, CT, 2, 16, 4>(a, mod, st);
+        else if constexpr (CBM == 4) lk_pa_run<128, RT, CT, 4, 16, 4>(a, mod, st);
+    }
+}
+
+static __device__ __align__(1024) char lk_pa_zeros[1024];      // never written
+
+// The device address of the zeros, looked up once a device.
+static const char * lk_pa_zeros_at(int & err) {
+    static const char * at[LK_MAX_DEVICES];
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess || dev < 0 || dev >= LK_MAX_DEVICES) {
+        err = lk_fail(e != hipSuccess ? (int) e : (int) hipErrorInvalidDevice, "lk_paged_attn: no usable current device");
+        return nullptr;
+    }
+    const char * p = __atomic_load_n(&at[dev], __ATOMIC_RELAXED);
+    if (!p) {
+        void * q = nullptr;
+        e = hipGetSymbolAddress(&q, HIP_SYMBOL(lk_pa_zeros));
+        if (e != hipSuccess || !q) {
+            err = lk_fail(e != hipSuccess ? (int) e : (int) hipErrorInvalidSymbol, "lk_paged_attn: zeros: %s", hipGetErrorString(e));
+            return nullptr;
+        }
+        p = (const char *) q;
+        __atomic_store_n(&at[dev], p, __ATOMIC_RELAXED);       // every thread stores the same
+    }
+    return p;
+}
+
+extern "C" size_t lk_paged_attn_work_bytes(const lk_pages * pages, int type, int max_new) {
+    static const char * const W = "lk_paged_attn_work_bytes";
+    if (lk_paged_check_pages(W, pages) || lk_paged_check_type(W, pages, type)) return 0;
+    if (max_new < 0) {
+        lk_fail(hipErrorInvalidValue, "%s: max_new %d", W, max_new);
+        return 0;
+    }
+    const size_t blocks = (size_t) 2 * LK_PA_WGS * lk_pa_blocks(lk_pa_shape(pages, type, max_new));
+    return blocks * (16 * pages->head_dim * 4 + 16 * 8) + LK_PA_WGS * 16;
+}
+
+extern "C" int lk_paged_attn(const lk_pages * pages, const lk_step * step, int type, const void * q, int ldq, float scale, float cap,
+                             const float * slopes, void * out, int ldo, void * work, size_t work_bytes, void * stream) {
+    static const char * const W = "lk_paged_attn";
+    if (const int e = lk_paged_check(W, pages, step)) return e;
+    if (const int e = lk_paged_check_type(W, pages, type)) return e;
+    const int d = pages->head_dim, hq = pages->n_heads;
+    if (!(scale > 0.0f) || !(scale < __builtin_inff()) || !(cap >= 0.0f) || !(cap < __builtin_inff()))
+        return lk_fail(hipErrorInvalidValue, "%s: scale %g, cap %g", W, (double) scale, (double) cap);
+    if (step->rows == 0 || step->n_seqs == 0) return 0;
+    if (!q || !out || !work) return lk_fail(hipErrorInvalidValue, "%s: null pointer argument", W);
+    if (ldq < hq * d || ldo < hq * d)
+        return lk_fail(hipErrorInvalidValue, "%s: row strides q %d, out %d for %d heads of %d", W, ldq, ldo, hq, d);
+    const uintptr_t em = (uintptr_t) lk_type_size(type) - 1;
+    if ((((uintptr_t) q | (uintptr_t) out) & em) || ((uintptr_t) slopes & 3) || ((uintptr_t) work & 15))
+        return lk_fail(hipErrorInvalidValue, "%s: misaligned argument (rows by their element, slopes 4 B, work 16 B)", W);
+    const size_t need = lk_paged_attn_work_bytes(pages, type, step->max_new);
+    if (work_bytes < need) return lk_fail(hipErrorInvalidValue, "%s: workspace of %zu bytes, %zu needed", W, work_bytes, need);
+    int err = 0;
+    const char * zeros = lk_pa_zeros_at(err);
+    if (!zeros) return err;
+    const LkPaShape s = lk_pa_shape(pages, type, step->max_new);
+    const int nblk = lk_pa_blocks(s), g = hq / pages->n_kv_heads, nhg = pages->n_kv_heads >> s.hg_sh;
+    const size_t blocks = (size_t) 2 * LK_PA_WGS * nblk;
+    float * acc = (float *) work;
+    float2 * ml = (float2 *) (acc + blocks * 16 * d);
+    const LkPaArgs a = { q, out, (const char *) pages->k, (const char *) pages->v, zeros, step->first, step->lens, step->table, step->pos,
+                         step->mask, slopes, acc, ml, (int4 *) (ml + blocks * 16), ldq, ldo, step->n_seqs, step->rows, step->ldt,
+                         step->width, lk_log2(pages->page), pages->n_pages, hq, pages->n_kv_heads, g, nhg, s.hg_sh, s.qw_sh, s.kw_sh, s.qc,
+                         scale * LK_LOG2E_F, scale, cap };
+    const hipStream_t st = lk_stream(stream);
+    const bool mod = cap > 0.0f || slopes;
+    if (type == LK_F32)      lk_pa_launch<LK_F32, LK_F16>(s, d, a, mod, st);
+    else if (type == LK_F16) lk_pa_launch<LK_F16, LK_F16>(s, d, a, mod, st);
+    else                     lk_pa_launch<LK_BF16, LK_BF16>(s, d, a, mod, st);
+    if (const int e = lk_launch_status(W)) return e;
+    // no more items are cut than there are, nor than there are borders between the workgroups
+    const long items = ((long) step->rows / s.qc + step->n_seqs) * nhg;
+    const dim3 grid((unsigned) (items < LK_PA_WGS - 1 ? items : LK_PA_WGS - 1), nblk);
+    const dim3 block(64 * LK_PA_JOIN_WAVES);
+    if (d == 64) {
+        if (type == LK_F32)      hipLaunchKernelGGL((lk_k_paged_join<64, LK_F32>), grid, block, 0, st, a, s.cb);
+        else if (type == LK_F16) hipLaunchKernelGGL((lk_k_paged_join<64, LK_F16>), grid, block, 0, st, a, s.cb);
+        else                     hipLaunchKernelGGL((lk_k_paged_join<64, LK_BF16>), grid, block, 0, st, a, s.cb);
+    } else {
+        if (type == LK_F32)      hipLaunchKernelGGL((lk_k_paged_join<128, LK_F32>), grid, block, 0, st, a, s.cb);
+        else if (type == LK_F16) hipLaunchKernelGGL((lk_k_paged_join<128, LK_F16>), grid, block, 0, st, a, s.cb);
+        else                     hipLaunchKernelGGL((lk_k_paged_join<128, LK_BF16>), grid, block, 0, st, a, s.cb);
+    }
+    return lk_launch_status(W);
+}

@@ -37,6 +37,7 @@ EXPORTS = (
     "lk_pf_part_bytes", "lk_pf_attn8_ws", "lk_pf_attn_ws", "lk_pf_gsync_limit", "lk_pf_gsync_faults",
     "lk_synth_f32", "lk_norm_q8", "lk_gemm_i8",
     "lk_moe_work_bytes", "lk_moe_q4_0",
+    "lk_paged_append", "lk_paged_attn_work_bytes", "lk_paged_attn", "lk_paged_commit",
 )
 
 
@@ -114,6 +115,10 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
         "lk_moe_work_bytes": ([P, I], S),
         "lk_moe_q4_0": ([P, I, P, I, I, P, I, P, I, P, P, P, S, P], I),
         "lk_gemm_i8": ([P, I, P, P, I, P, I, I, I, I, P, I, P, I, P], I),
+        "lk_paged_append": ([P, P, I, P, I, P, I, P, I, P, P, ctypes.c_float, P, I, I, P, I, P], I),
+        "lk_paged_attn_work_bytes": ([P, I, I], S),
+        "lk_paged_attn": ([P, P, I, P, I, ctypes.c_float, ctypes.c_float, P, P, I, P, S, P], I),
+        "lk_paged_commit": ([P, P, P, I, P, P, P], I),
     }
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)
@@ -678,6 +683,160 @@ class MoeQ4_0:
             _check(rc, "lk_moe_q4_0")
         if work is self._work:
             self._tell(stream)
+
+
+# ---- many sequences over a paged cache ---------------------------------------------
+ROPE_HALVES, ROPE_PAIRS = 0, 1
+
+
+class Pages(ctypes.Structure):
+    """lk_pages (include/lk_attn.h)."""
+    _fields_ = [(n, ctypes.c_int) for n in ("type", "n_heads", "n_kv_heads", "head_dim", "page", "n_pages")] + \
+        [("k", ctypes.c_void_p), ("v", ctypes.c_void_p)]
+
+
+class Step(ctypes.Structure):
+    """lk_step (include/lk_attn.h)."""
+    _fields_ = [("n_seqs", ctypes.c_int), ("rows", ctypes.c_int)] + \
+        [(n, ctypes.c_void_p) for n in ("first", "lens", "table")] + [("ldt", ctypes.c_int), ("width", ctypes.c_int)] + \
+        [("pos", ctypes.c_void_p), ("mask", ctypes.c_void_p), ("max_new", ctypes.c_int)]
+
+
+class PagedStep:
+    """A step's tables (lk_step), shared by all layers: first int32 [n_seqs + 1], lens int32
+    [n_seqs], table int32 [n_seqs][pages], `rows` rows of new tokens; pos int32 [rows] and
+    mask int64 [rows] (64 bits a row) where given; max_new, the largest number of new tokens a
+    sequence has, chooses a kernel.  The tables are read on the device during each call, so a
+    captured call goes on with what they hold when it is replayed.
+    Keeps the tables and the attention's workspace, made at its first use (or `work`, uint8 of
+    PagedCache.work_bytes()): attention calls on a step must be ordered (one stream, or
+    events); calls that may overlap, captured graphs among them, take steps of their own.  A step
+    may be dropped while streams still work on it as far as a workspace of its own goes."""
+
+    def __init__(self, first, lens, table, rows: int, pos=None, mask=None, max_new: int = 0, work=None):
+        import torch
+        if lens.dim() != 1 or table.dim() != 2:
+            raise ValueError("PagedStep: lens must be [sequences], table [sequences, pages]")
+        B, dev, i32 = lens.shape[0], lens.get_device(), torch.int32
+        if dev < 0:
+            raise ValueError("PagedStep: tensors must live in device memory")
+        pt, ldt = _rows2(table, (B, table.shape[1]), i32, dev, "PagedStep: table")
+        self._desc = Step(B, int(rows), _flat(first, (B + 1,), i32, dev, "PagedStep: first"),
+                          _flat(lens, (B,), i32, dev, "PagedStep: lens"), pt, ldt, table.shape[1],
+                          None if pos is None else _flat(pos, (rows,), i32, dev, "PagedStep: pos"),
+                          None if mask is None else _flat(mask, (rows,), torch.int64, dev, "PagedStep: mask"), int(max_new))
+        if work is not None and (work.dtype is not torch.uint8 or work.get_device() != dev or not work.is_contiguous()):
+            raise ValueError("PagedStep: work must be contiguous uint8 on the tables' device")
+        self._ref = ctypes.addressof(self._desc)
+        self._keep = (first, lens, table, pos, mask)
+        self._dev, self.n_seqs, self.rows, self.max_new = dev, B, int(rows), int(max_new)
+        self._work, self._own, self._streams = work, False, set()
+
+    def _workspace(self, n: int, stream):
+        """The workspace, of at least n bytes, known to the allocator as used by the call's stream."""
+        if self._work is None or (self._own and self._work.numel() < n):
+            self._work = _torch.empty(n, dtype=_torch.uint8, device=self._keep[1].device)
+            self._own = True
+            self._streams = {_torch.cuda.current_stream(self._dev).cuda_stream}
+        if self._own and not (stream is None and _raw_stream is not None and _raw_stream(self._dev) in self._streams):
+            s = _torch.cuda.current_stream(self._dev) if stream is None else stream
+            if s.cuda_stream not in self._streams:
+                self._work.record_stream(s)
+                self._streams.add(s.cuda_stream)
+        return self._work
+
+
+class PagedCache:
+    """A layer's paged KV cache: pools k and v, fp16 or bf16 [pages][positions a page][kv heads]
+    [head_dim], read by n_heads query heads.  Rows are fp32 or fp16 with fp16 pools, bf16 with
+    bf16 pools."""
+
+    def __init__(self, k, v, n_heads: int):
+        ty = _type_of(k, "PagedCache")
+        if k.dim() != 4:
+            raise ValueError("PagedCache: pools must be [pages, positions, kv heads, head_dim]")
+        n, page, hkv, d = k.shape
+        dev = k.get_device()
+        if dev < 0:
+            raise ValueError("PagedCache: tensors must live in device memory")
+        self._desc = Pages(ty, int(n_heads), hkv, d, page, n, _flat(k, k.shape, k.dtype, dev, "PagedCache: k"),
+                           _flat(v, k.shape, k.dtype, dev, "PagedCache: v"))
+        self._ref = ctypes.addressof(self._desc)
+        self.k, self.v = k, v
+        self._dev, self._hq, self._hkv, self._d = dev, int(n_heads) * d, hkv * d, d
+        self._scale, self._need = d ** -0.5, {}
+
+    def work_bytes(self, dtype, max_new: int = 0) -> int:
+        """Bytes of attention workspace for rows of a dtype."""
+        n = self._need.get((dtype, max_new))
+        if n is None:
+            ty = _types.get(dtype)
+            if ty is None:
+                raise ValueError(f"PagedCache: fp32, fp16 or bf16 rows, not {dtype}")
+            n = int(load().lk_paged_attn_work_bytes(self._ref, ty, int(max_new)))
+            if n == 0:
+                raise LkError(load().lk_last_error().decode(errors="replace"))
+            self._need[(dtype, max_new)] = n
+        return n
+
+    def append(self, step, k, v, q=None, q_out=None, qn=None, kn=None, freq=None, eps: float = 1e-5, pairs: bool = False,
+               stream=None) -> None:
+        """k and v rows [rows][kv heads * head_dim] to their slots, k normed (weights kn fp32
+        [head_dim], or None: not) and rotated (freq fp32 [pairs of values], or None: not; `pairs`:
+        neighbouring values instead of halves); q [rows][heads * head_dim] the same with qn into
+        q_out (which may be q) (lk_paged_append).  Rows may be parts of wider ones."""
+        ty = _type_of(k, "PagedCache.append")
+        rows, dev, dt = step.rows, self._dev, k.dtype
+        pk, ldk = _rows2(k, (rows, self._hkv), dt, dev, "PagedCache.append: k")
+        pv, ldv = _rows2(v, (rows, self._hkv), dt, dev, "PagedCache.append: v")
+        pq, ldq = _rows2(q, (rows, self._hq), dt, dev, "PagedCache.append: q")
+        po, ldo = _rows2(q_out, (rows, self._hq), dt, dev, "PagedCache.append: q_out")
+        f32 = _torch.float32
+        pqn = None if qn is None else _flat(qn, (self._d,), f32, dev, "PagedCache.append: qn")
+        pkn = None if kn is None else _flat(kn, (self._d,), f32, dev, "PagedCache.append: kn")
+        rot, pf = 0, None
+        if freq is not None:
+            rot, pf = 2 * freq.numel(), _flat(freq, (freq.numel(),), f32, dev, "PagedCache.append: freq")
+        if step._dev != dev:
+            raise ValueError("PagedCache: the step is on another device")
+        rc = _on(dev, stream, (_lib or load()).lk_paged_append, self._ref, step._ref, ty, pq, ldq, pk, ldk, pv, ldv, pqn, pkn, eps,
+                 pf, rot, ROPE_PAIRS if pairs else ROPE_HALVES, po, ldo)
+        if rc:
+            _check(rc, "lk_paged_append")
+
+    def attend(self, step, q, out, scale: Optional[float] = None, cap: float = 0.0, slopes=None, stream=None) -> None:
+        """out = attention of the step's rows q [rows][heads * head_dim] over their sequences' pages
+        and new tokens (lk_paged_attn); scale 1/sqrt(head_dim) unless given, cap > 0: scores capped
+        by cap * tanh(x / cap), slopes fp32 [heads]: a bias of slope times distance."""
+        ty = _type_of(q, "PagedCache.attend")
+        shape, dev, dt = (step.rows, self._hq), self._dev, q.dtype
+        pq, ldq = _rows2(q, shape, dt, dev, "PagedCache.attend: q")
+        po, ldo = _rows2(out, shape, dt, dev, "PagedCache.attend: out")
+        ps = None if slopes is None else _flat(slopes, (self._hq // self._d,), _torch.float32, dev, "PagedCache.attend: slopes")
+        if step._dev != dev:
+            raise ValueError("PagedCache: the step is on another device")
+        work = step._workspace(self.work_bytes(dt, step.max_new), stream)
+        rc = _on(dev, stream, (_lib or load()).lk_paged_attn, self._ref, step._ref, ty, pq, ldq,
+                 self._scale if scale is None else scale, cap, ps, po, ldo, work.data_ptr(), work.numel())
+        if rc:
+            _check(rc, "lk_paged_attn")
+
+    def commit(self, step, path, count, new_lens, stream=None) -> None:
+        """The accepted tokens of each sequence (places path int32 [sequences][most], strictly
+        increasing, count int32 [sequences] of them; path None: the first count) become its next
+        positions; new_lens int32 [sequences] (which may be the step's lens) (lk_paged_commit)."""
+        i32, dev, B = _torch.int32, self._dev, step.n_seqs
+        pp, ldp = None, 0
+        if path is not None:
+            ldp = path.shape[-1]
+            pp = _flat(path, (B, ldp), i32, dev, "PagedCache.commit: path")
+        if step._dev != dev:
+            raise ValueError("PagedCache: the step is on another device")
+        rc = _on(dev, stream, (_lib or load()).lk_paged_commit, self._ref, step._ref, pp, ldp,
+                 _flat(count, (B,), i32, dev, "PagedCache.commit: count"),
+                 _flat(new_lens, (B,), i32, dev, "PagedCache.commit: new_lens"))
+        if rc:
+            _check(rc, "lk_paged_commit")
 
 
 class PrefillCtx:
