@@ -27,6 +27,10 @@
 #define LK_PA_NBUF  4
 #define LK_PA_TILEB 32768          // K rows, then V rows
 #define LK_PA_HEADROOM 8.0f        // the running max is raised when a score passes it by 2^8
+#define LK_PA_NONE  3.0e38f        // minus the running max of no score: 2^(any score in sight - max) is 0 against it
+
+// Waves a workgroup: one kv head's piece of a tile with 16 keys for each where a group has as many heads.
+__host__ __device__ constexpr int lk_pa_waves(int d) { return d == 64 ? 8 : 4; }
 
 typedef short lk_s4 __attribute__((ext_vector_type(4)));
 typedef __bf16 lk_b8 __attribute__((ext_vector_type(8)));
@@ -144,6 +148,11 @@ __device__ __forceinline__ void lk_pa_next(const LkPaArgs & a, LkPaAt & p, int t
     lk_pa_item(a, p, tk_sh);
 }
 
+// 1 / the sum of the weights; a row that sees nothing has the sum 0 and gets zeros.
+__device__ __forceinline__ float lk_pa_inverse(float l) {
+    return l == 0.0f ? 0.0f : 1.0f / l;
+}
+
 // tanh of t: below 1/2 by its series (the difference of two numbers near 1 would lose what is
 // left), the first term left out below 2^-26 of the value; above by the exponential.
 __device__ __forceinline__ float lk_tanh(float t) {
@@ -162,9 +171,9 @@ __device__ __forceinline__ float lk_tanh(float t) {
 
 // D: head_dim.  RT: rows (LK_F32: q and the weights as two parts).  CT: pools.  CB: blocks of 16
 // columns a wave holds.  STEP: keys a wave takes at once, 32 by K = 32 products of both kinds, 16 by
-// K = 16 for P.V.  NW: waves.  MOD: capped or biased scores.
-template <int D, int RT, int CT, int CB, int STEP, int NW, bool MOD>
-__global__ void __launch_bounds__(64 * NW)
+// K = 16 for P.V.  MOD: capped or biased scores.
+template <int D, int RT, int CT, int CB, int STEP, bool MOD>
+__global__ void __launch_bounds__(64 * lk_pa_waves(D))
 lk_k_paged_attn(const LkPaArgs a) {
     typedef LkMm<CT> M;
     typedef typename M::T T;
@@ -172,8 +181,9 @@ lk_k_paged_attn(const LkPaArgs a) {
     typedef typename M::V4 V4;
     typedef typename LkElem<RT>::type RowT;
     constexpr bool TWO = RT == LK_F32;
+    constexpr int NW = lk_pa_waves(D);
     constexpr int KS = D / 32, DB = D / 16, DC = D / 8;        // steps of q.k, blocks of output dims, 16-byte pieces of a head's row
-    constexpr int RPW = 32 / NW;                               // DMAs of 1 KB a wave and tile
+    constexpr int NF = 16 / NW;                                // pieces of 1 KB a wave fetches of a tile's K, and of its V
     constexpr int AHEAD = LK_PA_NBUF - 1;
     __shared__ __attribute__((aligned(16))) unsigned char s_tile[LK_PA_NBUF][LK_PA_TILEB];
     __shared__ lk_f4 s_x[2][NW][64];                           // key shares' rows on their way to one wave
@@ -217,7 +227,7 @@ lk_k_paged_attn(const LkPaArgs a) {
         long sum = mine;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
-            const long t = lk_shfl64(sum, lane - o & 63);
+            const long t = lk_shfl64(sum, (lane - o) & 63);
             if (lane >= o) sum += t;
         }
         const uint64_t here = __ballot(before + sum > f0);
@@ -241,90 +251,85 @@ lk_k_paged_attn(const LkPaArgs a) {
         before += lk_uniform64(lk_shfl64(sum, 63));
     }
 
-    // ---- fetch: wave w brings the 1 KB pieces w, w + NW, .. of a tile, K before V ----------
-    // Piece i of K holds the keys i * rpp .. of the tile, all in one page (a page is a multiple of 16).
+    // ---- fetch: wave w brings the 1 KB pieces w, w + NW, .. of a tile's K and of its V -----
+    // Piece i holds the keys i * rpp .. of the tile, all in one page (a page is a multiple of 16).
     // Within a head's row the 16-byte pieces are permuted by the key, so that the lanes' reads below
-    // meet different banks.
-    const int rpp_sh = 10 - rb_sh;
+    // meet different banks.  The pages of the next tile are asked for a tile ahead.
+    const int rpp_sh = 10 - rb_sh, rpp = 1 << rpp_sh;
     const uint32_t lds0 = lk_lds_addr(&s_tile[0][0]);
-    const size_t row_bytes = (size_t) a.hkv * D * 2;
+    const uint32_t row_bytes = (uint32_t) a.hkv * D * 2;
     auto swk = [](int key) -> int { return key & (DC - 1); };
     auto swv = [](int key) -> int { return (((key & 3) << 1) | ((key >> 2) & 1) | (key & 8)) & (DC - 1); };
-    const int frow = lane >> (6 - rpp_sh), fpiece = lane & ((1 << (6 - rpp_sh)) - 1);
+    const int frow = lane >> (6 - rpp_sh);
+    uint32_t ko[NF], vo[NF];                                   // the lane's bytes from the piece's first row on
+#pragma unroll
+    for (int i = 0; i < NF; ++i) {
+        const int key = ((w + NW * i) << rpp_sh) + frow, piece = lane & ((1 << (6 - rpp_sh)) - 1);
+        const int hd = piece & ~(DC - 1), jj = piece & (DC - 1);
+        ko[i] = frow * row_bytes + 16 * (hd + (jj ^ swk(key)));
+        vo[i] = frow * row_bytes + 16 * (hd + (jj ^ swv(key)));
+    }
+    int pg[NF];
+    auto ask = [&](const LkPaAt & p) {
+#pragma unroll
+        for (int i = 0; i < NF; ++i) {
+            const int p0 = (p.t << tk_sh) + ((w + NW * i) << rpp_sh);
+            pg[i] = lk_sld(a.table, (long) p.b * a.ldt + ((p0 < p.vis ? p0 : 0) >> a.page_sh));
+        }
+    };
     auto fetch = [&](const LkPaAt & p, int slot) {
         const uint32_t base = lds0 + (uint32_t) slot * LK_PA_TILEB;
 #pragma unroll
-        for (int i = 0; i < RPW / 2; ++i) {
-            const int piece = w + NW * i, k0 = piece << rpp_sh, p0 = (p.t << tk_sh) + k0;
-            const int key = k0 + frow;
-            const int page = p0 < p.vis ? lk_sld(a.table, (long) p.b * a.ldt + (p0 >> a.page_sh)) : -1;
-            const bool ok = page >= 0 && page < a.n_pages;
-            const size_t off = (((size_t) (ok ? page : 0) << a.page_sh) + (p0 & ((1 << a.page_sh) - 1)) + frow) * row_bytes +
-                               (size_t) p.h * rb;
-            const bool live = ok && p0 + frow < p.vis;
-            const int hd = fpiece & ~(DC - 1), jj = fpiece & (DC - 1);
-            const char * ks = a.kp + off + 16 * (hd + (jj ^ swk(key)));
-            const char * vs = a.vp + off + 16 * (hd + (jj ^ swv(key)));
-            const char * zs = a.zeros + 16 * lane;
-            if constexpr (STEP == 16) {                        // few rows: what is read is not read again
-                lk_dma16(live ? ks : zs, base + piece * 1024);
-                lk_dma16(live ? vs : zs, base + LK_PA_TILEB / 2 + piece * 1024);
-            } else {
-                lk_dma16c(live ? ks : zs, base + piece * 1024);
-                lk_dma16c(live ? vs : zs, base + LK_PA_TILEB / 2 + piece * 1024);
+        for (int i = 0; i < NF; ++i) {
+            const int piece = w + NW * i, p0 = (p.t << tk_sh) + (piece << rpp_sh);
+            const bool ok = pg[i] >= 0 && pg[i] < a.n_pages;
+            const size_t off = (((size_t) (ok ? pg[i] : 0) << a.page_sh) + (p0 & ((1 << a.page_sh) - 1))) * row_bytes +
+                               ((size_t) p.h << rb_sh);
+            const uint32_t lk = base + piece * 1024, lv = lk + LK_PA_TILEB / 2;
+            if (ok && p0 + rpp <= p.vis) {
+                lk_dma16c_so(a.kp + off, ko[i], lk);
+                lk_dma16c_so(a.vp + off, vo[i], lv);
+            } else {                                           // rows that nobody sees are zeros
+                const bool live = ok && p0 + frow < p.vis;
+                const char * zs = a.zeros + 16 * lane;
+                lk_dma16c(live ? a.kp + off + ko[i] : zs, lk);
+                lk_dma16c(live ? a.vp + off + vo[i] : zs, lv);
             }
         }
     };
-    auto wait_tile = [&](long left) {                          // left: tiles of the run behind this one
-        if (left >= 2)      lk_wait_vm<2 * RPW>();
-        else if (left == 1) lk_wait_vm<RPW>();
-        else                lk_wait_vm<0>();
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-    };
-    static_assert(AHEAD == 3, "wait_tile: two tiles may stay in flight behind the awaited one");
-
-    LkPaAt ft = at;
-    for (int i = 0; i < AHEAD && f0 + i < f1; ++i) {
-        fetch(ft, i);
-        lk_pa_next(a, ft, tk_sh);
-    }
 
     // ---- a column's state ----------------------------------------------------------------
     V8 qh[CB][KS], ql[TWO ? CB : 1][KS];
     lk_f4 acc[CB][DB], accl[CB];
-    float mrun[CB], mneg[CB], csc[CB];                          // running max, -max (0 while it is -inf), score factor
-    uint64_t see[CB];                                           // of the 64 tokens from `base` on
-    float slope[CB];
-    int qpos[CB];
-    int base = 0, orow[CB], ohead[CB];                          // keys below base are seen by all; the column's row (-1: none) and head
-    int crow0 = 0, cm = 0;
-
+    float mneg[CB], fac[TWO ? CB : 1];                          // minus the running max (units of log2); score factor of a scaled q
+    float slope[MOD ? CB : 1];
+    int qpos[MOD ? CB : 1];
+    int base = 0;                                               // keys below it are seen by all of the chunk's rows
+    // column block cb: the token of the chunk, its row of the step, its query head; false: there is none
+    auto column = [&](int cb, int & i, int & row, int & head) -> bool {
+        const int c = (qw * CB + cb) * 16 + col, i0 = at.c * a.qc, m = at.s.n - i0 < a.qc ? at.s.n - i0 : a.qc;
+        i = c / a.g;
+        const int h = c - i * a.g;
+        const bool live = i < m;
+        i = live ? i : 0;
+        row = at.s.r0 + i0 + i;
+        head = ((at.h << a.hg_sh) + hh) * a.g + (live ? h : 0);
+        return live;
+    };
     auto begin = [&]() {
-        const int i0 = at.c * a.qc, blk = i0 & ~63;
-        crow0 = at.s.r0 + i0;
-        cm = at.s.n - i0 < a.qc ? at.s.n - i0 : a.qc;
-        const int cap = a.width << a.page_sh;
+        const int blk = (at.c * a.qc) & ~63, cap = a.width << a.page_sh;
         base = at.s.len + blk < cap ? at.s.len + blk : cap;
-        const int limit = at.vis - base;                        // new tokens of the block that have a slot, at most 64
-        const uint64_t lim = limit >= 64 ? ~0ull : limit > 0 ? (1ull << limit) - 1 : 0;
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) {
-            const int c = (qw * CB + cb) * 16 + col, i = c / a.g;
-            const bool live = i < cm;
-            const int row = crow0 + (live ? i : 0), head = (((at.h << a.hg_sh) + hh) * a.g) + (c - i * a.g);
-            orow[cb] = live ? row : -1;
-            ohead[cb] = live ? head : 0;
-            see[cb] = (a.mask ? a.mask[row] : ~0ull >> (63 - ((i0 + (live ? i : 0)) & 63))) & lim;
+            int i, row, head;
+            const bool live = column(cb, i, row, head);
             if constexpr (MOD) {
-                slope[cb] = a.slopes ? a.slopes[ohead[cb]] * LK_LOG2E_F : 0.0f;
+                slope[cb] = a.slopes ? a.slopes[head] * LK_LOG2E_F : 0.0f;
                 qpos[cb] = a.pos ? a.pos[row] : at.s.len + (row - at.s.r0);
             }
-            const RowT * src = (const RowT *) a.q + (size_t) row * a.ldq + (size_t) ohead[cb] * D + 8 * g;
-            csc[cb] = MOD ? a.scale : a.sc;
+            const RowT * src = (const RowT *) a.q + (size_t) row * a.ldq + (size_t) head * D + 8 * g;
             if constexpr (TWO) {
-                // both halves must be finite in fp16: a head whose largest value reaches 2^15 is scaled
+                // both parts must be finite in fp16: a head whose largest value reaches 2^15 is scaled
                 // by a power of two, and its scores back
                 float v[KS][8], am = 0.0f;
 #pragma unroll
@@ -341,8 +346,8 @@ lk_k_paged_attn(const LkPaArgs a) {
                 if (am >= 32768.0f && am <= 3.4e38f) {
                     (void) frexpf(am, &e2);
                     e2 -= 15;
-                    csc[cb] = ldexpf(csc[cb], e2);
                 }
+                fac[cb] = ldexpf(MOD ? a.scale : a.sc, e2);
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
@@ -360,23 +365,22 @@ lk_k_paged_attn(const LkPaArgs a) {
                     qh[cb][ks] = live ? v : V8{};
                 }
             }
-            mrun[cb] = -INFINITY;
-            mneg[cb] = 0.0f;
+            mneg[cb] = LK_PA_NONE;
             accl[cb] = (lk_f4){ 0.f, 0.f, 0.f, 0.f };
 #pragma unroll
             for (int db = 0; db < DB; ++db) acc[cb][db] = (lk_f4){ 0.f, 0.f, 0.f, 0.f };
         }
     };
 
-    // ---- one block of 16 keys ---------------------------------------------------------------
+    // ---- keys ---------------------------------------------------------------------------------
     const int kadr = hh * (D * 2) + col * rb, ksw = g ^ swk(col);
     const int vadr = hh * (D * 2) + (4 * g + (col >> 2)) * rb + 8 * (col & 1), vsw = swv(4 * g + (col >> 2)) ^ ((col >> 1) & 1);
-    auto kload = [&](const unsigned char * kt, int kb, V8 (&kf)[KS]) {
+    auto kload = [&](const unsigned char * kt, V8 (&kf)[KS]) {
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) kf[ks] = *(const V8 *) (kt + kadr + ((kb * 16) << rb_sh) + ((ksw ^ (4 * ks)) << 4));
+        for (int ks = 0; ks < KS; ++ks) kf[ks] = *(const V8 *) (kt + kadr + ((ksw ^ (4 * ks)) << 4));
     };
-    auto vload = [&](const unsigned char * vt, int kb, int db) -> V4 {
-        return __builtin_bit_cast(V4, lk_ds_tr4(vt + vadr + ((kb * 16) << rb_sh) + ((vsw ^ (2 * db)) << 4)));
+    auto vload = [&](const unsigned char * vt, int db) -> V4 {
+        return __builtin_bit_cast(V4, lk_ds_tr4(vt + vadr + ((vsw ^ (2 * db)) << 4)));
     };
     auto scores = [&](const V8 (&kf)[KS], int cb) -> lk_f4 {
         lk_f4 c = { 0.f, 0.f, 0.f, 0.f };
@@ -387,25 +391,24 @@ lk_k_paged_attn(const LkPaArgs a) {
         }
         return c;
     };
+    auto factor = [&](int cb) -> float { return TWO ? fac[cb] : MOD ? a.scale : a.sc; };
     // capped and biased scores in units of log2, of keys k0 .. k0 + 3 (k0: the lane's first)
     auto shaped = [&](lk_f4 & c, int cb, int k0) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            float x = c[r] * csc[cb];
+            float x = c[r] * factor(cb);
             if (a.cap > 0.0f) x = a.cap * lk_tanh(x / a.cap);
             int kp = k0 + r;
             if (a.pos && kp >= at.s.len && kp < at.vis) kp = a.pos[at.s.r0 + kp - at.s.len];
             c[r] = __builtin_fmaf(slope[cb], (float) (kp - qpos[cb]), x * LK_LOG2E_F);
         }
     };
-    const float one = 1.0f;
-    // raises the running max of column block cb to cover scores v (units of log2)
+    // raises the running max of column block cb to cover a lane's largest score (units of log2)
     auto raise = [&](int cb, float top) {
-        if (__ballot(top > mrun[cb] + LK_PA_HEADROOM)) {        // wave-uniform
+        if (__ballot(top > LK_PA_HEADROOM - mneg[cb])) {        // wave-uniform
             const float mx = lk_xrow_max(top);
-            if (mx > mrun[cb] + LK_PA_HEADROOM) {
-                const float f = lk_exp2(mrun[cb] - mx);
-                mrun[cb] = mx;
+            if (mx > LK_PA_HEADROOM - mneg[cb]) {
+                const float f = lk_exp2(-mneg[cb] - mx);
                 mneg[cb] = -mx;
 #pragma unroll
                 for (int db = 0; db < DB; ++db) acc[cb][db] *= f;
@@ -417,49 +420,46 @@ lk_k_paged_attn(const LkPaArgs a) {
     auto weights = [&](const lk_f4 & c, int cb, V4 & ph, V4 & pl) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const float p = lk_exp2(MOD ? c[r] + mneg[cb] : __builtin_fmaf(c[r], csc[cb], mneg[cb]));
+            const float p = lk_exp2(MOD ? c[r] + mneg[cb] : __builtin_fmaf(c[r], factor(cb), mneg[cb]));
             ph[r] = (T) p;
             if constexpr (TWO) pl[r] = (T) (p - (float) ph[r]);
         }
     };
-    auto top4 = [&](const lk_f4 & c, int cb) -> float {
-        const float t = fmaxf(fmaxf(c[0], c[1]), fmaxf(c[2], c[3]));
-        return MOD ? t : t * csc[cb];
-    };
+    auto top4 = [&](const lk_f4 & c) -> float { return fmaxf(fmaxf(c[0], c[1]), fmaxf(c[2], c[3])); };
+    auto units = [&](float top, int cb) -> float { return MOD ? top : top * factor(cb); };
+    auto join = [](const V4 & x, const V4 & y) -> V8 { return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7); };
     V4 ones4;
-    V8 ones8;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) ones4[i] = (T) one;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) ones8[i] = (T) one;
+    for (int i = 0; i < 4; ++i) ones4[i] = (T) 1.0f;
 
-    // Keys that every row sees.
-    auto step_open = [&](const unsigned char * kt, const unsigned char * vt, int kb, int key0) {
+    // STEP keys that every row sees, the first of them key0.
+    auto step_open = [&](const unsigned char * kt, const unsigned char * vt, int key0) {
         constexpr int NB = STEP / 16;
-        V8 kf[NB][KS];
         V4 ph[CB][NB], pl[TWO ? CB : 1][NB];
+        {
+            V8 kf[NB][KS];
 #pragma unroll
-        for (int n = 0; n < NB; ++n) kload(kt, kb + n, kf[n]);
+            for (int n = 0; n < NB; ++n) kload(kt + ((16 * n) << rb_sh), kf[n]);
 #pragma unroll
-        for (int cb = 0; cb < CB; ++cb) {
-            lk_f4 c[NB];
-            float top = -INFINITY;
+            for (int cb = 0; cb < CB; ++cb) {
+                lk_f4 c[NB];
+                float top = -INFINITY;
 #pragma unroll
-            for (int n = 0; n < NB; ++n) {
-                c[n] = scores(kf[n], cb);
-                if constexpr (MOD) shaped(c[n], cb, key0 + 16 * n + 4 * g);
-                top = fmaxf(top, top4(c[n], cb));
+                for (int n = 0; n < NB; ++n) {
+                    c[n] = scores(kf[n], cb);
+                    if constexpr (MOD) shaped(c[n], cb, key0 + 16 * n + 4 * g);
+                    top = fmaxf(top, top4(c[n]));
+                }
+                raise(cb, units(top, cb));
+#pragma unroll
+                for (int n = 0; n < NB; ++n) weights(c[n], cb, ph[cb][n], pl[TWO ? cb : 0][n]);
             }
-            raise(cb, top);
-#pragma unroll
-            for (int n = 0; n < NB; ++n) weights(c[n], cb, ph[cb][n], pl[TWO ? cb : 0][n]);
         }
-        auto join = [](const V4 & x, const V4 & y) -> V8 { return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7); };
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
             V4 vf[NB];
 #pragma unroll
-            for (int n = 0; n < NB; ++n) vf[n] = vload(vt, kb + n, db);
+            for (int n = 0; n < NB; ++n) vf[n] = vload(vt + ((16 * n) << rb_sh), db);
 #pragma unroll
             for (int cb = 0; cb < CB; ++cb) {
                 if constexpr (NB == 2) {
@@ -475,23 +475,23 @@ lk_k_paged_attn(const LkPaArgs a) {
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) {
             if constexpr (NB == 2) {
-                accl[cb] = M::k32(ones8, join(ph[cb][0], ph[cb][1]), accl[cb]);
-                if constexpr (TWO) accl[cb] = M::k32(ones8, join(pl[cb][0], pl[cb][1]), accl[cb]);
+                accl[cb] = M::k32(join(ones4, ones4), join(ph[cb][0], ph[cb][1]), accl[cb]);
+                if constexpr (TWO) accl[cb] = M::k32(join(ones4, ones4), join(pl[cb][0], pl[cb][1]), accl[cb]);
             } else {
                 accl[cb] = M::k16(ones4, ph[cb][0], accl[cb]);
                 if constexpr (TWO) accl[cb] = M::k16(ones4, pl[cb][0], accl[cb]);
             }
         }
     };
-    // 16 keys of which some rows see only some: the new tokens, and the keys around them.
-    auto step_masked = [&](const unsigned char * kt, const unsigned char * vt, int kb, int key0) {
+    // 16 keys of which some rows may see only some: the new tokens, and the keys around them.
+    auto step_masked = [&](const unsigned char * kt, const unsigned char * vt, int key0, const uint64_t (&see)[CB]) {
         V8 kf[KS];
-        kload(kt, kb, kf);
+        kload(kt, kf);
         V4 vf[DB];
         bool odd = false;                                       // an infinity or NaN among the values
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
-            vf[db] = vload(vt, kb, db);
+            vf[db] = vload(vt, db);
             const lk_u16x4 u = __builtin_bit_cast(lk_u16x4, vf[db]);
 #pragma unroll
             for (int r = 0; r < 4; ++r) odd |= (u[r] & M::INF) == M::INF;
@@ -509,15 +509,9 @@ lk_k_paged_attn(const LkPaArgs a) {
                 sees |= (uint32_t) s << r;
                 c[r] = s ? c[r] : -INFINITY;
             }
-            raise(cb, top4(c, cb));
+            raise(cb, units(top4(c), cb));
             V4 ph, pl;
             weights(c, cb, ph, pl);
-#pragma unroll
-            for (int r = 0; r < 4; ++r)                         // also where the max is still -inf, or a score is NaN
-                if (!((sees >> r) & 1)) {
-                    ph[r] = (T) 0.0f;
-                    if constexpr (TWO) pl[r] = (T) 0.0f;
-                }
             accl[cb] = M::k16(ones4, ph, accl[cb]);
             if constexpr (TWO) accl[cb] = M::k16(ones4, pl, accl[cb]);
             if (!any_odd) {
@@ -529,40 +523,25 @@ lk_k_paged_attn(const LkPaArgs a) {
                 continue;
             }
             // 0 times an infinity is NaN: one key after the other, and only the columns that see it
+#pragma clang loop unroll(disable)
             for (int k = 0; k < 16; ++k) {
                 const int kg = k >> 2, kr = k & 3;
                 const uint32_t s = __shfl((int) sees, 16 * kg + col, 64);
                 const bool take = (s >> kr) & 1;
 #pragma unroll
                 for (int db = 0; db < DB; ++db) {
-                    V4 v = {};
+                    V4 v, vl;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) v[r] = g == kg && r == kr ? vf[db][r] : (T) 0.0f;
+                    for (int r = 0; r < 4; ++r) {
+                        v[r] = g == kg && r == kr ? vf[db][r] : (T) 0.0f;
+                        // (a low part of 0 against an infinity would be NaN: it is left out there)
+                        vl[r] = (__builtin_bit_cast(lk_u16x4, vf[db])[r] & M::INF) == M::INF ? (T) 0.0f : v[r];
+                    }
                     lk_f4 o = { 0.f, 0.f, 0.f, 0.f };
                     o = M::k16(v, ph, o);
-                    if constexpr (TWO) {
-                        // (a low part of 0 against an infinity would be NaN: it is left out there)
-                        V4 vl = v;
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if ((__builtin_bit_cast(lk_u16x4, v)[r] & M::INF) == M::INF) vl[r] = (T) 0.0f;
-                        o = M::k16(vl, pl, o);
-                    }
+                    if constexpr (TWO) o = M::k16(vl, pl, o);
                     if (take) acc[cb][db] += o;
                 }
-            }
-        }
-    };
-    auto consume = [&](int slot) {
-        const unsigned char * kt = s_tile[slot], * vt = kt + LK_PA_TILEB / 2;
-        const int key_t = at.t << tk_sh;
-        for (int k = 0; k < kpw; k += STEP) {
-            const int kk = kw * kpw + k, key0 = key_t + kk;
-            if (key0 + STEP <= base) {
-                step_open(kt, vt, kk >> 4, key0);
-            } else {
-                for (int n = 0; n < STEP / 16; ++n)
-                    if (key0 + 16 * n < at.vis) step_masked(kt, vt, (kk >> 4) + n, key0 + 16 * n);
             }
         }
     };
@@ -571,22 +550,19 @@ lk_k_paged_attn(const LkPaArgs a) {
     // The key shares of a head and its columns meet in the wave with the first of them.
     auto join_shares = [&]() {
         const int kws = 1 << a.kw_sh;
-        for (int cb = 0; cb < CB; ++cb) {
-            // (a loop over registers must unroll: the block is picked by selects of the whole state)
-        }
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) {
-            if (g == 0) s_ml[w][col] = make_float2(mrun[cb], accl[cb][0]);
+            if (g == 0) s_ml[w][col] = make_float2(-mneg[cb], accl[cb][0]);
             __syncthreads();
-            float mx = mrun[cb];
+            float mx = -mneg[cb];
             for (int k = 0; k < kws; ++k) mx = fmaxf(mx, s_ml[w - kw + k][col].x);
-            const float f = mx == -INFINITY ? 0.0f : lk_exp2(mrun[cb] - mx);
+            const float f = lk_exp2(-mneg[cb] - mx);
             float l = 0.0f;
             for (int k = 0; k < kws; ++k) {
                 const float2 o = s_ml[w - kw + k][col];
-                l += mx == -INFINITY ? 0.0f : o.y * lk_exp2(o.x - mx);
+                l += o.y * lk_exp2(o.x - mx);
             }
-            mrun[cb] = mx;
+            mneg[cb] = -mx;
             accl[cb][0] = l;
 #pragma unroll
             for (int db = 0; db < DB; db += 2) {
@@ -606,18 +582,18 @@ lk_k_paged_attn(const LkPaArgs a) {
             }
         }
     };
-    int t_begin = at.t;                                         // the item's first tile in this run
     const int nblk = CB << (a.qw_sh + a.hg_sh);
-    auto finish = [&](bool whole) {
+    auto finish = [&](bool whole, bool from_first) {
         if (a.kw_sh) join_shares();
         if (kw != 0) return;
-        const int slot = 2 * blockIdx.x + (t_begin == 0);
+        const int slot = 2 * blockIdx.x + from_first;
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) {
-            if (orow[cb] < 0) continue;
+            int i, row, head;
+            if (!column(cb, i, row, head)) continue;
             if (whole) {
-                const float il = accl[cb][0] > 0.0f ? 1.0f / accl[cb][0] : accl[cb][0] == 0.0f ? 0.0f : __builtin_nanf("");
-                RowT * o = (RowT *) a.out + (size_t) orow[cb] * a.ldo + (size_t) ohead[cb] * D + 4 * g;
+                const float il = lk_pa_inverse(accl[cb][0]);
+                RowT * o = (RowT *) a.out + (size_t) row * a.ldo + (size_t) head * D + 4 * g;
 #pragma unroll
                 for (int db = 0; db < DB; ++db) {
                     const float v[4] = { acc[cb][db][0] * il, acc[cb][db][1] * il, acc[cb][db][2] * il, acc[cb][db][3] * il };
@@ -627,38 +603,85 @@ lk_k_paged_attn(const LkPaArgs a) {
                 const size_t blk = (size_t) slot * nblk + ((hh << a.qw_sh) + qw) * CB + cb;
 #pragma unroll
                 for (int db = 0; db < DB; ++db) *(lk_f4 *) (a.acc + ((blk * DB + db) * 64 + col * 4 + g) * 4) = acc[cb][db];
-                if (g == 0) a.ml[blk * 16 + col] = make_float2(mrun[cb], accl[cb][0]);
+                if (g == 0) a.ml[blk * 16 + col] = make_float2(-mneg[cb], accl[cb][0]);
             }
         }
     };
 
-    // ---- the run ---------------------------------------------------------------------------------
-    int4 cut = make_int4(0, 0, 0, 0);
-    bool fresh = true;
-    for (long f = f0; f < f1; ++f) {
-        const int slot = (int) ((f - f0) % LK_PA_NBUF);
-        wait_tile(f1 - 1 - f);
-        // the buffer of tile f - 1: every wave has read it before the barrier above
-        if (f + AHEAD < f1) {
-            fetch(ft, (slot + AHEAD) % LK_PA_NBUF);
+    // ---- the run: item by item, in each the tiles that all rows see whole, then the others -------
+    long left = f1 - f0, unfetched = left;                      // tiles of the run to take, to fetch
+    int slot = 0;
+    LkPaAt ft = at;
+    auto advance = [&](int to) {
+        ask(ft);
+        fetch(ft, to);
+        lk_pa_next(a, ft, tk_sh);
+        --unfetched;
+    };
+    for (int i = 0; i < AHEAD && unfetched > 0; ++i) advance(i);
+    if (unfetched > 0) ask(ft);
+    // waits for the tile in `slot`, then asks for the tile AHEAD further, into the buffer that every
+    // wave has read before the barrier
+    auto next_tile = [&]() {
+        if (left > 2)       lk_wait_vm<4 * NF>();
+        else if (left == 2) lk_wait_vm<2 * NF>();
+        else                lk_wait_vm<0>();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (unfetched > 0) {
+            fetch(ft, (slot + AHEAD) & (LK_PA_NBUF - 1));
             lk_pa_next(a, ft, tk_sh);
+            if (--unfetched > 0) ask(ft);
         }
-        if (fresh) {
-            begin();
-            t_begin = at.t;
-            fresh = false;
+    };
+    static_assert(AHEAD == 3, "next_tile: two tiles may stay in flight behind the awaited one");
+    auto done_tile = [&]() {
+        slot = (slot + 1) & (LK_PA_NBUF - 1);
+        --left;
+    };
+    int4 cut = make_int4(0, 0, 0, 0);
+    while (left > 0) {
+        begin();
+        const bool from_first = at.t == 0;
+        const int t_end = left < at.nt - at.t ? at.t + (int) left : at.nt;        // of this item in this run
+        const int t_open = lk_clamp(base >> tk_sh, at.t, t_end);
+        for (; at.t < t_open; ++at.t) {
+            next_tile();
+            const unsigned char * kt = s_tile[slot] + ((kw * kpw) << rb_sh);
+            for (int k = 0; k < kpw; k += STEP)
+                step_open(kt + (k << rb_sh), kt + (k << rb_sh) + LK_PA_TILEB / 2, (at.t << tk_sh) + kw * kpw + k);
+            done_tile();
         }
-        consume(slot);
-        const bool last = at.t == at.nt - 1;
-        if (last || f + 1 == f1) {
-            finish(last && t_begin == 0);
-            if (!last && t_begin == 0) {
-                // the workgroups that the rest of the item falls to, this one counted
-                const long end = f + (at.nt - at.t);            // behind the item's last tile
-                cut = make_int4((int) ((end - 1) / share - blockIdx.x + 1), crow0, cm, at.h);
+        if (at.t < t_end) {
+            uint64_t see[CB];                                   // which of the 64 tokens from `base` on
+            const int limit = at.vis - base;                    // of them the ones that have a slot
+            const uint64_t lim = limit >= 64 ? ~0ull : limit > 0 ? (1ull << limit) - 1 : 0;
+#pragma unroll
+            for (int cb = 0; cb < CB; ++cb) {
+                int i, row, head;
+                (void) column(cb, i, row, head);
+                see[cb] = (a.mask ? a.mask[row] : ~0ull >> (63 - ((at.c * a.qc + i) & 63))) & lim;
             }
-            fresh = true;
+            for (; at.t < t_end; ++at.t) {
+                next_tile();
+                const unsigned char * kt = s_tile[slot];
+                for (int k = kw * kpw; k < kw * kpw + kpw; k += 16) {
+                    const int key0 = (at.t << tk_sh) + k;
+                    if (key0 < at.vis) step_masked(kt + (k << rb_sh), kt + (k << rb_sh) + LK_PA_TILEB / 2, key0, see);
+                }
+                done_tile();
+            }
         }
+        const bool ends = t_end == at.nt;
+        finish(ends && from_first, from_first);
+        if (!ends && from_first) {
+            // the workgroups that the rest of the item falls to, this one counted
+            const long end = f1 + (at.nt - at.t);               // behind the item's last tile
+            const int m = at.s.n - at.c * a.qc;
+            cut = make_int4((int) ((end - 1) / share) - (int) blockIdx.x + 1, at.s.r0 + at.c * a.qc, m < a.qc ? m : a.qc, at.h);
+        }
+        at.t = at.nt - 1;
         lk_pa_next(a, at, tk_sh);
     }
     if (threadIdx.x == 0) a.cut[blockIdx.x] = cut;
@@ -706,7 +729,7 @@ lk_k_paged_join(const LkPaArgs a, int cb_n) {
         const int c = (qw * cb_n + cb) * 16 + col, i = c / a.g;
         const bool live = i < it.z;
         if (__ballot(live) == 0) continue;                     // the same for every wave
-        float m = -INFINITY, l = 0.0f;
+        float m = -LK_PA_NONE, l = 0.0f;
         lk_f4 o[DB];
 #pragma unroll
         for (int db = 0; db < DB; ++db) o[db] = (lk_f4){ 0.f, 0.f, 0.f, 0.f };
@@ -719,7 +742,7 @@ lk_k_paged_join(const LkPaArgs a, int cb_n) {
 #pragma unroll
                 for (int db = 0; db < DB; ++db) x4[db] = *(const lk_f4 *) (a.acc + ((p * DB + db) * 64 + lane) * 4);
                 const float mx = fmaxf(m, ml.x);
-                const float f0 = mx == -INFINITY ? 0.0f : lk_exp2(m - mx), f1 = mx == -INFINITY ? 0.0f : lk_exp2(ml.x - mx);
+                const float f0 = lk_exp2(m - mx), f1 = lk_exp2(ml.x - mx);
                 m = mx;
                 l = l * f0 + ml.y * f1;
 #pragma unroll
@@ -728,13 +751,13 @@ lk_k_paged_join(const LkPaArgs a, int cb_n) {
         }
         if (g == 0) s_ml[v][col] = make_float2(m, l);
         __syncthreads();
-        float mx = -INFINITY, sum = 0.0f;
+        float mx = -LK_PA_NONE, sum = 0.0f;
 #pragma unroll
         for (int k = 0; k < NV; ++k) mx = fmaxf(mx, s_ml[k][col].x);
 #pragma unroll
-        for (int k = 0; k < NV; ++k) sum += mx == -INFINITY ? 0.0f : s_ml[k][col].y * lk_exp2(s_ml[k][col].x - mx);
-        const float f = mx == -INFINITY ? 0.0f : lk_exp2(m - mx);
-        const float il = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : __builtin_nanf("");
+        for (int k = 0; k < NV; ++k) sum += s_ml[k][col].y * lk_exp2(s_ml[k][col].x - mx);
+        const float f = lk_exp2(m - mx);
+        const float il = lk_pa_inverse(sum);
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
             __syncthreads();
@@ -756,51 +779,42 @@ lk_k_paged_join(const LkPaArgs a, int cb_n) {
 
 // ---- host ---------------------------------------------------------------------------------------
 // How a workgroup's waves divide a tile, for chunks of `want` tokens of g query heads a kv head.
-struct LkPaShape { int cb, step, nw, hg_sh, qw_sh, kw_sh, qc; };
+struct LkPaShape { int cb, step, hg_sh, qw_sh, kw_sh, qc; };
 static LkPaShape lk_pa_shape(const lk_pages * p, int type, int max_new) {
-    const int g = p->n_heads / p->n_kv_heads, d = p->head_dim;
-    const int cb_max = type == LK_F32 ? 2 : 4, qw_max = type == LK_F32 ? 8 : 4;       // 256 columns
+    const int g = p->n_heads / p->n_kv_heads, d = p->head_dim, nw = lk_pa_waves(d);
+    const int cb_max = type == LK_F32 ? 2 : 4, qw_max = 16 / cb_max < nw ? 16 / cb_max : nw;     // up to 256 columns
     int want = max_new < 1 ? 1 : max_new > 64 ? 64 : max_new;
     LkPaShape s;
     const int nb = (want * g + 15) / 16;                       // blocks of columns
     s.cb = nb >= 3 ? cb_max : nb >= 2 ? 2 : 1;
     s.qw_sh = 0;
     while ((s.cb << s.qw_sh) < nb && (1 << s.qw_sh) < qw_max) ++s.qw_sh;
-    s.nw = d == 128 && s.qw_sh == 0 ? 4 : 8;
     const int qw = 1 << s.qw_sh;
     s.hg_sh = 0;
-    while ((2 << s.hg_sh) * qw <= s.nw && p->n_kv_heads % (2 << s.hg_sh) == 0) ++s.hg_sh;
-    s.kw_sh = lk_log2(s.nw / qw) - s.hg_sh;
-    // keys a wave and tile: 16 KB of K rows over the group's heads and the key shares
-    const int kpw = 8192 / d * qw / s.nw;
-    s.step = kpw >= 32 ? 32 : 16;
-    int qc = s.cb * 16 * qw / g;                               // at least 1: nb covers g columns
+    while ((2 << s.hg_sh) * qw <= nw && p->n_kv_heads % (2 << s.hg_sh) == 0) ++s.hg_sh;
+    s.kw_sh = lk_log2(nw / qw) - s.hg_sh;
+    // keys a wave and tile: 16 KB of K rows over the group's heads and the key shares, 16 * qw
+    s.step = qw > 1 ? 32 : 16;
+    int qc = s.cb * 16 * qw / g;                               // at least 1: up to 64 heads a kv head
     if (qc > 64) qc = 64;
     s.qc = 1 << lk_log2(qc);
     return s;
 }
 static int lk_pa_blocks(const LkPaShape & s) { return s.cb << (s.qw_sh + s.hg_sh); }
 
-template <int D, int RT, int CT, int CB, int STEP, int NW>
+template <int D, int RT, int CT, int CB, int STEP>
 static void lk_pa_run(const LkPaArgs & a, bool mod, hipStream_t st) {
-    if (mod) hipLaunchKernelGGL((lk_k_paged_attn<D, RT, CT, CB, STEP, NW, true>), dim3(LK_PA_WGS), dim3(64 * NW), 0, st, a);
-    else     hipLaunchKernelGGL((lk_k_paged_attn<D, RT, CT, CB, STEP, NW, false>), dim3(LK_PA_WGS), dim3(64 * NW), 0, st, a);
+    const dim3 block(64 * lk_pa_waves(D));
+    if (mod) hipLaunchKernelGGL((lk_k_paged_attn<D, RT, CT, CB, STEP, true>), dim3(LK_PA_WGS), block, 0, st, a);
+    else     hipLaunchKernelGGL((lk_k_paged_attn<D, RT, CT, CB, STEP, false>), dim3(LK_PA_WGS), block, 0, st, a);
 }
-template <int RT, int CT>
-static void lk_pa_launch(const LkPaShape & s, int d, const LkPaArgs & a, bool mod, hipStream_t st) {
+template <int D, int RT, int CT>
+static void lk_pa_launch(const LkPaShape & s, const LkPaArgs & a, bool mod, hipStream_t st) {
     constexpr int CBM = RT == LK_F32 ? 2 : 4;
-    if (d == 64) {
-        if (s.step == 32)    lk_pa_run<64, RT, CT, CBM, 32, 8>(a, mod, st);
-        else if (s.cb == 1)  lk_pa_run<64, RT, CT, 1, 16, 8>(a, mod, st);
-        else if (s.cb == 2)  lk_pa_run<64, RT, CT, 2, 16, 8>(a, mod, st);
-        else if constexpr (CBM == 4) lk_pa_run<64, RT, CT, 4, 16, 8>(a, mod, st);
-    } else {
-        if (s.step == 32)    lk_pa_run<128, RT, CT, CBM, 32, 8>(a, mod, st);
-        else if (s.nw == 8)  lk_pa_run<128, RT, CT, CBM, 16, 8>(a, mod, st);
-        else if (s.cb == 1)  lk_pa_run<128, RT, CT, 1, 16, 4>(a, mod, st);
-        else if (s.cb == 2)  lk_pa_run<128, RT, CT, 2, 16, 4>(a, mod, st);
-        else if constexpr (CBM == 4) lk_pa_run<128, RT, CT, 4, 16, 4>(a, mod, st);
-    }
+    if (s.step == 32)    lk_pa_run<D, RT, CT, CBM, 32>(a, mod, st);
+    else if (s.cb == 1)  lk_pa_run<D, RT, CT, 1, 16>(a, mod, st);
+    else if (s.cb == 2)  lk_pa_run<D, RT, CT, 2, 16>(a, mod, st);
+    else if constexpr (CBM == 4) lk_pa_run<D, RT, CT, 4, 16>(a, mod, st);
 }
 
 static __device__ __align__(1024) char lk_pa_zeros[1024];      // never written
@@ -870,9 +884,15 @@ extern "C" int lk_paged_attn(const lk_pages * pages, const lk_step * step, int t
                          scale * LK_LOG2E_F, scale, cap };
     const hipStream_t st = lk_stream(stream);
     const bool mod = cap > 0.0f || slopes;
-    if (type == LK_F32)      lk_pa_launch<LK_F32, LK_F16>(s, d, a, mod, st);
-    else if (type == LK_F16) lk_pa_launch<LK_F16, LK_F16>(s, d, a, mod, st);
-    else                     lk_pa_launch<LK_BF16, LK_BF16>(s, d, a, mod, st);
+    if (d == 64) {
+        if (type == LK_F32)      lk_pa_launch<64, LK_F32, LK_F16>(s, a, mod, st);
+        else if (type == LK_F16) lk_pa_launch<64, LK_F16, LK_F16>(s, a, mod, st);
+        else                     lk_pa_launch<64, LK_BF16, LK_BF16>(s, a, mod, st);
+    } else {
+        if (type == LK_F32)      lk_pa_launch<128, LK_F32, LK_F16>(s, a, mod, st);
+        else if (type == LK_F16) lk_pa_launch<128, LK_F16, LK_F16>(s, a, mod, st);
+        else                     lk_pa_launch<128, LK_BF16, LK_BF16>(s, a, mod, st);
+    }
     if (const int e = lk_launch_status(W)) return e;
     // no more items are cut than there are, nor than there are borders between the workgroups
     const long items = ((long) step->rows / s.qc + step->n_seqs) * nhg;
