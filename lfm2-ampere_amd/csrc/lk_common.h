@@ -350,9 +350,13 @@ __device__ __forceinline__ void lk_dma16c(const void * src, uint32_t lds) {
                  :: "v"(src), "s"(lds) : "memory", "m0");
 }
 // The same with a wave-uniform 64-bit base (SGPRs) plus a per-lane 32-bit
-// byte offset: moving the source costs only scalar adds.
+// byte offset: moving the source costs only scalar adds (lk_dma16_so: non-temporal).
 __device__ __forceinline__ void lk_dma16c_so(const void * sbase, uint32_t voff, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                 :: "v"(voff), "s"(sbase), "s"(lds) : "memory", "m0");
+}
+__device__ __forceinline__ void lk_dma16_so(const void * sbase, uint32_t voff, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt"
                  :: "v"(voff), "s"(sbase), "s"(lds) : "memory", "m0");
 }
 #pragma clang diagnostic pop

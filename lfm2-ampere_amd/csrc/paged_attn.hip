@@ -287,8 +287,13 @@ lk_k_paged_attn(const LkPaArgs a) {
                                ((size_t) p.h << rb_sh);
             const uint32_t lk = base + piece * 1024, lv = lk + LK_PA_TILEB / 2;
             if (ok && p0 + rpp <= p.vis) {
-                lk_dma16c_so(a.kp + off, ko[i], lk);
-                lk_dma16c_so(a.vp + off, vo[i], lv);
+                if constexpr (STEP == 16) {                    // up to 64 columns a head: few others read the tile
+                    lk_dma16_so(a.kp + off, ko[i], lk);
+                    lk_dma16_so(a.vp + off, vo[i], lv);
+                } else {
+                    lk_dma16c_so(a.kp + off, ko[i], lk);
+                    lk_dma16c_so(a.vp + off, vo[i], lv);
+                }
             } else {                                           // rows that nobody sees are zeros
                 const bool live = ok && p0 + frow < p.vis;
                 const char * zs = a.zeros + 16 * lane;
@@ -688,25 +693,27 @@ lk_k_paged_attn(const LkPaArgs a) {
 }
 
 // ---- joining cut items ------------------------------------------------------------------------
-// grid (k, blocks of 16 columns); workgroup (x, blk) joins column block blk of the cut items number x,
-// x + gridDim.x, .. .  Wave v takes the pieces v, v + NV, ..; the waves' sums are joined in order.
-#define LK_PA_JOIN_WAVES 16
-template <int D, int RT>
-__global__ void __launch_bounds__(64 * LK_PA_JOIN_WAVES)
+// grid (k, blocks of 16 columns x parts of their dims); workgroup (x, y) joins its block of the cut
+// items number x, x + k, ..  First all pieces' (max, sum) give their weights, then the rows are added
+// with loads that wait for nothing but each other: the threads are divided over the block's live
+// values and as many pieces at once as fit, and their sums are added in order.
+template <int D, int RT, int NT, int DBW>
+__global__ void __launch_bounds__(NT)
 lk_k_paged_join(const LkPaArgs a, int cb_n) {
     typedef typename LkElem<RT>::type RowT;
-    constexpr int DB = D / 16, NV = LK_PA_JOIN_WAVES;
+    constexpr int DB = D / 16, NV = NT / 64;
     __shared__ int s_list[LK_PA_WGS];
-    __shared__ int s_count[LK_PA_WGS / 64 + 1];
-    __shared__ float2 s_ml[NV][16];
-    __shared__ lk_f4 s_o[NV][64];
-    const int lane = threadIdx.x & 63, col = lane >> 2, g = lane & 3;      // the partials' order
-    const int v = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    __shared__ int s_count[LK_PA_WGS / 64];
+    __shared__ float2 s_ml[LK_PA_WGS][16];                     // (max, sum), then (weight, .)
+    __shared__ float s_r[2][NV][16];
+    __shared__ lk_f4 s_o[DBW][NT];
+    const int tid = threadIdx.x, lane = tid & 63, v = __builtin_amdgcn_readfirstlane(tid >> 6);
+    static_assert(NT >= LK_PA_WGS, "a thread for every workgroup's entry");
 
     int4 mine = make_int4(0, 0, 0, 0);
     uint64_t b = 0;
     if (v < LK_PA_WGS / 64) {
-        mine = a.cut[threadIdx.x];
+        mine = a.cut[tid];
         b = __ballot(mine.x > 0);
         if (lane == 0) s_count[v] = __builtin_popcountll(b);
     }
@@ -717,61 +724,73 @@ lk_k_paged_join(const LkPaArgs a, int cb_n) {
         if (k < v) off += s_count[k];
         n += s_count[k];
     }
-    if (mine.x > 0) s_list[off + __builtin_popcountll(b & ((1ull << lane) - 1))] = threadIdx.x;
+    if (mine.x > 0) s_list[off + __builtin_popcountll(b & ((1ull << lane) - 1))] = tid;
     __syncthreads();
 
-    const int blk = blockIdx.y, nblk = gridDim.y;
+    const int blk = blockIdx.y / (DB / DBW), db0 = blockIdx.y % (DB / DBW) * DBW, nblk = gridDim.y / (DB / DBW);
+    // the block's columns: kv head hh of the group, column group qw, block cb
+    const int cb = blk % cb_n, qw = (blk / cb_n) & ((1 << a.qw_sh) - 1), hh = (blk / cb_n) >> a.qw_sh;
+    const int c0 = (qw * cb_n + cb) * 16;
     for (int x = blockIdx.x; x < n; x += gridDim.x) {
         const int w0 = s_list[x];
         const int4 it = a.cut[w0];
-        // the block's columns: kv head hh of the group, column group qw, block cb
-        const int cb = blk % cb_n, qw = (blk / cb_n) & ((1 << a.qw_sh) - 1), hh = blk / cb_n >> a.qw_sh;
-        const int c = (qw * cb_n + cb) * 16 + col, i = c / a.g;
-        const bool live = i < it.z;
-        if (__ballot(live) == 0) continue;                     // the same for every wave
-        float m = -LK_PA_NONE, l = 0.0f;
-        lk_f4 o[DB];
+        const int live = lk_clamp(it.z * a.g - c0, 0, 16);     // columns are (token, head) in order: the live ones come first
+        if (live == 0) continue;                               // the same for every thread
+        auto piece = [&](int k) -> size_t { return (size_t) (2 * (w0 + k) + (k == 0)) * nblk + blk; };
+        // weights
+        const int col = tid & 15;
+        float m = -LK_PA_NONE;
+        for (int k = tid >> 4; k < it.x; k += NT / 16) {
+            const float2 ml = col < live ? a.ml[piece(k) * 16 + col] : make_float2(-LK_PA_NONE, 0.0f);
+            s_ml[k][col] = ml;
+            m = fmaxf(m, ml.x);
+        }
+        m = lk_xrow_max(m);
+        if (lane < 16) s_r[0][v][col] = m;
+        __syncthreads();
 #pragma unroll
-        for (int db = 0; db < DB; ++db) o[db] = (lk_f4){ 0.f, 0.f, 0.f, 0.f };
-        if (live) {
+        for (int k = 0; k < NV; ++k) m = fmaxf(m, s_r[0][k][col]);
+        float l = 0.0f;
+        for (int k = tid >> 4; k < it.x; k += NT / 16) {
+            const float2 ml = s_ml[k][col];
+            const float f = lk_exp2(ml.x - m);
+            s_ml[k][col].x = f;
+            l += ml.y * f;
+        }
+        l = lk_xrow_sum(l);
+        if (lane < 16) s_r[1][v][col] = l;
+        __syncthreads();
+        // rows: E a power of two of at least 4 * live values
+        const int e_sh = live > 8 ? 6 : live > 4 ? 5 : 4, e = tid & ((1 << e_sh) - 1), pp = NT >> e_sh;
+        lk_f4 o[DBW];
+#pragma unroll
+        for (int i = 0; i < DBW; ++i) o[i] = (lk_f4){ 0.f, 0.f, 0.f, 0.f };
+        if (e < 4 * live) {
 #pragma unroll 4
-            for (int k = v; k < it.x; k += NV) {
-                const size_t p = (size_t) (2 * (w0 + k) + (k == 0)) * nblk + blk;
-                const float2 ml = a.ml[p * 16 + col];
-                lk_f4 x4[DB];
+            for (int k = tid >> e_sh; k < it.x; k += pp) {
+                const lk_f4 * src = (const lk_f4 *) a.acc + (piece(k) * DB + db0) * 64 + e;
+                const float f = s_ml[k][e >> 2].x;
 #pragma unroll
-                for (int db = 0; db < DB; ++db) x4[db] = *(const lk_f4 *) (a.acc + ((p * DB + db) * 64 + lane) * 4);
-                const float mx = fmaxf(m, ml.x);
-                const float f0 = lk_exp2(m - mx), f1 = lk_exp2(ml.x - mx);
-                m = mx;
-                l = l * f0 + ml.y * f1;
-#pragma unroll
-                for (int db = 0; db < DB; ++db) o[db] = o[db] * f0 + x4[db] * f1;
+                for (int i = 0; i < DBW; ++i) o[i] += src[64 * i] * f;
             }
         }
-        if (g == 0) s_ml[v][col] = make_float2(m, l);
+#pragma unroll
+        for (int i = 0; i < DBW; ++i) s_o[i][tid] = o[i];
         __syncthreads();
-        float mx = -LK_PA_NONE, sum = 0.0f;
+        for (int u = tid; u < (DBW << e_sh); u += NT) {
+            const int i = u >> e_sh, ee = u & ((1 << e_sh) - 1), cc = ee >> 2;
+            if (cc >= live) continue;
+            lk_f4 r = s_o[i][ee];
+            const int most = pp < it.x ? pp : it.x;
+            for (int k = 1; k < most; ++k) r += s_o[i][(k << e_sh) + ee];
+            float sum = 0.0f;
 #pragma unroll
-        for (int k = 0; k < NV; ++k) mx = fmaxf(mx, s_ml[k][col].x);
-#pragma unroll
-        for (int k = 0; k < NV; ++k) sum += s_ml[k][col].y * lk_exp2(s_ml[k][col].x - mx);
-        const float f = lk_exp2(m - mx);
-        const float il = lk_pa_inverse(sum);
-#pragma unroll
-        for (int db = 0; db < DB; ++db) {
-            __syncthreads();
-            s_o[v][lane] = o[db] * f;
-            __syncthreads();
-            if (v == db % NV && live) {
-                lk_f4 r = s_o[0][lane];
-#pragma unroll
-                for (int k = 1; k < NV; ++k) r += s_o[k][lane];
-                const int head = ((it.w << a.hg_sh) + hh) * a.g + (c - i * a.g);
-                RowT * dst = (RowT *) a.out + (size_t) (it.y + i) * a.ldo + (size_t) head * D + 16 * db + 4 * g;
-                const float t[4] = { r[0] * il, r[1] * il, r[2] * il, r[3] * il };
-                lk_store<4>(dst, t);
-            }
+            for (int k = 0; k < NV; ++k) sum += s_r[1][k][cc];
+            const float il = lk_pa_inverse(sum);
+            const int c = c0 + cc, t = c / a.g, head = ((it.w << a.hg_sh) + hh) * a.g + (c - t * a.g);
+            RowT * dst = (RowT *) a.out + (size_t) (it.y + t) * a.ldo + (size_t) head * D + 16 * (db0 + i) + 4 * (ee & 3);
+            const float w[4] = { r[0] * il, r[1] * il, r[2] * il, r[3] * il };
+            lk_store<4>(dst, w);
         }
         __syncthreads();
     }
@@ -815,6 +834,16 @@ static void lk_pa_launch(const LkPaShape & s, const LkPaArgs & a, bool mod, hipS
     else if (s.cb == 1)  lk_pa_run<D, RT, CT, 1, 16>(a, mod, st);
     else if (s.cb == 2)  lk_pa_run<D, RT, CT, 2, 16>(a, mod, st);
     else if constexpr (CBM == 4) lk_pa_run<D, RT, CT, 4, 16>(a, mod, st);
+}
+
+// Few items are cut into many pieces each: large workgroups, one for every 16 dims of a block of
+// columns.  Many items into few: small ones.
+template <int D, int RT>
+static void lk_pa_join(const LkPaArgs & a, int cuts, int nblk, int cb, hipStream_t st) {
+    if (cuts * nblk <= 256)
+        hipLaunchKernelGGL((lk_k_paged_join<D, RT, 1024, 1>), dim3(cuts, nblk * (D / 16)), dim3(1024), 0, st, a, cb);
+    else
+        hipLaunchKernelGGL((lk_k_paged_join<D, RT, 256, D / 16>), dim3(cuts, nblk), dim3(256), 0, st, a, cb);
 }
 
 static __device__ __align__(1024) char lk_pa_zeros[1024];      // never written
@@ -896,16 +925,15 @@ extern "C" int lk_paged_attn(const lk_pages * pages, const lk_step * step, int t
     if (const int e = lk_launch_status(W)) return e;
     // no more items are cut than there are, nor than there are borders between the workgroups
     const long items = ((long) step->rows / s.qc + step->n_seqs) * nhg;
-    const dim3 grid((unsigned) (items < LK_PA_WGS - 1 ? items : LK_PA_WGS - 1), nblk);
-    const dim3 block(64 * LK_PA_JOIN_WAVES);
+    const int cuts = (int) (items < LK_PA_WGS - 1 ? items : LK_PA_WGS - 1);
     if (d == 64) {
-        if (type == LK_F32)      hipLaunchKernelGGL((lk_k_paged_join<64, LK_F32>), grid, block, 0, st, a, s.cb);
-        else if (type == LK_F16) hipLaunchKernelGGL((lk_k_paged_join<64, LK_F16>), grid, block, 0, st, a, s.cb);
-        else                     hipLaunchKernelGGL((lk_k_paged_join<64, LK_BF16>), grid, block, 0, st, a, s.cb);
+        if (type == LK_F32)      lk_pa_join<64, LK_F32>(a, cuts, nblk, s.cb, st);
+        else if (type == LK_F16) lk_pa_join<64, LK_F16>(a, cuts, nblk, s.cb, st);
+        else                     lk_pa_join<64, LK_BF16>(a, cuts, nblk, s.cb, st);
     } else {
-        if (type == LK_F32)      hipLaunchKernelGGL((lk_k_paged_join<128, LK_F32>), grid, block, 0, st, a, s.cb);
-        else if (type == LK_F16) hipLaunchKernelGGL((lk_k_paged_join<128, LK_F16>), grid, block, 0, st, a, s.cb);
-        else                     hipLaunchKernelGGL((lk_k_paged_join<128, LK_BF16>), grid, block, 0, st, a, s.cb);
+        if (type == LK_F32)      lk_pa_join<128, LK_F32>(a, cuts, nblk, s.cb, st);
+        else if (type == LK_F16) lk_pa_join<128, LK_F16>(a, cuts, nblk, s.cb, st);
+        else                     lk_pa_join<128, LK_BF16>(a, cuts, nblk, s.cb, st);
     }
     return lk_launch_status(W);
 }
