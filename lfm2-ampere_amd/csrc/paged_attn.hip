@@ -22,6 +22,7 @@
 // The sum of the weights comes from the same product (a row of ones), so weights and sum are
 // rounded alike.
 #include "lk_paged.h"
+#include <stdlib.h>
 
 #define LK_PA_WGS   256            // workgroups: one a CU (a ring of 128 KB each)
 #define LK_PA_NBUF  4
@@ -81,6 +82,7 @@ struct LkPaArgs {
     int hq, hkv, g;                // g = query heads a kv head
     int nhg, hg_sh, qw_sh, kw_sh;  // groups of 2^hg_sh kv heads; a workgroup's waves = heads x column groups x key shares
     int qc;                        // tokens a chunk, a power of two up to 64
+    int extra;                     // places of the line an item takes in front of its tiles
     float sc, scale, cap;          // sc = scale * log2(e)
 };
 
@@ -94,7 +96,8 @@ __device__ __forceinline__ int lk_sld(const int32_t * p, long i) {
 #endif
 }
 
-// ---- the line of tiles ----------------------------------------------------------------
+// ---- the line of tiles: every item has a.extra places, for what it costs to begin and end one, and then
+// its tiles ------------------------------------------------------------
 // Tiles of chunk c of a sequence: the keys up to the last one that a row of the chunk sees.
 __device__ __forceinline__ int lk_pa_vis(const LkPaArgs & a, const LkSeq & s, int c) {
     int e = a.mask ? ((c * a.qc) & ~63) + 64 : (c + 1) * a.qc;
@@ -111,7 +114,7 @@ __device__ __forceinline__ LkSeq lk_pa_seq(const LkPaArgs & a, int b) {     // b
 }
 __device__ __forceinline__ long lk_pa_seq_tiles(const LkPaArgs & a, const LkSeq & s, int tk_sh) {
     long n = 0;
-    for (int c = 0; c * a.qc < s.n; ++c) n += lk_pa_tiles(lk_pa_vis(a, s, c), tk_sh);
+    for (int c = 0; c * a.qc < s.n; ++c) n += lk_pa_tiles(lk_pa_vis(a, s, c), tk_sh) + a.extra;
     return n * a.nhg;
 }
 
@@ -168,6 +171,9 @@ __device__ __forceinline__ float lk_tanh(float t) {
     const float large = (1.0f - e) / (1.0f + e);
     return copysignf(u < 0.5f ? small : large, t);
 }
+
+struct LkYes { static constexpr bool value = true; };
+struct LkNo { static constexpr bool value = false; };
 
 // D: head_dim.  RT: rows (LK_F32: q and the weights as two parts).  CT: pools.  CB: blocks of 16
 // columns a wave holds.  STEP: keys a wave takes at once, 32 by K = 32 products of both kinds, 16 by
@@ -240,12 +246,12 @@ lk_k_paged_attn(const LkPaArgs a) {
             at.s.len = __builtin_amdgcn_readlane(ls.len, src);
             for (at.c = 0;; ++at.c) {                          // ends: rem is below the sequence's tiles
                 lk_pa_item(a, at, tk_sh);
-                const long u = (long) at.nt * a.nhg;
+                const long u = (long) (at.nt + a.extra) * a.nhg;
                 if (rem < u) break;
                 rem -= u;
             }
-            at.h = (int) (rem / at.nt);
-            at.t = (int) (rem % at.nt);
+            at.h = (int) (rem / (at.nt + a.extra));
+            at.t = (int) (rem % (at.nt + a.extra)) - a.extra;  // below 0: in front of the first tile
             break;
         }
         before += lk_uniform64(lk_shfl64(sum, 63));
@@ -437,27 +443,107 @@ lk_k_paged_attn(const LkPaArgs a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) ones4[i] = (T) 1.0f;
 
-    // STEP keys that every row sees, the first of them key0.
-    auto step_open = [&](const unsigned char * kt, const unsigned char * vt, int key0) {
+    // STEP keys, the first of them key0.  `some`: there are keys that only some of the rows see (the new
+    // tokens and what shares a step with them), told by `see`.
+    auto step = [&](auto some, const unsigned char * kt, const unsigned char * vt, int key0, const uint64_t (&see)[CB]) {
+        constexpr bool SOME = decltype(some)::value;
         constexpr int NB = STEP / 16;
         V4 ph[CB][NB], pl[TWO ? CB : 1][NB];
+        uint32_t sees[SOME ? CB : 1];                           // bit 4n + r: the column sees the lane's key r of block n
         {
             V8 kf[NB][KS];
 #pragma unroll
             for (int n = 0; n < NB; ++n) kload(kt + ((16 * n) << rb_sh), kf[n]);
+            // two blocks of columns at a time: their products have nothing to wait for each other, and one
+            // test for both says whether a max has to be raised
+            constexpr int CP = CB < 2 ? CB : 2;
 #pragma unroll
-            for (int cb = 0; cb < CB; ++cb) {
-                lk_f4 c[NB];
-                float top = -INFINITY;
+            for (int cp = 0; cp < CB; cp += CP) {
+                lk_f4 c[CP][NB];
+                float top[CP], over = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < CP; ++i)
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) c[i][n] = scores(kf[n], cp + i);
+#pragma unroll
+                for (int i = 0; i < CP; ++i) {
+                    top[i] = -INFINITY;
+                    if constexpr (SOME) sees[cp + i] = 0;
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) {
+                        if constexpr (MOD) shaped(c[i][n], cp + i, key0 + 16 * n + 4 * g);
+                        if constexpr (SOME) {
+                            const int d = key0 + 16 * n + 4 * g - base;
+                            const uint64_t e = see[cp + i];
+                            const uint32_t bits = (uint32_t) (d >= 0 ? (d < 64 ? e >> d : 0) : d > -4 ? e << -d | ((1 << -d) - 1) : 15) & 15;
+                            sees[cp + i] |= bits << (4 * n);
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) c[i][n][r] = (bits >> r) & 1 ? c[i][n][r] : -INFINITY;
+                        }
+                        top[i] = fmaxf(top[i], top4(c[i][n]));
+                    }
+                    over = fmaxf(over, MOD ? top[i] + mneg[cp + i] : __builtin_fmaf(top[i], factor(cp + i), mneg[cp + i]));
+                }
+                if (__ballot(over > LK_PA_HEADROOM)) {          // wave-uniform
+#pragma unroll
+                    for (int i = 0; i < CP; ++i) raise(cp + i, units(top[i], cp + i));
+                }
+#pragma unroll
+                for (int i = 0; i < CP; ++i)
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) weights(c[i][n], cp + i, ph[cp + i][n], pl[TWO ? cp + i : 0][n]);
+            }
+        }
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) {
+            if constexpr (NB == 2) {
+                accl[cb] = M::k32(join(ones4, ones4), join(ph[cb][0], ph[cb][1]), accl[cb]);
+                if constexpr (TWO) accl[cb] = M::k32(join(ones4, ones4), join(pl[cb][0], pl[cb][1]), accl[cb]);
+            } else {
+                accl[cb] = M::k16(ones4, ph[cb][0], accl[cb]);
+                if constexpr (TWO) accl[cb] = M::k16(ones4, pl[cb][0], accl[cb]);
+            }
+        }
+        if constexpr (SOME) {
+            bool odd = false;                                   // an infinity or NaN among the values
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
 #pragma unroll
                 for (int n = 0; n < NB; ++n) {
-                    c[n] = scores(kf[n], cb);
-                    if constexpr (MOD) shaped(c[n], cb, key0 + 16 * n + 4 * g);
-                    top = fmaxf(top, top4(c[n]));
-                }
-                raise(cb, units(top, cb));
+                    const lk_u16x4 u = __builtin_bit_cast(lk_u16x4, vload(vt + ((16 * n) << rb_sh), db));
 #pragma unroll
-                for (int n = 0; n < NB; ++n) weights(c[n], cb, ph[cb][n], pl[TWO ? cb : 0][n]);
+                    for (int r = 0; r < 4; ++r) odd |= (u[r] & M::INF) == M::INF;
+                }
+            if (__ballot(odd)) {                                // wave-uniform
+                // 0 times an infinity is NaN: one key after the other, and only the columns that see it
+#pragma unroll
+                for (int n = 0; n < NB; ++n)
+#pragma clang loop unroll(disable)
+                    for (int k = 0; k < 16; ++k) {
+                        const int kg = k >> 2, kr = k & 3;
+                        bool take[CB];
+#pragma unroll
+                        for (int cb = 0; cb < CB; ++cb) take[cb] = ((uint32_t) __shfl((int) sees[cb], 16 * kg + col, 64) >> (4 * n + kr)) & 1;
+#pragma unroll
+                        for (int db = 0; db < DB; ++db) {
+                            const V4 vf = vload(vt + ((16 * n) << rb_sh), db);
+                            V4 v, vl;
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                v[r] = g == kg && r == kr ? vf[r] : (T) 0.0f;
+                                // (a low part of 0 against an infinity would be NaN: it is left out there)
+                                vl[r] = (__builtin_bit_cast(lk_u16x4, vf)[r] & M::INF) == M::INF ? (T) 0.0f : v[r];
+                            }
+#pragma unroll
+                            for (int cb = 0; cb < CB; ++cb) {
+                                lk_f4 o = { 0.f, 0.f, 0.f, 0.f };
+                                o = M::k16(v, ph[cb][n], o);
+                                if constexpr (TWO) o = M::k16(vl, pl[cb][n], o);
+                                if (take[cb]) acc[cb][db] += o;
+                            }
+                        }
+                    }
+                return;
             }
         }
 #pragma unroll
@@ -474,78 +560,6 @@ lk_k_paged_attn(const LkPaArgs a) {
                 } else {
                     acc[cb][db] = M::k16(vf[0], ph[cb][0], acc[cb][db]);
                     if constexpr (TWO) acc[cb][db] = M::k16(vf[0], pl[cb][0], acc[cb][db]);
-                }
-            }
-        }
-#pragma unroll
-        for (int cb = 0; cb < CB; ++cb) {
-            if constexpr (NB == 2) {
-                accl[cb] = M::k32(join(ones4, ones4), join(ph[cb][0], ph[cb][1]), accl[cb]);
-                if constexpr (TWO) accl[cb] = M::k32(join(ones4, ones4), join(pl[cb][0], pl[cb][1]), accl[cb]);
-            } else {
-                accl[cb] = M::k16(ones4, ph[cb][0], accl[cb]);
-                if constexpr (TWO) accl[cb] = M::k16(ones4, pl[cb][0], accl[cb]);
-            }
-        }
-    };
-    // 16 keys of which some rows may see only some: the new tokens, and the keys around them.
-    auto step_masked = [&](const unsigned char * kt, const unsigned char * vt, int key0, const uint64_t (&see)[CB]) {
-        V8 kf[KS];
-        kload(kt, kf);
-        V4 vf[DB];
-        bool odd = false;                                       // an infinity or NaN among the values
-#pragma unroll
-        for (int db = 0; db < DB; ++db) {
-            vf[db] = vload(vt, db);
-            const lk_u16x4 u = __builtin_bit_cast(lk_u16x4, vf[db]);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) odd |= (u[r] & M::INF) == M::INF;
-        }
-        const bool any_odd = __ballot(odd) != 0;                // wave-uniform
-#pragma unroll
-        for (int cb = 0; cb < CB; ++cb) {
-            lk_f4 c = scores(kf, cb);
-            if constexpr (MOD) shaped(c, cb, key0 + 4 * g);
-            uint32_t sees = 0;                                  // bit r: the column sees the lane's key r
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int d = key0 + 4 * g + r - base;
-                const bool s = d < 0 || (d < 64 && ((see[cb] >> d) & 1));
-                sees |= (uint32_t) s << r;
-                c[r] = s ? c[r] : -INFINITY;
-            }
-            raise(cb, units(top4(c), cb));
-            V4 ph, pl;
-            weights(c, cb, ph, pl);
-            accl[cb] = M::k16(ones4, ph, accl[cb]);
-            if constexpr (TWO) accl[cb] = M::k16(ones4, pl, accl[cb]);
-            if (!any_odd) {
-#pragma unroll
-                for (int db = 0; db < DB; ++db) {
-                    acc[cb][db] = M::k16(vf[db], ph, acc[cb][db]);
-                    if constexpr (TWO) acc[cb][db] = M::k16(vf[db], pl, acc[cb][db]);
-                }
-                continue;
-            }
-            // 0 times an infinity is NaN: one key after the other, and only the columns that see it
-#pragma clang loop unroll(disable)
-            for (int k = 0; k < 16; ++k) {
-                const int kg = k >> 2, kr = k & 3;
-                const uint32_t s = __shfl((int) sees, 16 * kg + col, 64);
-                const bool take = (s >> kr) & 1;
-#pragma unroll
-                for (int db = 0; db < DB; ++db) {
-                    V4 v, vl;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        v[r] = g == kg && r == kr ? vf[db][r] : (T) 0.0f;
-                        // (a low part of 0 against an infinity would be NaN: it is left out there)
-                        vl[r] = (__builtin_bit_cast(lk_u16x4, vf[db])[r] & M::INF) == M::INF ? (T) 0.0f : v[r];
-                    }
-                    lk_f4 o = { 0.f, 0.f, 0.f, 0.f };
-                    o = M::k16(v, ph, o);
-                    if constexpr (TWO) o = M::k16(vl, pl, o);
-                    if (take) acc[cb][db] += o;
                 }
             }
         }
@@ -614,35 +628,43 @@ lk_k_paged_attn(const LkPaArgs a) {
     };
 
     // ---- the run: item by item, in each the tiles that all rows see whole, then the others -------
-    long left = f1 - f0, unfetched = left;                      // tiles of the run to take, to fetch
-    int slot = 0;
-    LkPaAt ft = at;
-    auto advance = [&](int to) {
-        ask(ft);
-        fetch(ft, to);
+    // Places of the run behind the current one; an item's last piece may end in front of its first tile.
+    long left = f1 - f0;
+    if (at.t < 0) {
+        left += at.t;
+        at.t = 0;
+        if (left <= 0) {
+            if (threadIdx.x == 0) a.cut[blockIdx.x] = make_int4(0, 0, 0, 0);
+            return;
+        }
+    }
+    LkPaAt ft = at;                                             // the next tile to fetch
+    long ft_left = left;                                        // places of the run from it on
+    int slot = 0, ahead = 0;                                    // the awaited tile's buffer; tiles fetched and not yet taken
+    auto fetch_next = [&]() {
+        fetch(ft, (slot + ahead) & (LK_PA_NBUF - 1));
+        ++ahead;
+        ft_left -= ft.t + 1 == ft.nt ? 1 + a.extra : 1;
         lk_pa_next(a, ft, tk_sh);
-        --unfetched;
+        if (ft_left > 0) ask(ft);
     };
-    for (int i = 0; i < AHEAD && unfetched > 0; ++i) advance(i);
-    if (unfetched > 0) ask(ft);
+    ask(ft);
+    for (int i = 0; i < AHEAD && ft_left > 0; ++i) fetch_next();
     // waits for the tile in `slot`, then asks for the tile AHEAD further, into the buffer that every
     // wave has read before the barrier
     auto next_tile = [&]() {
-        if (left > 2)       lk_wait_vm<4 * NF>();
-        else if (left == 2) lk_wait_vm<2 * NF>();
-        else                lk_wait_vm<0>();
+        if (ahead > 2)       lk_wait_vm<4 * NF>();
+        else if (ahead == 2) lk_wait_vm<2 * NF>();
+        else                 lk_wait_vm<0>();
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (unfetched > 0) {
-            fetch(ft, (slot + AHEAD) & (LK_PA_NBUF - 1));
-            lk_pa_next(a, ft, tk_sh);
-            if (--unfetched > 0) ask(ft);
-        }
+        if (ft_left > 0) fetch_next();
     };
     static_assert(AHEAD == 3, "next_tile: two tiles may stay in flight behind the awaited one");
     auto done_tile = [&]() {
         slot = (slot + 1) & (LK_PA_NBUF - 1);
+        --ahead;
         --left;
     };
     int4 cut = make_int4(0, 0, 0, 0);
@@ -651,16 +673,16 @@ lk_k_paged_attn(const LkPaArgs a) {
         const bool from_first = at.t == 0;
         const int t_end = left < at.nt - at.t ? at.t + (int) left : at.nt;        // of this item in this run
         const int t_open = lk_clamp(base >> tk_sh, at.t, t_end);
+        uint64_t see[CB] = {};
         for (; at.t < t_open; ++at.t) {
             next_tile();
             const unsigned char * kt = s_tile[slot] + ((kw * kpw) << rb_sh);
             for (int k = 0; k < kpw; k += STEP)
-                step_open(kt + (k << rb_sh), kt + (k << rb_sh) + LK_PA_TILEB / 2, (at.t << tk_sh) + kw * kpw + k);
+                step(LkNo(), kt + (k << rb_sh), kt + (k << rb_sh) + LK_PA_TILEB / 2, (at.t << tk_sh) + kw * kpw + k, see);
             done_tile();
         }
         if (at.t < t_end) {
-            uint64_t see[CB];                                   // which of the 64 tokens from `base` on
-            const int limit = at.vis - base;                    // of them the ones that have a slot
+            const int limit = at.vis - base;                    // of the 64 tokens from base on the ones that have a slot
             const uint64_t lim = limit >= 64 ? ~0ull : limit > 0 ? (1ull << limit) - 1 : 0;
 #pragma unroll
             for (int cb = 0; cb < CB; ++cb) {
@@ -670,10 +692,10 @@ lk_k_paged_attn(const LkPaArgs a) {
             }
             for (; at.t < t_end; ++at.t) {
                 next_tile();
-                const unsigned char * kt = s_tile[slot];
-                for (int k = kw * kpw; k < kw * kpw + kpw; k += 16) {
-                    const int key0 = (at.t << tk_sh) + k;
-                    if (key0 < at.vis) step_masked(kt + (k << rb_sh), kt + (k << rb_sh) + LK_PA_TILEB / 2, key0, see);
+                const unsigned char * kt = s_tile[slot] + ((kw * kpw) << rb_sh);
+                for (int k = 0; k < kpw; k += STEP) {
+                    const int key0 = (at.t << tk_sh) + kw * kpw + k;
+                    if (key0 < at.vis) step(LkYes(), kt + (k << rb_sh), kt + (k << rb_sh) + LK_PA_TILEB / 2, key0, see);
                 }
                 done_tile();
             }
@@ -682,10 +704,11 @@ lk_k_paged_attn(const LkPaArgs a) {
         finish(ends && from_first, from_first);
         if (!ends && from_first) {
             // the workgroups that the rest of the item falls to, this one counted
-            const long end = f1 + (at.nt - at.t);               // behind the item's last tile
+            const long end = f1 + (at.nt - t_end);              // behind the item's last tile
             const int m = at.s.n - at.c * a.qc;
             cut = make_int4((int) ((end - 1) / share) - (int) blockIdx.x + 1, at.s.r0 + at.c * a.qc, m < a.qc ? m : a.qc, at.h);
         }
+        left -= a.extra;
         at.t = at.nt - 1;
         lk_pa_next(a, at, tk_sh);
     }
@@ -695,18 +718,19 @@ lk_k_paged_attn(const LkPaArgs a) {
 // ---- joining cut items ------------------------------------------------------------------------
 // grid (k, blocks of 16 columns x parts of their dims); workgroup (x, y) joins its block of the cut
 // items number x, x + k, ..  First all pieces' (max, sum) give their weights, then the rows are added
-// with loads that wait for nothing but each other: the threads are divided over the block's live
-// values and as many pieces at once as fit, and their sums are added in order.
-template <int D, int RT, int NT, int DBW>
-__global__ void __launch_bounds__(NT)
+// with loads that wait for nothing but each other, in the order of the pieces or of the threads' shares
+// of them.  Few items (SPREAD): they are cut into many pieces, so a workgroup has 16 dims of a block, and its
+// threads share the pieces out among them.  Many items: a workgroup has all dims, each wave some of them.
+template <int D, int RT, bool SPREAD>
+__global__ void __launch_bounds__(SPREAD ? 1024 : 256)
 lk_k_paged_join(const LkPaArgs a, int cb_n) {
     typedef typename LkElem<RT>::type RowT;
-    constexpr int DB = D / 16, NV = NT / 64;
+    constexpr int DB = D / 16, NT = SPREAD ? 1024 : 256, NV = NT / 64, PARTS = SPREAD ? DB : 1;
     __shared__ int s_list[LK_PA_WGS];
     __shared__ int s_count[LK_PA_WGS / 64];
-    __shared__ float2 s_ml[LK_PA_WGS][16];                     // (max, sum), then (weight, .)
+    __shared__ float s_w[LK_PA_WGS][16];                       // max, then weight
     __shared__ float s_r[2][NV][16];
-    __shared__ lk_f4 s_o[DBW][NT];
+    __shared__ lk_f4 s_o[SPREAD ? NT : 1];
     const int tid = threadIdx.x, lane = tid & 63, v = __builtin_amdgcn_readfirstlane(tid >> 6);
     static_assert(NT >= LK_PA_WGS, "a thread for every workgroup's entry");
 
@@ -724,10 +748,11 @@ lk_k_paged_join(const LkPaArgs a, int cb_n) {
         if (k < v) off += s_count[k];
         n += s_count[k];
     }
+    if ((int) blockIdx.x >= n) return;
     if (mine.x > 0) s_list[off + __builtin_popcountll(b & ((1ull << lane) - 1))] = tid;
     __syncthreads();
 
-    const int blk = blockIdx.y / (DB / DBW), db0 = blockIdx.y % (DB / DBW) * DBW, nblk = gridDim.y / (DB / DBW);
+    const int blk = blockIdx.y / PARTS, nblk = gridDim.y / PARTS;
     // the block's columns: kv head hh of the group, column group qw, block cb
     const int cb = blk % cb_n, qw = (blk / cb_n) & ((1 << a.qw_sh) - 1), hh = (blk / cb_n) >> a.qw_sh;
     const int c0 = (qw * cb_n + cb) * 16;
@@ -741,9 +766,9 @@ lk_k_paged_join(const LkPaArgs a, int cb_n) {
         const int col = tid & 15;
         float m = -LK_PA_NONE;
         for (int k = tid >> 4; k < it.x; k += NT / 16) {
-            const float2 ml = col < live ? a.ml[piece(k) * 16 + col] : make_float2(-LK_PA_NONE, 0.0f);
-            s_ml[k][col] = ml;
-            m = fmaxf(m, ml.x);
+            const float x0 = col < live ? a.ml[piece(k) * 16 + col].x : -LK_PA_NONE;
+            s_w[k][col] = x0;
+            m = fmaxf(m, x0);
         }
         m = lk_xrow_max(m);
         if (lane < 16) s_r[0][v][col] = m;
@@ -752,45 +777,56 @@ lk_k_paged_join(const LkPaArgs a, int cb_n) {
         for (int k = 0; k < NV; ++k) m = fmaxf(m, s_r[0][k][col]);
         float l = 0.0f;
         for (int k = tid >> 4; k < it.x; k += NT / 16) {
-            const float2 ml = s_ml[k][col];
-            const float f = lk_exp2(ml.x - m);
-            s_ml[k][col].x = f;
-            l += ml.y * f;
+            const float f = lk_exp2(s_w[k][col] - m);
+            s_w[k][col] = f;
+            l += col < live ? a.ml[piece(k) * 16 + col].y * f : 0.0f;
         }
         l = lk_xrow_sum(l);
         if (lane < 16) s_r[1][v][col] = l;
         __syncthreads();
-        // rows: E a power of two of at least 4 * live values
-        const int e_sh = live > 8 ? 6 : live > 4 ? 5 : 4, e = tid & ((1 << e_sh) - 1), pp = NT >> e_sh;
-        lk_f4 o[DBW];
-#pragma unroll
-        for (int i = 0; i < DBW; ++i) o[i] = (lk_f4){ 0.f, 0.f, 0.f, 0.f };
-        if (e < 4 * live) {
-#pragma unroll 4
-            for (int k = tid >> e_sh; k < it.x; k += pp) {
-                const lk_f4 * src = (const lk_f4 *) a.acc + (piece(k) * DB + db0) * 64 + e;
-                const float f = s_ml[k][e >> 2].x;
-#pragma unroll
-                for (int i = 0; i < DBW; ++i) o[i] += src[64 * i] * f;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < DBW; ++i) s_o[i][tid] = o[i];
-        __syncthreads();
-        for (int u = tid; u < (DBW << e_sh); u += NT) {
-            const int i = u >> e_sh, ee = u & ((1 << e_sh) - 1), cc = ee >> 2;
-            if (cc >= live) continue;
-            lk_f4 r = s_o[i][ee];
-            const int most = pp < it.x ? pp : it.x;
-            for (int k = 1; k < most; ++k) r += s_o[i][(k << e_sh) + ee];
+        auto store = [&](int db, int e, lk_f4 r) {             // value e: column e / 4, dims 4 * (e % 4) of the block
+            const int cc = e >> 2;
             float sum = 0.0f;
 #pragma unroll
             for (int k = 0; k < NV; ++k) sum += s_r[1][k][cc];
             const float il = lk_pa_inverse(sum);
             const int c = c0 + cc, t = c / a.g, head = ((it.w << a.hg_sh) + hh) * a.g + (c - t * a.g);
-            RowT * dst = (RowT *) a.out + (size_t) (it.y + t) * a.ldo + (size_t) head * D + 16 * (db0 + i) + 4 * (ee & 3);
+            RowT * dst = (RowT *) a.out + (size_t) (it.y + t) * a.ldo + (size_t) head * D + 16 * db + 4 * (e & 3);
             const float w[4] = { r[0] * il, r[1] * il, r[2] * il, r[3] * il };
             lk_store<4>(dst, w);
+        };
+        if constexpr (SPREAD) {
+            const int db = blockIdx.y % PARTS;
+            const int e_sh = live > 8 ? 6 : live > 4 ? 5 : 4, e = tid & ((1 << e_sh) - 1), pp = NT >> e_sh;
+            lk_f4 o = { 0.f, 0.f, 0.f, 0.f };
+            if (e < 4 * live) {
+#pragma unroll 4
+                for (int k = tid >> e_sh; k < it.x; k += pp)
+                    o += ((const lk_f4 *) a.acc)[(piece(k) * DB + db) * 64 + e] * s_w[k][e >> 2];
+            }
+            s_o[tid] = o;
+            __syncthreads();
+            if (tid < 4 * live) {
+                lk_f4 r = s_o[tid];
+                const int most = pp < it.x ? pp : it.x;
+                for (int k = 1; k < most; ++k) r += s_o[(k << e_sh) + tid];
+                store(db, tid, r);
+            }
+        } else {
+            constexpr int W = DB / NV;                          // blocks of dims a wave
+            if (lane < 4 * live) {
+                lk_f4 o[W];
+#pragma unroll
+                for (int i = 0; i < W; ++i) o[i] = (lk_f4){ 0.f, 0.f, 0.f, 0.f };
+#pragma unroll 4
+                for (int k = 0; k < it.x; ++k) {
+                    const float f = s_w[k][lane >> 2];
+#pragma unroll
+                    for (int i = 0; i < W; ++i) o[i] += ((const lk_f4 *) a.acc)[(piece(k) * DB + v * W + i) * 64 + lane] * f;
+                }
+#pragma unroll
+                for (int i = 0; i < W; ++i) store(v * W + i, lane, o[i]);
+            }
         }
         __syncthreads();
     }
@@ -798,7 +834,7 @@ lk_k_paged_join(const LkPaArgs a, int cb_n) {
 
 // ---- host ---------------------------------------------------------------------------------------
 // How a workgroup's waves divide a tile, for chunks of `want` tokens of g query heads a kv head.
-struct LkPaShape { int cb, step, hg_sh, qw_sh, kw_sh, qc; };
+struct LkPaShape { int cb, step, hg_sh, qw_sh, kw_sh, qc, extra; };
 static LkPaShape lk_pa_shape(const lk_pages * p, int type, int max_new) {
     const int g = p->n_heads / p->n_kv_heads, d = p->head_dim, nw = lk_pa_waves(d);
     const int cb_max = type == LK_F32 ? 2 : 4, qw_max = 16 / cb_max < nw ? 16 / cb_max : nw;     // up to 256 columns
@@ -817,6 +853,10 @@ static LkPaShape lk_pa_shape(const lk_pages * p, int type, int max_new) {
     int qc = s.cb * 16 * qw / g;                               // at least 1: up to 64 heads a kv head
     if (qc > 64) qc = 64;
     s.qc = 1 << lk_log2(qc);
+    s.extra = s.step == 32 ? 6 : 2;
+#ifdef LK_PA_EXTRA
+    s.extra = getenv("LKX") ? atoi(getenv("LKX")) : s.extra;
+#endif
     return s;
 }
 static int lk_pa_blocks(const LkPaShape & s) { return s.cb << (s.qw_sh + s.hg_sh); }
@@ -841,9 +881,9 @@ static void lk_pa_launch(const LkPaShape & s, const LkPaArgs & a, bool mod, hipS
 template <int D, int RT>
 static void lk_pa_join(const LkPaArgs & a, int cuts, int nblk, int cb, hipStream_t st) {
     if (cuts * nblk <= 256)
-        hipLaunchKernelGGL((lk_k_paged_join<D, RT, 1024, 1>), dim3(cuts, nblk * (D / 16)), dim3(1024), 0, st, a, cb);
+        hipLaunchKernelGGL((lk_k_paged_join<D, RT, true>), dim3(cuts, nblk * (D / 16)), dim3(1024), 0, st, a, cb);
     else
-        hipLaunchKernelGGL((lk_k_paged_join<D, RT, 256, D / 16>), dim3(cuts, nblk), dim3(256), 0, st, a, cb);
+        hipLaunchKernelGGL((lk_k_paged_join<D, RT, false>), dim3(cuts, nblk), dim3(256), 0, st, a, cb);
 }
 
 static __device__ __align__(1024) char lk_pa_zeros[1024];      // never written
@@ -909,7 +949,7 @@ extern "C" int lk_paged_attn(const lk_pages * pages, const lk_step * step, int t
     float2 * ml = (float2 *) (acc + blocks * 16 * d);
     const LkPaArgs a = { q, out, (const char *) pages->k, (const char *) pages->v, zeros, step->first, step->lens, step->table, step->pos,
                          step->mask, slopes, acc, ml, (int4 *) (ml + blocks * 16), ldq, ldo, step->n_seqs, step->rows, step->ldt,
-                         step->width, lk_log2(pages->page), pages->n_pages, hq, pages->n_kv_heads, g, nhg, s.hg_sh, s.qw_sh, s.kw_sh, s.qc,
+                         step->width, lk_log2(pages->page), pages->n_pages, hq, pages->n_kv_heads, g, nhg, s.hg_sh, s.qw_sh, s.kw_sh, s.qc, s.extra,
                          scale * LK_LOG2E_F, scale, cap };
     const hipStream_t st = lk_stream(stream);
     const bool mod = cap > 0.0f || slopes;
