@@ -5,7 +5,7 @@
 //     out_i = sum_j exp(x_ij) v_j / sum_j exp(x_ij)      over the j that i sees
 //
 // The work is one line of key tiles: per sequence, chunk of its new tokens and group of kv
-// heads ("item") the tiles of the keys that the chunk sees.  Each of LK_PA_WGS workgroups
+// heads ("item") the tiles of the keys that the chunk sees.  Each of LK_PA_MAX_WGS workgroups
 // takes an equal run of that line, whatever the lengths are: it finds its place from the
 // lengths on the device, walks on from item to item, and its DMA runs ahead over the
 // borders.  An item inside one run is finished there; one that is cut leaves partials
@@ -24,14 +24,17 @@
 #include "lk_paged.h"
 #include <stdlib.h>
 
-#define LK_PA_WGS   256            // workgroups: one a CU (a ring of 128 KB each)
-#define LK_PA_NBUF  4
-#define LK_PA_TILEB 32768          // K rows, then V rows
+#define LK_PA_TILEB 32768          // a tile: K rows, then V rows
 #define LK_PA_HEADROOM 8.0f        // the running max is raised when a score passes it by 2^8
 #define LK_PA_NONE  3.0e38f        // minus the running max of no score: 2^(any score in sight - max) is 0 against it
 
-// Waves a workgroup: one kv head's piece of a tile with 16 keys for each where a group has as many heads.
-__host__ __device__ constexpr int lk_pa_waves(int d) { return d == 64 ? 8 : 4; }
+// Two kinds of workgroup.  For up to 32 columns a kv head (STEP 16) the cache's bytes bound it: one workgroup a
+// CU, a ring of four tiles, so that 96 KB are on their way.  For more (STEP 32) the products and exponentials
+// do: two workgroups a CU of one wave a SIMD each, which wait at barriers of their own, and two tiles.
+__host__ __device__ constexpr int lk_pa_waves(int d, int step) { return step == 16 && d == 64 ? 8 : 4; }
+__host__ __device__ constexpr int lk_pa_bufs(int step) { return step == 16 ? 4 : 2; }
+__host__ __device__ constexpr int lk_pa_wgs(int step) { return step == 16 ? 256 : 512; }
+#define LK_PA_MAX_WGS 512
 
 typedef short lk_s4 __attribute__((ext_vector_type(4)));
 typedef __bf16 lk_b8 __attribute__((ext_vector_type(8)));
@@ -96,10 +99,21 @@ __device__ __forceinline__ int lk_sld(const int32_t * p, long i) {
 #endif
 }
 
+// The arguments where the launch left them.  What is needed once an item or less is read there again each time
+// (args() below): kept for the whole kernel, the fifty values would spill, and each fetch wait for
+// lanes of a vector register to be read back.
+#ifdef __HIP_DEVICE_COMPILE__
+typedef __attribute__((address_space(4))) LkPaArgs LkPaC;
+__device__ __forceinline__ const LkPaC * lk_pa_kernarg() { return (const LkPaC *) __builtin_amdgcn_kernarg_segment_ptr(); }
+#else
+typedef LkPaArgs LkPaC;
+__device__ __forceinline__ const LkPaC * lk_pa_kernarg() { return nullptr; }
+#endif
+
 // ---- the line of tiles: every item has a.extra places, for what it costs to begin and end one, and then
 // its tiles ------------------------------------------------------------
 // Tiles of chunk c of a sequence: the keys up to the last one that a row of the chunk sees.
-__device__ __forceinline__ int lk_pa_vis(const LkPaArgs & a, const LkSeq & s, int c) {
+__device__ __forceinline__ int lk_pa_vis(const LkPaC & a, const LkSeq & s, int c) {
     int e = a.mask ? ((c * a.qc) & ~63) + 64 : (c + 1) * a.qc;
     e = s.len + (e < s.n ? e : s.n);
     const int cap = a.width << a.page_sh;
@@ -109,10 +123,10 @@ __device__ __forceinline__ int lk_pa_tiles(int vis, int tk_sh) {
     const int t = (vis + (1 << tk_sh) - 1) >> tk_sh;
     return t > 0 ? t : 1;                                  // a chunk that sees nothing still has its zeros to write
 }
-__device__ __forceinline__ LkSeq lk_pa_seq(const LkPaArgs & a, int b) {     // by a lane
+__device__ __forceinline__ LkSeq lk_pa_seq(const LkPaC & a, int b) {     // by a lane
     return lk_seq(a.first[b], a.first[b + 1], a.lens[b], a.rows, a.width << a.page_sh);
 }
-__device__ __forceinline__ long lk_pa_seq_tiles(const LkPaArgs & a, const LkSeq & s, int tk_sh) {
+__device__ __forceinline__ long lk_pa_seq_tiles(const LkPaC & a, const LkSeq & s, int tk_sh) {
     long n = 0;
     for (int c = 0; c * a.qc < s.n; ++c) n += lk_pa_tiles(lk_pa_vis(a, s, c), tk_sh) + a.extra;
     return n * a.nhg;
@@ -131,14 +145,14 @@ __device__ __forceinline__ long lk_uniform64(long v) {
 struct LkPaAt {
     int b, c, h, t, nt, vis;
     LkSeq s;
+    const int32_t * row;           // the sequence's pages
 };
-__device__ __forceinline__ void lk_pa_item(const LkPaArgs & a, LkPaAt & p, int tk_sh) {
+__device__ __forceinline__ void lk_pa_item(const LkPaC & a, LkPaAt & p, int tk_sh) {
     p.vis = lk_pa_vis(a, p.s, p.c);
     p.nt = lk_pa_tiles(p.vis, tk_sh);
 }
-// The next tile; behind the last one b is n_seqs.
-__device__ __forceinline__ void lk_pa_next(const LkPaArgs & a, LkPaAt & p, int tk_sh) {
-    if (++p.t < p.nt) return;
+// The next item's first tile; behind the last one b is n_seqs.
+__device__ __forceinline__ void lk_pa_next(const LkPaC & a, LkPaAt & p, int tk_sh) {
     p.t = 0;
     if (++p.h < a.nhg) return;
     p.h = 0;
@@ -147,8 +161,18 @@ __device__ __forceinline__ void lk_pa_next(const LkPaArgs & a, LkPaAt & p, int t
         p.c = 0;
         if (++p.b >= a.n_seqs) return;
         p.s = lk_seq(lk_sld(a.first, p.b), lk_sld(a.first, p.b + 1), lk_sld(a.lens, p.b), a.rows, a.width << a.page_sh);
+        p.row = a.table + (long) p.b * a.ldt;
     }
     lk_pa_item(a, p, tk_sh);
+}
+
+// v, for what is worked out of it to be worked out here: values that hold for the whole kernel and are used
+// once a tile or less would otherwise take registers from the start.
+__device__ __forceinline__ int lk_here(int v) {
+#ifdef __HIP_DEVICE_COMPILE__
+    asm volatile("" : "+v"(v));
+#endif
+    return v;
 }
 
 // 1 / the sum of the weights; a row that sees nothing has the sum 0 and gets zeros.
@@ -172,62 +196,69 @@ __device__ __forceinline__ float lk_tanh(float t) {
     return copysignf(u < 0.5f ? small : large, t);
 }
 
-struct LkYes { static constexpr bool value = true; };
-struct LkNo { static constexpr bool value = false; };
-
 // D: head_dim.  RT: rows (LK_F32: q and the weights as two parts).  CT: pools.  CB: blocks of 16
 // columns a wave holds.  STEP: keys a wave takes at once, 32 by K = 32 products of both kinds, 16 by
 // K = 16 for P.V.  MOD: capped or biased scores.
 template <int D, int RT, int CT, int CB, int STEP, bool MOD>
-__global__ void __launch_bounds__(64 * lk_pa_waves(D))
-lk_k_paged_attn(const LkPaArgs a) {
+__global__ void __launch_bounds__(64 * lk_pa_waves(D, STEP), STEP == 16 && D == 128 ? 1 : 2)
+lk_k_paged_attn(const LkPaArgs) {
+    const LkPaC * const karg = lk_pa_kernarg();
+    auto args = [&]() -> const LkPaC & {
+        const LkPaC * p = karg;
+#ifdef __HIP_DEVICE_COMPILE__
+        asm volatile("" : "+s"(p));
+#endif
+        return *p;
+    };
     typedef LkMm<CT> M;
     typedef typename M::T T;
     typedef typename M::V8 V8;
     typedef typename M::V4 V4;
     typedef typename LkElem<RT>::type RowT;
     constexpr bool TWO = RT == LK_F32;
-    constexpr int NW = lk_pa_waves(D);
+    constexpr int NW = lk_pa_waves(D, STEP), NBUF = lk_pa_bufs(STEP), NB = STEP / 16;
     constexpr int KS = D / 32, DB = D / 16, DC = D / 8;        // steps of q.k, blocks of output dims, 16-byte pieces of a head's row
     constexpr int NF = 16 / NW;                                // pieces of 1 KB a wave fetches of a tile's K, and of its V
-    constexpr int AHEAD = LK_PA_NBUF - 1;
-    __shared__ __attribute__((aligned(16))) unsigned char s_tile[LK_PA_NBUF][LK_PA_TILEB];
+    constexpr int AHEAD = NBUF - 1;
+    __shared__ __attribute__((aligned(16))) unsigned char s_tile[NBUF][LK_PA_TILEB];
     __shared__ lk_f4 s_x[2][NW][64];                           // key shares' rows on their way to one wave
     __shared__ float2 s_ml[NW][16];
+    __shared__ uint64_t s_see[NW][CB][16];                     // which of the 64 tokens from `base` on a column sees
 
     const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int kw = w & ((1 << a.kw_sh) - 1), qw = (w >> a.kw_sh) & ((1 << a.qw_sh) - 1), hh = w >> (a.kw_sh + a.qw_sh);
-    const int rb_sh = a.hg_sh + (D == 64 ? 7 : 8);             // bytes of a position's piece: its group's heads
+    const LkPaC & a0 = args();
+    const int kw_sh = a0.kw_sh, kw = w & ((1 << kw_sh) - 1), qw = (w >> kw_sh) & ((1 << a0.qw_sh) - 1), hh = w >> (kw_sh + a0.qw_sh);
+    const int rb_sh = a0.hg_sh + (D == 64 ? 7 : 8);             // bytes of a position's piece: its group's heads
     const int rb = 1 << rb_sh;
     const int tk_sh = 14 - rb_sh;                              // keys a tile: 16 KB of K rows
-    const int kpw = (1 << tk_sh) >> a.kw_sh;                   // of them the wave's
+    const int kpw = (1 << tk_sh) >> kw_sh;                   // of them the wave's
 
     // ---- this workgroup's run of the line ---------------------------------------------
     long total = 0, mine = 0, before = 0;
     LkSeq ls = { 0, 0, 0 };
-    for (int b = lane; b < a.n_seqs; b += 64) {
-        ls = lk_pa_seq(a, b);
-        mine = lk_pa_seq_tiles(a, ls, tk_sh);
+    for (int b = lane; b < a0.n_seqs; b += 64) {
+        ls = lk_pa_seq(a0, b);
+        mine = lk_pa_seq_tiles(a0, ls, tk_sh);
         total += mine;
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) total += lk_shfl64(total, lane ^ o);
     total = lk_uniform64(total);
-    const long share = (total + LK_PA_WGS - 1) / LK_PA_WGS;
+    const long share = (total + lk_pa_wgs(STEP) - 1) / lk_pa_wgs(STEP);
     const long f0 = share * blockIdx.x, f1 = f0 + share < total ? f0 + share : total;
     if (f0 >= f1) {
-        if (threadIdx.x == 0) a.cut[blockIdx.x] = make_int4(0, 0, 0, 0);
+        if (threadIdx.x == 0) args().cut[blockIdx.x] = make_int4(0, 0, 0, 0);
         return;
     }
     LkPaAt at;
     for (int b0 = 0;; b0 += 64) {                              // ends: f0 is below the total
         const int b = b0 + lane;
-        if (a.n_seqs > 64) {
+        if (a0.n_seqs > 64) {
             mine = 0;
-            if (b < a.n_seqs) {
-                ls = lk_pa_seq(a, b);
-                mine = lk_pa_seq_tiles(a, ls, tk_sh);
+            if (b < a0.n_seqs) {
+                ls = lk_pa_seq(a0, b);
+                mine = lk_pa_seq_tiles(a0, ls, tk_sh);
             }
         }
         long sum = mine;
@@ -241,17 +272,18 @@ lk_k_paged_attn(const LkPaArgs a) {
             const int src = __builtin_ctzll(here);
             long rem = lk_uniform64(lk_shfl64(f0 - before - (sum - mine), src));
             at.b = b0 + src;
+            at.row = a0.table + (long) at.b * a0.ldt;
             at.s.r0 = __builtin_amdgcn_readlane(ls.r0, src);
             at.s.n = __builtin_amdgcn_readlane(ls.n, src);
             at.s.len = __builtin_amdgcn_readlane(ls.len, src);
             for (at.c = 0;; ++at.c) {                          // ends: rem is below the sequence's tiles
-                lk_pa_item(a, at, tk_sh);
-                const long u = (long) (at.nt + a.extra) * a.nhg;
+                lk_pa_item(a0, at, tk_sh);
+                const long u = (long) (at.nt + a0.extra) * a0.nhg;
                 if (rem < u) break;
                 rem -= u;
             }
-            at.h = (int) (rem / (at.nt + a.extra));
-            at.t = (int) (rem % (at.nt + a.extra)) - a.extra;  // below 0: in front of the first tile
+            at.h = (int) (rem / (at.nt + a0.extra));
+            at.t = (int) (rem % (at.nt + a0.extra)) - a0.extra;  // below 0: in front of the first tile
             break;
         }
         before += lk_uniform64(lk_shfl64(sum, 63));
@@ -259,52 +291,50 @@ lk_k_paged_attn(const LkPaArgs a) {
 
     // ---- fetch: wave w brings the 1 KB pieces w, w + NW, .. of a tile's K and of its V -----
     // Piece i holds the keys i * rpp .. of the tile, all in one page (a page is a multiple of 16).
-    // Within a head's row the 16-byte pieces are permuted by the key, so that the lanes' reads below
-    // meet different banks.  The pages of the next tile are asked for a tile ahead.
+    // Within a row its 16-byte pieces are permuted by the key, so that the lanes' reads below meet
+    // different ones of the 64 banks: 16 keys of a K piece, 8 keys of two V pieces, over 256 bytes.
+    // The pages of the next tile are asked for a tile ahead.
     const int rpp_sh = 10 - rb_sh, rpp = 1 << rpp_sh;
     const uint32_t lds0 = lk_lds_addr(&s_tile[0][0]);
-    const uint32_t row_bytes = (uint32_t) a.hkv * D * 2;
-    auto swk = [](int key) -> int { return key & (DC - 1); };
-    auto swv = [](int key) -> int { return (((key & 3) << 1) | ((key >> 2) & 1) | (key & 8)) & (DC - 1); };
-    const int frow = lane >> (6 - rpp_sh);
-    uint32_t ko[NF], vo[NF];                                   // the lane's bytes from the piece's first row on
-#pragma unroll
-    for (int i = 0; i < NF; ++i) {
-        const int key = ((w + NW * i) << rpp_sh) + frow, piece = lane & ((1 << (6 - rpp_sh)) - 1);
-        const int hd = piece & ~(DC - 1), jj = piece & (DC - 1);
-        ko[i] = frow * row_bytes + 16 * (hd + (jj ^ swk(key)));
-        vo[i] = frow * row_bytes + 16 * (hd + (jj ^ swv(key)));
-    }
+    const uint32_t row_bytes = (uint32_t) a0.hkv * D * 2;
+    const char * const kp = a0.kp, * const vp = a0.vp;
+    const int page_sh = a0.page_sh, n_pages = a0.n_pages, extra = a0.extra;
+    auto swk = [&](int key) -> int { return rb == 128 ? (key >> 1) & 7 : key & 15; };
+    auto swv = [&](int key) -> int { return (rb == 128 ? (key >> 1) & 3 : key & 7) << 1; };
     int pg[NF];
     auto ask = [&](const LkPaAt & p) {
 #pragma unroll
         for (int i = 0; i < NF; ++i) {
             const int p0 = (p.t << tk_sh) + ((w + NW * i) << rpp_sh);
-            pg[i] = lk_sld(a.table, (long) p.b * a.ldt + ((p0 < p.vis ? p0 : 0) >> a.page_sh));
+            pg[i] = lk_sld(p.row, (p0 < p.vis ? p0 : 0) >> page_sh);
         }
     };
     auto fetch = [&](const LkPaAt & p, int slot) {
+        const int ln = lk_here(lane), frow = ln >> (6 - rpp_sh), part = ln & ((1 << (6 - rpp_sh)) - 1);
         const uint32_t base = lds0 + (uint32_t) slot * LK_PA_TILEB;
 #pragma unroll
         for (int i = 0; i < NF; ++i) {
             const int piece = w + NW * i, p0 = (p.t << tk_sh) + (piece << rpp_sh);
-            const bool ok = pg[i] >= 0 && pg[i] < a.n_pages;
-            const size_t off = (((size_t) (ok ? pg[i] : 0) << a.page_sh) + (p0 & ((1 << a.page_sh) - 1))) * row_bytes +
+            const bool ok = pg[i] >= 0 && pg[i] < n_pages;
+            const size_t off = (((size_t) (ok ? pg[i] : 0) << page_sh) + (p0 & ((1 << page_sh) - 1))) * row_bytes +
                                ((size_t) p.h << rb_sh);
+            // the lane's bytes from the piece's first row on
+            const int key = (piece << rpp_sh) + frow;
+            const uint32_t ko = frow * row_bytes + 16 * (part ^ swk(key)), vo = frow * row_bytes + 16 * (part ^ swv(key));
             const uint32_t lk = base + piece * 1024, lv = lk + LK_PA_TILEB / 2;
             if (ok && p0 + rpp <= p.vis) {
                 if constexpr (STEP == 16) {                    // up to 64 columns a head: few others read the tile
-                    lk_dma16_so(a.kp + off, ko[i], lk);
-                    lk_dma16_so(a.vp + off, vo[i], lv);
+                    lk_dma16_so(kp + off, ko, lk);
+                    lk_dma16_so(vp + off, vo, lv);
                 } else {
-                    lk_dma16c_so(a.kp + off, ko[i], lk);
-                    lk_dma16c_so(a.vp + off, vo[i], lv);
+                    lk_dma16c_so(kp + off, ko, lk);
+                    lk_dma16c_so(vp + off, vo, lv);
                 }
             } else {                                           // rows that nobody sees are zeros
                 const bool live = ok && p0 + frow < p.vis;
-                const char * zs = a.zeros + 16 * lane;
-                lk_dma16c(live ? a.kp + off + ko[i] : zs, lk);
-                lk_dma16c(live ? a.vp + off + vo[i] : zs, lv);
+                const char * zs = args().zeros + 16 * ln;
+                lk_dma16c(live ? kp + off + ko : zs, lk);
+                lk_dma16c(live ? vp + off + vo : zs, lv);
             }
         }
     };
@@ -317,8 +347,8 @@ lk_k_paged_attn(const LkPaArgs a) {
     int qpos[MOD ? CB : 1];
     int base = 0;                                               // keys below it are seen by all of the chunk's rows
     // column block cb: the token of the chunk, its row of the step, its query head; false: there is none
-    auto column = [&](int cb, int & i, int & row, int & head) -> bool {
-        const int c = (qw * CB + cb) * 16 + col, i0 = at.c * a.qc, m = at.s.n - i0 < a.qc ? at.s.n - i0 : a.qc;
+    auto column = [&](const LkPaC & a, int cb, int & i, int & row, int & head) -> bool {
+        const int c = (qw * CB + cb) * 16 + lk_here(col), i0 = at.c * a.qc, m = at.s.n - i0 < a.qc ? at.s.n - i0 : a.qc;
         i = c / a.g;
         const int h = c - i * a.g;
         const bool live = i < m;
@@ -327,13 +357,17 @@ lk_k_paged_attn(const LkPaArgs a) {
         head = ((at.h << a.hg_sh) + hh) * a.g + (live ? h : 0);
         return live;
     };
+    float sc = 0.0f, cap = 0.0f;                                // scale (times log2(e) but for MOD), cap
     auto begin = [&]() {
-        const int blk = (at.c * a.qc) & ~63, cap = a.width << a.page_sh;
-        base = at.s.len + blk < cap ? at.s.len + blk : cap;
+        const LkPaC & a = args();
+        sc = MOD ? a.scale : a.sc;
+        cap = a.cap;
+        const int blk = (at.c * a.qc) & ~63, slots = a.width << a.page_sh;
+        base = at.s.len + blk < slots ? at.s.len + blk : slots;
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) {
             int i, row, head;
-            const bool live = column(cb, i, row, head);
+            const bool live = column(a, cb, i, row, head);
             if constexpr (MOD) {
                 slope[cb] = a.slopes ? a.slopes[head] * LK_LOG2E_F : 0.0f;
                 qpos[cb] = a.pos ? a.pos[row] : at.s.len + (row - at.s.r0);
@@ -358,7 +392,7 @@ lk_k_paged_attn(const LkPaArgs a) {
                     (void) frexpf(am, &e2);
                     e2 -= 15;
                 }
-                fac[cb] = ldexpf(MOD ? a.scale : a.sc, e2);
+                fac[cb] = ldexpf(sc, e2);
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
@@ -376,6 +410,10 @@ lk_k_paged_attn(const LkPaArgs a) {
                     qh[cb][ks] = live ? v : V8{};
                 }
             }
+            // a wave reads its own words only
+            const int limit = at.vis - base;                    // of the 64 tokens from base on the ones that have a slot
+            const uint64_t lim = limit >= 64 ? ~0ull : limit > 0 ? (1ull << limit) - 1 : 0;
+            if (g == 0) s_see[w][cb][col] = (a.mask ? a.mask[row] : ~0ull >> (63 - ((at.c * a.qc + i) & 63))) & lim;
             mneg[cb] = LK_PA_NONE;
             accl[cb] = (lk_f4){ 0.f, 0.f, 0.f, 0.f };
 #pragma unroll
@@ -384,14 +422,17 @@ lk_k_paged_attn(const LkPaArgs a) {
     };
 
     // ---- keys ---------------------------------------------------------------------------------
-    const int kadr = hh * (D * 2) + col * rb, ksw = g ^ swk(col);
-    const int vadr = hh * (D * 2) + (4 * g + (col >> 2)) * rb + 8 * (col & 1), vsw = swv(4 * g + (col >> 2)) ^ ((col >> 1) & 1);
-    auto kload = [&](const unsigned char * kt, V8 (&kf)[KS]) {
+    // (a head's pieces start at a multiple of DC, so the parts of a piece's number do not overlap)
+    const int kadr = col * rb, ksw = (hh * DC | g) ^ swk(col);
+    const int vadr = (4 * g + (col >> 2)) * rb + 8 * (col & 1), vsw = (hh * DC | ((col >> 1) & 1)) ^ swv(4 * g + (col >> 2));
+    auto kload = [&](const unsigned char * kt, V8 (&kf)[NB][KS]) {
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) kf[ks] = *(const V8 *) (kt + kadr + ((ksw ^ (4 * ks)) << 4));
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) kf[n][ks] = *(const V8 *) (kt + kadr + ((16 * n) << rb_sh) + ((ksw ^ (4 * ks)) << 4));
     };
-    auto vload = [&](const unsigned char * vt, int db) -> V4 {
-        return __builtin_bit_cast(V4, lk_ds_tr4(vt + vadr + ((vsw ^ (2 * db)) << 4)));
+    auto vload = [&](const unsigned char * vt, int n, int db) -> V4 {
+        return __builtin_bit_cast(V4, lk_ds_tr4(vt + vadr + ((16 * n) << rb_sh) + ((vsw ^ (2 * db)) << 4)));
     };
     auto scores = [&](const V8 (&kf)[KS], int cb) -> lk_f4 {
         lk_f4 c = { 0.f, 0.f, 0.f, 0.f };
@@ -402,15 +443,16 @@ lk_k_paged_attn(const LkPaArgs a) {
         }
         return c;
     };
-    auto factor = [&](int cb) -> float { return TWO ? fac[cb] : MOD ? a.scale : a.sc; };
+    auto factor = [&](int cb) -> float { return TWO ? fac[cb] : sc; };
     // capped and biased scores in units of log2, of keys k0 .. k0 + 3 (k0: the lane's first)
     auto shaped = [&](lk_f4 & c, int cb, int k0) {
+        const int32_t * pos = args().pos;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             float x = c[r] * factor(cb);
-            if (a.cap > 0.0f) x = a.cap * lk_tanh(x / a.cap);
+            if (cap > 0.0f) x = cap * lk_tanh(x / cap);
             int kp = k0 + r;
-            if (a.pos && kp >= at.s.len && kp < at.vis) kp = a.pos[at.s.r0 + kp - at.s.len];
+            if (pos && kp >= at.s.len && kp < at.vis) kp = pos[at.s.r0 + kp - at.s.len];
             c[r] = __builtin_fmaf(slope[cb], (float) (kp - qpos[cb]), x * LK_LOG2E_F);
         }
     };
@@ -443,132 +485,118 @@ lk_k_paged_attn(const LkPaArgs a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) ones4[i] = (T) 1.0f;
 
-    // STEP keys, the first of them key0.  `some`: there are keys that only some of the rows see (the new
-    // tokens and what shares a step with them), told by `see`.
-    auto step = [&](auto some, const unsigned char * kt, const unsigned char * vt, int key0, const uint64_t (&see)[CB]) {
-        constexpr bool SOME = decltype(some)::value;
-        constexpr int NB = STEP / 16;
-        V4 ph[CB][NB], pl[TWO ? CB : 1][NB];
-        uint32_t sees[SOME ? CB : 1];                           // bit 4n + r: the column sees the lane's key r of block n
-        {
-            V8 kf[NB][KS];
+    // whether the column of block cb sees the lane's keys 4g .. 4g + 3 of the 16 from key0 on: four bits
+    auto sees = [&](int cb, int key0) -> uint32_t {
+        const int d = key0 + 4 * g - base;
+        const uint64_t e = s_see[w][cb][col];
+        return (uint32_t) (d >= 0 ? (d < 64 ? e >> d : 0) : d > -4 ? e << -d | ((1 << -d) - 1) : 15) & 15;
+    };
+    // STEP keys, the first of them key0, kf their K rows; `more`: the rows of the STEP keys behind are
+    // asked for.  From `base` on there are keys that only some of the rows see.
+    auto step = [&](const unsigned char * kt, const unsigned char * vt, int key0, V8 (&kf)[NB][KS], bool more) {
+        V4 ph[CB][NB], pl[TWO ? CB : 1][NB], vf[DB][NB];
+        lk_f4 c[CB][NB];
+        const bool some = key0 + STEP > base;                   // wave-uniform
 #pragma unroll
-            for (int n = 0; n < NB; ++n) kload(kt + ((16 * n) << rb_sh), kf[n]);
-            // two blocks of columns at a time: their products have nothing to wait for each other, and one
-            // test for both says whether a max has to be raised
-            constexpr int CP = CB < 2 ? CB : 2;
+        for (int db = 0; db < DB; ++db)
 #pragma unroll
-            for (int cp = 0; cp < CB; cp += CP) {
-                lk_f4 c[CP][NB];
-                float top[CP], over = -INFINITY;
+            for (int n = 0; n < NB; ++n) vf[db][n] = vload(vt, n, db);
 #pragma unroll
-                for (int i = 0; i < CP; ++i)
+        for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
-                    for (int n = 0; n < NB; ++n) c[i][n] = scores(kf[n], cp + i);
+            for (int n = 0; n < NB; ++n) c[cb][n] = scores(kf[n], cb);
+        if (more) kload(kt + (STEP << rb_sh), kf);
+        if constexpr (MOD) {
 #pragma unroll
-                for (int i = 0; i < CP; ++i) {
-                    top[i] = -INFINITY;
-                    if constexpr (SOME) sees[cp + i] = 0;
+            for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
-                    for (int n = 0; n < NB; ++n) {
-                        if constexpr (MOD) shaped(c[i][n], cp + i, key0 + 16 * n + 4 * g);
-                        if constexpr (SOME) {
-                            const int d = key0 + 16 * n + 4 * g - base;
-                            const uint64_t e = see[cp + i];
-                            const uint32_t bits = (uint32_t) (d >= 0 ? (d < 64 ? e >> d : 0) : d > -4 ? e << -d | ((1 << -d) - 1) : 15) & 15;
-                            sees[cp + i] |= bits << (4 * n);
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) c[i][n][r] = (bits >> r) & 1 ? c[i][n][r] : -INFINITY;
-                        }
-                        top[i] = fmaxf(top[i], top4(c[i][n]));
-                    }
-                    over = fmaxf(over, MOD ? top[i] + mneg[cp + i] : __builtin_fmaf(top[i], factor(cp + i), mneg[cp + i]));
-                }
-                if (__ballot(over > LK_PA_HEADROOM)) {          // wave-uniform
-#pragma unroll
-                    for (int i = 0; i < CP; ++i) raise(cp + i, units(top[i], cp + i));
-                }
-#pragma unroll
-                for (int i = 0; i < CP; ++i)
-#pragma unroll
-                    for (int n = 0; n < NB; ++n) weights(c[i][n], cp + i, ph[cp + i][n], pl[TWO ? cp + i : 0][n]);
-            }
+                for (int n = 0; n < NB; ++n) shaped(c[cb][n], cb, key0 + 16 * n + 4 * g);
         }
+        bool odd = false;                                       // an infinity or NaN among the values
+        if (some) {
 #pragma unroll
-        for (int cb = 0; cb < CB; ++cb) {
-            if constexpr (NB == 2) {
-                accl[cb] = M::k32(join(ones4, ones4), join(ph[cb][0], ph[cb][1]), accl[cb]);
-                if constexpr (TWO) accl[cb] = M::k32(join(ones4, ones4), join(pl[cb][0], pl[cb][1]), accl[cb]);
-            } else {
-                accl[cb] = M::k16(ones4, ph[cb][0], accl[cb]);
-                if constexpr (TWO) accl[cb] = M::k16(ones4, pl[cb][0], accl[cb]);
-            }
-        }
-        if constexpr (SOME) {
-            bool odd = false;                                   // an infinity or NaN among the values
+            for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+                for (int n = 0; n < NB; ++n) {
+                    const uint32_t bits = sees(cb, key0 + 16 * n);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) c[cb][n][r] = (bits >> r) & 1 ? c[cb][n][r] : -INFINITY;
+                }
+            // 0 times an infinity is NaN: such values are left out of the product, and added behind it
 #pragma unroll
             for (int db = 0; db < DB; ++db)
 #pragma unroll
                 for (int n = 0; n < NB; ++n) {
-                    const lk_u16x4 u = __builtin_bit_cast(lk_u16x4, vload(vt + ((16 * n) << rb_sh), db));
+                    lk_u16x4 u = __builtin_bit_cast(lk_u16x4, vf[db][n]);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) odd |= (u[r] & M::INF) == M::INF;
-                }
-            if (__ballot(odd)) {                                // wave-uniform
-                // 0 times an infinity is NaN: one key after the other, and only the columns that see it
-#pragma unroll
-                for (int n = 0; n < NB; ++n)
-#pragma clang loop unroll(disable)
-                    for (int k = 0; k < 16; ++k) {
-                        const int kg = k >> 2, kr = k & 3;
-                        bool take[CB];
-#pragma unroll
-                        for (int cb = 0; cb < CB; ++cb) take[cb] = ((uint32_t) __shfl((int) sees[cb], 16 * kg + col, 64) >> (4 * n + kr)) & 1;
-#pragma unroll
-                        for (int db = 0; db < DB; ++db) {
-                            const V4 vf = vload(vt + ((16 * n) << rb_sh), db);
-                            V4 v, vl;
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) {
-                                v[r] = g == kg && r == kr ? vf[r] : (T) 0.0f;
-                                // (a low part of 0 against an infinity would be NaN: it is left out there)
-                                vl[r] = (__builtin_bit_cast(lk_u16x4, vf)[r] & M::INF) == M::INF ? (T) 0.0f : v[r];
-                            }
-#pragma unroll
-                            for (int cb = 0; cb < CB; ++cb) {
-                                lk_f4 o = { 0.f, 0.f, 0.f, 0.f };
-                                o = M::k16(v, ph[cb][n], o);
-                                if constexpr (TWO) o = M::k16(vl, pl[cb][n], o);
-                                if (take[cb]) acc[cb][db] += o;
-                            }
-                        }
+                    for (int r = 0; r < 4; ++r) {
+                        const bool o = (u[r] & M::INF) == M::INF;
+                        odd |= o;
+                        u[r] = o ? 0 : u[r];
                     }
-                return;
-            }
+                    vf[db][n] = __builtin_bit_cast(V4, u);
+                }
+            odd = __ballot(odd) != 0;                           // wave-uniform
+        }
+        // one test for all blocks of columns says whether a max has to be raised
+        float top[CB], over = -INFINITY;
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) {
+            top[cb] = top4(c[cb][0]);
+            if constexpr (NB == 2) top[cb] = fmaxf(top[cb], top4(c[cb][1]));
+            over = fmaxf(over, MOD ? top[cb] + mneg[cb] : __builtin_fmaf(top[cb], factor(cb), mneg[cb]));
+        }
+        if (__ballot(over > LK_PA_HEADROOM)) {                  // wave-uniform
+#pragma unroll
+            for (int cb = 0; cb < CB; ++cb) raise(cb, units(top[cb], cb));
         }
 #pragma unroll
-        for (int db = 0; db < DB; ++db) {
-            V4 vf[NB];
+        for (int cb = 0; cb < CB; ++cb) {
 #pragma unroll
-            for (int n = 0; n < NB; ++n) vf[n] = vload(vt + ((16 * n) << rb_sh), db);
-#pragma unroll
-            for (int cb = 0; cb < CB; ++cb) {
+            for (int n = 0; n < NB; ++n) weights(c[cb][n], cb, ph[cb][n], pl[TWO ? cb : 0][n]);
+            auto product = [&](const V4 (&v)[NB], lk_f4 o) -> lk_f4 {
                 if constexpr (NB == 2) {
-                    const V8 v8 = join(vf[0], vf[1]);
-                    acc[cb][db] = M::k32(v8, join(ph[cb][0], ph[cb][1]), acc[cb][db]);
-                    if constexpr (TWO) acc[cb][db] = M::k32(v8, join(pl[cb][0], pl[cb][1]), acc[cb][db]);
+                    o = M::k32(join(v[0], v[1]), join(ph[cb][0], ph[cb][1]), o);
+                    if constexpr (TWO) o = M::k32(join(v[0], v[1]), join(pl[cb][0], pl[cb][1]), o);
                 } else {
-                    acc[cb][db] = M::k16(vf[0], ph[cb][0], acc[cb][db]);
-                    if constexpr (TWO) acc[cb][db] = M::k16(vf[0], pl[cb][0], acc[cb][db]);
+                    o = M::k16(v[0], ph[cb][0], o);
+                    if constexpr (TWO) o = M::k16(v[0], pl[cb][0], o);
                 }
-            }
+                return o;
+            };
+            V4 ones[NB];
+#pragma unroll
+            for (int n = 0; n < NB; ++n) ones[n] = ones4;
+            accl[cb] = product(ones, accl[cb]);
+#pragma unroll
+            for (int db = 0; db < DB; ++db) acc[cb][db] = product(vf[db], acc[cb][db]);
+        }
+        if (odd) {
+            // one key after the other, and only the columns that see it
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma clang loop unroll(disable)
+                for (int k = 0; k < 16; ++k) {
+                    const int d = key0 + 16 * n + k - base;
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) {
+                        lk_u16x4 u = __builtin_bit_cast(lk_u16x4, vload(vt, n, db));
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) u[r] = 4 * g + r == k && (u[r] & M::INF) == M::INF ? u[r] : 0;
+#pragma unroll
+                        for (int cb = 0; cb < CB; ++cb) {
+                            const lk_f4 o = M::k16(__builtin_bit_cast(V4, u), ph[cb][n], (lk_f4){ 0.f, 0.f, 0.f, 0.f });
+                            if (d < 0 || (d < 64 && ((s_see[w][cb][col] >> d) & 1))) acc[cb][db] += o;
+                        }
+                    }
+                }
         }
     };
 
     // ---- an item's end, or the run's ----------------------------------------------------------
     // The key shares of a head and its columns meet in the wave with the first of them.
     auto join_shares = [&]() {
-        const int kws = 1 << a.kw_sh;
+        const int kws = 1 << kw_sh;
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) {
             if (g == 0) s_ml[w][col] = make_float2(-mneg[cb], accl[cb][0]);
@@ -601,15 +629,16 @@ lk_k_paged_attn(const LkPaArgs a) {
             }
         }
     };
-    const int nblk = CB << (a.qw_sh + a.hg_sh);
     auto finish = [&](bool whole, bool from_first) {
-        if (a.kw_sh) join_shares();
+        if (kw_sh) join_shares();
         if (kw != 0) return;
+        const LkPaC & a = args();
+        const int nblk = CB << (a.qw_sh + a.hg_sh);
         const int slot = 2 * blockIdx.x + from_first;
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) {
             int i, row, head;
-            if (!column(cb, i, row, head)) continue;
+            if (!column(a, cb, i, row, head)) continue;
             if (whole) {
                 const float il = lk_pa_inverse(accl[cb][0]);
                 RowT * o = (RowT *) a.out + (size_t) row * a.ldo + (size_t) head * D + 4 * g;
@@ -634,7 +663,7 @@ lk_k_paged_attn(const LkPaArgs a) {
         left += at.t;
         at.t = 0;
         if (left <= 0) {
-            if (threadIdx.x == 0) a.cut[blockIdx.x] = make_int4(0, 0, 0, 0);
+            if (threadIdx.x == 0) args().cut[blockIdx.x] = make_int4(0, 0, 0, 0);
             return;
         }
     }
@@ -642,77 +671,63 @@ lk_k_paged_attn(const LkPaArgs a) {
     long ft_left = left;                                        // places of the run from it on
     int slot = 0, ahead = 0;                                    // the awaited tile's buffer; tiles fetched and not yet taken
     auto fetch_next = [&]() {
-        fetch(ft, (slot + ahead) & (LK_PA_NBUF - 1));
+        fetch(ft, (slot + ahead) & (NBUF - 1));
         ++ahead;
-        ft_left -= ft.t + 1 == ft.nt ? 1 + a.extra : 1;
-        lk_pa_next(a, ft, tk_sh);
+        if (++ft.t == ft.nt) {
+            ft_left -= extra;
+            lk_pa_next(args(), ft, tk_sh);
+        }
+        --ft_left;
         if (ft_left > 0) ask(ft);
     };
     ask(ft);
     for (int i = 0; i < AHEAD && ft_left > 0; ++i) fetch_next();
-    // waits for the tile in `slot`, then asks for the tile AHEAD further, into the buffer that every
-    // wave has read before the barrier
-    auto next_tile = [&]() {
-        if (ahead > 2)       lk_wait_vm<4 * NF>();
-        else if (ahead == 2) lk_wait_vm<2 * NF>();
-        else                 lk_wait_vm<0>();
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        if (ft_left > 0) fetch_next();
-    };
-    static_assert(AHEAD == 3, "next_tile: two tiles may stay in flight behind the awaited one");
-    auto done_tile = [&]() {
-        slot = (slot + 1) & (LK_PA_NBUF - 1);
-        --ahead;
-        --left;
-    };
     int4 cut = make_int4(0, 0, 0, 0);
     while (left > 0) {
         begin();
         const bool from_first = at.t == 0;
         const int t_end = left < at.nt - at.t ? at.t + (int) left : at.nt;        // of this item in this run
-        const int t_open = lk_clamp(base >> tk_sh, at.t, t_end);
-        uint64_t see[CB] = {};
-        for (; at.t < t_open; ++at.t) {
-            next_tile();
-            const unsigned char * kt = s_tile[slot] + ((kw * kpw) << rb_sh);
-            for (int k = 0; k < kpw; k += STEP)
-                step(LkNo(), kt + (k << rb_sh), kt + (k << rb_sh) + LK_PA_TILEB / 2, (at.t << tk_sh) + kw * kpw + k, see);
-            done_tile();
-        }
-        if (at.t < t_end) {
-            const int limit = at.vis - base;                    // of the 64 tokens from base on the ones that have a slot
-            const uint64_t lim = limit >= 64 ? ~0ull : limit > 0 ? (1ull << limit) - 1 : 0;
-#pragma unroll
-            for (int cb = 0; cb < CB; ++cb) {
-                int i, row, head;
-                (void) column(cb, i, row, head);
-                see[cb] = (a.mask ? a.mask[row] : ~0ull >> (63 - ((at.c * a.qc + i) & 63))) & lim;
+        for (; at.t < t_end; ++at.t) {
+            // waits for the tile in `slot`, then asks for the tile AHEAD further, into the buffer that every
+            // wave has read before the barrier
+            if constexpr (AHEAD == 3) {
+                if (ahead > 2)       lk_wait_vm<4 * NF>();
+                else if (ahead == 2) lk_wait_vm<2 * NF>();
+                else                 lk_wait_vm<0>();
+            } else {
+                static_assert(AHEAD == 1 || AHEAD == 3, "tiles that may stay in flight behind the awaited one: none, or two");
+                lk_wait_vm<0>();
             }
-            for (; at.t < t_end; ++at.t) {
-                next_tile();
-                const unsigned char * kt = s_tile[slot] + ((kw * kpw) << rb_sh);
-                for (int k = 0; k < kpw; k += STEP) {
-                    const int key0 = (at.t << tk_sh) + kw * kpw + k;
-                    if (key0 < at.vis) step(LkYes(), kt + (k << rb_sh), kt + (k << rb_sh) + LK_PA_TILEB / 2, key0, see);
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            if (ft_left > 0) fetch_next();
+            const int k0 = (at.t << tk_sh) + kw * kpw;
+            if (k0 < at.vis) {                                  // the wave's share may lie behind the last key
+                const unsigned char * kt = s_tile[slot] + ((kw * kpw) << rb_sh), * vt = kt + LK_PA_TILEB / 2;
+                const int n = k0 + kpw < at.vis ? kpw : at.vis - k0;
+                V8 kf[NB][KS];
+                kload(kt, kf);
+                for (int k = 0; k < n; k += STEP) {
+                    step(kt + (k << rb_sh), vt + (k << rb_sh), k0 + k, kf, STEP == 32 && k + STEP < n);
                 }
-                done_tile();
             }
+            slot = (slot + 1) & (NBUF - 1);
+            --ahead;
+            --left;
         }
         const bool ends = t_end == at.nt;
         finish(ends && from_first, from_first);
         if (!ends && from_first) {
             // the workgroups that the rest of the item falls to, this one counted
             const long end = f1 + (at.nt - t_end);              // behind the item's last tile
-            const int m = at.s.n - at.c * a.qc;
-            cut = make_int4((int) ((end - 1) / share) - (int) blockIdx.x + 1, at.s.r0 + at.c * a.qc, m < a.qc ? m : a.qc, at.h);
+            const int qc = args().qc, m = at.s.n - at.c * qc;
+            cut = make_int4((int) ((end - 1) / share) - (int) blockIdx.x + 1, at.s.r0 + at.c * qc, m < qc ? m : qc, at.h);
         }
-        left -= a.extra;
-        at.t = at.nt - 1;
-        lk_pa_next(a, at, tk_sh);
+        left -= extra;
+        if (left > 0) lk_pa_next(args(), at, tk_sh);
     }
-    if (threadIdx.x == 0) a.cut[blockIdx.x] = cut;
+    if (threadIdx.x == 0) args().cut[blockIdx.x] = cut;
 }
 
 // ---- joining cut items ------------------------------------------------------------------------
@@ -723,33 +738,34 @@ lk_k_paged_attn(const LkPaArgs a) {
 // threads share the pieces out among them.  Many items: a workgroup has all dims, each wave some of them.
 template <int D, int RT, bool SPREAD>
 __global__ void __launch_bounds__(SPREAD ? 1024 : 256)
-lk_k_paged_join(const LkPaArgs a, int cb_n) {
+lk_k_paged_join(const LkPaArgs a, int cb_n, int wgs) {
     typedef typename LkElem<RT>::type RowT;
     constexpr int DB = D / 16, NT = SPREAD ? 1024 : 256, NV = NT / 64, PARTS = SPREAD ? DB : 1;
-    __shared__ int s_list[LK_PA_WGS];
-    __shared__ int s_count[LK_PA_WGS / 64];
-    __shared__ float s_w[LK_PA_WGS][16];                       // max, then weight
+    __shared__ int s_list[LK_PA_MAX_WGS];
+    __shared__ int s_count[LK_PA_MAX_WGS / 64];
+    __shared__ float s_w[LK_PA_MAX_WGS][16];                       // max, then weight
     __shared__ float s_r[2][NV][16];
     __shared__ lk_f4 s_o[SPREAD ? NT : 1];
     const int tid = threadIdx.x, lane = tid & 63, v = __builtin_amdgcn_readfirstlane(tid >> 6);
-    static_assert(NT >= LK_PA_WGS, "a thread for every workgroup's entry");
-
-    int4 mine = make_int4(0, 0, 0, 0);
-    uint64_t b = 0;
-    if (v < LK_PA_WGS / 64) {
-        mine = a.cut[tid];
-        b = __ballot(mine.x > 0);
-        if (lane == 0) s_count[v] = __builtin_popcountll(b);
+    uint64_t b[LK_PA_MAX_WGS / 64 / NV + 1];                   // the workgroups' entries of the wave that begin a cut item
+#pragma unroll
+    for (int i = 0; i * NV < LK_PA_MAX_WGS / 64; ++i) {
+        const int e = (i * NV + v) * 64 + lane;
+        const bool has = e < wgs && a.cut[e < wgs ? e : 0].x > 0;
+        b[i] = __ballot(has);
+        if (lane == 0 && i * NV + v < LK_PA_MAX_WGS / 64) s_count[i * NV + v] = __builtin_popcountll(b[i]);
     }
     __syncthreads();
-    int n = 0, off = 0;
+    int n = 0;
 #pragma unroll
-    for (int k = 0; k < LK_PA_WGS / 64; ++k) {
-        if (k < v) off += s_count[k];
-        n += s_count[k];
-    }
+    for (int k = 0; k < LK_PA_MAX_WGS / 64; ++k) n += s_count[k];
     if ((int) blockIdx.x >= n) return;
-    if (mine.x > 0) s_list[off + __builtin_popcountll(b & ((1ull << lane) - 1))] = tid;
+#pragma unroll
+    for (int i = 0; i * NV < LK_PA_MAX_WGS / 64; ++i) {
+        int off = 0;
+        for (int k = 0; k < i * NV + v && k < LK_PA_MAX_WGS / 64; ++k) off += s_count[k];
+        if ((b[i] >> lane) & 1) s_list[off + __builtin_popcountll(b[i] & ((1ull << lane) - 1))] = (i * NV + v) * 64 + lane;
+    }
     __syncthreads();
 
     const int blk = blockIdx.y / PARTS, nblk = gridDim.y / PARTS;
@@ -835,23 +851,28 @@ lk_k_paged_join(const LkPaArgs a, int cb_n) {
 // ---- host ---------------------------------------------------------------------------------------
 // How a workgroup's waves divide a tile, for chunks of `want` tokens of g query heads a kv head.
 struct LkPaShape { int cb, step, hg_sh, qw_sh, kw_sh, qc, extra; };
+// Column blocks a wave of the STEP 32 kernels holds: as many as its registers take.
+constexpr int lk_pa_cb32(int d, int type) { return (d == 64 ? 4 : 2) / (type == LK_F32 ? 2 : 1); }
 static LkPaShape lk_pa_shape(const lk_pages * p, int type, int max_new) {
-    const int g = p->n_heads / p->n_kv_heads, d = p->head_dim, nw = lk_pa_waves(d);
-    const int cb_max = type == LK_F32 ? 2 : 4, qw_max = 16 / cb_max < nw ? 16 / cb_max : nw;     // up to 256 columns
-    int want = max_new < 1 ? 1 : max_new > 64 ? 64 : max_new;
+    const int g = p->n_heads / p->n_kv_heads, d = p->head_dim;
+    const int want = max_new < 1 ? 1 : max_new > 64 ? 64 : max_new;
     LkPaShape s;
     const int nb = (want * g + 15) / 16;                       // blocks of columns
-    s.cb = nb >= 3 ? cb_max : nb >= 2 ? 2 : 1;
-    s.qw_sh = 0;
-    while ((s.cb << s.qw_sh) < nb && (1 << s.qw_sh) < qw_max) ++s.qw_sh;
+    s.step = nb > 2 ? 32 : 16;
+    s.cb = nb > 2 ? lk_pa_cb32(d, type) : nb;
+    const int nw = lk_pa_waves(d, s.step);
+    s.qw_sh = s.step == 32 && d == 128 ? 1 : 0;                // (a wave's share of a tile is 16 * 2^qw_sh keys and more)
+    while ((s.cb << s.qw_sh) < nb && (1 << s.qw_sh) < nw) ++s.qw_sh;
     const int qw = 1 << s.qw_sh;
     s.hg_sh = 0;
     while ((2 << s.hg_sh) * qw <= nw && p->n_kv_heads % (2 << s.hg_sh) == 0) ++s.hg_sh;
+#ifdef LK_PA_EXTRA
+    if (s.step == 32 && getenv("LKH")) while (s.hg_sh > atoi(getenv("LKH"))) --s.hg_sh;
+#endif
     s.kw_sh = lk_log2(nw / qw) - s.hg_sh;
-    // keys a wave and tile: 16 KB of K rows over the group's heads and the key shares, 16 * qw
-    s.step = qw > 1 ? 32 : 16;
-    int qc = s.cb * 16 * qw / g;                               // at least 1: up to 64 heads a kv head
+    int qc = s.cb * 16 * qw / g;
     if (qc > 64) qc = 64;
+    if (qc < 1) qc = 1;
     s.qc = 1 << lk_log2(qc);
     s.extra = s.step == 32 ? 6 : 2;
 #ifdef LK_PA_EXTRA
@@ -863,27 +884,26 @@ static int lk_pa_blocks(const LkPaShape & s) { return s.cb << (s.qw_sh + s.hg_sh
 
 template <int D, int RT, int CT, int CB, int STEP>
 static void lk_pa_run(const LkPaArgs & a, bool mod, hipStream_t st) {
-    const dim3 block(64 * lk_pa_waves(D));
-    if (mod) hipLaunchKernelGGL((lk_k_paged_attn<D, RT, CT, CB, STEP, true>), dim3(LK_PA_WGS), block, 0, st, a);
-    else     hipLaunchKernelGGL((lk_k_paged_attn<D, RT, CT, CB, STEP, false>), dim3(LK_PA_WGS), block, 0, st, a);
+    const dim3 grid(lk_pa_wgs(STEP)), block(64 * lk_pa_waves(D, STEP));
+    if (mod) hipLaunchKernelGGL((lk_k_paged_attn<D, RT, CT, CB, STEP, true>), grid, block, 0, st, a);
+    else     hipLaunchKernelGGL((lk_k_paged_attn<D, RT, CT, CB, STEP, false>), grid, block, 0, st, a);
 }
 template <int D, int RT, int CT>
 static void lk_pa_launch(const LkPaShape & s, const LkPaArgs & a, bool mod, hipStream_t st) {
-    constexpr int CBM = RT == LK_F32 ? 2 : 4;
-    if (s.step == 32)    lk_pa_run<D, RT, CT, CBM, 32>(a, mod, st);
+    if (s.step == 32)    lk_pa_run<D, RT, CT, lk_pa_cb32(D, RT), 32>(a, mod, st);
     else if (s.cb == 1)  lk_pa_run<D, RT, CT, 1, 16>(a, mod, st);
-    else if (s.cb == 2)  lk_pa_run<D, RT, CT, 2, 16>(a, mod, st);
-    else if constexpr (CBM == 4) lk_pa_run<D, RT, CT, 4, 16>(a, mod, st);
+    else                 lk_pa_run<D, RT, CT, 2, 16>(a, mod, st);
 }
 
 // Few items are cut into many pieces each: large workgroups, one for every 16 dims of a block of
 // columns.  Many items into few: small ones.
 template <int D, int RT>
-static void lk_pa_join(const LkPaArgs & a, int cuts, int nblk, int cb, hipStream_t st) {
+static void lk_pa_join(const LkPaArgs & a, int cuts, int nblk, const LkPaShape & s, hipStream_t st) {
+    const int wgs = lk_pa_wgs(s.step);
     if (cuts * nblk <= 256)
-        hipLaunchKernelGGL((lk_k_paged_join<D, RT, true>), dim3(cuts, nblk * (D / 16)), dim3(1024), 0, st, a, cb);
+        hipLaunchKernelGGL((lk_k_paged_join<D, RT, true>), dim3(cuts, nblk * (D / 16)), dim3(1024), 0, st, a, s.cb, wgs);
     else
-        hipLaunchKernelGGL((lk_k_paged_join<D, RT, false>), dim3(cuts, nblk), dim3(256), 0, st, a, cb);
+        hipLaunchKernelGGL((lk_k_paged_join<D, RT, false>), dim3(cuts, nblk), dim3(256), 0, st, a, s.cb, wgs);
 }
 
 static __device__ __align__(1024) char lk_pa_zeros[1024];      // never written
@@ -918,8 +938,9 @@ extern "C" size_t lk_paged_attn_work_bytes(const lk_pages * pages, int type, int
         lk_fail(hipErrorInvalidValue, "%s: max_new %d", W, max_new);
         return 0;
     }
-    const size_t blocks = (size_t) 2 * LK_PA_WGS * lk_pa_blocks(lk_pa_shape(pages, type, max_new));
-    return blocks * (16 * pages->head_dim * 4 + 16 * 8) + LK_PA_WGS * 16;
+    const LkPaShape s = lk_pa_shape(pages, type, max_new);
+    const size_t blocks = (size_t) 2 * lk_pa_wgs(s.step) * lk_pa_blocks(s);
+    return blocks * (16 * pages->head_dim * 4 + 16 * 8) + lk_pa_wgs(s.step) * 16;
 }
 
 extern "C" int lk_paged_attn(const lk_pages * pages, const lk_step * step, int type, const void * q, int ldq, float scale, float cap,
@@ -944,7 +965,7 @@ extern "C" int lk_paged_attn(const lk_pages * pages, const lk_step * step, int t
     if (!zeros) return err;
     const LkPaShape s = lk_pa_shape(pages, type, step->max_new);
     const int nblk = lk_pa_blocks(s), g = hq / pages->n_kv_heads, nhg = pages->n_kv_heads >> s.hg_sh;
-    const size_t blocks = (size_t) 2 * LK_PA_WGS * nblk;
+    const size_t blocks = (size_t) 2 * lk_pa_wgs(s.step) * nblk;
     float * acc = (float *) work;
     float2 * ml = (float2 *) (acc + blocks * 16 * d);
     const LkPaArgs a = { q, out, (const char *) pages->k, (const char *) pages->v, zeros, step->first, step->lens, step->table, step->pos,
@@ -965,15 +986,15 @@ extern "C" int lk_paged_attn(const lk_pages * pages, const lk_step * step, int t
     if (const int e = lk_launch_status(W)) return e;
     // no more items are cut than there are, nor than there are borders between the workgroups
     const long items = ((long) step->rows / s.qc + step->n_seqs) * nhg;
-    const int cuts = (int) (items < LK_PA_WGS - 1 ? items : LK_PA_WGS - 1);
+    const int cuts = (int) (items < lk_pa_wgs(s.step) - 1 ? items : lk_pa_wgs(s.step) - 1);
     if (d == 64) {
-        if (type == LK_F32)      lk_pa_join<64, LK_F32>(a, cuts, nblk, s.cb, st);
-        else if (type == LK_F16) lk_pa_join<64, LK_F16>(a, cuts, nblk, s.cb, st);
-        else                     lk_pa_join<64, LK_BF16>(a, cuts, nblk, s.cb, st);
+        if (type == LK_F32)      lk_pa_join<64, LK_F32>(a, cuts, nblk, s, st);
+        else if (type == LK_F16) lk_pa_join<64, LK_F16>(a, cuts, nblk, s, st);
+        else                     lk_pa_join<64, LK_BF16>(a, cuts, nblk, s, st);
     } else {
-        if (type == LK_F32)      lk_pa_join<128, LK_F32>(a, cuts, nblk, s.cb, st);
-        else if (type == LK_F16) lk_pa_join<128, LK_F16>(a, cuts, nblk, s.cb, st);
-        else                     lk_pa_join<128, LK_BF16>(a, cuts, nblk, s.cb, st);
+        if (type == LK_F32)      lk_pa_join<128, LK_F32>(a, cuts, nblk, s, st);
+        else if (type == LK_F16) lk_pa_join<128, LK_F16>(a, cuts, nblk, s, st);
+        else                     lk_pa_join<128, LK_BF16>(a, cuts, nblk, s, st);
     }
     return lk_launch_status(W);
 }
