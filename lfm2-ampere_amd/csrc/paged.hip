@@ -4,7 +4,7 @@
 //
 // Append, per row t (token i of sequence b, slot lens[b] + i) and head row x of D values:
 //     y = x * inv * w,  inv = 1 / sqrt(sum x^2 / D + eps)                  (fp32)
-//     a_i = position * freq_i                                             (fp64, exact: 31 + 24 bits)
+//     a_i = position * freq_i                                             (fp64, exact below position 2^29)
 //     (u, v) -> (u cos a - v sin a, u sin a + v cos a)                     (fp32; cos and sin fp64, rounded once)
 // q to its rows, k and v to the slot's page, each rounded once.  An angle in fp32 would be
 // off by 2^-24 of itself: 0.008 at position 131072, far above the rounding of 16-bit rows.
@@ -86,22 +86,22 @@ __device__ __forceinline__ float lk_head_sum(float v) {
     return v;
 }
 
-// A workgroup has one row and (of grid.y parts) a share of its head rows (q, k, then v heads),
+// A workgroup has R rows and (of grid.y parts) a share of their head rows (q, k, then v heads),
 // LPH lanes a head row.  A lane holds the two runs of four values that the rotation pairs: 4j and
 // rot/2 + 4j with halves, 8j and 8j + 4 with pairs or behind `rot`, so that nothing is exchanged between
-// lanes.  The rows are asked for first; meanwhile the lanes look for the row's sequence, all of
+// lanes.  The rows are asked for first; meanwhile the lanes look for the rows' sequences, all of
 // `first` at once, and one lane an angle forms the sines and cosines.
 // Bound by latency for few rows (three loads one behind the other: bounds, page, and the launch) and by
 // memory for many.
-template <int TYPE, int CTYPE, int LPH>
+template <int TYPE, int CTYPE, int LPH, int R>
 __global__ void __launch_bounds__(512)
 lk_k_paged_append(const LkAppendArgs a) {
     typedef typename LkElem<TYPE>::type T;
     typedef typename LkElem<CTYPE>::type C;
     constexpr int D = LPH * 8;
-    __shared__ __attribute__((aligned(16))) float s_c[D / 2], s_s[D / 2];
-    __shared__ int s_seq;
-    const int t = blockIdx.x, tid = threadIdx.x;
+    __shared__ __attribute__((aligned(16))) float s_c[R][D / 2], s_s[R][D / 2];
+    __shared__ unsigned long long s_seq[R];
+    const int t0 = blockIdx.x * R, tid = threadIdx.x;
     const int unit = blockIdx.y * blockDim.x + tid;
     const int head = unit / LPH, j = unit % LPH;
     const int nq = a.q ? a.hq : 0;
@@ -110,98 +110,120 @@ lk_k_paged_append(const LkAppendArgs a) {
     const bool split = !a.pairs && 8 * j < a.rot && !isv;
     const int lo = split ? 4 * j : 8 * j, hi = split ? a.rot / 2 + 4 * j : 8 * j + 4;
 
-    const T * src = isq ? (const T *) a.q + (size_t) t * a.ldq : isk ? (const T *) a.k + (size_t) t * a.ldk
-                                                                     : (const T *) a.v + (size_t) t * a.ldv;
-    src += hh * D;
+    const T * src = (const T *) (isq ? a.q : isk ? a.k : a.v) + hh * D;
+    const size_t ld = isq ? a.ldq : isk ? a.ldk : a.ldv;
     const float * w = isq ? a.qn : isk ? a.kn : nullptr;
-    float x0[4] = {}, x1[4] = {}, w0[4] = { 1, 1, 1, 1 }, w1[4] = { 1, 1, 1, 1 };
+    float x0[R][4] = {}, x1[R][4] = {}, w0[4] = { 1, 1, 1, 1 }, w1[4] = { 1, 1, 1, 1 };
     if (isq | isk | isv) {
-        lk_load<4>(src + lo, x0);
-        lk_load<4>(src + hi, x1);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int t = t0 + r < a.rows ? t0 + r : a.rows - 1;
+            lk_load<4>(src + t * ld + lo, x0[r]);
+            lk_load<4>(src + t * ld + hi, x1[r]);
+        }
         if (w) {
             lk_load<4>(w + lo, w0);
             lk_load<4>(w + hi, w1);
         }
     }
-    const float f = tid < a.rot / 2 ? a.freq[tid] : 0.0f;
-
-    // the row's sequence: of those that name the row the first
-    if (tid == 0) s_seq = 0x7FFFFFFF;
+    // the rows' sequences (of those that name a row the first) and slots
+    const int slots = a.width << a.page_sh;
+    if (tid < R) s_seq[tid] = ~0ull;
     __syncthreads();
     for (int b = tid; b < a.n_seqs; b += blockDim.x) {
-        const LkSeq s = lk_seq(a.first[b], a.first[b + 1], 0, a.rows, 0);
-        if (t >= s.r0 && t < s.r0 + s.n) atomicMin(&s_seq, b);
+        const LkSeq s = lk_seq(a.first[b], a.first[b + 1], a.lens[b], a.rows, slots);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int i = t0 + r - s.r0;
+            if (i >= 0 && i < s.n) atomicMin(&s_seq[r], (unsigned long long) b << 32 | (unsigned) (s.len + i));
+        }
     }
     __syncthreads();
-    const int b = __builtin_amdgcn_readfirstlane(s_seq);
-    if (b == 0x7FFFFFFF) return;                              // padding
-    const LkSeq s = lk_seq(a.first[b], a.first[b + 1], a.lens[b], a.rows, a.width << a.page_sh);
-    const int slot = s.len + (t - s.r0);
-    const bool in = slot < a.width << a.page_sh;
-    const int page = in ? a.table[(size_t) b * a.ldt + (slot >> a.page_sh)] : -1;
-    const int pos = a.pos ? a.pos[t] : slot;
-    if (tid < a.rot / 2) {
+    int page[R], slot[R];                                     // page -2: padding, nothing is written
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const unsigned b = __builtin_amdgcn_readfirstlane((int) (s_seq[r] >> 32));
+        slot[r] = b == ~0u ? 0 : __builtin_amdgcn_readfirstlane((int) s_seq[r]);
+        page[r] = a.table[(size_t) (b == ~0u ? 0 : b) * a.ldt + ((slot[r] < slots ? slot[r] : 0) >> a.page_sh)];
+        page[r] = b == ~0u ? -2 : slot[r] < slots && page[r] >= 0 ? page[r] : -1;
+    }
+    for (int i = tid; i < R * (a.rot / 2); i += blockDim.x) {
+        const int r = i / (a.rot / 2), k = i - r * (a.rot / 2);
+        int pos = 0;
+#pragma unroll
+        for (int u = 0; u < R; ++u) pos = u == r ? slot[u] : pos;
+        if (a.pos && t0 + r < a.rows) pos = a.pos[t0 + r];
         double sn, cs;
-        lk_sincos((double) pos * (double) f, sn, cs);
-        s_c[tid] = (float) cs;
-        s_s[tid] = (float) sn;
+        lk_sincos((double) pos * (double) a.freq[k], sn, cs);
+        s_c[r][k] = (float) cs;
+        s_s[r][k] = (float) sn;
     }
     __syncthreads();
     if (!(isq | isk | isv)) return;
-
-    if (w) {
-        float ss = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) ss = __builtin_fmaf(x0[i], x0[i], ss);
+    for (int r = 0; r < R; ++r) {
+        if (page[r] == -2) continue;
+        float (&y0)[4] = x0[r], (&y1)[4] = x1[r];
+        if (w) {
+            float ss = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) ss = __builtin_fmaf(x1[i], x1[i], ss);
-        ss = lk_head_sum<LPH>(ss);
-        const float inv = lk_rsqrt(__builtin_fmaf(ss, 1.0f / D, a.eps));
+            for (int i = 0; i < 4; ++i) ss = __builtin_fmaf(y0[i], y0[i], ss);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x0[i] = x0[i] * inv * w0[i];
-            x1[i] = x1[i] * inv * w1[i];
-        }
-    }
-    if (!isv && 8 * j < a.rot) {
-        const lk_f4 c = *(const lk_f4 *) (s_c + 4 * j), sn = *(const lk_f4 *) (s_s + 4 * j);
-        if (split) {
+            for (int i = 0; i < 4; ++i) ss = __builtin_fmaf(y1[i], y1[i], ss);
+            ss = lk_head_sum<LPH>(ss);
+            const float inv = lk_rsqrt(__builtin_fmaf(ss, 1.0f / D, a.eps));
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float u = x0[i], v = x1[i];
-                x0[i] = u * c[i] - v * sn[i];
-                x1[i] = u * sn[i] + v * c[i];
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float & e0 = i < 2 ? x0[2 * i] : x1[2 * i - 4], & e1 = i < 2 ? x0[2 * i + 1] : x1[2 * i - 3];
-                const float u = e0, v = e1;
-                e0 = u * c[i] - v * sn[i];
-                e1 = u * sn[i] + v * c[i];
+                y0[i] = y0[i] * inv * w0[i];
+                y1[i] = y1[i] * inv * w1[i];
             }
         }
-    }
-    if (isq) {
-        if (!a.qo) return;
-        T * o = (T *) a.qo + (size_t) t * a.ldqo + hh * D;
-        lk_store<4>(o + lo, x0);
-        lk_store<4>(o + hi, x1);
-    } else if (page >= 0 && page < a.n_pages) {
-        const size_t at = ((size_t) page << a.page_sh) + (slot & ((1 << a.page_sh) - 1));
-        C * o = (C *) (isk ? a.kp : a.vp) + (at * a.hkv + hh) * D;
-        lk_store<4>(o + lo, x0);
-        lk_store<4>(o + hi, x1);
+        if (!isv && 8 * j < a.rot) {
+            const lk_f4 c = *(const lk_f4 *) (s_c[r] + 4 * j), sn = *(const lk_f4 *) (s_s[r] + 4 * j);
+            if (split) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float u = y0[i], v = y1[i];
+                    y0[i] = u * c[i] - v * sn[i];
+                    y1[i] = u * sn[i] + v * c[i];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float & e0 = i < 2 ? y0[2 * i] : y1[2 * i - 4], & e1 = i < 2 ? y0[2 * i + 1] : y1[2 * i - 3];
+                    const float u = e0, v = e1;
+                    e0 = u * c[i] - v * sn[i];
+                    e1 = u * sn[i] + v * c[i];
+                }
+            }
+        }
+        if (isq) {
+            T * o = (T *) a.qo + (size_t) (t0 + r) * a.ldqo + hh * D;
+            lk_store<4>(o + lo, y0);
+            lk_store<4>(o + hi, y1);
+        } else if (page[r] >= 0 && page[r] < a.n_pages) {
+            const size_t at = ((size_t) page[r] << a.page_sh) + (slot[r] & ((1 << a.page_sh) - 1));
+            C * o = (C *) (isk ? a.kp : a.vp) + (at * a.hkv + hh) * D;
+            lk_store<4>(o + lo, y0);
+            lk_store<4>(o + hi, y1);
+        }
     }
 }
 
+template <int TYPE, int CTYPE, int LPH>
+static void lk_append_launch(const LkAppendArgs & a, hipStream_t st) {
+    const int units = ((a.q ? a.hq : 0) + 2 * a.hkv) * LPH;
+    const int ny = (units + 511) / 512, nt = ((units + ny - 1) / ny + 63) / 64 * 64;    // whole head rows a workgroup
+    // four rows a workgroup where that still fills the GPU
+    if ((long) a.rows * ny >= 2048)
+        hipLaunchKernelGGL((lk_k_paged_append<TYPE, CTYPE, LPH, 4>), dim3((a.rows + 3) / 4, ny), dim3(nt), 0, st, a);
+    else
+        hipLaunchKernelGGL((lk_k_paged_append<TYPE, CTYPE, LPH, 1>), dim3(a.rows, ny), dim3(nt), 0, st, a);
+}
 template <int TYPE, int CTYPE>
 static void lk_append_launch(const LkAppendArgs & a, int d, hipStream_t st) {
-    const int units = ((a.q ? a.hq : 0) + 2 * a.hkv) * (d / 8);
-    const int ny = (units + 511) / 512, nt = ((units + ny - 1) / ny + 63) / 64 * 64;
-    // whole head rows a workgroup: nt is a multiple of 16 lanes
-    if (d == 64) hipLaunchKernelGGL((lk_k_paged_append<TYPE, CTYPE, 8>), dim3(a.rows, ny), dim3(nt), 0, st, a);
-    else         hipLaunchKernelGGL((lk_k_paged_append<TYPE, CTYPE, 16>), dim3(a.rows, ny), dim3(nt), 0, st, a);
+    if (d == 64) lk_append_launch<TYPE, CTYPE, 8>(a, st);
+    else         lk_append_launch<TYPE, CTYPE, 16>(a, st);
 }
 
 extern "C" int lk_paged_append(const lk_pages * pages, const lk_step * step, int type, const void * q, int ldq, const void * k,

@@ -731,118 +731,158 @@ lk_k_paged_attn(const LkPaArgs) {
 }
 
 // ---- joining cut items ------------------------------------------------------------------------
-// grid (k, blocks of 16 columns x parts of their dims); workgroup (x, y) joins its block of the cut
-// items number x, x + k, ..  First all pieces' (max, sum) give their weights, then the rows are added
-// with loads that wait for nothing but each other, in the order of the pieces or of the threads' shares
-// of them.  Few items (SPREAD): they are cut into many pieces, so a workgroup has 16 dims of a block, and its
-// threads share the pieces out among them.  Many items: a workgroup has all dims, each wave some of them.
-template <int D, int RT, bool SPREAD>
-__global__ void __launch_bounds__(SPREAD ? 1024 : 256)
-lk_k_paged_join(const LkPaArgs a, int cb_n, int wgs) {
-    typedef typename LkElem<RT>::type RowT;
-    constexpr int DB = D / 16, NT = SPREAD ? 1024 : 256, NV = NT / 64, PARTS = SPREAD ? DB : 1;
-    __shared__ int s_list[LK_PA_MAX_WGS];
-    __shared__ int s_count[LK_PA_MAX_WGS / 64];
-    __shared__ float s_w[LK_PA_MAX_WGS][16];                       // max, then weight
-    __shared__ float s_r[2][NV][16];
-    __shared__ lk_f4 s_o[SPREAD ? NT : 1];
-    const int tid = threadIdx.x, lane = tid & 63, v = __builtin_amdgcn_readfirstlane(tid >> 6);
-    uint64_t b[LK_PA_MAX_WGS / 64 / NV + 1];                   // the workgroups' entries of the wave that begin a cut item
-#pragma unroll
-    for (int i = 0; i * NV < LK_PA_MAX_WGS / 64; ++i) {
-        const int e = (i * NV + v) * 64 + lane;
-        const bool has = e < wgs && a.cut[e < wgs ? e : 0].x > 0;
-        b[i] = __ballot(has);
-        if (lane == 0 && i * NV + v < LK_PA_MAX_WGS / 64) s_count[i * NV + v] = __builtin_popcountll(b[i]);
+// A block of 16 columns of a cut item: where its output goes, and which of its columns are there.
+struct LkPaBlock {
+    int c0, hh, live;              // first column of the chunk, kv head of the group, columns
+    __device__ __forceinline__ LkPaBlock(const LkPaArgs & a, const int4 & it, int blk, int cb_n) {
+        const int cb = blk % cb_n, qw = (blk / cb_n) & ((1 << a.qw_sh) - 1);
+        hh = (blk / cb_n) >> a.qw_sh;
+        c0 = (qw * cb_n + cb) * 16;
+        live = lk_clamp(it.z * a.g - c0, 0, 16);            // columns are (token, head) in order: the live ones come first
     }
+    // value e of dims 16 db ..: column e / 4, its dims 4 (e % 4) ..
+    template <int D, typename RowT>
+    __device__ __forceinline__ void store(const LkPaArgs & a, const int4 & it, int db, int e, const lk_f4 & r, float l) const {
+        const int c = c0 + (e >> 2), t = c / a.g, head = ((it.w << a.hg_sh) + hh) * a.g + (c - t * a.g);
+        const float il = lk_pa_inverse(l), v[4] = { r[0] * il, r[1] * il, r[2] * il, r[3] * il };
+        lk_store<4>((RowT *) a.out + (size_t) (it.y + t) * a.ldo + (size_t) head * D + 16 * db + 4 * (e & 3), v);
+    }
+};
+
+// Many items, cut into few pieces each: workgroup (x, blk) joins block blk of the item that begins in
+// workgroup x, each wave some of its dims, four pieces asked for at once.
+template <int D, int RT>
+__global__ void __launch_bounds__(256)
+lk_k_paged_join(const LkPaArgs a, int cb_n) {
+    constexpr int DB = D / 16, W = DB / 4;
+    const int4 it = a.cut[blockIdx.x];
+    if (it.x == 0) return;
+    const int lane = threadIdx.x & 63, db0 = (threadIdx.x >> 6) * W;
+    const int blk = blockIdx.y, nblk = gridDim.y;
+    const LkPaBlock B(a, it, blk, cb_n);
+    if (lane >= 4 * B.live) return;
+    float m = -LK_PA_NONE, l = 0.0f;
+    lk_f4 o[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) o[i] = (lk_f4){ 0.f, 0.f, 0.f, 0.f };
+    for (int k0 = 0; k0 < it.x; k0 += 4) {
+        float2 ml[4];
+        lk_f4 x[4][W];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int k = k0 + j < it.x ? k0 + j : k0;
+            const size_t p = (size_t) (2 * (blockIdx.x + k) + (k == 0)) * nblk + blk;
+            ml[j] = a.ml[p * 16 + (lane >> 2)];
+#pragma unroll
+            for (int i = 0; i < W; ++i) x[j][i] = ((const lk_f4 *) a.acc)[(p * DB + db0 + i) * 64 + lane];
+        }
+        float mx = m;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mx = fmaxf(mx, ml[j].x);
+        const float f = lk_exp2(m - mx);
+        m = mx;
+        l *= f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) o[i] *= f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float fj = k0 + j < it.x ? lk_exp2(ml[j].x - mx) : 0.0f;
+            l = __builtin_fmaf(ml[j].y, fj, l);
+#pragma unroll
+            for (int i = 0; i < W; ++i) o[i] += x[j][i] * fj;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i) B.template store<D, typename LkElem<RT>::type>(a, it, db0 + i, lane, o[i], l);
+}
+
+// Few items, cut into many pieces: workgroup (x, y) joins 16 dims of a block of the cut items number x,
+// x + gridDim.x, ..  All pieces' (max, sum) first give their weights; then the threads are divided over the
+// block's live values and as many pieces at once as fit, and their sums are added in order.
+template <int D, int RT>
+__global__ void __launch_bounds__(1024)
+lk_k_paged_spread(const LkPaArgs a, int cb_n, int wgs) {
+    constexpr int DB = D / 16, NT = 1024, NV = NT / 64, MW = LK_PA_MAX_WGS / 64;
+    __shared__ int4 s_item[LK_PA_MAX_WGS];
+    __shared__ int s_from[LK_PA_MAX_WGS], s_count[MW];
+    __shared__ float s_w[LK_PA_MAX_WGS][16], s_r[2][NV][16];
+    __shared__ lk_f4 s_o[NT];
+    const int tid = threadIdx.x, lane = tid & 63, v = __builtin_amdgcn_readfirstlane(tid >> 6);
+    static_assert(NT >= LK_PA_MAX_WGS, "a thread for every workgroup's entry");
+    // the items that are cut, in order
+    int4 mine = make_int4(0, 0, 0, 0);
+    if (tid < wgs) mine = a.cut[tid];
+    const uint64_t has = __ballot(mine.x > 0);
+    if (lane == 0 && v < MW) s_count[v] = __builtin_popcountll(has);
     __syncthreads();
-    int n = 0;
+    int n = 0, off = 0;
 #pragma unroll
-    for (int k = 0; k < LK_PA_MAX_WGS / 64; ++k) n += s_count[k];
-    if ((int) blockIdx.x >= n) return;
-#pragma unroll
-    for (int i = 0; i * NV < LK_PA_MAX_WGS / 64; ++i) {
-        int off = 0;
-        for (int k = 0; k < i * NV + v && k < LK_PA_MAX_WGS / 64; ++k) off += s_count[k];
-        if ((b[i] >> lane) & 1) s_list[off + __builtin_popcountll(b[i] & ((1ull << lane) - 1))] = (i * NV + v) * 64 + lane;
+    for (int k = 0; k < MW; ++k) {
+        if (k < v) off += s_count[k];
+        n += s_count[k];
+    }
+    if (mine.x > 0) {
+        off += __builtin_popcountll(has & ((1ull << lane) - 1));
+        s_item[off] = mine;
+        s_from[off] = tid;
     }
     __syncthreads();
 
-    const int blk = blockIdx.y / PARTS, nblk = gridDim.y / PARTS;
-    // the block's columns: kv head hh of the group, column group qw, block cb
-    const int cb = blk % cb_n, qw = (blk / cb_n) & ((1 << a.qw_sh) - 1), hh = (blk / cb_n) >> a.qw_sh;
-    const int c0 = (qw * cb_n + cb) * 16;
+    const int blk = blockIdx.y / DB, db = blockIdx.y % DB, nblk = gridDim.y / DB, col = tid & 15;
     for (int x = blockIdx.x; x < n; x += gridDim.x) {
-        const int w0 = s_list[x];
-        const int4 it = a.cut[w0];
-        const int live = lk_clamp(it.z * a.g - c0, 0, 16);     // columns are (token, head) in order: the live ones come first
-        if (live == 0) continue;                               // the same for every thread
+        const int4 it = s_item[x];
+        const int w0 = s_from[x];
+        const LkPaBlock B(a, it, blk, cb_n);
+        if (B.live == 0) continue;                             // the same for every thread
         auto piece = [&](int k) -> size_t { return (size_t) (2 * (w0 + k) + (k == 0)) * nblk + blk; };
-        // weights
-        const int col = tid & 15;
-        float m = -LK_PA_NONE;
-        for (int k = tid >> 4; k < it.x; k += NT / 16) {
-            const float x0 = col < live ? a.ml[piece(k) * 16 + col].x : -LK_PA_NONE;
-            s_w[k][col] = x0;
-            m = fmaxf(m, x0);
+        float2 ml[LK_PA_MAX_WGS * 16 / NT];                    // of the thread's (piece, column) pairs
+        float m = -LK_PA_NONE, l = 0.0f;
+#pragma unroll
+        for (int j = 0; j < LK_PA_MAX_WGS * 16 / NT; ++j) {
+            const int k = (tid >> 4) + j * (NT / 16);
+            ml[j] = make_float2(-LK_PA_NONE, 0.0f);
+            if (k < it.x && col < B.live) ml[j] = a.ml[piece(k) * 16 + col];
+            m = fmaxf(m, ml[j].x);
         }
         m = lk_xrow_max(m);
         if (lane < 16) s_r[0][v][col] = m;
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < NV; ++k) m = fmaxf(m, s_r[0][k][col]);
-        float l = 0.0f;
-        for (int k = tid >> 4; k < it.x; k += NT / 16) {
-            const float f = lk_exp2(s_w[k][col] - m);
-            s_w[k][col] = f;
-            l += col < live ? a.ml[piece(k) * 16 + col].y * f : 0.0f;
+#pragma unroll
+        for (int j = 0; j < LK_PA_MAX_WGS * 16 / NT; ++j) {
+            const int k = (tid >> 4) + j * (NT / 16);
+            const float f = lk_exp2(ml[j].x - m);
+            if (k < it.x) s_w[k][col] = f;
+            l = __builtin_fmaf(ml[j].y, f, l);
         }
         l = lk_xrow_sum(l);
         if (lane < 16) s_r[1][v][col] = l;
         __syncthreads();
-        auto store = [&](int db, int e, lk_f4 r) {             // value e: column e / 4, dims 4 * (e % 4) of the block
-            const int cc = e >> 2;
+        const int e_sh = B.live > 8 ? 6 : B.live > 4 ? 5 : 4, e = tid & ((1 << e_sh) - 1), pp = NT >> e_sh;
+        lk_f4 o = { 0.f, 0.f, 0.f, 0.f };
+        if (e < 4 * B.live) {
+#pragma unroll 8
+            for (int k = tid >> e_sh; k < it.x; k += pp)
+                o += ((const lk_f4 *) a.acc)[(piece(k) * DB + db) * 64 + e] * s_w[k][e >> 2];
+        }
+        s_o[tid] = o;
+        __syncthreads();
+        // eight threads' sums at a time, then those
+        if ((tid >> e_sh) % 8 == 0) {
+            lk_f4 r = s_o[tid];
+#pragma unroll
+            for (int k = 1; k < 8; ++k) r += s_o[tid + (k << e_sh)];
+            s_o[tid] = r;
+        }
+        __syncthreads();
+        if (tid < 4 * B.live) {
+            lk_f4 r = s_o[tid];
+            for (int k = 8; k < pp; k += 8) r += s_o[(k << e_sh) + tid];
             float sum = 0.0f;
 #pragma unroll
-            for (int k = 0; k < NV; ++k) sum += s_r[1][k][cc];
-            const float il = lk_pa_inverse(sum);
-            const int c = c0 + cc, t = c / a.g, head = ((it.w << a.hg_sh) + hh) * a.g + (c - t * a.g);
-            RowT * dst = (RowT *) a.out + (size_t) (it.y + t) * a.ldo + (size_t) head * D + 16 * db + 4 * (e & 3);
-            const float w[4] = { r[0] * il, r[1] * il, r[2] * il, r[3] * il };
-            lk_store<4>(dst, w);
-        };
-        if constexpr (SPREAD) {
-            const int db = blockIdx.y % PARTS;
-            const int e_sh = live > 8 ? 6 : live > 4 ? 5 : 4, e = tid & ((1 << e_sh) - 1), pp = NT >> e_sh;
-            lk_f4 o = { 0.f, 0.f, 0.f, 0.f };
-            if (e < 4 * live) {
-#pragma unroll 4
-                for (int k = tid >> e_sh; k < it.x; k += pp)
-                    o += ((const lk_f4 *) a.acc)[(piece(k) * DB + db) * 64 + e] * s_w[k][e >> 2];
-            }
-            s_o[tid] = o;
-            __syncthreads();
-            if (tid < 4 * live) {
-                lk_f4 r = s_o[tid];
-                const int most = pp < it.x ? pp : it.x;
-                for (int k = 1; k < most; ++k) r += s_o[(k << e_sh) + tid];
-                store(db, tid, r);
-            }
-        } else {
-            constexpr int W = DB / NV;                          // blocks of dims a wave
-            if (lane < 4 * live) {
-                lk_f4 o[W];
-#pragma unroll
-                for (int i = 0; i < W; ++i) o[i] = (lk_f4){ 0.f, 0.f, 0.f, 0.f };
-#pragma unroll 4
-                for (int k = 0; k < it.x; ++k) {
-                    const float f = s_w[k][lane >> 2];
-#pragma unroll
-                    for (int i = 0; i < W; ++i) o[i] += ((const lk_f4 *) a.acc)[(piece(k) * DB + v * W + i) * 64 + lane] * f;
-                }
-#pragma unroll
-                for (int i = 0; i < W; ++i) store(v * W + i, lane, o[i]);
-            }
+            for (int k = 0; k < NV; ++k) sum += s_r[1][k][tid >> 2];
+            B.template store<D, typename LkElem<RT>::type>(a, it, db, tid, r, sum);
         }
         __syncthreads();
     }
@@ -865,7 +905,8 @@ static LkPaShape lk_pa_shape(const lk_pages * p, int type, int max_new) {
     while ((s.cb << s.qw_sh) < nb && (1 << s.qw_sh) < nw) ++s.qw_sh;
     const int qw = 1 << s.qw_sh;
     s.hg_sh = 0;
-    while ((2 << s.hg_sh) * qw <= nw && p->n_kv_heads % (2 << s.hg_sh) == 0) ++s.hg_sh;
+    // few heads a group where the columns are many: what a cut item leaves behind is 16 KB a wave and more
+    while ((2 << s.hg_sh) * qw <= nw && p->n_kv_heads % (2 << s.hg_sh) == 0 && (s.step == 16 || s.hg_sh < 1)) ++s.hg_sh;
 #ifdef LK_PA_EXTRA
     if (s.step == 32 && getenv("LKH")) while (s.hg_sh > atoi(getenv("LKH"))) --s.hg_sh;
 #endif
@@ -874,7 +915,7 @@ static LkPaShape lk_pa_shape(const lk_pages * p, int type, int max_new) {
     if (qc > 64) qc = 64;
     if (qc < 1) qc = 1;
     s.qc = 1 << lk_log2(qc);
-    s.extra = s.step == 32 ? 6 : 2;
+    s.extra = s.step == 32 ? 5 : 2;
 #ifdef LK_PA_EXTRA
     s.extra = getenv("LKX") ? atoi(getenv("LKX")) : s.extra;
 #endif
@@ -895,15 +936,13 @@ static void lk_pa_launch(const LkPaShape & s, const LkPaArgs & a, bool mod, hipS
     else                 lk_pa_run<D, RT, CT, 2, 16>(a, mod, st);
 }
 
-// Few items are cut into many pieces each: large workgroups, one for every 16 dims of a block of
-// columns.  Many items into few: small ones.
 template <int D, int RT>
-static void lk_pa_join(const LkPaArgs & a, int cuts, int nblk, const LkPaShape & s, hipStream_t st) {
+static void lk_pa_join(const LkPaArgs & a, long items, int nblk, const LkPaShape & s, hipStream_t st) {
     const int wgs = lk_pa_wgs(s.step);
-    if (cuts * nblk <= 256)
-        hipLaunchKernelGGL((lk_k_paged_join<D, RT, true>), dim3(cuts, nblk * (D / 16)), dim3(1024), 0, st, a, s.cb, wgs);
+    if (items <= wgs / 32)
+        hipLaunchKernelGGL((lk_k_paged_spread<D, RT>), dim3((unsigned) items, nblk * (D / 16)), dim3(1024), 0, st, a, s.cb, wgs);
     else
-        hipLaunchKernelGGL((lk_k_paged_join<D, RT, false>), dim3(cuts, nblk), dim3(256), 0, st, a, s.cb, wgs);
+        hipLaunchKernelGGL((lk_k_paged_join<D, RT>), dim3(wgs - 1, nblk), dim3(256), 0, st, a, s.cb);
 }
 
 static __device__ __align__(1024) char lk_pa_zeros[1024];      // never written
@@ -984,17 +1023,15 @@ extern "C" int lk_paged_attn(const lk_pages * pages, const lk_step * step, int t
         else                     lk_pa_launch<128, LK_BF16, LK_BF16>(s, a, mod, st);
     }
     if (const int e = lk_launch_status(W)) return e;
-    // no more items are cut than there are, nor than there are borders between the workgroups
-    const long items = ((long) step->rows / s.qc + step->n_seqs) * nhg;
-    const int cuts = (int) (items < lk_pa_wgs(s.step) - 1 ? items : lk_pa_wgs(s.step) - 1);
+    const long items = ((long) step->rows / s.qc + step->n_seqs) * nhg;       // at most
     if (d == 64) {
-        if (type == LK_F32)      lk_pa_join<64, LK_F32>(a, cuts, nblk, s, st);
-        else if (type == LK_F16) lk_pa_join<64, LK_F16>(a, cuts, nblk, s, st);
-        else                     lk_pa_join<64, LK_BF16>(a, cuts, nblk, s, st);
+        if (type == LK_F32)      lk_pa_join<64, LK_F32>(a, items, nblk, s, st);
+        else if (type == LK_F16) lk_pa_join<64, LK_F16>(a, items, nblk, s, st);
+        else                     lk_pa_join<64, LK_BF16>(a, items, nblk, s, st);
     } else {
-        if (type == LK_F32)      lk_pa_join<128, LK_F32>(a, cuts, nblk, s, st);
-        else if (type == LK_F16) lk_pa_join<128, LK_F16>(a, cuts, nblk, s, st);
-        else                     lk_pa_join<128, LK_BF16>(a, cuts, nblk, s, st);
+        if (type == LK_F32)      lk_pa_join<128, LK_F32>(a, items, nblk, s, st);
+        else if (type == LK_F16) lk_pa_join<128, LK_F16>(a, items, nblk, s, st);
+        else                     lk_pa_join<128, LK_BF16>(a, items, nblk, s, st);
     }
     return lk_launch_status(W);
 }
