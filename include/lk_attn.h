@@ -581,7 +581,7 @@ typedef struct lk_step {
  *   a_i = position * freq_i, i < rot / 2, the product and its sine and cosine in fp64;
  *   LK_ROPE_HALVES: the pair is (y_i, y_{i + rot/2}), LK_ROPE_PAIRS: (y_2i, y_{2i+1});
  *   (u, v) -> (u cos a - v sin a, u sin a + v cos a); values from rot on are not rotated
- * in fp32, rounded once.  freq fp32 [rot / 2], rot a multiple of 8 up to head_dim, or freq NULL
+ * in fp32, rounded once.  freq fp32 [rot / 2], rot a multiple of 16 up to head_dim, or freq NULL
  * with rot 0: no rotation.  |a_i| below 2^31.  Squares are summed in fp32.
  * q, k, v, qo are rows of `type` (LK_F32 or LK_F16 with fp16 pools, LK_BF16 with bf16 pools) of
  * n_heads or n_kv_heads heads side by side, ld* elements apart (parts of one wide row as

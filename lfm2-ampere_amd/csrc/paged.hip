@@ -76,29 +76,31 @@ __device__ __forceinline__ float lk_rsqrt(float a) {
     return __builtin_fmaf(r * 0.5f, e, r);
 }
 
-// Sum over the 8 or 16 lanes of a head row.
+// Sum over the 4 or 8 lanes of a head row.
 template <int LPH>
 __device__ __forceinline__ float lk_head_sum(float v) {
     v += lk_dpp<LK_DPP_QP_XOR1>(v);
     v += lk_dpp<LK_DPP_QP_XOR2>(v);
-    v += lk_dpp<LK_DPP_HMIRROR>(v);
-    if constexpr (LPH == 16) v += lk_dpp<LK_DPP_MIRROR>(v);
+    if constexpr (LPH == 8) v += lk_dpp<LK_DPP_HMIRROR>(v);
     return v;
 }
 
 // A workgroup has R rows and (of grid.y parts) a share of their head rows (q, k, then v heads),
-// LPH lanes a head row.  A lane holds the two runs of four values that the rotation pairs: 4j and
-// rot/2 + 4j with halves, 8j and 8j + 4 with pairs or behind `rot`, so that nothing is exchanged between
+// LPH lanes a head row.  A lane holds the two runs of eight values that the rotation pairs: 8j and
+// rot/2 + 8j with halves, 16j and 16j + 8 with pairs or behind `rot`, so that nothing is exchanged between
 // lanes.  The rows are asked for first; meanwhile the lanes look for the rows' sequences, all of
 // `first` at once, and one lane an angle forms the sines and cosines.
-// Bound by latency for few rows (three loads one behind the other: bounds, page, and the launch) and by
-// memory for many.
+// Bound by latency for few rows (three loads one behind the other: bounds, page, and the launch; one row of
+// 32 + 8 + 8 heads of 64 in fp32 3.2 us in a graph) and by memory for many: 8192 rows of fp16 19.6 us, 4.3 TB/s,
+// next to 5.15 of a large copy.  Eight values a run: with four (twice the lanes, loads of 8 bytes) the
+// instructions bound it, 23.8 us.
+#define LK_APPEND_ROWS 2           // per workgroup, where there are many; 1: 21.1 us, 4: 20.7 us
 template <int TYPE, int CTYPE, int LPH, int R>
 __global__ void __launch_bounds__(512)
 lk_k_paged_append(const LkAppendArgs a) {
     typedef typename LkElem<TYPE>::type T;
     typedef typename LkElem<CTYPE>::type C;
-    constexpr int D = LPH * 8;
+    constexpr int D = LPH * 16;
     __shared__ __attribute__((aligned(16))) float s_c[R][D / 2], s_s[R][D / 2];
     __shared__ unsigned long long s_seq[R];
     const int t0 = blockIdx.x * R, tid = threadIdx.x;
@@ -107,23 +109,23 @@ lk_k_paged_append(const LkAppendArgs a) {
     const int nq = a.q ? a.hq : 0;
     const bool isq = head < nq, isk = !isq && head < nq + a.hkv, isv = !isq && !isk && head < nq + 2 * a.hkv;
     const int hh = isq ? head : isk ? head - nq : isv ? head - nq - a.hkv : 0;
-    const bool split = !a.pairs && 8 * j < a.rot && !isv;
-    const int lo = split ? 4 * j : 8 * j, hi = split ? a.rot / 2 + 4 * j : 8 * j + 4;
+    const bool split = !a.pairs && 16 * j < a.rot && !isv;
+    const int lo = split ? 8 * j : 16 * j, hi = split ? a.rot / 2 + 8 * j : 16 * j + 8;
 
     const T * src = (const T *) (isq ? a.q : isk ? a.k : a.v) + hh * D;
     const size_t ld = isq ? a.ldq : isk ? a.ldk : a.ldv;
     const float * w = isq ? a.qn : isk ? a.kn : nullptr;
-    float x0[R][4] = {}, x1[R][4] = {}, w0[4] = { 1, 1, 1, 1 }, w1[4] = { 1, 1, 1, 1 };
+    float x0[R][8], x1[R][8], w0[8], w1[8];
     if (isq | isk | isv) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int t = t0 + r < a.rows ? t0 + r : a.rows - 1;
-            lk_load<4>(src + t * ld + lo, x0[r]);
-            lk_load<4>(src + t * ld + hi, x1[r]);
+            lk_load<8>(src + t * ld + lo, x0[r]);
+            lk_load<8>(src + t * ld + hi, x1[r]);
         }
         if (w) {
-            lk_load<4>(w + lo, w0);
-            lk_load<4>(w + hi, w1);
+            lk_load<8>(w + lo, w0);
+            lk_load<8>(w + hi, w1);
         }
     }
     // the rows' sequences (of those that name a row the first) and slots
@@ -163,49 +165,50 @@ lk_k_paged_append(const LkAppendArgs a) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         if (page[r] == -2) continue;
-        float (&y0)[4] = x0[r], (&y1)[4] = x1[r];
+        float (&y0)[8] = x0[r], (&y1)[8] = x1[r];
         if (w) {
             float ss = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) ss = __builtin_fmaf(y0[i], y0[i], ss);
+            for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(y0[i], y0[i], ss);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) ss = __builtin_fmaf(y1[i], y1[i], ss);
+            for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(y1[i], y1[i], ss);
             ss = lk_head_sum<LPH>(ss);
             const float inv = lk_rsqrt(__builtin_fmaf(ss, 1.0f / D, a.eps));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < 8; ++i) {
                 y0[i] = y0[i] * inv * w0[i];
                 y1[i] = y1[i] * inv * w1[i];
             }
         }
-        if (!isv && 8 * j < a.rot) {
-            const lk_f4 c = *(const lk_f4 *) (s_c[r] + 4 * j), sn = *(const lk_f4 *) (s_s[r] + 4 * j);
+        if (!isv && 16 * j < a.rot) {
+            float c[8], sn[8];
+            lk_load<8>(s_c[r] + 8 * j, c);
+            lk_load<8>(s_s[r] + 8 * j, sn);
+            auto turn = [&](float & u, float & v, int i) {
+                const float p = u;
+                u = p * c[i] - v * sn[i];
+                v = p * sn[i] + v * c[i];
+            };
             if (split) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float u = y0[i], v = y1[i];
-                    y0[i] = u * c[i] - v * sn[i];
-                    y1[i] = u * sn[i] + v * c[i];
-                }
+                for (int i = 0; i < 8; ++i) turn(y0[i], y1[i], i);
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    float & e0 = i < 2 ? y0[2 * i] : y1[2 * i - 4], & e1 = i < 2 ? y0[2 * i + 1] : y1[2 * i - 3];
-                    const float u = e0, v = e1;
-                    e0 = u * c[i] - v * sn[i];
-                    e1 = u * sn[i] + v * c[i];
+                    turn(y0[2 * i], y0[2 * i + 1], i);
+                    turn(y1[2 * i], y1[2 * i + 1], 4 + i);
                 }
             }
         }
         if (isq) {
             T * o = (T *) a.qo + (size_t) (t0 + r) * a.ldqo + hh * D;
-            lk_store<4>(o + lo, y0);
-            lk_store<4>(o + hi, y1);
+            lk_store<8>(o + lo, y0);
+            lk_store<8>(o + hi, y1);
         } else if (page[r] >= 0 && page[r] < a.n_pages) {
             const size_t at = ((size_t) page[r] << a.page_sh) + (slot[r] & ((1 << a.page_sh) - 1));
             C * o = (C *) (isk ? a.kp : a.vp) + (at * a.hkv + hh) * D;
-            lk_store<4>(o + lo, y0);
-            lk_store<4>(o + hi, y1);
+            lk_store<8>(o + lo, y0);
+            lk_store<8>(o + hi, y1);
         }
     }
 }
@@ -214,16 +217,16 @@ template <int TYPE, int CTYPE, int LPH>
 static void lk_append_launch(const LkAppendArgs & a, hipStream_t st) {
     const int units = ((a.q ? a.hq : 0) + 2 * a.hkv) * LPH;
     const int ny = (units + 511) / 512, nt = ((units + ny - 1) / ny + 63) / 64 * 64;    // whole head rows a workgroup
-    // four rows a workgroup where that still fills the GPU
+    // several rows a workgroup where that still fills the GPU
     if ((long) a.rows * ny >= 2048)
-        hipLaunchKernelGGL((lk_k_paged_append<TYPE, CTYPE, LPH, 4>), dim3((a.rows + 3) / 4, ny), dim3(nt), 0, st, a);
+        hipLaunchKernelGGL((lk_k_paged_append<TYPE, CTYPE, LPH, LK_APPEND_ROWS>), dim3((a.rows - 1) / LK_APPEND_ROWS + 1, ny), dim3(nt), 0, st, a);
     else
         hipLaunchKernelGGL((lk_k_paged_append<TYPE, CTYPE, LPH, 1>), dim3(a.rows, ny), dim3(nt), 0, st, a);
 }
 template <int TYPE, int CTYPE>
 static void lk_append_launch(const LkAppendArgs & a, int d, hipStream_t st) {
-    if (d == 64) lk_append_launch<TYPE, CTYPE, 8>(a, st);
-    else         lk_append_launch<TYPE, CTYPE, 16>(a, st);
+    if (d == 64) lk_append_launch<TYPE, CTYPE, 4>(a, st);
+    else         lk_append_launch<TYPE, CTYPE, 8>(a, st);
 }
 
 extern "C" int lk_paged_append(const lk_pages * pages, const lk_step * step, int type, const void * q, int ldq, const void * k,
@@ -234,8 +237,8 @@ extern "C" int lk_paged_append(const lk_pages * pages, const lk_step * step, int
     if (const int e = lk_paged_check_type(W, pages, type)) return e;
     const int d = pages->head_dim, hq = pages->n_heads, hkv = pages->n_kv_heads;
     if (style != LK_ROPE_HALVES && style != LK_ROPE_PAIRS) return lk_fail(hipErrorInvalidValue, "%s: style %d", W, style);
-    if (rot < 0 || rot > d || rot % 8 != 0 || (rot > 0) != (freq != nullptr))
-        return lk_fail(hipErrorInvalidValue, "%s: rot %d (a multiple of 8 up to %d; 0 without freq)", W, rot, d);
+    if (rot < 0 || rot > d || rot % 16 != 0 || (rot > 0) != (freq != nullptr))
+        return lk_fail(hipErrorInvalidValue, "%s: rot %d (a multiple of 16 up to %d; 0 without freq)", W, rot, d);
     if (!(eps >= 0.0f)) return lk_fail(hipErrorInvalidValue, "%s: eps %g", W, (double) eps);
     if (step->rows == 0 || step->n_seqs == 0) return 0;
     if (!k || !v || (q != nullptr) != (qo != nullptr))

@@ -141,6 +141,29 @@ __device__ __forceinline__ long lk_uniform64(long v) {
     return (long) ((unsigned long) hi << 32 | lo);
 }
 
+// Sum of a value over the lanes up to each, by lane shifts where the sums fit 32 bits.
+__device__ __forceinline__ long lk_pa_scan(long v) {
+    const int lane = threadIdx.x & 63;
+    if (__ballot(v >> 25) == 0) {
+        uint32_t s = (uint32_t) v;
+#ifdef __HIP_DEVICE_COMPILE__
+        s += __builtin_amdgcn_update_dpp(0, (int) s, 0x111, 0xF, 0xF, false);      // row_shr 1, 2, 4, 8: within 16 lanes
+        s += __builtin_amdgcn_update_dpp(0, (int) s, 0x112, 0xF, 0xF, false);
+        s += __builtin_amdgcn_update_dpp(0, (int) s, 0x114, 0xF, 0xF, false);
+        s += __builtin_amdgcn_update_dpp(0, (int) s, 0x118, 0xF, 0xF, false);
+        s += __builtin_amdgcn_update_dpp(0, (int) s, 0x142, 0xA, 0xF, false);      // lane 15 of a row to the next, for rows 1 and 3
+        s += __builtin_amdgcn_update_dpp(0, (int) s, 0x143, 0xC, 0xF, false);      // lane 31 to rows 2 and 3
+#endif
+        return s;
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const long t = lk_shfl64(v, (lane - o) & 63);
+        if (lane >= o) v += t;
+    }
+    return v;
+}
+
 // A place on the line: tile t of the nt tiles of (sequence b, chunk c, head group h).
 struct LkPaAt {
     int b, c, h, t, nt, vis;
@@ -235,16 +258,22 @@ lk_k_paged_attn(const LkPaArgs) {
     const int kpw = (1 << tk_sh) >> kw_sh;                   // of them the wave's
 
     // ---- this workgroup's run of the line ---------------------------------------------
-    long total = 0, mine = 0, before = 0;
+    long total = 0, mine = 0, sum = 0, before = 0;             // sum: of the sequences up to the lane's
     LkSeq ls = { 0, 0, 0 };
     for (int b = lane; b < a0.n_seqs; b += 64) {
         ls = lk_pa_seq(a0, b);
         mine = lk_pa_seq_tiles(a0, ls, tk_sh);
         total += mine;
     }
+    const bool one_pass = a0.n_seqs <= 64;
+    if (one_pass) {
+        sum = lk_pa_scan(mine);
+        total = lk_uniform64(lk_shfl64(sum, 63));
+    } else {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) total += lk_shfl64(total, lane ^ o);
-    total = lk_uniform64(total);
+        for (int o = 32; o > 0; o >>= 1) total += lk_shfl64(total, lane ^ o);
+        total = lk_uniform64(total);
+    }
     const long share = (total + lk_pa_wgs(STEP) - 1) / lk_pa_wgs(STEP);
     const long f0 = share * blockIdx.x, f1 = f0 + share < total ? f0 + share : total;
     if (f0 >= f1) {
@@ -253,19 +282,14 @@ lk_k_paged_attn(const LkPaArgs) {
     }
     LkPaAt at;
     for (int b0 = 0;; b0 += 64) {                              // ends: f0 is below the total
-        const int b = b0 + lane;
-        if (a0.n_seqs > 64) {
+        if (!one_pass) {
+            const int b = b0 + lane;
             mine = 0;
             if (b < a0.n_seqs) {
                 ls = lk_pa_seq(a0, b);
                 mine = lk_pa_seq_tiles(a0, ls, tk_sh);
             }
-        }
-        long sum = mine;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const long t = lk_shfl64(sum, (lane - o) & 63);
-            if (lane >= o) sum += t;
+            sum = lk_pa_scan(mine);
         }
         const uint64_t here = __ballot(before + sum > f0);
         if (here) {
@@ -276,14 +300,14 @@ lk_k_paged_attn(const LkPaArgs) {
             at.s.r0 = __builtin_amdgcn_readlane(ls.r0, src);
             at.s.n = __builtin_amdgcn_readlane(ls.n, src);
             at.s.len = __builtin_amdgcn_readlane(ls.len, src);
-            for (at.c = 0;; ++at.c) {                          // ends: rem is below the sequence's tiles
+            for (at.c = 0;; ++at.c) {                          // ends: rem is below the sequence's places
                 lk_pa_item(a0, at, tk_sh);
                 const long u = (long) (at.nt + a0.extra) * a0.nhg;
                 if (rem < u) break;
                 rem -= u;
             }
-            at.h = (int) (rem / (at.nt + a0.extra));
-            at.t = (int) (rem % (at.nt + a0.extra)) - a0.extra;  // below 0: in front of the first tile
+            for (at.h = 0; rem >= at.nt + a0.extra; ++at.h) rem -= at.nt + a0.extra;
+            at.t = (int) rem - a0.extra;                       // below 0: in front of the first tile
             break;
         }
         before += lk_uniform64(lk_shfl64(sum, 63));
@@ -722,7 +746,9 @@ lk_k_paged_attn(const LkPaArgs) {
             // the workgroups that the rest of the item falls to, this one counted
             const long end = f1 + (at.nt - t_end);              // behind the item's last tile
             const int qc = args().qc, m = at.s.n - at.c * qc;
-            cut = make_int4((int) ((end - 1) / share) - (int) blockIdx.x + 1, at.s.r0 + at.c * qc, m < qc ? m : qc, at.h);
+            const long last = end - 1 - f0;                     // its last place, counted from this workgroup's first
+            const int more = last >> 31 ? (int) (last / share) : (int) ((uint32_t) last / (uint32_t) share);
+            cut = make_int4(more + 1, at.s.r0 + at.c * qc, m < qc ? m : qc, at.h);
         }
         left -= extra;
         if (left > 0) lk_pa_next(args(), at, tk_sh);
