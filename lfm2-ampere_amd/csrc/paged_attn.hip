@@ -22,7 +22,6 @@
 // The sum of the weights comes from the same product (a row of ones), so weights and sum are
 // rounded alike.
 #include "lk_paged.h"
-#include <stdlib.h>
 
 #define LK_PA_TILEB 32768          // a tile: K rows, then V rows
 #define LK_PA_HEADROOM 8.0f        // the running max is raised when a score passes it by 2^8
@@ -370,6 +369,7 @@ lk_k_paged_attn(const LkPaArgs) {
     float slope[MOD ? CB : 1];
     int qpos[MOD ? CB : 1];
     int base = 0;                                               // keys below it are seen by all of the chunk's rows
+    bool busy = false;                                          // the wave has columns
     // column block cb: the token of the chunk, its row of the step, its query head; false: there is none
     auto column = [&](const LkPaC & a, int cb, int & i, int & row, int & head) -> bool {
         const int c = (qw * CB + cb) * 16 + lk_here(col), i0 = at.c * a.qc, m = at.s.n - i0 < a.qc ? at.s.n - i0 : a.qc;
@@ -388,10 +388,12 @@ lk_k_paged_attn(const LkPaArgs) {
         cap = a.cap;
         const int blk = (at.c * a.qc) & ~63, slots = a.width << a.page_sh;
         base = at.s.len + blk < slots ? at.s.len + blk : slots;
+        busy = false;
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) {
             int i, row, head;
             const bool live = column(a, cb, i, row, head);
+            busy |= __ballot(live) != 0;                        // wave-uniform
             if constexpr (MOD) {
                 slope[cb] = a.slopes ? a.slopes[head] * LK_LOG2E_F : 0.0f;
                 qpos[cb] = a.pos ? a.pos[row] : at.s.len + (row - at.s.r0);
@@ -727,7 +729,7 @@ lk_k_paged_attn(const LkPaArgs) {
             asm volatile("" ::: "memory");
             if (ft_left > 0) fetch_next();
             const int k0 = (at.t << tk_sh) + kw * kpw;
-            if (k0 < at.vis) {                                  // the wave's share may lie behind the last key
+            if (k0 < at.vis && busy) {                          // the wave's share may lie behind the last key
                 const unsigned char * kt = s_tile[slot] + ((kw * kpw) << rb_sh), * vt = kt + LK_PA_TILEB / 2;
                 const int n = k0 + kpw < at.vis ? kpw : at.vis - k0;
                 V8 kf[NB][KS];
@@ -933,18 +935,12 @@ static LkPaShape lk_pa_shape(const lk_pages * p, int type, int max_new) {
     s.hg_sh = 0;
     // few heads a group where the columns are many: what a cut item leaves behind is 16 KB a wave and more
     while ((2 << s.hg_sh) * qw <= nw && p->n_kv_heads % (2 << s.hg_sh) == 0 && (s.step == 16 || s.hg_sh < 1)) ++s.hg_sh;
-#ifdef LK_PA_EXTRA
-    if (s.step == 32 && getenv("LKH")) while (s.hg_sh > atoi(getenv("LKH"))) --s.hg_sh;
-#endif
     s.kw_sh = lk_log2(nw / qw) - s.hg_sh;
     int qc = s.cb * 16 * qw / g;
     if (qc > 64) qc = 64;
     if (qc < 1) qc = 1;
     s.qc = 1 << lk_log2(qc);
     s.extra = s.step == 32 ? 5 : 2;
-#ifdef LK_PA_EXTRA
-    s.extra = getenv("LKX") ? atoi(getenv("LKX")) : s.extra;
-#endif
     return s;
 }
 static int lk_pa_blocks(const LkPaShape & s) { return s.cb << (s.qw_sh + s.hg_sh); }

@@ -733,17 +733,26 @@ class PagedStep:
         self._work, self._own, self._streams = work, False, set()
 
     def _workspace(self, n: int, stream):
-        """The workspace, of at least n bytes, known to the allocator as used by the call's stream."""
+        """The workspace, of at least n bytes where it is the step's own; made on the stream of the call,
+        whose turn on the memory is then the next one."""
         if self._work is None or (self._own and self._work.numel() < n):
-            self._work = _torch.empty(n, dtype=_torch.uint8, device=self._keep[1].device)
-            self._own = True
-            self._streams = {_torch.cuda.current_stream(self._dev).cuda_stream}
-        if self._own and not (stream is None and _raw_stream is not None and _raw_stream(self._dev) in self._streams):
-            s = _torch.cuda.current_stream(self._dev) if stream is None else stream
-            if s.cuda_stream not in self._streams:
-                self._work.record_stream(s)
-                self._streams.add(s.cuda_stream)
+            if getattr(stream, "device_index", self._dev) != self._dev:
+                raise ValueError("lk_attn: the stream is one of another device than the tensors'")
+            with _torch.cuda.device(self._dev), _torch.cuda.stream(stream):       # None: the current stream
+                self._work = _torch.empty(n, dtype=_torch.uint8, device=self._keep[1].device)
+                self._own = True
+                self._streams = {_torch.cuda.current_stream(self._dev).cuda_stream}
         return self._work
+
+    def _tell(self, stream) -> None:
+        """Tells the allocator of a stream that uses the step's own workspace, so that a step dropped while
+        the stream has work left does not give the memory away."""
+        if stream is None and _raw_stream is not None and _raw_stream(self._dev) in self._streams:
+            return
+        s = _torch.cuda.current_stream(self._dev) if stream is None else stream
+        if s.cuda_stream not in self._streams:
+            self._work.record_stream(s)
+            self._streams.add(s.cuda_stream)
 
 
 class PagedCache:
@@ -820,6 +829,8 @@ class PagedCache:
                  self._scale if scale is None else scale, cap, ps, po, ldo, work.data_ptr(), work.numel())
         if rc:
             _check(rc, "lk_paged_attn")
+        if step._own:
+            step._tell(stream)
 
     def commit(self, step, path, count, new_lens, stream=None) -> None:
         """The accepted tokens of each sequence (places path int32 [sequences][most], strictly
