@@ -604,10 +604,11 @@ int lk_paged_append(const lk_pages * pages, const lk_step * step, int type, cons
  * and zeros for a row that sees nothing.  Keys and values a row does not see do not touch
  * it, infinities and NaN among them.
  * q, out rows of `type` as in lk_paged_append, n_heads heads side by side; scale > 0;
- * slopes fp32 [n_heads] or NULL.  Scores, softmax and sums are fp32.  For 16-bit rows the weights
- * enter the product with v rounded to the type, and so does their sum; for fp32 rows q and the
- * weights enter as two fp16 parts (22 bits).  Results do not depend on the run; the last bits
- * depend on how the batch's keys are divided among the workgroups.
+ * slopes fp32 [n_heads] or NULL.  Scores, softmax and sums are fp32.  The weights enter the product
+ * with v as two parts of the pools' type (what the first one's rounding leaves is the second),
+ * and so does q where the rows are fp32; for 16-bit rows of more than 32 (new token, query head) pairs a
+ * kv head, by max_new, as one part.  Sums of the weights are rounded alike.  Results do not depend on the
+ * run; the last bits depend on how the batch's keys are divided among the workgroups.
  * work: 16-byte aligned device memory of lk_paged_attn_work_bytes() (0 on bad arguments;
  * lk_last_error() says which); launches that share it must be ordered (one stream, or the
  * caller's events), and graphs that may run at once need two. */

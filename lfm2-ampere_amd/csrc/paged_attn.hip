@@ -85,7 +85,7 @@ struct LkPaArgs {
     int nhg, hg_sh, qw_sh, kw_sh;  // groups of 2^hg_sh kv heads; a workgroup's waves = heads x column groups x key shares
     int qc;                        // tokens a chunk, a power of two up to 64
     int extra;                     // places of the line an item takes in front of its tiles
-    float sc, scale, cap;          // sc = scale * log2(e)
+    float sc, scale, cap, inv_cap; // sc = scale * log2(e), inv_cap = 1 / cap
 };
 
 // Wave-uniform loads of the tables by the scalar unit: they are counted apart from the DMA in flight,
@@ -203,7 +203,8 @@ __device__ __forceinline__ float lk_pa_inverse(float l) {
 }
 
 // tanh of t: below 1/2 by its series (the difference of two numbers near 1 would lose what is
-// left), the first term left out below 2^-26 of the value; above by the exponential.
+// left), the first term left out below 2^-26 of the value; above by the exponential, with the hardware's
+// reciprocal (1 ulp): three half steps of the value, where an IEEE division costs ten instructions more.
 __device__ __forceinline__ float lk_tanh(float t) {
     const float u = fabsf(t), z = t * t;
     float p = 21844.0f / 6081075.0f;
@@ -214,13 +215,20 @@ __device__ __forceinline__ float lk_tanh(float t) {
     p = __builtin_fmaf(-p, z, 1.0f / 3.0f);
     const float small = __builtin_fmaf(-p * z, u, u);
     const float e = lk_exp2(u * (-2.0f * LK_LOG2E_F));
+#if defined(__HIP_DEVICE_COMPILE__)
+    const float large = (1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e);
+#else
     const float large = (1.0f - e) / (1.0f + e);
+#endif
     return copysignf(u < 0.5f ? small : large, t);
 }
 
-// D: head_dim.  RT: rows (LK_F32: q and the weights as two parts).  CT: pools.  CB: blocks of 16
+// D: head_dim.  RT: rows (LK_F32: q as two parts).  CT: pools.  CB: blocks of 16
 // columns a wave holds.  STEP: keys a wave takes at once, 32 by K = 32 products of both kinds, 16 by
 // K = 16 for P.V.  MOD: capped or biased scores.
+// The weights enter P.V as two parts of the pools' type, a second product for what the first part's rounding
+// leaves, where the kernel waits for memory (STEP 16: no slower, and the result is off by its own rounding
+// alone, bf16 1.7e-3 relative; one part 2.3e-3) and for fp32 rows; elsewhere as one part.
 template <int D, int RT, int CT, int CB, int STEP, bool MOD>
 __global__ void __launch_bounds__(64 * lk_pa_waves(D, STEP), STEP == 16 && D == 128 ? 1 : 2)
 lk_k_paged_attn(const LkPaArgs) {
@@ -237,7 +245,7 @@ lk_k_paged_attn(const LkPaArgs) {
     typedef typename M::V8 V8;
     typedef typename M::V4 V4;
     typedef typename LkElem<RT>::type RowT;
-    constexpr bool TWO = RT == LK_F32;
+    constexpr bool TWO = RT == LK_F32, TWOW = TWO || STEP == 16;
     constexpr int NW = lk_pa_waves(D, STEP), NBUF = lk_pa_bufs(STEP), NB = STEP / 16;
     constexpr int KS = D / 32, DB = D / 16, DC = D / 8;        // steps of q.k, blocks of output dims, 16-byte pieces of a head's row
     constexpr int NF = 16 / NW;                                // pieces of 1 KB a wave fetches of a tile's K, and of its V
@@ -381,11 +389,16 @@ lk_k_paged_attn(const LkPaArgs) {
         head = ((at.h << a.hg_sh) + hh) * a.g + (live ? h : 0);
         return live;
     };
-    float sc = 0.0f, cap = 0.0f;                                // scale (times log2(e) but for MOD), cap
+    float sc = 0.0f, cap = 0.0f, inv_cap = 0.0f;                // scale (times log2(e) but for MOD), cap
+    bool biased = false;
     auto begin = [&]() {
         const LkPaC & a = args();
         sc = MOD ? a.scale : a.sc;
-        cap = a.cap;
+        if constexpr (MOD) {
+            cap = a.cap;
+            inv_cap = a.inv_cap;
+            biased = a.slopes != nullptr;
+        }
         const int blk = (at.c * a.qc) & ~63, slots = a.width << a.page_sh;
         base = at.s.len + blk < slots ? at.s.len + blk : slots;
         busy = false;
@@ -472,14 +485,20 @@ lk_k_paged_attn(const LkPaArgs) {
     auto factor = [&](int cb) -> float { return TWO ? fac[cb] : sc; };
     // capped and biased scores in units of log2, of keys k0 .. k0 + 3 (k0: the lane's first)
     auto shaped = [&](lk_f4 & c, int cb, int k0) {
-        const int32_t * pos = args().pos;
+        c *= factor(cb);
+        if (cap > 0.0f) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            float x = c[r] * factor(cb);
-            if (cap > 0.0f) x = cap * lk_tanh(x / cap);
-            int kp = k0 + r;
-            if (pos && kp >= at.s.len && kp < at.vis) kp = pos[at.s.r0 + kp - at.s.len];
-            c[r] = __builtin_fmaf(slope[cb], (float) (kp - qpos[cb]), x * LK_LOG2E_F);
+            for (int r = 0; r < 4; ++r) c[r] = cap * lk_tanh(c[r] * inv_cap);
+        }
+        c *= LK_LOG2E_F;
+        if (biased) {
+            const int32_t * pos = args().pos;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                int kp = k0 + r;
+                if (pos && kp >= at.s.len && kp < at.vis) kp = pos[at.s.r0 + kp - at.s.len];
+                c[r] = __builtin_fmaf(slope[cb], (float) (kp - qpos[cb]), c[r]);
+            }
         }
     };
     // raises the running max of column block cb to cover a lane's largest score (units of log2)
@@ -495,13 +514,13 @@ lk_k_paged_attn(const LkPaArgs) {
             }
         }
     };
-    // weights of four scores, and (fp32 rows) what their rounding leaves
+    // weights of four scores, and what their rounding leaves
     auto weights = [&](const lk_f4 & c, int cb, V4 & ph, V4 & pl) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const float p = lk_exp2(MOD ? c[r] + mneg[cb] : __builtin_fmaf(c[r], factor(cb), mneg[cb]));
             ph[r] = (T) p;
-            if constexpr (TWO) pl[r] = (T) (p - (float) ph[r]);
+            if constexpr (TWOW) pl[r] = (T) (p - (float) ph[r]);
         }
     };
     auto top4 = [&](const lk_f4 & c) -> float { return fmaxf(fmaxf(c[0], c[1]), fmaxf(c[2], c[3])); };
@@ -520,7 +539,7 @@ lk_k_paged_attn(const LkPaArgs) {
     // STEP keys, the first of them key0, kf their K rows; `more`: the rows of the STEP keys behind are
     // asked for.  From `base` on there are keys that only some of the rows see.
     auto step = [&](const unsigned char * kt, const unsigned char * vt, int key0, V8 (&kf)[NB][KS], bool more) {
-        V4 ph[CB][NB], pl[TWO ? CB : 1][NB], vf[DB][NB];
+        V4 ph[CB][NB], pl[TWOW ? CB : 1][NB], vf[DB][NB];
         lk_f4 c[CB][NB];
         const bool some = key0 + STEP > base;                   // wave-uniform
 #pragma unroll
@@ -538,6 +557,9 @@ lk_k_paged_attn(const LkPaArgs) {
 #pragma unroll
                 for (int n = 0; n < NB; ++n) shaped(c[cb][n], cb, key0 + 16 * n + 4 * g);
         }
+        // the softmax first: of the two waves of a SIMD one then multiplies while the other forms weights (2 x 4096 new
+        // tokens 210 -> 200 us; no other order of the two parts' instructions within a wave gained anything)
+        if constexpr (STEP == 32) __builtin_amdgcn_s_setprio(1);
         bool odd = false;                                       // an infinity or NaN among the values
         if (some) {
 #pragma unroll
@@ -579,14 +601,14 @@ lk_k_paged_attn(const LkPaArgs) {
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) {
 #pragma unroll
-            for (int n = 0; n < NB; ++n) weights(c[cb][n], cb, ph[cb][n], pl[TWO ? cb : 0][n]);
+            for (int n = 0; n < NB; ++n) weights(c[cb][n], cb, ph[cb][n], pl[TWOW ? cb : 0][n]);
             auto product = [&](const V4 (&v)[NB], lk_f4 o) -> lk_f4 {
                 if constexpr (NB == 2) {
                     o = M::k32(join(v[0], v[1]), join(ph[cb][0], ph[cb][1]), o);
-                    if constexpr (TWO) o = M::k32(join(v[0], v[1]), join(pl[cb][0], pl[cb][1]), o);
+                    if constexpr (TWOW) o = M::k32(join(v[0], v[1]), join(pl[cb][0], pl[cb][1]), o);
                 } else {
                     o = M::k16(v[0], ph[cb][0], o);
-                    if constexpr (TWO) o = M::k16(v[0], pl[cb][0], o);
+                    if constexpr (TWOW) o = M::k16(v[0], pl[cb][0], o);
                 }
                 return o;
             };
@@ -597,6 +619,7 @@ lk_k_paged_attn(const LkPaArgs) {
 #pragma unroll
             for (int db = 0; db < DB; ++db) acc[cb][db] = product(vf[db], acc[cb][db]);
         }
+        if constexpr (STEP == 32) __builtin_amdgcn_s_setprio(0);
         if (odd) {
             // one key after the other, and only the columns that see it
 #pragma unroll
@@ -863,22 +886,33 @@ lk_k_paged_spread(const LkPaArgs a, int cb_n, int wgs) {
         const LkPaBlock B(a, it, blk, cb_n);
         if (B.live == 0) continue;                             // the same for every thread
         auto piece = [&](int k) -> size_t { return (size_t) (2 * (w0 + k) + (k == 0)) * nblk + blk; };
-        float2 ml[LK_PA_MAX_WGS * 16 / NT];                    // of the thread's (piece, column) pairs
-        float m = -LK_PA_NONE, l = 0.0f;
+        // all that is needed is asked for at once: the thread's (max, sum) pairs, and its rows of up to 8 pieces
+        constexpr int NP = LK_PA_MAX_WGS * 16 / NT, NR = 8;
+        const int e_sh = B.live > 8 ? 6 : B.live > 4 ? 5 : 4, e = tid & ((1 << e_sh) - 1), p0 = tid >> e_sh, pp = NT >> e_sh;
+        auto rows = [&](int k) -> lk_f4 { return ((const lk_f4 *) a.acc)[(piece(k) * DB + db) * 64 + e]; };
+        float2 ml[NP];
+        lk_f4 x4[NR];
 #pragma unroll
-        for (int j = 0; j < LK_PA_MAX_WGS * 16 / NT; ++j) {
+        for (int j = 0; j < NP; ++j) {
             const int k = (tid >> 4) + j * (NT / 16);
             ml[j] = make_float2(-LK_PA_NONE, 0.0f);
             if (k < it.x && col < B.live) ml[j] = a.ml[piece(k) * 16 + col];
-            m = fmaxf(m, ml[j].x);
         }
+#pragma unroll
+        for (int j = 0; j < NR; ++j) {
+            x4[j] = (lk_f4){ 0.f, 0.f, 0.f, 0.f };
+            if (p0 + j * pp < it.x && e < 4 * B.live) x4[j] = rows(p0 + j * pp);
+        }
+        float m = -LK_PA_NONE, l = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NP; ++j) m = fmaxf(m, ml[j].x);
         m = lk_xrow_max(m);
         if (lane < 16) s_r[0][v][col] = m;
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < NV; ++k) m = fmaxf(m, s_r[0][k][col]);
 #pragma unroll
-        for (int j = 0; j < LK_PA_MAX_WGS * 16 / NT; ++j) {
+        for (int j = 0; j < NP; ++j) {
             const int k = (tid >> 4) + j * (NT / 16);
             const float f = lk_exp2(ml[j].x - m);
             if (k < it.x) s_w[k][col] = f;
@@ -887,12 +921,13 @@ lk_k_paged_spread(const LkPaArgs a, int cb_n, int wgs) {
         l = lk_xrow_sum(l);
         if (lane < 16) s_r[1][v][col] = l;
         __syncthreads();
-        const int e_sh = B.live > 8 ? 6 : B.live > 4 ? 5 : 4, e = tid & ((1 << e_sh) - 1), pp = NT >> e_sh;
         lk_f4 o = { 0.f, 0.f, 0.f, 0.f };
         if (e < 4 * B.live) {
+#pragma unroll
+            for (int j = 0; j < NR; ++j)
+                if (p0 + j * pp < it.x) o += x4[j] * s_w[p0 + j * pp][e >> 2];
 #pragma unroll 8
-            for (int k = tid >> e_sh; k < it.x; k += pp)
-                o += ((const lk_f4 *) a.acc)[(piece(k) * DB + db) * 64 + e] * s_w[k][e >> 2];
+            for (int k = p0 + NR * pp; k < it.x; k += pp) o += rows(k) * s_w[k][e >> 2];
         }
         s_o[tid] = o;
         __syncthreads();
@@ -1032,7 +1067,7 @@ extern "C" int lk_paged_attn(const lk_pages * pages, const lk_step * step, int t
     const LkPaArgs a = { q, out, (const char *) pages->k, (const char *) pages->v, zeros, step->first, step->lens, step->table, step->pos,
                          step->mask, slopes, acc, ml, (int4 *) (ml + blocks * 16), ldq, ldo, step->n_seqs, step->rows, step->ldt,
                          step->width, lk_log2(pages->page), pages->n_pages, hq, pages->n_kv_heads, g, nhg, s.hg_sh, s.qw_sh, s.kw_sh, s.qc, s.extra,
-                         scale * LK_LOG2E_F, scale, cap };
+                         scale * LK_LOG2E_F, scale, cap, 1.0f / cap };
     const hipStream_t st = lk_stream(stream);
     const bool mod = cap > 0.0f || slopes;
     if (d == 64) {
