@@ -801,7 +801,7 @@ struct LkPaBlock {
 };
 
 // Many items, cut into few pieces each: workgroup (x, blk) joins block blk of the item that begins in
-// workgroup x, each wave some of its dims, four pieces asked for at once.
+// workgroup x, each wave some of its dims.
 template <int D, int RT>
 __global__ void __launch_bounds__(256)
 lk_k_paged_join(const LkPaArgs a, int cb_n) {
@@ -816,28 +816,34 @@ lk_k_paged_join(const LkPaArgs a, int cb_n) {
     lk_f4 o[W];
 #pragma unroll
     for (int i = 0; i < W; ++i) o[i] = (lk_f4){ 0.f, 0.f, 0.f, 0.f };
-    for (int k0 = 0; k0 < it.x; k0 += 4) {
-        float2 ml[4];
-        lk_f4 x[4][W];
+    constexpr int NP = 8 / W;                                  // pieces asked for at once
+    for (int k0 = 0; k0 < it.x; k0 += NP) {
+        float2 ml[NP];
+        lk_f4 x[NP][W];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int k = k0 + j < it.x ? k0 + j : k0;
-            const size_t p = (size_t) (2 * (blockIdx.x + k) + (k == 0)) * nblk + blk;
-            ml[j] = a.ml[p * 16 + (lane >> 2)];
+        for (int j = 0; j < NP; ++j) {
+            ml[j] = make_float2(-LK_PA_NONE, 0.0f);
 #pragma unroll
-            for (int i = 0; i < W; ++i) x[j][i] = ((const lk_f4 *) a.acc)[(p * DB + db0 + i) * 64 + lane];
+            for (int i = 0; i < W; ++i) x[j][i] = (lk_f4){ 0.f, 0.f, 0.f, 0.f };
+            const int k = k0 + j;
+            if (k < it.x) {                                    // the same for every thread
+                const size_t p = (size_t) (2 * (blockIdx.x + k) + (k == 0)) * nblk + blk;
+                ml[j] = a.ml[p * 16 + (lane >> 2)];
+#pragma unroll
+                for (int i = 0; i < W; ++i) x[j][i] = ((const lk_f4 *) a.acc)[(p * DB + db0 + i) * 64 + lane];
+            }
         }
         float mx = m;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) mx = fmaxf(mx, ml[j].x);
+        for (int j = 0; j < NP; ++j) mx = fmaxf(mx, ml[j].x);
         const float f = lk_exp2(m - mx);
         m = mx;
         l *= f;
 #pragma unroll
         for (int i = 0; i < W; ++i) o[i] *= f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float fj = k0 + j < it.x ? lk_exp2(ml[j].x - mx) : 0.0f;
+        for (int j = 0; j < NP; ++j) {
+            const float fj = lk_exp2(ml[j].x - mx);
             l = __builtin_fmaf(ml[j].y, fj, l);
 #pragma unroll
             for (int i = 0; i < W; ++i) o[i] += x[j][i] * fj;
