@@ -582,7 +582,8 @@ typedef struct lk_step {
  *   LK_ROPE_HALVES: the pair is (y_i, y_{i + rot/2}), LK_ROPE_PAIRS: (y_2i, y_{2i+1});
  *   (u, v) -> (u cos a - v sin a, u sin a + v cos a); values from rot on are not rotated
  * in fp32, rounded once.  freq fp32 [rot / 2], rot a multiple of 16 up to head_dim, or freq NULL
- * with rot 0: no rotation.  |a_i| below 2^31.  Squares are summed in fp32.
+ * with rot 0: no rotation.  |a_i| below 2^31.  Squares are summed in fp32: a head whose sum overflows
+ * is NaN, and so is one of zeros with eps 0.
  * q, k, v, qo are rows of `type` (LK_F32 or LK_F16 with fp16 pools, LK_BF16 with bf16 pools) of
  * n_heads or n_kv_heads heads side by side, ld* elements apart (parts of one wide row as
  * well); q and qo may be NULL (keys and values only), and qo may be q.  Rows need the
@@ -603,7 +604,7 @@ int lk_paged_append(const lk_pages * pages, const lk_step * step, int type, cons
  *   the key - position of the row), a cached key's position being its slot;  out = softmax(x) . v
  * and zeros for a row that sees nothing.  Keys and values a row does not see do not touch
  * it, infinities and NaN among them.
- * q, out rows of `type` as in lk_paged_append, n_heads heads side by side; scale > 0;
+ * q, out rows of `type` as in lk_paged_append, n_heads heads side by side; scale > 0, cap 0 or at least 2^-100;
  * slopes fp32 [n_heads] or NULL.  Scores, softmax and sums are fp32.  The weights enter the product
  * with v as two parts of the pools' type (what the first one's rounding leaves is the second),
  * and so does q where the rows are fp32; for 16-bit rows of more than 32 (new token, query head) pairs a

@@ -73,7 +73,6 @@ struct LkPaArgs {
     const void * q;
     void * out;
     const char * kp, * vp;
-    const char * zeros;            // 1 KB of zeros: what keys that no row sees are fetched from
     const int32_t * first, * lens, * table, * pos;
     const uint64_t * mask;
     const float * slopes;
@@ -87,6 +86,9 @@ struct LkPaArgs {
     int extra;                     // places of the line an item takes in front of its tiles
     float sc, scale, cap, inv_cap; // sc = scale * log2(e), inv_cap = 1 / cap
 };
+
+// What keys that no row sees are fetched from; never written.
+static __device__ __align__(1024) char lk_pa_zeros[1024];
 
 // Wave-uniform loads of the tables by the scalar unit: they are counted apart from the DMA in flight,
 // which a vector load would be waited for together with.
@@ -361,9 +363,11 @@ lk_k_paged_attn(const LkPaArgs) {
                     lk_dma16c_so(kp + off, ko, lk);
                     lk_dma16c_so(vp + off, vo, lv);
                 }
-            } else {                                           // rows that nobody sees are zeros
+            } else {
+                // rows that nobody sees are zeros: what lies there must not meet weights of 0 as an infinity or NaN
+                // (zeros written to LDS instead cost 4 to 15%: the branch over the lanes)
                 const bool live = ok && p0 + frow < p.vis;
-                const char * zs = args().zeros + 16 * ln;
+                const char * zs = lk_pa_zeros + 16 * ln;
                 lk_dma16c(live ? kp + off + ko : zs, lk);
                 lk_dma16c(live ? vp + off + vo : zs, lv);
             }
@@ -1008,31 +1012,6 @@ static void lk_pa_join(const LkPaArgs & a, long items, int nblk, const LkPaShape
         hipLaunchKernelGGL((lk_k_paged_join<D, RT>), dim3(wgs - 1, nblk), dim3(256), 0, st, a, s.cb);
 }
 
-static __device__ __align__(1024) char lk_pa_zeros[1024];      // never written
-
-// The device address of the zeros, looked up once a device.
-static const char * lk_pa_zeros_at(int & err) {
-    static const char * at[LK_MAX_DEVICES];
-    int dev = 0;
-    hipError_t e = hipGetDevice(&dev);
-    if (e != hipSuccess || dev < 0 || dev >= LK_MAX_DEVICES) {
-        err = lk_fail(e != hipSuccess ? (int) e : (int) hipErrorInvalidDevice, "lk_paged_attn: no usable current device");
-        return nullptr;
-    }
-    const char * p = __atomic_load_n(&at[dev], __ATOMIC_RELAXED);
-    if (!p) {
-        void * q = nullptr;
-        e = hipGetSymbolAddress(&q, HIP_SYMBOL(lk_pa_zeros));
-        if (e != hipSuccess || !q) {
-            err = lk_fail(e != hipSuccess ? (int) e : (int) hipErrorInvalidSymbol, "lk_paged_attn: zeros: %s", hipGetErrorString(e));
-            return nullptr;
-        }
-        p = (const char *) q;
-        __atomic_store_n(&at[dev], p, __ATOMIC_RELAXED);       // every thread stores the same
-    }
-    return p;
-}
-
 extern "C" size_t lk_paged_attn_work_bytes(const lk_pages * pages, int type, int max_new) {
     static const char * const W = "lk_paged_attn_work_bytes";
     if (lk_paged_check_pages(W, pages) || lk_paged_check_type(W, pages, type)) return 0;
@@ -1051,8 +1030,9 @@ extern "C" int lk_paged_attn(const lk_pages * pages, const lk_step * step, int t
     if (const int e = lk_paged_check(W, pages, step)) return e;
     if (const int e = lk_paged_check_type(W, pages, type)) return e;
     const int d = pages->head_dim, hq = pages->n_heads;
-    if (!(scale > 0.0f) || !(scale < __builtin_inff()) || !(cap >= 0.0f) || !(cap < __builtin_inff()))
-        return lk_fail(hipErrorInvalidValue, "%s: scale %g, cap %g", W, (double) scale, (double) cap);
+    if (!(scale > 0.0f) || !(scale < __builtin_inff()) || !(cap == 0.0f || cap >= 0x1p-100f) ||
+        !(cap < __builtin_inff()))
+        return lk_fail(hipErrorInvalidValue, "%s: scale %g, cap %g (0: none)", W, (double) scale, (double) cap);
     if (step->rows == 0 || step->n_seqs == 0) return 0;
     if (!q || !out || !work) return lk_fail(hipErrorInvalidValue, "%s: null pointer argument", W);
     if (ldq < hq * d || ldo < hq * d)
@@ -1062,15 +1042,12 @@ extern "C" int lk_paged_attn(const lk_pages * pages, const lk_step * step, int t
         return lk_fail(hipErrorInvalidValue, "%s: misaligned argument (rows by their element, slopes 4 B, work 16 B)", W);
     const size_t need = lk_paged_attn_work_bytes(pages, type, step->max_new);
     if (work_bytes < need) return lk_fail(hipErrorInvalidValue, "%s: workspace of %zu bytes, %zu needed", W, work_bytes, need);
-    int err = 0;
-    const char * zeros = lk_pa_zeros_at(err);
-    if (!zeros) return err;
     const LkPaShape s = lk_pa_shape(pages, type, step->max_new);
     const int nblk = lk_pa_blocks(s), g = hq / pages->n_kv_heads, nhg = pages->n_kv_heads >> s.hg_sh;
     const size_t blocks = (size_t) 2 * lk_pa_wgs(s.step) * nblk;
     float * acc = (float *) work;
     float2 * ml = (float2 *) (acc + blocks * 16 * d);
-    const LkPaArgs a = { q, out, (const char *) pages->k, (const char *) pages->v, zeros, step->first, step->lens, step->table, step->pos,
+    const LkPaArgs a = { q, out, (const char *) pages->k, (const char *) pages->v, step->first, step->lens, step->table, step->pos,
                          step->mask, slopes, acc, ml, (int4 *) (ml + blocks * 16), ldq, ldo, step->n_seqs, step->rows, step->ldt,
                          step->width, lk_log2(pages->page), pages->n_pages, hq, pages->n_kv_heads, g, nhg, s.hg_sh, s.qw_sh, s.kw_sh, s.qc, s.extra,
                          scale * LK_LOG2E_F, scale, cap, 1.0f / cap };

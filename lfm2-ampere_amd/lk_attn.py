@@ -730,7 +730,7 @@ class PagedStep:
         self._ref = ctypes.addressof(self._desc)
         self._keep = (first, lens, table, pos, mask)
         self._dev, self.n_seqs, self.rows, self.max_new = dev, B, int(rows), int(max_new)
-        self._work, self._own, self._streams = work, False, set()
+        self._work, self._own, self._streams, self._old = work, False, set(), []
 
     def _workspace(self, n: int, stream):
         """The workspace, of at least n bytes where it is the step's own; made on the stream of the call,
@@ -739,6 +739,7 @@ class PagedStep:
             if getattr(stream, "device_index", self._dev) != self._dev:
                 raise ValueError("lk_attn: the stream is one of another device than the tensors'")
             with _torch.cuda.device(self._dev), _torch.cuda.stream(stream):       # None: the current stream
+                self._old.append(self._work)             # a captured call may still have it
                 self._work = _torch.empty(n, dtype=_torch.uint8, device=self._keep[1].device)
                 self._own = True
                 self._streams = {_torch.cuda.current_stream(self._dev).cuda_stream}

@@ -112,6 +112,13 @@ def test_append_rows_without_queries_and_in_place(lk):
     _check(lk, 402, b, 8, 2, 128, "f32", inplace=True)
 
 
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+def test_append_rows_at_any_alignment(lk, t):
+    """Rows an odd number of elements apart."""
+    _check(lk, 450, Batch(15, [10, 3], [4, 3000], 16, pad=1), 5, 1, 64, t, extra=7)
+    _check(lk, 451, Batch(15, [10, 3], [4, 3], 16, pad=1), 5, 1, 128, t, extra=1)
+
+
 def test_append_far_and_given_positions(lk):
     """Angles in 64 bits: positions far past 2^24, negative ones, and not those of the slots."""
     b = Batch(8, [10, 20], [4, 30], 16)

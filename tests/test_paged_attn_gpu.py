@@ -304,6 +304,48 @@ def test_long_contexts(lk, lens, news, hq, hkv, d, t):
     _check(lk, 51, b, hq, hkv, d, t, max_new=max(news))
 
 
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+def test_rows_at_any_alignment_and_wide_tables(lk, t):
+    """Rows that begin at odd elements and lie an odd number apart; a table that is a part of a wider one."""
+    b = Batch(55, [100, 33], [1, 20], 16, pad=2)
+    dt = TYPES[t]
+    k, v = pools(56, b, 2, 64, t)
+    q = _q(57, b.rows, 512, dt)
+    i = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    wide = torch.full((2, b.width + 5), -1, dtype=torch.int32, device="cuda")
+    wide[:, 2:b.width + 2] = i(b.table)
+    for hint in (1, 64):
+        step = lk.PagedStep(i(b.first), i(b.lens), wide[:, 2:b.width + 2], b.rows, max_new=hint)
+        qd = torch.zeros(b.rows, 517, dtype=dt, device="cuda")[:, 1:513]
+        qd.copy_(q)
+        out = torch.full((b.rows, 519), 77.0, dtype=dt, device="cuda")
+        note(f"odd rows {t}, hint {hint}")
+        lk.PagedCache(k.cuda(), v.cuda(), 8).attend(step, qd, out[:, 3:515])
+        torch.cuda.synchronize()
+        want, tol = _want(b, q, k, v, 8, t, None, None, 0.125, 0.0, None)
+        got = out.cpu().double()
+        assert bool(((got[:21, 3:515].view(21, 8, 64) - want).abs() <= tol).all())
+        got[:21, 3:515] = 77
+        assert bool((got == 77).all())
+
+
+def test_a_workspace_that_grows(lk):
+    """One step with caches of different needs: the larger workspace replaces the smaller, whose memory
+    a captured call may still use."""
+    b = Batch(58, [700, 33], [1, 1], 16)
+    step = b.step(lk, max_new=1)
+    outs = []
+    for hq, hkv, d in ((8, 8, 64), (64, 8, 64), (8, 8, 64)):
+        k, v = (x.cuda() for x in pools(59, b, hkv, d, "f16"))
+        q = _q(60, 2, hq * d, torch.float16).cuda()
+        out = torch.empty_like(q)
+        note(f"workspace of {hq} heads")
+        lk.PagedCache(k, v, hq).attend(step, q, out)
+        outs.append(out)
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], outs[2]) and len(step._old) <= 2
+
+
 def test_runs_are_the_same_bits(lk):
     """No atomics: every call gives the same bits, whatever the workspace held before."""
     b = Batch(60, [3000, 100, 700], [1, 30, 5], 16)

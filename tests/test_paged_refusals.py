@@ -76,7 +76,7 @@ def test_attn_c_refusals(lk_host):
         return lib.lk_paged_attn(*a.values())
     _descriptions(lk, rc, b"lk_paged_attn")
     inf, nan = float("inf"), float("nan")
-    for bad in (dict(type=2), dict(type=3), dict(scale=F(0.0)), dict(scale=F(-1.0)), dict(scale=F(inf)), dict(scale=F(nan)), dict(cap=F(-1.0)),
+    for bad in (dict(type=2), dict(type=3), dict(scale=F(0.0)), dict(scale=F(-1.0)), dict(scale=F(inf)), dict(scale=F(nan)), dict(cap=F(-1.0)), dict(cap=F(1e-31)),
                 dict(cap=F(inf)), dict(cap=F(nan)), dict(q=None), dict(out=None), dict(work=None), dict(work_bytes=need - 1),
                 dict(work=ctypes.c_void_p(0x1008)), dict(ldq=2047), dict(ldo=2047), dict(q=O), dict(out=O),
                 dict(slopes=ctypes.c_void_p(0x1002)), dict(type=0, q=ctypes.c_void_p(0x1002)),
