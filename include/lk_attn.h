@@ -607,7 +607,7 @@ int lk_paged_append(const lk_pages * pages, const lk_step * step, int type, cons
  * q, out rows of `type` as in lk_paged_append, n_heads heads side by side; scale > 0, cap 0 or at least 2^-100;
  * slopes fp32 [n_heads] or NULL.  Scores, softmax and sums are fp32.  The weights enter the product
  * with v as two parts of the pools' type (what the first one's rounding leaves is the second),
- * and so does q where the rows are fp32; for 16-bit rows of more than 32 (new token, query head) pairs a
+ * and so does q where the rows are fp32; for 16-bit rows of more than 16 (new token, query head) pairs a
  * kv head, by max_new, as one part.  Sums of the weights are rounded alike.  Results do not depend on the
  * run; the last bits depend on how the batch's keys are divided among the workgroups.
  * work: 16-byte aligned device memory of lk_paged_attn_work_bytes() (0 on bad arguments;

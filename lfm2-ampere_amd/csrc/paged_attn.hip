@@ -5,7 +5,7 @@
 //     out_i = sum_j exp(x_ij) v_j / sum_j exp(x_ij)      over the j that i sees
 //
 // The work is one line of key tiles: per sequence, chunk of its new tokens and group of kv
-// heads ("item") the tiles of the keys that the chunk sees.  Each of LK_PA_MAX_WGS workgroups
+// heads ("item") the tiles of the keys that the chunk sees.  Each of a fixed number of workgroups
 // takes an equal run of that line, whatever the lengths are: it finds its place from the
 // lengths on the device, walks on from item to item, and its DMA runs ahead over the
 // borders.  An item inside one run is finished there; one that is cut leaves partials
@@ -27,9 +27,13 @@
 #define LK_PA_HEADROOM 8.0f        // the running max is raised when a score passes it by 2^8
 #define LK_PA_NONE  3.0e38f        // minus the running max of no score: 2^(any score in sight - max) is 0 against it
 
-// Two kinds of workgroup.  For up to 32 columns a kv head (STEP 16) the cache's bytes bound it: one workgroup a
-// CU, a ring of four tiles, so that 96 KB are on their way.  For more (STEP 32) the products and exponentials
-// do: two workgroups a CU of one wave a SIMD each, which wait at barriers of their own, and two tiles.
+// Two kinds of workgroup.  For up to 16 columns a kv head (STEP 16) the cache's bytes bound it: one workgroup a
+// CU, a ring of four tiles, so that 96 KB are on their way (64 sequences of 8192, 32 / 8 heads of 64, bf16: 214 us,
+// 6.4 TB/s; one of 131072 in 42 us, 6.4 TB/s, the pieces' sum 6 more).  For more (STEP 32) the products and
+// exponentials do: two workgroups a CU of one wave a SIMD each, which wait at barriers of their own, and two tiles
+// (2 x 4096 new tokens 197 us, 592 TFLOP/s of products; at K = 32 a tile's 16 x 16 products and its exponentials
+// take 139 us of issue, one behind the other on a SIMD).  Between the two, 8 tokens of 4 heads a kv head, STEP 32
+// too: one sequence at 30000 21.7 us against 29.9, 16 at 1000 13.9 against 18.9.
 __host__ __device__ constexpr int lk_pa_waves(int d, int step) { return step == 16 && d == 64 ? 8 : 4; }
 __host__ __device__ constexpr int lk_pa_bufs(int step) { return step == 16 ? 4 : 2; }
 __host__ __device__ constexpr int lk_pa_wgs(int step) { return step == 16 ? 256 : 512; }
@@ -80,7 +84,7 @@ struct LkPaArgs {
     float2 * ml;                   // and their (max, sum): [..][..][16]
     int4 * cut;                    // per workgroup the cut item that begins in it: (pieces, first row, rows, kv head group)
     int ldq, ldo, n_seqs, rows, ldt, width, page_sh, n_pages;
-    int hq, hkv, g;                // g = query heads a kv head
+    int hkv, g;                    // g = query heads a kv head
     int nhg, hg_sh, qw_sh, kw_sh;  // groups of 2^hg_sh kv heads; a workgroup's waves = heads x column groups x key shares
     int qc;                        // tokens a chunk, a power of two up to 64
     int extra;                     // places of the line an item takes in front of its tiles
@@ -230,7 +234,7 @@ __device__ __forceinline__ float lk_tanh(float t) {
 // K = 16 for P.V.  MOD: capped or biased scores.
 // The weights enter P.V as two parts of the pools' type, a second product for what the first part's rounding
 // leaves, where the kernel waits for memory (STEP 16: no slower, and the result is off by its own rounding
-// alone, bf16 1.7e-3 relative; one part 2.3e-3) and for fp32 rows; elsewhere as one part.
+// alone: bf16 1.7e-3 relative; one part 2.3e-3) and for fp32 rows; elsewhere as one part.
 template <int D, int RT, int CT, int CB, int STEP, bool MOD>
 __global__ void __launch_bounds__(64 * lk_pa_waves(D, STEP), STEP == 16 && D == 128 ? 1 : 2)
 lk_k_paged_attn(const LkPaArgs) {
@@ -356,7 +360,7 @@ lk_k_paged_attn(const LkPaArgs) {
             const uint32_t ko = frow * row_bytes + 16 * (part ^ swk(key)), vo = frow * row_bytes + 16 * (part ^ swv(key));
             const uint32_t lk = base + piece * 1024, lv = lk + LK_PA_TILEB / 2;
             if (ok && p0 + rpp <= p.vis) {
-                if constexpr (STEP == 16) {                    // up to 64 columns a head: few others read the tile
+                if constexpr (STEP == 16) {                    // up to 16 columns a head: few others read the tile
                     lk_dma16_so(kp + off, ko, lk);
                     lk_dma16_so(vp + off, vo, lv);
                 } else {
@@ -805,7 +809,9 @@ struct LkPaBlock {
 };
 
 // Many items, cut into few pieces each: workgroup (x, blk) joins block blk of the item that begins in
-// workgroup x, each wave some of its dims.
+// workgroup x, each wave some of its dims.  A load of each piece is all it does: eight are asked for at once, so
+// that their latencies overlap (in place of two: 2 x 4096 new tokens 222 -> 210 us as a whole, 19 sequences of up
+// to 5003 21.5 -> 19.5).  Of 2 x 4096 new tokens it takes 11.7 us for at most 64 MB, 5.5 TB/s.
 template <int D, int RT>
 __global__ void __launch_bounds__(256)
 lk_k_paged_join(const LkPaArgs a, int cb_n) {
@@ -859,7 +865,9 @@ lk_k_paged_join(const LkPaArgs a, int cb_n) {
 
 // Few items, cut into many pieces: workgroup (x, y) joins 16 dims of a block of the cut items number x,
 // x + gridDim.x, ..  All pieces' (max, sum) first give their weights; then the threads are divided over the
-// block's live values and as many pieces at once as fit, and their sums are added in order.
+// block's live values and as many pieces at once as fit, and their sums are added in order.  Latency bounds it: the
+// list of cut items, one round of loads, two barriers of the weights, three of the sums (256 pieces of one token,
+// 32 heads of 64: 5.5 us).
 template <int D, int RT>
 __global__ void __launch_bounds__(1024)
 lk_k_paged_spread(const LkPaArgs a, int cb_n, int wgs) {
@@ -964,15 +972,26 @@ lk_k_paged_spread(const LkPaArgs a, int cb_n, int wgs) {
 // ---- host ---------------------------------------------------------------------------------------
 // How a workgroup's waves divide a tile, for chunks of `want` tokens of g query heads a kv head.
 struct LkPaShape { int cb, step, hg_sh, qw_sh, kw_sh, qc, extra; };
-// Column blocks a wave of the STEP 32 kernels holds: as many as its registers take.
-constexpr int lk_pa_cb32(int d, int type) { return (d == 64 ? 4 : 2) / (type == LK_F32 ? 2 : 1); }
+// Column blocks a wave of the STEP 32 kernels holds, its columns being spread over up to four waves first: with
+// more than one chunk a sequence (max_new above 64) as many as the registers take, so that a tile is read from
+// LDS once for all of them; for up to 64 rows, whose items are cut into many pieces, one or two, since what a
+// workgroup leaves behind grows with its columns; one for chunks of four blocks in all until there are enough
+// of them to go round.  Measured, us, 32 / 8 heads of 64 (1, 2, 4 blocks):
+//   one tree of 16 at 2000      12.4  15.0  19.3     four of 24 at 2000            17.9  25.5
+//   one of 16 at 32768          25.9  28.7  32.8     one of 64 at 8000             25.4  40.0
+//   one of 16 at 131072         57.2  56.1  59.9     13 of up to 64 at 4096        47.0  48.9
+//   2 x 4096 new tokens                245  200      one of 64 at 131072          125   120
+// 16 / 16 heads of 64 (1, 4): 5 x 500 new tokens behind 500 31.0, 37.1; 2 x 4096 behind 4096 395, 351.
+constexpr int lk_pa_cb32(int d, int type, int max_new, int nb) {
+    return (nb <= 4 && max_new < 1024) || (d == 128 && type == LK_F32) ? 1 : d == 64 && type != LK_F32 && max_new > 64 ? 4 : 2;
+}
 static LkPaShape lk_pa_shape(const lk_pages * p, int type, int max_new) {
     const int g = p->n_heads / p->n_kv_heads, d = p->head_dim;
     const int want = max_new < 1 ? 1 : max_new > 64 ? 64 : max_new;
     LkPaShape s;
     const int nb = (want * g + 15) / 16;                       // blocks of columns
-    s.step = nb > 2 ? 32 : 16;
-    s.cb = nb > 2 ? lk_pa_cb32(d, type) : nb;
+    s.step = nb > 1 ? 32 : 16;
+    s.cb = nb > 1 ? lk_pa_cb32(d, type, max_new, nb) : 1;
     const int nw = lk_pa_waves(d, s.step);
     s.qw_sh = s.step == 32 && d == 128 ? 1 : 0;                // (a wave's share of a tile is 16 * 2^qw_sh keys and more)
     while ((s.cb << s.qw_sh) < nb && (1 << s.qw_sh) < nw) ++s.qw_sh;
@@ -998,13 +1017,23 @@ static void lk_pa_run(const LkPaArgs & a, bool mod, hipStream_t st) {
 }
 template <int D, int RT, int CT>
 static void lk_pa_launch(const LkPaShape & s, const LkPaArgs & a, bool mod, hipStream_t st) {
-    if (s.step == 32)    lk_pa_run<D, RT, CT, lk_pa_cb32(D, RT), 32>(a, mod, st);
-    else if (s.cb == 1)  lk_pa_run<D, RT, CT, 1, 16>(a, mod, st);
-    else                 lk_pa_run<D, RT, CT, 2, 16>(a, mod, st);
+    if (s.step == 32) {
+        if (s.cb == 1) lk_pa_run<D, RT, CT, 1, 32>(a, mod, st);
+        if constexpr (D == 64 || RT != LK_F32) {
+            if (s.cb == 2) lk_pa_run<D, RT, CT, 2, 32>(a, mod, st);
+        }
+        if constexpr (D == 64 && RT != LK_F32) {
+            if (s.cb == 4) lk_pa_run<D, RT, CT, 4, 32>(a, mod, st);
+        }
+        return;
+    }
+    lk_pa_run<D, RT, CT, 1, 16>(a, mod, st);
 }
 
 template <int D, int RT>
 static void lk_pa_join(const LkPaArgs & a, long items, int nblk, const LkPaShape & s, hipStream_t st) {
+    // attention and its join, us, spread and join: one token at 131072 51, 78; one at 4096 13.0, 26.8; a tree of 16
+    // at 32768 25, 28; 16 of up to 1000 22.5, 15.0; 64 of 8192 272, 222; 13 trees of up to 64 103, 45
     const int wgs = lk_pa_wgs(s.step);
     if (items <= wgs / 32)
         hipLaunchKernelGGL((lk_k_paged_spread<D, RT>), dim3((unsigned) items, nblk * (D / 16)), dim3(1024), 0, st, a, s.cb, wgs);
@@ -1049,7 +1078,7 @@ extern "C" int lk_paged_attn(const lk_pages * pages, const lk_step * step, int t
     float2 * ml = (float2 *) (acc + blocks * 16 * d);
     const LkPaArgs a = { q, out, (const char *) pages->k, (const char *) pages->v, step->first, step->lens, step->table, step->pos,
                          step->mask, slopes, acc, ml, (int4 *) (ml + blocks * 16), ldq, ldo, step->n_seqs, step->rows, step->ldt,
-                         step->width, lk_log2(pages->page), pages->n_pages, hq, pages->n_kv_heads, g, nhg, s.hg_sh, s.qw_sh, s.kw_sh, s.qc, s.extra,
+                         step->width, lk_log2(pages->page), pages->n_pages, pages->n_kv_heads, g, nhg, s.hg_sh, s.qw_sh, s.kw_sh, s.qc, s.extra,
                          scale * LK_LOG2E_F, scale, cap, 1.0f / cap };
     const hipStream_t st = lk_stream(stream);
     const bool mod = cap > 0.0f || slopes;

@@ -110,6 +110,12 @@ def test_every_number_of_new_tokens(lk, hq, hkv, d, t, n):
     _check(lk, n, Batch(n, lens, [n] * 3, 16), hq, hkv, d, t, max_new=n)
 
 
+@pytest.mark.parametrize("hq,hkv,d,t", [(2, 2, 64, "f16"), (2, 2, 64, "f32"), (2, 2, 128, "bf16"), (8, 1, 64, "f32")])
+def test_runs_of_many_chunks(lk, hq, hkv, d, t):
+    """Beyond a thousand new tokens a wave holds more columns."""
+    _check(lk, hq + d, Batch(d, [30, 0], [1030, 9], 64), hq, hkv, d, t, max_new=1030)
+
+
 @pytest.mark.parametrize("cap,bias", [(20.0, False), (0.0, True), (5.0, True), (0.25, False)])
 @pytest.mark.parametrize("hq,hkv,d,t", [(32, 8, 64, "f16"), (12, 4, 128, "bf16"), (16, 2, 64, "f32"), (8, 1, 128, "f32")])
 def test_capped_and_biased_scores(lk, hq, hkv, d, t, cap, bias):
