@@ -604,8 +604,8 @@ int lk_paged_append(const lk_pages * pages, const lk_step * step, int type, cons
  *   the key - position of the row), a cached key's position being its slot;  out = softmax(x) . v
  * and zeros for a row that sees nothing.  Keys and values a row does not see do not touch
  * it, infinities and NaN among them.
- * q, out rows of `type` as in lk_paged_append, n_heads heads side by side; scale > 0, cap 0 or at least 2^-100;
- * slopes fp32 [n_heads] or NULL.  Scores, softmax and sums are fp32.  The weights enter the product
+ * q, out rows of `type` as in lk_paged_append, n_heads heads side by side (out may be q); scale > 0, cap 0 or at least 2^-100;
+ * slopes fp32 [n_heads] or NULL.  Scores (below 2^27), softmax and sums are fp32.  The weights enter the product
  * with v as two parts of the pools' type (what the first one's rounding leaves is the second),
  * and so does q where the rows are fp32; for 16-bit rows of more than 16 (new token, query head) pairs a
  * kv head, by max_new, as one part.  Sums of the weights are rounded alike.  Results do not depend on the

@@ -24,8 +24,12 @@
 #include "lk_paged.h"
 
 #define LK_PA_TILEB 32768          // a tile: K rows, then V rows
-#define LK_PA_HEADROOM 8.0f        // the running max is raised when a score passes it by 2^8
-#define LK_PA_NONE  3.0e38f        // minus the running max of no score: 2^(any score in sight - max) is 0 against it
+// Weights are 2^(score - offset).  The offset is set to 2^-LK_PA_LIFT of the largest score and raised when a score
+// passes it by 2^LK_PA_HEADROOM, so that the largest weight is 2^7 to 2^15: in fp16, whose steps below 2^-14 are
+// 2^-24 whatever the value, a weight keeps its 11 bits down to 2^-21 of the row's first maximum.
+#define LK_PA_LIFT 7.0f
+#define LK_PA_HEADROOM 15.0f
+#define LK_PA_NONE  3.0e38f        // minus the offset of no score: 2^(offset - any score in sight) is 0 against it
 
 // Two kinds of workgroup.  For up to 16 columns a kv head (STEP 16) the cache's bytes bound it: one workgroup a
 // CU, a ring of four tiles, so that 96 KB are on their way (64 sequences of 8192, 32 / 8 heads of 64, bf16: 214 us,
@@ -381,7 +385,7 @@ lk_k_paged_attn(const LkPaArgs) {
     // ---- a column's state ----------------------------------------------------------------
     V8 qh[CB][KS], ql[TWO ? CB : 1][KS];
     lk_f4 acc[CB][DB], accl[CB];
-    float mneg[CB], fac[TWO ? CB : 1];                          // minus the running max (units of log2); score factor of a scaled q
+    float mneg[CB], fac[TWO ? CB : 1];                          // minus the weights' offset (units of log2); score factor of a scaled q
     float slope[MOD ? CB : 1];
     int qpos[MOD ? CB : 1];
     int base = 0;                                               // keys below it are seen by all of the chunk's rows
@@ -421,8 +425,8 @@ lk_k_paged_attn(const LkPaArgs) {
             }
             const RowT * src = (const RowT *) a.q + (size_t) row * a.ldq + (size_t) head * D + 8 * g;
             if constexpr (TWO) {
-                // both parts must be finite in fp16: a head whose largest value reaches 2^15 is scaled
-                // by a power of two, and its scores back
+                // a head is scaled by a power of two to a largest value of 2^14 to 2^15, so that both parts are
+                // finite and 22 bits of it count whatever its size is, and its scores back
                 float v[KS][8], am = 0.0f;
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
@@ -435,7 +439,7 @@ lk_k_paged_attn(const LkPaArgs) {
                 }
                 am = lk_xrow_max(am);
                 int e2 = 0;
-                if (am >= 32768.0f && am <= 3.4e38f) {
+                if (am >= 0x1p-60f && am <= 3.4e38f) {         // (below, the scores' factor could vanish)
                     (void) frexpf(am, &e2);
                     e2 -= 15;
                 }
@@ -509,13 +513,13 @@ lk_k_paged_attn(const LkPaArgs) {
             }
         }
     };
-    // raises the running max of column block cb to cover a lane's largest score (units of log2)
+    // raises the offset of column block cb to cover a lane's largest score (units of log2)
     auto raise = [&](int cb, float top) {
-        if (__ballot(top > LK_PA_HEADROOM - mneg[cb])) {        // wave-uniform
+        if (__ballot(top + mneg[cb] > LK_PA_HEADROOM)) {        // wave-uniform (a difference: exact for large scores)
             const float mx = lk_xrow_max(top);
-            if (mx > LK_PA_HEADROOM - mneg[cb]) {
-                const float f = lk_exp2(-mneg[cb] - mx);
-                mneg[cb] = -mx;
+            if (mx + mneg[cb] > LK_PA_HEADROOM) {
+                const float to = LK_PA_LIFT - mx, f = lk_exp2(to - mneg[cb]);
+                mneg[cb] = to;
 #pragma unroll
                 for (int db = 0; db < DB; ++db) acc[cb][db] *= f;
                 accl[cb] *= f;

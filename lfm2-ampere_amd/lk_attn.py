@@ -711,7 +711,8 @@ class PagedStep:
     Keeps the tables and the attention's workspace, made at its first use (or `work`, uint8 of
     PagedCache.work_bytes()): attention calls on a step must be ordered (one stream, or
     events); calls that may overlap, captured graphs among them, take steps of their own.  A step
-    may be dropped while streams still work on it as far as a workspace of its own goes."""
+    may be dropped while streams still work on it as far as a workspace of its own goes; a captured
+    graph needs its steps kept."""
 
     def __init__(self, first, lens, table, rows: int, pos=None, mask=None, max_new: int = 0, work=None):
         import torch
@@ -816,7 +817,7 @@ class PagedCache:
 
     def attend(self, step, q, out, scale: Optional[float] = None, cap: float = 0.0, slopes=None, stream=None) -> None:
         """out = attention of the step's rows q [rows][heads * head_dim] over their sequences' pages
-        and new tokens (lk_paged_attn); scale 1/sqrt(head_dim) unless given, cap > 0: scores capped
+        and new tokens, which may be written over q (lk_paged_attn); scale 1/sqrt(head_dim) unless given, cap > 0: scores capped
         by cap * tanh(x / cap), slopes fp32 [heads]: a bias of slope times distance."""
         ty = _type_of(q, "PagedCache.attend")
         shape, dev, dt = (step.rows, self._hq), self._dev, q.dtype

@@ -1,6 +1,7 @@
 """lk_paged_attn on the GPU against 64 bits: single tokens, trees, causal runs, every head
 layout and type, and the places where it can go wrong.  The bound of every comparison is
 derived in paged_util.attend_ref."""
+import math
 import random
 
 import pytest
@@ -285,6 +286,81 @@ def test_queries_past_the_range_of_fp16(lk):
         k = k * 1e-3
         for hint in (1, 64):
             _check(lk, 43, b, hq, hkv, d, "f32", q=q, kv=(k.half(), v), max_new=hint)
+
+
+@pytest.mark.parametrize("shift", [-50, -20, 20])
+def test_fp32_queries_of_any_size(lk, shift):
+    """A power of two moved from the scale to the queries leaves every bit as it was."""
+    b = Batch(46, [50, 200, 700], [3, 20, 1], 16)
+    for d, hq, hkv in ((64, 8, 2), (128, 4, 4)):
+        q, kv = _q(47, b.rows, hq * d, torch.float32), pools(48, b, hkv, d, "f32")
+        for hint in (1, 64):
+            for cap in (0.0, 8.0):
+                want = _check(lk, 49, b, hq, hkv, d, "f32", q=q, kv=kv, max_new=hint, scale=0.25, cap=cap)
+                got = _check(lk, 49, b, hq, hkv, d, "f32", q=q * 2.0 ** shift, kv=kv, max_new=hint, scale=0.25 * 2.0 ** -shift, cap=cap)
+                assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_many_small_weights_beside_a_large_one(lk, d, t):
+    """3000 keys of weight 2^-14 of the first one's, whose values lie on the other side."""
+    b = Batch(50, [3000], [1], 16)
+    k, v = torch.zeros(b.n_pages, 16, 2, d, dtype=pools(1, b, 2, d, t)[0].dtype), None
+    v = torch.full_like(k, -1.0)
+    at = b.slots(0, 0, 3001)
+    k.view(-1, 2, d)[at[0], :, 0] = 14 * math.log(2.0)
+    v.view(-1, 2, d)[at[0]] = 1.0
+    q = torch.zeros(b.rows, 4 * d, dtype=TYPES[t])
+    q.view(-1, 4, d)[:, :, 0] = 1.0
+    k.view(-1, 2, d)[at[1:], :, 1] = torch.linspace(-0.2, 0.2, 3000)[:, None].to(k.dtype)
+    q.view(-1, 4, d)[:, :, 1] = 1.0
+    for hint in (1, 64):
+        _check(lk, 51, b, 4, 2, d, t, q=q, kv=(k, v), scale=1.0, max_new=hint)
+
+
+@pytest.mark.parametrize("up", [True, False])
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+def test_scores_of_many_millions(lk, t, up):
+    """The key of the largest score is all of the row: the next one is 2^18 below."""
+    for d, page in ((64, 16), (128, 64)):
+        b = Batch(55, [1500, 900], [1, 20], page)
+        k, v = pools(56, b, 2, d, t)
+        k.zero_()
+        for s, n in enumerate((1501, 920)):
+            at = b.slots(s, 0, n)
+            steps = torch.arange(n)[:, None] % 250
+            k.view(-1, 2, d)[at, :, 0] = (128.0 * (steps if up else 250 - steps)).to(k.dtype)
+        q = torch.zeros(b.rows, 4, d, dtype=TYPES[t])
+        q[:, :, 0] = 2048.0
+        for hint in (1, 64):
+            out = torch.empty(b.rows, 4 * d, dtype=TYPES[t], device="cuda")
+            note(f"scores to 2^26 {t} {d} up {up} hint {hint}")
+            lk.PagedCache(k.cuda(), v.cuda(), 4).attend(b.step(lk, max_new=hint), q.cuda().view(b.rows, -1), out, scale=1.0)
+            torch.cuda.synchronize()
+            got = out.cpu().double().view(-1, 4, d)
+            assert bool(torch.isfinite(got).all())
+            for r in range(21):
+                s, n = (0, 1501) if r == 0 else (1, 901 + r - 1)
+                at = b.slots(s, 0, n)
+                top = k.view(-1, 2, d)[at, 0, 0].double()
+                rows = v.view(-1, 2, d)[at[top == top.max()]].double().repeat_interleave(2, 1)
+                # equal weights: their common rounding cancels, the sums and the one rounding stay
+                assert bool(((got[r] - rows.mean(0)).abs() <= 2.0 ** -18 * rows.abs().amax(0) +
+                             torch.finfo(TYPES[t]).eps * rows.mean(0).abs()).all())
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+def test_outputs_over_the_queries(lk, t):
+    for lens, news in (([300, 0, 5000], [1, 1, 1]), ([40, 0, 900], [20, 3, 64]), ([0, 30], [200, 65])):
+        b = Batch(52, lens, news, 16)
+        k, v = pools(53, b, 2, 64, t)
+        q = _q(54, b.rows, 512, TYPES[t]).cuda()
+        cache, step, out = lk.PagedCache(k.cuda(), v.cuda(), 8), b.step(lk, max_new=max(news)), torch.empty_like(q)
+        cache.attend(step, q, out)
+        cache.attend(step, q, q)
+        torch.cuda.synchronize()
+        assert torch.equal(q, out)
 
 
 def test_scores_that_grow_along_the_keys(lk):
