@@ -32,12 +32,13 @@
 #define LK_PA_NONE  3.0e38f        // minus the offset of no score: 2^(offset - any score in sight) is 0 against it
 
 // Two kinds of workgroup.  For up to 16 columns a kv head (STEP 16) the cache's bytes bound it: one workgroup a
-// CU, a ring of four tiles, so that 96 KB are on their way (64 sequences of 8192, 32 / 8 heads of 64, bf16: 214 us,
-// 6.4 TB/s; one of 131072 in 42 us, 6.4 TB/s, the pieces' sum 6 more).  For more (STEP 32) the products and
+// CU, a ring of four tiles, so that 96 KB are on their way (64 sequences of up to 8192, 32 / 8 heads of 128, bf16: 213 us,
+// 6.6 TB/s; one of 131072 in 42 us, 6.4 TB/s, the pieces' sum 6 more).  For more (STEP 32) the products and
 // exponentials do: two workgroups a CU of one wave a SIMD each, which wait at barriers of their own, and two tiles
-// (2 x 4096 new tokens 197 us, 592 TFLOP/s of products; at K = 32 a tile's 16 x 16 products and its exponentials
-// take 139 us of issue, one behind the other on a SIMD).  Between the two, 8 tokens of 4 heads a kv head, STEP 32
-// too: one sequence at 30000 21.7 us against 29.9, 16 at 1000 13.9 against 18.9.
+// (2 x 4096 new tokens 185 us, 635 TFLOP/s, and their join; of 457 thousand cycles a SIMD issues matrix
+// instructions for 129 and others for 207, which hardly overlap).  Between the two, 8 tokens of 4 heads a kv head, STEP 32
+// too: one sequence at 30000 21.7 us against 29.9, 16 at 1000 13.9 against 18.9.  DMA and products of short runs wait
+// for each other: 13 trees of up to 64 at 4096 40 us, where a SIMD issues for 43 of 110 thousand cycles.
 __host__ __device__ constexpr int lk_pa_waves(int d, int step) { return step == 16 && d == 64 ? 8 : 4; }
 __host__ __device__ constexpr int lk_pa_bufs(int step) { return step == 16 ? 4 : 2; }
 __host__ __device__ constexpr int lk_pa_wgs(int step) { return step == 16 ? 256 : 512; }
@@ -84,9 +85,9 @@ struct LkPaArgs {
     const int32_t * first, * lens, * table, * pos;
     const uint64_t * mask;
     const float * slopes;
-    float * acc;                   // partials: [2 * workgroup + end][block of columns][D / 16][column][4][4 dims]
+    float * acc;                   // partials: [2 * run + end][block of columns][D / 16][column][4][4 dims]
     float2 * ml;                   // and their (max, sum): [..][..][16]
-    int4 * cut;                    // per workgroup the cut item that begins in it: (pieces, first row, rows, kv head group)
+    int4 * cut;                    // per run the cut item that begins in it: (pieces, first row, rows, kv head group)
     int ldq, ldo, n_seqs, rows, ldt, width, page_sh, n_pages;
     int hkv, g;                    // g = query heads a kv head
     int nhg, hg_sh, qw_sh, kw_sh;  // groups of 2^hg_sh kv heads; a workgroup's waves = heads x column groups x key shares
@@ -292,9 +293,13 @@ lk_k_paged_attn(const LkPaArgs) {
         total = lk_uniform64(total);
     }
     const long share = (total + lk_pa_wgs(STEP) - 1) / lk_pa_wgs(STEP);
-    const long f0 = share * blockIdx.x, f1 = f0 + share < total ? f0 + share : total;
+    // Workgroups go round the eight XCDs; runs side by side, whose chunks read the same keys, are given to one XCD and
+    // its L2 (2 x 4096 new tokens 200 -> 195 us, 13 trees 46.0 -> 44.7), but for short runs, which may be fewer than the
+    // workgroups and would then be on few XCDs (a tree of 16 at 32768 26.2 that way, 25.2 round).
+    const int wgi = share >= 8 ? (blockIdx.x & 7) * (lk_pa_wgs(STEP) / 8) + (blockIdx.x >> 3) : blockIdx.x;
+    const long f0 = share * wgi, f1 = f0 + share < total ? f0 + share : total;
     if (f0 >= f1) {
-        if (threadIdx.x == 0) args().cut[blockIdx.x] = make_int4(0, 0, 0, 0);
+        if (threadIdx.x == 0) args().cut[wgi] = make_int4(0, 0, 0, 0);
         return;
     }
     LkPaAt at;
@@ -695,7 +700,7 @@ lk_k_paged_attn(const LkPaArgs) {
         if (kw != 0) return;
         const LkPaC & a = args();
         const int nblk = CB << (a.qw_sh + a.hg_sh);
-        const int slot = 2 * blockIdx.x + from_first;
+        const int slot = 2 * wgi + from_first;
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) {
             int i, row, head;
@@ -724,7 +729,7 @@ lk_k_paged_attn(const LkPaArgs) {
         left += at.t;
         at.t = 0;
         if (left <= 0) {
-            if (threadIdx.x == 0) args().cut[blockIdx.x] = make_int4(0, 0, 0, 0);
+            if (threadIdx.x == 0) args().cut[wgi] = make_int4(0, 0, 0, 0);
             return;
         }
     }
@@ -790,7 +795,7 @@ lk_k_paged_attn(const LkPaArgs) {
         left -= extra;
         if (left > 0) lk_pa_next(args(), at, tk_sh);
     }
-    if (threadIdx.x == 0) args().cut[blockIdx.x] = cut;
+    if (threadIdx.x == 0) args().cut[wgi] = cut;
 }
 
 // ---- joining cut items ------------------------------------------------------------------------
@@ -813,7 +818,7 @@ struct LkPaBlock {
 };
 
 // Many items, cut into few pieces each: workgroup (x, blk) joins block blk of the item that begins in
-// workgroup x, each wave some of its dims.  A load of each piece is all it does: eight are asked for at once, so
+// run x, each wave some of its dims.  A load of each piece is all it does: eight are asked for at once, so
 // that their latencies overlap (in place of two: 2 x 4096 new tokens 222 -> 210 us as a whole, 19 sequences of up
 // to 5003 21.5 -> 19.5).  Of 2 x 4096 new tokens it takes 11.7 us for at most 64 MB, 5.5 TB/s.
 template <int D, int RT>
