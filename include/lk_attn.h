@@ -606,10 +606,10 @@ int lk_paged_append(const lk_pages * pages, const lk_step * step, int type, cons
  * it, infinities and NaN among them.
  * q, out rows of `type` as in lk_paged_append, n_heads heads side by side (out may be q); scale > 0, cap 0 or at least 2^-100;
  * slopes fp32 [n_heads] or NULL.  Scores (below 2^27), softmax and sums are fp32.  The weights enter the product
- * with v as two parts of the pools' type (what the first one's rounding leaves is the second),
- * and so does q where the rows are fp32; for 16-bit rows of more than 16 (new token, query head) pairs a
- * kv head, by max_new, as one part.  Sums of the weights are rounded alike.  Results do not depend on the
- * run; the last bits depend on how the batch's keys are divided among the workgroups.
+ * with v as two parts of the pools' type (what the first one leaves is the second: 2^-22 of a
+ * weight is lost with fp16 pools, 2^-16 with bf16), and so does q where the rows are fp32.  Sums of the weights
+ * are rounded alike.  Results do not depend on the run; the last bits depend on how the batch's keys
+ * are divided among the workgroups, which max_new has a part in.
  * work: 16-byte aligned device memory of lk_paged_attn_work_bytes() (0 on bad arguments;
  * lk_last_error() says which); launches that share it must be ordered (one stream, or the
  * caller's events), and graphs that may run at once need two. */

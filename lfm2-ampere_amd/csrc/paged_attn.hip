@@ -61,6 +61,7 @@ template <> struct LkMm<LK_F16> {
     static __device__ __forceinline__ lk_f4 k16(V4, V4, lk_f4 c) { return c; }
 #endif
     static constexpr uint16_t INF = 0x7C00;
+    static constexpr uint32_t LEAD = 0xFFFFE000;               // the bits of an fp32 number that the type holds
 };
 template <> struct LkMm<LK_BF16> {
     typedef __bf16 T;
@@ -76,6 +77,7 @@ template <> struct LkMm<LK_BF16> {
     static __device__ __forceinline__ lk_f4 k16(V4, V4, lk_f4 c) { return c; }
 #endif
     static constexpr uint16_t INF = 0x7F80;
+    static constexpr uint32_t LEAD = 0xFFFF0000;
 };
 
 struct LkPaArgs {
@@ -237,9 +239,10 @@ __device__ __forceinline__ float lk_tanh(float t) {
 // D: head_dim.  RT: rows (LK_F32: q as two parts).  CT: pools.  CB: blocks of 16
 // columns a wave holds.  STEP: keys a wave takes at once, 32 by K = 32 products of both kinds, 16 by
 // K = 16 for P.V.  MOD: capped or biased scores.
-// The weights enter P.V as two parts of the pools' type, a second product for what the first part's rounding
-// leaves, where the kernel waits for memory (STEP 16: no slower, and the result is off by its own rounding
-// alone: bf16 1.7e-3 relative; one part 2.3e-3) and for fp32 rows; elsewhere as one part.
+// The weights enter P.V as two parts of the pools' type, a second product for what the first part leaves,
+// so that the result is off by its own rounding alone, whatever kernel `max_new` chose (bf16 1.7e-3 relative,
+// fp16 2.1e-4; one part 2.3e-3 and 2.9e-4).  Where memory bounds the kernel that costs nothing; 2 x 4096 new
+// tokens take 262 us so, 197 with one part, 13 trees of up to 64 at 4096 52 and 45.
 template <int D, int RT, int CT, int CB, int STEP, bool MOD>
 __global__ void __launch_bounds__(64 * lk_pa_waves(D, STEP), STEP == 16 && D == 128 ? 1 : 2)
 lk_k_paged_attn(const LkPaArgs) {
@@ -256,7 +259,7 @@ lk_k_paged_attn(const LkPaArgs) {
     typedef typename M::V8 V8;
     typedef typename M::V4 V4;
     typedef typename LkElem<RT>::type RowT;
-    constexpr bool TWO = RT == LK_F32, TWOW = TWO || STEP == 16;
+    constexpr bool TWO = RT == LK_F32;
     constexpr int NW = lk_pa_waves(D, STEP), NBUF = lk_pa_bufs(STEP), NB = STEP / 16;
     constexpr int KS = D / 32, DB = D / 16, DC = D / 8;        // steps of q.k, blocks of output dims, 16-byte pieces of a head's row
     constexpr int NF = 16 / NW;                                // pieces of 1 KB a wave fetches of a tile's K, and of its V
@@ -531,14 +534,20 @@ lk_k_paged_attn(const LkPaArgs) {
             }
         }
     };
-    // weights of four scores, and what their rounding leaves
+    // weights of four scores in two parts: the leading bits that the type holds, cut off by a mask, and the rest,
+    // rounded: 2^-22 of the weight is lost in fp16, 2^-16 in bf16.  (The first part rounded to nearest has to be
+    // converted back: a prompt of 4096 with heads of 128, bf16, 279 us for 264, 2 x 4096 in fp16 259 for 262.)
     auto weights = [&](const lk_f4 & c, int cb, V4 & ph, V4 & pl) {
+        lk_f4 p, h;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const float p = lk_exp2(MOD ? c[r] + mneg[cb] : __builtin_fmaf(c[r], factor(cb), mneg[cb]));
-            ph[r] = (T) p;
-            if constexpr (TWOW) pl[r] = (T) (p - (float) ph[r]);
+            const float x = lk_exp2(MOD ? c[r] + mneg[cb] : __builtin_fmaf(c[r], factor(cb), mneg[cb]));
+            h[r] = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & M::LEAD);
+            p[r] = x;
         }
+        ph = __builtin_convertvector(h, V4);
+        p -= h;
+        pl = __builtin_convertvector(p, V4);
     };
     auto top4 = [&](const lk_f4 & c) -> float { return fmaxf(fmaxf(c[0], c[1]), fmaxf(c[2], c[3])); };
     auto units = [&](float top, int cb) -> float { return MOD ? top : top * factor(cb); };
@@ -556,7 +565,7 @@ lk_k_paged_attn(const LkPaArgs) {
     // STEP keys, the first of them key0, kf their K rows; `more`: the rows of the STEP keys behind are
     // asked for.  From `base` on there are keys that only some of the rows see.
     auto step = [&](const unsigned char * kt, const unsigned char * vt, int key0, V8 (&kf)[NB][KS], bool more) {
-        V4 ph[CB][NB], pl[TWOW ? CB : 1][NB], vf[DB][NB];
+        V4 ph[CB][NB], pl[CB][NB], vf[DB][NB];
         lk_f4 c[CB][NB];
         const bool some = key0 + STEP > base;                   // wave-uniform
 #pragma unroll
@@ -618,14 +627,14 @@ lk_k_paged_attn(const LkPaArgs) {
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) {
 #pragma unroll
-            for (int n = 0; n < NB; ++n) weights(c[cb][n], cb, ph[cb][n], pl[TWOW ? cb : 0][n]);
+            for (int n = 0; n < NB; ++n) weights(c[cb][n], cb, ph[cb][n], pl[cb][n]);
             auto product = [&](const V4 (&v)[NB], lk_f4 o) -> lk_f4 {
                 if constexpr (NB == 2) {
                     o = M::k32(join(v[0], v[1]), join(ph[cb][0], ph[cb][1]), o);
-                    if constexpr (TWOW) o = M::k32(join(v[0], v[1]), join(pl[cb][0], pl[cb][1]), o);
+                    o = M::k32(join(v[0], v[1]), join(pl[cb][0], pl[cb][1]), o);
                 } else {
                     o = M::k16(v[0], ph[cb][0], o);
-                    if constexpr (TWOW) o = M::k16(v[0], pl[cb][0], o);
+                    o = M::k16(v[0], pl[cb][0], o);
                 }
                 return o;
             };
