@@ -433,7 +433,7 @@ lk_k_paged_attn(const LkPaArgs) {
             }
             const RowT * src = (const RowT *) a.q + (size_t) row * a.ldq + (size_t) head * D + 8 * g;
             if constexpr (TWO) {
-                // a head is scaled by a power of two to a largest value of 2^14 to 2^15, so that both parts are
+                // a head is scaled by a power of two to a largest finite value of 2^14 to 2^15, so that both parts are
                 // finite and 22 bits of it count whatever its size is, and its scores back
                 float v[KS][8], am = 0.0f;
 #pragma unroll
@@ -442,24 +442,26 @@ lk_k_paged_attn(const LkPaArgs) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         v[ks][e] = live ? v[ks][e] : 0.0f;
-                        am = fmaxf(am, fabsf(v[ks][e]));
+                        am = fabsf(v[ks][e]) < INFINITY ? fmaxf(am, fabsf(v[ks][e])) : am;
                     }
                 }
                 am = lk_xrow_max(am);
                 int e2 = 0;
-                if (am >= 0x1p-60f && am <= 3.4e38f) {         // (below, the scores' factor could vanish)
+                if (am > 0.0f) {
                     (void) frexpf(am, &e2);
-                    e2 -= 15;
+                    e2 = e2 - 15 > -74 ? e2 - 15 : -74;         // (below, the scores' factor could vanish)
                 }
                 fac[cb] = ldexpf(sc, e2);
+                // where the key's value is infinite the first part alone gives the score (finite_scores), so it is
+                // 0 where the value is 0 alone: below 2^-14 it is that, and the second part takes it back
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const float x = ldexpf(v[ks][e], -e2);
-                        const T h = (T) x;
-                        qh[cb][ks][e] = h;
-                        ql[cb][ks][e] = (T) (x - (float) h);
+                        const float h = (float) (T) (x != 0.0f && fabsf(x) < 0x1p-14f ? copysignf(0x1p-14f, x) : x);
+                        qh[cb][ks][e] = (T) h;
+                        ql[cb][ks][e] = (T) (fabsf(x) < INFINITY ? x - h : 0.0f);
                     }
             } else {
 #pragma unroll
@@ -501,6 +503,26 @@ lk_k_paged_attn(const LkPaArgs) {
             if constexpr (TWO) c = M::k32(kf[ks], ql[cb][ks], c);
         }
         return c;
+    };
+    // An infinity among the keys times a second part, which is 0 or of either sign, is no number.  Scores that are not
+    // finite are those of the first part alone, of the value's sign.  (Finite ones are below 2^39: their sum is finite.)
+    auto finite_scores = [&](const V8 (&kf)[NB][KS], lk_f4 (&c)[CB][NB]) {
+        float all = 0.0f;
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+            for (int n = 0; n < NB; ++n) all += (c[cb][n][0] + c[cb][n][1]) + (c[cb][n][2] + c[cb][n][3]);
+        if (__ballot(!(fabsf(all) < INFINITY)) == 0) return;    // wave-uniform
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                lk_f4 o = { 0.f, 0.f, 0.f, 0.f };
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) o = M::k32(kf[n][ks], qh[cb][ks], o);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) c[cb][n][r] = fabsf(c[cb][n][r]) < INFINITY ? c[cb][n][r] : o[r];
+            }
     };
     auto factor = [&](int cb) -> float { return TWO ? fac[cb] : sc; };
     // capped and biased scores in units of log2, of keys k0 .. k0 + 3 (k0: the lane's first)
@@ -576,6 +598,7 @@ lk_k_paged_attn(const LkPaArgs) {
         for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
             for (int n = 0; n < NB; ++n) c[cb][n] = scores(kf[n], cb);
+        if constexpr (TWO) finite_scores(kf, c);
         if (more) kload(kt + (STEP << rb_sh), kf);
         if constexpr (MOD) {
 #pragma unroll

@@ -1,0 +1,130 @@
+"""Infinities and NaN among the keys, values and queries that a row of lk_paged_attn does see, in earlier
+and in new positions, against the definition in 64 bits: softmax(x) . v, in which a score of -inf has the
+weight 0, one of +inf or NaN makes the row NaN, and the weight of a finite score, however small, is
+above 0.  (0 times an infinity is NaN.)"""
+import math
+
+import pytest
+import torch
+
+from gpu_util import note
+from paged_util import HALF_STEP, TYPES, U, Batch, causal, pools
+
+pytestmark = pytest.mark.gpu
+INF = math.inf
+LOST = {"f32": 2.0 ** -21, "f16": 2.0 ** -21, "bf16": 2.0 ** -16}      # of a weight in two parts (fp32 rows: and of q)
+
+
+def _row(x, S, v, t):
+    """softmax(x) . v for visible scores x [N] and values v [N][d] in 64 bits, with how far finite results may be
+    off: as paged_util.attend_ref, the weight's own part by LOST.  S: largest sum of |q k|, scaled."""
+    d = v.shape[1]
+    if len(x) == 0:
+        return torch.zeros(d, dtype=torch.float64), torch.zeros(d, dtype=torch.float64)
+    top = x.max()
+    if bool(torch.isnan(x).any()) or not bool(torch.isfinite(top)):
+        return torch.full((d,), math.nan, dtype=torch.float64), torch.zeros(d, dtype=torch.float64)
+    p = torch.exp(x - top)
+    fin = torch.isfinite(v)
+    vf = torch.where(fin, v, 0.0)
+    z = p.sum()
+    o, A = (p[:, None] * vf).sum(0) / z, (p[:, None] * vf.abs()).sum(0) / z
+    # nothing finite is left beside an infinity
+    odd = torch.where(fin, 0.0, torch.where((x > -INF)[:, None], v, math.nan)).sum(0)
+    ends = torch.isfinite(x)
+    e = LOST[t] + U * (42 * S + 4 * x[ends].abs().max() + 2 * (x[ends] - top).abs().max() + 2) + 2.0 ** -22 * S
+    w = e * (A + o.abs()) + (len(x) / 16 + 48) * U * A
+    return torch.where(fin.all(0), o, odd), w + HALF_STEP[TYPES[t]] * (o.abs() + w) + (2.0 ** -25 if t == "f16" else 0)
+
+
+def _defined(b, q, k, v, t, scale, cap=0.0, masks=None):
+    hkv, d = k.shape[2:]
+    hq = q.shape[1] // d
+    want, tol = [], []
+    for s, (a, n) in enumerate(zip(b.lens, b.news)):
+        at = b.slots(s, 0, a + n)
+        ks, vs = (x.view(-1, hkv, d)[at].double() for x in (k, v))
+        sees = causal(n, a)
+        if masks is not None:
+            sees[:, a:] = torch.tensor([[bool(masks[b.first[s] + i] >> j & 1) for j in range(n)] for i in range(n)]).view(n, n)
+        for i in range(n):
+            for h in range(hq):
+                kv = h * hkv // hq
+                prod = q[b.first[s] + i].view(hq, d)[h].double() * ks[sees[i], kv]
+                x = prod.sum(-1) * scale
+                x = cap * torch.tanh(x / cap) if cap else x
+                S = float((torch.where(torch.isfinite(prod), prod, 0.0).abs().sum(-1) * scale).max()) if len(x) else 0.0
+                w, e = _row(x, S, vs[sees[i], kv], t)
+                want.append(w)
+                tol.append(e)
+    return torch.stack(want).view(-1, hq, d), torch.stack(tol).view(-1, hq, d)
+
+
+def _check(lk, what, b, q, k, v, t, hints, scale=0.25, cap=0.0, masks=None):
+    """Compares finite outputs by the bound, infinities and NaN as such.  Returns the expected rows."""
+    hkv, d = k.shape[2:]
+    hq = q.shape[1] // d
+    want, tol = _defined(b, q, k, v, t, scale, cap, masks)
+    cache, qd = lk.PagedCache(k.cuda(), v.cuda(), hq), q.cuda()
+    for hint in hints:
+        out = torch.full((b.rows, hq * d), 77.0, dtype=TYPES[t], device="cuda")
+        note(f"{what}, {t}, {hq}/{hkv}/{d}, lens {b.lens}, hint {hint}")
+        cache.attend(b.step(lk, mask=masks, max_new=hint), qd, out, scale=scale, cap=cap)
+        torch.cuda.synchronize()
+        got = out.cpu().double().view(-1, hq, d)
+        good = (torch.isnan(got) & torch.isnan(want)) | (got == want) | \
+            (torch.isfinite(got) & torch.isfinite(want) & ((got - want).abs() <= tol))
+        bad = (~good).nonzero()
+        assert len(bad) == 0, (hint, len(bad), [(r.tolist(), got[tuple(r)].item(), want[tuple(r)].item()) for r in bad[:4]])
+    return want
+
+
+def _rows(seed, n, dtype, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(n, generator=g) * scale).to(dtype)
+
+
+SHAPES = [(4, 2, 64), (4, 2, 128), (33, 1, 64)]
+TINY = {"f32": 1e-30, "f16": 2.0 ** -20, "bf16": 2.0 ** -100}
+
+
+def _batches():
+    """(batch, hints): one token behind few and many keys, a run, a run of many chunks."""
+    return ((Batch(1, [50, 900], [1, 1], 16), (1, 16, 64)), (Batch(2, [50, 300], [20, 3], 32), (1, 16, 64, 300)))
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hq,hkv,d", SHAPES)
+@pytest.mark.parametrize("value", [INF, -INF])
+@pytest.mark.parametrize("cap", [0.0, 5.0])
+def test_infinite_keys(lk, hq, hkv, d, t, value, cap):
+    """A key whose score is -inf counts as none, one of +inf, or a 0 against the infinity, makes the row NaN; capped
+    scores are plus or minus the cap.  The query's value may be as small as the type has any."""
+    for b, hints in _batches():
+        for where in ("first", "late", "new"):
+            k, v = pools(3, b, hkv, d, t)
+            for s in range(2):
+                at = {"first": 7, "late": b.lens[s] - 2, "new": b.lens[s]}[where]
+                k.view(-1, hkv, d)[b.slot(s, at), 0, 3] = value
+            q = _rows(4, b.rows * hq * d, TYPES[t]).view(b.rows, hq * d)
+            heads = q.view(b.rows, hq, d)
+            heads[:, :, 3] = torch.where(heads[:, :, 3] >= 0, 0.5, -0.5)
+            heads[0, 1, 3], heads[-1, 0, 3], heads[-1, -1, 3] = 0.0, TINY[t], -TINY[t]
+            want = _check(lk, f"a {where} key of {value}, cap {cap}", b, q, k, v, t, hints, cap=cap)
+            assert bool(torch.isfinite(want).all(-1).any()) and bool(torch.isnan(want).any())
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hq,hkv,d", SHAPES)
+@pytest.mark.parametrize("value", [INF, -INF, math.nan])
+def test_queries_that_are_not_finite(lk, hq, hkv, d, t, value):
+    """The row and head are NaN, or, capped, see every score at plus or minus the cap; no other row changes."""
+    for b, hints in _batches():
+        for cap in (0.0, 5.0):
+            k, v = pools(5, b, hkv, d, t)
+            q = _rows(6, b.rows * hq * d, TYPES[t]).view(b.rows, hq * d)
+            q.view(b.rows, hq, d)[0, 0, 9] = value
+            q.view(b.rows, hq, d)[0, 0, 10] = 6e4 if t == "f16" else 1e30
+            if cap:
+                k.view(-1, hkv, d)[:, :, 9] = torch.where(k.view(-1, hkv, d)[:, :, 9] >= 0, 0.5, -0.5).to(k.dtype)
+            _check(lk, f"a query of {value}, cap {cap}", b, q, k, v, t, hints, cap=cap)
