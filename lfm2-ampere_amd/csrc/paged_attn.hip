@@ -30,6 +30,7 @@
 #define LK_PA_LIFT 7.0f
 #define LK_PA_HEADROOM 15.0f
 #define LK_PA_NONE  3.0e38f        // minus the offset of no score: 2^(offset - any score in sight) is 0 against it
+#define LK_PA_SOME  2.0e38f        // the same for a column that sees keys, none of which had a weight yet
 
 // Two kinds of workgroup.  For up to 16 columns a kv head (STEP 16) the cache's bytes bound it: one workgroup a
 // CU, a ring of four tiles, so that 96 KB are on their way (64 sequences of up to 8192, 32 / 8 heads of 128, bf16: 213 us,
@@ -210,9 +211,10 @@ __device__ __forceinline__ int lk_here(int v) {
     return v;
 }
 
-// 1 / the sum of the weights; a row that sees nothing has the sum 0 and gets zeros.
-__device__ __forceinline__ float lk_pa_inverse(float l) {
-    return l == 0.0f ? 0.0f : 1.0f / l;
+// 1 / the sum l of the weights, m their offset.  Without any weight a row that sees nothing gets zeros, one that
+// sees keys of score -inf alone is no number.
+__device__ __forceinline__ float lk_pa_inverse(float l, float m) {
+    return l != 0.0f ? 1.0f / l : m > -LK_PA_NONE ? NAN : 0.0f;
 }
 
 // tanh of t: below 1/2 by its series (the difference of two numbers near 1 would lose what is
@@ -474,8 +476,9 @@ lk_k_paged_attn(const LkPaArgs) {
             // a wave reads its own words only
             const int limit = at.vis - base;                    // of the 64 tokens from base on the ones that have a slot
             const uint64_t lim = limit >= 64 ? ~0ull : limit > 0 ? (1ull << limit) - 1 : 0;
-            if (g == 0) s_see[w][cb][col] = (a.mask ? a.mask[row] : ~0ull >> (63 - ((at.c * a.qc + i) & 63))) & lim;
-            mneg[cb] = LK_PA_NONE;
+            const uint64_t see = (a.mask ? a.mask[row] : ~0ull >> (63 - ((at.c * a.qc + i) & 63))) & lim;
+            if (g == 0) s_see[w][cb][col] = see;
+            mneg[cb] = base > 0 || see != 0 ? LK_PA_SOME : LK_PA_NONE;
             accl[cb] = (lk_f4){ 0.f, 0.f, 0.f, 0.f };
 #pragma unroll
             for (int db = 0; db < DB; ++db) acc[cb][db] = (lk_f4){ 0.f, 0.f, 0.f, 0.f };
@@ -738,7 +741,7 @@ lk_k_paged_attn(const LkPaArgs) {
             int i, row, head;
             if (!column(a, cb, i, row, head)) continue;
             if (whole) {
-                const float il = lk_pa_inverse(accl[cb][0]);
+                const float il = lk_pa_inverse(accl[cb][0], -mneg[cb]);
                 RowT * o = (RowT *) a.out + (size_t) row * a.ldo + (size_t) head * D + 4 * g;
 #pragma unroll
                 for (int db = 0; db < DB; ++db) {
@@ -842,9 +845,9 @@ struct LkPaBlock {
     }
     // value e of dims 16 db ..: column e / 4, its dims 4 (e % 4) ..
     template <int D, typename RowT>
-    __device__ __forceinline__ void store(const LkPaArgs & a, const int4 & it, int db, int e, const lk_f4 & r, float l) const {
+    __device__ __forceinline__ void store(const LkPaArgs & a, const int4 & it, int db, int e, const lk_f4 & r, float l, float m) const {
         const int c = c0 + (e >> 2), t = c / a.g, head = ((it.w << a.hg_sh) + hh) * a.g + (c - t * a.g);
-        const float il = lk_pa_inverse(l), v[4] = { r[0] * il, r[1] * il, r[2] * il, r[3] * il };
+        const float il = lk_pa_inverse(l, m), v[4] = { r[0] * il, r[1] * il, r[2] * il, r[3] * il };
         lk_store<4>((RowT *) a.out + (size_t) (it.y + t) * a.ldo + (size_t) head * D + 16 * db + 4 * (e & 3), v);
     }
 };
@@ -901,7 +904,7 @@ lk_k_paged_join(const LkPaArgs a, int cb_n) {
         }
     }
 #pragma unroll
-    for (int i = 0; i < W; ++i) B.template store<D, typename LkElem<RT>::type>(a, it, db0 + i, lane, o[i], l);
+    for (int i = 0; i < W; ++i) B.template store<D, typename LkElem<RT>::type>(a, it, db0 + i, lane, o[i], l, m);
 }
 
 // Few items, cut into many pieces: workgroup (x, y) joins 16 dims of a block of the cut items number x,
@@ -1001,10 +1004,13 @@ lk_k_paged_spread(const LkPaArgs a, int cb_n, int wgs) {
         if (tid < 4 * B.live) {
             lk_f4 r = s_o[tid];
             for (int k = 8; k < pp; k += 8) r += s_o[(k << e_sh) + tid];
-            float sum = 0.0f;
+            float sum = 0.0f, mx = -LK_PA_NONE;
 #pragma unroll
-            for (int k = 0; k < NV; ++k) sum += s_r[1][k][tid >> 2];
-            B.template store<D, typename LkElem<RT>::type>(a, it, db, tid, r, sum);
+            for (int k = 0; k < NV; ++k) {
+                sum += s_r[1][k][tid >> 2];
+                mx = fmaxf(mx, s_r[0][k][tid >> 2]);
+            }
+            B.template store<D, typename LkElem<RT>::type>(a, it, db, tid, r, sum, mx);
         }
         __syncthreads();
     }

@@ -128,3 +128,28 @@ def test_queries_that_are_not_finite(lk, hq, hkv, d, t, value):
             if cap:
                 k.view(-1, hkv, d)[:, :, 9] = torch.where(k.view(-1, hkv, d)[:, :, 9] >= 0, 0.5, -0.5).to(k.dtype)
             _check(lk, f"a query of {value}, cap {cap}", b, q, k, v, t, hints, cap=cap)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hq,hkv,d", SHAPES)
+def test_rows_whose_scores_are_all_minus_infinity(lk, hq, hkv, d, t):
+    """No number, as the quotient of two sums of 0 is, however the keys are divided among workgroups; beside
+    it a row that sees nothing is zeros."""
+    for lens, news, hints in (([50, 900], [1, 1], (1, 64)), ([40000], [1], (1, 64)), ([0, 300], [20, 3], (1, 16, 64, 300))):
+        b = Batch(7, lens, news, 16)
+        k, v = pools(8, b, hkv, d, t)
+        k.view(-1, hkv, d)[:, :, 3] = -INF
+        q = _rows(9, b.rows * hq * d, TYPES[t]).view(b.rows, hq * d)
+        heads = q.view(b.rows, hq, d)
+        heads[:, :, 3] = heads[:, :, 3].abs() + 0.5
+        heads[0, 0, 3] = -1.0                                   # scores of +inf
+        # of the run of 20 rows, 4 see nothing and one a key that is finite
+        masks = [0 if i % 5 == 0 else 1 << i for i in range(b.rows)] if lens[0] == 0 else None
+        if masks:
+            k.view(-1, hkv, d)[b.slot(0, 6), :, 3] = 1.0
+        want = _check(lk, "scores of -inf", b, q, k, v, t, hints, masks=masks)
+        if masks:
+            assert bool((want[[0, 5, 10, 15]] == 0).all()) and bool(torch.isfinite(want[6]).all())
+            assert bool(torch.isnan(want[[1, 2, 3, 4, 7]]).all())
+        else:
+            assert bool(torch.isnan(want).all())
