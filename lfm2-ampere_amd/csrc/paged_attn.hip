@@ -435,7 +435,7 @@ lk_k_paged_attn(const LkPaArgs) {
             }
             const RowT * src = (const RowT *) a.q + (size_t) row * a.ldq + (size_t) head * D + 8 * g;
             if constexpr (TWO) {
-                // a head is scaled by a power of two to a largest finite value of 2^14 to 2^15, so that both parts are
+                // a head is scaled by a power of two to a largest value of 2^14 to 2^15, so that both parts are
                 // finite and 22 bits of it count whatever its size is, and its scores back
                 float v[KS][8], am = 0.0f;
 #pragma unroll
@@ -444,26 +444,24 @@ lk_k_paged_attn(const LkPaArgs) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         v[ks][e] = live ? v[ks][e] : 0.0f;
-                        am = fabsf(v[ks][e]) < INFINITY ? fmaxf(am, fabsf(v[ks][e])) : am;
+                        am = fmaxf(am, fabsf(v[ks][e]));
                     }
                 }
                 am = lk_xrow_max(am);
                 int e2 = 0;
-                if (am > 0.0f) {
+                if (am >= 0x1p-60f && am <= 3.4e38f) {         // (below, the scores' factor could vanish)
                     (void) frexpf(am, &e2);
-                    e2 = e2 - 15 > -74 ? e2 - 15 : -74;         // (below, the scores' factor could vanish)
+                    e2 -= 15;
                 }
                 fac[cb] = ldexpf(sc, e2);
-                // where the key's value is infinite the first part alone gives the score (finite_scores), so it is
-                // 0 where the value is 0 alone: below 2^-14 it is that, and the second part takes it back
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const float x = ldexpf(v[ks][e], -e2);
-                        const float h = (float) (T) (x != 0.0f && fabsf(x) < 0x1p-14f ? copysignf(0x1p-14f, x) : x);
-                        qh[cb][ks][e] = (T) h;
-                        ql[cb][ks][e] = (T) (fabsf(x) < INFINITY ? x - h : 0.0f);
+                        const T h = (T) x;
+                        qh[cb][ks][e] = h;
+                        ql[cb][ks][e] = (T) (x - (float) h);
                     }
             } else {
 #pragma unroll
@@ -507,25 +505,37 @@ lk_k_paged_attn(const LkPaArgs) {
         }
         return c;
     };
-    // An infinity among the keys times a second part, which is 0 or of either sign, is no number.  Scores that are not
-    // finite are those of the first part alone, of the value's sign.  (Finite ones are below 2^39: their sum is finite.)
-    auto finite_scores = [&](const V8 (&kf)[NB][KS], lk_f4 (&c)[CB][NB]) {
-        float all = 0.0f;
+    // fp32 rows: an infinity among the keys times a query's second part, which is 0 or of either sign, is no number, and
+    // the first part of a small value is 0.  Scores that are not finite are formed again from the signs of the
+    // query's finite values and its other values.
+    auto endless_scores = [&](const V8 (&kf)[NB][KS], lk_f4 (&c)[CB][NB]) {
+        const LkPaC & a = args();
 #pragma unroll
-        for (int cb = 0; cb < CB; ++cb)
+        for (int cb = 0; cb < CB; ++cb) {
+            int i, row, head;
+            const bool live = column(a, cb, i, row, head);
+            const RowT * src = (const RowT *) a.q + (size_t) row * a.ldq + (size_t) head * D + 8 * g;
+            lk_f4 o[NB];
 #pragma unroll
-            for (int n = 0; n < NB; ++n) all += (c[cb][n][0] + c[cb][n][1]) + (c[cb][n][2] + c[cb][n][3]);
-        if (__ballot(!(fabsf(all) < INFINITY)) == 0) return;    // wave-uniform
+            for (int n = 0; n < NB; ++n) o[n] = (lk_f4){ 0.f, 0.f, 0.f, 0.f };
 #pragma unroll
-        for (int cb = 0; cb < CB; ++cb)
+            for (int ks = 0; ks < KS; ++ks) {
+                float v[8];
+                V8 q;
+                lk_load<8>(src + 32 * ks, v);
 #pragma unroll
-            for (int n = 0; n < NB; ++n) {
-                lk_f4 o = { 0.f, 0.f, 0.f, 0.f };
+                for (int e = 0; e < 8; ++e) {
+                    const float x = live ? v[e] : 0.0f;
+                    q[e] = (T) (x != 0.0f && fabsf(x) < INFINITY ? copysignf(1.0f, x) : x);
+                }
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) o = M::k32(kf[n][ks], qh[cb][ks], o);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) c[cb][n][r] = fabsf(c[cb][n][r]) < INFINITY ? c[cb][n][r] : o[r];
+                for (int n = 0; n < NB; ++n) o[n] = M::k32(kf[n][ks], q, o[n]);
             }
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) c[cb][n][r] = fabsf(c[cb][n][r]) < INFINITY ? c[cb][n][r] : o[n][r];
+        }
     };
     auto factor = [&](int cb) -> float { return TWO ? fac[cb] : sc; };
     // capped and biased scores in units of log2, of keys k0 .. k0 + 3 (k0: the lane's first)
@@ -574,7 +584,12 @@ lk_k_paged_attn(const LkPaArgs) {
         p -= h;
         pl = __builtin_convertvector(p, V4);
     };
-    auto top4 = [&](const lk_f4 & c) -> float { return fmaxf(fmaxf(c[0], c[1]), fmaxf(c[2], c[3])); };
+    // (of fp32 rows' scores NaN is the largest)
+    auto larger = [](float x, float y) -> float {
+        if constexpr (TWO) return __builtin_elementwise_maximum(x, y);
+        else               return fmaxf(x, y);
+    };
+    auto top4 = [&](const lk_f4 & c) -> float { return larger(larger(c[0], c[1]), larger(c[2], c[3])); };
     auto units = [&](float top, int cb) -> float { return MOD ? top : top * factor(cb); };
     auto join = [](const V4 & x, const V4 & y) -> V8 { return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7); };
     V4 ones4;
@@ -601,19 +616,16 @@ lk_k_paged_attn(const LkPaArgs) {
         for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
             for (int n = 0; n < NB; ++n) c[cb][n] = scores(kf[n], cb);
-        if constexpr (TWO) finite_scores(kf, c);
         if (more) kload(kt + (STEP << rb_sh), kf);
-        if constexpr (MOD) {
+        auto shape = [&]() {
+            if constexpr (MOD) {
 #pragma unroll
-            for (int cb = 0; cb < CB; ++cb)
+                for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
-                for (int n = 0; n < NB; ++n) shaped(c[cb][n], cb, key0 + 16 * n + 4 * g);
-        }
-        // the softmax first: of the two waves of a SIMD one then multiplies while the other forms weights (2 x 4096 new
-        // tokens 210 -> 200 us; no other order of the two parts' instructions within a wave gained anything)
-        if constexpr (STEP == 32) __builtin_amdgcn_s_setprio(1);
-        bool odd = false;                                       // an infinity or NaN among the values
-        if (some) {
+                    for (int n = 0; n < NB; ++n) shaped(c[cb][n], cb, key0 + 16 * n + 4 * g);
+            }
+        };
+        auto hide = [&]() {
 #pragma unroll
             for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
@@ -622,6 +634,14 @@ lk_k_paged_attn(const LkPaArgs) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) c[cb][n][r] = (bits >> r) & 1 ? c[cb][n][r] : -INFINITY;
                 }
+        };
+        shape();
+        // the softmax first: of the two waves of a SIMD one then multiplies while the other forms weights (2 x 4096 new
+        // tokens 210 -> 200 us; no other order of the two parts' instructions within a wave gained anything)
+        if constexpr (STEP == 32) __builtin_amdgcn_s_setprio(1);
+        bool odd = false;                                       // an infinity or NaN among the values
+        if (some) {
+            hide();
             // 0 times an infinity is NaN: such values are left out of the product, and added behind it
 #pragma unroll
             for (int db = 0; db < DB; ++db)
@@ -639,12 +659,30 @@ lk_k_paged_attn(const LkPaArgs) {
             odd = __ballot(odd) != 0;                           // wave-uniform
         }
         // one test for all blocks of columns says whether a max has to be raised
-        float top[CB], over = -INFINITY;
+        float top[CB], over;
+        auto tops = [&]() {
+            over = -INFINITY;
 #pragma unroll
-        for (int cb = 0; cb < CB; ++cb) {
-            top[cb] = top4(c[cb][0]);
-            if constexpr (NB == 2) top[cb] = fmaxf(top[cb], top4(c[cb][1]));
-            over = fmaxf(over, MOD ? top[cb] + mneg[cb] : __builtin_fmaf(top[cb], factor(cb), mneg[cb]));
+            for (int cb = 0; cb < CB; ++cb) {
+                top[cb] = top4(c[cb][0]);
+                if constexpr (NB == 2) top[cb] = larger(top[cb], top4(c[cb][1]));
+                over = larger(over, MOD ? top[cb] + mneg[cb] : __builtin_fmaf(top[cb], factor(cb), mneg[cb]));
+            }
+        };
+        tops();
+        if constexpr (TWO) {
+            if (__ballot(over != over)) {                       // wave-uniform
+                V8 kx[NB][KS];
+                kload(kt, kx);
+#pragma unroll
+                for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) c[cb][n] = scores(kx[n], cb);
+                endless_scores(kx, c);
+                shape();
+                if (some) hide();
+                tops();
+            }
         }
         if (__ballot(over > LK_PA_HEADROOM)) {                  // wave-uniform
 #pragma unroll
