@@ -89,7 +89,7 @@ struct LkPaArgs {
     const uint64_t * mask;
     const float * slopes;
     float * acc;                   // partials: [2 * run + end][block of columns][D / 16][column][4][4 dims]
-    float2 * ml;                   // and their (max, sum): [..][..][16]
+    float2 * ml;                   // and their (max, sum; lk_pa_factor): [..][..][16]
     int4 * cut;                    // per run the cut item that begins in it: (pieces, first row, rows, kv head group)
     int ldq, ldo, n_seqs, rows, ldt, width, page_sh, n_pages;
     int hkv, g;                    // g = query heads a kv head
@@ -211,6 +211,10 @@ __device__ __forceinline__ int lk_here(int v) {
     return v;
 }
 
+// The factor f of a piece's rows where they are joined, l its sum of weights: with the sign bit set (which the
+// joins take off) there are infinities among the rows, and the factor is above 0, as their weights are.
+__device__ __forceinline__ float lk_pa_factor(float f, float l) { return signbit(l) ? fmaxf(f, 0x1p-149f) : f; }
+
 // 1 / the sum l of the weights, m their offset.  Without any weight a row that sees nothing gets zeros, one that
 // sees keys of score -inf alone is no number.
 __device__ __forceinline__ float lk_pa_inverse(float l, float m) {
@@ -270,6 +274,8 @@ lk_k_paged_attn(const LkPaArgs) {
     __shared__ lk_f4 s_x[2][NW][64];                           // key shares' rows on their way to one wave
     __shared__ float2 s_ml[NW][16];
     __shared__ uint64_t s_see[NW][CB][16];                     // which of the 64 tokens from `base` on a column sees
+    __shared__ int s_left[NW], s_start[NW][4];                 // a wave's left_out; the run's first item and tile
+    __shared__ long s_places[NW];                              // and its places from there on, of which each wave keeps a copy
 
     const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -400,6 +406,7 @@ lk_k_paged_attn(const LkPaArgs) {
     int qpos[MOD ? CB : 1];
     int base = 0;                                               // keys below it are seen by all of the chunk's rows
     bool busy = false;                                          // the wave has columns
+    bool left_out = false;                                      // the run met infinities or NaN of V (or a row of NaN)
     // column block cb: the token of the chunk, its row of the step, its query head; false: there is none
     auto column = [&](const LkPaC & a, int cb, int & i, int & row, int & head) -> bool {
         const int c = (qw * CB + cb) * 16 + lk_here(col), i0 = at.c * a.qc, m = at.s.n - i0 < a.qc ? at.s.n - i0 : a.qc;
@@ -413,6 +420,16 @@ lk_k_paged_attn(const LkPaArgs) {
     };
     float sc = 0.0f, cap = 0.0f, inv_cap = 0.0f;                // scale (times log2(e) but for MOD), cap
     bool biased = false;
+    // the item's `base`, and the tokens from it on that a column sees
+    auto set_base = [&](const LkPaC & a) {
+        const int blk = (at.c * a.qc) & ~63, slots = a.width << a.page_sh;
+        base = at.s.len + blk < slots ? at.s.len + blk : slots;
+    };
+    auto seen = [&](const LkPaC & a, int i, int row) -> uint64_t {
+        const int limit = at.vis - base;                        // of the 64 tokens from base on the ones that have a slot
+        const uint64_t lim = limit >= 64 ? ~0ull : limit > 0 ? (1ull << limit) - 1 : 0;
+        return (a.mask ? a.mask[row] : ~0ull >> (63 - ((at.c * a.qc + i) & 63))) & lim;
+    };
     auto begin = [&]() {
         const LkPaC & a = args();
         sc = MOD ? a.scale : a.sc;
@@ -421,8 +438,7 @@ lk_k_paged_attn(const LkPaArgs) {
             inv_cap = a.inv_cap;
             biased = a.slopes != nullptr;
         }
-        const int blk = (at.c * a.qc) & ~63, slots = a.width << a.page_sh;
-        base = at.s.len + blk < slots ? at.s.len + blk : slots;
+        set_base(a);
         busy = false;
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) {
@@ -471,10 +487,7 @@ lk_k_paged_attn(const LkPaArgs) {
                     qh[cb][ks] = live ? v : V8{};
                 }
             }
-            // a wave reads its own words only
-            const int limit = at.vis - base;                    // of the 64 tokens from base on the ones that have a slot
-            const uint64_t lim = limit >= 64 ? ~0ull : limit > 0 ? (1ull << limit) - 1 : 0;
-            const uint64_t see = (a.mask ? a.mask[row] : ~0ull >> (63 - ((at.c * a.qc + i) & 63))) & lim;
+            const uint64_t see = seen(a, i, row);               // (a wave reads its own words only)
             if (g == 0) s_see[w][cb][col] = see;
             mneg[cb] = base > 0 || see != 0 ? LK_PA_SOME : LK_PA_NONE;
             accl[cb] = (lk_f4){ 0.f, 0.f, 0.f, 0.f };
@@ -639,10 +652,11 @@ lk_k_paged_attn(const LkPaArgs) {
         // the softmax first: of the two waves of a SIMD one then multiplies while the other forms weights (2 x 4096 new
         // tokens 210 -> 200 us; no other order of the two parts' instructions within a wave gained anything)
         if constexpr (STEP == 32) __builtin_amdgcn_s_setprio(1);
-        bool odd = false;                                       // an infinity or NaN among the values
         if (some) {
             hide();
-            // 0 times an infinity is NaN: such values are left out of the product, and added behind it
+            // 0 times an infinity is NaN: such values are left out of the product, which would spoil the rows that
+            // do not see them, and added at the run's end
+            bool odd = false;
 #pragma unroll
             for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -656,7 +670,7 @@ lk_k_paged_attn(const LkPaArgs) {
                     }
                     vf[db][n] = __builtin_bit_cast(V4, u);
                 }
-            odd = __ballot(odd) != 0;                           // wave-uniform
+            left_out |= __ballot(odd) != 0;                     // wave-uniform
         }
         // one test for all blocks of columns says whether a max has to be raised
         float top[CB], over;
@@ -710,26 +724,6 @@ lk_k_paged_attn(const LkPaArgs) {
             for (int db = 0; db < DB; ++db) acc[cb][db] = product(vf[db], acc[cb][db]);
         }
         if constexpr (STEP == 32) __builtin_amdgcn_s_setprio(0);
-        if (odd) {
-            // one key after the other, and only the columns that see it
-#pragma unroll
-            for (int n = 0; n < NB; ++n)
-#pragma clang loop unroll(disable)
-                for (int k = 0; k < 16; ++k) {
-                    const int d = key0 + 16 * n + k - base;
-#pragma unroll
-                    for (int db = 0; db < DB; ++db) {
-                        lk_u16x4 u = __builtin_bit_cast(lk_u16x4, vload(vt, n, db));
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) u[r] = 4 * g + r == k && (u[r] & M::INF) == M::INF ? u[r] : 0;
-#pragma unroll
-                        for (int cb = 0; cb < CB; ++cb) {
-                            const lk_f4 o = M::k16(__builtin_bit_cast(V4, u), ph[cb][n], (lk_f4){ 0.f, 0.f, 0.f, 0.f });
-                            if (d < 0 || (d < 64 && ((s_see[w][cb][col] >> d) & 1))) acc[cb][db] += o;
-                        }
-                    }
-                }
-        }
     };
 
     // ---- an item's end, or the run's ----------------------------------------------------------
@@ -739,7 +733,11 @@ lk_k_paged_attn(const LkPaArgs) {
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) {
             if (g == 0) s_ml[w][col] = make_float2(-mneg[cb], accl[cb][0]);
+            if (lane == 0) s_left[w] = left_out;
             __syncthreads();
+            int met = 0;
+            for (int k = 0; k < kws; ++k) met |= s_left[w - kw + k];
+            left_out = __builtin_amdgcn_readfirstlane(met) != 0;
             float mx = -mneg[cb];
             for (int k = 0; k < kws; ++k) mx = fmaxf(mx, s_ml[w - kw + k][col].x);
             const float f = lk_exp2(-mneg[cb] - mx);
@@ -771,6 +769,14 @@ lk_k_paged_attn(const LkPaArgs) {
     auto finish = [&](bool whole, bool from_first) {
         if (kw_sh) join_shares();
         if (kw != 0) return;
+        lk_f4 all = { 0.f, 0.f, 0.f, 0.f };                     // NaN with an infinity or NaN among the sums
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) all[r] = __builtin_fmaf(acc[cb][db][r], 0.0f, all[r]);
+        left_out |= __ballot((all[0] + all[1]) + (all[2] + all[3]) != 0.0f) != 0;        // wave-uniform
         const LkPaC & a = args();
         const int nblk = CB << (a.qw_sh + a.hg_sh);
         const int slot = 2 * wgi + from_first;
@@ -783,7 +789,11 @@ lk_k_paged_attn(const LkPaArgs) {
                 RowT * o = (RowT *) a.out + (size_t) row * a.ldo + (size_t) head * D + 4 * g;
 #pragma unroll
                 for (int db = 0; db < DB; ++db) {
-                    const float v[4] = { acc[cb][db][0] * il, acc[cb][db][1] * il, acc[cb][db][2] * il, acc[cb][db][3] * il };
+                    float v[4] = { acc[cb][db][0] * il, acc[cb][db][1] * il, acc[cb][db][2] * il, acc[cb][db][3] * il };
+                    if (left_out) {                             // NaN by the values, not by the scores: marked for add_endless
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) v[r] = v[r] == v[r] ? v[r] : il == il ? -NAN : NAN;
+                    }
                     lk_store<4>(o + 16 * db, v);
                 }
             } else {
@@ -805,6 +815,10 @@ lk_k_paged_attn(const LkPaArgs) {
             if (threadIdx.x == 0) args().cut[wgi] = make_int4(0, 0, 0, 0);
             return;
         }
+    }
+    if (lane == 0) {
+        s_start[w][0] = at.b, s_start[w][1] = at.c, s_start[w][2] = at.h, s_start[w][3] = at.t;
+        s_places[w] = left;
     }
     LkPaAt ft = at;                                             // the next tile to fetch
     long ft_left = left;                                        // places of the run from it on
@@ -869,6 +883,104 @@ lk_k_paged_attn(const LkPaArgs) {
         if (left > 0) lk_pa_next(args(), at, tk_sh);
     }
     if (threadIdx.x == 0) args().cut[wgi] = cut;
+
+    // ---- infinities and NaN of V, where the run met any ---------------------------------------
+    // In the products above they were left out, or met a second part of a weight, which may be 0 or of either sign, a weight
+    // that is 0 in the pools' type, or a factor of 0.  The results of the dims in which a column sees some are formed
+    // again here from them alone, since nothing finite is left beside them: each counts as it is, its weight
+    // being above 0, but for a score of -inf, whose weight is 0 and 0 times it NaN.  (Such a key has an infinite value itself and
+    // its score no cap; an infinite query makes its whole row NaN anyway.)  The run's V is scanned once more, behind all
+    // that the usual call does (at each item's end these lines took scalar registers from the products' loop:
+    // 64 sequences of up to 8192 323 us for 222).
+    if (kw != 0 || !left_out) return;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");      // what the wave's lanes wrote is read and written again
+    const LkPaC & a = args();
+    at.b = __builtin_amdgcn_readfirstlane(s_start[w][0]);
+    at.c = __builtin_amdgcn_readfirstlane(s_start[w][1]);
+    at.h = __builtin_amdgcn_readfirstlane(s_start[w][2]);
+    at.t = __builtin_amdgcn_readfirstlane(s_start[w][3]);
+    left = lk_uniform64(s_places[w]);
+    at.s = lk_seq(lk_sld(a.first, at.b), lk_sld(a.first, at.b + 1), lk_sld(a.lens, at.b), a.rows, a.width << a.page_sh);
+    at.row = a.table + (long) at.b * a.ldt;
+    lk_pa_item(a, at, tk_sh);
+    auto endless = [](uint16_t u) -> bool { return (u & M::INF) == M::INF; };
+    while (left > 0) {
+        const int t0 = at.t, t1 = left < at.nt - t0 ? t0 + (int) left : at.nt;
+        const int end = (t1 << tk_sh) < at.vis ? t1 << tk_sh : at.vis, m = (1 << a.page_sh) - 1;
+        set_base(a);
+#pragma clang loop unroll(disable)
+        for (int cb = 0; cb < CB; ++cb) {
+            int i, row, head;
+            const bool live = column(a, cb, i, row, head);
+            const uint64_t see = seen(a, i, row);
+            lk_f4 sum[DB];
+            uint32_t found = 0;                                 // a bit for each of the lane's dims
+#pragma unroll
+            for (int db = 0; db < DB; ++db) sum[db] = (lk_f4){ 0.f, 0.f, 0.f, 0.f };
+#pragma clang loop unroll(disable)
+            for (int k0 = t0 << tk_sh; k0 < end; k0 += 4) {     // four keys of a page at once
+                const int page = lk_sld(at.row, k0 >> a.page_sh);
+                if (page < 0 || page >= a.n_pages) continue;
+                const size_t row0 = (((size_t) page << a.page_sh) + (k0 & m)) * row_bytes + ((size_t) at.h << rb_sh) + hh * (D * 2);
+                auto values = [&](int j, lk_u16x4 (&u)[DB]) -> bool {
+                    bool odd = false;
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) u[db] = *(const lk_u16x4 *) (a.vp + row0 + (size_t) j * row_bytes + 32 * db + 8 * g);
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) odd |= endless(u[db][0]) || endless(u[db][1]) || endless(u[db][2]) || endless(u[db][3]);
+                    return odd;
+                };
+                lk_u16x4 u0[DB], u1[DB], u2[DB], u3[DB];
+                const bool o0 = values(0, u0), o1 = values(1, u1), o2 = values(2, u2), o3 = values(3, u3);
+                if (__ballot(o0 || o1 || o2 || o3) == 0) continue;        // wave-uniform
+#pragma clang loop unroll(disable)
+                for (int k = k0; k < k0 + 4 && k < end; ++k) {
+                    if (__ballot(values(k - k0, u0)) == 0) continue;
+                    bool none = false;                          // the key's score is -inf, if it is not +inf or NaN
+                    if (!(a.cap > 0.0f)) {
+                        const uint16_t * key = (const uint16_t *) (a.kp + row0 + (size_t) (k - k0) * row_bytes);
+#pragma unroll
+                        for (int e = 0; e < D / 64; ++e) none |= endless(key[lane + 64 * e]);
+                        none = __ballot(none) != 0;
+                    }
+                    const int d = k - base;
+                    if (!(d < 0 || (d < 64 && ((see >> d) & 1)))) continue;
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) {
+                        const V4 v = __builtin_bit_cast(V4, u0[db]);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (endless(u0[db][r])) {
+                                sum[db][r] += none ? NAN : (float) v[r];
+                                found |= 1u << (4 * db + r);
+                            }
+                    }
+                }
+            }
+            if (!live || found == 0) continue;
+            const bool whole = t0 == 0 && t1 == at.nt;
+            RowT * o = (RowT *) a.out + (size_t) row * a.ldo + (size_t) head * D + 4 * g;
+            const size_t blk = (size_t) (2 * wgi + (t0 == 0)) * (CB << (a.qw_sh + a.hg_sh)) + ((hh << a.qw_sh) + qw) * CB + cb;
+            if (!whole) {                                       // (lanes of a column write the same)
+                float * const l = &a.ml[blk * 16 + col].y;
+                *l = copysignf(*l, -1.0f);
+            }
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    if (((found >> (4 * db + r)) & 1) == 0) continue;
+                    if (whole) {                                // but for rows that the scores made NaN
+                        const float was = (float) o[16 * db + r];
+                        if (was == was || signbit(was)) o[16 * db + r] = (RowT) sum[db][r];
+                    } else {
+                        a.acc[((blk * DB + db) * 64 + col * 4 + g) * 4 + r] = sum[db][r];
+                    }
+                }
+        }
+        left -= t1 - t0 + extra;
+        if (left > 0) lk_pa_next(a, at, tk_sh);
+    }
 }
 
 // ---- joining cut items ------------------------------------------------------------------------
@@ -904,7 +1016,7 @@ lk_k_paged_join(const LkPaArgs a, int cb_n) {
     const int blk = blockIdx.y, nblk = gridDim.y;
     const LkPaBlock B(a, it, blk, cb_n);
     if (lane >= 4 * B.live) return;
-    float m = -LK_PA_NONE, l = 0.0f;
+    float m = -LK_PA_NONE, l = 0.0f, odd = 0.0f;               // odd: its sign, of the pieces so far
     lk_f4 o[W];
 #pragma unroll
     for (int i = 0; i < W; ++i) o[i] = (lk_f4){ 0.f, 0.f, 0.f, 0.f };
@@ -930,15 +1042,18 @@ lk_k_paged_join(const LkPaArgs a, int cb_n) {
         for (int j = 0; j < NP; ++j) mx = fmaxf(mx, ml[j].x);
         const float f = lk_exp2(m - mx);
         m = mx;
+        const float fo = lk_pa_factor(f, odd);
         l *= f;
 #pragma unroll
-        for (int i = 0; i < W; ++i) o[i] *= f;
+        for (int i = 0; i < W; ++i) o[i] *= fo;
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
             const float fj = lk_exp2(ml[j].x - mx);
-            l = __builtin_fmaf(ml[j].y, fj, l);
+            l = __builtin_fmaf(fabsf(ml[j].y), fj, l);
+            const float fx = lk_pa_factor(fj, ml[j].y);
+            odd = signbit(ml[j].y) ? ml[j].y : odd;
 #pragma unroll
-            for (int i = 0; i < W; ++i) o[i] += x[j][i] * fj;
+            for (int i = 0; i < W; ++i) o[i] += x[j][i] * fx;
         }
     }
 #pragma unroll
@@ -1015,8 +1130,8 @@ lk_k_paged_spread(const LkPaArgs a, int cb_n, int wgs) {
         for (int j = 0; j < NP; ++j) {
             const int k = (tid >> 4) + j * (NT / 16);
             const float f = lk_exp2(ml[j].x - m);
-            if (k < it.x) s_w[k][col] = f;
-            l = __builtin_fmaf(ml[j].y, f, l);
+            if (k < it.x) s_w[k][col] = lk_pa_factor(f, ml[j].y);
+            l = __builtin_fmaf(fabsf(ml[j].y), f, l);
         }
         l = lk_xrow_sum(l);
         if (lane < 16) s_r[1][v][col] = l;

@@ -153,3 +153,61 @@ def test_rows_whose_scores_are_all_minus_infinity(lk, hq, hkv, d, t):
             assert bool(torch.isnan(want[[1, 2, 3, 4, 7]]).all())
         else:
             assert bool(torch.isnan(want).all())
+
+
+def _spoiled(b, v, s, at, dims, value):
+    v.view(-1, *v.shape[2:])[b.slot(s, at), 0, dims] = value
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hq,hkv,d", SHAPES)
+@pytest.mark.parametrize("lens,news,hints", [([50, 900], [1, 1], (1, 64)), ([50, 300], [20, 3], (1, 16, 64, 300)), ([40000], [1], (1, 64)),
+                                             ([200] * 40, [1] * 40, (1,)), ([60] * 30, [9] * 30, (16,)), ([5000], [130], (130,))])
+def test_infinite_values(lk, hq, hkv, d, t, lens, news, hints):
+    """Each dim of the output is the sum of the infinities and NaN that the row sees there, in earlier and in new
+    positions, alone or several; the other dims, heads and rows do not notice."""
+    if sum(lens) * hq > 400000:
+        hq, hkv = 2, 1
+    b = Batch(11, lens, news, 16)
+    k, v = pools(12, b, hkv, d, t)
+    for s in range(0, len(lens), 3):
+        a, n = lens[s], news[s]
+        _spoiled(b, v, s, 7, 5, INF)
+        _spoiled(b, v, s, a - 1, 6, -INF)
+        _spoiled(b, v, s, a, 17, INF)                           # a new token
+        _spoiled(b, v, s, a + n - 1, 18, -INF)                  # the last one: of a run its own row alone sees it
+        _spoiled(b, v, s, 20, 33, math.nan)
+        _spoiled(b, v, s, a // 2, 34, INF)                      # two of one sign, two of both
+        _spoiled(b, v, s, a // 2 + 9, 34, INF)
+        _spoiled(b, v, s, a // 2, 63, INF)
+        _spoiled(b, v, s, a // 2 + 9, 63, -INF)
+        _spoiled(b, v, s, 30, [0, d - 1], 1e30 if t == "bf16" else 6e4)
+    q = _rows(13, b.rows * hq * d, TYPES[t]).view(b.rows, hq * d)
+    want = _check(lk, "infinite values", b, q, k, v, t, hints)
+    assert bool((want[0, 0, [5, 34]] == INF).all()) and float(want[0, 0, 6]) == -INF and math.isnan(float(want[0, 0, 33]))
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hq,hkv,d", SHAPES)
+@pytest.mark.parametrize("gap", [12.0, 80.0, 400.0])
+def test_infinite_values_of_small_weights(lk, hq, hkv, d, t, gap):
+    """A weight e^-gap of the largest, far below what its type or fp32 holds, is above 0: its infinity counts.  One of a
+    score of -inf makes the dim NaN."""
+    for lens, news, hints in (([50, 900], [1, 1], (1, 64)), ([50, 300], [20, 3], (1, 16, 64, 300)), ([9000], [1], (1, 64))):
+        b = Batch(14, lens, news, 16)
+        k, v = pools(15, b, hkv, d, t)
+        flat = k.view(-1, hkv, d)
+        for s in range(len(lens)):
+            a, n = lens[s], news[s]
+            for at, dim in ((3, 40), (a - 1, 41), (a, 42), (a // 2, 43)):
+                flat[b.slot(s, at), 0, 0] = -gap
+                _spoiled(b, v, s, at, dim, INF)
+            if gap > 100:
+                flat[b.slot(s, 30), 0, 1] = -INF
+                _spoiled(b, v, s, 30, 50, -INF)
+        q = _rows(16, b.rows * hq * d, TYPES[t], 0.1).view(b.rows, hq * d)
+        q.view(b.rows, hq, d)[:, :, 0] = 4.0
+        q.view(b.rows, hq, d)[:, :, 1] = 0.5
+        want = _check(lk, f"weights of e^-{gap}", b, q, k, v, t, hints)
+        assert bool((want[:, 0, [40, 41, 43]] == INF).all())
+        assert gap < 100 or bool(torch.isnan(want[:, 0, 50]).all())
