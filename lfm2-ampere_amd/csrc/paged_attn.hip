@@ -24,11 +24,10 @@
 #include "lk_paged.h"
 
 #define LK_PA_TILEB 32768          // a tile: K rows, then V rows
-// Weights are 2^(score - offset).  The offset is set to 2^-LK_PA_LIFT of the largest score and raised when a score
-// passes it by 2^LK_PA_HEADROOM, so that the largest weight is 2^7 to 2^15: in fp16, whose steps below 2^-14 are
-// 2^-24 whatever the value, a weight keeps its 11 bits down to 2^-21 of the row's first maximum.
-#define LK_PA_LIFT 7.0f
-#define LK_PA_HEADROOM 15.0f
+// Weights are 2^(score - offset).  The offset is set so that the largest weight is 2^LIFT, and raised when one passes
+// 2^HEADROOM.  In fp16, whose steps below 2^-14 are 2^-24 whatever the value, the largest is 2^7 to 2^15, so that
+// a weight keeps its 11 bits down to 2^-21 of the row's first maximum.  In bf16, whose values reach the end of fp32,
+// it is 2^-8 to 1: a weight times a value stays finite.
 #define LK_PA_NONE  3.0e38f        // minus the offset of no score: 2^(offset - any score in sight) is 0 against it
 #define LK_PA_SOME  2.0e38f        // the same for a column that sees keys, none of which had a weight yet
 
@@ -63,6 +62,7 @@ template <> struct LkMm<LK_F16> {
 #endif
     static constexpr uint16_t INF = 0x7C00;
     static constexpr uint32_t LEAD = 0xFFFFE000;               // the bits of an fp32 number that the type holds
+    static constexpr float LIFT = 7.0f, HEADROOM = 15.0f;
 };
 template <> struct LkMm<LK_BF16> {
     typedef __bf16 T;
@@ -79,6 +79,7 @@ template <> struct LkMm<LK_BF16> {
 #endif
     static constexpr uint16_t INF = 0x7F80;
     static constexpr uint32_t LEAD = 0xFFFF0000;
+    static constexpr float LIFT = -8.0f, HEADROOM = 0.0f;
 };
 
 struct LkPaArgs {
@@ -571,10 +572,10 @@ lk_k_paged_attn(const LkPaArgs) {
     };
     // raises the offset of column block cb to cover a lane's largest score (units of log2)
     auto raise = [&](int cb, float top) {
-        if (__ballot(top + mneg[cb] > LK_PA_HEADROOM)) {        // wave-uniform (a difference: exact for large scores)
+        if (__ballot(top + mneg[cb] > M::HEADROOM)) {        // wave-uniform (a difference: exact for large scores)
             const float mx = lk_xrow_max(top);
-            if (mx + mneg[cb] > LK_PA_HEADROOM) {
-                const float to = LK_PA_LIFT - mx, f = lk_exp2(to - mneg[cb]);
+            if (mx + mneg[cb] > M::HEADROOM) {
+                const float to = M::LIFT - mx, f = lk_exp2(to - mneg[cb]);
                 mneg[cb] = to;
 #pragma unroll
                 for (int db = 0; db < DB; ++db) acc[cb][db] *= f;
@@ -698,7 +699,7 @@ lk_k_paged_attn(const LkPaArgs) {
                 tops();
             }
         }
-        if (__ballot(over > LK_PA_HEADROOM)) {                  // wave-uniform
+        if (__ballot(over > M::HEADROOM)) {                  // wave-uniform
 #pragma unroll
             for (int cb = 0; cb < CB; ++cb) raise(cb, units(top[cb], cb));
         }

@@ -211,3 +211,14 @@ def test_infinite_values_of_small_weights(lk, hq, hkv, d, t, gap):
         want = _check(lk, f"weights of e^-{gap}", b, q, k, v, t, hints)
         assert bool((want[:, 0, [40, 41, 43]] == INF).all())
         assert gap < 100 or bool(torch.isnan(want[:, 0, 50]).all())
+
+
+@pytest.mark.parametrize("hq,hkv,d", SHAPES)
+def test_values_near_the_end_of_the_type(lk, hq, hkv, d):
+    """bf16 values up to 2^125, whose weighted sums are finite: no weight is above 1."""
+    for b, hints in _batches():
+        k, v = pools(17, b, hkv, d, "bf16")
+        v = v.float().clamp(-4, 4).mul(2.0 ** 123).bfloat16()
+        q = _rows(18, b.rows * hq * d, TYPES["bf16"]).view(b.rows, hq * d)
+        want = _check(lk, "large values", b, q, k, v, "bf16", hints, scale=0.25)
+        assert bool(torch.isfinite(want).all())
