@@ -227,7 +227,8 @@ __device__ __forceinline__ float lk_pa_inverse(float l, float m) {
 // reciprocal (1 ulp): three half steps of the value, where an IEEE division costs ten instructions more.
 __device__ __forceinline__ float lk_tanh(float t) {
     const float u = fabsf(t), z = t * t;
-    float p = 21844.0f / 6081075.0f;
+    float p = 929569.0f / 638512875.0f;
+    p = __builtin_fmaf(-p, z, 21844.0f / 6081075.0f);
     p = __builtin_fmaf(-p, z, 1382.0f / 155925.0f);
     p = __builtin_fmaf(-p, z, 62.0f / 2835.0f);
     p = __builtin_fmaf(-p, z, 17.0f / 315.0f);
