@@ -573,7 +573,9 @@ typedef struct lk_step {
     int ldt, width;
     const int32_t * pos;            /* [rows] positions of the new tokens, or NULL: lens[b] + i */
     const uint64_t * mask;          /* [rows] which new tokens a row sees, or NULL: causal */
-    int max_new;                    /* the largest n_b, for the choice of a kernel only (0: unknown) */
+    int max_new;                    /* the largest n_b, for the choice of a kernel only (0: unknown;
+                                       lk_paged_attn then takes rows / n_seqs, rounded up, where work has
+                                       the lk_paged_attn_work_bytes() of that, and 1 where not) */
 } lk_step;
 
 /* Per row: q and k heads normed and rotated, q to qo, k and v to the row's slot.

@@ -1271,9 +1271,15 @@ extern "C" int lk_paged_attn(const lk_pages * pages, const lk_step * step, int t
     const uintptr_t em = (uintptr_t) lk_type_size(type) - 1;
     if ((((uintptr_t) q | (uintptr_t) out) & em) || ((uintptr_t) slopes & 3) || ((uintptr_t) work & 15))
         return lk_fail(hipErrorInvalidValue, "%s: misaligned argument (rows by their element, slopes 4 B, work 16 B)", W);
-    const size_t need = lk_paged_attn_work_bytes(pages, type, step->max_new);
+    // max_new 0: the mean, where the workspace has room for its kernel (a prompt of 4096: 190 us, as single tokens 798)
+    int most = step->max_new;
+    if (most == 0) {
+        most = (step->rows - 1) / step->n_seqs + 1;
+        if (work_bytes < lk_paged_attn_work_bytes(pages, type, most)) most = 1;
+    }
+    const size_t need = lk_paged_attn_work_bytes(pages, type, most);
     if (work_bytes < need) return lk_fail(hipErrorInvalidValue, "%s: workspace of %zu bytes, %zu needed", W, work_bytes, need);
-    const LkPaShape s = lk_pa_shape(pages, type, step->max_new);
+    const LkPaShape s = lk_pa_shape(pages, type, most);
     const int nblk = lk_pa_blocks(s), g = hq / pages->n_kv_heads, nhg = pages->n_kv_heads >> s.hg_sh;
     const size_t blocks = (size_t) 2 * lk_pa_wgs(s.step) * nblk;
     float * acc = (float *) work;

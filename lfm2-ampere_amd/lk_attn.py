@@ -706,7 +706,7 @@ class PagedStep:
     """A step's tables (lk_step), shared by all layers: first int32 [n_seqs + 1], lens int32
     [n_seqs], table int32 [n_seqs][pages], `rows` rows of new tokens; pos int32 [rows] and
     mask int64 [rows] (64 bits a row) where given; max_new, the largest number of new tokens a
-    sequence has, chooses a kernel.  The tables are read on the device during each call, so a
+    sequence has, chooses a kernel (0: by rows a sequence).  The tables are read on the device during each call, so a
     captured call goes on with what they hold when it is replayed.
     Keeps the tables and the attention's workspace, made at its first use (or `work`, uint8 of
     PagedCache.work_bytes()): attention calls on a step must be ordered (one stream, or
@@ -731,6 +731,7 @@ class PagedStep:
         self._ref = ctypes.addressof(self._desc)
         self._keep = (first, lens, table, pos, mask)
         self._dev, self.n_seqs, self.rows, self.max_new = dev, B, int(rows), int(max_new)
+        self._most = self.max_new or (-(-self.rows // B) if B else 0)       # what lk_paged_attn takes for an unknown one
         self._work, self._own, self._streams, self._old = work, False, set(), []
 
     def _workspace(self, n: int, stream):
@@ -826,7 +827,7 @@ class PagedCache:
         ps = None if slopes is None else _flat(slopes, (self._hq // self._d,), _torch.float32, dev, "PagedCache.attend: slopes")
         if step._dev != dev:
             raise ValueError("PagedCache: the step is on another device")
-        work = step._workspace(self.work_bytes(dt, step.max_new), stream)
+        work = step._workspace(self.work_bytes(dt, step._most), stream)
         rc = _on(dev, stream, (_lib or load()).lk_paged_attn, self._ref, step._ref, ty, pq, ldq,
                  self._scale if scale is None else scale, cap, ps, po, ldo, work.data_ptr(), work.numel())
         if rc:

@@ -68,3 +68,31 @@ def test_weights_in_two_parts(lk, hq, hkv, d, t, n_keys):
             got = out.cpu().double().view(n, hkv, hq // hkv, d)
             off = (got - o[None, :, None]).abs() / tol[None, :, None]
             assert float(off.max()) <= 1, (n, hint, float(off.max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+def test_an_unknown_number_of_new_tokens(lk, t):
+    """max_new 0 is the mean, rounded up, where the workspace has room for that, and 1 where not: the same bits as
+    of those."""
+    hq, hkv, d = 8, 2, 64
+    for news in ([130, 65], [1, 1, 1], [40, 0, 0, 3], [1]):
+        b = Batch(1, [37, 200, 9, 0][:len(news)], news, 16, pad=1)
+        g = torch.Generator().manual_seed(2)
+        k, v = (torch.randn(b.n_pages, 16, hkv, d, generator=g).to(pool_type(t)).cuda() for _ in range(2))
+        q = torch.randn(b.rows, hq * d, generator=g).to(TYPES[t]).cuda()
+        cache, mean = lk.PagedCache(k, v, hq), -(-b.rows // len(news))
+        small, large = (cache.work_bytes(TYPES[t], n) for n in (1, mean))
+        works = {"own": None, "small": torch.empty(small, dtype=torch.uint8, device="cuda"),
+                 "large": torch.empty(large, dtype=torch.uint8, device="cuda")}
+        outs = {}
+        for name, hint, work in (("one", 1, None), ("mean", mean, None), *(("0 " + w, 0, works[w]) for w in works)):
+            outs[name] = torch.zeros_like(q)
+            note(f"max_new {hint}, {name}, {t}, news {news}")
+            step = b.step(lk, max_new=hint, work=work)
+            cache.attend(step, q, outs[name])
+            torch.cuda.synchronize()
+            if work is None:
+                assert step._work.numel() == (small if hint == 1 else large)
+        same = lambda x, y: torch.equal(outs[x].view(torch.int16), outs[y].view(torch.int16))  # noqa: E731
+        assert same("0 own", "mean") and same("0 large", "mean") and same("0 small", "mean" if small >= large else "one")
