@@ -588,7 +588,7 @@ typedef struct lk_step {
  * is NaN, and so is one of zeros with eps 0.
  * q, k, v, qo are rows of `type` (LK_F32 or LK_F16 with fp16 pools, LK_BF16 with bf16 pools) of
  * n_heads or n_kv_heads heads side by side, ld* elements apart (parts of one wide row as
- * well); q and qo may be NULL (keys and values only), and qo may be q.  Rows need the
+ * well); q and qo may be NULL (keys and values only), and qo may be q (ldqo = ldq).  Rows need the
  * alignment of their elements; qn, kn, freq 16 bytes.  k, v and the pools must not overlap. */
 #define LK_ROPE_HALVES 0
 #define LK_ROPE_PAIRS  1
@@ -606,7 +606,7 @@ int lk_paged_append(const lk_pages * pages, const lk_step * step, int type, cons
  *   the key - position of the row), a cached key's position being its slot;  out = softmax(x) . v
  * and zeros for a row that sees nothing.  Keys and values a row does not see do not touch
  * it, infinities and NaN among them.
- * q, out rows of `type` as in lk_paged_append, n_heads heads side by side (out may be q); scale > 0, cap 0 or at least 2^-100;
+ * q, out rows of `type` as in lk_paged_append, n_heads heads side by side (out may be q, ldo = ldq); scale > 0, cap 0 or at least 2^-100;
  * slopes fp32 [n_heads] or NULL.  Scores (below 2^27), softmax and sums are fp32.  The weights enter the product
  * with v as two parts of the pools' type (what the first one leaves is the second: 2^-22 of a
  * weight is lost with fp16 pools, 2^-16 with bf16), and so does q where the rows are fp32.  Sums of the weights

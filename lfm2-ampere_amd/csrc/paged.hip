@@ -246,6 +246,8 @@ extern "C" int lk_paged_append(const lk_pages * pages, const lk_step * step, int
     if ((q && (ldq < hq * d || ldqo < hq * d)) || ldk < hkv * d || ldv < hkv * d)
         return lk_fail(hipErrorInvalidValue, "%s: row strides q %d, k %d, v %d, qo %d for %d and %d heads of %d", W, ldq, ldk, ldv, ldqo,
                        hq, hkv, d);
+    if (q && q == qo && ldq != ldqo && step->rows > 1)
+        return lk_fail(hipErrorInvalidValue, "%s: output over queries %d apart in rows %d apart", W, ldq, ldqo);
     const uintptr_t em = (uintptr_t) lk_type_size(type) - 1;
     if ((((uintptr_t) q | (uintptr_t) k | (uintptr_t) v | (uintptr_t) qo) & em) ||
         (((uintptr_t) qn | (uintptr_t) kn | (uintptr_t) freq) & 15))

@@ -1268,6 +1268,8 @@ extern "C" int lk_paged_attn(const lk_pages * pages, const lk_step * step, int t
     if (!q || !out || !work) return lk_fail(hipErrorInvalidValue, "%s: null pointer argument", W);
     if (ldq < hq * d || ldo < hq * d)
         return lk_fail(hipErrorInvalidValue, "%s: row strides q %d, out %d for %d heads of %d", W, ldq, ldo, hq, d);
+    if (q == out && ldq != ldo && step->rows > 1)
+        return lk_fail(hipErrorInvalidValue, "%s: output over queries %d apart in rows %d apart", W, ldq, ldo);
     const uintptr_t em = (uintptr_t) lk_type_size(type) - 1;
     if ((((uintptr_t) q | (uintptr_t) out) & em) || ((uintptr_t) slopes & 3) || ((uintptr_t) work & 15))
         return lk_fail(hipErrorInvalidValue, "%s: misaligned argument (rows by their element, slopes 4 B, work 16 B)", W);
