@@ -585,7 +585,7 @@ typedef struct lk_step {
  *   (u, v) -> (u cos a - v sin a, u sin a + v cos a); values from rot on are not rotated
  * in fp32, rounded once.  freq fp32 [rot / 2], rot a multiple of 16 up to head_dim, or freq NULL
  * with rot 0: no rotation.  |a_i| below 2^31.  Squares are summed in fp32: a head whose sum overflows
- * is NaN, and so is one of zeros with eps 0.
+ * is NaN, and so is one of a mean below 2^-126 with eps 0 (zeros, or no value above 2^-63).
  * q, k, v, qo are rows of `type` (LK_F32 or LK_F16 with fp16 pools, LK_BF16 with bf16 pools) of
  * n_heads or n_kv_heads heads side by side, ld* elements apart (parts of one wide row as
  * well); q and qo may be NULL (keys and values only), and qo may be q (ldqo = ldq).  Rows need the
