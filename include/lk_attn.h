@@ -605,7 +605,8 @@ int lk_paged_append(const lk_pages * pages, const lk_step * step, int type, cons
  *   x = scale * q.k;  cap > 0: x = cap * tanh(x / cap);  slopes: x += slopes[h] * (position of
  *   the key - position of the row), a cached key's position being its slot;  out = softmax(x) . v
  * and zeros for a row that sees nothing.  Keys and values a row does not see do not touch
- * it, infinities and NaN among them.
+ * it, infinities and NaN among them; of those it sees a score of -inf has the weight 0 (a row of
+ * such alone is NaN) and a finite one a weight above 0, however small, for infinite values.
  * q, out rows of `type` as in lk_paged_append, n_heads heads side by side (out may be q, ldo = ldq); scale > 0, cap 0 or at least 2^-100;
  * slopes fp32 [n_heads] or NULL.  Scores (below 2^27), softmax and sums are fp32.  The weights enter the product
  * with v as two parts of the pools' type (what the first one leaves is the second: 2^-22 of a

@@ -32,13 +32,13 @@
 #define LK_PA_SOME  2.0e38f        // the same for a column that sees keys, none of which had a weight yet
 
 // Two kinds of workgroup.  For up to 16 columns a kv head (STEP 16) the cache's bytes bound it: one workgroup a
-// CU, a ring of four tiles, so that 96 KB are on their way (64 sequences of up to 8192, 32 / 8 heads of 128, bf16: 213 us,
-// 6.6 TB/s; one of 131072 in 42 us, 6.4 TB/s, the pieces' sum 6 more).  For more (STEP 32) the products and
+// CU, a ring of four tiles, so that 96 KB are on their way (64 sequences of up to 8192, 32 / 8 heads of 128, bf16: 214 us,
+// 6.6 TB/s; one of 131072 in 43 us, 6.3 TB/s, the pieces' sum 6 more).  For more (STEP 32) the products and
 // exponentials do: two workgroups a CU of one wave a SIMD each, which wait at barriers of their own, and two tiles
-// (2 x 4096 new tokens 185 us, 635 TFLOP/s, and their join; of 457 thousand cycles a SIMD issues matrix
-// instructions for 129 and others for 207, which hardly overlap).  Between the two, 8 tokens of 4 heads a kv head, STEP 32
-// too: one sequence at 30000 21.7 us against 29.9, 16 at 1000 13.9 against 18.9.  DMA and products of short runs wait
-// for each other: 13 trees of up to 64 at 4096 40 us, where a SIMD issues for 43 of 110 thousand cycles.
+// (2 x 4096 new tokens 244 us, 483 TFLOP/s, and their join; of 593 thousand cycles a SIMD issues matrix
+// instructions for 201 and others for 284, which hardly overlap).  Between the two, 8 tokens of 4 heads a kv head, STEP 32
+// too: one sequence at 30000 22.4 us against 28.6, 16 at 1000 15.1 against 19.9.  DMA and products of short runs wait
+// for each other: 13 trees of up to 64 at 4096 44 us, where a SIMD issues for 60 of 122 thousand cycles.
 __host__ __device__ constexpr int lk_pa_waves(int d, int step) { return step == 16 && d == 64 ? 8 : 4; }
 __host__ __device__ constexpr int lk_pa_bufs(int step) { return step == 16 ? 4 : 2; }
 __host__ __device__ constexpr int lk_pa_wgs(int step) { return step == 16 ? 256 : 512; }
@@ -114,8 +114,9 @@ __device__ __forceinline__ int lk_sld(const int32_t * p, long i) {
 }
 
 // The arguments where the launch left them.  What is needed once an item or less is read there again each time
-// (args() below): kept for the whole kernel, the fifty values would spill, and each fetch wait for
-// lanes of a vector register to be read back.
+// (args() below): kept for the whole kernel, the fifty values would take the scalar registers that a tile's
+// loops need.  These are free of spilled scalars but for a few reads; around them, where tiles are fetched and
+// items begin and end, 180 to 360 scalars of an instance pass through lanes of vector registers.
 #ifdef __HIP_DEVICE_COMPILE__
 typedef __attribute__((address_space(4))) LkPaArgs LkPaC;
 __device__ __forceinline__ const LkPaC * lk_pa_kernarg() { return (const LkPaC *) __builtin_amdgcn_kernarg_segment_ptr(); }
@@ -307,8 +308,8 @@ lk_k_paged_attn(const LkPaArgs) {
     }
     const long share = (total + lk_pa_wgs(STEP) - 1) / lk_pa_wgs(STEP);
     // Workgroups go round the eight XCDs; runs side by side, whose chunks read the same keys, are given to one XCD and
-    // its L2 (2 x 4096 new tokens 200 -> 195 us, 13 trees 46.0 -> 44.7), but for short runs, which may be fewer than the
-    // workgroups and would then be on few XCDs (a tree of 16 at 32768 26.2 that way, 25.2 round).
+    // its L2 (13 trees 52.5 -> 51.4 us, 2 x 4096 new tokens, which the products bound, 260 -> 262), but for short runs, which
+    // may be fewer than the workgroups and would then be on few XCDs (a tree of 16 at 32768 28.4 that way, 27.1 round).
     const int wgi = share >= 8 ? (blockIdx.x & 7) * (lk_pa_wgs(STEP) / 8) + (blockIdx.x >> 3) : blockIdx.x;
     const long f0 = share * wgi, f1 = f0 + share < total ? f0 + share : total;
     if (f0 >= f1) {
@@ -652,7 +653,7 @@ lk_k_paged_attn(const LkPaArgs) {
         };
         shape();
         // the softmax first: of the two waves of a SIMD one then multiplies while the other forms weights (2 x 4096 new
-        // tokens 210 -> 200 us; no other order of the two parts' instructions within a wave gained anything)
+        // tokens 271 -> 262 us; no other order of the two parts' instructions within a wave gained anything)
         if constexpr (STEP == 32) __builtin_amdgcn_s_setprio(1);
         if (some) {
             hide();
@@ -1006,8 +1007,8 @@ struct LkPaBlock {
 
 // Many items, cut into few pieces each: workgroup (x, blk) joins block blk of the item that begins in
 // run x, each wave some of its dims.  A load of each piece is all it does: eight are asked for at once, so
-// that their latencies overlap (in place of two: 2 x 4096 new tokens 222 -> 210 us as a whole, 19 sequences of up
-// to 5003 21.5 -> 19.5).  Of 2 x 4096 new tokens it takes 11.7 us for at most 64 MB, 5.5 TB/s.
+// that their latencies overlap (in place of two: 16 sequences at up to 1000 18.0 -> 15.2 us as a whole, 19 at up
+// to 5003 20.0 -> 17.9).  Of 2 x 4096 new tokens it takes 11.7 us for at most 64 MB, 5.5 TB/s.
 template <int D, int RT>
 __global__ void __launch_bounds__(256)
 lk_k_paged_join(const LkPaArgs a, int cb_n) {
@@ -1179,11 +1180,14 @@ struct LkPaShape { int cb, step, hg_sh, qw_sh, kw_sh, qc, extra; };
 // LDS once for all of them; for up to 64 rows, whose items are cut into many pieces, one or two, since what a
 // workgroup leaves behind grows with its columns; one for chunks of four blocks in all until there are enough
 // of them to go round.  Measured, us, 32 / 8 heads of 64 (1, 2, 4 blocks):
-//   one tree of 16 at 2000      12.4  15.0  19.3     four of 24 at 2000            17.9  25.5
-//   one of 16 at 32768          25.9  28.7  32.8     one of 64 at 8000             25.4  40.0
-//   one of 16 at 131072         57.2  56.1  59.9     13 of up to 64 at 4096        47.0  48.9
-//   2 x 4096 new tokens                245  200      one of 64 at 131072          125   120
-// 16 / 16 heads of 64 (1, 4): 5 x 500 new tokens behind 500 31.0, 37.1; 2 x 4096 behind 4096 395, 351.
+//   one tree of 16 at 2000      13.1  16.0  21.1     four of 24 at 2000            17.6  20.0  23.9
+//   one of 16 at 32768          27.2  30.1  35.8     one of 64 at 8000             27.0  28.5  42.4
+//   one of 16 at 131072         62.9  63.9  68.4     13 of up to 64 at 4096        57.7  51.9  57.9
+//   2 x 4096 new tokens          390   308   271     one of 64 at 131072            191   161   156
+//   8 x up to 512 new tokens    43.0  36.4  38.2     5 x up to 500 behind 500      55.0  46.7  58.8
+// (the last two have few chunks, which this rule does not see); fp32 rows 13 trees 63.6, 56.2, 2 x 4096 new tokens
+// 452, 346; heads of 128, bf16, 13 trees 90.8, 73.9, a prompt of 4096 415, 273; 16 / 16 heads of 64 5 x 500 behind 500
+// 36.3, 36.8, 42.1; 2 x 4096 behind 4096 433, 408, 404.
 constexpr int lk_pa_cb32(int d, int type, int max_new, int nb) {
     return (nb <= 4 && max_new < 1024) || (d == 128 && type == LK_F32) ? 1 : d == 64 && type != LK_F32 && max_new > 64 ? 4 : 2;
 }
@@ -1234,8 +1238,8 @@ static void lk_pa_launch(const LkPaShape & s, const LkPaArgs & a, bool mod, hipS
 
 template <int D, int RT>
 static void lk_pa_join(const LkPaArgs & a, long items, int nblk, const LkPaShape & s, hipStream_t st) {
-    // attention and its join, us, spread and join: one token at 131072 51, 78; one at 4096 13.0, 26.8; a tree of 16
-    // at 32768 25, 28; 16 of up to 1000 22.5, 15.0; 64 of 8192 272, 222; 13 trees of up to 64 103, 45
+    // attention and its join, us, spread and join: one token at 131072 50, 86; one at 4096 13.1, 33; a tree of 16
+    // at 32768 27.1, 30.6; 16 of up to 1000 23.2, 15.4; 64 of up to 8192 293, 231; 13 trees of up to 64 123, 51
     const int wgs = lk_pa_wgs(s.step);
     if (items <= wgs / 32)
         hipLaunchKernelGGL((lk_k_paged_spread<D, RT>), dim3((unsigned) items, nblk * (D / 16)), dim3(1024), 0, st, a, s.cb, wgs);
