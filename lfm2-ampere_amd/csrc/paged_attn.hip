@@ -701,7 +701,7 @@ lk_k_paged_attn(const LkPaArgs) {
                 tops();
             }
         }
-        if (__ballot(over > M::HEADROOM)) {                  // wave-uniform
+        if (__ballot(!(over <= M::HEADROOM))) {                 // wave-uniform (NaN of one column hides no other's)
 #pragma unroll
             for (int cb = 0; cb < CB; ++cb) raise(cb, units(top[cb], cb));
         }

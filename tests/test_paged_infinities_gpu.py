@@ -222,3 +222,21 @@ def test_values_near_the_end_of_the_type(lk, hq, hkv, d):
         q = _rows(18, b.rows * hq * d, TYPES["bf16"]).view(b.rows, hq * d)
         want = _check(lk, "large values", b, q, k, v, "bf16", hints, scale=0.25)
         assert bool(torch.isfinite(want).all())
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hq,d", [(1, 64), (2, 64), (2, 128), (4, 64)])
+def test_rows_of_nan_beside_others(lk, t, hq, d):
+    """Half of the rows a wave holds are NaN; the scores of the others grow along the keys."""
+    for lens, n in (([300], 64), ([2000], 130)):
+        b = Batch(19, lens, [n], 16)
+        k, v = pools(20, b, 1, d, t)
+        at = b.slots(0, 0, lens[0] + n)
+        k.view(-1, 1, d)[at, :, 0] = torch.linspace(0.0, 40.0, lens[0] + n)[:, None].to(k.dtype)
+        q = _rows(21, n * hq * d, TYPES[t], 0.1).view(n, hq, d)
+        q[:, :, 0] = 4.0
+        for nan in (slice(0, 8), slice(8, 16), slice(0, 16), slice(0, n, 2)):
+            spoiled = q.clone()
+            spoiled[nan, :, 7] = math.nan
+            want = _check(lk, f"NaN in rows {nan}", b, spoiled.view(n, -1), k, v, t, (1, 64, 300))
+            assert int(torch.isnan(want[:, 0, 0]).sum()) == len(range(n)[nan])
