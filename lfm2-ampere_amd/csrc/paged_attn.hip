@@ -468,11 +468,11 @@ lk_k_paged_attn(const LkPaArgs) {
                 }
                 am = lk_xrow_max(am);
                 int e2 = 0;
-                if (am >= 0x1p-60f && am <= 3.4e38f) {         // (below, the scores' factor could vanish)
+                if (am > 0.0f && am < INFINITY) {
                     (void) frexpf(am, &e2);
                     e2 -= 15;
                 }
-                fac[cb] = ldexpf(sc, e2);
+                fac[cb] = fmaxf(ldexpf(sc, e2), 0x1p-126f);     // (smaller, it could be 0 against an infinity)
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks)
 #pragma unroll

@@ -240,3 +240,25 @@ def test_rows_of_nan_beside_others(lk, t, hq, d):
             spoiled[nan, :, 7] = math.nan
             want = _check(lk, f"NaN in rows {nan}", b, spoiled.view(n, -1), k, v, t, (1, 64, 300))
             assert int(torch.isnan(want[:, 0, 0]).sum()) == len(range(n)[nan])
+
+
+@pytest.mark.parametrize("shift", [-120, -70, 100, 125])
+@pytest.mark.parametrize("hq,hkv,d", SHAPES)
+def test_fp32_queries_to_the_ends_of_the_type(lk, hq, hkv, d, shift):
+    """A power of two moved from the scale to the queries leaves every bit as it was, beyond 2^60 either way, and with
+    an infinite key.  (By 2^-120 queries below 2^-6, by 2^125 the scale 2^-127 and its product with log2(e), are below the
+    normal numbers of fp32 and have bits fewer: there the bound alone holds.)"""
+    for b, hints in _batches():
+        k, v = pools(22, b, hkv, d, "f32")
+        q = _rows(23, b.rows * hq * d, TYPES["f32"]).clamp(-3.9, 3.9).view(b.rows, hq * d)
+        for value in (1.0, -INF):
+            k.view(-1, hkv, d)[b.slot(0, 9), 0, 3] = value
+            _check(lk, f"queries by 2^{shift}", b, q * 2.0 ** shift, k, v, "f32", hints, scale=0.25 * 2.0 ** -shift)
+            if shift in (-120, 125):
+                continue
+            cache, outs = lk.PagedCache(k.cuda(), v.cuda(), hq), []
+            for f in (0, shift):
+                outs.append(torch.empty(b.rows, hq * d, device="cuda"))
+                cache.attend(b.step(lk, max_new=16), (q * 2.0 ** f).cuda(), outs[-1], scale=0.25 * 2.0 ** -f)
+            torch.cuda.synchronize()
+            assert torch.equal(outs[0].view(torch.int32), outs[1].view(torch.int32))
