@@ -409,7 +409,7 @@ lk_k_paged_attn(const LkPaArgs) {
     int qpos[MOD ? CB : 1];
     int base = 0;                                               // keys below it are seen by all of the chunk's rows
     bool busy = false;                                          // the wave has columns
-    bool left_out = false;                                      // the run met infinities or NaN of V (or a row of NaN)
+    bool left_out = false;                                      // the run met infinities or NaN of V
     // column block cb: the token of the chunk, its row of the step, its query head; false: there is none
     auto column = [&](const LkPaC & a, int cb, int & i, int & row, int & head) -> bool {
         const int c = (qw * CB + cb) * 16 + lk_here(col), i0 = at.c * a.qc, m = at.s.n - i0 < a.qc ? at.s.n - i0 : a.qc;
@@ -772,14 +772,18 @@ lk_k_paged_attn(const LkPaArgs) {
     auto finish = [&](bool whole, bool from_first) {
         if (kw_sh) join_shares();
         if (kw != 0) return;
-        lk_f4 all = { 0.f, 0.f, 0.f, 0.f };                     // NaN with an infinity or NaN among the sums
+        // infinities or NaN among the sums of a column that are not its scores'
+        bool odd = false;
 #pragma unroll
-        for (int cb = 0; cb < CB; ++cb)
+        for (int cb = 0; cb < CB; ++cb) {
+            lk_f4 all = { 0.f, 0.f, 0.f, 0.f };
 #pragma unroll
             for (int db = 0; db < DB; ++db)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) all[r] = __builtin_fmaf(acc[cb][db][r], 0.0f, all[r]);
-        left_out |= __ballot((all[0] + all[1]) + (all[2] + all[3]) != 0.0f) != 0;        // wave-uniform
+            odd |= (all[0] + all[1]) + (all[2] + all[3]) != 0.0f && accl[cb][0] == accl[cb][0];
+        }
+        left_out |= __ballot(odd) != 0;                         // wave-uniform
         const LkPaC & a = args();
         const int nblk = CB << (a.qw_sh + a.hg_sh);
         const int slot = 2 * wgi + from_first;
@@ -793,7 +797,7 @@ lk_k_paged_attn(const LkPaArgs) {
 #pragma unroll
                 for (int db = 0; db < DB; ++db) {
                     float v[4] = { acc[cb][db][0] * il, acc[cb][db][1] * il, acc[cb][db][2] * il, acc[cb][db][3] * il };
-                    if (left_out) {                             // NaN by the values, not by the scores: marked for add_endless
+                    if (left_out || il != il) {                 // NaN by the values is marked, by its sign, for the run's end
 #pragma unroll
                         for (int r = 0; r < 4; ++r) v[r] = v[r] == v[r] ? v[r] : il == il ? -NAN : NAN;
                     }
@@ -894,7 +898,8 @@ lk_k_paged_attn(const LkPaArgs) {
     // being above 0, but for a score of -inf, whose weight is 0 and 0 times it NaN.  (Such a key has an infinite value itself and
     // its score no cap; an infinite query makes its whole row NaN anyway.)  The run's V is scanned once more, behind all
     // that the usual call does (at each item's end these lines took scalar registers from the products' loop:
-    // 64 sequences of up to 8192 323 us for 222).
+    // 64 sequences of up to 8192 323 us for 222).  With an infinite value in one of the sequences: 64 of up to 8192
+    // 342 us for 229, 2 x 4096 new tokens 495 for 292.
     if (kw != 0 || !left_out) return;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");      // what the wave's lanes wrote is read and written again
     const LkPaC & a = args();
@@ -911,57 +916,82 @@ lk_k_paged_attn(const LkPaArgs) {
         const int t0 = at.t, t1 = left < at.nt - t0 ? t0 + (int) left : at.nt;
         const int end = (t1 << tk_sh) < at.vis ? t1 << tk_sh : at.vis, m = (1 << a.page_sh) - 1;
         set_base(a);
-#pragma clang loop unroll(disable)
+        uint64_t see[CB];
+        lk_f4 sum[CB][DB];
+        uint32_t found[CB];                                     // a bit for each of the lane's dims
+#pragma unroll
         for (int cb = 0; cb < CB; ++cb) {
             int i, row, head;
-            const bool live = column(a, cb, i, row, head);
-            const uint64_t see = seen(a, i, row);
-            lk_f4 sum[DB];
-            uint32_t found = 0;                                 // a bit for each of the lane's dims
+            (void) column(a, cb, i, row, head);
+            see[cb] = seen(a, i, row);
+            found[cb] = 0;
 #pragma unroll
-            for (int db = 0; db < DB; ++db) sum[db] = (lk_f4){ 0.f, 0.f, 0.f, 0.f };
+            for (int db = 0; db < DB; ++db) sum[cb][db] = (lk_f4){ 0.f, 0.f, 0.f, 0.f };
+        }
+        // 32 keys at a time, some in each of D / 16 loads, 16 bytes a lane; then one by one those that have any
+        constexpr int LPK = D / 8, KPL = 64 / LPK, NL = D / 16;
+        const size_t head0 = ((size_t) at.h << rb_sh) + hh * (D * 2);
 #pragma clang loop unroll(disable)
-            for (int k0 = t0 << tk_sh; k0 < end; k0 += 4) {     // four keys of a page at once
-                const int page = lk_sld(at.row, k0 >> a.page_sh);
-                if (page < 0 || page >= a.n_pages) continue;
-                const size_t row0 = (((size_t) page << a.page_sh) + (k0 & m)) * row_bytes + ((size_t) at.h << rb_sh) + hh * (D * 2);
-                auto values = [&](int j, lk_u16x4 (&u)[DB]) -> bool {
-                    bool odd = false;
+        for (int k0 = t0 << tk_sh; k0 < end; k0 += KPL * NL) {
+            uint64_t odd[NL];
+            size_t row0[NL];                                    // of each load's first key (all in a page)
+            lk_u16x8 u8[NL];
 #pragma unroll
-                    for (int db = 0; db < DB; ++db) u[db] = *(const lk_u16x4 *) (a.vp + row0 + (size_t) j * row_bytes + 32 * db + 8 * g);
+            for (int j = 0; j < NL; ++j) {
+                const int k = k0 + KPL * j, page = lk_sld(at.row, (k < end ? k : k0) >> a.page_sh);
+                const bool ok = k < end && page >= 0 && page < a.n_pages;
+                row0[j] = (((size_t) (ok ? page : 0) << a.page_sh) + (k & m)) * row_bytes + head0;
+                u8[j] = lk_u16x8{};
+                if (ok) u8[j] = *(const lk_u16x8 *) (a.vp + row0[j] + (size_t) (lane / LPK) * row_bytes + 16 * (lane % LPK));
+            }
+            uint64_t any = 0;
 #pragma unroll
-                    for (int db = 0; db < DB; ++db) odd |= endless(u[db][0]) || endless(u[db][1]) || endless(u[db][2]) || endless(u[db][3]);
-                    return odd;
-                };
-                lk_u16x4 u0[DB], u1[DB], u2[DB], u3[DB];
-                const bool o0 = values(0, u0), o1 = values(1, u1), o2 = values(2, u2), o3 = values(3, u3);
-                if (__ballot(o0 || o1 || o2 || o3) == 0) continue;        // wave-uniform
+            for (int j = 0; j < NL; ++j) {
+                bool o = false;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o |= endless(u8[j][e]);
+                odd[j] = __ballot(o);
+                any |= odd[j];
+            }
+            if (any == 0) continue;                             // wave-uniform
+#pragma unroll
+            for (int j = 0; j < NL; ++j)
 #pragma clang loop unroll(disable)
-                for (int k = k0; k < k0 + 4 && k < end; ++k) {
-                    if (__ballot(values(k - k0, u0)) == 0) continue;
+                while (odd[j]) {
+                    const int f = __builtin_ctzll(odd[j]) / LPK, k = k0 + KPL * j + f;
+                    odd[j] &= ~(((1ull << LPK) - 1) << (f * LPK));
+                    if (k >= end) break;
+                    const size_t at0 = row0[j] + (size_t) f * row_bytes;
                     bool none = false;                          // the key's score is -inf, if it is not +inf or NaN
                     if (!(a.cap > 0.0f)) {
-                        const uint16_t * key = (const uint16_t *) (a.kp + row0 + (size_t) (k - k0) * row_bytes);
+                        const uint16_t * key = (const uint16_t *) (a.kp + at0);
 #pragma unroll
                         for (int e = 0; e < D / 64; ++e) none |= endless(key[lane + 64 * e]);
                         none = __ballot(none) != 0;
                     }
                     const int d = k - base;
-                    if (!(d < 0 || (d < 64 && ((see >> d) & 1)))) continue;
 #pragma unroll
                     for (int db = 0; db < DB; ++db) {
-                        const V4 v = __builtin_bit_cast(V4, u0[db]);
+                        const lk_u16x4 u = *(const lk_u16x4 *) (a.vp + at0 + 32 * db + 8 * g);
+                        const V4 v = __builtin_bit_cast(V4, u);
 #pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (endless(u0[db][r])) {
-                                sum[db][r] += none ? NAN : (float) v[r];
-                                found |= 1u << (4 * db + r);
-                            }
+                        for (int r = 0; r < 4; ++r) {
+                            if (!endless(u[r])) continue;
+#pragma unroll
+                            for (int cb = 0; cb < CB; ++cb)
+                                if (d < 0 || (d < 64 && ((see[cb] >> d) & 1))) {
+                                    sum[cb][db][r] += none ? NAN : (float) v[r];
+                                    found[cb] |= 1u << (4 * db + r);
+                                }
+                        }
                     }
                 }
-            }
-            if (!live || found == 0) continue;
-            const bool whole = t0 == 0 && t1 == at.nt;
+        }
+        const bool whole = t0 == 0 && t1 == at.nt;
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) {
+            int i, row, head;
+            if (!column(a, cb, i, row, head) || found[cb] == 0) continue;
             RowT * o = (RowT *) a.out + (size_t) row * a.ldo + (size_t) head * D + 4 * g;
             const size_t blk = (size_t) (2 * wgi + (t0 == 0)) * (CB << (a.qw_sh + a.hg_sh)) + ((hh << a.qw_sh) + qw) * CB + cb;
             if (!whole) {                                       // (lanes of a column write the same)
@@ -972,12 +1002,12 @@ lk_k_paged_attn(const LkPaArgs) {
             for (int db = 0; db < DB; ++db)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    if (((found >> (4 * db + r)) & 1) == 0) continue;
+                    if (((found[cb] >> (4 * db + r)) & 1) == 0) continue;
                     if (whole) {                                // but for rows that the scores made NaN
                         const float was = (float) o[16 * db + r];
-                        if (was == was || signbit(was)) o[16 * db + r] = (RowT) sum[db][r];
+                        if (was == was || signbit(was)) o[16 * db + r] = (RowT) sum[cb][db][r];
                     } else {
-                        a.acc[((blk * DB + db) * 64 + col * 4 + g) * 4 + r] = sum[db][r];
+                        a.acc[((blk * DB + db) * 64 + col * 4 + g) * 4 + r] = sum[cb][db][r];
                     }
                 }
         }

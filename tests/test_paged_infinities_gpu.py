@@ -262,3 +262,22 @@ def test_fp32_queries_to_the_ends_of_the_type(lk, hq, hkv, d, shift):
                 cache.attend(b.step(lk, max_new=16), (q * 2.0 ** f).cuda(), outs[-1], scale=0.25 * 2.0 ** -f)
             torch.cuda.synchronize()
             assert torch.equal(outs[0].view(torch.int32), outs[1].view(torch.int32))
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hq,hkv,d", SHAPES)
+def test_rows_of_nan_that_see_infinite_values(lk, hq, hkv, d, t):
+    """A row whose scores make it NaN stays so in every dim, the infinite values' among them; its neighbours get those."""
+    for lens, news, hints in (([50, 900], [1, 1], (1, 64)), ([60] * 30, [9] * 30, (1, 16)), ([0, 300], [20, 150], (1, 16, 64, 300)),
+                              ([9000], [2], (1, 64))):
+        b = Batch(24, lens, news, 16)
+        k, v = pools(25, b, hkv, d, t)
+        q = _rows(26, b.rows * hq * d, TYPES[t]).view(b.rows, hq, d)
+        for s, (a, n) in enumerate(zip(lens, news)):
+            for at in {a // 2, a, a + n - 1}:
+                _spoiled(b, v, s, at, [2, d - 2], INF if s % 2 else -INF)
+            _spoiled(b, v, s, a + n // 2, slice(None), INF)     # all dims of one token
+            q[b.first[s]:b.first[s + 1]:2, s % hq, 4] = (math.nan, INF)[s % 2]
+            if s % 3 == 1:
+                k.view(-1, hkv, d)[b.slot(s, a), -1, 5] = math.nan
+        _check(lk, "NaN rows and infinite values", b, q.view(b.rows, -1), k, v, t, hints)
