@@ -32,13 +32,13 @@
 #define LK_PA_SOME  2.0e38f        // the same for a column that sees keys, none of which had a weight yet
 
 // Two kinds of workgroup.  For up to 16 columns a kv head (STEP 16) the cache's bytes bound it: one workgroup a
-// CU, a ring of four tiles, so that 96 KB are on their way (64 sequences of up to 8192, 32 / 8 heads of 128, bf16: 214 us,
-// 6.6 TB/s; one of 131072 in 43 us, 6.3 TB/s, the pieces' sum 6 more).  For more (STEP 32) the products and
+// CU, a ring of four tiles, so that 96 KB are on their way (64 sequences of up to 8192, 32 / 8 heads of 128, bf16: 212 us,
+// 6.6 TB/s; one of 131072 in 42 us, 6.3 TB/s, the pieces' sum 6 more).  For more (STEP 32) the products and
 // exponentials do: two workgroups a CU of one wave a SIMD each, which wait at barriers of their own, and two tiles
-// (2 x 4096 new tokens 244 us, 483 TFLOP/s, and their join; of 593 thousand cycles a SIMD issues matrix
+// (2 x 4096 new tokens 238 us, 493 TFLOP/s, and their join; of 586 thousand cycles a SIMD issues matrix
 // instructions for 201 and others for 284, which hardly overlap).  Between the two, 8 tokens of 4 heads a kv head, STEP 32
 // too: one sequence at 30000 22.4 us against 28.6, 16 at 1000 15.1 against 19.9.  DMA and products of short runs wait
-// for each other: 13 trees of up to 64 at 4096 44 us, where a SIMD issues for 60 of 122 thousand cycles.
+// for each other: 13 trees of up to 64 at 4096 45 us, where a SIMD issues for 60 of 126 thousand cycles.
 __host__ __device__ constexpr int lk_pa_waves(int d, int step) { return step == 16 && d == 64 ? 8 : 4; }
 __host__ __device__ constexpr int lk_pa_bufs(int step) { return step == 16 ? 4 : 2; }
 __host__ __device__ constexpr int lk_pa_wgs(int step) { return step == 16 ? 256 : 512; }
@@ -251,7 +251,7 @@ __device__ __forceinline__ float lk_tanh(float t) {
 // The weights enter P.V as two parts of the pools' type, a second product for what the first part leaves,
 // so that the result is off by its own rounding alone, whatever kernel `max_new` chose (bf16 1.7e-3 relative,
 // fp16 2.1e-4; one part 2.3e-3 and 2.9e-4).  Where memory bounds the kernel that costs nothing; 2 x 4096 new
-// tokens take 262 us so, 197 with one part, 13 trees of up to 64 at 4096 52 and 45.
+// tokens take 254 us so, 197 with one part, 13 trees of up to 64 at 4096 51 and 45.
 template <int D, int RT, int CT, int CB, int STEP, bool MOD>
 __global__ void __launch_bounds__(64 * lk_pa_waves(D, STEP), STEP == 16 && D == 128 ? 1 : 2)
 lk_k_paged_attn(const LkPaArgs) {
